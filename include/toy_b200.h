@@ -197,6 +197,165 @@ int tb2_q8_0_quantize(const float *x, void *q, long long rows, int K, void *stre
 /* Q8_0 blocks -> split-bf16 planes (and exact f32 values when f32 != NULL). */
 int tb2_q8_0_dequantize(const void *q, void *hi, void *lo, float *f32, long long rows, int K, void *stream);
 
+/* ===================================================================== */
+/* Paged KV cache (device-pointer primitives). No counterpart in the     */
+/* reference, whose KV engine keeps one contiguous cache per sequence.   */
+/* ===================================================================== */
+/* A serving step over a paged cache is: tb2_paged_plan (pages for the tokens
+ * each request appends, on the GPU, from the requests' lengths), then per
+ * layer tb2_paged_append (RoPE, K and V into their pages) and
+ * tb2_paged_attend (one new token per request over its pages);
+ * tb2_paged_release gives a finished request's pages back. All four enqueue
+ * on `stream` of the current device, read lengths and tables on the device
+ * only (nothing is synchronised) and may be captured into a CUDA graph after
+ * tb2_paged_prepare. They return 0, -1 for a bad argument, -3 for a failed
+ * launch. A page id, slot or position that is out of range on the device is
+ * not followed: the access is skipped and tb2_device_error() reports 0x5001
+ * (page), 0x5002 (slot) or 0x5003 (position).
+ *
+ * One layer's page pools. Page p, key / value head j and offset o of a page
+ * hold a row of d_head values at element p * page_stride + j * head_stride +
+ * o * tok_stride of k and of v, so both [pages][heads][tokens] and
+ * [pages][tokens][heads] layouts, and pools of several layers or of K and V
+ * interleaved, are described by strides. d_head is 32, 64, 96 or 128; a row
+ * starts on a 16-byte boundary (k, v and the strides in bytes are multiples
+ * of 16); rows do not overlap. kv_type is a ggml type id: 0 f32, 1 f16,
+ * 30 bf16, or 8 Q8_0 with the blocks' int8 quants in k / v and their fp16
+ * scale bits in k_scale / v_scale, the scale of the block at element e at
+ * index e / 32 (strides are multiples of 32). A slot is page * page_size +
+ * offset, 64 bits wide. */
+typedef struct tb2_paged_kv {
+  void *k, *v;
+  void *k_scale, *v_scale; /* Q8_0 only */
+  int kv_type;
+  int n_pages, page_size;
+  int n_kv, d_head;
+  long long page_stride, head_stride, tok_stride; /* elements */
+} tb2_paged_kv;
+
+/* One-time set-up of the paged operators on the current device (the device
+ * error word, shared-memory limits); call it before capturing any of them. */
+int tb2_paged_prepare(void);
+
+/* Pages for a step's new tokens. Request b holds lens[b] tokens in the pages
+ * table[b][0 .. ceil(lens[b] / page_size)) and appends add[b] >= 0 more. The
+ * free pages are the stack free_pages[0 .. state[0]); new pages are taken
+ * from its top in request order and written to the table's next entries.
+ * Results: lens_out[b] = lens[b] + add[b]; state_out = {pages left on the
+ * stack, status, tokens appended, pages taken}; cu_tokens[0 .. n_req] the
+ * running sum of add; and for the i-th appended token (request by request)
+ * slots[i], positions[i] (its index in its request) and requests[i]. Entries
+ * past the appended tokens, up to n_tokens, get slot -1, position 0 and
+ * request -1. status: 0; 1 not enough free pages; 2 a request outgrows its
+ * table row; 3 more than n_tokens tokens; 4 a negative length, a negative
+ * add, or a stack count outside [0, n_free]. With a status other than 0
+ * nothing is taken: the table, the lengths and the stack count stay and every
+ * slot is -1. lens_out may be lens and state_out may be state (in place);
+ * other arrays do not overlap. All arrays are device memory. n_req is at most
+ * 16384. */
+typedef struct tb2_paged_plan_args {
+  const int *lens, *add;
+  int n_req;
+  int *table; /* [n_req][table_stride], table_width entries used */
+  int table_width;
+  long long table_stride;
+  const int *free_pages;
+  int n_free; /* entries of free_pages */
+  const int *state;
+  int page_size, n_pages;
+  int n_tokens;
+  int *lens_out, *state_out, *cu_tokens;
+  long long *slots;
+  int *positions, *requests;
+} tb2_paged_plan_args;
+int tb2_paged_plan(const tb2_paged_plan_args *args, void *stream);
+
+/* Finished requests give their pages back: for every b with done[b] != 0, in
+ * order, the pages table[b][0 .. ceil(lens[b] / page_size)) are pushed on the
+ * stack (the first page first), their table entries become -1 and lens_out[b]
+ * = 0; other lengths are copied. state_out = {pages on the stack, status, 0,
+ * pages pushed}; status 1: the stack would pass n_free entries; 4: a negative
+ * length, one past its table row, or a stack count outside [0, n_free]; with
+ * either nothing is changed. In place as tb2_paged_plan. n_req is at most
+ * 16384. */
+typedef struct tb2_paged_release_args {
+  const int *lens, *done;
+  int n_req;
+  int *table;
+  int table_width;
+  long long table_stride;
+  int *free_pages;
+  int n_free;
+  const int *state;
+  int page_size, n_pages;
+  int *lens_out, *state_out;
+} tb2_paged_release_args;
+int tb2_paged_release(const tb2_paged_release_args *args, void *stream);
+
+/* New rows into the cache. Token i's rows are q + i ldq [n_heads][d_head],
+ * k + i ldk and v + i ldv [n_kv][d_head] of row_type 0 f32, 1 f16 or 30 bf16
+ * (a packed q|k|v row is three pointers with one stride). bias (f32
+ * [n_heads + 2 n_kv][d_head], or NULL) is added first; with rope (f32 (cos,
+ * sin) pairs [rope_rows][d_head / 2], or NULL) the pairs (e, e + d_head / 2)
+ * of q and k are turned by the row positions[i] of the table (NEOX). q goes
+ * to q_out + i ldqo in row_type (q_out may be q with the same stride; q NULL:
+ * only k and v), k and v into the page row of slots[i] in the cache's type
+ * (Q8_0: ggml's quantiser). A negative slot leaves the cache as it is; its q
+ * is still turned. The slots of one call are distinct. Sums and products are
+ * f32, each rounded, products and sums not contracted. q, k, v and q_out
+ * start on 16-byte boundaries with strides that are multiples of 16 bytes. */
+typedef struct tb2_paged_append_args {
+  int n_tokens, n_heads, row_type;
+  const void *q;
+  long long ldq;
+  const void *k;
+  long long ldk;
+  const void *v;
+  long long ldv;
+  void *q_out;
+  long long ldqo;
+  const float *bias;
+  const float *rope;
+  int rope_rows;
+  const int *positions;
+  const long long *slots;
+} tb2_paged_append_args;
+int tb2_paged_append(const tb2_paged_kv *kv, const tb2_paged_append_args *args, void *stream);
+
+/* Attention of one new token per request over its pages: for request b and
+ * query head h of key / value head j = h / (n_heads / n_kv), over the keys t
+ * in [0, lens[b]) found through table[b]:
+ *   out[b][h] = sum_t softmax_t(scale q . k_t) v_t,
+ *   lse[b][h] = log sum_t exp(scale q . k_t)   (when lse != NULL).
+ * lens[b] counts the new token itself once it is appended. An empty request
+ * gives zeros and lse -inf; lengths past the table row are cut to it. q and
+ * out are [n_req][n_heads][d_head] with request strides ldq, ldo, of row_type
+ * 0 f32, 1 f16 or 30 bf16, independent of the cache's type; the softmax
+ * statistics and sums are f32. The history is split over the GPU and joined
+ * in a fixed order, so the same call gives the same bits; another batch, or
+ * another table width, may split a request's history elsewhere. workspace
+ * holds tb2_paged_attend_workspace() bytes (16-byte aligned) set up once by
+ * tb2_paged_attend_workspace_init; calls that may overlap on the GPU (two
+ * streams, two graphs) need one each. */
+typedef struct tb2_paged_attend_args {
+  int n_req, n_heads, row_type;
+  const void *q;
+  long long ldq;
+  void *out;
+  long long ldo;
+  const int *table;
+  int table_width;
+  long long table_stride;
+  const int *lens;
+  float scale;
+  float *lse;
+  void *workspace;
+  size_t workspace_bytes;
+} tb2_paged_attend_args;
+size_t tb2_paged_attend_workspace(void);
+int tb2_paged_attend_workspace_init(void *workspace, size_t bytes, void *stream);
+int tb2_paged_attend(const tb2_paged_kv *kv, const tb2_paged_attend_args *args, void *stream);
+
 /* Read and clear the device-side error word of the current device
  * (non-zero when a kernel's bounded wait gave up). Synchronises the device. */
 int tb2_device_error(void);

@@ -36,6 +36,44 @@ class LlamaConfigC(C.Structure):
                 ("n_experts", C.c_int), ("n_experts_used", C.c_int), ("norm_topk", C.c_int), ("qk_norm", C.c_int)]
 
 
+class PagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("kv_type", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv", C.c_int),
+                ("d_head", C.c_int), ("page_stride", C.c_longlong), ("head_stride", C.c_longlong),
+                ("tok_stride", C.c_longlong)]
+
+
+class PagedPlanArgs(C.Structure):
+    _fields_ = [("lens", C.c_void_p), ("add", C.c_void_p), ("n_req", C.c_int), ("table", C.c_void_p),
+                ("table_width", C.c_int), ("table_stride", C.c_longlong), ("free_pages", C.c_void_p),
+                ("n_free", C.c_int), ("state", C.c_void_p), ("page_size", C.c_int), ("n_pages", C.c_int),
+                ("n_tokens", C.c_int), ("lens_out", C.c_void_p), ("state_out", C.c_void_p),
+                ("cu_tokens", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p),
+                ("requests", C.c_void_p)]
+
+
+class PagedReleaseArgs(C.Structure):
+    _fields_ = [("lens", C.c_void_p), ("done", C.c_void_p), ("n_req", C.c_int), ("table", C.c_void_p),
+                ("table_width", C.c_int), ("table_stride", C.c_longlong), ("free_pages", C.c_void_p),
+                ("n_free", C.c_int), ("state", C.c_void_p), ("page_size", C.c_int), ("n_pages", C.c_int),
+                ("lens_out", C.c_void_p), ("state_out", C.c_void_p)]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [("n_tokens", C.c_int), ("n_heads", C.c_int), ("row_type", C.c_int), ("q", C.c_void_p),
+                ("ldq", C.c_longlong), ("k", C.c_void_p), ("ldk", C.c_longlong), ("v", C.c_void_p),
+                ("ldv", C.c_longlong), ("q_out", C.c_void_p), ("ldqo", C.c_longlong), ("bias", C.c_void_p),
+                ("rope", C.c_void_p), ("rope_rows", C.c_int), ("positions", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class PagedAttendArgs(C.Structure):
+    _fields_ = [("n_req", C.c_int), ("n_heads", C.c_int), ("row_type", C.c_int), ("q", C.c_void_p),
+                ("ldq", C.c_longlong), ("out", C.c_void_p), ("ldo", C.c_longlong), ("table", C.c_void_p),
+                ("table_width", C.c_int), ("table_stride", C.c_longlong), ("lens", C.c_void_p),
+                ("scale", C.c_float), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 _lib = None
 VP, D, DP, LP, SZ, I, LL = C.c_void_p, C.c_double, C.POINTER(C.c_double), C.POINTER(C.c_long), C.c_size_t, C.c_int, \
     C.c_longlong
@@ -109,6 +147,13 @@ _SIGS = [
     ("tb2_set_plan_alone", C.c_int, [C.c_int]),
     ("tb2_set_f16_wgrad", C.c_int, [C.c_int]),
     ("tb2_device_error", C.c_int, []),
+    ("tb2_paged_prepare", C.c_int, []),
+    ("tb2_paged_plan", C.c_int, [C.POINTER(PagedPlanArgs), C.c_void_p]),
+    ("tb2_paged_release", C.c_int, [C.POINTER(PagedReleaseArgs), C.c_void_p]),
+    ("tb2_paged_append", C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAppendArgs), C.c_void_p]),
+    ("tb2_paged_attend_workspace", C.c_size_t, []),
+    ("tb2_paged_attend_workspace_init", C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
+    ("tb2_paged_attend", C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAttendArgs), C.c_void_p]),
     ("tb2_q8_0_quantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p]),
     ("tb2_q8_0_dequantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_longlong, C.c_int,
                                       C.c_void_p]),
