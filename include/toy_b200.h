@@ -222,8 +222,10 @@ int tb2_q8_0_dequantize(const void *q, void *hi, void *lo, float *f32, long long
  * of 16); rows do not overlap. kv_type is a ggml type id: 0 f32, 1 f16,
  * 30 bf16, or 8 Q8_0 with the blocks' int8 quants in k / v and their fp16
  * scale bits in k_scale / v_scale, the scale of the block at element e at
- * index e / 32 (strides are multiples of 32). A slot is page * page_size +
- * offset, 64 bits wide. */
+ * index e / 32 (strides are multiples of d_head; k_scale and v_scale start
+ * on d_head / 16 bytes, 2 at least, for d_head 64 and 128). A slot is
+ * page * page_size + offset, 64 bits wide. A block table spans less than
+ * 2^31 - 256 tokens. */
 typedef struct tb2_paged_kv {
   void *k, *v;
   void *k_scale, *v_scale; /* Q8_0 only */

@@ -59,7 +59,7 @@ def values(pool, scale):
 
 
 def attend(k, v, q, table, lens, scale):
-    """out, lse and the two sums the error bound needs, in 64 bits. k, v: 64-bit pools [pages, kv, page, dh]."""
+    """out, lse and the sums the error bound needs, in 64 bits. k, v: 64-bit pools [pages, kv, page, dh]."""
     n, H, dh = q.shape
     n_kv, page = k.shape[1], k.shape[2]
     G = H // n_kv
@@ -67,6 +67,7 @@ def attend(k, v, q, table, lens, scale):
     lse = torch.full((n, H), -math.inf, dtype=torch.float64, device=q.device)
     absv = torch.zeros_like(out)      # sum p |v| / sum p
     ds = torch.zeros_like(lse)        # largest scale sum |q| |k| over the keys
+    vmax = torch.zeros_like(lse)      # largest |v|
     for b in range(n):
         L = int(lens[b])
         if L <= 0:
@@ -82,14 +83,15 @@ def attend(k, v, q, table, lens, scale):
         out[b] = (torch.einsum("jgt,jtd->jgd", p, vb) / z).reshape(H, dh)
         absv[b] = (torch.einsum("jgt,jtd->jgd", p, vb.abs()) / z).reshape(H, dh)
         lse[b] = (m + torch.log(z)).reshape(H)
+        vmax[b] = vb.abs().amax((1, 2)).repeat_interleave(G)
         ds[b] = (torch.einsum("jgd,jtd->jgt", qb.abs(), kb.abs()).amax(-1) * abs(scale)).reshape(H)
-    return out, lse, absv, ds
+    return out, lse, (absv, vmax), ds
 
 
 U = 2.0 ** -24
 
 
-def attend_bounds(out, lse, absv, ds, lens, dh, dtype):
+def attend_bounds(out, lse, sums, ds, lens, dh, dtype):
     """Largest |error| of out and lse that the kernel's arithmetic allows.
 
     A score: operands taken to 2^-21 or better, a product rounded and a sum of
@@ -100,11 +102,22 @@ def attend_bounds(out, lse, absv, ds, lens, dh, dtype):
     below 2 ds. A weight is used to 2^-21 (8 u). The weighted sums add 16 keys
     at a time, one tile after another and then warps and splits:
     (len / 16 + 256) u of sum p |v|. Then one rounding to the result's type.
+
+    A weight has a floor too: taken as f16 planes it is 2^14 p at most 2^14
+    (for Q8_0 times a block scale over a power of two D at or below the largest
+    one, so at most 2^15), and the second plane ends at the f16 grid's 2^-24:
+    each is off by 2^-25, which is 2^-39 of the largest weight (Q8_0: 2^-39 D,
+    times a quant of at most 127, where 127 D is at most the largest |v|). A
+    weight below 2^-126 of the largest is 0 for every type. Over len keys, with
+    sum p >= 1: len 2^-39 max |v|, seen where the keys of large weight have a
+    value of 0.
     """
+    absv, vmax = sums
     steps = (lens.double().clamp(min=0) / 16 + 256)[:, None]
     rel = 2 * ((dh + 16) * U * ds + 8 * U + 4 * U * ds) + 2 * steps * U
     step = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
     tiny = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[dtype]
-    b_out = rel[..., None] * absv * (1 + step) + step * out.abs() + tiny
+    floor = (lens.double().clamp(min=0)[:, None] * 2.0 ** -39 * vmax)[..., None]
+    b_out = (rel[..., None] * absv + floor) * (1 + step) + step * out.abs() + tiny
     b_lse = (dh + 20) * U * ds + (steps + 8) * U + 2 * U * torch.nan_to_num(lse, neginf=0.0).abs()
     return b_out, b_lse

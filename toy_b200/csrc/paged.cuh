@@ -28,8 +28,8 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 
 // Everything the kernels rely on about a descriptor: rows of d_head values
 // (a multiple of 32, at most 128) that start on 16-byte boundaries, pages and
-// heads that do not overlap by their strides, and for Q8_0 strides that are
-// whole blocks of 32.
+// heads that do not overlap by their strides, and for Q8_0 strides of whole
+// rows.
 inline bool paged_kv_ok(const tb2_paged_kv* c) {
   if (!c || !c->k || !c->v || c->n_pages < 1 || c->page_size < 1 || c->n_kv < 1) return false;
   if (!row_type_ok(c->kv_type) && c->kv_type != kTypeQ8_0) return false;
@@ -40,8 +40,9 @@ inline bool paged_kv_ok(const tb2_paged_kv* c) {
     if (s < c->d_head || (s * e) % 16) return false;
   if (!aligned(c->k, 16) || !aligned(c->v, 16)) return false;
   if (c->kv_type == kTypeQ8_0) {
-    if (!c->k_scale || !c->v_scale || !aligned(c->k_scale, 2) || !aligned(c->v_scale, 2)) return false;
-    if (c->page_stride % 32 || c->head_stride % 32 || c->tok_stride % 32) return false;
+    const size_t row = c->d_head == 128 ? 8 : c->d_head == 64 ? 4 : 2;   // a row's scales in one aligned read
+    if (!c->k_scale || !c->v_scale || !aligned(c->k_scale, row) || !aligned(c->v_scale, row)) return false;
+    if (c->page_stride % c->d_head || c->head_stride % c->d_head || c->tok_stride % c->d_head) return false;
   }
   return true;
 }

@@ -1,0 +1,1055 @@
+// Attention of one new token per request over a paged key-value cache: the
+// kernel, instantiated per cache type in paged_attn_*.cu.
+//
+//   out[b][h] = sum_t p_t v_t / sum_t p_t,  p_t = 2^(c q . k_t - m),
+//
+// c = scale log2(e), t over the request's history through its block table,
+// m a running maximum, h one of the G = H / KV query heads of key head j.
+//
+// Bound: every K and V byte is read once, so HBM: at 6.5 TB/s an SM receives
+// 23 bytes a clock. A 16-bit cache is then 11.5 values a clock, each multiplied
+// by G heads: at G = 8 that is most of what the FMA units can do with the
+// conversions and loads on top, so the products run on the tensor cores. One
+// token has at most 16 heads to a key head, far below the 128 rows of a
+// tcgen05 tile, and its operands would cross shared memory and TMEM twice; the
+// warp-level m16n8k16 shape fits and is 3 to 4 times faster than the memory.
+//
+// f32 accuracy from 16-bit operands: K and V of an f16 / bf16 / Q8_0 cache are
+// exact tensor-core operands (int8 quants as f16; their block scales are
+// applied to the scores and folded into P); q and P are split into planes that
+// sum to them (f16: 2 planes of 11 bits after a power-of-two scaling, bf16: 3
+// planes of 8 bits, 2 when the result is rounded to 16 bits anyway). Rows 8..15
+// of the 16-row operand hold the second plane of rows 0..7 (HT = 8 heads), so
+// two planes cost one instruction; with G > 8 (HT = 16) each plane is one. An
+// f32 cache is split the same way into tf32 hi + lo, q and P too.
+//
+// Split: the work is a list of units (kWarps tiles of TK keys of one request
+// and key head), cut into equal ranges, one per CTA, whatever the lengths. A
+// CTA's warps take the tiles of a range in turn, each through a ring of its own
+// in shared memory filled by cp.async (no barrier between warps inside a
+// history), the next history's tiles already in flight while the last one's
+// sums are joined. A history that one CTA holds whole is written at once;
+// pieces go to the workspace and the CTA that finishes last adds them up in
+// order (a ticket per history), so the result does not depend on timing.
+#pragma once
+#include <algorithm>
+
+#include "paged.cuh"
+#include "pdl.cuh"
+#include "runtime.cuh"
+
+namespace tb2 {
+
+constexpr int kAttnWarps = 4;
+constexpr int kAttnMaxCtas = 2 * 148;   // the workspace's slots
+constexpr int kAttnSlotFloats = 16 * 128 + 2 * 16;
+// tickets, then two partial slots per CTA
+constexpr size_t kAttnTicketBytes = (kAttnMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
+constexpr size_t kAttnWorkspace = kAttnTicketBytes + (size_t)kAttnMaxCtas * 2 * kAttnSlotFloats * sizeof(float);
+
+enum AttnCache : int { kCacheF32 = 0, kCacheF16 = 1, kCacheBF16 = 2, kCacheQ8 = 3 };
+
+struct PagedAttnArgs {
+  PagedKv kv;
+  const void* q;
+  void* out;
+  long long ldq, ldo, table_stride;
+  const int* table;
+  const int* lens;
+  float* lse;
+  unsigned* tickets;
+  float* slots;
+  int* err;
+  float c;             // scale * log2(e)
+  int n_req, n_heads, group, width, row_type, page_shift;   // page_shift < 0: page_size is no power of two
+};
+
+namespace attn {
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;   // 0: the 16 bytes are zeros and nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+template <int B>
+__device__ __forceinline__ void cp_small(uint32_t dst, const void* src, bool on) {
+  const int n = on ? B : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(B) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint16_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+
+// D += A B: A [16 x k] (rows g and g + 8 of lane group g), B [k x 8].
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+template <int CT>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  if constexpr (CT == kCacheBF16) mma_bf16(d, a, b0, b1);
+  else mma_f16(d, a, b0, b1);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t tf32(float x) {
+  uint32_t y;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
+  return y;
+}
+
+// Two values as one register of plane values (lower half first), what is left
+// of them going on to the next plane.
+__device__ __forceinline__ uint32_t plane_f16(float& x, float& y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  x -= f.x;
+  y -= f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t plane_bf16(float& x, float& y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 f = __bfloat1622float2(h);
+  x -= f.x;
+  y -= f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int CT>
+__device__ __forceinline__ uint32_t plane16(float& x, float& y) {
+  if constexpr (CT == kCacheBF16) return plane_bf16(x, y);
+  else return plane_f16(x, y);
+}
+
+// Four int8 (as u8 words after ^ 0x80808080, i.e. value + 128) in the bytes
+// (s0, s1) selected from w: f16 of 1024 + u has u in its low bits, so the pair
+// is 0x64u0 | 0x64u1 minus 1152, exact.
+__device__ __forceinline__ uint32_t i8pair_f16(uint32_t w, uint32_t sel) {
+  const uint32_t p = __byte_perm(w, 0x64646464u, sel);
+  const uint32_t k = 0x64806480u;   // 1152
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int CT, int DH, int HT, int PL>
+struct Cfg {
+  static constexpr int E = CT == kCacheF32 ? 4 : CT == kCacheQ8 ? 1 : 2;
+  static constexpr int CR = DH * E / 16;   // 16-byte chunks of a row
+  // keys of a tile: about 8 KB of K and V together (a multiple of 16 keys for
+  // 16-bit products, 8 for tf32)
+  static constexpr int TK = CT == kCacheF32    ? (DH == 32 ? 32 : DH == 64 ? 16 : 8)
+                            : CT == kCacheQ8 ? (DH == 32 ? 64 : 32)
+                                               : (DH == 32 ? 64 : DH == 64 ? 32 : 16);
+  static constexpr int UK = TK * kAttnWarps;   // keys of a unit
+  static constexpr int ST = CT == kCacheQ8 && DH <= 64 ? 4 : 3;
+  // row pitches in shared memory: rows lie dense and are swizzled, but for
+  // Q8_0 widths whose rows are too short to swizzle
+  static constexpr int KP = DH * E;
+  static constexpr int VP = DH * E + (CT == kCacheQ8 && DH != 128 ? 16 : 0);
+  static constexpr int NB = DH / 32;   // Q8_0 blocks of a row
+  static constexpr int SB = CT == kCacheQ8 ? TK * NB * 2 : 0;
+  static constexpr int kOffV = TK * KP, kOffKS = kOffV + TK * VP, kOffVS = kOffKS + SB;
+  static constexpr int kStage = (kOffVS + SB + 15) / 16 * 16;
+  static constexpr int RPL = TK > 32 ? TK / 32 : 1;   // rows of a tile per lane
+  static constexpr int NT = TK / 8;
+  static constexpr int OT = DH / 8;                   // 8-column tiles of the output
+  static constexpr int R = HT / 8;                    // heads per lane group
+  static constexpr int OV = HT == 8 ? 2 : 4;          // values of an output tile per lane, planes added
+  static constexpr int KS = CT == kCacheF32 ? DH / 8 : DH / 16;   // k steps of q . k
+  // register sets of q: planes that do not share an instruction
+  static constexpr int QS = CT == kCacheBF16 ? (HT == 8 ? PL - 1 : PL) : (HT == 8 ? 1 : 2);
+  static constexpr int kQBytes = QS * KS * 512;
+  static constexpr int kBufs = HT == 8 ? 2 : 1;       // join buffers
+  static constexpr int kBufFloats = (OT * OV + 2 * R) * 32;
+  static constexpr int kJoinBytes = kBufs * kBufFloats * 4;
+  static constexpr int kScanBytes = (kAttnWarps * 32 + 1) * 8;
+  static constexpr int kRegion0 = kQBytes > kJoinBytes ? kQBytes : kJoinBytes;
+  static constexpr int kRegion = kRegion0 > kScanBytes ? kRegion0 : (kScanBytes + 15) / 16 * 16;
+  static constexpr int kSmem = kAttnWarps * ST * kStage + kRegion;
+
+  // byte offset of 16-byte chunk ch of row r, so that the lanes that read at
+  // once meet no bank twice. K: the reads of two neighbouring rows (four for
+  // Q8_0) take 64 (32) bytes each; V: see the reads.
+  static __device__ __forceinline__ uint32_t k_at(int r, int ch) {
+    if constexpr (CT == kCacheQ8) {
+      if constexpr (DH == 128) ch ^= (r & 3) << 1;
+      if constexpr (DH == 64) ch ^= ((r >> 1) & 1) << 1;
+    } else if constexpr (CR % 8 == 0) {
+      ch ^= ((r & 1) << 2) | ((r >> 1) & 3);
+    } else {
+      ch ^= (r >> 1) & 3;
+    }
+    return r * KP + ch * 16;
+  }
+  static __device__ __forceinline__ uint32_t v_at(int r, int ch) {
+    if constexpr (CT == kCacheQ8) {
+      if constexpr (DH == 128) ch ^= ((r >> 1) & 3) << 1;
+    } else if constexpr (CT == kCacheF32) {
+      ch ^= ((r >> 1) & 3) << 1;
+    } else if constexpr (CR % 8 == 0) {
+      ch ^= ((r & 1) << 2) | ((r >> 1) & 3);
+    } else {
+      ch ^= (r >> 1) & 3;
+    }
+    return r * VP + ch * 16;
+  }
+};
+
+__device__ __forceinline__ float load_row(const void* p, int type, long long at) {
+  if (type == kTypeF32) return static_cast<const float*>(p)[at];
+  if (type == kTypeF16) return __half2float(static_cast<const __half*>(p)[at]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
+}
+__device__ __forceinline__ void store_row(void* p, int type, long long at, float x) {
+  if (type == kTypeF32) static_cast<float*>(p)[at] = x;
+  else if (type == kTypeF16) static_cast<__half*>(p)[at] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(x);
+}
+
+// A place in the list of units: unit t of key head (and head tile) jt of
+// request b, whose history has nt units.
+struct Cursor {
+  int b, jt, t, nt, len;
+};
+
+template <int CT, int DH, int HT, int PL>
+__global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const PagedAttnArgs a) {
+  using C = Cfg<CT, DH, HT, PL>;
+  constexpr int TK = C::TK, UK = C::UK, NT = C::NT, OT = C::OT, R = C::R, ST = C::ST;
+  // weights are kept times 2^14 where they are rounded to f16, so that small
+  // ones keep their bits (the factor is in the sums too and cancels)
+  constexpr float kLift = CT == kCacheF16 || CT == kCacheQ8 ? 14.f : 0.f;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint64_t valid[kAttnWarps][ST];   // keys of a staged tile that count
+  __shared__ int last_flag;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  uint8_t* region = smem + kAttnWarps * ST * C::kStage;
+  const uint32_t ring = smem_u32(smem) + warp * ST * C::kStage;
+  griddep_wait_release();
+
+  const int n = a.n_req, P = a.kv.page_size;
+  const long long most = (long long)a.width * P;
+  const int tiles_h = (a.group + HT - 1) / HT, KVH = a.kv.n_kv * tiles_h;
+  auto length = [&](int b) { return (int)min(most, (long long)max(0, __ldg(a.lens + b))); };
+
+  // ---- the list's length and this CTA's range of it
+  long long total;
+  long long* pre = reinterpret_cast<long long*>(region);   // units before each thread's run of requests
+  const int per = (n + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
+  {
+    const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
+    long long s = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int len = length(b);
+      s += (len + UK - 1) / UK;
+    }
+    long long inc = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    __shared__ long long wsum[kAttnWarps];
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    long long base = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) {
+      if (w < warp) base += wsum[w];
+      total += wsum[w];
+    }
+    pre[tid] = base + inc - s;
+    __syncthreads();
+  }
+  // requests without a key: zeros
+  for (int b = blockIdx.x; b < n; b += gridDim.x) {
+    if (length(b) > 0) continue;
+    for (int i = tid; i < a.n_heads * DH; i += blockDim.x) store_row(a.out, a.row_type, b * a.ldo + i, 0.f);
+    if (a.lse)
+      for (int h = tid; h < a.n_heads; h += blockDim.x) a.lse[(long long)b * a.n_heads + h] = -INFINITY;
+  }
+  const long long units = total * KVH;
+  const long long G = min((long long)gridDim.x, units);
+  if (blockIdx.x >= G) return;
+  const long long u_lo = blockIdx.x * units / G, u_hi = (blockIdx.x + 1) * units / G;
+
+  Cursor cur;
+  long long cur_first;   // the list's index of the cursor's request
+  {
+    const long long key = u_lo / KVH;
+    int lo = 0, hi = kAttnWarps * 32;   // the last thread whose run starts at or before key
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= key) lo = mid;
+      else hi = mid;
+    }
+    long long base = pre[lo];
+    int b = lo * per;
+    for (;;) {
+      const int i = b + lane;
+      const int nt = i < n ? (length(i) + UK - 1) / UK : 0;
+      long long inc = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, base + inc > key);
+      if (past) {
+        const int f = __ffs(past) - 1;
+        cur.b = b + f;
+        base += __shfl_sync(0xffffffffu, inc - nt, f);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, inc, 31);
+      b += 32;
+    }
+    cur.len = length(cur.b);
+    cur.nt = (cur.len + UK - 1) / UK;
+    cur_first = base * KVH;
+    const long long r = u_lo - cur_first;
+    cur.jt = (int)(r / cur.nt);
+    cur.t = (int)(r - (long long)cur.jt * cur.nt);
+  }
+  __syncthreads();   // pre is read: the region is free
+
+  // the next (request, head) of the list; the caller knows that there is one
+  auto next_history = [&](Cursor& k, long long* first) {
+    k.t = 0;
+    if (++k.jt < KVH) return;
+    k.jt = 0;
+    if (first) *first += (long long)k.nt * KVH;
+    do {
+      ++k.b;
+      k.len = length(k.b);
+    } while (k.len == 0);
+    k.nt = (k.len + UK - 1) / UK;
+  };
+
+  // ---- the ring: tiles of this warp in list order
+  Cursor pc = cur;             // the producer's place
+  long long pu = u_lo;         // list index of its unit
+  int row_page[C::RPL];        // page ids of the next tile's rows (one per lane and 32 rows)
+  auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / P; };
+  auto skip_empty = [&]() {    // the last unit of a history may hold no tile of this warp
+    while (pu < u_hi && (pc.t * kAttnWarps + warp) * TK >= pc.len) {
+      ++pu;
+      if (++pc.t == pc.nt && pu < u_hi) next_history(pc, nullptr);
+    }
+  };
+  auto fetch_pages = [&]() {
+    skip_empty();
+    if (pu >= u_hi) return;
+#pragma unroll
+    for (int i = 0; i < C::RPL; ++i) {
+      const int key = (pc.t * kAttnWarps + warp) * TK + (TK < 32 ? lane % TK : lane + 32 * i);
+      row_page[i] = key < pc.len ? __ldg(a.table + pc.b * a.table_stride + page_of(key)) : -1;
+    }
+  };
+  int stage_in = 0;
+  auto issue = [&]() {
+    if (pu < u_hi) {
+      const uint32_t s = ring + stage_in * C::kStage;
+      const int j = pc.jt / tiles_h;
+      long long off[C::RPL];
+      uint64_t ok = 0;
+#pragma unroll
+      for (int i = 0; i < C::RPL; ++i) {
+        const int key = (pc.t * kAttnWarps + warp) * TK + (TK < 32 ? lane % TK : lane + 32 * i);
+        const int page = row_page[i];
+        const bool in = key < pc.len;
+        const bool good = in && page >= 0 && page < a.kv.n_pages;
+        if (in && !good) *a.err = kErrPagedPage;
+        off[i] = good ? page * a.kv.page_stride + j * a.kv.head_stride + (key - page_of(key) * P) * a.kv.tok_stride : -1;
+        ok |= (uint64_t)__ballot_sync(0xffffffffu, good) << (32 * i);
+      }
+      if (lane == 0) valid[warp][stage_in] = ok;
+      constexpr int kIter = TK * C::CR / 32;
+#pragma unroll
+      for (int it = 0; it < kIter; ++it) {
+        const int i = it * 32 + lane, r = i / C::CR, ch = i % C::CR;
+        const long long o = __shfl_sync(0xffffffffu, off[C::RPL > 1 ? it * 32 / C::CR / 32 : 0], r & 31);
+        const bool on = o >= 0;
+        const long long at = on ? o * C::E + ch * 16 : 0;
+        cp16(s + C::k_at(r, ch), static_cast<const uint8_t*>(a.kv.k) + at, on);
+        cp16(s + C::kOffV + C::v_at(r, ch), static_cast<const uint8_t*>(a.kv.v) + at, on);
+      }
+      if constexpr (CT == kCacheQ8) {
+#pragma unroll
+        for (int i = 0; i < C::RPL; ++i) {
+          const int r = lane + 32 * i;
+          const bool on = off[i] >= 0;
+          const long long at = on ? off[i] / 32 : 0;
+          const uint32_t dk = s + C::kOffKS + r * C::NB * 2, dv = s + C::kOffVS + r * C::NB * 2;
+          if constexpr (DH == 128 || DH == 64) {
+            cp_small<C::NB * 2>(dk, a.kv.ks + at, on);
+            cp_small<C::NB * 2>(dv, a.kv.vs + at, on);
+          } else {
+#pragma unroll
+            for (int e = 0; e < C::NB; ++e) {
+              sts16(dk + 2 * e, on ? __ldg(a.kv.ks + at + e) : 0);
+              sts16(dv + 2 * e, on ? __ldg(a.kv.vs + at + e) : 0);
+            }
+          }
+        }
+      }
+      ++pu;
+      if (++pc.t == pc.nt && pu < u_hi) next_history(pc, nullptr);
+      fetch_pages();
+    }
+    cp_commit();   // (an empty group at the list's end keeps the count)
+    stage_in = stage_in + 1 == ST ? 0 : stage_in + 1;
+  };
+  fetch_pages();
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) issue();
+
+  // ---- this warp's sums over the current history
+  float o[OT][4], m[R], l[R], fac[R];
+  float inv_d = 0.f;   // Q8_0: V's block scales are used times inv_d, a power of two near 1 / the largest so far
+  int stage_out = 0;
+  long long u = u_lo;
+  while (u < u_hi) {
+    const int t0 = cur.t, t1 = (int)min((long long)cur.nt, t0 + (u_hi - u));
+    const int jh = cur.jt / tiles_h, h0 = (cur.jt - jh * tiles_h) * HT;   // key head, first head of the tile
+    const int heads = min(HT, a.group - h0);
+    const long long qrow = (long long)cur.b * a.ldq + ((long long)jh * a.group + h0) * DH;
+
+    // q as operand registers: lane (g, c) of step s holds rows g and g + 8
+    float rs[R];   // what the scores of the lane group's heads are multiplied by
+    {
+      float qv[R][DH / 4];   // the lane's part of its rows: 8 values of every 32 (f32 cache: 4 of every 16)
+      constexpr int kW = CT == kCacheF32 ? 4 : 8;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < DH / 4; ++i) {
+          const int d = i / kW * (4 * kW) + c * kW + i % kW;
+          qv[r][i] = g + 8 * r < heads ? load_row(a.q, a.row_type, qrow + (long long)(g + 8 * r) * DH + d) : 0.f;
+        }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        rs[r] = a.c;
+        if constexpr (CT == kCacheF16 || CT == kCacheQ8) {   // the largest |q| of the row into [16, 32)
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < DH / 4; ++i) x = fmaxf(x, fabsf(qv[r][i]));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          int e = (int)(__float_as_uint(x) >> 23) - 127 - 4;   // x < 2^(e + 5)
+          e = max(-100, min(100, e));
+          const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+          for (int i = 0; i < DH / 4; ++i) qv[r][i] *= up;
+          rs[r] = a.c * __uint_as_float((uint32_t)(127 + e) << 23);
+        }
+      }
+      uint4* qf = reinterpret_cast<uint4*>(region);
+#pragma unroll
+      for (int s = 0; s < C::KS; ++s) {
+        if (s % kAttnWarps != warp) {   // each warp writes its share of the steps
+          continue;
+        }
+        if constexpr (CT == kCacheF32) {
+          const int i = s * 2;   // values i, i + 1 of the lane's part
+          if constexpr (HT == 8) {
+            const uint32_t h0_ = tf32(qv[0][i]), h1_ = tf32(qv[0][i + 1]);
+            qf[s * 32 + lane] = make_uint4(h0_, tf32(qv[0][i] - __uint_as_float(h0_)), h1_,
+                                           tf32(qv[0][i + 1] - __uint_as_float(h1_)));
+          } else {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float x = qv[k & 1][i + (k >> 1)];
+              hi[k] = tf32(x);
+              lo[k] = tf32(x - __uint_as_float(hi[k]));
+            }
+            qf[s * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            qf[(C::KS + s) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        } else {
+          const int i = s * 4;
+          if constexpr (HT == 8) {
+            float x0 = qv[0][i], x1 = qv[0][i + 1], x2 = qv[0][i + 2], x3 = qv[0][i + 3];
+            uint4 v;
+            v.x = plane16<CT>(x0, x1);
+            v.z = plane16<CT>(x2, x3);
+            v.y = plane16<CT>(x0, x1);
+            v.w = plane16<CT>(x2, x3);
+            qf[s * 32 + lane] = v;
+            if constexpr (C::QS == 2) {
+              v.x = plane16<CT>(x0, x1);
+              v.z = plane16<CT>(x2, x3);
+              v.y = v.w = 0;
+              qf[(C::KS + s) * 32 + lane] = v;
+            }
+          } else {
+            float x[2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) x[r][k] = qv[r][i + k];
+#pragma unroll
+            for (int p = 0; p < C::QS; ++p) {
+              uint4 v;
+              v.x = plane16<CT>(x[0][0], x[0][1]);
+              v.y = plane16<CT>(x[1][0], x[1][1]);
+              v.z = plane16<CT>(x[0][2], x[0][3]);
+              v.w = plane16<CT>(x[1][2], x[1][3]);
+              qf[(p * C::KS + s) * 32 + lane] = v;
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+      fac[r] = rs[r];
+    }
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+    if constexpr (CT == kCacheQ8) inv_d = 0.f;
+    const uint32_t qb = smem_u32(region) + lane * 16;
+
+    for (int t = t0; t < t1; ++t) {
+      if ((t * kAttnWarps + warp) * TK >= cur.len) break;
+      cp_wait<ST - 2>();
+      __syncwarp();
+      const uint32_t ks = ring + stage_out * C::kStage, vs = ks + C::kOffV;
+      const uint64_t ok = valid[warp][stage_out];
+
+      // scores of the tile: lane (g, c) has keys 8 i + 2 c, + 1 of rows g (and g + 8)
+      float s[NT][2 * R];
+      if constexpr (CT == kCacheQ8) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int k = 0; k < 2 * R; ++k) s[i][k] = 0.f;
+#pragma unroll
+        for (int blk = 0; blk < C::NB; ++blk) {
+          uint4 qa[C::QS][2];
+#pragma unroll
+          for (int p = 0; p < C::QS; ++p)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) qa[p][k] = lds128(qb + (p * C::KS + 2 * blk + k) * 512);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const int r = 8 * i + g;
+            const uint2 w = lds64(ks + C::k_at(r, 2 * blk + (c >> 1)) + (c & 1) * 8);
+            const uint32_t w0 = w.x ^ 0x80808080u, w1 = w.y ^ 0x80808080u;
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t b0 = i8pair_f16(w0, 0x4140), b1 = i8pair_f16(w0, 0x4342), b2 = i8pair_f16(w1, 0x4140),
+                           b3 = i8pair_f16(w1, 0x4342);
+#pragma unroll
+            for (int p = 0; p < C::QS; ++p) {
+              mma_f16(d, qa[p][0], b0, b1);
+              mma_f16(d, qa[p][1], b2, b3);
+            }
+            const uint32_t sc = ks + C::kOffKS + ((8 * i + 2 * c) * C::NB + blk) * 2;
+            const float s0 = __half2float(__ushort_as_half(lds16(sc)));
+            const float s1 = __half2float(__ushort_as_half(lds16(sc + C::NB * 2)));
+            if constexpr (HT == 8) {
+              s[i][0] = fmaf(s0, d[0] + d[2], s[i][0]);
+              s[i][1] = fmaf(s1, d[1] + d[3], s[i][1]);
+            } else {
+              s[i][0] = fmaf(s0, d[0], s[i][0]);
+              s[i][1] = fmaf(s1, d[1], s[i][1]);
+              s[i][2] = fmaf(s0, d[2], s[i][2]);
+              s[i][3] = fmaf(s1, d[3], s[i][3]);
+            }
+          }
+        }
+      } else {
+        float d[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d[i][k] = 0.f;
+#pragma unroll
+        for (int st = 0; st < C::KS; st += 2) {   // one 16-byte read of each key row feeds two steps
+          uint4 qa[C::QS][2];
+#pragma unroll
+          for (int p = 0; p < C::QS; ++p)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) qa[p][k] = lds128(qb + (p * C::KS + st + k) * 512);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const uint4 w = lds128(ks + C::k_at(8 * i + g, st * 2 + c));
+            if constexpr (CT == kCacheF32) {
+              const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                hi[k] = tf32(__uint_as_float(x[k]));
+                lo[k] = tf32(__uint_as_float(x[k]) - __uint_as_float(hi[k]));
+              }
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                mma_tf32(d[i], qa[0][k], lo[2 * k], lo[2 * k + 1]);
+                if constexpr (HT == 16) mma_tf32(d[i], qa[1][k], hi[2 * k], hi[2 * k + 1]);
+                mma_tf32(d[i], qa[0][k], hi[2 * k], hi[2 * k + 1]);
+              }
+            } else {
+#pragma unroll
+              for (int p = C::QS - 1; p >= 0; --p) {
+                mma16<CT>(d[i], qa[p][0], w.x, w.y);
+                mma16<CT>(d[i], qa[p][1], w.z, w.w);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          if constexpr (HT == 8) {
+            s[i][0] = d[i][0] + d[i][2];
+            s[i][1] = d[i][1] + d[i][3];
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[i][k] = d[i][k];
+          }
+        }
+      }
+
+      // running maximum and weights
+      constexpr uint64_t kAll = TK == 64 ? ~0ull : ((1ull << (TK & 63)) - 1);
+      const bool masked = (ok & kAll) != kAll;
+      float mx[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) mx[r] = m[r];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int k = 0; k < 2 * R; ++k) {
+          float x = s[i][k] * fac[k >> 1];
+          if (masked && !((ok >> (8 * i + 2 * c + (k & 1))) & 1)) x = -INFINITY;
+          s[i][k] = x;
+          mx[k >> 1] = fmaxf(mx[k >> 1], x);
+        }
+      bool grew = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        grew |= mx[r] != m[r];
+      }
+      float shrink[R];
+      float new_inv = inv_d;
+      if constexpr (CT == kCacheQ8) {
+        uint32_t big = 0;   // the tile's largest |V scale|, as fp16 bits
+#pragma unroll
+        for (int i = 0; i < C::RPL; ++i)
+#pragma unroll
+          for (int e = 0; e < C::NB; ++e)
+            big = max(big, (uint32_t)lds16(ks + C::kOffVS + ((lane + 32 * i) * C::NB + e) * 2) & 0x7fffu);
+        big = __reduce_max_sync(0xffffffffu, big);
+        const float top = fmaxf(__half2float(__ushort_as_half((uint16_t)big)), 0x1p-24f);
+        // 1 / the power of two at or below it (an infinite scale makes the sums NaN)
+        const float inv = __uint_as_float((254u << 23) - (__float_as_uint(top) & 0x7f800000u));
+        if (inv_d == 0.f || inv < inv_d) new_inv = inv;
+        grew |= new_inv != inv_d;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          shrink[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx[r]);
+          m[r] = mx[r];
+          l[r] *= shrink[r];
+        }
+        if constexpr (CT == kCacheQ8) {
+          if (inv_d != 0.f) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) shrink[r] *= new_inv / inv_d;
+          }
+          inv_d = new_inv;
+        }
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[i][k] *= shrink[R == 1 ? 0 : k >> 1];
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float base = m[r] == -INFINITY ? 0.f : m[r] - kLift;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float p = ex2(s[i][2 * r + k] - base);
+            s[i][2 * r + k] = p;
+            l[r] += p;
+          }
+      }
+
+      // sums of weighted values
+      if constexpr (CT == kCacheF32) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {   // 8 keys: step k holds key 2 k, step k + 4 key 2 k + 1
+          uint4 ph, pl;
+          if constexpr (HT == 8) {
+            ph.x = tf32(s[i][0]);
+            ph.z = tf32(s[i][1]);
+            ph.y = tf32(s[i][0] - __uint_as_float(ph.x));
+            ph.w = tf32(s[i][1] - __uint_as_float(ph.z));
+          } else {
+            ph.x = tf32(s[i][0]);
+            ph.y = tf32(s[i][2]);
+            ph.z = tf32(s[i][1]);
+            ph.w = tf32(s[i][3]);
+            pl.x = tf32(s[i][0] - __uint_as_float(ph.x));
+            pl.y = tf32(s[i][2] - __uint_as_float(ph.y));
+            pl.z = tf32(s[i][1] - __uint_as_float(ph.z));
+            pl.w = tf32(s[i][3] - __uint_as_float(ph.w));
+          }
+#pragma unroll
+          for (int q4 = 0; q4 < DH / 32; ++q4) {   // columns 32 q4 + 4 g .. + 3: one per output tile
+            const uint4 w0 = lds128(vs + C::v_at(8 * i + 2 * c, 8 * q4 + g));
+            const uint4 w1 = lds128(vs + C::v_at(8 * i + 2 * c + 1, 8 * q4 + g));
+            const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t a0 = tf32(__uint_as_float(x0[k])), a1 = tf32(__uint_as_float(x1[k]));
+              const uint32_t e0 = tf32(__uint_as_float(x0[k]) - __uint_as_float(a0));
+              const uint32_t e1 = tf32(__uint_as_float(x1[k]) - __uint_as_float(a1));
+              mma_tf32(o[4 * q4 + k], ph, e0, e1);
+              if constexpr (HT == 16) mma_tf32(o[4 * q4 + k], pl, a0, a1);
+              mma_tf32(o[4 * q4 + k], ph, a0, a1);
+            }
+          }
+        }
+      } else if constexpr (CT == kCacheQ8) {
+#pragma unroll
+        for (int i = 0; i < NT; i += 2) {   // 16 keys
+#pragma unroll
+          for (int blk = 0; blk < C::NB; ++blk) {
+            float dv[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              dv[k] = inv_d * __half2float(__ushort_as_half(lds16(
+                                  ks + C::kOffVS + ((8 * (i + (k >> 1)) + 2 * c + (k & 1)) * C::NB + blk) * 2)));
+            uint4 ph, pl;
+            if constexpr (HT == 8) {
+              float x0 = s[i][0] * dv[0], x1 = s[i][1] * dv[1], x2 = s[i + 1][0] * dv[2], x3 = s[i + 1][1] * dv[3];
+              ph.x = plane_f16(x0, x1);
+              ph.z = plane_f16(x2, x3);
+              ph.y = plane_f16(x0, x1);
+              ph.w = plane_f16(x2, x3);
+            } else {
+              float x[8];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                x[k] = s[i][k] * dv[k & 1];
+                x[4 + k] = s[i + 1][k] * dv[2 + (k & 1)];
+              }
+              ph.x = plane_f16(x[0], x[1]);
+              ph.y = plane_f16(x[2], x[3]);
+              ph.z = plane_f16(x[4], x[5]);
+              ph.w = plane_f16(x[6], x[7]);
+              pl.x = plane_f16(x[0], x[1]);
+              pl.y = plane_f16(x[2], x[3]);
+              pl.z = plane_f16(x[4], x[5]);
+              pl.w = plane_f16(x[6], x[7]);
+            }
+            uint32_t w[4];   // columns 32 blk + 4 g .. + 3 of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = lds32(vs + C::v_at(8 * (i + (k >> 1)) + 2 * c + (k & 1), 2 * blk + (g >> 2)) + (g & 3) * 4) ^
+                     0x80808080u;
+            const uint32_t p0 = __byte_perm(w[0], w[1], 0x5140), p1 = __byte_perm(w[0], w[1], 0x7362);
+            const uint32_t p2 = __byte_perm(w[2], w[3], 0x5140), p3 = __byte_perm(w[2], w[3], 0x7362);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t sel = k & 1 ? 0x4342 : 0x4140;
+              const uint32_t b0 = i8pair_f16(k < 2 ? p0 : p1, sel), b1 = i8pair_f16(k < 2 ? p2 : p3, sel);
+              if constexpr (HT == 16) mma_f16(o[4 * blk + k], pl, b0, b1);
+              mma_f16(o[4 * blk + k], ph, b0, b1);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NT; i += 2) {   // 16 keys
+          constexpr int kP = HT == 8 ? (PL == 3 ? 2 : 1) : PL;   // operand sets
+          uint4 pp[kP];
+          if constexpr (HT == 8) {
+            float x0 = s[i][0], x1 = s[i][1], x2 = s[i + 1][0], x3 = s[i + 1][1];
+            pp[0].x = plane16<CT>(x0, x1);
+            pp[0].z = plane16<CT>(x2, x3);
+            pp[0].y = plane16<CT>(x0, x1);
+            pp[0].w = plane16<CT>(x2, x3);
+            if constexpr (kP == 2) {
+              pp[1].x = plane16<CT>(x0, x1);
+              pp[1].z = plane16<CT>(x2, x3);
+              pp[1].y = pp[1].w = 0;
+            }
+          } else {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              x[k] = s[i][k];
+              x[4 + k] = s[i + 1][k];
+            }
+#pragma unroll
+            for (int p = 0; p < kP; ++p) {
+              pp[p].x = plane16<CT>(x[0], x[1]);
+              pp[p].y = plane16<CT>(x[2], x[3]);
+              pp[p].z = plane16<CT>(x[4], x[5]);
+              pp[p].w = plane16<CT>(x[6], x[7]);
+            }
+          }
+#pragma unroll
+          for (int d2 = 0; d2 < OT; d2 += 2) {
+            uint32_t b[4];   // keys 0..7 and 8..15 of columns 8 d2 .., then of 8 d2 + 8 ..
+            ldmatrix_x4_trans(vs + C::v_at(8 * i + (lane & 15), d2 + (lane >> 4)), b);
+#pragma unroll
+            for (int p = kP - 1; p >= 0; --p) {
+              mma16<CT>(o[d2], pp[p], b[0], b[1]);
+              mma16<CT>(o[d2 + 1], pp[p], b[2], b[3]);
+            }
+          }
+        }
+      }
+      __syncwarp();   // the stage is read
+      stage_out = stage_out + 1 == ST ? 0 : stage_out + 1;
+      issue();
+    }
+
+    // ---- the warps' sums joined: planes added, weights of a lane group summed
+    float ov[OT][C::OV];
+    const float back = CT == kCacheQ8 ? (inv_d == 0.f ? 0.f : 1.f / inv_d) : 1.f;
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int k = 0; k < C::OV; ++k) ov[i][k] = (HT == 8 ? o[i][k] + o[i][(k + 2) & 3] : o[i][k]) * back;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    float* buf = reinterpret_cast<float*>(region);
+    auto put = [&](float* d) {
+#pragma unroll
+      for (int i = 0; i < OT; ++i)
+#pragma unroll
+        for (int k = 0; k < C::OV; ++k) d[(i * C::OV + k) * 32 + lane] = ov[i][k];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        d[(OT * C::OV + 2 * r) * 32 + lane] = m[r];
+        d[(OT * C::OV + 2 * r + 1) * 32 + lane] = l[r];
+      }
+    };
+    auto add = [&](const float* d) {
+      float f[R], e[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float mo = d[(OT * C::OV + 2 * r) * 32 + lane], lo = d[(OT * C::OV + 2 * r + 1) * 32 + lane];
+        const float mn = fmaxf(m[r], mo);
+        // a warp without keys has sums of 0, which any finite factor keeps (and NaN sums stay NaN)
+        f[r] = m[r] == -INFINITY ? 1.f : ex2(m[r] - mn);
+        e[r] = mo == -INFINITY ? 1.f : ex2(mo - mn);
+        l[r] = l[r] * f[r] + lo * e[r];
+        m[r] = mn;
+      }
+#pragma unroll
+      for (int i = 0; i < OT; ++i)
+#pragma unroll
+        for (int k = 0; k < C::OV; ++k) {
+          const int r = R == 1 ? 0 : k >> 1;
+          ov[i][k] = ov[i][k] * f[r] + d[(i * C::OV + k) * 32 + lane] * e[r];
+        }
+    };
+    __syncthreads();   // q is read by every warp
+    if constexpr (C::kBufs == 2) {
+      if (warp >= 2) put(buf + (warp - 2) * C::kBufFloats);
+      __syncthreads();
+      if (warp < 2) add(buf + warp * C::kBufFloats);
+      __syncthreads();
+      if (warp == 1) put(buf);
+      __syncthreads();
+      if (warp == 0) add(buf);
+    } else {
+      for (int w = kAttnWarps - 1; w >= 1; --w) {
+        if (warp == w) put(buf);
+        __syncthreads();
+        if (warp == 0) add(buf);
+        __syncthreads();
+      }
+    }
+
+    // element e of the lane's value k of output tile i: its column
+    auto col = [&](int i, int k) {
+      if constexpr (CT == kCacheF32 || CT == kCacheQ8) return 32 * (i >> 2) + 4 * (2 * c + (k & 1)) + (i & 3);
+      else return 8 * i + 2 * c + (k & 1);
+    };
+    const long long out0 = (long long)cur.b * a.ldo + ((long long)jh * a.group + h0) * DH;
+    const long long lse0 = (long long)cur.b * a.n_heads + (long long)jh * a.group + h0;
+    const bool whole = t0 == 0 && t1 == cur.nt;
+    if (whole) {
+      if (warp == 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (g + 8 * r >= heads) continue;
+          const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+          for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              store_row(a.out, a.row_type, out0 + (long long)(g + 8 * r) * DH + col(i, k), ov[i][2 * r + k] * inv);
+          if (a.lse && c == 0)
+            a.lse[lse0 + g + 8 * r] = l[r] == 0.f ? -INFINITY : (m[r] - kLift + log2f(l[r])) * 0.693147180559945f;
+        }
+      }
+      __syncthreads();   // the region is read
+    } else {
+      // the CTAs that hold this history: first .. lastc
+      const long long ub = cur_first + (long long)cur.jt * cur.nt;
+      const int first = (int)(((ub + 1) * G - 1) / units), lastc = (int)(((ub + cur.nt) * G - 1) / units);
+      const int pieces = lastc - first + 1;
+      auto slot_of = [&](int cta) { return a.slots + ((long long)cta * 2 + (cta == first)) * kAttnSlotFloats; };
+      if (warp == 0) {
+        float* d = slot_of(blockIdx.x);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) __stcg(d + (g + 8 * r) * DH + col(i, k), ov[i][2 * r + k]);
+          if (c == 0) {
+            __stcg(d + HT * DH + g + 8 * r, m[r]);
+            __stcg(d + HT * DH + HT + g + 8 * r, l[r]);
+          }
+        }
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) last_flag = atomicAdd(a.tickets + first, 1u) == (unsigned)pieces - 1;
+      }
+      __syncthreads();
+      if (last_flag) {   // this CTA adds the pieces up, in order
+        __threadfence();
+        for (int e0 = tid * 4; e0 < heads * DH; e0 += kAttnWarps * 32 * 4) {
+          const int h = e0 / DH;
+          float mm = -INFINITY;
+#pragma unroll 8
+          for (int p = 0; p < pieces; ++p) mm = fmaxf(mm, __ldcg(slot_of(first + p) + HT * DH + h));
+          float ll = 0.f;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int p = 0; p < pieces; ++p) {
+            const float* d = slot_of(first + p);
+            const float mp = __ldcg(d + HT * DH + h), f = mp == -INFINITY ? 1.f : ex2(mp - mm);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(d + e0));
+            ll += f * __ldcg(d + HT * DH + HT + h);
+            x.x += f * y.x;
+            x.y += f * y.y;
+            x.z += f * y.z;
+            x.w += f * y.w;
+          }
+          const float inv = ll == 0.f ? 0.f : 1.f / ll;
+          const long long at = out0 + e0;
+          store_row(a.out, a.row_type, at, x.x * inv);
+          store_row(a.out, a.row_type, at + 1, x.y * inv);
+          store_row(a.out, a.row_type, at + 2, x.z * inv);
+          store_row(a.out, a.row_type, at + 3, x.w * inv);
+          if (a.lse && e0 % DH == 0)
+            a.lse[lse0 + h] = ll == 0.f ? -INFINITY : (mm - kLift + log2f(ll)) * 0.693147180559945f;
+        }
+        if (tid == 0) a.tickets[first] = 0;   // ready for the next call
+      }
+      __syncthreads();   // the region and the flag are read
+    }
+
+    u += t1 - t0;
+    cur.t = t1;
+    if (u < u_hi) next_history(cur, &cur_first);
+  }
+  cp_wait<0>();
+}
+
+template <int CT, int DH, int HT, int PL>
+int launch_one(const PagedAttnArgs& a, cudaStream_t st) {
+  using C = Cfg<CT, DH, HT, PL>;
+  auto* k = paged_attend_kernel<CT, DH, HT, PL>;
+  static DeviceOnce setup;
+  if (setup.ensure([&](int) {
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) == cudaSuccess ? 0 : -3;
+      }))
+    return -3;
+  const long long most = (long long)a.width * a.kv.page_size;
+  const long long units =
+      (long long)a.n_req * a.kv.n_kv * ((a.group + HT - 1) / HT) * ((most + C::UK - 1) / C::UK);
+  const int grid = (int)std::max<long long>(1, std::min<long long>(kAttnMaxCtas, units));
+  return launch_pdl(k, dim3(grid), dim3(kAttnWarps * 32), C::kSmem, st, a);
+}
+
+template <int CT, int PL>
+int launch_type(const PagedAttnArgs& a, cudaStream_t st) {
+  const bool wide = a.group > 8;
+  switch (a.kv.dh) {
+    case 32: return wide ? launch_one<CT, 32, 16, PL>(a, st) : launch_one<CT, 32, 8, PL>(a, st);
+    case 64: return wide ? launch_one<CT, 64, 16, PL>(a, st) : launch_one<CT, 64, 8, PL>(a, st);
+    case 96: return wide ? launch_one<CT, 96, 16, PL>(a, st) : launch_one<CT, 96, 8, PL>(a, st);
+    default: return wide ? launch_one<CT, 128, 16, PL>(a, st) : launch_one<CT, 128, 8, PL>(a, st);
+  }
+}
+
+}  // namespace attn
+
+int paged_attend_f32(const PagedAttnArgs& a, cudaStream_t st);
+int paged_attend_f16(const PagedAttnArgs& a, cudaStream_t st);
+int paged_attend_bf16(const PagedAttnArgs& a, cudaStream_t st);
+int paged_attend_q8(const PagedAttnArgs& a, cudaStream_t st);
+
+}  // namespace tb2

@@ -1,0 +1,6 @@
+// Paged decode attention over an f16 cache.
+#include "paged_attn.cuh"
+
+namespace tb2 {
+int paged_attend_f16(const PagedAttnArgs& a, cudaStream_t st) { return attn::launch_type<kCacheF16, 2>(a, st); }
+}  // namespace tb2

@@ -1,0 +1,6 @@
+// Paged decode attention over an f32 cache.
+#include "paged_attn.cuh"
+
+namespace tb2 {
+int paged_attend_f32(const PagedAttnArgs& a, cudaStream_t st) { return attn::launch_type<kCacheF32, 2>(a, st); }
+}  // namespace tb2

@@ -1,0 +1,6 @@
+// Paged decode attention over an Q8_0 cache.
+#include "paged_attn.cuh"
+
+namespace tb2 {
+int paged_attend_q8(const PagedAttnArgs& a, cudaStream_t st) { return attn::launch_type<kCacheQ8, 2>(a, st); }
+}  // namespace tb2

@@ -273,7 +273,7 @@ int tb2_paged_plan(const tb2_paged_plan_args* a, void* stream) {
   if (!a->lens || !a->add || !a->table || !a->state || !a->lens_out || !a->state_out || !a->cu_tokens ||
       (a->n_free && !a->free_pages) || (a->n_tokens && (!a->slots || !a->positions || !a->requests)))
     return -1;
-  if ((long long)a->table_width * a->page_size > 0x7fffffffLL) return -1;   // positions are 32 bits wide
+  if ((long long)a->table_width * a->page_size > 0x7fffff00LL) return -1;   // positions are 32 bits wide
   int* err = tb2::device_error_word();
   if (!err) return -3;
   return tb2::paged_plan_launch(*a, err, static_cast<cudaStream_t>(stream));
@@ -286,7 +286,7 @@ int tb2_paged_release(const tb2_paged_release_args* a, void* stream) {
   if (!a->lens || !a->done || !a->table || !a->state || !a->lens_out || !a->state_out ||
       (a->n_free && !a->free_pages))
     return -1;
-  if ((long long)a->table_width * a->page_size > 0x7fffffffLL) return -1;
+  if ((long long)a->table_width * a->page_size > 0x7fffff00LL) return -1;
   int* err = tb2::device_error_word();
   if (!err) return -3;
   return tb2::paged_release_launch(*a, err, static_cast<cudaStream_t>(stream));
