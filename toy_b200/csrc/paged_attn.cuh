@@ -41,7 +41,7 @@
 namespace tb2 {
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnMaxCtas = 2 * 148;   // the workspace's slots
+constexpr int kAttnMaxCtas = 3 * 148;   // the workspace's slots
 constexpr int kAttnSlotFloats = 16 * 128 + 2 * 16;
 // tickets, then two partial slots per CTA
 constexpr size_t kAttnTicketBytes = (kAttnMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
@@ -135,6 +135,7 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint4& a, uint32_t b0
   if constexpr (CT == kCacheBF16) mma_bf16(d, a, b0, b1);
   else mma_f16(d, a, b0, b1);
 }
+__device__ __forceinline__ void zero(float (&d)[4]) { d[0] = d[1] = d[2] = d[3] = 0.f; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -189,7 +190,8 @@ struct Cfg {
                             : CT == kCacheQ8 ? (DH == 32 ? 64 : 32)
                                                : (DH == 32 ? 64 : DH == 64 ? 32 : 16);
   static constexpr int UK = TK * kAttnWarps;   // keys of a unit
-  static constexpr int ST = CT == kCacheQ8 && DH <= 64 ? 4 : 3;
+  static constexpr int ST = CT == kCacheQ8 && DH <= 64 ? 3 : 2;
+  static constexpr int OCC = HT == 8 ? 3 : 2;   // CTAs on an SM
   // row pitches in shared memory: rows lie dense and are swizzled, but for
   // Q8_0 widths whose rows are too short to swizzle
   static constexpr int KP = DH * E;
@@ -207,7 +209,10 @@ struct Cfg {
   // register sets of q: planes that do not share an instruction
   static constexpr int QS = CT == kCacheBF16 ? (HT == 8 ? PL - 1 : PL) : (HT == 8 ? 1 : 2);
   static constexpr int kQBytes = QS * KS * 512;
-  static constexpr int kBufs = HT == 8 ? 2 : 1;       // join buffers
+  static constexpr int kBufs = HT == 8 && !(CT == kCacheQ8 && DH == 128) ? 2 : 1;   // join buffers
+  // separate score accumulators (short chains of dependent products; an f32
+  // cache's small products apart from its large ones)
+  static constexpr int A = CT == kCacheF32 ? (NT >= 4 ? 2 : 4) : NT >= 8 ? 1 : 2;
   static constexpr int kBufFloats = (OT * OV + 2 * R) * 32;
   static constexpr int kJoinBytes = kBufs * kBufFloats * 4;
   static constexpr int kScanBytes = (kAttnWarps * 32 + 1) * 8;
@@ -261,7 +266,7 @@ struct Cursor {
 };
 
 template <int CT, int DH, int HT, int PL>
-__global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) paged_attend_kernel(const PagedAttnArgs a) {
   using C = Cfg<CT, DH, HT, PL>;
   constexpr int TK = C::TK, UK = C::UK, NT = C::NT, OT = C::OT, R = C::R, ST = C::ST;
   // weights are kept times 2^14 where they are rounded to f16, so that small
@@ -451,10 +456,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
   };
   fetch_pages();
 #pragma unroll
-  for (int i = 0; i < ST - 1; ++i) issue();
+  for (int i = 0; i < ST; ++i) issue();
 
   // ---- this warp's sums over the current history
-  float o[OT][4], m[R], l[R], fac[R];
+  float o[OT][C::OV], m[R], l[R], fac[R];
   float inv_d = 0.f;   // Q8_0: V's block scales are used times inv_d, a power of two near 1 / the largest so far
   int stage_out = 0;
   long long u = u_lo;
@@ -561,13 +566,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+      for (int k = 0; k < C::OV; ++k) o[i][k] = 0.f;
     if constexpr (CT == kCacheQ8) inv_d = 0.f;
     const uint32_t qb = smem_u32(region) + lane * 16;
 
     for (int t = t0; t < t1; ++t) {
       if ((t * kAttnWarps + warp) * TK >= cur.len) break;
-      cp_wait<ST - 2>();
+      cp_wait<ST - 1>();
       __syncwarp();
       const uint32_t ks = ring + stage_out * C::kStage, vs = ks + C::kOffV;
       const uint64_t ok = valid[warp][stage_out];
@@ -614,11 +619,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
           }
         }
       } else {
-        float d[NT][4];
+        float d[NT][C::A][4];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) d[i][k] = 0.f;
+          for (int k = 0; k < C::A; ++k) zero(d[i][k]);
 #pragma unroll
         for (int st = 0; st < C::KS; st += 2) {   // one 16-byte read of each key row feeds two steps
           uint4 qa[C::QS][2];
@@ -639,28 +644,30 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
               }
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                mma_tf32(d[i], qa[0][k], lo[2 * k], lo[2 * k + 1]);
-                if constexpr (HT == 16) mma_tf32(d[i], qa[1][k], hi[2 * k], hi[2 * k + 1]);
-                mma_tf32(d[i], qa[0][k], hi[2 * k], hi[2 * k + 1]);
+                float (&small)[4] = d[i][C::A == 4 ? 2 + k : 1], (&large)[4] = d[i][C::A == 4 ? k : 0];
+                mma_tf32(small, qa[0][k], lo[2 * k], lo[2 * k + 1]);
+                if constexpr (HT == 16) mma_tf32(small, qa[1][k], hi[2 * k], hi[2 * k + 1]);
+                mma_tf32(large, qa[0][k], hi[2 * k], hi[2 * k + 1]);
               }
             } else {
 #pragma unroll
               for (int p = C::QS - 1; p >= 0; --p) {
-                mma16<CT>(d[i], qa[p][0], w.x, w.y);
-                mma16<CT>(d[i], qa[p][1], w.z, w.w);
+                mma16<CT>(d[i][0], qa[p][0], w.x, w.y);
+                mma16<CT>(d[i][C::A - 1], qa[p][1], w.z, w.w);
               }
             }
           }
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          if constexpr (HT == 8) {
-            s[i][0] = d[i][0] + d[i][2];
-            s[i][1] = d[i][1] + d[i][3];
-          } else {
+          float x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[i][k] = d[i][k];
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (C::A == 4) x[k] = (d[i][0][k] + d[i][1][k]) + (d[i][2][k] + d[i][3][k]);
+            else x[k] = C::A == 2 ? d[i][0][k] + d[i][C::A - 1][k] : d[i][0][k];
           }
+#pragma unroll
+          for (int k = 0; k < 2 * R; ++k) s[i][k] = HT == 8 ? x[k] + x[(k + 2) & 3] : x[k];
         }
       }
 
@@ -719,7 +726,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
 #pragma unroll
         for (int i = 0; i < OT; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[i][k] *= shrink[R == 1 ? 0 : k >> 1];
+          for (int k = 0; k < C::OV; ++k) o[i][k] *= shrink[R == 1 ? 0 : k >> 1];
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -734,28 +741,40 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
           }
       }
 
-      // sums of weighted values
+      // sums of weighted values: a tile's products in fresh accumulators, added
+      // to the running sums by f32 adds (the tensor core's own sums are cut,
+      // not rounded, which would add up over a long history)
+      auto gather = [&](int i, const float (&d)[4]) {
+#pragma unroll
+        for (int k = 0; k < C::OV; ++k) o[i][k] += HT == 8 ? d[k] + d[(k + 2) & 3] : d[k];
+      };
       if constexpr (CT == kCacheF32) {
+        uint4 ph[NT], pl[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {   // 8 keys: step k holds key 2 k, step k + 4 key 2 k + 1
-          uint4 ph, pl;
           if constexpr (HT == 8) {
-            ph.x = tf32(s[i][0]);
-            ph.z = tf32(s[i][1]);
-            ph.y = tf32(s[i][0] - __uint_as_float(ph.x));
-            ph.w = tf32(s[i][1] - __uint_as_float(ph.z));
+            ph[i].x = tf32(s[i][0]);
+            ph[i].z = tf32(s[i][1]);
+            ph[i].y = tf32(s[i][0] - __uint_as_float(ph[i].x));
+            ph[i].w = tf32(s[i][1] - __uint_as_float(ph[i].z));
           } else {
-            ph.x = tf32(s[i][0]);
-            ph.y = tf32(s[i][2]);
-            ph.z = tf32(s[i][1]);
-            ph.w = tf32(s[i][3]);
-            pl.x = tf32(s[i][0] - __uint_as_float(ph.x));
-            pl.y = tf32(s[i][2] - __uint_as_float(ph.y));
-            pl.z = tf32(s[i][1] - __uint_as_float(ph.z));
-            pl.w = tf32(s[i][3] - __uint_as_float(ph.w));
+            ph[i].x = tf32(s[i][0]);
+            ph[i].y = tf32(s[i][2]);
+            ph[i].z = tf32(s[i][1]);
+            ph[i].w = tf32(s[i][3]);
+            pl[i].x = tf32(s[i][0] - __uint_as_float(ph[i].x));
+            pl[i].y = tf32(s[i][2] - __uint_as_float(ph[i].y));
+            pl[i].z = tf32(s[i][1] - __uint_as_float(ph[i].z));
+            pl[i].w = tf32(s[i][3] - __uint_as_float(ph[i].w));
           }
+        }
 #pragma unroll
-          for (int q4 = 0; q4 < DH / 32; ++q4) {   // columns 32 q4 + 4 g .. + 3: one per output tile
+        for (int q4 = 0; q4 < DH / 32; ++q4) {   // columns 32 q4 + 4 g .. + 3: one per output tile
+          float d[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) zero(d[k]);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
             const uint4 w0 = lds128(vs + C::v_at(8 * i + 2 * c, 8 * q4 + g));
             const uint4 w1 = lds128(vs + C::v_at(8 * i + 2 * c + 1, 8 * q4 + g));
             const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
@@ -764,17 +783,22 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
               const uint32_t a0 = tf32(__uint_as_float(x0[k])), a1 = tf32(__uint_as_float(x1[k]));
               const uint32_t e0 = tf32(__uint_as_float(x0[k]) - __uint_as_float(a0));
               const uint32_t e1 = tf32(__uint_as_float(x1[k]) - __uint_as_float(a1));
-              mma_tf32(o[4 * q4 + k], ph, e0, e1);
-              if constexpr (HT == 16) mma_tf32(o[4 * q4 + k], pl, a0, a1);
-              mma_tf32(o[4 * q4 + k], ph, a0, a1);
+              mma_tf32(d[k], ph[i], e0, e1);
+              if constexpr (HT == 16) mma_tf32(d[k], pl[i], a0, a1);
+              mma_tf32(d[k], ph[i], a0, a1);
             }
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) gather(4 * q4 + k, d[k]);
         }
       } else if constexpr (CT == kCacheQ8) {
 #pragma unroll
-        for (int i = 0; i < NT; i += 2) {   // 16 keys
+        for (int blk = 0; blk < C::NB; ++blk) {
+          float d[4][4];
 #pragma unroll
-          for (int blk = 0; blk < C::NB; ++blk) {
+          for (int k = 0; k < 4; ++k) zero(d[k]);
+#pragma unroll
+          for (int i = 0; i < NT; i += 2) {   // 16 keys
             float dv[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -814,26 +838,29 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
             for (int k = 0; k < 4; ++k) {
               const uint32_t sel = k & 1 ? 0x4342 : 0x4140;
               const uint32_t b0 = i8pair_f16(k < 2 ? p0 : p1, sel), b1 = i8pair_f16(k < 2 ? p2 : p3, sel);
-              if constexpr (HT == 16) mma_f16(o[4 * blk + k], pl, b0, b1);
-              mma_f16(o[4 * blk + k], ph, b0, b1);
+              if constexpr (HT == 16) mma_f16(d[k], pl, b0, b1);
+              mma_f16(d[k], ph, b0, b1);
             }
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) gather(4 * blk + k, d[k]);
         }
       } else {
+        constexpr int kP = HT == 8 ? (PL == 3 ? 2 : 1) : PL;   // operand sets
+        uint4 pp[NT / 2][kP];
 #pragma unroll
         for (int i = 0; i < NT; i += 2) {   // 16 keys
-          constexpr int kP = HT == 8 ? (PL == 3 ? 2 : 1) : PL;   // operand sets
-          uint4 pp[kP];
+          uint4 (&p)[kP] = pp[i / 2];
           if constexpr (HT == 8) {
             float x0 = s[i][0], x1 = s[i][1], x2 = s[i + 1][0], x3 = s[i + 1][1];
-            pp[0].x = plane16<CT>(x0, x1);
-            pp[0].z = plane16<CT>(x2, x3);
-            pp[0].y = plane16<CT>(x0, x1);
-            pp[0].w = plane16<CT>(x2, x3);
+            p[0].x = plane16<CT>(x0, x1);
+            p[0].z = plane16<CT>(x2, x3);
+            p[0].y = plane16<CT>(x0, x1);
+            p[0].w = plane16<CT>(x2, x3);
             if constexpr (kP == 2) {
-              pp[1].x = plane16<CT>(x0, x1);
-              pp[1].z = plane16<CT>(x2, x3);
-              pp[1].y = pp[1].w = 0;
+              p[1].x = plane16<CT>(x0, x1);
+              p[1].z = plane16<CT>(x2, x3);
+              p[1].y = p[1].w = 0;
             }
           } else {
             float x[8];
@@ -843,23 +870,31 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
               x[4 + k] = s[i + 1][k];
             }
 #pragma unroll
-            for (int p = 0; p < kP; ++p) {
-              pp[p].x = plane16<CT>(x[0], x[1]);
-              pp[p].y = plane16<CT>(x[2], x[3]);
-              pp[p].z = plane16<CT>(x[4], x[5]);
-              pp[p].w = plane16<CT>(x[6], x[7]);
+            for (int q = 0; q < kP; ++q) {
+              p[q].x = plane16<CT>(x[0], x[1]);
+              p[q].y = plane16<CT>(x[2], x[3]);
+              p[q].z = plane16<CT>(x[4], x[5]);
+              p[q].w = plane16<CT>(x[6], x[7]);
             }
           }
+        }
 #pragma unroll
-          for (int d2 = 0; d2 < OT; d2 += 2) {
+        for (int d2 = 0; d2 < OT; d2 += 2) {
+          float e0[4], e1[4];
+          zero(e0);
+          zero(e1);
+#pragma unroll
+          for (int i = 0; i < NT; i += 2) {
             uint32_t b[4];   // keys 0..7 and 8..15 of columns 8 d2 .., then of 8 d2 + 8 ..
             ldmatrix_x4_trans(vs + C::v_at(8 * i + (lane & 15), d2 + (lane >> 4)), b);
 #pragma unroll
             for (int p = kP - 1; p >= 0; --p) {
-              mma16<CT>(o[d2], pp[p], b[0], b[1]);
-              mma16<CT>(o[d2 + 1], pp[p], b[2], b[3]);
+              mma16<CT>(e0, pp[i / 2][p], b[0], b[1]);
+              mma16<CT>(e1, pp[i / 2][p], b[2], b[3]);
             }
           }
+          gather(d2, e0);
+          gather(d2 + 1, e1);
         }
       }
       __syncwarp();   // the stage is read
@@ -873,7 +908,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attend_kernel(const Pag
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int k = 0; k < C::OV; ++k) ov[i][k] = (HT == 8 ? o[i][k] + o[i][(k + 2) & 3] : o[i][k]) * back;
+      for (int k = 0; k < C::OV; ++k) ov[i][k] = o[i][k] * back;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -1030,7 +1065,7 @@ int launch_one(const PagedAttnArgs& a, cudaStream_t st) {
   const long long most = (long long)a.width * a.kv.page_size;
   const long long units =
       (long long)a.n_req * a.kv.n_kv * ((a.group + HT - 1) / HT) * ((most + C::UK - 1) / C::UK);
-  const int grid = (int)std::max<long long>(1, std::min<long long>(kAttnMaxCtas, units));
+  const int grid = (int)std::max<long long>(1, std::min<long long>(C::OCC * 148, units));
   return launch_pdl(k, dim3(grid), dim3(kAttnWarps * 32), C::kSmem, st, a);
 }
 

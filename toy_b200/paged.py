@@ -24,36 +24,44 @@ from ._lib import PagedAppendArgs, PagedAttendArgs, PagedKV, PagedPlanArgs, Page
 _ROW = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _CACHE = {**_ROW, torch.int8: 8}
 _prepared: set = set()
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError("toy_b200.paged: " + what)
+def _bad(what: str):
+    raise ValueError("toy_b200.paged: " + what)
 
 
-class _on:
-    """The device of a call's tensors made current where it is not (and its error word set up once)."""
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-        self.prev = torch.cuda.current_device()
-
-    def __enter__(self) -> int:
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        if self.index not in _prepared:
-            check(lib().tb2_paged_prepare(), "tb2_paged_prepare")
-            _prepared.add(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _ints(t: torch.Tensor, n: int, device, what: str, dtype=torch.int32) -> int:
-    _need(t.dtype == dtype and t.device == device and t.is_contiguous() and t.numel() >= n,
-          f"{what}: a contiguous {dtype} tensor of {n} or more on {device}")
+# (the same handle without the Stream object around it, where torch has it: these calls cost microseconds)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _prepare(index: int) -> None:
+    with torch.cuda.device(index):
+        check(lib().tb2_paged_prepare(), "tb2_paged_prepare")
+    _prepared.add(index)
+
+
+def _call(index: int, what: str, *args) -> None:
+    """An entry point on torch's current stream of GPU `index`, which is made current for the call where it is not."""
+    if index not in _prepared:
+        _prepare(index)
+    f = getattr(lib(), what)
+    if torch.cuda.current_device() == index:
+        rc = f(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
+
+
+def _ints(t: torch.Tensor, n: int, index: int, what: str, dtype=_I32) -> int:
+    if t.dtype is not dtype or t.get_device() != index or t.numel() < n or not t.is_contiguous():
+        _bad(f"{what}: a contiguous {dtype} tensor of {n} or more on cuda:{index}")
     return t.data_ptr()
 
 
@@ -65,26 +73,30 @@ class PagedCache:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
-        _need(k.is_cuda and k.dim() == 4 and k.dtype in _CACHE, "k: a CUDA tensor [n_pages, n_kv, page_size, d_head]")
-        _need(v.shape == k.shape and v.dtype == k.dtype and v.device == k.device and v.stride() == k.stride(),
-              "v: shape, type, device and strides of k")
-        _need(k.stride(3) == 1, "rows of d_head values are contiguous")
+        if not k.is_cuda or k.dim() != 4 or k.dtype not in _CACHE:
+            _bad("k: a CUDA tensor [n_pages, n_kv, page_size, d_head]")
+        if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or v.stride() != k.stride():
+            _bad("v: shape, type, device and strides of k")
+        if k.stride(3) != 1:
+            _bad("rows of d_head values are contiguous")
         q8 = k.dtype == torch.int8
-        _need((k_scale is not None) == q8 and (v_scale is not None) == q8, "scales belong to int8 pools, and only there")
+        if (k_scale is not None) != q8 or (v_scale is not None) != q8:
+            _bad("scales belong to int8 pools, and only there")
         # an axis of size 1 has no stride of its own
         n_pages, n_kv, page, dh = k.shape
         strides = [k.stride(i) if k.shape[i] > 1 else k.numel() for i in range(3)]
         if q8:
             for s in (k_scale, v_scale):
-                _need(s.dtype == torch.float16 and s.device == k.device and s.shape == k.shape[:3] + (dh // 32,),
-                      "scales: fp16 [n_pages, n_kv, page_size, d_head / 32] on the pools' device")
-                _need(all(s.shape[i] == 1 or s.stride(i) * 32 == k.stride(i) for i in range(3)) and
-                      (s.shape[3] == 1 or s.stride(3) == 1), "scales: the pools' strides divided by 32")
+                if s.dtype != torch.float16 or s.device != k.device or s.shape != k.shape[:3] + (dh // 32,):
+                    _bad("scales: fp16 [n_pages, n_kv, page_size, d_head / 32] on the pools' device")
+                if any(s.shape[i] > 1 and s.stride(i) * 32 != k.stride(i) for i in range(3)) or \
+                        (s.shape[3] > 1 and s.stride(3) != 1):
+                    _bad("scales: the pools' strides divided by 32")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device, self.shape = k.device, k.shape
+        self.device, self.index, self.shape = k.device, k.get_device(), k.shape
         self.c = PagedKV(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None,
                          v_scale.data_ptr() if q8 else None, _CACHE[k.dtype], n_pages, page, n_kv, dh, *strides)
-        self._ref = C.byref(self.c)
+        self.ref = C.byref(self.c)
 
 
 class Plan(NamedTuple):
@@ -97,14 +109,15 @@ class Plan(NamedTuple):
     requests: torch.Tensor    # [n_tokens] i32, -1 past the step's tokens
 
 
-def _table(table: torch.Tensor, n: int, device) -> None:
-    _need(table.dim() == 2 and table.shape[0] >= n and table.dtype == torch.int32 and table.device == device and
-          table.shape[1] >= 1 and table.stride(1) == 1 and (table.shape[0] == 1 or table.stride(0) >= table.shape[1]),
-          "table: int32 [n_req, width] on the lengths' device, rows contiguous")
-
-
-def _table_stride(table: torch.Tensor) -> int:
-    return max(table.stride(0), table.shape[1])
+def _table(table: torch.Tensor, n: int, index: int) -> tuple:
+    """(pointer, width, row stride) of a block table [n or more, width]."""
+    if table.dim() != 2 or table.dtype is not _I32 or table.get_device() != index:
+        _bad(f"table: int32 [n_req, width] on cuda:{index}")
+    rows, width = table.shape
+    stride, one = table.stride()
+    if rows < n or width < 1 or (one != 1 and width > 1) or (rows > 1 and stride < width):
+        _bad("table: a contiguous row of at least one page per request")
+    return table.data_ptr(), width, stride if rows > 1 else width
 
 
 def plan(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, state: torch.Tensor, *,
@@ -113,22 +126,27 @@ def plan(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages:
     int32 {free pages on the stack, ..}; `table` is extended in place; n_tokens is the room of the slot map (at least
     the sum of add). `out` may hold lens and state themselves. Check state[1] of the result when it reaches the host:
     a status other than 0 left everything as it was."""
-    n, dev = lens.numel(), lens.device
-    _need(lens.is_cuda and n >= 1 and 0 <= n_tokens < 2**31, "lens on a GPU, n_tokens not negative")
-    _table(table, n, dev)
-    if out is None:
-        i32 = lambda k: torch.empty(k, device=dev, dtype=torch.int32)  # noqa: E731
-        out = Plan(i32(n), i32(4), i32(n + 1), torch.empty(n_tokens, device=dev, dtype=torch.int64), i32(n_tokens),
-                   i32(n_tokens))
-    a = PagedPlanArgs(_ints(lens, n, dev, "lens"), _ints(add, n, dev, "add"), n, table.data_ptr(), table.shape[1],
-                      _table_stride(table), _ints(free_pages, 0, dev, "free_pages"), free_pages.numel(),
-                      _ints(state, 4, dev, "state"), page_size, n_pages, n_tokens, _ints(out.lens, n, dev, "out.lens"),
-                      _ints(out.state, 4, dev, "out.state"), _ints(out.cu_tokens, n + 1, dev, "out.cu_tokens"),
-                      _ints(out.slots, n_tokens, dev, "out.slots", torch.int64),
-                      _ints(out.positions, n_tokens, dev, "out.positions"),
-                      _ints(out.requests, n_tokens, dev, "out.requests"))
-    with _on(dev) as st:
-        check(lib().tb2_paged_plan(C.byref(a), st), "tb2_paged_plan")
+    n, dev = lens.numel(), lens.get_device()
+    if dev < 0 or n < 1 or not 0 <= n_tokens < 2**31:
+        _bad("lens: on a GPU, of one request or more; n_tokens not negative")
+    tp, width, stride = _table(table, n, dev)
+    if out is None:   # two allocations, each part on a 16-byte boundary
+        n4, t4 = (n + 4) & ~3, (n_tokens + 3) & ~3
+        part = lens.new_empty(2 * n4 + 4 + 2 * t4, dtype=_I32)
+        cu = n4 + 4
+        out = Plan(part[:n], part[n4:cu], part[cu:cu + n + 1], lens.new_empty(n_tokens, dtype=_I64),
+                   part[cu + n4:cu + n4 + n_tokens], part[cu + n4 + t4:cu + n4 + t4 + n_tokens])
+        lp = part.data_ptr()
+        outs = (lp, lp + 4 * n4, lp + 4 * cu, out.slots.data_ptr(), lp + 4 * (cu + n4), lp + 4 * (cu + n4 + t4))
+    else:
+        outs = (_ints(out.lens, n, dev, "out.lens"), _ints(out.state, 4, dev, "out.state"),
+                _ints(out.cu_tokens, n + 1, dev, "out.cu_tokens"), _ints(out.slots, n_tokens, dev, "out.slots", _I64),
+                _ints(out.positions, n_tokens, dev, "out.positions"),
+                _ints(out.requests, n_tokens, dev, "out.requests"))
+    a = PagedPlanArgs(_ints(lens, n, dev, "lens"), _ints(add, n, dev, "add"), n, tp, width, stride,
+                      _ints(free_pages, 0, dev, "free_pages"), free_pages.numel(), _ints(state, 4, dev, "state"),
+                      page_size, n_pages, n_tokens, *outs)
+    _call(dev, "tb2_paged_plan", C.byref(a))
     return out
 
 
@@ -137,24 +155,26 @@ def release(lens: torch.Tensor, done: torch.Tensor, table: torch.Tensor, free_pa
             state_out: Optional[torch.Tensor] = None) -> None:
     """The pages of every request with done[b] != 0 go back on the stack, its table row is cleared and its length set
     to 0; lens and state are updated in place unless other tensors are given."""
-    n, dev = lens.numel(), lens.device
-    _need(lens.is_cuda and n >= 1, "lens on a GPU")
-    _table(table, n, dev)
-    a = PagedReleaseArgs(_ints(lens, n, dev, "lens"), _ints(done, n, dev, "done"), n, table.data_ptr(),
-                         table.shape[1], _table_stride(table), _ints(free_pages, 0, dev, "free_pages"),
-                         free_pages.numel(), _ints(state, 4, dev, "state"), page_size, n_pages,
-                         _ints(lens if lens_out is None else lens_out, n, dev, "lens_out"),
+    n, dev = lens.numel(), lens.get_device()
+    if dev < 0 or n < 1:
+        _bad("lens: on a GPU, of one request or more")
+    a = PagedReleaseArgs(_ints(lens, n, dev, "lens"), _ints(done, n, dev, "done"), n, *_table(table, n, dev),
+                         _ints(free_pages, 0, dev, "free_pages"), free_pages.numel(), _ints(state, 4, dev, "state"),
+                         page_size, n_pages, _ints(lens if lens_out is None else lens_out, n, dev, "lens_out"),
                          _ints(state if state_out is None else state_out, 4, dev, "state_out"))
-    with _on(dev) as st:
-        check(lib().tb2_paged_release(C.byref(a), st), "tb2_paged_release")
+    _call(dev, "tb2_paged_release", C.byref(a))
 
 
-def _rows(t: torch.Tensor, n: int, heads: int, dh: int, dtype, device, what: str) -> int:
-    """[n, heads, dh] with the last two axes dense: the row stride."""
-    _need(t.dim() == 3 and t.shape == (n, heads, dh) and t.dtype == dtype and t.device == device and
-          t.stride(2) == 1 and (heads == 1 or t.stride(1) == dh) and (n == 1 or t.stride(0) >= heads * dh),
-          f"{what}: {dtype} [{n}, {heads}, {dh}] on {device}, each token's heads contiguous")
-    return t.stride(0) if n > 1 else heads * dh
+def _rows(t: torch.Tensor, n: int, heads: int, dh: int, dtype, index: int, what: str) -> int:
+    """The row stride of t [n, heads, dh], its last two axes dense."""
+    if t.dim() == 3 and t.dtype is dtype and t.get_device() == index:
+        s0, s1, s2 = t.stride()
+        if t.shape == (n, heads, dh) and s2 == 1 and (s1 == dh or heads == 1):
+            if n <= 1:
+                return heads * dh
+            if s0 >= heads * dh:
+                return s0
+    _bad(f"{what}: {dtype} [{n}, {heads}, {dh}] on cuda:{index}, each token's heads contiguous")
 
 
 def append(cache: PagedCache, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -165,45 +185,49 @@ def append(cache: PagedCache, slots: torch.Tensor, k: torch.Tensor, v: torch.Ten
     into q_out (made when None; may be q). rope: f32 [rows, d_head / 2, 2] (cos, sin), indexed by positions; bias:
     f32 [(n_heads + 2 n_kv) d_head], added first. Returns q_out."""
     _, n_kv, _, dh = cache.shape
-    n, dev = k.shape[0], cache.device
-    _need(k.dtype in _ROW, "rows are f32, f16 or bf16")
-    ldk, ldv = _rows(k, n, n_kv, dh, k.dtype, dev, "k"), _rows(v, n, n_kv, dh, k.dtype, dev, "v")
+    dev, dt = cache.index, k.dtype
+    n = k.shape[0]
+    if dt not in _ROW:
+        _bad("rows are f32, f16 or bf16")
+    ldk, ldv = _rows(k, n, n_kv, dh, dt, dev, "k"), _rows(v, n, n_kv, dh, dt, dev, "v")
     heads = ldq = ldqo = 0
+    qp = op = bp = rp = pp = None
+    rows = 0
     if q is not None:
-        heads = q.shape[1]
-        ldq = _rows(q, n, heads, dh, k.dtype, dev, "q")
+        heads = q.shape[1] if q.dim() == 3 else 0
+        ldq = _rows(q, n, heads, dh, dt, dev, "q")
         if q_out is None:
-            q_out = torch.empty((n, heads, dh), device=dev, dtype=q.dtype)
-        ldqo = _rows(q_out, n, heads, dh, k.dtype, dev, "q_out")
-    _need(rope is None or (positions is not None and rope.dtype == torch.float32 and rope.device == dev and
-                           rope.is_contiguous() and rope.shape[1:] == (dh // 2, 2)),
-          "rope: contiguous f32 [rows, d_head / 2, 2] with positions")
+            q_out = q.new_empty((n, heads, dh))
+        ldqo = _rows(q_out, n, heads, dh, dt, dev, "q_out")
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    if rope is not None:
+        if positions is None or rope.dtype is not _F32 or rope.get_device() != dev or not rope.is_contiguous() or \
+                rope.dim() != 3 or rope.shape[1:] != (dh // 2, 2):
+            _bad("rope: contiguous f32 [rows, d_head / 2, 2] with positions")
+        rp, rows = rope.data_ptr(), rope.shape[0]
+    if positions is not None:
+        pp = _ints(positions, n, dev, "positions")
     if bias is not None:
         # without q the bias still has the layout of a whole row: [n_heads | n_kv | n_kv], n_heads from its length
         if q is None:
             heads = bias.numel() // dh - 2 * n_kv
-        _need(bias.dtype == torch.float32 and bias.device == dev and bias.is_contiguous() and heads >= 0 and
-              bias.numel() == (heads + 2 * n_kv) * dh, "bias: contiguous f32 [(n_heads + 2 n_kv) d_head]")
-    a = PagedAppendArgs(n, heads, _ROW[k.dtype], q.data_ptr() if q is not None else None, ldq, k.data_ptr(), ldk,
-                        v.data_ptr(), ldv, q_out.data_ptr() if q is not None else None, ldqo,
-                        bias.data_ptr() if bias is not None else None, rope.data_ptr() if rope is not None else None,
-                        rope.shape[0] if rope is not None else 0,
-                        _ints(positions, n, dev, "positions") if positions is not None else None,
-                        _ints(slots, n, dev, "slots", torch.int64))
-    with _on(dev) as st:
-        check(lib().tb2_paged_append(cache._ref, C.byref(a), st), "tb2_paged_append")
+        if bias.dtype is not _F32 or bias.get_device() != dev or not bias.is_contiguous() or heads < 0 or \
+                bias.numel() != (heads + 2 * n_kv) * dh:
+            _bad("bias: contiguous f32 [(n_heads + 2 n_kv) d_head]")
+        bp = bias.data_ptr()
+    a = PagedAppendArgs(n, heads, _ROW[dt], qp, ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, op, ldqo, bp, rp, rows, pp,
+                        _ints(slots, n, dev, "slots", _I64))
+    _call(dev, "tb2_paged_append", cache.ref, C.byref(a))
     return q_out
 
 
 def attend_workspace(device=None) -> torch.Tensor:
     """A workspace for `attend` on one GPU, set up. Calls that may overlap (two streams, two captured graphs) need one
     each."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    with _on(dev) as st:
-        w = torch.empty(lib().tb2_paged_attend_workspace(), device=dev, dtype=torch.uint8)
-        check(lib().tb2_paged_attend_workspace_init(w.data_ptr(), w.numel(), st), "tb2_paged_attend_workspace_init")
+    dev = torch.device("cuda" if device is None else device)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    w = torch.empty(lib().tb2_paged_attend_workspace(), device=torch.device("cuda", index), dtype=torch.uint8)
+    _call(index, "tb2_paged_attend_workspace_init", w.data_ptr(), w.numel())
     return w
 
 
@@ -214,25 +238,27 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lens: torch.
     lens int32 [n] (the new token counted); out [n, n_heads, d_head] of q's type, lse f32 [n, n_heads] when given.
     scale defaults to d_head^-0.5; a workspace is made for the call when None."""
     _, n_kv, _, dh = cache.shape
-    dev = cache.device
-    _need(q.dim() == 3 and q.dtype in _ROW, "q: f32, f16 or bf16 [n, n_heads, d_head]")
-    n, heads = q.shape[0], q.shape[1]
-    _need(heads >= 1 and heads % n_kv == 0, "n_heads is a multiple of the cache's n_kv")
-    ldq = _rows(q, n, heads, dh, q.dtype, dev, "q")
+    dev, dt = cache.index, q.dtype
+    if q.dim() != 3 or dt not in _ROW:
+        _bad("q: f32, f16 or bf16 [n, n_heads, d_head]")
+    n, heads, _ = q.shape
+    if heads < 1 or heads % n_kv:
+        _bad("n_heads is a multiple of the cache's n_kv")
+    ldq = _rows(q, n, heads, dh, dt, dev, "q")
     if out is None:
-        out = torch.empty((n, heads, dh), device=dev, dtype=q.dtype)
-    ldo = _rows(out, n, heads, dh, q.dtype, dev, "out")
-    _table(table, n, dev)
-    _need(lse is None or (lse.dtype == torch.float32 and lse.device == dev and lse.is_contiguous() and
-                          lse.shape == (n, heads)), "lse: contiguous f32 [n, n_heads]")
+        out = q.new_empty((n, heads, dh))
+    ldo = _rows(out, n, heads, dh, dt, dev, "out")
+    lp = None
+    if lse is not None:
+        if lse.dtype is not _F32 or lse.get_device() != dev or not lse.is_contiguous() or lse.shape != (n, heads):
+            _bad("lse: contiguous f32 [n, n_heads]")
+        lp = lse.data_ptr()
     if workspace is None:
-        workspace = attend_workspace(dev)
-    _need(workspace.device == dev and workspace.dtype == torch.uint8 and workspace.is_contiguous(),
-          "workspace: from attend_workspace, on the cache's device")
-    a = PagedAttendArgs(n, heads, _ROW[q.dtype], q.data_ptr(), ldq, out.data_ptr(), ldo, table.data_ptr(),
-                        table.shape[1], _table_stride(table), _ints(lens, n, dev, "lens"),
-                        dh ** -0.5 if scale is None else scale, lse.data_ptr() if lse is not None else None,
-                        workspace.data_ptr(), workspace.numel())
-    with _on(dev) as st:
-        check(lib().tb2_paged_attend(cache._ref, C.byref(a), st), "tb2_paged_attend")
+        workspace = attend_workspace(cache.device)
+    elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        _bad("workspace: from attend_workspace, on the cache's device")
+    a = PagedAttendArgs(n, heads, _ROW[dt], q.data_ptr(), ldq, out.data_ptr(), ldo, *_table(table, n, dev),
+                        _ints(lens, n, dev, "lens"), dh ** -0.5 if scale is None else scale, lp, workspace.data_ptr(),
+                        workspace.numel())
+    _call(dev, "tb2_paged_attend", cache.ref, C.byref(a))
     return out
