@@ -61,6 +61,7 @@ struct PagedAttnArgs {
   float* slots;
   int* err;
   float c;             // scale * log2(e)
+  bool q_vec;          // q rows start on 16-byte boundaries
   int n_req, n_heads, group, width, row_type, page_shift;   // page_shift < 0: page_size is no power of two
 };
 
@@ -147,6 +148,21 @@ __device__ __forceinline__ uint32_t tf32(float x) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
   return y;
 }
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 
 // Two values as one register of plane values (lower half first), what is left
 // of them going on to the next plane.
@@ -180,6 +196,29 @@ __device__ __forceinline__ uint32_t i8pair_f16(uint32_t w, uint32_t sel) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// The fp16 block scales of two neighbouring rows.
+template <int NB>
+struct ScalePair {
+  uint32_t w[NB];
+  __device__ __forceinline__ void load(uint32_t a) {   // a: a multiple of 4 NB bytes
+    if constexpr (NB == 4) {
+      const uint4 v = lds128(a);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (NB == 2) {
+      const uint2 v = lds64(a);
+      w[0] = v.x; w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) w[i] = lds32(a + 4 * i);
+    }
+  }
+  __device__ __forceinline__ float at(int row, int blk) const {
+    const int i = row * NB + blk;
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[i / 2]);
+    return i & 1 ? __high2float(h) : __low2float(h);
+  }
+};
+
 template <int CT, int DH, int HT, int PL>
 struct Cfg {
   static constexpr int E = CT == kCacheF32 ? 4 : CT == kCacheQ8 ? 1 : 2;
@@ -192,10 +231,13 @@ struct Cfg {
   static constexpr int UK = TK * kAttnWarps;   // keys of a unit
   static constexpr int ST = CT == kCacheQ8 && DH <= 64 ? 3 : 2;
   static constexpr int OCC = HT == 8 ? 3 : 2;   // CTAs on an SM
-  // row pitches in shared memory: rows lie dense and are swizzled, but for
-  // Q8_0 widths whose rows are too short to swizzle
-  static constexpr int KP = DH * E;
-  static constexpr int VP = DH * E + (CT == kCacheQ8 && DH != 128 ? 16 : 0);
+  // Row pitches in shared memory, so that the lanes that read at once meet no
+  // bank twice. 16-bit and f32 rows: 16 bytes of padding (a read covers chunks
+  // 2 c + e of rows g and g + 1, or one chunk of eight rows). Q8_0: K is read 8
+  // bytes at a time over four rows, V 4 bytes over every other row: rows of 128
+  // and 64 bytes are swizzled (k_swz, v_swz), narrow V rows padded.
+  static constexpr int KP = CT == kCacheQ8 ? DH : DH * E + 16;
+  static constexpr int VP = CT == kCacheQ8 ? (DH == 128 ? DH : DH + 16) : DH * E + 16;
   static constexpr int NB = DH / 32;   // Q8_0 blocks of a row
   static constexpr int SB = CT == kCacheQ8 ? TK * NB * 2 : 0;
   static constexpr int kOffV = TK * KP, kOffKS = kOffV + TK * VP, kOffVS = kOffKS + SB;
@@ -205,11 +247,13 @@ struct Cfg {
   static constexpr int OT = DH / 8;                   // 8-column tiles of the output
   static constexpr int R = HT / 8;                    // heads per lane group
   static constexpr int OV = HT == 8 ? 2 : 4;          // values of an output tile per lane, planes added
-  static constexpr int KS = CT == kCacheF32 ? DH / 8 : DH / 16;   // k steps of q . k
+  static constexpr int KS = 2 * (CT == kCacheF32 ? DH / 16 : DH / 32);   // k steps of q . k
   // register sets of q: planes that do not share an instruction
   static constexpr int QS = CT == kCacheBF16 ? (HT == 8 ? PL - 1 : PL) : (HT == 8 ? 1 : 2);
-  static constexpr int kQBytes = QS * KS * 512;
-  static constexpr int kBufs = HT == 8 && !(CT == kCacheQ8 && DH == 128) ? 2 : 1;   // join buffers
+  // (the third bf16 plane alone in its rows: half a set)
+  static constexpr bool kHalf = CT == kCacheBF16 && HT == 8 && PL == 3;
+  static constexpr int kQBytes = kHalf ? KS * 768 : QS * KS * 512;
+  static constexpr int kBufs = HT == 8 && DH < 128 ? 2 : 1;   // join buffers (one where three CTAs just fit)
   // separate score accumulators (short chains of dependent products; an f32
   // cache's small products apart from its large ones)
   static constexpr int A = CT == kCacheF32 ? (NT >= 4 ? 2 : 4) : NT >= 8 ? 1 : 2;
@@ -220,38 +264,58 @@ struct Cfg {
   static constexpr int kRegion = kRegion0 > kScanBytes ? kRegion0 : (kScanBytes + 15) / 16 * 16;
   static constexpr int kSmem = kAttnWarps * ST * kStage + kRegion;
 
-  // byte offset of 16-byte chunk ch of row r, so that the lanes that read at
-  // once meet no bank twice. K: the reads of two neighbouring rows (four for
-  // Q8_0) take 64 (32) bytes each; V: see the reads.
-  static __device__ __forceinline__ uint32_t k_at(int r, int ch) {
-    if constexpr (CT == kCacheQ8) {
-      if constexpr (DH == 128) ch ^= (r & 3) << 1;
-      if constexpr (DH == 64) ch ^= ((r >> 1) & 1) << 1;
-    } else if constexpr (CR % 8 == 0) {
-      ch ^= ((r & 1) << 2) | ((r >> 1) & 3);
-    } else {
-      ch ^= (r >> 1) & 3;
-    }
-    return r * KP + ch * 16;
+  // Q8_0: what the 16-byte chunks of row r are exchanged by.
+  static __device__ __forceinline__ int k_swz(int r) {
+    return CT != kCacheQ8 ? 0 : DH == 128 ? (r & 3) << 1 : DH == 64 ? ((r >> 1) & 1) << 1 : 0;
   }
-  static __device__ __forceinline__ uint32_t v_at(int r, int ch) {
-    if constexpr (CT == kCacheQ8) {
-      if constexpr (DH == 128) ch ^= ((r >> 1) & 3) << 1;
-    } else if constexpr (CT == kCacheF32) {
-      ch ^= ((r >> 1) & 3) << 1;
-    } else if constexpr (CR % 8 == 0) {
-      ch ^= ((r & 1) << 2) | ((r >> 1) & 3);
-    } else {
-      ch ^= (r >> 1) & 3;
-    }
-    return r * VP + ch * 16;
+  static __device__ __forceinline__ int v_swz(int r) { return CT == kCacheQ8 && DH == 128 ? ((r >> 1) & 3) << 1 : 0; }
+  // The 16-byte chunk of a key row that lane c of a group takes for step pair
+  // sp of q . k (for Q8_0 the 8 bytes c of block sp, in units of 8 bytes).
+  static __device__ __forceinline__ int chunk(int sp, int c) {
+    if constexpr (CT == kCacheQ8) return 4 * sp + c;
+    else return sp / 2 * 8 + (sp / 2 * 8 + 8 <= CR ? 2 * c + sp % 2 : c);
   }
+  static constexpr int QW = CT == kCacheF32 ? 4 : 8;   // values of q in such a chunk
+  static constexpr int SP = DH / (4 * QW);              // step pairs
+  // Rows of a tile that lie in one page when the page size is a multiple of 16.
+  static constexpr int PR = TK < 16 ? TK : 16;
+  static constexpr int NP = TK / PR;
 };
 
 __device__ __forceinline__ float load_row(const void* p, int type, long long at) {
   if (type == kTypeF32) return static_cast<const float*>(p)[at];
   if (type == kTypeF16) return __half2float(static_cast<const __half*>(p)[at]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
+}
+// W values from element `at`; vec: they start on a 16-byte (8 for 4 16-bit ones) boundary.
+template <int W>
+__device__ __forceinline__ void load_rows(const void* p, int type, bool vec, long long at, float* x) {
+  if (!vec) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) x[k] = load_row(p, type, at + k);
+  } else if (type == kTypeF32) {
+#pragma unroll
+    for (int k = 0; k < W; k += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + k);
+      x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
+    }
+  } else {
+    uint32_t w[W / 2];
+    if constexpr (W == 8) {
+      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+      w[0] = v.x; w[1] = v.y;
+    }
+#pragma unroll
+    for (int k = 0; k < W / 2; ++k) {
+      const float2 f = type == kTypeF16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
+                                        : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+      x[2 * k] = f.x;
+      x[2 * k + 1] = f.y;
+    }
+  }
 }
 __device__ __forceinline__ void store_row(void* p, int type, long long at, float x) {
   if (type == kTypeF32) static_cast<float*>(p)[at] = x;
@@ -381,70 +445,114 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   };
 
   // ---- the ring: tiles of this warp in list order
+  // Where the page size is a multiple of 16, the 16 rows (or the tile, if it
+  // has fewer) from a multiple of 16 on lie in one page: lane i reads the page
+  // id of piece i of the next tile, and a full tile of good pages is copied
+  // with an address per piece. Other page sizes, and the last tile of a
+  // history, take an address per row.
   Cursor pc = cur;             // the producer's place
   long long pu = u_lo;         // list index of its unit
-  int row_page[C::RPL];        // page ids of the next tile's rows (one per lane and 32 rows)
+  int page_id[C::RPL];         // page ids of the next tile's pieces (lane % NP), or rows (lane + 32 i)
+  constexpr bool kEven = 32 % C::CR == 0;   // a lane copies the same chunk of every row it has (not at d_head 96)
+  const bool pieces16 = kEven && P % 16 == 0;
   auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / P; };
-  auto skip_empty = [&]() {    // the last unit of a history may hold no tile of this warp
-    while (pu < u_hi && (pc.t * kAttnWarps + warp) * TK >= pc.len) {
+  auto tile_key = [&]() { return (pc.t * kAttnWarps + warp) * TK; };
+  auto row_key = [&](int i) { return tile_key() + (TK < 32 ? lane % TK : lane + 32 * i); };
+  auto read_page = [&](int key) {
+    return key < pc.len ? __ldg(a.table + pc.b * a.table_stride + page_of(key)) : -1;
+  };
+  auto fetch_pages = [&]() {
+    // (the last unit of a history may hold no tile of this warp)
+    while (pu < u_hi && tile_key() >= pc.len) {
       ++pu;
       if (++pc.t == pc.nt && pu < u_hi) next_history(pc, nullptr);
     }
-  };
-  auto fetch_pages = [&]() {
-    skip_empty();
     if (pu >= u_hi) return;
+    if (pieces16) {
+      page_id[0] = read_page(tile_key() + lane % C::NP * C::PR);
+    } else {
 #pragma unroll
-    for (int i = 0; i < C::RPL; ++i) {
-      const int key = (pc.t * kAttnWarps + warp) * TK + (TK < 32 ? lane % TK : lane + 32 * i);
-      row_page[i] = key < pc.len ? __ldg(a.table + pc.b * a.table_stride + page_of(key)) : -1;
+      for (int i = 0; i < C::RPL; ++i) page_id[i] = read_page(row_key(i));
+    }
+  };
+  // this lane's part of a copy: 16-byte chunk lc of rows lr, lr + kStep, ..
+  constexpr int kIter = TK * C::CR / 32;
+  constexpr int kStep = kEven ? 32 / C::CR : 1;
+  const int lr = lane / C::CR, lc = lane % C::CR;
+  const long long row_bytes = a.kv.tok_stride * C::E;
+  const long long lane_off = lr * row_bytes + lc * 16;
+  auto scales = [&](uint32_t s, int r, long long at, bool on) {   // Q8_0: the scales of row r, from block `at`
+    const uint32_t dk = s + C::kOffKS + r * C::NB * 2, dv = s + C::kOffVS + r * C::NB * 2;
+    if constexpr (CT == kCacheQ8 && (DH == 128 || DH == 64)) {
+      cp_small<C::NB * 2>(dk, a.kv.ks + at, on);
+      cp_small<C::NB * 2>(dv, a.kv.vs + at, on);
+    } else if constexpr (CT == kCacheQ8) {
+#pragma unroll
+      for (int e = 0; e < C::NB; ++e) {
+        sts16(dk + 2 * e, on ? __ldg(a.kv.ks + at + e) : 0);
+        sts16(dv + 2 * e, on ? __ldg(a.kv.vs + at + e) : 0);
+      }
     }
   };
   int stage_in = 0;
   auto issue = [&]() {
     if (pu < u_hi) {
       const uint32_t s = ring + stage_in * C::kStage;
-      const int j = pc.jt / tiles_h;
-      long long off[C::RPL];
-      uint64_t ok = 0;
+      const int j = pc.jt / tiles_h, key0 = tile_key();
+      const long long head = j * a.kv.head_stride;
+      const bool fast = pieces16 && key0 + TK <= pc.len &&
+                        __all_sync(0xffffffffu, page_id[0] >= 0 && page_id[0] < a.kv.n_pages);
+      if (fast) {
+        const int pk = key0 + lane % C::NP * C::PR;
+        const long long piece = page_id[0] * a.kv.page_stride + head + (pk - page_of(pk) * P) * a.kv.tok_stride;
+        if (lane == 0) valid[warp][stage_in] = ~0ull;
+        long long base = 0;
 #pragma unroll
-      for (int i = 0; i < C::RPL; ++i) {
-        const int key = (pc.t * kAttnWarps + warp) * TK + (TK < 32 ? lane % TK : lane + 32 * i);
-        const int page = row_page[i];
-        const bool in = key < pc.len;
-        const bool good = in && page >= 0 && page < a.kv.n_pages;
-        if (in && !good) *a.err = kErrPagedPage;
-        off[i] = good ? page * a.kv.page_stride + j * a.kv.head_stride + (key - page_of(key) * P) * a.kv.tok_stride : -1;
-        ok |= (uint64_t)__ballot_sync(0xffffffffu, good) << (32 * i);
-      }
-      if (lane == 0) valid[warp][stage_in] = ok;
-      constexpr int kIter = TK * C::CR / 32;
+        for (int it = 0; it < kIter; ++it) {
+          constexpr int kPer = kIter / C::NP;   // copies of a piece
+          if (it % kPer == 0) base = __shfl_sync(0xffffffffu, piece, it / kPer) * C::E + lane_off;
+          const int r = it * kStep;             // (+ lr, whose part of the swizzle only v has to be told)
+          const long long at = base + (it % kPer) * kStep * row_bytes;
+          cp16(s + lr * C::KP + ((lc ^ C::k_swz(lr)) * 16) + r * C::KP, static_cast<const uint8_t*>(a.kv.k) + at, true);
+          cp16(s + C::kOffV + lr * C::VP + ((lc ^ C::v_swz(lr + r)) * 16) + r * C::VP,
+               static_cast<const uint8_t*>(a.kv.v) + at, true);
+        }
+        if constexpr (CT == kCacheQ8) {
 #pragma unroll
-      for (int it = 0; it < kIter; ++it) {
-        const int i = it * 32 + lane, r = i / C::CR, ch = i % C::CR;
-        const long long o = __shfl_sync(0xffffffffu, off[C::RPL > 1 ? it * 32 / C::CR / 32 : 0], r & 31);
-        const bool on = o >= 0;
-        const long long at = on ? o * C::E + ch * 16 : 0;
-        cp16(s + C::k_at(r, ch), static_cast<const uint8_t*>(a.kv.k) + at, on);
-        cp16(s + C::kOffV + C::v_at(r, ch), static_cast<const uint8_t*>(a.kv.v) + at, on);
-      }
-      if constexpr (CT == kCacheQ8) {
+          for (int i = 0; i < C::RPL; ++i) {
+            const int r = lane + 32 * i;
+            const long long p0 = __shfl_sync(0xffffffffu, piece, r / C::PR);
+            scales(s, r, (p0 + (r % C::PR) * a.kv.tok_stride) / 32, true);
+          }
+        }
+      } else {
+        if (pieces16) {   // ids of rows in place of pieces
+#pragma unroll
+          for (int i = 0; i < C::RPL; ++i) page_id[i] = read_page(row_key(i));
+        }
+        long long off[C::RPL];
+        uint64_t ok = 0;
 #pragma unroll
         for (int i = 0; i < C::RPL; ++i) {
-          const int r = lane + 32 * i;
-          const bool on = off[i] >= 0;
-          const long long at = on ? off[i] / 32 : 0;
-          const uint32_t dk = s + C::kOffKS + r * C::NB * 2, dv = s + C::kOffVS + r * C::NB * 2;
-          if constexpr (DH == 128 || DH == 64) {
-            cp_small<C::NB * 2>(dk, a.kv.ks + at, on);
-            cp_small<C::NB * 2>(dv, a.kv.vs + at, on);
-          } else {
+          const int key = row_key(i), page = page_id[i];
+          const bool in = key < pc.len, good = in && page >= 0 && page < a.kv.n_pages;
+          if (in && !good) *a.err = kErrPagedPage;
+          off[i] = good ? page * a.kv.page_stride + head + (key - page_of(key) * P) * a.kv.tok_stride : -1;
+          ok |= (uint64_t)__ballot_sync(0xffffffffu, good) << (32 * i);
+        }
+        if (lane == 0) valid[warp][stage_in] = ok;
 #pragma unroll
-            for (int e = 0; e < C::NB; ++e) {
-              sts16(dk + 2 * e, on ? __ldg(a.kv.ks + at + e) : 0);
-              sts16(dv + 2 * e, on ? __ldg(a.kv.vs + at + e) : 0);
-            }
-          }
+        for (int it = 0; it < kIter; ++it) {
+          const int i = it * 32 + lane, r = i / C::CR, ch = i % C::CR;
+          const long long o = __shfl_sync(0xffffffffu, off[C::RPL > 1 ? it * 32 / C::CR / 32 : 0], r & 31);
+          const bool on = o >= 0;
+          const long long at = on ? o * C::E + ch * 16 : 0;
+          cp16(s + r * C::KP + (ch ^ C::k_swz(r)) * 16, static_cast<const uint8_t*>(a.kv.k) + at, on);
+          cp16(s + C::kOffV + r * C::VP + (ch ^ C::v_swz(r)) * 16, static_cast<const uint8_t*>(a.kv.v) + at, on);
+        }
+        if constexpr (CT == kCacheQ8) {
+#pragma unroll
+          for (int i = 0; i < C::RPL; ++i) scales(s, lane + 32 * i, off[i] >= 0 ? off[i] / 32 : 0, off[i] >= 0);
         }
       }
       ++pu;
@@ -455,11 +563,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     stage_in = stage_in + 1 == ST ? 0 : stage_in + 1;
   };
   fetch_pages();
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < ST; ++i) issue();
 
   // ---- this warp's sums over the current history
-  float o[OT][C::OV], m[R], l[R], fac[R];
+  float2 o[OT][R];
+  float m[R], l[R], fac[R];
   float inv_d = 0.f;   // Q8_0: V's block scales are used times inv_d, a power of two near 1 / the largest so far
   int stage_out = 0;
   long long u = u_lo;
@@ -472,18 +581,24 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     // q as operand registers: lane (g, c) of step s holds rows g and g + 8
     float rs[R];   // what the scores of the lane group's heads are multiplied by
     {
-      float qv[R][DH / 4];   // the lane's part of its rows: 8 values of every 32 (f32 cache: 4 of every 16)
-      constexpr int kW = CT == kCacheF32 ? 4 : 8;
+      float qv[R][DH / 4];   // the lane's part of its rows: the chunks its key rows are read by
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < DH / 4; ++i) {
-          const int d = i / kW * (4 * kW) + c * kW + i % kW;
-          qv[r][i] = g + 8 * r < heads ? load_row(a.q, a.row_type, qrow + (long long)(g + 8 * r) * DH + d) : 0.f;
+        for (int sp = 0; sp < C::SP; ++sp) {
+          float* x = qv[r] + sp * C::QW;
+          if (g + 8 * r < heads) {
+            load_rows<C::QW>(a.q, a.row_type, a.q_vec, qrow + (long long)(g + 8 * r) * DH + C::chunk(sp, c) * C::QW, x);
+#pragma unroll
+            for (int k = 0; k < C::QW; ++k) x[k] = a.c < 0.f ? -x[k] : x[k];   // the factor's sign
+          } else {
+#pragma unroll
+            for (int k = 0; k < C::QW; ++k) x[k] = 0.f;
+          }
         }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        rs[r] = a.c;
+        rs[r] = fabsf(a.c);
         if constexpr (CT == kCacheF16 || CT == kCacheQ8) {   // the largest |q| of the row into [16, 32)
           float x = 0.f;
 #pragma unroll
@@ -495,7 +610,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
           const float up = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
           for (int i = 0; i < DH / 4; ++i) qv[r][i] *= up;
-          rs[r] = a.c * __uint_as_float((uint32_t)(127 + e) << 23);
+          rs[r] *= __uint_as_float((uint32_t)(127 + e) << 23);
         }
       }
       uint4* qf = reinterpret_cast<uint4*>(region);
@@ -534,8 +649,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             if constexpr (C::QS == 2) {
               v.x = plane16<CT>(x0, x1);
               v.z = plane16<CT>(x2, x3);
-              v.y = v.w = 0;
-              qf[(C::KS + s) * 32 + lane] = v;
+              reinterpret_cast<uint2*>(qf + C::KS * 32)[s * 32 + lane] = make_uint2(v.x, v.z);
             }
           } else {
             float x[2][4];
@@ -566,9 +680,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int k = 0; k < C::OV; ++k) o[i][k] = 0.f;
+      for (int r = 0; r < R; ++r) o[i][r] = make_float2(0.f, 0.f);
     if constexpr (CT == kCacheQ8) inv_d = 0.f;
-    const uint32_t qb = smem_u32(region) + lane * 16;
+    const uint32_t qb = smem_u32(region) + lane * 16, qh = smem_u32(region) + C::KS * 512 + lane * 8;
+    auto q_at = [&](int p, int st) {   // register set p of step st
+      if (C::kHalf && p == 1) {
+        const uint2 v = lds64(qh + st * 256);
+        return make_uint4(v.x, 0, v.y, 0);
+      }
+      return lds128(qb + (p * C::KS + st) * 512);
+    };
 
     for (int t = t0; t < t1; ++t) {
       if ((t * kAttnWarps + warp) * TK >= cur.len) break;
@@ -584,17 +705,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int k = 0; k < 2 * R; ++k) s[i][k] = 0.f;
+        ScalePair<C::NB> ksc[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) ksc[i].load(ks + C::kOffKS + (8 * i + 2 * c) * C::NB * 2);
 #pragma unroll
         for (int blk = 0; blk < C::NB; ++blk) {
           uint4 qa[C::QS][2];
 #pragma unroll
           for (int p = 0; p < C::QS; ++p)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) qa[p][k] = lds128(qb + (p * C::KS + 2 * blk + k) * 512);
+            for (int k = 0; k < 2; ++k) qa[p][k] = q_at(p, 2 * blk + k);
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            const int r = 8 * i + g;
-            const uint2 w = lds64(ks + C::k_at(r, 2 * blk + (c >> 1)) + (c & 1) * 8);
+            const uint2 w =
+                lds64(ks + g * C::KP + (((2 * blk + (c >> 1)) ^ C::k_swz(g)) * 16 + (c & 1) * 8) + 8 * i * C::KP);
             const uint32_t w0 = w.x ^ 0x80808080u, w1 = w.y ^ 0x80808080u;
             float d[4] = {0.f, 0.f, 0.f, 0.f};
             const uint32_t b0 = i8pair_f16(w0, 0x4140), b1 = i8pair_f16(w0, 0x4342), b2 = i8pair_f16(w1, 0x4140),
@@ -604,9 +728,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
               mma_f16(d, qa[p][0], b0, b1);
               mma_f16(d, qa[p][1], b2, b3);
             }
-            const uint32_t sc = ks + C::kOffKS + ((8 * i + 2 * c) * C::NB + blk) * 2;
-            const float s0 = __half2float(__ushort_as_half(lds16(sc)));
-            const float s1 = __half2float(__ushort_as_half(lds16(sc + C::NB * 2)));
+            const float s0 = ksc[i].at(0, blk), s1 = ksc[i].at(1, blk);
             if constexpr (HT == 8) {
               s[i][0] = fmaf(s0, d[0] + d[2], s[i][0]);
               s[i][1] = fmaf(s1, d[1] + d[3], s[i][1]);
@@ -630,10 +752,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
           for (int p = 0; p < C::QS; ++p)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) qa[p][k] = lds128(qb + (p * C::KS + st + k) * 512);
+            for (int k = 0; k < 2; ++k) qa[p][k] = q_at(p, st + k);
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            const uint4 w = lds128(ks + C::k_at(8 * i + g, st * 2 + c));
+            const uint4 w = lds128(ks + g * C::KP + C::chunk(st / 2, c) * 16 + 8 * i * C::KP);
             if constexpr (CT == kCacheF32) {
               const uint32_t x[4] = {w.x, w.y, w.z, w.w};
               uint32_t hi[4], lo[4];
@@ -671,38 +793,39 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         }
       }
 
-      // running maximum and weights
+      // running maximum and weights: m = factor * the largest raw score
       constexpr uint64_t kAll = TK == 64 ? ~0ull : ((1ull << (TK & 63)) - 1);
       const bool masked = (ok & kAll) != kAll;
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int k = 0; k < 2 * R; ++k)
+            if (!((ok >> (8 * i + 2 * c + (k & 1))) & 1)) s[i][k] = -INFINITY;
+      }
       float mx[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) mx[r] = m[r];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int k = 0; k < 2 * R; ++k) {
-          float x = s[i][k] * fac[k >> 1];
-          if (masked && !((ok >> (8 * i + 2 * c + (k & 1))) & 1)) x = -INFINITY;
-          s[i][k] = x;
-          mx[k >> 1] = fmaxf(mx[k >> 1], x);
-        }
       bool grew = false;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        float x = s[0][2 * r];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) x = fmaxf(x, fmaxf(s[i][2 * r], s[i][2 * r + 1]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        mx[r] = fmaxf(m[r], x * fac[r]);   // (a NaN, or -inf times a factor of 0, leaves m)
         grew |= mx[r] != m[r];
       }
-      float shrink[R];
       float new_inv = inv_d;
+      ScalePair<C::NB> vsc[CT == kCacheQ8 ? NT : 1];
       if constexpr (CT == kCacheQ8) {
         uint32_t big = 0;   // the tile's largest |V scale|, as fp16 bits
 #pragma unroll
-        for (int i = 0; i < C::RPL; ++i)
+        for (int i = 0; i < NT; ++i) {
+          vsc[i].load(ks + C::kOffVS + (8 * i + 2 * c) * C::NB * 2);
 #pragma unroll
-          for (int e = 0; e < C::NB; ++e)
-            big = max(big, (uint32_t)lds16(ks + C::kOffVS + ((lane + 32 * i) * C::NB + e) * 2) & 0x7fffu);
-        big = __reduce_max_sync(0xffffffffu, big);
+          for (int e = 0; e < C::NB; ++e) big = __vmaxu2(big, vsc[i].w[e] & 0x7fff7fffu);
+        }
+        big = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
         const float top = fmaxf(__half2float(__ushort_as_half((uint16_t)big)), 0x1p-24f);
         // 1 / the power of two at or below it (an infinite scale makes the sums NaN)
         const float inv = __uint_as_float((254u << 23) - (__float_as_uint(top) & 0x7f800000u));
@@ -710,6 +833,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         grew |= new_inv != inv_d;
       }
       if (__any_sync(0xffffffffu, grew)) {
+        float shrink[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           shrink[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx[r]);
@@ -726,16 +850,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
         for (int i = 0; i < OT; ++i)
 #pragma unroll
-          for (int k = 0; k < C::OV; ++k) o[i][k] *= shrink[R == 1 ? 0 : k >> 1];
+          for (int r = 0; r < R; ++r) o[i][r] = mul2(o[i][r], make_float2(shrink[r], shrink[r]));
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float base = m[r] == -INFINITY ? 0.f : m[r] - kLift;
+        const float base = m[r] == -INFINITY ? 0.f : kLift - m[r];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float p = ex2(s[i][2 * r + k] - base);
+            float p = ex2(fmaf(s[i][2 * r + k], fac[r], base));
+            if (masked && !((ok >> (8 * i + 2 * c + k)) & 1)) p = 0.f;   // (a factor of 0 makes -inf NaN)
             s[i][2 * r + k] = p;
             l[r] += p;
           }
@@ -745,8 +870,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       // to the running sums by f32 adds (the tensor core's own sums are cut,
       // not rounded, which would add up over a long history)
       auto gather = [&](int i, const float (&d)[4]) {
-#pragma unroll
-        for (int k = 0; k < C::OV; ++k) o[i][k] += HT == 8 ? d[k] + d[(k + 2) & 3] : d[k];
+        const float2 x = make_float2(d[0], d[1]), y = make_float2(d[2], d[3]);
+        if constexpr (HT == 8) {
+          o[i][0] = add2(o[i][0], add2(x, y));
+        } else {
+          o[i][0] = add2(o[i][0], x);
+          o[i][R - 1] = add2(o[i][R - 1], y);
+        }
       };
       if constexpr (CT == kCacheF32) {
         uint4 ph[NT], pl[NT];
@@ -775,8 +905,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
           for (int k = 0; k < 4; ++k) zero(d[k]);
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            const uint4 w0 = lds128(vs + C::v_at(8 * i + 2 * c, 8 * q4 + g));
-            const uint4 w1 = lds128(vs + C::v_at(8 * i + 2 * c + 1, 8 * q4 + g));
+            const uint4 w0 = lds128(vs + 2 * c * C::VP + g * 16 + 8 * i * C::VP + q4 * 128);
+            const uint4 w1 = lds128(vs + 2 * c * C::VP + g * 16 + (8 * i + 1) * C::VP + q4 * 128);
             const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -801,9 +931,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
           for (int i = 0; i < NT; i += 2) {   // 16 keys
             float dv[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              dv[k] = inv_d * __half2float(__ushort_as_half(lds16(
-                                  ks + C::kOffVS + ((8 * (i + (k >> 1)) + 2 * c + (k & 1)) * C::NB + blk) * 2)));
+            for (int k = 0; k < 4; ++k) dv[k] = inv_d * vsc[i + (k >> 1)].at(k & 1, blk);
             uint4 ph, pl;
             if constexpr (HT == 8) {
               float x0 = s[i][0] * dv[0], x1 = s[i][1] * dv[1], x2 = s[i + 1][0] * dv[2], x3 = s[i + 1][1] * dv[3];
@@ -830,7 +958,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             uint32_t w[4];   // columns 32 blk + 4 g .. + 3 of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              w[k] = lds32(vs + C::v_at(8 * (i + (k >> 1)) + 2 * c + (k & 1), 2 * blk + (g >> 2)) + (g & 3) * 4) ^
+              w[k] = lds32(vs + 2 * c * C::VP + (((2 * blk + (g >> 2)) ^ C::v_swz(2 * c)) * 16 + (g & 3) * 4) +
+                           (8 * (i + (k >> 1)) + (k & 1)) * C::VP) ^
                      0x80808080u;
             const uint32_t p0 = __byte_perm(w[0], w[1], 0x5140), p1 = __byte_perm(w[0], w[1], 0x7362);
             const uint32_t p2 = __byte_perm(w[2], w[3], 0x5140), p3 = __byte_perm(w[2], w[3], 0x7362);
@@ -886,7 +1015,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
           for (int i = 0; i < NT; i += 2) {
             uint32_t b[4];   // keys 0..7 and 8..15 of columns 8 d2 .., then of 8 d2 + 8 ..
-            ldmatrix_x4_trans(vs + C::v_at(8 * i + (lane & 15), d2 + (lane >> 4)), b);
+            ldmatrix_x4_trans(vs + (lane & 15) * C::VP + (lane >> 4) * 16 + 8 * i * C::VP + d2 * 16, b);
 #pragma unroll
             for (int p = kP - 1; p >= 0; --p) {
               mma16<CT>(e0, pp[i / 2][p], b[0], b[1]);
@@ -908,7 +1037,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int k = 0; k < C::OV; ++k) ov[i][k] = o[i][k] * back;
+      for (int k = 0; k < C::OV; ++k) ov[i][k] = (k & 1 ? o[i][k >> 1].y : o[i][k >> 1].x) * back;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
