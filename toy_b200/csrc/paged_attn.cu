@@ -22,6 +22,7 @@ int paged_attend_launch(const tb2_paged_kv& c, const tb2_paged_attend_args& a, i
   k.err = err;
   k.c = (float)(a.scale * 1.4426950408889634);   // log2(e)
   k.q_vec = aligned(a.q, 16) && (a.ldq * type_bytes(a.row_type)) % 16 == 0;
+  k.out_vec = aligned(a.out, 16) && (a.ldo * type_bytes(a.row_type)) % 16 == 0;
   k.n_req = a.n_req;
   k.n_heads = a.n_heads;
   k.group = a.n_heads / c.n_kv;

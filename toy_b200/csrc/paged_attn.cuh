@@ -33,6 +33,7 @@
 // order (a ticket per history), so the result does not depend on timing.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "pdl.cuh"
@@ -41,7 +42,8 @@
 namespace tb2 {
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnMaxCtas = 3 * 148;   // the workspace's slots
+constexpr int kMinUnits = 2;            // units that are worth a CTA
+constexpr int kAttnMaxCtas = 4 * 148;   // the workspace's slots
 constexpr int kAttnSlotFloats = 16 * 128 + 2 * 16;
 // tickets, then two partial slots per CTA
 constexpr size_t kAttnTicketBytes = (kAttnMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
@@ -61,7 +63,7 @@ struct PagedAttnArgs {
   float* slots;
   int* err;
   float c;             // scale * log2(e)
-  bool q_vec;          // q rows start on 16-byte boundaries
+  bool q_vec, out_vec; // rows of q, of out start on 16-byte boundaries
   int n_req, n_heads, group, width, row_type, page_shift;   // page_shift < 0: page_size is no power of two
 };
 
@@ -72,6 +74,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;   // 0: the 16 bytes are zeros and nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int B>
 __device__ __forceinline__ void cp_small(uint32_t dst, const void* src, bool on) {
@@ -219,6 +224,15 @@ struct ScalePair {
   }
 };
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 template <int CT, int DH, int HT, int PL>
 struct Cfg {
   static constexpr int E = CT == kCacheF32 ? 4 : CT == kCacheQ8 ? 1 : 2;
@@ -229,8 +243,8 @@ struct Cfg {
                             : CT == kCacheQ8 ? (DH == 32 ? 64 : 32)
                                                : (DH == 32 ? 64 : DH == 64 ? 32 : 16);
   static constexpr int UK = TK * kAttnWarps;   // keys of a unit
-  static constexpr int ST = CT == kCacheQ8 && DH <= 64 ? 3 : 2;
-  static constexpr int OCC = HT == 8 ? 3 : 2;   // CTAs on an SM
+  static constexpr int ST = 2;
+  static constexpr int OCC = HT == 16 ? 2 : CT == kCacheQ8 && DH <= 64 ? 4 : 3;   // CTAs on an SM
   // Row pitches in shared memory, so that the lanes that read at once meet no
   // bank twice. 16-bit and f32 rows: 16 bytes of padding (a read covers chunks
   // 2 c + e of rows g and g + 1, or one chunk of eight rows). Q8_0: K is read 8
@@ -246,7 +260,6 @@ struct Cfg {
   static constexpr int NT = TK / 8;
   static constexpr int OT = DH / 8;                   // 8-column tiles of the output
   static constexpr int R = HT / 8;                    // heads per lane group
-  static constexpr int OV = HT == 8 ? 2 : 4;          // values of an output tile per lane, planes added
   static constexpr int KS = 2 * (CT == kCacheF32 ? DH / 16 : DH / 32);   // k steps of q . k
   // register sets of q: planes that do not share an instruction
   static constexpr int QS = CT == kCacheBF16 ? (HT == 8 ? PL - 1 : PL) : (HT == 8 ? 1 : 2);
@@ -257,7 +270,7 @@ struct Cfg {
   // separate score accumulators (short chains of dependent products; an f32
   // cache's small products apart from its large ones)
   static constexpr int A = CT == kCacheF32 ? (NT >= 4 ? 2 : 4) : NT >= 8 ? 1 : 2;
-  static constexpr int kBufFloats = (OT * OV + 2 * R) * 32;
+  static constexpr int kBufFloats = (OT * 2 + 2) * R * 32;
   static constexpr int kJoinBytes = kBufs * kBufFloats * 4;
   static constexpr int kScanBytes = (kAttnWarps * 32 + 1) * 8;
   static constexpr int kRegion0 = kQBytes > kJoinBytes ? kQBytes : kJoinBytes;
@@ -323,6 +336,37 @@ __device__ __forceinline__ void store_row(void* p, int type, long long at, float
   else static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(x);
 }
 
+// N values times f from element `at` on (a multiple of N); vec: rows start on 16-byte boundaries.
+template <int N>
+__device__ __forceinline__ void store_rows(void* p, int type, bool vec, long long at, const float* v, float f) {
+  if (!vec) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) store_row(p, type, at + k, v[k] * f);
+  } else if (type == kTypeF32) {
+    float* d = static_cast<float*>(p) + at;
+    if constexpr (N == 2) {
+      *reinterpret_cast<float2*>(d) = make_float2(v[0] * f, v[1] * f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; k += 4)
+        *reinterpret_cast<float4*>(d + k) = make_float4(v[k] * f, v[k + 1] * f, v[k + 2] * f, v[k + 3] * f);
+    }
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      const float x = v[2 * k] * f, y = v[2 * k + 1] * f;
+      const __half2 h = __floats2half2_rn(x, y);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+      w[k] = type == kTypeF16 ? *reinterpret_cast<const uint32_t*>(&h) : *reinterpret_cast<const uint32_t*>(&b);
+    }
+    uint16_t* d = static_cast<uint16_t*>(p) + at;
+    if constexpr (N == 2) *reinterpret_cast<uint32_t*>(d) = w[0];
+    else if constexpr (N == 4) *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // A place in the list of units: unit t of key head (and head tile) jt of
 // request b, whose history has nt units.
 struct Cursor {
@@ -339,6 +383,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint64_t valid[kAttnWarps][ST];   // keys of a staged tile that count
   __shared__ int last_flag;
+  __shared__ float qmax[kAttnWarps][HT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   uint8_t* region = smem + kAttnWarps * ST * C::kStage;
   const uint32_t ring = smem_u32(smem) + warp * ST * C::kStage;
@@ -387,8 +432,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       for (int h = tid; h < a.n_heads; h += blockDim.x) a.lse[(long long)b * a.n_heads + h] = -INFINITY;
   }
   const long long units = total * KVH;
-  const long long G = min((long long)gridDim.x, units);
-  if (blockIdx.x >= G) return;
+  const long long G = max(1LL, min((long long)gridDim.x, units / kMinUnits));
+  if (units == 0 || blockIdx.x >= G) return;
   const long long u_lo = blockIdx.x * units / G, u_hi = (blockIdx.x + 1) * units / G;
 
   Cursor cur;
@@ -458,15 +503,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / P; };
   auto tile_key = [&]() { return (pc.t * kAttnWarps + warp) * TK; };
   auto row_key = [&](int i) { return tile_key() + (TK < 32 ? lane % TK : lane + 32 * i); };
-  auto read_page = [&](int key) {
-    return key < pc.len ? __ldg(a.table + pc.b * a.table_stride + page_of(key)) : -1;
+  const int* pages = nullptr;  // the history's row of the block table
+  long long head = 0;          // and its key head's offset in a page
+  auto enter = [&]() {
+    pages = a.table + pc.b * a.table_stride;
+    head = pc.jt / tiles_h * a.kv.head_stride;
   };
+  auto next_unit = [&]() {
+    ++pu;
+    if (++pc.t == pc.nt && pu < u_hi) {
+      next_history(pc, nullptr);
+      enter();
+    }
+  };
+  auto read_page = [&](int key) { return key < pc.len ? __ldg(pages + page_of(key)) : -1; };
   auto fetch_pages = [&]() {
     // (the last unit of a history may hold no tile of this warp)
-    while (pu < u_hi && tile_key() >= pc.len) {
-      ++pu;
-      if (++pc.t == pc.nt && pu < u_hi) next_history(pc, nullptr);
-    }
+    while (pu < u_hi && tile_key() >= pc.len) next_unit();
     if (pu >= u_hi) return;
     if (pieces16) {
       page_id[0] = read_page(tile_key() + lane % C::NP * C::PR);
@@ -481,6 +534,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   const int lr = lane / C::CR, lc = lane % C::CR;
   const long long row_bytes = a.kv.tok_stride * C::E;
   const long long lane_off = lr * row_bytes + lc * 16;
+  const bool dense = a.kv.tok_stride == DH;   // a page's rows of a head are one run of bytes
   auto scales = [&](uint32_t s, int r, long long at, bool on) {   // Q8_0: the scales of row r, from block `at`
     const uint32_t dk = s + C::kOffKS + r * C::NB * 2, dv = s + C::kOffVS + r * C::NB * 2;
     if constexpr (CT == kCacheQ8 && (DH == 128 || DH == 64)) {
@@ -498,24 +552,36 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   auto issue = [&]() {
     if (pu < u_hi) {
       const uint32_t s = ring + stage_in * C::kStage;
-      const int j = pc.jt / tiles_h, key0 = tile_key();
-      const long long head = j * a.kv.head_stride;
+      const int key0 = tile_key();
       const bool fast = pieces16 && key0 + TK <= pc.len &&
                         __all_sync(0xffffffffu, page_id[0] >= 0 && page_id[0] < a.kv.n_pages);
       if (fast) {
         const int pk = key0 + lane % C::NP * C::PR;
         const long long piece = page_id[0] * a.kv.page_stride + head + (pk - page_of(pk) * P) * a.kv.tok_stride;
         if (lane == 0) valid[warp][stage_in] = ~0ull;
-        long long base = 0;
+        constexpr int kPer = kIter / C::NP;   // copies of a piece
+        const uint32_t dk = s + lr * C::KP + (lc ^ C::k_swz(lr)) * 16;
+        auto dv = [&](int r) { return s + C::kOffV + lr * C::VP + (lc ^ C::v_swz(lr + r)) * 16 + r * C::VP; };
 #pragma unroll
-        for (int it = 0; it < kIter; ++it) {
-          constexpr int kPer = kIter / C::NP;   // copies of a piece
-          if (it % kPer == 0) base = __shfl_sync(0xffffffffu, piece, it / kPer) * C::E + lane_off;
-          const int r = it * kStep;             // (+ lr, whose part of the swizzle only v has to be told)
-          const long long at = base + (it % kPer) * kStep * row_bytes;
-          cp16(s + lr * C::KP + ((lc ^ C::k_swz(lr)) * 16) + r * C::KP, static_cast<const uint8_t*>(a.kv.k) + at, true);
-          cp16(s + C::kOffV + lr * C::VP + ((lc ^ C::v_swz(lr + r)) * 16) + r * C::VP,
-               static_cast<const uint8_t*>(a.kv.v) + at, true);
+        for (int p = 0; p < C::NP; ++p) {
+          const long long base = __shfl_sync(0xffffffffu, piece, p) * C::E + lane_off;
+          const uint8_t* sk = static_cast<const uint8_t*>(a.kv.k) + base;
+          const uint8_t* sv = static_cast<const uint8_t*>(a.kv.v) + base;
+          if (dense) {   // (addresses of one register and constants)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const int r = (p * kPer + i) * kStep;
+              cp16(dk + r * C::KP, sk + i * kStep * (DH * C::E));
+              cp16(dv(r), sv + i * kStep * (DH * C::E));
+            }
+          } else {
+#pragma unroll 1
+            for (int i = 0; i < kPer; ++i) {
+              const int r = (p * kPer + i) * kStep;
+              cp16(dk + r * C::KP, sk + i * kStep * row_bytes);
+              cp16(dv(r), sv + i * kStep * row_bytes);
+            }
+          }
         }
         if constexpr (CT == kCacheQ8) {
 #pragma unroll
@@ -541,10 +607,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
           ok |= (uint64_t)__ballot_sync(0xffffffffu, good) << (32 * i);
         }
         if (lane == 0) valid[warp][stage_in] = ok;
-#pragma unroll
+        // (rolled: this path is rare and the code of the others has to stay in the instruction cache)
+#pragma unroll 1
         for (int it = 0; it < kIter; ++it) {
           const int i = it * 32 + lane, r = i / C::CR, ch = i % C::CR;
-          const long long o = __shfl_sync(0xffffffffu, off[C::RPL > 1 ? it * 32 / C::CR / 32 : 0], r & 31);
+          const long long lo = __shfl_sync(0xffffffffu, off[0], r & 31);
+          const long long hi = C::RPL > 1 ? __shfl_sync(0xffffffffu, off[C::RPL - 1], r & 31) : lo;
+          const long long o = r < 32 ? lo : hi;
           const bool on = o >= 0;
           const long long at = on ? o * C::E + ch * 16 : 0;
           cp16(s + r * C::KP + (ch ^ C::k_swz(r)) * 16, static_cast<const uint8_t*>(a.kv.k) + at, on);
@@ -555,13 +624,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
           for (int i = 0; i < C::RPL; ++i) scales(s, lane + 32 * i, off[i] >= 0 ? off[i] / 32 : 0, off[i] >= 0);
         }
       }
-      ++pu;
-      if (++pc.t == pc.nt && pu < u_hi) next_history(pc, nullptr);
+      next_unit();
       fetch_pages();
     }
     cp_commit();   // (an empty group at the list's end keeps the count)
     stage_in = stage_in + 1 == ST ? 0 : stage_in + 1;
   };
+  enter();
   fetch_pages();
 #pragma unroll 1
   for (int i = 0; i < ST; ++i) issue();
@@ -578,92 +647,102 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     const int heads = min(HT, a.group - h0);
     const long long qrow = (long long)cur.b * a.ldq + ((long long)jh * a.group + h0) * DH;
 
-    // q as operand registers: lane (g, c) of step s holds rows g and g + 8
+    // q as operand registers: lane (g, c) of step s holds rows g and g + 8.
+    // Step pairs are dealt to the warps.
     float rs[R];   // what the scores of the lane group's heads are multiplied by
     {
-      float qv[R][DH / 4];   // the lane's part of its rows: the chunks its key rows are read by
+      constexpr int kOwn = (C::SP + kAttnWarps - 1) / kAttnWarps;
+      float qv[kOwn][R][C::QW];   // the chunks of the lane's rows that its key rows are read by
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int own = 0; own < kOwn; ++own)
 #pragma unroll
-        for (int sp = 0; sp < C::SP; ++sp) {
-          float* x = qv[r] + sp * C::QW;
-          if (g + 8 * r < heads) {
-            load_rows<C::QW>(a.q, a.row_type, a.q_vec, qrow + (long long)(g + 8 * r) * DH + C::chunk(sp, c) * C::QW, x);
+        for (int r = 0; r < R; ++r) {
+          const int sp = warp + own * kAttnWarps;
+          if (g + 8 * r < heads && sp < C::SP) {
+            load_rows<C::QW>(a.q, a.row_type, a.q_vec, qrow + (long long)(g + 8 * r) * DH + C::chunk(sp, c) * C::QW,
+                             qv[own][r]);
 #pragma unroll
-            for (int k = 0; k < C::QW; ++k) x[k] = a.c < 0.f ? -x[k] : x[k];   // the factor's sign
+            for (int k = 0; k < C::QW; ++k) qv[own][r][k] = a.c < 0.f ? -qv[own][r][k] : qv[own][r][k];   // the factor's sign
           } else {
 #pragma unroll
-            for (int k = 0; k < C::QW; ++k) x[k] = 0.f;
+            for (int k = 0; k < C::QW; ++k) qv[own][r][k] = 0.f;
           }
         }
+      if constexpr (CT == kCacheF16 || CT == kCacheQ8) {   // the largest |q| of a row into [16, 32)
+        float x[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        rs[r] = fabsf(a.c);
-        if constexpr (CT == kCacheF16 || CT == kCacheQ8) {   // the largest |q| of the row into [16, 32)
-          float x = 0.f;
+        for (int r = 0; r < R; ++r) {
+          x[r] = 0.f;
 #pragma unroll
-          for (int i = 0; i < DH / 4; ++i) x = fmaxf(x, fabsf(qv[r][i]));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          int e = (int)(__float_as_uint(x) >> 23) - 127 - 4;   // x < 2^(e + 5)
+          for (int own = 0; own < kOwn; ++own)
+#pragma unroll
+            for (int k = 0; k < C::QW; ++k) x[r] = fmaxf(x[r], fabsf(qv[own][r][k]));
+          x[r] = fmaxf(x[r], __shfl_xor_sync(0xffffffffu, x[r], 1));
+          x[r] = fmaxf(x[r], __shfl_xor_sync(0xffffffffu, x[r], 2));
+          if (c == 0) qmax[warp][g + 8 * r] = x[r];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int w = 0; w < kAttnWarps; ++w) x[r] = fmaxf(x[r], qmax[w][g + 8 * r]);
+          int e = (int)(__float_as_uint(x[r]) >> 23) - 127 - 4;   // x < 2^(e + 5)
           e = max(-100, min(100, e));
           const float up = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-          for (int i = 0; i < DH / 4; ++i) qv[r][i] *= up;
-          rs[r] *= __uint_as_float((uint32_t)(127 + e) << 23);
+          for (int own = 0; own < kOwn; ++own)
+#pragma unroll
+            for (int k = 0; k < C::QW; ++k) qv[own][r][k] *= up;
+          rs[r] = fabsf(a.c) * __uint_as_float((uint32_t)(127 + e) << 23);
         }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) rs[r] = fabsf(a.c);
       }
       uint4* qf = reinterpret_cast<uint4*>(region);
 #pragma unroll
-      for (int s = 0; s < C::KS; ++s) {
-        if (s % kAttnWarps != warp) {   // each warp writes its share of the steps
-          continue;
-        }
-        if constexpr (CT == kCacheF32) {
-          const int i = s * 2;   // values i, i + 1 of the lane's part
-          if constexpr (HT == 8) {
-            const uint32_t h0_ = tf32(qv[0][i]), h1_ = tf32(qv[0][i + 1]);
-            qf[s * 32 + lane] = make_uint4(h0_, tf32(qv[0][i] - __uint_as_float(h0_)), h1_,
-                                           tf32(qv[0][i + 1] - __uint_as_float(h1_)));
-          } else {
-            uint32_t hi[4], lo[4];
+      for (int own = 0; own < kOwn; ++own) {
+        const int sp = warp + own * kAttnWarps;
+        if (sp >= C::SP) break;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float x = qv[k & 1][i + (k >> 1)];
-              hi[k] = tf32(x);
-              lo[k] = tf32(x - __uint_as_float(hi[k]));
+        for (int half = 0; half < 2; ++half) {
+          const int s = 2 * sp + half, i = half * C::QW / 2;
+          float (&x)[R][C::QW] = qv[own];
+          if constexpr (CT == kCacheF32) {
+            uint32_t hi[2][2], lo[2][2];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                hi[r][k] = tf32(x[r][i + k]);
+                lo[r][k] = tf32(x[r][i + k] - __uint_as_float(hi[r][k]));
+              }
+            if constexpr (HT == 8) {
+              qf[s * 32 + lane] = make_uint4(hi[0][0], lo[0][0], hi[0][1], lo[0][1]);
+            } else {
+              qf[s * 32 + lane] = make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
+              qf[(C::KS + s) * 32 + lane] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
             }
-            qf[s * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            qf[(C::KS + s) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          }
-        } else {
-          const int i = s * 4;
-          if constexpr (HT == 8) {
-            float x0 = qv[0][i], x1 = qv[0][i + 1], x2 = qv[0][i + 2], x3 = qv[0][i + 3];
+          } else if constexpr (HT == 8) {
             uint4 v;
-            v.x = plane16<CT>(x0, x1);
-            v.z = plane16<CT>(x2, x3);
-            v.y = plane16<CT>(x0, x1);
-            v.w = plane16<CT>(x2, x3);
+            v.x = plane16<CT>(x[0][i], x[0][i + 1]);
+            v.z = plane16<CT>(x[0][i + 2], x[0][i + 3]);
+            v.y = plane16<CT>(x[0][i], x[0][i + 1]);
+            v.w = plane16<CT>(x[0][i + 2], x[0][i + 3]);
             qf[s * 32 + lane] = v;
             if constexpr (C::QS == 2) {
-              v.x = plane16<CT>(x0, x1);
-              v.z = plane16<CT>(x2, x3);
+              v.x = plane16<CT>(x[0][i], x[0][i + 1]);
+              v.z = plane16<CT>(x[0][i + 2], x[0][i + 3]);
               reinterpret_cast<uint2*>(qf + C::KS * 32)[s * 32 + lane] = make_uint2(v.x, v.z);
             }
           } else {
-            float x[2][4];
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) x[r][k] = qv[r][i + k];
 #pragma unroll
             for (int p = 0; p < C::QS; ++p) {
               uint4 v;
-              v.x = plane16<CT>(x[0][0], x[0][1]);
-              v.y = plane16<CT>(x[1][0], x[1][1]);
-              v.z = plane16<CT>(x[0][2], x[0][3]);
-              v.w = plane16<CT>(x[1][2], x[1][3]);
+              v.x = plane16<CT>(x[0][i], x[0][i + 1]);
+              v.y = plane16<CT>(x[R - 1][i], x[R - 1][i + 1]);
+              v.z = plane16<CT>(x[0][i + 2], x[0][i + 3]);
+              v.w = plane16<CT>(x[R - 1][i + 2], x[R - 1][i + 3]);
               qf[(p * C::KS + s) * 32 + lane] = v;
             }
           }
@@ -1031,13 +1110,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       issue();
     }
 
-    // ---- the warps' sums joined: planes added, weights of a lane group summed
-    float ov[OT][C::OV];
-    const float back = CT == kCacheQ8 ? (inv_d == 0.f ? 0.f : 1.f / inv_d) : 1.f;
+    // ---- the warps' sums joined: weights of a lane group summed
+    float2 (&ov)[OT][R] = o;
+    if constexpr (CT == kCacheQ8) {
+      const float back = inv_d == 0.f ? 0.f : 1.f / inv_d;
 #pragma unroll
-    for (int i = 0; i < OT; ++i)
+      for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int k = 0; k < C::OV; ++k) ov[i][k] = (k & 1 ? o[i][k >> 1].y : o[i][k >> 1].x) * back;
+        for (int r = 0; r < R; ++r) ov[i][r] = mul2(ov[i][r], make_float2(back, back));
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -1045,35 +1126,33 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     }
     float* buf = reinterpret_cast<float*>(region);
     auto put = [&](float* d) {
-#pragma unroll
-      for (int i = 0; i < OT; ++i)
-#pragma unroll
-        for (int k = 0; k < C::OV; ++k) d[(i * C::OV + k) * 32 + lane] = ov[i][k];
+      float4* d4 = reinterpret_cast<float4*>(d) + lane;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        d[(OT * C::OV + 2 * r) * 32 + lane] = m[r];
-        d[(OT * C::OV + 2 * r + 1) * 32 + lane] = l[r];
+#pragma unroll
+        for (int i = 0; i < OT; i += 2)
+          d4[(r * (OT / 2) + i / 2) * 32] = make_float4(ov[i][r].x, ov[i][r].y, ov[i + 1][r].x, ov[i + 1][r].y);
+        reinterpret_cast<float2*>(d + OT * 2 * R * 32)[r * 32 + lane] = make_float2(m[r], l[r]);
       }
     };
     auto add = [&](const float* d) {
-      float f[R], e[R];
+      const float4* d4 = reinterpret_cast<const float4*>(d) + lane;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float mo = d[(OT * C::OV + 2 * r) * 32 + lane], lo = d[(OT * C::OV + 2 * r + 1) * 32 + lane];
-        const float mn = fmaxf(m[r], mo);
+        const float2 ml = reinterpret_cast<const float2*>(d + OT * 2 * R * 32)[r * 32 + lane];
+        const float mn = fmaxf(m[r], ml.x);
         // a warp without keys has sums of 0, which any finite factor keeps (and NaN sums stay NaN)
-        f[r] = m[r] == -INFINITY ? 1.f : ex2(m[r] - mn);
-        e[r] = mo == -INFINITY ? 1.f : ex2(mo - mn);
-        l[r] = l[r] * f[r] + lo * e[r];
+        const float f = m[r] == -INFINITY ? 1.f : ex2(m[r] - mn), e = ml.x == -INFINITY ? 1.f : ex2(ml.x - mn);
+        l[r] = l[r] * f + ml.y * e;
         m[r] = mn;
-      }
 #pragma unroll
-      for (int i = 0; i < OT; ++i)
-#pragma unroll
-        for (int k = 0; k < C::OV; ++k) {
-          const int r = R == 1 ? 0 : k >> 1;
-          ov[i][k] = ov[i][k] * f[r] + d[(i * C::OV + k) * 32 + lane] * e[r];
+        for (int i = 0; i < OT; i += 2) {
+          const float4 y = d4[(r * (OT / 2) + i / 2) * 32];
+          const float2 e2 = make_float2(e, e), f2 = make_float2(f, f);
+          ov[i][r] = fma2(make_float2(y.x, y.y), e2, mul2(ov[i][r], f2));
+          ov[i + 1][r] = fma2(make_float2(y.z, y.w), e2, mul2(ov[i + 1][r], f2));
         }
+      }
     };
     __syncthreads();   // q is read by every warp
     if constexpr (C::kBufs == 2) {
@@ -1093,10 +1172,22 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       }
     }
 
-    // element e of the lane's value k of output tile i: its column
-    auto col = [&](int i, int k) {
-      if constexpr (CT == kCacheF32 || CT == kCacheQ8) return 32 * (i >> 2) + 4 * (2 * c + (k & 1)) + (i & 3);
-      else return 8 * i + 2 * c + (k & 1);
+    // The lane's sums of row r as runs of consecutive columns: f(column, values, count).
+    auto runs = [&](int r, auto&& f) {
+      if constexpr (CT == kCacheF32 || CT == kCacheQ8) {   // tile 4 q + k has column 4 n + k of block q at n
+#pragma unroll
+        for (int q = 0; q < OT; q += 4) {
+          const float v[8] = {ov[q][r].x, ov[q + 1][r].x, ov[q + 2][r].x, ov[q + 3][r].x,
+                              ov[q][r].y, ov[q + 1][r].y, ov[q + 2][r].y, ov[q + 3][r].y};
+          f(8 * q + 8 * c, v, std::integral_constant<int, 8>{});
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < OT; ++i) {
+          const float v[2] = {ov[i][r].x, ov[i][r].y};
+          f(8 * i + 2 * c, v, std::integral_constant<int, 2>{});
+        }
+      }
     };
     const long long out0 = (long long)cur.b * a.ldo + ((long long)jh * a.group + h0) * DH;
     const long long lse0 = (long long)cur.b * a.n_heads + (long long)jh * a.group + h0;
@@ -1107,11 +1198,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         for (int r = 0; r < R; ++r) {
           if (g + 8 * r >= heads) continue;
           const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-#pragma unroll
-          for (int i = 0; i < OT; ++i)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              store_row(a.out, a.row_type, out0 + (long long)(g + 8 * r) * DH + col(i, k), ov[i][2 * r + k] * inv);
+          runs(r, [&](int col, const float* v, auto count) {
+            store_rows<decltype(count)::value>(a.out, a.row_type, a.out_vec, out0 + (long long)(g + 8 * r) * DH + col, v,
+                                               inv);
+          });
           if (a.lse && c == 0)
             a.lse[lse0 + g + 8 * r] = l[r] == 0.f ? -INFINITY : (m[r] - kLift + log2f(l[r])) * 0.693147180559945f;
         }
@@ -1127,10 +1217,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         float* d = slot_of(blockIdx.x);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-#pragma unroll
-          for (int i = 0; i < OT; ++i)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) __stcg(d + (g + 8 * r) * DH + col(i, k), ov[i][2 * r + k]);
+          runs(r, [&](int col, const float* v, auto count) {
+            float* to = d + (g + 8 * r) * DH + col;
+            if constexpr (decltype(count)::value == 8) {
+              __stcg(reinterpret_cast<float4*>(to), make_float4(v[0], v[1], v[2], v[3]));
+              __stcg(reinterpret_cast<float4*>(to) + 1, make_float4(v[4], v[5], v[6], v[7]));
+            } else {
+              __stcg(reinterpret_cast<float2*>(to), make_float2(v[0], v[1]));
+            }
+          });
           if (c == 0) {
             __stcg(d + HT * DH + g + 8 * r, m[r]);
             __stcg(d + HT * DH + HT + g + 8 * r, l[r]);
@@ -1143,32 +1238,81 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       __syncthreads();
       if (last_flag) {   // this CTA adds the pieces up, in order
         __threadfence();
-        for (int e0 = tid * 4; e0 < heads * DH; e0 += kAttnWarps * 32 * 4) {
-          const int h = e0 / DH;
-          float mm = -INFINITY;
-#pragma unroll 8
-          for (int p = 0; p < pieces; ++p) mm = fmaxf(mm, __ldcg(slot_of(first + p) + HT * DH + h));
-          float ll = 0.f;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int p = 0; p < pieces; ++p) {
-            const float* d = slot_of(first + p);
-            const float mp = __ldcg(d + HT * DH + h), f = mp == -INFINITY ? 1.f : ex2(mp - mm);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(d + e0));
-            ll += f * __ldcg(d + HT * DH + HT + h);
-            x.x += f * y.x;
-            x.y += f * y.y;
-            x.z += f * y.z;
-            x.w += f * y.w;
+        // HW heads to a warp, a lane for four columns (d_head 128; fewer lanes below): the pieces' weights first, a
+        // lane a piece, then the weighted sums, kFly pieces' loads in flight (an L2 read here takes 0.5 us or more,
+        // and one after another they were most of the time of a short call)
+        constexpr int HW = HT / kAttnWarps, kFly = HT == 8 ? 8 : 4;
+        float mm[HW], ll[HW];
+        float4 x[HW];
+#pragma unroll
+        for (int i = 0; i < HW; ++i) {
+          mm[i] = -INFINITY;
+          ll[i] = 0.f;
+          x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const int col4 = min(lane, DH / 4 - 1);
+        for (int p0 = 0; p0 < pieces; p0 += 32) {
+          // this lane's piece (a lane past the end repeats the last one with weight 0)
+          const bool on = p0 + lane < pieces;
+          const float* d = slot_of(first + min(p0 + lane, pieces - 1)) + HT * DH + warp;
+          float mp[HW], f[HW];
+#pragma unroll
+          for (int i = 0; i < HW; ++i) {
+            mp[i] = on ? __ldcg(d + i * kAttnWarps) : -INFINITY;
+            f[i] = on ? __ldcg(d + HT + i * kAttnWarps) : 0.f;
           }
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          const long long at = out0 + e0;
-          store_row(a.out, a.row_type, at, x.x * inv);
-          store_row(a.out, a.row_type, at + 1, x.y * inv);
-          store_row(a.out, a.row_type, at + 2, x.z * inv);
-          store_row(a.out, a.row_type, at + 3, x.w * inv);
-          if (a.lse && e0 % DH == 0)
-            a.lse[lse0 + h] = ll == 0.f ? -INFINITY : (mm - kLift + log2f(ll)) * 0.693147180559945f;
+#pragma unroll
+          for (int i = 0; i < HW; ++i) {
+            float top = fmaxf(mm[i], mp[i]);
+#pragma unroll
+            for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float keep = mm[i] == -INFINITY ? 1.f : ex2(mm[i] - top);
+            const float wp = mp[i] == -INFINITY ? 1.f : ex2(mp[i] - top);
+            ll[i] = ll[i] * keep + f[i] * wp;
+            x[i].x *= keep;
+            x[i].y *= keep;
+            x[i].z *= keep;
+            x[i].w *= keep;
+            mm[i] = top;
+            f[i] = on ? wp : 0.f;
+          }
+          const int k1 = min(32, pieces - p0);
+          for (int k0 = 0; k0 < k1; k0 += kFly) {
+            float4 y[kFly][HW];
+#pragma unroll
+            for (int k = 0; k < kFly; ++k) {
+              const float4* src =
+                  reinterpret_cast<const float4*>(slot_of(first + p0 + min(k0 + k, k1 - 1)) + warp * DH) + col4;
+#pragma unroll
+              for (int i = 0; i < HW; ++i) y[k][i] = __ldcg(src + i * kAttnWarps * (DH / 4));
+            }
+#pragma unroll
+            for (int k = 0; k < kFly; ++k)
+#pragma unroll
+              for (int i = 0; i < HW; ++i) {
+                const float fk = __shfl_sync(0xffffffffu, f[i], (k0 + k) & 31);
+                if (k0 + k >= k1) continue;
+                x[i].x += fk * y[k][i].x;
+                x[i].y += fk * y[k][i].y;
+                x[i].z += fk * y[k][i].z;
+                x[i].w += fk * y[k][i].w;
+              }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < HW; ++i) {
+          const int h = warp + i * kAttnWarps;
+#pragma unroll
+          for (int w = 16; w; w >>= 1) ll[i] += __shfl_xor_sync(0xffffffffu, ll[i], w);
+          if (h >= heads) continue;
+          if (lane < DH / 4) {
+            const float inv = ll[i] == 0.f ? 0.f : 1.f / ll[i];
+            const long long at = out0 + (long long)h * DH + lane * 4;
+            const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            store_rows<4>(a.out, a.row_type, a.out_vec, at, v, inv);
+          }
+          if (a.lse && lane == 0)
+            a.lse[lse0 + h] = ll[i] == 0.f ? -INFINITY : (mm[i] - kLift + log2f(ll[i])) * 0.693147180559945f;
         }
         if (tid == 0) a.tickets[first] = 0;   // ready for the next call
       }
