@@ -115,33 +115,40 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t a, uint32_t (&r)[4]) 
                : "r"(a));
 }
 
-// D += A B: A [16 x k] (rows g and g + 8 of lane group g), B [k x 8].
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
-      "%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
-      "%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
+// D += A B: A [16 x k] (rows g and g + 8 of lane group g), B [k x 8]; FIRST:
+// D = A B, without registers of zeros to start from.
+#define TB2_MMA(name, shape_types)                                                                                   \
+  template <bool FIRST = false>                                                                                      \
+  __device__ __forceinline__ void name(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {                    \
+    if constexpr (FIRST) {                                                                                           \
+      asm("mma.sync.aligned." shape_types " {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"     \
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                           \
+          : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));                                     \
+    } else {                                                                                                         \
+      asm("mma.sync.aligned." shape_types " {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"         \
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                           \
+          : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));                                               \
+    }                                                                                                                \
+  }
+TB2_MMA(mma_f16, "m16n8k16.row.col.f32.f16.f16.f32")
+TB2_MMA(mma_bf16, "m16n8k16.row.col.f32.bf16.bf16.f32")
+TB2_MMA(mma_tf32, "m16n8k8.row.col.f32.tf32.tf32.f32")
+#undef TB2_MMA
 template <int CT>
-__device__ __forceinline__ void mma16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  if constexpr (CT == kCacheBF16) mma_bf16(d, a, b0, b1);
-  else mma_f16(d, a, b0, b1);
+__device__ __forceinline__ void mma16(bool first, float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  // (`first` is a constant once the loops around it are unrolled)
+  if constexpr (CT == kCacheBF16) {
+    if (first) mma_bf16<true>(d, a, b0, b1);
+    else mma_bf16(d, a, b0, b1);
+  } else {
+    if (first) mma_f16<true>(d, a, b0, b1);
+    else mma_f16(d, a, b0, b1);
+  }
 }
-__device__ __forceinline__ void zero(float (&d)[4]) { d[0] = d[1] = d[2] = d[3] = 0.f; }
+__device__ __forceinline__ void mma8(bool first, float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  if (first) mma_tf32<true>(d, a, b0, b1);
+  else mma_tf32(d, a, b0, b1);
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -169,20 +176,29 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return r;
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 // Two values as one register of plane values (lower half first), what is left
 // of them going on to the next plane.
 __device__ __forceinline__ uint32_t plane_f16(float& x, float& y) {
   const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  x -= f.x;
-  y -= f.y;
+  const float2 f = __half22float2(h), r = fma2(f, make_float2(-1.f, -1.f), make_float2(x, y));
+  x = r.x;
+  y = r.y;
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t plane_bf16(float& x, float& y) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  const float2 f = __bfloat1622float2(h);
-  x -= f.x;
-  y -= f.y;
+  const float2 f = __bfloat1622float2(h), r = fma2(f, make_float2(-1.f, -1.f), make_float2(x, y));
+  x = r.x;
+  y = r.y;
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <int CT>
@@ -223,15 +239,6 @@ struct ScalePair {
     return i & 1 ? __high2float(h) : __low2float(h);
   }
 };
-
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
-      "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
 
 template <int CT, int DH, int HT, int PL>
 struct Cfg {
@@ -534,6 +541,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   const int lr = lane / C::CR, lc = lane % C::CR;
   const long long row_bytes = a.kv.tok_stride * C::E;
   const long long lane_off = lr * row_bytes + lc * 16;
+  const long long scale_off = lane % C::PR * (a.kv.tok_stride / 32);
   const bool dense = a.kv.tok_stride == DH;   // a page's rows of a head are one run of bytes
   auto scales = [&](uint32_t s, int r, long long at, bool on) {   // Q8_0: the scales of row r, from block `at`
     const uint32_t dk = s + C::kOffKS + r * C::NB * 2, dv = s + C::kOffVS + r * C::NB * 2;
@@ -587,8 +595,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
           for (int i = 0; i < C::RPL; ++i) {
             const int r = lane + 32 * i;
-            const long long p0 = __shfl_sync(0xffffffffu, piece, r / C::PR);
-            scales(s, r, (p0 + (r % C::PR) * a.kv.tok_stride) / 32, true);
+            scales(s, r, (long long)((unsigned long long)__shfl_sync(0xffffffffu, piece, r / C::PR) >> 5) + scale_off,
+                   true);
           }
         }
       } else {
@@ -638,7 +646,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   // ---- this warp's sums over the current history
   float2 o[OT][R];
   float m[R], l[R], fac[R];
-  float inv_d = 0.f;   // Q8_0: V's block scales are used times inv_d, a power of two near 1 / the largest so far
+  // Q8_0: the weights carry 2^lift_d, near 1 / the largest |V scale| so far, so that their products with the scales
+  // fill the f16 range (the factor is in l too and cancels)
+  int lift_d = 0;
+  bool have_d = false;
   int stage_out = 0;
   long long u = u_lo;
   while (u < u_hi) {
@@ -760,7 +771,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int r = 0; r < R; ++r) o[i][r] = make_float2(0.f, 0.f);
-    if constexpr (CT == kCacheQ8) inv_d = 0.f;
+    have_d = false;
+    lift_d = 0;
     const uint32_t qb = smem_u32(region) + lane * 16, qh = smem_u32(region) + C::KS * 512 + lane * 8;
     auto q_at = [&](int p, int st) {   // register set p of step st
       if (C::kHalf && p == 1) {
@@ -780,10 +792,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       // scores of the tile: lane (g, c) has keys 8 i + 2 c, + 1 of rows g (and g + 8)
       float s[NT][2 * R];
       if constexpr (CT == kCacheQ8) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int k = 0; k < 2 * R; ++k) s[i][k] = 0.f;
         ScalePair<C::NB> ksc[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) ksc[i].load(ks + C::kOffKS + (8 * i + 2 * c) * C::NB * 2);
@@ -799,32 +807,31 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             const uint2 w =
                 lds64(ks + g * C::KP + (((2 * blk + (c >> 1)) ^ C::k_swz(g)) * 16 + (c & 1) * 8) + 8 * i * C::KP);
             const uint32_t w0 = w.x ^ 0x80808080u, w1 = w.y ^ 0x80808080u;
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            float d[4];
             const uint32_t b0 = i8pair_f16(w0, 0x4140), b1 = i8pair_f16(w0, 0x4342), b2 = i8pair_f16(w1, 0x4140),
                            b3 = i8pair_f16(w1, 0x4342);
 #pragma unroll
             for (int p = 0; p < C::QS; ++p) {
-              mma_f16(d, qa[p][0], b0, b1);
-              mma_f16(d, qa[p][1], b2, b3);
+              mma16<CT>(p == 0, d, qa[p][0], b0, b1);
+              mma16<CT>(false, d, qa[p][1], b2, b3);
             }
             const float s0 = ksc[i].at(0, blk), s1 = ksc[i].at(1, blk);
-            if constexpr (HT == 8) {
-              s[i][0] = fmaf(s0, d[0] + d[2], s[i][0]);
-              s[i][1] = fmaf(s1, d[1] + d[3], s[i][1]);
-            } else {
-              s[i][0] = fmaf(s0, d[0], s[i][0]);
-              s[i][1] = fmaf(s1, d[1], s[i][1]);
-              s[i][2] = fmaf(s0, d[2], s[i][2]);
-              s[i][3] = fmaf(s1, d[3], s[i][3]);
+            const float2 sc = make_float2(s0, s1);
+            float2 x = make_float2(d[0], d[1]);
+            const float2 y = make_float2(d[2], d[3]);
+            if constexpr (HT == 8) x = add2(x, y);
+            x = blk == 0 ? mul2(x, sc) : fma2(x, sc, make_float2(s[i][0], s[i][1]));
+            s[i][0] = x.x;
+            s[i][1] = x.y;
+            if constexpr (HT == 16) {
+              const float2 z = blk == 0 ? mul2(y, sc) : fma2(y, sc, make_float2(s[i][2 * R - 2], s[i][2 * R - 1]));
+              s[i][2 * R - 2] = z.x;
+              s[i][2 * R - 1] = z.y;
             }
           }
         }
       } else {
         float d[NT][C::A][4];
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int k = 0; k < C::A; ++k) zero(d[i][k]);
 #pragma unroll
         for (int st = 0; st < C::KS; st += 2) {   // one 16-byte read of each key row feeds two steps
           uint4 qa[C::QS][2];
@@ -846,29 +853,35 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 float (&small)[4] = d[i][C::A == 4 ? 2 + k : 1], (&large)[4] = d[i][C::A == 4 ? k : 0];
-                mma_tf32(small, qa[0][k], lo[2 * k], lo[2 * k + 1]);
-                if constexpr (HT == 16) mma_tf32(small, qa[1][k], hi[2 * k], hi[2 * k + 1]);
-                mma_tf32(large, qa[0][k], hi[2 * k], hi[2 * k + 1]);
+                const bool first = st == 0 && (C::A == 4 || k == 0);
+                mma8(first, small, qa[0][k], lo[2 * k], lo[2 * k + 1]);
+                if constexpr (HT == 16) mma8(false, small, qa[C::QS - 1][k], hi[2 * k], hi[2 * k + 1]);
+                mma8(first, large, qa[0][k], hi[2 * k], hi[2 * k + 1]);
               }
             } else {
 #pragma unroll
               for (int p = C::QS - 1; p >= 0; --p) {
-                mma16<CT>(d[i][0], qa[p][0], w.x, w.y);
-                mma16<CT>(d[i][C::A - 1], qa[p][1], w.z, w.w);
+                mma16<CT>(st == 0 && p == C::QS - 1, d[i][0], qa[p][0], w.x, w.y);
+                mma16<CT>(C::A == 2 && st == 0 && p == C::QS - 1, d[i][C::A - 1], qa[p][1], w.z, w.w);
               }
             }
           }
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          float x[4];
+          float2 x[2];   // rows g, rows g + 8
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (C::A == 4) x[k] = (d[i][0][k] + d[i][1][k]) + (d[i][2][k] + d[i][3][k]);
-            else x[k] = C::A == 2 ? d[i][0][k] + d[i][C::A - 1][k] : d[i][0][k];
+          for (int h = 0; h < 2; ++h) {
+            x[h] = make_float2(d[i][0][2 * h], d[i][0][2 * h + 1]);
+#pragma unroll
+            for (int k = 1; k < C::A; ++k) x[h] = add2(x[h], make_float2(d[i][k][2 * h], d[i][k][2 * h + 1]));
           }
+          if constexpr (HT == 8) x[0] = add2(x[0], x[1]);
 #pragma unroll
-          for (int k = 0; k < 2 * R; ++k) s[i][k] = HT == 8 ? x[k] + x[(k + 2) & 3] : x[k];
+          for (int r = 0; r < R; ++r) {
+            s[i][2 * r] = x[r].x;
+            s[i][2 * r + 1] = x[r].y;
+          }
         }
       }
 
@@ -894,7 +907,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         mx[r] = fmaxf(m[r], x * fac[r]);   // (a NaN, or -inf times a factor of 0, leaves m)
         grew |= mx[r] != m[r];
       }
-      float new_inv = inv_d;
+      int new_lift = lift_d;
       ScalePair<C::NB> vsc[CT == kCacheQ8 ? NT : 1];
       if constexpr (CT == kCacheQ8) {
         uint32_t big = 0;   // the tile's largest |V scale|, as fp16 bits
@@ -905,11 +918,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
           for (int e = 0; e < C::NB; ++e) big = __vmaxu2(big, vsc[i].w[e] & 0x7fff7fffu);
         }
         big = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
-        const float top = fmaxf(__half2float(__ushort_as_half((uint16_t)big)), 0x1p-24f);
-        // 1 / the power of two at or below it (an infinite scale makes the sums NaN)
-        const float inv = __uint_as_float((254u << 23) - (__float_as_uint(top) & 0x7f800000u));
-        if (inv_d == 0.f || inv < inv_d) new_inv = inv;
-        grew |= new_inv != inv_d;
+        // below 2^(1 - lift) (an infinite scale makes the sums NaN whatever the lift)
+        const int lift = 127 - (int)(__float_as_uint(fmaxf(__half2float(__ushort_as_half((uint16_t)big)), 0x1p-24f)) >> 23);
+        if (!have_d || lift < lift_d) new_lift = lift;
+        grew |= !have_d || new_lift != lift_d;
       }
       if (__any_sync(0xffffffffu, grew)) {
         float shrink[R];
@@ -917,15 +929,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         for (int r = 0; r < R; ++r) {
           shrink[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx[r]);
           m[r] = mx[r];
+          if constexpr (CT == kCacheQ8) shrink[r] *= ex2((float)(new_lift - (have_d ? lift_d : new_lift)));
           l[r] *= shrink[r];
         }
-        if constexpr (CT == kCacheQ8) {
-          if (inv_d != 0.f) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) shrink[r] *= new_inv / inv_d;
-          }
-          inv_d = new_inv;
-        }
+        lift_d = new_lift;
+        have_d = true;
 #pragma unroll
         for (int i = 0; i < OT; ++i)
 #pragma unroll
@@ -933,7 +941,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float base = m[r] == -INFINITY ? 0.f : kLift - m[r];
+        const float lifted = CT == kCacheQ8 ? kLift + (float)lift_d : kLift;
+        const float base = m[r] == -INFINITY ? 0.f : lifted - m[r];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -981,8 +990,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         for (int q4 = 0; q4 < DH / 32; ++q4) {   // columns 32 q4 + 4 g .. + 3: one per output tile
           float d[4][4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) zero(d[k]);
-#pragma unroll
           for (int i = 0; i < NT; ++i) {
             const uint4 w0 = lds128(vs + 2 * c * C::VP + g * 16 + 8 * i * C::VP + q4 * 128);
             const uint4 w1 = lds128(vs + 2 * c * C::VP + g * 16 + (8 * i + 1) * C::VP + q4 * 128);
@@ -992,9 +999,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
               const uint32_t a0 = tf32(__uint_as_float(x0[k])), a1 = tf32(__uint_as_float(x1[k]));
               const uint32_t e0 = tf32(__uint_as_float(x0[k]) - __uint_as_float(a0));
               const uint32_t e1 = tf32(__uint_as_float(x1[k]) - __uint_as_float(a1));
-              mma_tf32(d[k], ph[i], e0, e1);
-              if constexpr (HT == 16) mma_tf32(d[k], pl[i], a0, a1);
-              mma_tf32(d[k], ph[i], a0, a1);
+              mma8(i == 0, d[k], ph[i], e0, e1);
+              if constexpr (HT == 16) mma8(false, d[k], pl[i], a0, a1);
+              mma8(false, d[k], ph[i], a0, a1);
             }
           }
 #pragma unroll
@@ -1005,25 +1012,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         for (int blk = 0; blk < C::NB; ++blk) {
           float d[4][4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) zero(d[k]);
-#pragma unroll
           for (int i = 0; i < NT; i += 2) {   // 16 keys
-            float dv[4];
+            float2 dv[2];   // their scales of this block
 #pragma unroll
-            for (int k = 0; k < 4; ++k) dv[k] = inv_d * vsc[i + (k >> 1)].at(k & 1, blk);
+            for (int k = 0; k < 2; ++k) dv[k] = make_float2(vsc[i + k].at(0, blk), vsc[i + k].at(1, blk));
             uint4 ph, pl;
             if constexpr (HT == 8) {
-              float x0 = s[i][0] * dv[0], x1 = s[i][1] * dv[1], x2 = s[i + 1][0] * dv[2], x3 = s[i + 1][1] * dv[3];
-              ph.x = plane_f16(x0, x1);
-              ph.z = plane_f16(x2, x3);
-              ph.y = plane_f16(x0, x1);
-              ph.w = plane_f16(x2, x3);
+              float2 x = mul2(make_float2(s[i][0], s[i][1]), dv[0]), y = mul2(make_float2(s[i + 1][0], s[i + 1][1]), dv[1]);
+              ph.x = plane_f16(x.x, x.y);
+              ph.z = plane_f16(y.x, y.y);
+              ph.y = plane_f16(x.x, x.y);
+              ph.w = plane_f16(y.x, y.y);
             } else {
               float x[8];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                x[k] = s[i][k] * dv[k & 1];
-                x[4 + k] = s[i + 1][k] * dv[2 + (k & 1)];
+                x[k] = s[i][k] * (k & 1 ? dv[0].y : dv[0].x);
+                x[4 + k] = s[i + 1][k] * (k & 1 ? dv[1].y : dv[1].x);
               }
               ph.x = plane_f16(x[0], x[1]);
               ph.y = plane_f16(x[2], x[3]);
@@ -1046,8 +1051,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             for (int k = 0; k < 4; ++k) {
               const uint32_t sel = k & 1 ? 0x4342 : 0x4140;
               const uint32_t b0 = i8pair_f16(k < 2 ? p0 : p1, sel), b1 = i8pair_f16(k < 2 ? p2 : p3, sel);
-              if constexpr (HT == 16) mma_f16(d[k], pl, b0, b1);
-              mma_f16(d[k], ph, b0, b1);
+              if constexpr (HT == 16) mma16<CT>(i == 0, d[k], pl, b0, b1);
+              mma16<CT>(HT == 8 && i == 0, d[k], ph, b0, b1);
             }
           }
 #pragma unroll
@@ -1089,16 +1094,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
         for (int d2 = 0; d2 < OT; d2 += 2) {
           float e0[4], e1[4];
-          zero(e0);
-          zero(e1);
 #pragma unroll
           for (int i = 0; i < NT; i += 2) {
             uint32_t b[4];   // keys 0..7 and 8..15 of columns 8 d2 .., then of 8 d2 + 8 ..
             ldmatrix_x4_trans(vs + (lane & 15) * C::VP + (lane >> 4) * 16 + 8 * i * C::VP + d2 * 16, b);
 #pragma unroll
             for (int p = kP - 1; p >= 0; --p) {
-              mma16<CT>(e0, pp[i / 2][p], b[0], b[1]);
-              mma16<CT>(e1, pp[i / 2][p], b[2], b[3]);
+              mma16<CT>(i == 0 && p == kP - 1, e0, pp[i / 2][p], b[0], b[1]);
+              mma16<CT>(i == 0 && p == kP - 1, e1, pp[i / 2][p], b[2], b[3]);
             }
           }
           gather(d2, e0);
@@ -1112,12 +1115,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 
     // ---- the warps' sums joined: weights of a lane group summed
     float2 (&ov)[OT][R] = o;
-    if constexpr (CT == kCacheQ8) {
-      const float back = inv_d == 0.f ? 0.f : 1.f / inv_d;
+    if constexpr (CT == kCacheQ8) {   // the same lift in every warp
+      const float back = ex2(-(float)lift_d);
 #pragma unroll
-      for (int i = 0; i < OT; ++i)
+      for (int r = 0; r < R; ++r) {
+        l[r] *= back;
 #pragma unroll
-        for (int r = 0; r < R; ++r) ov[i][r] = mul2(ov[i][r], make_float2(back, back));
+        for (int i = 0; i < OT; ++i) ov[i][r] = mul2(ov[i][r], make_float2(back, back));
+      }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
