@@ -48,8 +48,7 @@ size_t tb2_paged_attend_workspace(void) { return tb2::kAttnWorkspace; }
 int tb2_paged_attend_workspace_init(void* workspace, size_t bytes, void* stream) {
   if (!workspace || bytes < tb2::kAttnWorkspace || !tb2::aligned(workspace, 16)) return -1;
   // the tickets are what a call expects to find at 0
-  return cudaMemsetAsync(workspace, 0, tb2::kAttnTicketBytes, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0
-                                                                                                               : -3;
+  return cudaMemsetAsync(workspace, 0, tb2::kAttnTicketBytes, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0 : -3;
 }
 
 int tb2_paged_attend(const tb2_paged_kv* kv, const tb2_paged_attend_args* a, void* stream) {
@@ -64,6 +63,9 @@ int tb2_paged_attend(const tb2_paged_kv* kv, const tb2_paged_attend_args* a, voi
   if (a->table_width < 1 || a->table_stride < a->table_width ||
       (long long)a->table_width * kv->page_size > 0x7fffff00LL)
     return -1;
+  // (the units of every table row filled, at the smallest unit, are numbered in 31 bits)
+  const long long tiles_h = (a->n_heads / kv->n_kv + 7) / 8;
+  if ((((long long)a->table_width * kv->page_size + 31) / 32) * kv->n_kv * tiles_h > 0x7fffffffLL / a->n_req) return -1;
   if (!std::isfinite(a->scale)) return -1;
   if (!a->workspace || a->workspace_bytes < tb2::kAttnWorkspace || !tb2::aligned(a->workspace, 16)) return -1;
   int* err = tb2::device_error_word();

@@ -42,12 +42,12 @@
 namespace tb2 {
 
 constexpr int kAttnWarps = 4;
-constexpr int kMinUnits = 2;            // units that are worth a CTA
-constexpr int kAttnMaxCtas = 4 * 148;   // the workspace's slots
-constexpr int kAttnSlotFloats = 16 * 128 + 2 * 16;
-// tickets, then two partial slots per CTA
+constexpr int kMinUnits = 2;    // units that are worth a CTA
+constexpr int kAttnMaxCtas = 4 * 148;
+// workspace: a ticket per CTA (0 between calls), two partial slots per CTA
 constexpr size_t kAttnTicketBytes = (kAttnMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
-constexpr size_t kAttnWorkspace = kAttnTicketBytes + (size_t)kAttnMaxCtas * 2 * kAttnSlotFloats * sizeof(float);
+constexpr size_t kAttnWorkspace =
+    kAttnTicketBytes + (size_t)2 * 148 * 2 * sizeof(float) * (16 * 128 + 2 * 16);   // (two CTAs of 16 heads an SM)
 
 enum AttnCache : int { kCacheF32 = 0, kCacheF16 = 1, kCacheBF16 = 2, kCacheQ8 = 3 };
 
@@ -375,9 +375,9 @@ __device__ __forceinline__ void store_rows(void* p, int type, bool vec, long lon
 }
 
 // A place in the list of units: unit t of key head (and head tile) jt of
-// request b, whose history has nt units.
+// request b, whose history has len keys.
 struct Cursor {
-  int b, jt, t, nt, len;
+  int b, jt, t, len;
 };
 
 template <int CT, int DH, int HT, int PL>
@@ -390,6 +390,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint64_t valid[kAttnWarps][ST];   // keys of a staged tile that count
   __shared__ int last_flag;
+  __shared__ int pre[kAttnWarps * 32];   // units (of one key head) before each thread's run of requests
   __shared__ float qmax[kAttnWarps][HT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   uint8_t* region = smem + kAttnWarps * ST * C::kStage;
@@ -401,27 +402,24 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   const int tiles_h = (a.group + HT - 1) / HT, KVH = a.kv.n_kv * tiles_h;
   auto length = [&](int b) { return (int)min(most, (long long)max(0, __ldg(a.lens + b))); };
 
-  // ---- the list's length and this CTA's range of it
-  long long total;
-  long long* pre = reinterpret_cast<long long*>(region);   // units before each thread's run of requests
+  // ---- the list's length (below 2^31 by the host's limit)
+  auto units_of = [](int len) { return (len + UK - 1) / UK; };
+  int total;
   const int per = (n + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
   {
     const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
-    long long s = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int len = length(b);
-      s += (len + UK - 1) / UK;
-    }
-    long long inc = s;
+    int s = 0;
+    for (int b = b0; b < b1; ++b) s += units_of(length(b));
+    int inc = s;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    __shared__ long long wsum[kAttnWarps];
+    __shared__ int wsum[kAttnWarps];
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    long long base = 0;
+    int base = 0;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kAttnWarps; ++w) {
@@ -438,102 +436,108 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     if (a.lse)
       for (int h = tid; h < a.n_heads; h += blockDim.x) a.lse[(long long)b * a.n_heads + h] = -INFINITY;
   }
-  const long long units = total * KVH;
-  const long long G = max(1LL, min((long long)gridDim.x, units / kMinUnits));
-  if (units == 0 || blockIdx.x >= G) return;
-  const long long u_lo = blockIdx.x * units / G, u_hi = (blockIdx.x + 1) * units / G;
+  const int units = total * KVH;
+  if (units == 0) return;
+  // Equal ranges of the list (a unit more or less), kMinUnits at least. (The memory does not serve all SMs alike: on a
+  // long bf16 history the first CTA is done after 62 us and the last after 92. Smaller ranges, handed out as CTAs
+  // become free, did not make the last one earlier: the memory is busy to the end, and every range costs 2 us.)
+  const int G = max(1, min((int)gridDim.x, units / kMinUnits));
+  if (blockIdx.x >= G) return;
+  auto range = [&](int i) { return (int)((long long)i * units / G); };
+  auto cta_of = [&](int u) { return (int)(((u + 1LL) * G - 1) / units); };   // whose range holds unit u
 
-  Cursor cur;
-  long long cur_first;   // the list's index of the cursor's request
-  {
-    const long long key = u_lo / KVH;
+  // the place of list index u, and the list index at which its request starts
+  auto locate = [&](int u, Cursor& k, int& first) {
+    const int key = u / KVH;
     int lo = 0, hi = kAttnWarps * 32;   // the last thread whose run starts at or before key
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (pre[mid] <= key) lo = mid;
       else hi = mid;
     }
-    long long base = pre[lo];
-    int b = lo * per;
-    for (;;) {
-      const int i = b + lane;
-      const int nt = i < n ? (length(i) + UK - 1) / UK : 0;
-      long long inc = nt;
+    int base = pre[lo], b = lo * per;
+    for (;;) {   // (32 requests of the run at a time)
+      const int i = b + lane, nt = i < n && lane < per ? units_of(length(i)) : 0;
+      int inc = nt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += x;
       }
       const unsigned past = __ballot_sync(0xffffffffu, base + inc > key);
       if (past) {
         const int f = __ffs(past) - 1;
-        cur.b = b + f;
+        k.b = b + f;
         base += __shfl_sync(0xffffffffu, inc - nt, f);
         break;
       }
       base += __shfl_sync(0xffffffffu, inc, 31);
       b += 32;
     }
-    cur.len = length(cur.b);
-    cur.nt = (cur.len + UK - 1) / UK;
-    cur_first = base * KVH;
-    const long long r = u_lo - cur_first;
-    cur.jt = (int)(r / cur.nt);
-    cur.t = (int)(r - (long long)cur.jt * cur.nt);
-  }
-  __syncthreads();   // pre is read: the region is free
+    k.len = length(k.b);
+    first = base * KVH;
+    const int nt = units_of(k.len);
+    k.jt = (u - first) / nt;
+    k.t = u - first - k.jt * nt;
+  };
 
   // the next (request, head) of the list; the caller knows that there is one
-  auto next_history = [&](Cursor& k, long long* first) {
+  auto next_history = [&](Cursor& k, int& first) {
     k.t = 0;
     if (++k.jt < KVH) return;
     k.jt = 0;
-    if (first) *first += (long long)k.nt * KVH;
+    first += units_of(k.len) * KVH;
     do {
       ++k.b;
       k.len = length(k.b);
     } while (k.len == 0);
-    k.nt = (k.len + UK - 1) / UK;
   };
+
+  Cursor cur;                  // this CTA's place
+  int u = range(blockIdx.x), cur_first;
+  const int u_hi = range(blockIdx.x + 1);
+  locate(u, cur, cur_first);
+  Cursor pc = cur;             // and the producer's
+  int pu = u;
 
   // ---- the ring: tiles of this warp in list order
   // Where the page size is a multiple of 16, the 16 rows (or the tile, if it
-  // has fewer) from a multiple of 16 on lie in one page: lane i reads the page
-  // id of piece i of the next tile, and a full tile of good pages is copied
-  // with an address per piece. Other page sizes, and the last tile of a
-  // history, take an address per row.
-  Cursor pc = cur;             // the producer's place
-  long long pu = u_lo;         // list index of its unit
-  int page_id[C::RPL];         // page ids of the next tile's pieces (lane % NP), or rows (lane + 32 i)
+  // has fewer) from a multiple of 16 on lie in one page: the lanes read the
+  // page ids of the next tiles' pieces together, and a full tile of good pages
+  // is copied with an address per piece. Other page sizes, and the last tile
+  // of a history, take an address per row.
   constexpr bool kEven = 32 % C::CR == 0;   // a lane copies the same chunk of every row it has (not at d_head 96)
+  constexpr int kWin = 32 / C::NP;          // tiles whose page ids are read at once
   const bool pieces16 = kEven && P % 16 == 0;
-  auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / P; };
-  auto tile_key = [&]() { return (pc.t * kAttnWarps + warp) * TK; };
-  auto row_key = [&](int i) { return tile_key() + (TK < 32 ? lane % TK : lane + 32 * i); };
+  int win = 0, win_t = 0;      // lane's page id; the unit that the window starts at
   const int* pages = nullptr;  // the history's row of the block table
   long long head = 0;          // and its key head's offset in a page
+  auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / P; };
+  auto tile_key = [&]() { return (pc.t * kAttnWarps + warp) * TK; };
+  auto read_page = [&](int key) { return key < pc.len ? __ldg(pages + page_of(key)) : -1; };
+  auto read_window = [&]() {
+    win_t = pc.t;
+    // (units past the history: a key beyond its length; the sum stays in 32 bits, see the limit on tables)
+    const long long key = ((long long)(win_t + lane / C::NP) * kAttnWarps + warp) * TK + lane % C::NP * C::PR;
+    win = key < pc.len ? read_page((int)key) : -1;
+  };
   auto enter = [&]() {
     pages = a.table + pc.b * a.table_stride;
     head = pc.jt / tiles_h * a.kv.head_stride;
+    if (pieces16) read_window();
   };
   auto next_unit = [&]() {
     ++pu;
-    if (++pc.t == pc.nt && pu < u_hi) {
-      next_history(pc, nullptr);
+    if (++pc.t * UK >= pc.len && pu < u_hi) {
+      int unused = 0;
+      next_history(pc, unused);
       enter();
     }
   };
-  auto read_page = [&](int key) { return key < pc.len ? __ldg(pages + page_of(key)) : -1; };
-  auto fetch_pages = [&]() {
-    // (the last unit of a history may hold no tile of this warp)
+  // whether there is a tile to fetch (the last unit of a history may hold none of this warp's)
+  auto has_tile = [&]() {
     while (pu < u_hi && tile_key() >= pc.len) next_unit();
-    if (pu >= u_hi) return;
-    if (pieces16) {
-      page_id[0] = read_page(tile_key() + lane % C::NP * C::PR);
-    } else {
-#pragma unroll
-      for (int i = 0; i < C::RPL; ++i) page_id[i] = read_page(row_key(i));
-    }
+    return pu < u_hi;
   };
   // this lane's part of a copy: 16-byte chunk lc of rows lr, lr + kStep, ..
   constexpr int kIter = TK * C::CR / 32;
@@ -556,92 +560,107 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       }
     }
   };
-  int stage_in = 0;
-  auto issue = [&]() {
-    if (pu < u_hi) {
-      const uint32_t s = ring + stage_in * C::kStage;
-      const int key0 = tile_key();
-      const bool fast = pieces16 && key0 + TK <= pc.len &&
-                        __all_sync(0xffffffffu, page_id[0] >= 0 && page_id[0] < a.kv.n_pages);
-      if (fast) {
-        const int pk = key0 + lane % C::NP * C::PR;
-        const long long piece = page_id[0] * a.kv.page_stride + head + (pk - page_of(pk) * P) * a.kv.tok_stride;
-        if (lane == 0) valid[warp][stage_in] = ~0ull;
-        constexpr int kPer = kIter / C::NP;   // copies of a piece
-        const uint32_t dk = s + lr * C::KP + (lc ^ C::k_swz(lr)) * 16;
-        auto dv = [&](int r) { return s + C::kOffV + lr * C::VP + (lc ^ C::v_swz(lr + r)) * 16 + r * C::VP; };
+  int used = 0, staged = 0;   // tiles consumed; tiles fetched and not consumed
+  auto issue = [&]() {        // fetch the next tile into the stage that is free
+    const int stage = (used + staged) & 1;
+    const uint32_t s = ring + stage * C::kStage;
+    const int key0 = tile_key();
+    if (pieces16 && pc.t - win_t >= kWin) read_window();
+    int page = -1;
+    if (pieces16) page = __shfl_sync(0xffffffffu, win, (pc.t - win_t) * C::NP + lane % C::NP);
+    const bool fast = pieces16 && key0 + TK <= pc.len && __all_sync(0xffffffffu, page >= 0 && page < a.kv.n_pages);
+    if (fast) {
+      const int pk = key0 + lane % C::NP * C::PR;
+      const long long piece = page * a.kv.page_stride + head + (pk - page_of(pk) * P) * a.kv.tok_stride;
+      if (lane == 0) valid[warp][stage] = ~0ull;
+      constexpr int kPer = kIter / C::NP;   // copies of a piece
+      const uint32_t dk = s + lr * C::KP + (lc ^ C::k_swz(lr)) * 16;
+      auto dv = [&](int r) { return s + C::kOffV + lr * C::VP + (lc ^ C::v_swz(lr + r)) * 16 + r * C::VP; };
 #pragma unroll
-        for (int p = 0; p < C::NP; ++p) {
-          const long long base = __shfl_sync(0xffffffffu, piece, p) * C::E + lane_off;
-          const uint8_t* sk = static_cast<const uint8_t*>(a.kv.k) + base;
-          const uint8_t* sv = static_cast<const uint8_t*>(a.kv.v) + base;
-          if (dense) {   // (addresses of one register and constants)
+      for (int p = 0; p < C::NP; ++p) {
+        const long long base = __shfl_sync(0xffffffffu, piece, p) * C::E + lane_off;
+        const uint8_t* sk = static_cast<const uint8_t*>(a.kv.k) + base;
+        const uint8_t* sv = static_cast<const uint8_t*>(a.kv.v) + base;
+        if (dense) {   // (addresses of one register and constants)
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const int r = (p * kPer + i) * kStep;
-              cp16(dk + r * C::KP, sk + i * kStep * (DH * C::E));
-              cp16(dv(r), sv + i * kStep * (DH * C::E));
-            }
-          } else {
-#pragma unroll 1
-            for (int i = 0; i < kPer; ++i) {
-              const int r = (p * kPer + i) * kStep;
-              cp16(dk + r * C::KP, sk + i * kStep * row_bytes);
-              cp16(dv(r), sv + i * kStep * row_bytes);
-            }
+          for (int i = 0; i < kPer; ++i) {
+            const int r = (p * kPer + i) * kStep;
+            cp16(dk + r * C::KP, sk + i * kStep * (DH * C::E));
+            cp16(dv(r), sv + i * kStep * (DH * C::E));
           }
-        }
-        if constexpr (CT == kCacheQ8) {
-#pragma unroll
-          for (int i = 0; i < C::RPL; ++i) {
-            const int r = lane + 32 * i;
-            scales(s, r, (long long)((unsigned long long)__shfl_sync(0xffffffffu, piece, r / C::PR) >> 5) + scale_off,
-                   true);
-          }
-        }
-      } else {
-        if (pieces16) {   // ids of rows in place of pieces
-#pragma unroll
-          for (int i = 0; i < C::RPL; ++i) page_id[i] = read_page(row_key(i));
-        }
-        long long off[C::RPL];
-        uint64_t ok = 0;
-#pragma unroll
-        for (int i = 0; i < C::RPL; ++i) {
-          const int key = row_key(i), page = page_id[i];
-          const bool in = key < pc.len, good = in && page >= 0 && page < a.kv.n_pages;
-          if (in && !good) *a.err = kErrPagedPage;
-          off[i] = good ? page * a.kv.page_stride + head + (key - page_of(key) * P) * a.kv.tok_stride : -1;
-          ok |= (uint64_t)__ballot_sync(0xffffffffu, good) << (32 * i);
-        }
-        if (lane == 0) valid[warp][stage_in] = ok;
-        // (rolled: this path is rare and the code of the others has to stay in the instruction cache)
+        } else {
 #pragma unroll 1
-        for (int it = 0; it < kIter; ++it) {
-          const int i = it * 32 + lane, r = i / C::CR, ch = i % C::CR;
-          const long long lo = __shfl_sync(0xffffffffu, off[0], r & 31);
-          const long long hi = C::RPL > 1 ? __shfl_sync(0xffffffffu, off[C::RPL - 1], r & 31) : lo;
-          const long long o = r < 32 ? lo : hi;
-          const bool on = o >= 0;
-          const long long at = on ? o * C::E + ch * 16 : 0;
-          cp16(s + r * C::KP + (ch ^ C::k_swz(r)) * 16, static_cast<const uint8_t*>(a.kv.k) + at, on);
-          cp16(s + C::kOffV + r * C::VP + (ch ^ C::v_swz(r)) * 16, static_cast<const uint8_t*>(a.kv.v) + at, on);
-        }
-        if constexpr (CT == kCacheQ8) {
-#pragma unroll
-          for (int i = 0; i < C::RPL; ++i) scales(s, lane + 32 * i, off[i] >= 0 ? off[i] / 32 : 0, off[i] >= 0);
+          for (int i = 0; i < kPer; ++i) {
+            const int r = (p * kPer + i) * kStep;
+            cp16(dk + r * C::KP, sk + i * kStep * row_bytes);
+            cp16(dv(r), sv + i * kStep * row_bytes);
+          }
         }
       }
-      next_unit();
-      fetch_pages();
+      if constexpr (CT == kCacheQ8) {
+#pragma unroll
+        for (int i = 0; i < C::RPL; ++i) {
+          const int r = lane + 32 * i;
+          scales(s, r, (long long)((unsigned long long)__shfl_sync(0xffffffffu, piece, r / C::PR) >> 5) + scale_off,
+                 true);
+        }
+      }
+    } else {
+      long long off[C::RPL];
+      uint64_t ok = 0;
+#pragma unroll
+      for (int i = 0; i < C::RPL; ++i) {
+        const int key = key0 + (TK < 32 ? lane % TK : lane + 32 * i), id = read_page(key);
+        const bool in = key < pc.len, good = in && id >= 0 && id < a.kv.n_pages;
+        if (in && !good) *a.err = kErrPagedPage;
+        off[i] = good ? id * a.kv.page_stride + head + (key - page_of(key) * P) * a.kv.tok_stride : -1;
+        ok |= (uint64_t)__ballot_sync(0xffffffffu, good) << (32 * i);
+      }
+      if (lane == 0) valid[warp][stage] = ok;
+      // (rolled: this path is rare and the code of the others has to stay in the instruction cache)
+#pragma unroll 1
+      for (int it = 0; it < kIter; ++it) {
+        const int i = it * 32 + lane, r = i / C::CR, ch = i % C::CR;
+        const long long lo = __shfl_sync(0xffffffffu, off[0], r & 31);
+        const long long hi = C::RPL > 1 ? __shfl_sync(0xffffffffu, off[C::RPL - 1], r & 31) : lo;
+        const long long o = r < 32 ? lo : hi;
+        const bool on = o >= 0;
+        const long long at = on ? o * C::E + ch * 16 : 0;
+        cp16(s + r * C::KP + (ch ^ C::k_swz(r)) * 16, static_cast<const uint8_t*>(a.kv.k) + at, on);
+        cp16(s + C::kOffV + r * C::VP + (ch ^ C::v_swz(r)) * 16, static_cast<const uint8_t*>(a.kv.v) + at, on);
+      }
+      if constexpr (CT == kCacheQ8) {
+#pragma unroll
+        for (int i = 0; i < C::RPL; ++i) scales(s, lane + 32 * i, off[i] >= 0 ? off[i] / 32 : 0, off[i] >= 0);
+      }
     }
-    cp_commit();   // (an empty group at the list's end keeps the count)
-    stage_in = stage_in + 1 == ST ? 0 : stage_in + 1;
+    cp_commit();
+    ++staged;
+    next_unit();
   };
   enter();
-  fetch_pages();
-#pragma unroll 1
-  for (int i = 0; i < ST; ++i) issue();
+
+  // this warp's share of a history's q: step pairs are dealt to the warps
+  constexpr int kOwn = (C::SP + kAttnWarps - 1) / kAttnWarps;
+  float qv[kOwn][R][C::QW];   // the chunks of the lane's rows that its key rows are read by
+  auto load_q = [&](const Cursor& k) {
+    const int jh = k.jt / tiles_h, h0 = (k.jt - jh * tiles_h) * HT, heads = min(HT, a.group - h0);
+    const long long row = (long long)k.b * a.ldq + ((long long)jh * a.group + h0) * DH;
+#pragma unroll
+    for (int own = 0; own < kOwn; ++own)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int sp = warp + own * kAttnWarps;
+        if (g + 8 * r < heads && sp < C::SP) {
+          load_rows<C::QW>(a.q, a.row_type, a.q_vec, row + (long long)(g + 8 * r) * DH + C::chunk(sp, c) * C::QW,
+                           qv[own][r]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < C::QW; ++k) qv[own][r][k] = 0.f;
+        }
+      }
+  };
+  load_q(cur);
 
   // ---- this warp's sums over the current history
   float2 o[OT][R];
@@ -650,35 +669,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   // fill the f16 range (the factor is in l too and cancels)
   int lift_d = 0;
   bool have_d = false;
-  int stage_out = 0;
-  long long u = u_lo;
-  while (u < u_hi) {
-    const int t0 = cur.t, t1 = (int)min((long long)cur.nt, t0 + (u_hi - u));
+  for (;;) {
+    const int nt = units_of(cur.len), t0 = cur.t, t1 = min(nt, t0 + (u_hi - u));
     const int jh = cur.jt / tiles_h, h0 = (cur.jt - jh * tiles_h) * HT;   // key head, first head of the tile
     const int heads = min(HT, a.group - h0);
-    const long long qrow = (long long)cur.b * a.ldq + ((long long)jh * a.group + h0) * DH;
 
+#pragma unroll 1
+    while (staged < ST && has_tile()) issue();
     // q as operand registers: lane (g, c) of step s holds rows g and g + 8.
-    // Step pairs are dealt to the warps.
     float rs[R];   // what the scores of the lane group's heads are multiplied by
     {
-      constexpr int kOwn = (C::SP + kAttnWarps - 1) / kAttnWarps;
-      float qv[kOwn][R][C::QW];   // the chunks of the lane's rows that its key rows are read by
-#pragma unroll
-      for (int own = 0; own < kOwn; ++own)
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int sp = warp + own * kAttnWarps;
-          if (g + 8 * r < heads && sp < C::SP) {
-            load_rows<C::QW>(a.q, a.row_type, a.q_vec, qrow + (long long)(g + 8 * r) * DH + C::chunk(sp, c) * C::QW,
-                             qv[own][r]);
-#pragma unroll
-            for (int k = 0; k < C::QW; ++k) qv[own][r][k] = a.c < 0.f ? -qv[own][r][k] : qv[own][r][k];   // the factor's sign
-          } else {
-#pragma unroll
-            for (int k = 0; k < C::QW; ++k) qv[own][r][k] = 0.f;
-          }
-        }
       if constexpr (CT == kCacheF16 || CT == kCacheQ8) {   // the largest |q| of a row into [16, 32)
         float x[R];
 #pragma unroll
@@ -703,12 +703,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
           for (int own = 0; own < kOwn; ++own)
 #pragma unroll
-            for (int k = 0; k < C::QW; ++k) qv[own][r][k] *= up;
+            for (int k = 0; k < C::QW; ++k) qv[own][r][k] *= a.c < 0.f ? -up : up;   // (the factor's sign too)
           rs[r] = fabsf(a.c) * __uint_as_float((uint32_t)(127 + e) << 23);
         }
       } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r) rs[r] = fabsf(a.c);
+        for (int r = 0; r < R; ++r) {
+          rs[r] = fabsf(a.c);
+#pragma unroll
+          for (int own = 0; own < kOwn; ++own)
+#pragma unroll
+            for (int k = 0; k < C::QW; ++k) qv[own][r][k] = a.c < 0.f ? -qv[own][r][k] : qv[own][r][k];
+        }
       }
       uint4* qf = reinterpret_cast<uint4*>(region);
 #pragma unroll
@@ -784,10 +790,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 
     for (int t = t0; t < t1; ++t) {
       if ((t * kAttnWarps + warp) * TK >= cur.len) break;
-      cp_wait<ST - 1>();
+      // this tile's copies, the newer one's still in flight if there is one
+      if (staged == 2) cp_wait<1>();
+      else cp_wait<0>();
       __syncwarp();
-      const uint32_t ks = ring + stage_out * C::kStage, vs = ks + C::kOffV;
-      const uint64_t ok = valid[warp][stage_out];
+      const uint32_t ks = ring + (used & 1) * C::kStage, vs = ks + C::kOffV;
+      const uint64_t ok = valid[warp][used & 1];
 
       // scores of the tile: lane (g, c) has keys 8 i + 2 c, + 1 of rows g (and g + 8)
       float s[NT][2 * R];
@@ -1109,9 +1117,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         }
       }
       __syncwarp();   // the stage is read
-      stage_out = stage_out + 1 == ST ? 0 : stage_out + 1;
-      issue();
+      ++used;
+      --staged;
+      if (has_tile()) issue();
     }
+
+    // ---- the next history of this CTA: its q is read while this one's sums are joined
+    Cursor next = cur;
+    int next_first = cur_first;
+    u += t1 - t0;
+    const bool more = u < u_hi;
+    if (more) next_history(next, next_first);
+    if (more) load_q(next);
 
     // ---- the warps' sums joined: weights of a lane group summed
     float2 (&ov)[OT][R] = o;
@@ -1196,7 +1213,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     };
     const long long out0 = (long long)cur.b * a.ldo + ((long long)jh * a.group + h0) * DH;
     const long long lse0 = (long long)cur.b * a.n_heads + (long long)jh * a.group + h0;
-    const bool whole = t0 == 0 && t1 == cur.nt;
+    const bool whole = t0 == 0 && t1 == nt;
     if (whole) {
       if (warp == 0) {
 #pragma unroll
@@ -1213,11 +1230,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       }
       __syncthreads();   // the region is read
     } else {
-      // the CTAs that hold this history: first .. lastc
-      const long long ub = cur_first + (long long)cur.jt * cur.nt;
-      const int first = (int)(((ub + 1) * G - 1) / units), lastc = (int)(((ub + cur.nt) * G - 1) / units);
-      const int pieces = lastc - first + 1;
-      auto slot_of = [&](int cta) { return a.slots + ((long long)cta * 2 + (cta == first)) * kAttnSlotFloats; };
+      // the CTAs that hold this history: first .. first + pieces - 1
+      const int ub = cur_first + cur.jt * nt, first = cta_of(ub), pieces = cta_of(ub + nt - 1) - first + 1;
+      auto slot_of = [&](int cta) { return a.slots + ((long long)cta * 2 + (cta == first)) * (HT * DH + 2 * HT); };
       if (warp == 0) {
         float* d = slot_of(blockIdx.x);
 #pragma unroll
@@ -1241,12 +1256,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         if (lane == 0) last_flag = atomicAdd(a.tickets + first, 1u) == (unsigned)pieces - 1;
       }
       __syncthreads();
-      if (last_flag) {   // this CTA adds the pieces up, in order
+      if (last_flag) {   // this CTA is the last of them: it adds the pieces up, in order
         __threadfence();
-        // HW heads to a warp, a lane for four columns (d_head 128; fewer lanes below): the pieces' weights first, a
-        // lane a piece, then the weighted sums, kFly pieces' loads in flight (an L2 read here takes 0.5 us or more,
-        // and one after another they were most of the time of a short call)
-        constexpr int HW = HT / kAttnWarps, kFly = HT == 8 ? 8 : 4;
+        // HW heads to a warp, a lane for four columns (d_head 128; fewer lanes below), kFly pieces' loads in flight (an
+        // L2 read here takes 0.5 us or more, and one after another they were most of the time of a short call)
+        constexpr int HW = HT / kAttnWarps, kFly = C::OCC == 3 ? 8 : 4;
         float mm[HW], ll[HW];
         float4 x[HW];
 #pragma unroll
@@ -1257,33 +1271,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         }
         const int col4 = min(lane, DH / 4 - 1);
         for (int p0 = 0; p0 < pieces; p0 += 32) {
-          // this lane's piece (a lane past the end repeats the last one with weight 0)
-          const bool on = p0 + lane < pieces;
-          const float* d = slot_of(first + min(p0 + lane, pieces - 1)) + HT * DH + warp;
+          const int k1 = min(32, pieces - p0);
+          // this lane's piece of 32 (a lane past the end repeats the last one with weight 0), and the first sums
+          const bool on = lane < k1;
+          const float* d = slot_of(first + p0 + min(lane, k1 - 1)) + HT * DH + warp;
           float mp[HW], f[HW];
 #pragma unroll
           for (int i = 0; i < HW; ++i) {
-            mp[i] = on ? __ldcg(d + i * kAttnWarps) : -INFINITY;
-            f[i] = on ? __ldcg(d + HT + i * kAttnWarps) : 0.f;
+            mp[i] = __ldcg(d + i * kAttnWarps);
+            f[i] = __ldcg(d + HT + i * kAttnWarps);
           }
-#pragma unroll
-          for (int i = 0; i < HW; ++i) {
-            float top = fmaxf(mm[i], mp[i]);
-#pragma unroll
-            for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            const float keep = mm[i] == -INFINITY ? 1.f : ex2(mm[i] - top);
-            const float wp = mp[i] == -INFINITY ? 1.f : ex2(mp[i] - top);
-            ll[i] = ll[i] * keep + f[i] * wp;
-            x[i].x *= keep;
-            x[i].y *= keep;
-            x[i].z *= keep;
-            x[i].w *= keep;
-            mm[i] = top;
-            f[i] = on ? wp : 0.f;
-          }
-          const int k1 = min(32, pieces - p0);
-          for (int k0 = 0; k0 < k1; k0 += kFly) {
-            float4 y[kFly][HW];
+          float4 y[kFly][HW];
+          auto read = [&](int k0) {
 #pragma unroll
             for (int k = 0; k < kFly; ++k) {
               const float4* src =
@@ -1291,6 +1290,26 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
               for (int i = 0; i < HW; ++i) y[k][i] = __ldcg(src + i * kAttnWarps * (DH / 4));
             }
+          };
+          read(0);
+#pragma unroll
+          for (int i = 0; i < HW; ++i) {
+            float top = fmaxf(mm[i], mp[i]);   // (a repeat changes no maximum)
+#pragma unroll
+            for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            // (a piece without a key, or with NaN scores only, has m -inf: its sums count as they are)
+            const float keep = mm[i] == -INFINITY ? 1.f : ex2(mm[i] - top);
+            const float wp = !on ? 0.f : mp[i] == -INFINITY ? 1.f : ex2(mp[i] - top);
+            ll[i] = ll[i] * keep + (on ? f[i] * wp : 0.f);
+            x[i].x *= keep;
+            x[i].y *= keep;
+            x[i].z *= keep;
+            x[i].w *= keep;
+            mm[i] = top;
+            f[i] = wp;
+          }
+#pragma unroll 1
+          for (int k0 = 0;;) {
 #pragma unroll
             for (int k = 0; k < kFly; ++k)
 #pragma unroll
@@ -1302,19 +1321,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
                 x[i].z += fk * y[k][i].z;
                 x[i].w += fk * y[k][i].w;
               }
+            k0 += kFly;
+            if (k0 >= k1) break;
+            read(k0);
           }
         }
 #pragma unroll
-        for (int i = 0; i < HW; ++i) {
-          const int h = warp + i * kAttnWarps;
+        for (int i = 0; i < HW; ++i)
 #pragma unroll
           for (int w = 16; w; w >>= 1) ll[i] += __shfl_xor_sync(0xffffffffu, ll[i], w);
+#pragma unroll
+        for (int i = 0; i < HW; ++i) {
+          const int h = warp + i * kAttnWarps;
           if (h >= heads) continue;
           if (lane < DH / 4) {
             const float inv = ll[i] == 0.f ? 0.f : 1.f / ll[i];
-            const long long at = out0 + (long long)h * DH + lane * 4;
             const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            store_rows<4>(a.out, a.row_type, a.out_vec, at, v, inv);
+            store_rows<4>(a.out, a.row_type, a.out_vec, out0 + (long long)h * DH + lane * 4, v, inv);
           }
           if (a.lse && lane == 0)
             a.lse[lse0 + h] = ll[i] == 0.f ? -INFINITY : (mm[i] - kLift + log2f(ll[i])) * 0.693147180559945f;
@@ -1323,10 +1346,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       }
       __syncthreads();   // the region and the flag are read
     }
-
-    u += t1 - t0;
-    cur.t = t1;
-    if (u < u_hi) next_history(cur, &cur_first);
+    if (!more) break;
+    cur = next;
+    cur_first = next_first;
   }
   cp_wait<0>();
 }
