@@ -92,7 +92,7 @@ def test_bad_attend(bad):
     dict(table_stride=2), dict(free_pages=None), dict(n_free=-1), dict(state=None), dict(page_size=0),
     dict(page_size=(1 << 20) + 1), dict(n_pages=0), dict(n_tokens=-1), dict(lens_out=None), dict(state_out=None),
     dict(cu_tokens=None), dict(slots=None), dict(positions=None), dict(requests=None),
-    dict(table_width=1 << 28, table_stride=1 << 28)], ids=str)
+    dict(table_width=1 << 28, table_stride=1 << 28), dict(lens_out=P + 4), dict(state_out=P - 8)], ids=str)
 def test_bad_plan(bad):
     from toy_b200._lib import lib
     assert lib().tb2_paged_plan(C.byref(plan_args(**bad)), None) == -1
@@ -101,7 +101,7 @@ def test_bad_plan(bad):
 @pytest.mark.parametrize("bad", [
     dict(n_req=0), dict(n_req=16385), dict(lens=None), dict(done=None), dict(table=None), dict(table_width=0),
     dict(table_stride=2), dict(free_pages=None), dict(n_free=-1), dict(state=None), dict(page_size=0),
-    dict(n_pages=0), dict(lens_out=None), dict(state_out=None)], ids=str)
+    dict(n_pages=0), dict(lens_out=None), dict(state_out=None), dict(lens_out=P - 4), dict(state_out=P + 12)], ids=str)
 def test_bad_release(bad):
     from toy_b200._lib import lib
     assert lib().tb2_paged_release(C.byref(release_args(**bad)), None) == -1

@@ -13,7 +13,7 @@
 //
 // The work is small (16 bytes written per token) and bound by latency: one
 // launch, in which every CTA computes the whole prefix sums for itself in
-// shared memory (n_req <= 16384; two loads per request) and fills its slice of
+// shared memory (n_req <= 16384; each length is read once) and fills its slice of
 // tokens and pages, instead of a scan, a barrier over the grid and a fill.
 // Lengths and the stack's count may be updated in place: a single CTA writes
 // them after its own reads; a larger grid leaves that to a second, tiny
@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kMaxReq = 16384;
 constexpr int kThreads = 1024;
+constexpr int kRun = 4;   // consecutive tokens of a thread
 
 // The totals of a scan: tokens and pages of every request, and whether any
 // input was bad (codes as the C API documents them).
@@ -40,25 +41,20 @@ struct Totals {
 __device__ __forceinline__ int div_up(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 
 // Exclusive prefix sums of two values per request into st[0 .. n] and
-// sp[0 .. n]; item(b, tok, pg) returns a status and the two values. Sums are
-// 64 bits wide and stored cut to 32; totals that do not fit are reported by
-// the caller's own limits before the stored values are used.
-template <class F>
-__device__ Totals scan_requests(int n, int* st, int* sp, F&& item) {
+// sp[0 .. n]: the caller has put the values themselves there and synchronised.
+// Sums are 64 bits wide and stored cut to 32; totals that do not fit are
+// reported by the caller's own limits before the stored values are used. `bad`
+// is this thread's; the result's is the CTA's largest.
+__device__ Totals scan_requests(int n, int* st, int* sp, int bad) {
   __shared__ long long wt[32], wp[32];
-  __shared__ int sbad;
+  __shared__ int wb[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  if (tid == 0) sbad = 0;
-  __syncthreads();
   const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
   const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
   long long ts = 0, ps = 0;
-  int bad = 0;
   for (int b = b0; b < b1; ++b) {
-    int tok = 0, pg = 0;
-    bad = max(bad, item(b, tok, pg));
-    ts += tok;
-    ps += pg;
+    ts += st[b];
+    ps += sp[b];
   }
   long long ti = ts, pi = ps;
 #pragma unroll
@@ -69,26 +65,31 @@ __device__ Totals scan_requests(int n, int* st, int* sp, F&& item) {
       pi += c;
     }
   }
+  bad = __reduce_max_sync(0xffffffffu, bad);
   if (lane == 31) {
     wt[warp] = ti;
     wp[warp] = pi;
+    wb[warp] = bad;
   }
-  if (bad) atomicMax(&sbad, bad);
   __syncthreads();
-  long long bt = 0, bp = 0, tt = 0, tp = 0;
-  for (int w = 0; w < nw; ++w) {
-    if (w < warp) {
-      bt += wt[w];
-      bp += wp[w];
+  // the warps' totals, scanned by every warp for itself
+  long long at = lane < nw ? wt[lane] : 0, ap = lane < nw ? wp[lane] : 0;
+  bad = __reduce_max_sync(0xffffffffu, lane < nw ? wb[lane] : 0);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, at, o), c = __shfl_up_sync(0xffffffffu, ap, o);
+    if (lane >= o) {
+      at += a;
+      ap += c;
     }
-    tt += wt[w];
-    tp += wp[w];
   }
+  const long long tt = __shfl_sync(0xffffffffu, at, 31), tp = __shfl_sync(0xffffffffu, ap, 31);
+  long long bt = __shfl_sync(0xffffffffu, at, max(0, warp - 1)), bp = __shfl_sync(0xffffffffu, ap, max(0, warp - 1));
+  if (warp == 0) bt = bp = 0;
   bt += ti - ts;
   bp += pi - ps;
   for (int b = b0; b < b1; ++b) {
-    int tok = 0, pg = 0;
-    item(b, tok, pg);
+    const int tok = st[b], pg = sp[b];
     st[b] = (int)bt;
     sp[b] = (int)bp;
     bt += tok;
@@ -99,7 +100,7 @@ __device__ Totals scan_requests(int n, int* st, int* sp, F&& item) {
     sp[n] = (int)tp;
   }
   __syncthreads();
-  return {tt, tp, sbad};
+  return {tt, tp, bad};
 }
 
 // The request b with cu[b] <= i < cu[b + 1].
@@ -113,22 +114,54 @@ __device__ __forceinline__ int find_request(const int* cu, int n, int i) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kThreads) paged_plan_kernel(const tb2_paged_plan_args a, int* err) {
+// Four values from element i on, one 16-byte store where the address allows it.
+__device__ __forceinline__ void store4(int* p, int i, int n, const int (&v)[kRun]) {
+  if (i + kRun <= n && (reinterpret_cast<uintptr_t>(p + i) & 15) == 0) {
+    *reinterpret_cast<int4*>(p + i) = make_int4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRun; ++k)
+      if (i + k < n) p[i + k] = v[k];
+  }
+}
+__device__ __forceinline__ void store4(long long* p, int i, int n, const long long (&v)[kRun]) {
+  if (i + kRun <= n && (reinterpret_cast<uintptr_t>(p + i) & 15) == 0) {
+    *reinterpret_cast<longlong2*>(p + i) = make_longlong2(v[0], v[1]);
+    *reinterpret_cast<longlong2*>(p + i + 2) = make_longlong2(v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRun; ++k)
+      if (i + k < n) p[i + k] = v[k];
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) paged_plan_kernel(const tb2_paged_plan_args a, int in_place, int* err) {
   extern __shared__ int sm[];
-  int* cu_tok = sm;
-  int* cu_pg = sm + a.n_req + 1;
-  griddep_wait_release();
   const int P = a.page_size, n = a.n_req;
+  int* cu_tok = sm;
+  int* cu_pg = sm + n + 1;
+  int* held = cu_pg + n + 1;   // the lengths
+  griddep_wait_release();
   const int count = a.state[0];
-  const Totals tot = scan_requests(n, cu_tok, cu_pg, [&](int b, int& tok, int& pg) {
+  int bad = 0;
+  for (int b = threadIdx.x; b < n; b += blockDim.x) {
     const int len = a.lens[b], add = a.add[b];
-    if (len < 0 || add < 0) return 4;
     const long long end = (long long)len + add;
-    if ((end + P - 1) / P > a.table_width) return 2;
-    tok = add;
-    pg = div_up((int)end, P) - div_up(len, P);
-    return 0;
-  });
+    int tok = 0, pg = 0;
+    if (len < 0 || add < 0) {
+      bad = 4;
+    } else if (end > (long long)a.table_width * P) {
+      bad = max(bad, 2);
+    } else {
+      tok = add;
+      pg = div_up((int)end, P) - div_up(len, P);
+    }
+    cu_tok[b] = tok;
+    cu_pg[b] = pg;
+    held[b] = len;
+  }
+  __syncthreads();
+  const Totals tot = scan_requests(n, cu_tok, cu_pg, bad);
   int status = tot.bad;
   if (count < 0 || count > a.n_free) status = 4;
   else if (!status && tot.tokens > a.n_tokens) status = 3;
@@ -136,41 +169,56 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const tb2_paged_pl
   const int tokens = status ? 0 : (int)tot.tokens, pages = status ? 0 : (int)tot.pages;
   const int step = gridDim.x * blockDim.x, first = blockIdx.x * blockDim.x + threadIdx.x;
   for (int i = first; i < pages; i += step) {
-    const int b = find_request(cu_pg, n, i);
-    a.table[b * a.table_stride + div_up(a.lens[b], P) + (i - cu_pg[b])] = a.free_pages[count - 1 - i];
+    const int page = a.free_pages[count - 1 - i], b = find_request(cu_pg, n, i);
+    a.table[b * a.table_stride + div_up(held[b], P) + (i - cu_pg[b])] = page;
   }
-  for (int t = first; t < a.n_tokens; t += step) {
-    long long slot = -1;
-    int pos = 0, req = -1;
-    if (t < tokens) {
-      req = find_request(cu_tok, n, t);
-      const int len = a.lens[req], held = div_up(len, P);
-      pos = len + (t - cu_tok[req]);
-      const int blk = pos / P;
-      const int page =
-          blk < held ? a.table[req * a.table_stride + blk] : a.free_pages[count - 1 - (cu_pg[req] + blk - held)];
-      if (page >= 0 && page < a.n_pages) slot = (long long)page * P + (pos - blk * P);
+  for (long long t0 = (long long)first * kRun; t0 < a.n_tokens; t0 += (long long)step * kRun) {
+    long long slot[kRun];
+    int pos[kRun], req[kRun];
+    int b = t0 < tokens ? find_request(cu_tok, n, (int)t0) : -1, blk = -1, page = 0;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      slot[k] = req[k] = -1;
+      pos[k] = 0;
+      const int t = (int)t0 + k;
+      if (t >= tokens) continue;
+      while (t >= cu_tok[b + 1]) {   // the next request with a token
+        ++b;
+        blk = -1;
+      }
+      req[k] = b;
+      pos[k] = held[b] + (t - cu_tok[b]);
+      const int at = pos[k] / P;
+      if (at != blk) {
+        blk = at;
+        const int old = div_up(held[b], P);
+        page = at < old ? a.table[b * a.table_stride + at] : a.free_pages[count - 1 - (cu_pg[b] + at - old)];
+      }
+      if (page >= 0 && page < a.n_pages) slot[k] = (long long)page * P + (pos[k] - at * P);
       else *err = kErrPagedPage;
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
-    a.requests[t] = req;
+    store4(a.slots, (int)t0, a.n_tokens, slot);
+    store4(a.positions, (int)t0, a.n_tokens, pos);
+    store4(a.requests, (int)t0, a.n_tokens, req);
   }
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b <= n; b += blockDim.x) a.cu_tokens[b] = status ? 0 : cu_tok[b];
+  // lengths and count: by this kernel unless another CTA may still have to read what they overwrite
   const bool alone = gridDim.x == 1;
-  if (alone) __syncthreads();   // every read of lens and state is done
-  if (alone)
-    for (int b = threadIdx.x; b < n; b += blockDim.x) a.lens_out[b] = a.lens[b] + (status ? 0 : a.add[b]);
+  if (alone) __syncthreads();
+  if (blockIdx.x == 0 && (alone || !in_place)) {
+    for (int b = threadIdx.x; b < n; b += blockDim.x)
+      a.lens_out[b] = status ? held[b] : held[b] + (cu_tok[b + 1] - cu_tok[b]);
+    if (threadIdx.x == 0) a.state_out[0] = count - pages;
+  }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.state_out[1] = status;
     a.state_out[2] = tokens;
     a.state_out[3] = pages;
-    if (alone) a.state_out[0] = count - pages;
   }
 }
 
-// After a plan on more than one CTA: the lengths and the stack's count.
+// After a plan in place on more than one CTA: the lengths and the stack's count.
 __global__ void paged_plan_commit_kernel(const tb2_paged_plan_args a) {
   griddep_wait_release();
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
@@ -178,20 +226,23 @@ __global__ void paged_plan_commit_kernel(const tb2_paged_plan_args a) {
   if (b == 0) a.state_out[0] = a.state[0] - a.state_out[3];
 }
 
-__global__ void __launch_bounds__(kThreads) paged_release_kernel(const tb2_paged_release_args a, int* err) {
+__global__ void __launch_bounds__(kThreads) paged_release_kernel(const tb2_paged_release_args a, int in_place, int* err) {
   extern __shared__ int sm[];
-  int* cu_pg = sm;
-  int* unused = sm + a.n_req + 1;
-  griddep_wait_release();
   const int P = a.page_size, n = a.n_req;
+  int* gone = sm;   // requests that are done, counted like tokens
+  int* cu_pg = sm + n + 1;
+  griddep_wait_release();
   const int count = a.state[0];
-  const Totals tot = scan_requests(n, unused, cu_pg, [&](int b, int& tok, int& pg) {
+  int bad = 0;
+  for (int b = threadIdx.x; b < n; b += blockDim.x) {
     const int len = a.lens[b];
-    if (len < 0 || ((long long)len + P - 1) / P > a.table_width) return 4;
-    pg = a.done[b] ? div_up(len, P) : 0;
-    tok = 0;
-    return 0;
-  });
+    const bool fits = len >= 0 && len <= (long long)a.table_width * P, done = a.done[b] != 0;
+    if (!fits) bad = 4;
+    gone[b] = fits && done;
+    cu_pg[b] = fits && done ? div_up(len, P) : 0;
+  }
+  __syncthreads();
+  const Totals tot = scan_requests(n, gone, cu_pg, bad);
   int status = tot.bad;
   if (count < 0 || count > a.n_free) status = 4;
   else if (!status && tot.pages > a.n_free - count) status = 1;
@@ -206,15 +257,15 @@ __global__ void __launch_bounds__(kThreads) paged_release_kernel(const tb2_paged
     *e = -1;
   }
   const bool alone = gridDim.x == 1;
-  if (alone) {
-    __syncthreads();
-    for (int b = threadIdx.x; b < n; b += blockDim.x) a.lens_out[b] = !status && a.done[b] ? 0 : a.lens[b];
+  if (blockIdx.x == 0 && (alone || !in_place)) {
+    // (a length is read and written by one thread, and read by no other CTA after the first barrier of this one)
+    for (int b = threadIdx.x; b < n; b += blockDim.x) a.lens_out[b] = !status && gone[b + 1] > gone[b] ? 0 : a.lens[b];
+    if (threadIdx.x == 0) a.state_out[0] = count + pages;
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.state_out[1] = status;
     a.state_out[2] = 0;
     a.state_out[3] = pages;
-    if (alone) a.state_out[0] = count + pages;
   }
 }
 
@@ -226,7 +277,7 @@ __global__ void paged_release_commit_kernel(const tb2_paged_release_args a) {
 }
 
 int smem_setup(int) {
-  const int bytes = 2 * (kMaxReq + 1) * (int)sizeof(int);
+  const int bytes = 3 * (kMaxReq + 1) * (int)sizeof(int);
   if (cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return -3;
   return cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
@@ -234,21 +285,26 @@ int smem_setup(int) {
              : -3;
 }
 
-// CTAs for `items` tokens and pages: four a thread before another CTA pays
-// for its own prefix sums.
-int grid_for(long long items) {
-  return (int)std::max<long long>(1, std::min<long long>(148, items / (4 * kThreads)));
-}
+// CTAs for `items` threads' worth of work: a full CTA before another one pays
+// for its own prefix sums; one CTA of fewer threads (cheaper barriers) where
+// requests and work are few.
+int grid_for(long long items) { return (int)std::max<long long>(1, std::min<long long>(148, items / kThreads)); }
+int threads_for(int n_req, long long items) { return n_req <= 256 && items <= 512 ? 256 : kThreads; }
+
+// n ints that are updated: in place (1), elsewhere (0), or in part over themselves (-1).
+int placed(const int* x, const int* y, long long n) { return x == y ? 1 : x < y + n && y < x + n ? -1 : 0; }
 
 }  // namespace
 
 int paged_plan_launch(const tb2_paged_plan_args& a, int* err, cudaStream_t st) {
   static DeviceOnce setup;
   if (setup.ensure(smem_setup)) return -3;
-  const size_t smem = 2 * (size_t)(a.n_req + 1) * sizeof(int);
-  const int grid = grid_for(a.n_tokens);
-  if (launch_pdl(paged_plan_kernel, dim3(grid), dim3(kThreads), smem, st, a, err)) return -3;
-  if (grid == 1) return 0;
+  const size_t smem = 3 * (size_t)(a.n_req + 1) * sizeof(int);
+  const long long items = ((long long)a.n_tokens + kRun - 1) / kRun;
+  const int grid = grid_for(items);
+  const int in_place = placed(a.lens, a.lens_out, a.n_req) || placed(a.state, a.state_out, 4);
+  if (launch_pdl(paged_plan_kernel, dim3(grid), dim3(threads_for(a.n_req, items)), smem, st, a, in_place, err)) return -3;
+  if (grid == 1 || !in_place) return 0;
   return launch_pdl(paged_plan_commit_kernel, dim3((a.n_req + 255) / 256), dim3(256), 0, st, a);
 }
 
@@ -256,9 +312,12 @@ int paged_release_launch(const tb2_paged_release_args& a, int* err, cudaStream_t
   static DeviceOnce setup;
   if (setup.ensure(smem_setup)) return -3;
   const size_t smem = 2 * (size_t)(a.n_req + 1) * sizeof(int);
-  const int grid = grid_for((long long)a.n_req * a.table_width);
-  if (launch_pdl(paged_release_kernel, dim3(grid), dim3(kThreads), smem, st, a, err)) return -3;
-  if (grid == 1) return 0;
+  const long long items = (long long)a.n_req * a.table_width;   // (at most: the lengths are on the device)
+  const int grid = grid_for(items / 4);
+  const int in_place = placed(a.lens, a.lens_out, a.n_req) || placed(a.state, a.state_out, 4);
+  if (launch_pdl(paged_release_kernel, dim3(grid), dim3(threads_for(a.n_req, items)), smem, st, a, in_place, err))
+    return -3;
+  if (grid == 1 || !in_place) return 0;
   return launch_pdl(paged_release_commit_kernel, dim3((a.n_req + 255) / 256), dim3(256), 0, st, a);
 }
 
@@ -273,6 +332,7 @@ int tb2_paged_plan(const tb2_paged_plan_args* a, void* stream) {
   if (!a->lens || !a->add || !a->table || !a->state || !a->lens_out || !a->state_out || !a->cu_tokens ||
       (a->n_free && !a->free_pages) || (a->n_tokens && (!a->slots || !a->positions || !a->requests)))
     return -1;
+  if (tb2::placed(a->lens, a->lens_out, a->n_req) < 0 || tb2::placed(a->state, a->state_out, 4) < 0) return -1;
   if ((long long)a->table_width * a->page_size > 0x7fffff00LL) return -1;   // positions are 32 bits wide
   int* err = tb2::device_error_word();
   if (!err) return -3;
@@ -286,6 +346,7 @@ int tb2_paged_release(const tb2_paged_release_args* a, void* stream) {
   if (!a->lens || !a->done || !a->table || !a->state || !a->lens_out || !a->state_out ||
       (a->n_free && !a->free_pages))
     return -1;
+  if (tb2::placed(a->lens, a->lens_out, a->n_req) < 0 || tb2::placed(a->state, a->state_out, 4) < 0) return -1;
   if ((long long)a->table_width * a->page_size > 0x7fffff00LL) return -1;
   int* err = tb2::device_error_word();
   if (!err) return -3;

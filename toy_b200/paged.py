@@ -130,14 +130,14 @@ def plan(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages:
     if dev < 0 or n < 1 or not 0 <= n_tokens < 2**31:
         _bad("lens: on a GPU, of one request or more; n_tokens not negative")
     tp, width, stride = _table(table, n, dev)
-    if out is None:   # two allocations, each part on a 16-byte boundary
-        n4, t4 = (n + 4) & ~3, (n_tokens + 3) & ~3
-        part = lens.new_empty(2 * n4 + 4 + 2 * t4, dtype=_I32)
-        cu = n4 + 4
-        out = Plan(part[:n], part[n4:cu], part[cu:cu + n + 1], lens.new_empty(n_tokens, dtype=_I64),
-                   part[cu + n4:cu + n4 + n_tokens], part[cu + n4 + t4:cu + n4 + t4 + n_tokens])
-        lp = part.data_ptr()
-        outs = (lp, lp + 4 * n4, lp + 4 * cu, out.slots.data_ptr(), lp + 4 * (cu + n4), lp + 4 * (cu + n4 + t4))
+    if out is None:   # two allocations, as each call into torch is a microsecond or more
+        slots = lens.new_empty(n_tokens, dtype=_I64)
+        part = lens.new_empty(2 * n_tokens + 2 * n + 5, dtype=_I32)
+        positions, requests, st, new_lens, cu = part.split((n_tokens, n_tokens, 4, n, n + 1))
+        out = Plan(new_lens, st, cu, slots, positions, requests)
+        p = part.data_ptr()
+        outs = (p + 4 * (2 * n_tokens + 4), p + 8 * n_tokens, p + 4 * (2 * n_tokens + 4 + n), slots.data_ptr(), p,
+                p + 4 * n_tokens)
     else:
         outs = (_ints(out.lens, n, dev, "out.lens"), _ints(out.state, 4, dev, "out.state"),
                 _ints(out.cu_tokens, n + 1, dev, "out.cu_tokens"), _ints(out.slots, n_tokens, dev, "out.slots", _I64),
