@@ -772,6 +772,27 @@ int tb2_kv_run(void *sess, int steps, float *ms);
 int tb2_kv_launches(void *sess);
 int tb2_kv_free(void *sess);
 
+/* The same step over a paged cache: n_seq (1-8 or 16) sequences of unlike
+ * lengths (each at most max_T tokens) that share n_pages pages of page_size
+ * tokens, K and V in kv_type 0 f32, 1 f16, 30 bf16 or 8 Q8_0. Pages are taken
+ * on the GPU as a sequence grows and shared by every layer's pools. No
+ * counterpart in the reference, whose sequences decode in lockstep. One decode
+ * engine per session: tb2_kv_free before the other kind; tb2_kv_reset empties
+ * every sequence; tb2_kv_logits and tb2_kv_launches as above. Returns 0, -1,
+ * -2 or -3 as tb2_kv_realize. */
+int tb2_kv_realize_paged(void *sess, int max_T, int n_seq, int kv_type, int page_size, int n_pages);
+/* One step: tokens[b] >= 0 is appended to sequence b at its next position and
+ * the logits of the token after it computed; -1 leaves sequence b as it is
+ * (its row of the logits means nothing). The first call captures the step as a
+ * CUDA graph. Returns 0; -1 for a token out of range, a sequence that already
+ * holds max_T tokens, or no token at all; -2 without a paged cache; -5 when
+ * the pool has too few free pages for the step, which then changed nothing. */
+int tb2_kv_decode_paged(void *sess, const long long *tokens, int n_seq, float *logits);
+/* Sequences with done[b] != 0 are emptied and their pages given back. */
+int tb2_kv_release(void *sess, const int *done, int n_seq);
+/* The sequences' lengths and the number of free pages. */
+int tb2_kv_paged_state(void *sess, int *lens, int n_seq, int *free_pages);
+
 /* ===================================================================== */
 /* GGUF files (tinynn/tinynn_gguf.h; writer tinynn/tinynn_ggml.h:538-545) */
 /* ===================================================================== */

@@ -299,6 +299,10 @@ _SIGS = [
     ("tb2_kv_run", I, [VP, I, C.POINTER(C.c_float)]),
     ("tb2_kv_launches", I, [VP]),
     ("tb2_kv_free", I, [VP]),
+    ("tb2_kv_realize_paged", I, [VP, I, I, I, I, I]),
+    ("tb2_kv_decode_paged", I, [VP, C.POINTER(C.c_longlong), I, C.POINTER(C.c_float)]),
+    ("tb2_kv_release", I, [VP, C.POINTER(C.c_int), I]),
+    ("tb2_kv_paged_state", I, [VP, C.POINTER(C.c_int), I, C.POINTER(C.c_int)]),
     ("tb2_llama_save_gguf", I, [VP, C.c_char_p, I]),
 ]
 

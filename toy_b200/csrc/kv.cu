@@ -21,6 +21,14 @@
 // residual add; then the final norm folded into the LM-head GEMV. The whole
 // step is one CUDA graph; tokens and positions are copied in before it.
 //
+// With a paged cache (PagedState) the sequences are ragged: pages come from a
+// pool shared by all of them, taken on the GPU by the step's plan as sequences
+// grow and given back when they are released; a sequence without a token in a
+// step stays as it is. K and V may be f32, f16, bf16 or Q8_0, and append and
+// attention are the paged operators (paged_append.cu, paged_attn.cuh): the
+// history of every sequence is read once per key head, split over the GPU by
+// length, and the o GEMV reads the joined result.
+//
 // The weights are the realised training engine's (same session): decoding
 // after training, or after tb2_llama_load_gguf, uses them in place. Adapters
 // are not applied on this path.
@@ -32,6 +40,7 @@
 #include <memory>
 #include <vector>
 
+#include "paged.cuh"
 #include "pdl.cuh"
 #include "runtime.cuh"
 #include "session.cuh"
@@ -558,7 +567,36 @@ __global__ void __launch_bounds__(kChunk) kv_attn_kernel(const AttnArgs a) {
   }
 }
 
+// A step's slots and positions by sequence (the plan numbers only the sequences
+// that append): sequence b's token is number cu[b] when it has one.
+__global__ void kv_rows_kernel(const int* __restrict__ add, const int* __restrict__ cu,
+                               const long long* __restrict__ slots, const int* __restrict__ positions, int n,
+                               long long* __restrict__ row_slot, int* __restrict__ row_pos) {
+  griddep_wait_release();
+  const int b = threadIdx.x;
+  if (b >= n) return;
+  // (a plan that found no room has every cu 0 and every slot -1)
+  row_slot[b] = add[b] ? slots[cu[b]] : -1;
+  row_pos[b] = add[b] ? positions[cu[b]] : 0;
+}
+
 }  // namespace
+
+// The paged cache of a decode engine: pools [layers][pages][KV][page_size][dh]
+// of K and of V, the sequences' block tables and lengths, the stack of free
+// pages, and the arrays a step's plan fills (tb2_paged_plan).
+struct PagedState {
+  int page_size = 0, n_pages = 0, width = 0, type = 0;
+  uint8_t *k = nullptr, *v = nullptr;
+  uint16_t *ks = nullptr, *vs = nullptr;
+  int *lens = nullptr, *add = nullptr, *table = nullptr, *free_pages = nullptr, *state = nullptr, *cu = nullptr,
+      *positions = nullptr, *requests = nullptr, *row_pos = nullptr, *done = nullptr;
+  long long *slots = nullptr, *row_slot = nullptr;
+  float* att = nullptr;          // attention output [n_seq][H dh]
+  void* workspace = nullptr;
+  int* err = nullptr;
+  std::vector<int> host_len;     // the lengths, as the host has followed them
+};
 
 // ---------------------------------------------------------------- the decode engine
 // adapter parameter names by target, in the training engine's order (q, k, v, o, gate, up, down)
@@ -567,6 +605,14 @@ const char* const kAdName[7] = {"attn_q", "attn_k", "attn_v", "attn_output", "ff
 class KvEngine {
  public:
   KvEngine(LlamaEngine& e, int max_T, int n_seq, int kv_type) : e_(e), max_T_(max_T), nb_(n_seq), q8_(kv_type == 8) {}
+  KvEngine(LlamaEngine& e, int max_T, int n_seq, int kv_type, int page_size, int n_pages)
+      : e_(e), max_T_(max_T), nb_(n_seq), q8_(false), pg_(std::make_unique<PagedState>()) {
+    pg_->type = kv_type;
+    pg_->page_size = page_size;
+    pg_->n_pages = n_pages;
+    pg_->width = (int)(((long long)max_T + page_size - 1) / page_size);
+  }
+  bool paged() const { return pg_ != nullptr; }
   ~KvEngine() {
     cudaSetDevice(e_.device());
     if (graph_) cudaGraphExecDestroy(graph_);
@@ -580,7 +626,7 @@ class KvEngine {
     if (max_T_ < 1 || max_T_ > e_.rope_rows() || nb_ < 1 || (nb_ > 8 && nb_ != kMaxSeq)) return -1;
     if (c.d_head % 32 || c.d_head > 128 || c.d_model % 16 || c.d_ff % 16) return -1;
     if (c.qk_norm || c.n_experts) return -1;   // QK-RMSNorm and expert blocks: training-step only
-    const long long nsplit = (max_T_ + kChunk - 1) / kChunk;
+    const long long nsplit = pg_ ? 0 : (max_T_ + kChunk - 1) / kChunk;   // (partials of the contiguous cache's attention)
     const long long max_k = std::max(c.d_ff, std::max(c.d_model, c.n_heads * c.d_head));
     if (((long long)nb_ * max_k + (long long)nb_ * c.n_heads * nsplit + max_k) * 4 > 200 * 1024)
       return -1;
@@ -588,7 +634,7 @@ class KvEngine {
     if (cudaStreamCreateWithFlags(&st_, cudaStreamNonBlocking) != cudaSuccess) return -3;
     const int d = c.d_model, H = c.n_heads, KV = c.n_kv, dh = c.d_head, ff = c.d_ff, V = c.vocab, L = c.n_layers;
     const int W = (H + 2 * KV) * dh;
-    nsplit_ = (max_T_ + kChunk - 1) / kChunk;
+    nsplit_ = (int)nsplit;
     attn_smem_ = q8_ ? (size_t)kChunk * dh + (size_t)kChunk * (dh / 32) * 2 : (size_t)kChunk * dh * 4;
     static DeviceOnce attn_setup;   // the largest chunk any engine stages: f32 rows of d_head 128
     if (attn_setup.ensure([](int) {
@@ -615,7 +661,9 @@ class KvEngine {
     tok_ = io;
     pos_ = io + kMaxSeq;
     const long long cache = (long long)L * nb_ * KV * max_T_ * dh;
-    if (q8_) {
+    if (pg_) {
+      if (int rc = realize_paged(L, KV, dh, H)) return rc;
+    } else if (q8_) {
       void* p = nullptr;
       for (int w = 0; w < 2; ++w) {
         if (cudaMalloc(&p, (size_t)cache) != cudaSuccess) return -3;
@@ -660,6 +708,7 @@ class KvEngine {
   int reset() {
     cudaSetDevice(e_.device());
     const LlamaConfig& c = e_.cfg();
+    if (pg_) return reset_paged();
     const long long cache = (long long)c.n_layers * nb_ * c.n_kv * max_T_ * c.d_head;
     if (q8_) {
       if (cudaMemsetAsync(kq_, 0, cache, st_) || cudaMemsetAsync(vq_, 0, cache, st_)) return -3;
@@ -685,16 +734,7 @@ class KvEngine {
       return -3;
     if (!graph_) {   // first step: eager (validates every launch), then captured for replay
       if (int rc = enqueue()) return rc;
-      cudaGraph_t g = nullptr;
-      if (cudaStreamBeginCapture(st_, cudaStreamCaptureModeThreadLocal) != cudaSuccess) return -3;
-      const int rc = enqueue();
-      if (cudaStreamEndCapture(st_, &g) != cudaSuccess || rc) {
-        if (g) cudaGraphDestroy(g);
-        return rc ? rc : -3;
-      }
-      const cudaError_t ce = cudaGraphInstantiate(&graph_, g, 0);
-      cudaGraphDestroy(g);
-      if (ce != cudaSuccess) return -3;
+      if (int rc = capture()) return rc;
     } else if (cudaGraphLaunch(graph_, st_) != cudaSuccess) {
       return -3;
     }
@@ -705,8 +745,67 @@ class KvEngine {
     return cudaStreamSynchronize(st_) == cudaSuccess ? 0 : -3;
   }
 
+  // One step over the paged cache: token[b] >= 0 is appended to sequence b and its logits computed, -1 leaves b alone.
+  int decode_paged(const long long* tokens, int n, float* logits_host) {
+    const LlamaConfig& c = e_.cfg();
+    if (!tokens || n != nb_) return -1;
+    int total = 0;
+    for (int b = 0; b < nb_; ++b) {
+      if (tokens[b] < -1 || tokens[b] >= c.vocab || (tokens[b] >= 0 && pg_->host_len[b] >= max_T_)) return -1;
+      total += tokens[b] >= 0;
+    }
+    if (!total) return -1;
+    if (cudaSetDevice(e_.device()) != cudaSuccess) return -3;
+    if (cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    if (e_.sync()) return -3;   // weights written by training steps are final
+    for (int b = 0; b < nb_; ++b) {
+      host_in_[b] = tokens[b] >= 0 ? (int)tokens[b] : 0;
+      host_in_[kMaxSeq + b] = tokens[b] >= 0;
+    }
+    if (cudaMemcpyAsync(tok_, host_in_, nb_ * sizeof(int), cudaMemcpyHostToDevice, st_) != cudaSuccess ||
+        cudaMemcpyAsync(pg_->add, host_in_ + kMaxSeq, nb_ * sizeof(int), cudaMemcpyHostToDevice, st_) != cudaSuccess)
+      return -3;
+    if (!graph_) {   // first step: eager (validates every launch), then captured for replay
+      if (int rc = enqueue()) return rc;
+      if (int rc = capture()) return rc;
+    } else if (cudaGraphLaunch(graph_, st_) != cudaSuccess) {
+      return -3;
+    }
+    if (logits_host && cudaMemcpyAsync(logits_host, logits_, (size_t)nb_ * c.vocab * 4, cudaMemcpyDeviceToHost, st_) !=
+                           cudaSuccess)
+      return -3;
+    int state[4] = {0, 0, 0, 0};
+    if (cudaMemcpyAsync(state, pg_->state, sizeof state, cudaMemcpyDeviceToHost, st_) != cudaSuccess) return -3;
+    if (cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    if (state[1]) return state[1] == 1 ? -5 : -3;   // no room: the plan, and so the step, changed nothing
+    for (int b = 0; b < nb_; ++b) pg_->host_len[b] += tokens[b] >= 0;
+    return 0;
+  }
+
+  int release(const int* done, int n) {
+    if (!done || n != nb_) return -1;
+    if (cudaSetDevice(e_.device()) != cudaSuccess || cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    for (int b = 0; b < nb_; ++b) host_in_[b] = done[b] != 0;
+    if (cudaMemcpyAsync(pg_->done, host_in_, nb_ * sizeof(int), cudaMemcpyHostToDevice, st_) != cudaSuccess) return -3;
+    const tb2_paged_release_args a = {pg_->lens,       pg_->done,   nb_,        pg_->table, pg_->width,
+                                      pg_->width,      pg_->free_pages, pg_->n_pages, pg_->state, pg_->page_size,
+                                      pg_->n_pages,    pg_->lens,   pg_->state};
+    if (int rc = paged_release_launch(a, pg_->err, st_)) return rc;
+    if (cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    for (int b = 0; b < nb_; ++b)
+      if (done[b]) pg_->host_len[b] = 0;
+    return 0;
+  }
+
+  int paged_state(int* lens, int n, int* free_pages) {
+    if (!lens || !free_pages || n != nb_) return -1;
+    if (cudaSetDevice(e_.device()) != cudaSuccess || cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    if (cudaMemcpy(lens, pg_->lens, nb_ * sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -3;
+    return cudaMemcpy(free_pages, pg_->state, sizeof(int), cudaMemcpyDeviceToHost) == cudaSuccess ? 0 : -3;
+  }
+
   int run(int steps, float* ms) {   // n graph replays at the positions last copied in, timed by events
-    if (!graph_ || steps < 1 || !ms) return -2;
+    if (!graph_ || steps < 1 || !ms || pg_) return -2;   // (a replay over a paged cache appends)
     cudaEvent_t a, b;
     if (cudaEventCreate(&a) || cudaEventCreate(&b)) return -3;
     cudaEventRecord(a, st_);
@@ -730,6 +829,100 @@ class KvEngine {
   int launches() const { return launches_; }
 
  private:
+  // The step's launches as a graph, for replay.
+  int capture() {
+    cudaGraph_t g = nullptr;
+    if (cudaStreamBeginCapture(st_, cudaStreamCaptureModeThreadLocal) != cudaSuccess) return -3;
+    const int rc = enqueue();
+    if (cudaStreamEndCapture(st_, &g) != cudaSuccess || rc) {
+      if (g) cudaGraphDestroy(g);
+      return rc ? rc : -3;
+    }
+    const cudaError_t ce = cudaGraphInstantiate(&graph_, g, 0);
+    cudaGraphDestroy(g);
+    return ce == cudaSuccess ? 0 : -3;
+  }
+
+  int realize_paged(int L, int KV, int dh, int H) {
+    PagedState& p = *pg_;
+    auto get = [&](auto*& to, size_t bytes) {
+      void* m = nullptr;
+      if (cudaMalloc(&m, std::max<size_t>(bytes, 16)) != cudaSuccess) return false;
+      bufs_.push_back(m);
+      to = static_cast<std::remove_reference_t<decltype(to)>>(m);
+      return cudaMemset(m, 0, std::max<size_t>(bytes, 16)) == cudaSuccess;
+    };
+    const size_t rows = (size_t)L * p.n_pages * KV * p.page_size, ws = tb2_paged_attend_workspace();
+    if (!get(p.k, rows * dh * type_bytes(p.type)) || !get(p.v, rows * dh * type_bytes(p.type))) return -3;
+    if (p.type == kTypeQ8_0 && (!get(p.ks, rows * (dh / 32) * 2) || !get(p.vs, rows * (dh / 32) * 2))) return -3;
+    const size_t i4 = sizeof(int);
+    uint8_t* work = nullptr;
+    if (!get(p.lens, nb_ * i4) || !get(p.add, nb_ * i4) || !get(p.table, (size_t)nb_ * p.width * i4) ||
+        !get(p.free_pages, p.n_pages * i4) || !get(p.state, 4 * i4) || !get(p.cu, (nb_ + 1) * i4) ||
+        !get(p.positions, nb_ * i4) || !get(p.requests, nb_ * i4) || !get(p.row_pos, nb_ * i4) ||
+        !get(p.done, nb_ * i4) || !get(p.slots, nb_ * 8) || !get(p.row_slot, nb_ * 8) ||
+        !get(p.att, (size_t)nb_ * H * dh * 4) || !get(work, ws))
+      return -3;
+    p.workspace = work;   // (zeroed, as tb2_paged_attend_workspace_init leaves it)
+    p.err = device_error_word();
+    if (!p.err) return -3;
+    return reset_paged();
+  }
+
+  int reset_paged() {
+    PagedState& p = *pg_;
+    p.host_len.assign(nb_, 0);
+    std::vector<int> ids(p.n_pages);
+    for (int i = 0; i < p.n_pages; ++i) ids[i] = p.n_pages - 1 - i;   // page 0 on top
+    const int state[4] = {p.n_pages, 0, 0, 0};
+    if (cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    if (cudaMemcpy(p.free_pages, ids.data(), ids.size() * sizeof(int), cudaMemcpyHostToDevice) != cudaSuccess ||
+        cudaMemcpy(p.state, state, sizeof state, cudaMemcpyHostToDevice) != cudaSuccess ||
+        cudaMemset(p.lens, 0, nb_ * sizeof(int)) != cudaSuccess ||
+        cudaMemset(p.table, 0xff, (size_t)nb_ * p.width * sizeof(int)) != cudaSuccess)
+      return -3;
+    return cudaDeviceSynchronize() == cudaSuccess ? 0 : -3;
+  }
+
+  // The step's pages and slots, before the first block (two launches).
+  int enqueue_plan() {
+    PagedState& p = *pg_;
+    const tb2_paged_plan_args a = {p.lens,   p.add,       nb_, p.table,   p.width, p.width, p.free_pages,
+                                   p.n_pages, p.state,    p.page_size, p.n_pages, nb_, p.lens, p.state,
+                                   p.cu,     p.slots,     p.positions, p.requests};
+    launches_ += 2;
+    if (int rc = paged_plan_launch(a, p.err, st_)) return rc;
+    return launch_pdl(kv_rows_kernel, dim3(1), dim3(32), 0, st_, (const int*)p.add, (const int*)p.cu,
+                      (const long long*)p.slots, (const int*)p.positions, nb_, p.row_slot, p.row_pos);
+  }
+
+  // Block l's append and attention: qkv_ -> p.att.
+  int enqueue_paged_attention(int l, const float* bias) {
+    const LlamaConfig& c = e_.cfg();
+    PagedState& p = *pg_;
+    const int H = c.n_heads, KV = c.n_kv, dh = c.d_head, W = (H + 2 * KV) * dh;
+    const long long page = (long long)KV * p.page_size * dh, off = (long long)l * p.n_pages * page;
+    tb2_paged_kv kv = {p.k + off * type_bytes(p.type), p.v + off * type_bytes(p.type),
+                       p.ks ? p.ks + off / 32 : nullptr, p.vs ? p.vs + off / 32 : nullptr,
+                       p.type, p.n_pages, p.page_size, KV, dh, page, (long long)p.page_size * dh, dh};
+    tb2_paged_append_args ap = {};
+    ap.n_tokens = nb_; ap.n_heads = H; ap.row_type = kTypeF32;
+    ap.q = qkv_; ap.k = qkv_ + H * dh; ap.v = qkv_ + (H + KV) * dh; ap.q_out = qkv_;
+    ap.ldq = ap.ldk = ap.ldv = ap.ldqo = W;
+    ap.bias = bias;
+    ap.rope = e_.rope_table(); ap.rope_rows = e_.rope_rows();
+    ap.positions = p.row_pos; ap.slots = p.row_slot;
+    tb2_paged_attend_args at = {};
+    at.n_req = nb_; at.n_heads = H; at.row_type = kTypeF32;
+    at.q = qkv_; at.ldq = W; at.out = p.att; at.ldo = H * dh;
+    at.table = p.table; at.table_width = p.width; at.table_stride = p.width; at.lens = p.lens;
+    at.scale = 1.0f / std::sqrt((float)dh);
+    at.workspace = p.workspace; at.workspace_bytes = tb2_paged_attend_workspace();
+    launches_ += 2;
+    if (int rc = paged_append_launch(kv, ap, p.err, st_)) return rc;
+    return paged_attend_launch(kv, at, p.err, st_);
+  }
+
   template <int NB>
   int gemv_nb(const GemvArgs& g) {
     const bool q8 = g.wq != nullptr;
@@ -803,13 +996,15 @@ class KvEngine {
     const LlamaEngine::WeightView E = e_.weight("token_embd.weight");
     ++launches_;
     if (launch_pdl(kv_embed_kernel, dim3(nb_), dim3(256), 0, st_, E.f32, (const int*)tok_, d, x_)) return -3;
+    if (pg_)
+      if (int rc = enqueue_plan()) return rc;
     KvCache cache;
     for (int l = 0; l < c.n_layers; ++l) {
       const std::string pre = "blk." + std::to_string(l) + ".";
       const long long loff = (long long)l * nb_ * KV * max_T_ * dh;
       if (q8_) {
         cache.kq = kq_ + loff; cache.vq = vq_ + loff; cache.ks = ks_ + loff / 32; cache.vs = vs_ + loff / 32;
-      } else {
+      } else if (!pg_) {
         cache.k32 = k32_ + loff; cache.v32 = v32_ + loff;
       }
       // q | k | v with the attention RMSNorm folded in (and their adapters)
@@ -822,22 +1017,29 @@ class KvEngine {
       add_lora(g, l, 1, H * dh, KV * dh, 0);
       add_lora(g, l, 2, (H + KV) * dh, KV * dh, 0);
       if (int rc = gemv(g)) return rc;
-      AppendArgs ap;
-      ap.qkv = qkv_;
-      ap.bias = c.qkv_bias ? e_.weight(pre + "attn_q.bias").f32 : nullptr;
-      ap.pos = pos_; ap.cs = reinterpret_cast<const float2*>(e_.rope_table()); ap.tab_rows = e_.rope_rows();
-      ap.H = H; ap.KV = KV; ap.dh = dh; ap.max_T = max_T_; ap.c = cache;
-      ++launches_;
-      if (launch_pdl(kv_append_kernel, dim3(nb_, H + KV), dim3(dh), (size_t)2 * dh * 4, st_, ap)) return -3;
-      AttnArgs at;
-      at.qkv = qkv_; at.pos = pos_; at.c = cache; at.H = H; at.KV = KV; at.dh = dh; at.max_T = max_T_;
-      at.nsplit = nsplit_; at.scale = 1.0f / std::sqrt((float)dh); at.part = part_;
-      ++launches_;
-      if (launch_pdl(kv_attn_kernel, dim3(nb_ * H, nsplit_), dim3(kChunk), attn_smem_, st_, at)) return -3;
-      // x1 = x + att Wo^T, the attention output assembled from the chunks while staging
-      g = wargs(pre + "attn_output.weight", d, H * dh);
-      g.part = part_; g.nsplit = nsplit_; g.dh = dh;
-      g.ldx = H * dh; g.out = x1_; g.ldo = d; g.res = x_; g.mode = 1;
+      const float* bias = c.qkv_bias ? e_.weight(pre + "attn_q.bias").f32 : nullptr;
+      if (pg_) {
+        if (int rc = enqueue_paged_attention(l, bias)) return rc;
+        g = wargs(pre + "attn_output.weight", d, H * dh);
+        g.x = pg_->att; g.ldx = H * dh; g.out = x1_; g.ldo = d; g.res = x_; g.mode = 1;
+      } else {
+        AppendArgs ap;
+        ap.qkv = qkv_;
+        ap.bias = bias;
+        ap.pos = pos_; ap.cs = reinterpret_cast<const float2*>(e_.rope_table()); ap.tab_rows = e_.rope_rows();
+        ap.H = H; ap.KV = KV; ap.dh = dh; ap.max_T = max_T_; ap.c = cache;
+        ++launches_;
+        if (launch_pdl(kv_append_kernel, dim3(nb_, H + KV), dim3(dh), (size_t)2 * dh * 4, st_, ap)) return -3;
+        AttnArgs at;
+        at.qkv = qkv_; at.pos = pos_; at.c = cache; at.H = H; at.KV = KV; at.dh = dh; at.max_T = max_T_;
+        at.nsplit = nsplit_; at.scale = 1.0f / std::sqrt((float)dh); at.part = part_;
+        ++launches_;
+        if (launch_pdl(kv_attn_kernel, dim3(nb_ * H, nsplit_), dim3(kChunk), attn_smem_, st_, at)) return -3;
+        // x1 = x + att Wo^T, the attention output assembled from the chunks while staging
+        g = wargs(pre + "attn_output.weight", d, H * dh);
+        g.part = part_; g.nsplit = nsplit_; g.dh = dh;
+        g.ldx = H * dh; g.out = x1_; g.ldo = d; g.res = x_; g.mode = 1;
+      }
       if (int rc = adapter_u(l, 3, g)) return rc;
       add_lora(g, l, 3, 0, d, 0);
       if (int rc = gemv(g)) return rc;
@@ -867,6 +1069,7 @@ class KvEngine {
   LlamaEngine& e_;
   int max_T_, nb_;
   bool q8_;
+  std::unique_ptr<PagedState> pg_;   // set: a paged cache
   int nsplit_ = 1, launches_ = 0;
   size_t attn_smem_ = 0;   // dynamic shared memory of the attention kernel (the chunk's V rows)
   // adapters by target (q, k, v, o, gate, up, down): u = A x buffer [n_seq][rows]
@@ -910,6 +1113,40 @@ int tb2_kv_realize(void* sess, int max_T, int n_seq, int kv_type) {
   return 0;
 }
 
+int tb2_kv_realize_paged(void* sess, int max_T, int n_seq, int kv_type, int page_size, int n_pages) {
+  if (!sess || (kv_type != 8 && !tb2::row_type_ok(kv_type)) || max_T < 1 || page_size < 1 || page_size > (1 << 20) ||
+      n_pages < 1 || max_T > 0x7fffff00 - page_size)
+    return -1;
+  tb2::Session* s = static_cast<tb2::Session*>(sess);
+  if (!s->eng || s->kv) return -2;
+  auto k = std::make_unique<tb2::KvEngine>(*s->eng, max_T, n_seq, kv_type, page_size, n_pages);
+  const int rc = k->realize();
+  if (rc) return rc;
+  s->kv = k.release();
+  return 0;
+}
+
+int tb2_kv_decode_paged(void* sess, const long long* tokens, int n_seq, float* logits) {
+  if (!sess) return -1;
+  tb2::Session* s = static_cast<tb2::Session*>(sess);
+  if (!s->kv || !s->kv->paged()) return -2;
+  return s->kv->decode_paged(tokens, n_seq, logits);
+}
+
+int tb2_kv_release(void* sess, const int* done, int n_seq) {
+  if (!sess) return -1;
+  tb2::Session* s = static_cast<tb2::Session*>(sess);
+  if (!s->kv || !s->kv->paged()) return -2;
+  return s->kv->release(done, n_seq);
+}
+
+int tb2_kv_paged_state(void* sess, int* lens, int n_seq, int* free_pages) {
+  if (!sess) return -1;
+  tb2::Session* s = static_cast<tb2::Session*>(sess);
+  if (!s->kv || !s->kv->paged()) return -2;
+  return s->kv->paged_state(lens, n_seq, free_pages);
+}
+
 int tb2_kv_reset(void* sess) {
   if (!sess || !static_cast<tb2::Session*>(sess)->kv) return -2;
   return static_cast<tb2::Session*>(sess)->kv->reset();
@@ -918,7 +1155,7 @@ int tb2_kv_reset(void* sess) {
 int tb2_kv_decode(void* sess, const long long* tokens, const long long* positions, int n_seq, float* logits) {
   if (!sess) return -1;
   tb2::Session* s = static_cast<tb2::Session*>(sess);
-  if (!s->kv) return -2;
+  if (!s->kv || s->kv->paged()) return -2;
   return s->kv->decode(tokens, positions, n_seq, logits);
 }
 

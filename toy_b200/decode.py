@@ -55,3 +55,71 @@ class KVDecoder:
 
     def close(self) -> None:
         lib().tb2_kv_free(self.eng.sess)
+
+
+_KV_TYPES = {"f32": 0, "f16": 1, "q8_0": 8, "bf16": 30}
+
+
+class PagedKVDecoder:
+    """Decode over a paged cache: up to n_seq sequences of unlike lengths share n_pages pages of page_size tokens
+    (tb2_kv_*_paged). kv_type: "f32", "f16", "bf16" or "q8_0"."""
+
+    def __init__(self, engine, max_T: int, n_seq: int, n_pages: int, page_size: int = 16, kv_type: str = "bf16"):
+        if kv_type not in _KV_TYPES:
+            raise ValueError(f"toy_b200: kv_type is one of {', '.join(_KV_TYPES)}, not {kv_type!r}")
+        self.eng = engine
+        self.max_T, self.n_seq, self.n_pages, self.page_size = max_T, n_seq, n_pages, page_size
+        self.vocab = engine.cfg.vocab
+        check(lib().tb2_kv_realize_paged(engine.sess, max_T, n_seq, _KV_TYPES[kv_type], page_size, n_pages),
+              "tb2_kv_realize_paged")
+        self._logits = np.empty((n_seq, self.vocab), np.float32)
+
+    def reset(self) -> None:
+        check(lib().tb2_kv_reset(self.eng.sess), "tb2_kv_reset")
+
+    def decode_step(self, tokens: Sequence[int]) -> np.ndarray:
+        """tokens[b] appended to sequence b (-1: nothing); logits [n_seq, vocab] of the tokens after them. MemoryError
+        when the pool has too few free pages: the step did nothing, and may be repeated after a release."""
+        t = np.ascontiguousarray(np.asarray(tokens, np.int64).reshape(self.n_seq))
+        rc = lib().tb2_kv_decode_paged(self.eng.sess, t.ctypes.data_as(C.POINTER(C.c_longlong)), self.n_seq,
+                                       self._logits.ctypes.data_as(C.POINTER(C.c_float)))
+        if rc == -5:
+            raise MemoryError("toy_b200: no free pages for this decode step")
+        check(rc, "tb2_kv_decode_paged")
+        return self._logits.copy()
+
+    def release(self, seqs: Sequence[int]) -> None:
+        """Empty these sequences and give their pages back."""
+        d = np.zeros(self.n_seq, np.int32)
+        d[np.asarray(seqs, np.int64)] = 1
+        check(lib().tb2_kv_release(self.eng.sess, d.ctypes.data_as(C.POINTER(C.c_int)), self.n_seq), "tb2_kv_release")
+
+    def state(self) -> tuple:
+        """(lengths [n_seq], free pages)."""
+        lens, free = np.zeros(self.n_seq, np.int32), C.c_int(0)
+        check(lib().tb2_kv_paged_state(self.eng.sess, lens.ctypes.data_as(C.POINTER(C.c_int)), self.n_seq,
+                                       C.byref(free)), "tb2_kv_paged_state")
+        return lens, free.value
+
+    def generate(self, prompts: Sequence[Sequence[int]], n_new: int) -> list:
+        """Greedy continuations of prompts of any lengths (one per sequence, at least a token each) by n_new tokens."""
+        feed = [list(map(int, p)) for p in prompts]
+        if len(feed) != self.n_seq or any(not p for p in feed):
+            raise ValueError("toy_b200: one prompt of a token or more per sequence")
+        out = [[] for _ in feed]
+        at = [0] * self.n_seq
+        while any(len(o) < n_new for o in out):
+            toks = [feed[b][at[b]] if len(out[b]) < n_new else -1 for b in range(self.n_seq)]
+            logits = self.decode_step(toks)
+            for b in range(self.n_seq):
+                if toks[b] < 0:
+                    continue
+                at[b] += 1
+                if at[b] == len(feed[b]):
+                    nxt = int(np.argmax(logits[b]))
+                    out[b].append(nxt)
+                    feed[b].append(nxt)
+        return out
+
+    def close(self) -> None:
+        lib().tb2_kv_free(self.eng.sess)
