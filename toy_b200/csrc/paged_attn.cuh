@@ -155,10 +155,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t tf32(float x) {
-  uint32_t y;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
-  return y;
+// An f32 value as two tf32 ones: its leading 11 bits, and 11 of the 13 that
+// follow (cut, not rounded: at most 3 / 2^24 of the value is left out).
+struct Split {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Split tf32x2(float x) {
+  const uint32_t hi = __float_as_uint(x) & 0xffffe000u;
+  return {hi, __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u};
 }
 // Two f32 operations in one instruction.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -731,8 +735,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             for (int r = 0; r < R; ++r)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                hi[r][k] = tf32(x[r][i + k]);
-                lo[r][k] = tf32(x[r][i + k] - __uint_as_float(hi[r][k]));
+                const Split v = tf32x2(x[r][i + k]);
+                hi[r][k] = v.hi;
+                lo[r][k] = v.lo;
               }
             if constexpr (HT == 8) {
               qf[s * 32 + lane] = make_uint4(hi[0][0], lo[0][0], hi[0][1], lo[0][1]);
@@ -855,8 +860,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
               uint32_t hi[4], lo[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                hi[k] = tf32(__uint_as_float(x[k]));
-                lo[k] = tf32(__uint_as_float(x[k]) - __uint_as_float(hi[k]));
+                const Split v = tf32x2(__uint_as_float(x[k]));
+                hi[k] = v.hi;
+                lo[k] = v.lo;
               }
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
@@ -918,14 +924,25 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       int new_lift = lift_d;
       ScalePair<C::NB> vsc[CT == kCacheQ8 ? NT : 1];
       if constexpr (CT == kCacheQ8) {
-        uint32_t big = 0;   // the tile's largest |V scale|, as fp16 bits
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          vsc[i].load(ks + C::kOffVS + (8 * i + 2 * c) * C::NB * 2);
+        for (int i = 0; i < NT; ++i) vsc[i].load(ks + C::kOffVS + (8 * i + 2 * c) * C::NB * 2);
+        // the tile's largest |V scale|, as fp16 bits: a lane looks at a row (two of them at 64 keys)
+        uint32_t big = 0;
 #pragma unroll
-          for (int e = 0; e < C::NB; ++e) big = __vmaxu2(big, vsc[i].w[e] & 0x7fff7fffu);
+        for (int i = 0; i < C::RPL; ++i) {
+          const uint32_t row = ks + C::kOffVS + (lane + 32 * i) * C::NB * 2;
+          if constexpr (C::NB == 4) {
+            const uint2 w = lds64(row);
+            big = max(max(w.x & 0x7fffu, w.x >> 16 & 0x7fffu), max(w.y & 0x7fffu, w.y >> 16 & 0x7fffu));
+          } else if constexpr (C::NB == 2) {
+            const uint32_t w = lds32(row);
+            big = max(w & 0x7fffu, w >> 16 & 0x7fffu);
+          } else {
+#pragma unroll
+            for (int e = 0; e < C::NB; ++e) big = max(big, lds16(row + 2 * e) & 0x7fffu);
+          }
         }
-        big = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
+        big = __reduce_max_sync(0xffffffffu, big);
         // below 2^(1 - lift) (an infinite scale makes the sums NaN whatever the lift)
         const int lift = 127 - (int)(__float_as_uint(fmaxf(__half2float(__ushort_as_half((uint16_t)big)), 0x1p-24f)) >> 23);
         if (!have_d || lift < lift_d) new_lift = lift;
@@ -978,20 +995,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         uint4 ph[NT], pl[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {   // 8 keys: step k holds key 2 k, step k + 4 key 2 k + 1
+          Split v[2 * R];
+#pragma unroll
+          for (int k = 0; k < 2 * R; ++k) v[k] = tf32x2(s[i][k]);
           if constexpr (HT == 8) {
-            ph[i].x = tf32(s[i][0]);
-            ph[i].z = tf32(s[i][1]);
-            ph[i].y = tf32(s[i][0] - __uint_as_float(ph[i].x));
-            ph[i].w = tf32(s[i][1] - __uint_as_float(ph[i].z));
+            ph[i] = make_uint4(v[0].hi, v[0].lo, v[1].hi, v[1].lo);
           } else {
-            ph[i].x = tf32(s[i][0]);
-            ph[i].y = tf32(s[i][2]);
-            ph[i].z = tf32(s[i][1]);
-            ph[i].w = tf32(s[i][3]);
-            pl[i].x = tf32(s[i][0] - __uint_as_float(ph[i].x));
-            pl[i].y = tf32(s[i][2] - __uint_as_float(ph[i].y));
-            pl[i].z = tf32(s[i][1] - __uint_as_float(ph[i].z));
-            pl[i].w = tf32(s[i][3] - __uint_as_float(ph[i].w));
+            ph[i] = make_uint4(v[0].hi, v[2 * R - 2].hi, v[1].hi, v[2 * R - 1].hi);
+            pl[i] = make_uint4(v[0].lo, v[2 * R - 2].lo, v[1].lo, v[2 * R - 1].lo);
           }
         }
 #pragma unroll
@@ -1004,12 +1015,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint32_t a0 = tf32(__uint_as_float(x0[k])), a1 = tf32(__uint_as_float(x1[k]));
-              const uint32_t e0 = tf32(__uint_as_float(x0[k]) - __uint_as_float(a0));
-              const uint32_t e1 = tf32(__uint_as_float(x1[k]) - __uint_as_float(a1));
-              mma8(i == 0, d[k], ph[i], e0, e1);
-              if constexpr (HT == 16) mma8(false, d[k], pl[i], a0, a1);
-              mma8(false, d[k], ph[i], a0, a1);
+              const Split v0 = tf32x2(__uint_as_float(x0[k])), v1 = tf32x2(__uint_as_float(x1[k]));
+              mma8(i == 0, d[k], ph[i], v0.lo, v1.lo);
+              if constexpr (HT == 16) mma8(false, d[k], pl[i], v0.hi, v1.hi);
+              mma8(false, d[k], ph[i], v0.hi, v1.hi);
             }
           }
 #pragma unroll
