@@ -31,6 +31,15 @@
 // sums are joined. A history that one CTA holds whole is written at once;
 // pieces go to the workspace and the CTA that finishes last adds them up in
 // order (a ticket per history), so the result does not depend on timing.
+//
+// Measured on one B200 (cold inputs): 131072 tokens of one request, 32 / 8
+// heads of 128, bf16: 104 us, 5.2 TB/s with the launch and 6.3 TB/s between
+// 65536 and 131072 tokens; 64 histories up to 8191 (28 / 4 heads of 128, f32
+// rows over bf16): 113 us, 4.8 TB/s; 16 up to 2048 (16 / 16 of 128, f32): 74
+// us, 5.0 TB/s; 128 up to 4096 (9 / 3 of 64, Q8_0): 42 us, 2.6 TB/s; 77 tokens:
+// 6.3 us. A 16-bit or f32 cache waits for the memory (a third of the issue
+// slots used); Q8_0 at d_head 64 is bound by its 750 instructions per 32 keys,
+// half of them the conversions of quants and scales.
 #pragma once
 #include <algorithm>
 #include <type_traits>
