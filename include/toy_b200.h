@@ -254,7 +254,7 @@ int tb2_paged_prepare(void);
  * nothing is taken: the table, the lengths and the stack count stay and every
  * slot is -1. lens_out may be lens and state_out may be state (in place);
  * other arrays do not overlap. All arrays are device memory. n_req is at most
- * 16384. */
+ * 16384, n_tokens at most 2^31 - 256. */
 typedef struct tb2_paged_plan_args {
   const int *lens, *add;
   int n_req;
@@ -336,6 +336,8 @@ int tb2_paged_append(const tb2_paged_kv *kv, const tb2_paged_append_args *args, 
  * statistics and sums are f32. The history is split over the GPU and joined
  * in a fixed order, so the same call gives the same bits; another batch, or
  * another table width, may split a request's history elsewhere. workspace
+ * n_req * n_kv * ceil(n_heads / n_kv / 8) * (tokens a table row spans) is
+ * below 2^36. workspace
  * holds tb2_paged_attend_workspace() bytes (16-byte aligned) set up once by
  * tb2_paged_attend_workspace_init; calls that may overlap on the GPU (two
  * streams, two graphs) need one each. */

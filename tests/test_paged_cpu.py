@@ -80,7 +80,7 @@ def test_bad_append(bad):
     dict(n_req=-1), dict(n_heads=0), dict(n_heads=3), dict(row_type=8), dict(q=None), dict(out=None),
     dict(lens=None), dict(table=None), dict(ldq=255), dict(ldo=128), dict(q=P + 2), dict(out=P + 1),
     dict(table_width=0), dict(table_stride=2), dict(table_width=1 << 28, table_stride=1 << 28),
-    dict(scale=float("nan")), dict(scale=float("inf")), dict(workspace=None), dict(workspace_bytes=8),
+    dict(n_req=1 << 20, table_width=1 << 17, table_stride=1 << 17), dict(scale=float("nan")), dict(scale=float("inf")), dict(workspace=None), dict(workspace_bytes=8),
     dict(workspace=P + 8)], ids=str)
 def test_bad_attend(bad):
     from toy_b200._lib import lib
@@ -90,7 +90,7 @@ def test_bad_attend(bad):
 @pytest.mark.parametrize("bad", [
     dict(n_req=0), dict(n_req=16385), dict(lens=None), dict(add=None), dict(table=None), dict(table_width=0),
     dict(table_stride=2), dict(free_pages=None), dict(n_free=-1), dict(state=None), dict(page_size=0),
-    dict(page_size=(1 << 20) + 1), dict(n_pages=0), dict(n_tokens=-1), dict(lens_out=None), dict(state_out=None),
+    dict(page_size=(1 << 20) + 1), dict(n_pages=0), dict(n_tokens=-1), dict(n_tokens=0x7fffff01), dict(lens_out=None), dict(state_out=None),
     dict(cu_tokens=None), dict(slots=None), dict(positions=None), dict(requests=None),
     dict(table_width=1 << 28, table_stride=1 << 28), dict(lens_out=P + 4), dict(state_out=P - 8)], ids=str)
 def test_bad_plan(bad):

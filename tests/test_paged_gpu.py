@@ -429,6 +429,61 @@ def test_attend_bad_pages(cuda):
     assert lib().tb2_device_error() == 0x5001 and bool((bad == 0).all())
 
 
+def test_attend_lengths_past_the_table(cuda):
+    """A length beyond what the table row spans is cut to it."""
+    import torch
+    from toy_b200 import paged
+    g = torch.Generator(device=cuda).manual_seed(0)
+    k, v, _, _ = R.make_pools(12, 2, 16, 64, "f16", "heads", g, cuda)
+    q = torch.randn((2, 6, 64), generator=g, device=cuda)
+    table = torch.arange(12, dtype=torch.int32, device=cuda).view(2, 6)
+    c = paged.PagedCache(k, v)
+    want = paged.attend(c, q, table, i32([96, 40], cuda))
+    for long in (97, 1000, 2 ** 31 - 1):
+        assert torch.equal(paged.attend(c, q, table, i32([long, 40], cuda)), want)
+    no_error()
+
+
+def test_attend_huge_queries(cuda):
+    """Queries near the end of the f32 range still pick the key of the largest score."""
+    import torch
+    from toy_b200 import paged
+    for cache in ("f32", "f16", "bf16", "q8_0"):
+        g = torch.Generator(device=cuda).manual_seed(0)
+        k, v, ks, vs = R.make_pools(4, 1, 16, 64, cache, "heads", g, cuda)
+        q = torch.randn((1, 2, 64), generator=g, device=cuda) * torch.tensor([1e35, 1e-30], device=cuda)[:, None]
+        table = torch.arange(4, dtype=torch.int32, device=cuda)[None, :]
+        out = paged.attend(paged.PagedCache(k, v, ks, vs), q, table, i32([60], cuda))
+        kd, vd = (R.values(a, b).reshape(-1, 64)[:60] for a, b in ((k, ks), (v, vs)))
+        top = vd[(kd @ q[0, 0].double()).argmax()]
+        assert float((out[0, 0].double() - top).abs().max()) <= 2e-6 * float(top.abs().max())
+        mean = vd.mean(0)      # all scores are 0
+        assert float((out[0, 1].double() - mean).abs().max()) <= 2e-6 * float(vd.abs().mean())
+    no_error()
+
+
+def test_own_workspace_in_a_graph(cuda):
+    """Without a workspace the call makes its own, in a captured graph too."""
+    import torch
+    from toy_b200 import paged
+    g = torch.Generator(device=cuda).manual_seed(3)
+    k, v, _, _ = R.make_pools(200, 2, 16, 64, "bf16", "heads", g, cuda)
+    c = paged.PagedCache(k, v)
+    q = torch.randn((2, 8, 64), generator=g, device=cuda)
+    table, lens = torch.arange(200, dtype=torch.int32, device=cuda).view(2, 100), i32([1600, 900], cuda)
+    want = paged.attend(c, q, table, lens)
+    out = torch.empty_like(want)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        paged.attend(c, q, table, lens, out=out)
+    for _ in range(3):
+        out.fill_(7)
+        gr.replay()
+        assert torch.equal(out, want)
+    no_error()
+
+
 def test_attend_past_32_bits(cuda):
     """A pool of more than 2^31 elements: pages at its far end."""
     import torch

@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 #pragma unroll
           for (int w = 0; w < kAttnWarps; ++w) x[r] = fmaxf(x[r], qmax[w][g + 8 * r]);
           int e = (int)(__float_as_uint(x[r]) >> 23) - 127 - 4;   // x < 2^(e + 5)
-          e = max(-100, min(100, e));
+          e = max(-100, min(123, e));   // (a row of inf or NaN stays one)
           const float up = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
           for (int own = 0; own < kOwn; ++own)
@@ -995,7 +995,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float p = ex2(fmaf(s[i][2 * r + k], fac[r], base));
+            // (rounded as the maximum was: with a fused product the largest key's exponent would be the rounding of m,
+            // which passes any range for scores of 2^30)
+            float p = ex2(__fadd_rn(__fmul_rn(s[i][2 * r + k], fac[r]), base));
             if (masked && !((ok >> (8 * i + 2 * c + k)) & 1)) p = 0.f;   // (a factor of 0 makes -inf NaN)
             s[i][2 * r + k] = p;
             l[r] += p;

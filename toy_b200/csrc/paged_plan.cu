@@ -328,7 +328,8 @@ extern "C" {
 
 int tb2_paged_plan(const tb2_paged_plan_args* a, void* stream) {
   if (!a || a->n_req < 1 || a->n_req > tb2::kMaxReq || a->table_width < 1 || a->table_stride < a->table_width ||
-      a->page_size < 1 || a->page_size > (1 << 20) || a->n_pages < 1 || a->n_free < 0 || a->n_tokens < 0)
+      a->page_size < 1 || a->page_size > (1 << 20) || a->n_pages < 1 || a->n_free < 0 || a->n_tokens < 0 ||
+      a->n_tokens > 0x7fffff00)
     return -1;
   if (!a->lens || !a->add || !a->table || !a->state || !a->lens_out || !a->state_out || !a->cu_tokens ||
       (a->n_free && !a->free_pages) || (a->n_tokens && (!a->slots || !a->positions || !a->requests)))

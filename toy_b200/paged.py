@@ -97,6 +97,8 @@ class PagedCache:
         self.c = PagedKV(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None,
                          v_scale.data_ptr() if q8 else None, _CACHE[k.dtype], n_pages, page, n_kv, dh, *strides)
         self.ref = C.byref(self.c)
+        if self.index not in _prepared:   # (so that a first call may be captured into a CUDA graph)
+            _prepare(self.index)
 
 
 class Plan(NamedTuple):
@@ -127,8 +129,8 @@ def plan(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages:
     the sum of add). `out` may hold lens and state themselves. Check state[1] of the result when it reaches the host:
     a status other than 0 left everything as it was."""
     n, dev = lens.numel(), lens.get_device()
-    if dev < 0 or n < 1 or not 0 <= n_tokens < 2**31:
-        _bad("lens: on a GPU, of one request or more; n_tokens not negative")
+    if dev < 0 or n < 1 or max(page_size, n_pages, n_tokens) >= 2**31 or n_tokens < 0:
+        _bad("lens: on a GPU, of one request or more; page_size, n_pages and n_tokens below 2^31")
     tp, width, stride = _table(table, n, dev)
     if out is None:   # two allocations, as each call into torch is a microsecond or more
         slots = lens.new_empty(n_tokens, dtype=_I64)
@@ -156,8 +158,8 @@ def release(lens: torch.Tensor, done: torch.Tensor, table: torch.Tensor, free_pa
     """The pages of every request with done[b] != 0 go back on the stack, its table row is cleared and its length set
     to 0; lens and state are updated in place unless other tensors are given."""
     n, dev = lens.numel(), lens.get_device()
-    if dev < 0 or n < 1:
-        _bad("lens: on a GPU, of one request or more")
+    if dev < 0 or n < 1 or max(page_size, n_pages) >= 2**31:
+        _bad("lens: on a GPU, of one request or more; page_size and n_pages below 2^31")
     a = PagedReleaseArgs(_ints(lens, n, dev, "lens"), _ints(done, n, dev, "done"), n, *_table(table, n, dev),
                          _ints(free_pages, 0, dev, "free_pages"), free_pages.numel(), _ints(state, 4, dev, "state"),
                          page_size, n_pages, _ints(lens if lens_out is None else lens_out, n, dev, "lens_out"),
