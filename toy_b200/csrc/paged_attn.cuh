@@ -469,7 +469,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   // become free, did not make the last one earlier: the memory is busy to the end, and every range costs 2 us.)
   // A CTA for each history where there are as many (eight of one unit: 6.1 us, 8.9 when four CTAs take two each); more
   // only for kMinUnits each.
-  const int G = min((int)gridDim.x, max(units / kMinUnits, histories * KVH));
+  // Short ranges and several CTAs to a history: a whole number of them, where that leaves three quarters of the CTAs, so
+  // that equal histories are cut alike: a CTA with the end of one and the start of the next does the second one's share
+  // 8 us later.
+  int G = min((int)gridDim.x, max(units / kMinUnits, histories * KVH));
+  const int even = G / (histories * KVH) * (histories * KVH);
+  if (units < 16 * G && even * 4 >= G * 3) G = even;
   if (blockIdx.x >= G) return;
   auto range = [&](int i) { return (int)((long long)i * units / G); };
   auto cta_of = [&](int u) { return (int)(((u + 1LL) * G - 1) / units); };   // whose range holds unit u
