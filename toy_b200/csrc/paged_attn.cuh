@@ -33,11 +33,11 @@
 // order (a ticket per history), so the result does not depend on timing.
 //
 // Measured on one B200 (cold inputs): 131072 tokens of one request, 32 / 8
-// heads of 128, bf16: 104 us, 5.2 TB/s with the launch and 6.3 TB/s between
+// heads of 128, bf16: 101 us, 5.3 TB/s with the launch and 6.3 TB/s between
 // 65536 and 131072 tokens; 64 histories up to 8191 (28 / 4 heads of 128, f32
-// rows over bf16): 113 us, 4.8 TB/s; 16 up to 2048 (16 / 16 of 128, f32): 74
-// us, 5.0 TB/s; 128 up to 4096 (9 / 3 of 64, Q8_0): 42 us, 2.6 TB/s; 77 tokens:
-// 6.3 us. A 16-bit or f32 cache waits for the memory (a third of the issue
+// rows over bf16): 113 us, 4.8 TB/s; 16 up to 2048 (16 / 16 of 128, f32): 73
+// us, 5.1 TB/s; 128 up to 4096 (9 / 3 of 64, Q8_0): 42 us, 2.6 TB/s; 77 tokens:
+// 6.5 us. A 16-bit or f32 cache waits for the memory (a third of the issue
 // slots used); Q8_0 at d_head 64 is bound by its 750 instructions per 32 keys,
 // half of them the conversions of quants and scales.
 #pragma once
@@ -421,27 +421,30 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
 
   // ---- the list's length (below 2^31 by the host's limit)
   auto units_of = [](int len) { return (len + UK - 1) / UK; };
-  int total, histories = 0;   // (of one key head)
+  int total, histories = 0, longest = 0;   // (of one key head)
   const int per = (n + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
   {
     const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
-    int s = 0, live = 0;
+    int s = 0, live = 0, top = 0;
     for (int b = b0; b < b1; ++b) {
       const int len = length(b);
       s += units_of(len);
       live += len > 0;
+      top = max(top, units_of(len));
     }
     live = __reduce_add_sync(0xffffffffu, live);
+    top = __reduce_max_sync(0xffffffffu, top);
     int inc = s;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    __shared__ int wsum[kAttnWarps], wlive[kAttnWarps];
+    __shared__ int wsum[kAttnWarps], wlive[kAttnWarps], wtop[kAttnWarps];
     if (lane == 31) {
       wsum[warp] = inc;
       wlive[warp] = live;
+      wtop[warp] = top;
     }
     __syncthreads();
     int base = 0;
@@ -451,6 +454,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       if (w < warp) base += wsum[w];
       total += wsum[w];
       histories += wlive[w];
+      longest = max(longest, wtop[w]);
     }
     pre[tid] = base + inc - s;
     __syncthreads();
@@ -469,12 +473,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   // become free, did not make the last one earlier: the memory is busy to the end, and every range costs 2 us.)
   // A CTA for each history where there are as many (eight of one unit: 6.1 us, 8.9 when four CTAs take two each); more
   // only for kMinUnits each.
-  // Short ranges and several CTAs to a history: a whole number of them, where that leaves three quarters of the CTAs, so
-  // that equal histories are cut alike: a CTA with the end of one and the start of the next does the second one's share
-  // 8 us later.
+  // Equal histories and several CTAs to each: a whole number of them, where that leaves three quarters of the CTAs, so
+  // that none has the end of one and the start of the next, whose share it would do several us later (8 x 1024 tokens
+  // 19.6 us, 15.6 so; 1 x 8192: 24.9 and 19.3).
   int G = min((int)gridDim.x, max(units / kMinUnits, histories * KVH));
   const int even = G / (histories * KVH) * (histories * KVH);
-  if (units < 16 * G && even * 4 >= G * 3) G = even;
+  if ((long long)longest * histories == total && even * 4 >= G * 3) G = even;
   if (blockIdx.x >= G) return;
   auto range = [&](int i) { return (int)((long long)i * units / G); };
   auto cta_of = [&](int u) { return (int)(((u + 1LL) * G - 1) / units); };   // whose range holds unit u
