@@ -296,9 +296,7 @@ struct Cfg {
   static constexpr int A = CT == kCacheF32 ? (NT >= 4 ? 2 : 4) : NT >= 8 ? 1 : 2;
   static constexpr int kBufFloats = (OT * 2 + 2) * R * 32;
   static constexpr int kJoinBytes = kBufs * kBufFloats * 4;
-  static constexpr int kScanBytes = (kAttnWarps * 32 + 1) * 8;
-  static constexpr int kRegion0 = kQBytes > kJoinBytes ? kQBytes : kJoinBytes;
-  static constexpr int kRegion = kRegion0 > kScanBytes ? kRegion0 : (kScanBytes + 15) / 16 * 16;
+  static constexpr int kRegion = kQBytes > kJoinBytes ? kQBytes : kJoinBytes;
   static constexpr int kSmem = kAttnWarps * ST * kStage + kRegion;
 
   // Q8_0: what the 16-byte chunks of row r are exchanged by.
@@ -417,9 +415,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   const int n = a.n_req, P = a.kv.page_size;
   const long long most = (long long)a.width * P;
   const int tiles_h = (a.group + HT - 1) / HT, KVH = a.kv.n_kv * tiles_h;
-  auto length = [&](int b) { return (int)min(most, (long long)max(0, __ldg(a.lens + b))); };
+  // (lengths, tables and scales may be written by the kernel before, beside which this one may have been launched: read
+  // after the grid wait and not through the read-only path)
+  auto length = [&](int b) { return (int)min(most, (long long)max(0, a.lens[b])); };
 
-  // ---- the list's length (below 2^31 by the host's limit)
+  // ---- the list's length (below 2^31 by the host's limit), each thread a run of requests
   auto units_of = [](int len) { return (len + UK - 1) / UK; };
   int total, histories = 0, longest = 0;   // (of one key head)
   const int per = (n + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
@@ -551,10 +551,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   long long head = 0;          // and its key head's offset in a page
   auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / P; };
   auto tile_key = [&]() { return (pc.t * kAttnWarps + warp) * TK; };
-  auto read_page = [&](int key) { return key < pc.len ? __ldg(pages + page_of(key)) : -1; };
+  auto read_page = [&](int key) { return key < pc.len ? pages[page_of(key)] : -1; };
   auto read_window = [&]() {
     win_t = pc.t;
-    // (units past the history: a key beyond its length; the sum stays in 32 bits, see the limit on tables)
+    // (units past the history have no page)
     const long long key = ((long long)(win_t + lane / C::NP) * kAttnWarps + warp) * TK + lane % C::NP * C::PR;
     win = key < pc.len ? read_page((int)key) : -1;
   };
@@ -592,8 +592,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
     } else if constexpr (CT == kCacheQ8) {
 #pragma unroll
       for (int e = 0; e < C::NB; ++e) {
-        sts16(dk + 2 * e, on ? __ldg(a.kv.ks + at + e) : 0);
-        sts16(dv + 2 * e, on ? __ldg(a.kv.vs + at + e) : 0);
+        sts16(dk + 2 * e, on ? a.kv.ks[at + e] : 0);
+        sts16(dv + 2 * e, on ? a.kv.vs[at + e] : 0);
       }
     }
   };
