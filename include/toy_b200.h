@@ -303,9 +303,10 @@ int tb2_paged_release(const tb2_paged_release_args *args, void *stream);
  * to q_out + i ldqo in row_type (q_out may be q with the same stride; q NULL:
  * only k and v), k and v into the page row of slots[i] in the cache's type
  * (Q8_0: ggml's quantiser). A negative slot leaves the cache as it is; its q
- * is still turned. The slots of one call are distinct. Sums and products are
- * f32, each rounded, products and sums not contracted. q, k, v and q_out
- * start on 16-byte boundaries with strides that are multiples of 16 bytes. */
+ * is still turned. The slots of one call are distinct, and rows and pools do
+ * not overlap. Sums and products are f32, each rounded, products and sums not
+ * contracted. q, k, v and q_out start on 16-byte boundaries with strides that
+ * are multiples of 16 bytes. */
 typedef struct tb2_paged_append_args {
   int n_tokens, n_heads, row_type;
   const void *q;
@@ -335,12 +336,11 @@ int tb2_paged_append(const tb2_paged_kv *kv, const tb2_paged_append_args *args, 
  * 0 f32, 1 f16 or 30 bf16, independent of the cache's type; the softmax
  * statistics and sums are f32. The history is split over the GPU and joined
  * in a fixed order, so the same call gives the same bits; another batch, or
- * another table width, may split a request's history elsewhere. workspace
- * n_req * n_kv * ceil(n_heads / n_kv / 8) * (tokens a table row spans) is
- * below 2^36. workspace
- * holds tb2_paged_attend_workspace() bytes (16-byte aligned) set up once by
- * tb2_paged_attend_workspace_init; calls that may overlap on the GPU (two
- * streams, two graphs) need one each. */
+ * another table width, may split a request's history elsewhere. out does not
+ * overlap q. n_req * n_kv * ceil(n_heads / n_kv / 8) * (tokens a table row
+ * spans) is below 2^36. workspace holds tb2_paged_attend_workspace() bytes
+ * (16-byte aligned) set up once by tb2_paged_attend_workspace_init; calls that
+ * may overlap on the GPU (two streams, two graphs) need one each. */
 typedef struct tb2_paged_attend_args {
   int n_req, n_heads, row_type;
   const void *q;

@@ -171,6 +171,48 @@ def test_generate_matches_contiguous(cuda):
     dec.close()
 
 
+def family(name):
+    from toy_b200 import LlamaConfig
+    if name == "bias":
+        return (O.LlamaCfg(vocab=512, d_model=256, n_heads=4, n_kv=2, d_head=128, d_ff=640, n_layers=2, rope_base=1e6,
+                           rms_eps=1e-6, qkv_bias=True),
+                LlamaConfig(512, 256, 4, 2, 128, 640, 2, 1e6, 1e-6, qkv_bias=True))
+    ff = O.llama3_freq_factors(64, 5.0e5, 8192, 32.0, 1.0, 4.0)
+    return (O.LlamaCfg(vocab=640, d_model=256, n_heads=10, n_kv=1, d_head=64, d_ff=512, n_layers=2, rope_base=5.0e5,
+                       rope_freq_factors=ff),
+            LlamaConfig(640, 256, 10, 1, 64, 512, 2, 5.0e5, 1e-5, rope_freq_factors=list(ff)))
+
+
+@pytest.mark.parametrize("name", ["bias", "freq_factors"])
+@pytest.mark.parametrize("mode", ["q8", "f32"])
+@pytest.mark.parametrize("cache", ["f32", "q8_0"])
+def test_families(cuda, name, mode, cache, monkeypatch):
+    """q, k and v biases; scaled RoPE frequencies with one key head for ten query heads: 24 tokens of a sequence beside
+    one that starts 9 tokens later, against the oracle's rows."""
+    from toy_b200.decode import PagedKVDecoder
+    from toy_b200._lib import lib
+    oc, gc = family(name)
+    eng, mdl = base_model(mode, oc, gc, 3)
+    kv_q8 = rounded(cache, monkeypatch)
+    ids = O.token_ids(31, 24, oc.vocab)
+    dec = PagedKVDecoder(eng, max_T=24, n_seq=2, n_pages=10, page_size=7, kv_type=cache)
+    late, got = 9, [[], []]
+    for t in range(24 + late):
+        toks = [ids[t] if t < 24 else -1, ids[t - late] if t >= late else -1]
+        logits = dec.decode_step(toks)
+        for b in range(2):
+            if toks[b] >= 0:
+                got[b].append(logits[b])
+    dec.close()
+    ref = rows_of(mdl, oc, ids, kv_q8)
+    errs = np.array([rel(got[b][t], ref[t]) for b in range(2) for t in range(24)])
+    if kv_q8:
+        assert float(np.median(errs)) < 1e-3 and float(errs.max()) < 1e-2, (float(np.median(errs)), float(errs.max()))
+    else:
+        assert float(errs.max()) < 1e-4, float(errs.max())
+    assert lib().tb2_device_error() == 0
+
+
 def test_smollm2_shape(cuda):
     """The SmolLM2-135M shape, 16 sequences of unlike lengths, against single-sequence oracle rows."""
     from toy_b200 import LlamaConfig
