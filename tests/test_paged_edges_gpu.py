@@ -1,0 +1,79 @@
+"""The paged KV-cache operators at the ends of their ranges: scores far from 0
+against the values that a single key leaves, and the calls the other paged
+tests do not make."""
+import math
+import os
+import sys
+
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import paged_ref as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(x, dev):
+    import torch
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def no_error():
+    from toy_b200._lib import lib
+    assert lib().tb2_device_error() == 0
+
+
+def pools(x, cache):
+    """(pool, scale) of f32 rows x in the cache's type."""
+    return R.q8_0(x) if cache == "q8_0" else (x.to(R.TORCH[cache]), None)
+
+
+# ------------------------------------------------------------------ attend
+@pytest.mark.parametrize("cache", ["f32", "f16", "bf16", "q8_0"])
+@pytest.mark.parametrize("G,dh", [(3, 64), (12, 64), (7, 128), (2, 32)])
+def test_attend_far_scores(cuda, cache, G, dh):
+    """Largest scores of 2^18 to 2^31 (in powers of two), above and below 0, histories of one key, of one tile and of
+    many: the key of the largest score takes all the weight, so the output is its value row and lse its score.
+
+    The keys' scores differ by 1 / 64 of 2^18 at least, so every other weight is 0 in 32 bits. What is left: the
+    weight's planes (2^-23 of it), the value's (f32: 2^-22), sums, the quotient and its rounding (4 u), 2^-20 together
+    with room for a factor of two; a score's are its operands' (2^-22 each at most), 3 roundings on the way in and 3
+    out: 2^-20 as well."""
+    import torch
+    from toy_b200 import paged
+    g = torch.Generator(device=cuda).manual_seed(dh + G)
+    P, lens = 16, [1, 40, 700]
+    width = 44
+    n = len(lens)
+    rows = torch.zeros((n, width * P, dh), device=cuda)
+    vals = torch.randn((n, width * P, dh), generator=g, device=cuda)
+    if cache == "q8_0":                             # (scales of unlike sizes: from 2^-9 to 2^4 times the usual)
+        vals *= 2.0 ** torch.randint(-9, 5, (n, width * P, 1), generator=g, device=cuda)
+    for b, L in enumerate(lens):
+        order = torch.randperm(L, generator=g, device=cuda)
+        rows[b, :L, 0] = 1 + order % 64 / 64.0      # the largest of many keys is met more than once
+        top = int((order % 64).max())
+        keep = (order % 64 == top).nonzero()[0]
+        rows[b, :L, 0][order % 64 == top] -= 1 / 64.0
+        rows[b, keep, 0] += 1 / 64.0
+    for sign in (1.0, -1.0):                        # below 0: the smallest |score| is the largest, made one as well
+        shape = rows if sign > 0 else torch.where(rows > 0, 3.0 - rows, rows)
+        (k, ks), (v, vs) = (pools(x.view(n * width, 1, P, dh), cache) for x in (shape, vals))
+        kd, vd = R.values(k, ks).view(n, -1, dh), R.values(v, vs).view(n, -1, dh)
+        c = paged.PagedCache(k, v, ks, vs)
+        table = torch.arange(n * width, dtype=torch.int32, device=cuda).view(n, width)
+        for e in range(18, 32):
+            for mant in (1.0, 1.3, 1.7):
+                q = torch.zeros((n, G, dh), device=cuda)
+                q[:, :, 0] = sign * mant * 2.0 ** e / 1.4427 * (1 + torch.arange(G, device=cuda) / 64.0)
+                lse = torch.empty((n, G), device=cuda)
+                out = paged.attend(c, q, table, i32(lens, cuda), lse=lse, scale=0.5)
+                for b, L in enumerate(lens):
+                    s = q[b, :, :1].double() * kd[b, :L, 0] * 0.5
+                    top, at = s.max(-1)
+                    assert bool((s.topk(min(2, L), -1).values.diff().abs() > 300).all())   # (the case's own promise)
+                    want = vd[b, at]
+                    err = (out[b].double() - want).abs()
+                    assert bool((err <= 2.0 ** -20 * want.abs()).all()), (sign, e, mant, L, float(err.max()))
+                    assert bool(((lse[b].double() - top).abs() <= 2.0 ** -20 * top.abs()).all()), (sign, e, mant, L)
+    no_error()

@@ -999,19 +999,24 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        // 2^(s fac - m + lift), rounded at each of the three steps. The product as the maximum's was: with a fused one the
+        // largest key's exponent would be the rounding of m, which passes any range for scores of 2^30. The lift last:
+        // lift - m is a multiple of m's last place, so for m of 2^26 the largest weight would be 2^16 instead of 2^14,
+        // which f16 cannot hold.
+        const float less = m[r] == -INFINITY ? 0.f : -m[r];
         const float lifted = CT == kCacheQ8 ? kLift + (float)lift_d : kLift;
-        const float base = m[r] == -INFINITY ? 0.f : lifted - m[r];
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < NT; ++i) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            // (rounded as the maximum was: with a fused product the largest key's exponent would be the rounding of m,
-            // which passes any range for scores of 2^30)
-            float p = ex2(__fadd_rn(__fmul_rn(s[i][2 * r + k], fac[r]), base));
+            float x = __fadd_rn(__fmul_rn(s[i][2 * r + k], fac[r]), less);
+            if constexpr (CT == kCacheF16 || CT == kCacheQ8) x = __fadd_rn(x, lifted);
+            float p = ex2(x);
             if (masked && !((ok >> (8 * i + 2 * c + k)) & 1)) p = 0.f;   // (a factor of 0 makes -inf NaN)
             s[i][2 * r + k] = p;
             l[r] += p;
           }
+        }
       }
 
       // sums of weighted values: a tile's products in fresh accumulators, added
@@ -1269,7 +1274,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
                                                inv);
           });
           if (a.lse && c == 0)
-            a.lse[lse0 + g + 8 * r] = l[r] == 0.f ? -INFINITY : (m[r] - kLift + log2f(l[r])) * 0.693147180559945f;
+            a.lse[lse0 + g + 8 * r] = l[r] == 0.f ? -INFINITY : (m[r] + (log2f(l[r]) - kLift)) * 0.693147180559945f;
         }
       }
       __syncthreads();   // the region is read
@@ -1417,7 +1422,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             store_rows<4>(a.out, a.row_type, a.out_vec, out0 + (long long)h * DH + lane * 4, v, inv);
           }
           if (a.lse && lane == 0)
-            a.lse[lse0 + h] = ll[i] == 0.f ? -INFINITY : (mm[i] - kLift + log2f(ll[i])) * 0.693147180559945f;
+            a.lse[lse0 + h] = ll[i] == 0.f ? -INFINITY : (mm[i] + (log2f(ll[i]) - kLift)) * 0.693147180559945f;
         }
         break;
       }
