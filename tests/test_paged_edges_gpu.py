@@ -77,3 +77,75 @@ def test_attend_far_scores(cuda, cache, G, dh):
                     assert bool((err <= 2.0 ** -20 * want.abs()).all()), (sign, e, mant, L, float(err.max()))
                     assert bool(((lse[b].double() - top).abs() <= 2.0 ** -20 * top.abs()).all()), (sign, e, mant, L)
     no_error()
+
+
+def finite(x):
+    import torch
+    return torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0)
+
+
+@pytest.mark.parametrize("row", ["f32", "bf16"])
+@pytest.mark.parametrize("cache", ["f32", "f16", "bf16", "q8_0"])
+@pytest.mark.parametrize("H,KV,dh,P,lens", [
+    (6, 2, 64, 16, [3, 40, 0, 700]), (12, 1, 128, 16, [1, 20000]), (3, 3, 32, 5, [9, 300, 2000]),
+    (10, 1, 96, 32, [70, 5000])])
+def test_attend_infinities(cuda, row, cache, H, KV, dh, P, lens):
+    """Keys and values with infinities in a live history, against the formula in 64 bits: a key whose score is -inf
+    weighs nothing, one of +inf makes its head NaN, an infinite value of positive weight its column infinite, values of
+    both signs NaN. Over Q8_0 an infinity is a block's scale. What stays finite is held to paged_ref's bounds with the
+    finite keys' scores and values: parts with infinities are summed key by key, at most 512 roundings here, where the
+    bounds have room for 2 (len / 16 + 256)."""
+    import torch
+    from toy_b200 import paged
+    g = torch.Generator(device=cuda).manual_seed(dh)
+    n, G = len(lens), H // KV
+    width = max(-(-x // P) for x in lens)
+    x, y = (torch.randn((n * width, KV, P, dh), generator=g, device=cuda) for _ in range(2))
+    q = (torch.randn((n, H, dh), generator=g, device=cuda)).to(R.TORCH[row])
+    q[:, :, :32] = q[:, :, :32].abs() + 0.5           # block 0: all of one sign, by the head
+    q[:, 1::3, :32] *= -1
+    (k, ks), (v, vs) = (pools(t, cache) for t in (x, y))
+    table = torch.randperm(n * width, generator=g, device=cuda).int().view(n, width)
+    for what in ("minus key", "plus key", "value", "values", "mixed key"):
+        pk, pv, pks, pvs = (None if t is None else t.clone() for t in (k, v, ks, vs))
+        for b, L in enumerate(lens):
+            for at in {L // 3, max(0, L - 1)} if L > 2 else ():
+                page, off = int(table[b, at // P]), at % P
+                if what == "mixed key":               # products of both signs: NaN
+                    if cache == "q8_0":
+                        pk[page, :, off, :2] = torch.tensor([5, -5], dtype=torch.int8, device=cuda)
+                        pk[page, :, off, 2:32] = 3
+                        pks[page, :, off, 0] = math.inf
+                    else:
+                        pk[page, :, off, 0], pk[page, :, off, 1] = math.inf, -math.inf
+                elif "key" in what:
+                    sign = -1 if what == "minus key" else 1
+                    if cache == "q8_0":
+                        pk[page, :, off, :32] = pk[page, :, off, :32].abs().clamp(min=1) * sign
+                        pks[page, :, off, 0] = math.inf
+                    else:
+                        pk[page, :, off, 3] = sign * math.inf
+                else:
+                    sign = -1 if what == "values" and at == L // 3 else 1
+                    if cache == "q8_0":
+                        pv[page, :, off, :32] = pv[page, :, off, :32].abs().clamp(min=1) * sign
+                        pvs[page, :, off, 0] = math.inf
+                    else:
+                        pv[page, :, off, 5] = sign * math.inf
+        lt = i32(lens, cuda)
+        lse = torch.empty((n, H), device=cuda)
+        out = paged.attend(paged.PagedCache(pk, pv, pks, pvs), q, table, lt, lse=lse, scale=0.1)
+        kd, vd = R.values(pk, pks), R.values(pv, pvs)
+        o, l, (absv, _), _ = R.attend(kd, vd, q, table, lens, 0.1)
+        _, _, (_, vmax), ds = R.attend(finite(kd), finite(vd), q, table, lens, 0.1)
+        bo, bl = R.attend_bounds(finite(o), finite(l), (finite(absv), vmax), ds, lt, dh, q.dtype)
+        assert torch.equal(out.isnan(), o.isnan()), what
+        assert torch.equal(out.isinf(), o.isinf()) and torch.equal(out[o.isinf()].double(), o[o.isinf()]), what
+        ok = o.isfinite()
+        assert bool(((out.double() - o).abs()[ok] <= bo[ok]).all()), what
+        assert torch.equal(lse.isfinite(), l.isfinite()), what
+        ok = l.isfinite()
+        assert bool(((lse.double() - l).abs()[ok] <= bl[ok]).all()), what
+        again = paged.attend(paged.PagedCache(pk, pv, pks, pvs), q, table, lt, scale=0.1)
+        assert torch.equal(torch.nan_to_num(again, nan=7.0), torch.nan_to_num(out, nan=7.0))
+    no_error()

@@ -21,7 +21,11 @@
 // planes of 8 bits, 2 when the result is rounded to 16 bits anyway). Rows 8..15
 // of the 16-row operand hold the second plane of rows 0..7 (HT = 8 heads), so
 // two planes cost one instruction; with G > 8 (HT = 16) each plane is one. An
-// f32 cache is split the same way into tf32 hi + lo, q and P too.
+// f32 cache is split the same way into tf32 hi + lo, q and P too. An infinity
+// has no such planes (it meets one that is 0, or of the other sign): heads
+// whose sums are not finite take their CTA's part of the history again in
+// plain f32 (plain_part), so that such keys and values count as the formula
+// says.
 //
 // Split: the work is a list of units (kWarps tiles of TK keys of one request
 // and key head), cut into equal ranges, one per CTA, whatever the lengths. A
@@ -284,6 +288,9 @@ struct Cfg {
   static constexpr int NT = TK / 8;
   static constexpr int OT = DH / 8;                   // 8-column tiles of the output
   static constexpr int R = HT / 8;                    // heads per lane group
+  // weights are kept times 2^14 where they are rounded to f16, so that small
+  // ones keep their bits (the factor is in the sums too and cancels)
+  static constexpr float kLift = CT == kCacheF16 || CT == kCacheQ8 ? 14.f : 0.f;
   static constexpr int KS = 2 * (CT == kCacheF32 ? DH / 16 : DH / 32);   // k steps of q . k
   // register sets of q: planes that do not share an instruction
   static constexpr int QS = CT == kCacheBF16 ? (HT == 8 ? PL - 1 : PL) : (HT == 8 ? 1 : 2);
@@ -395,13 +402,101 @@ struct Cursor {
   int b, jt, t, len;
 };
 
+// Value e of a cache's rows of K (of V) as f32.
+template <int CT>
+__device__ __forceinline__ float load_cache(const PagedKv& kv, bool v, long long e) {
+  const void* p = v ? kv.v : kv.k;
+  if constexpr (CT == kCacheF32) return static_cast<const float*>(p)[e];
+  else if constexpr (CT == kCacheF16) return __half2float(static_cast<const __half*>(p)[e]);
+  else if constexpr (CT == kCacheBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[e]);
+  else return (float)static_cast<const int8_t*>(p)[e] * __half2float(__ushort_as_half((v ? kv.vs : kv.ks)[e / 32]));
+}
+
+// Units t0 .. t1 - 1 of a history in plain f32, by one warp, a head and four
+// keys at a time: the running maximum, the sum of the weights and of the
+// weighted values, to `buf` as the warps' sums are exchanged. For parts that
+// hold infinities or NaN only: keys whose score is -inf weigh 0, and an
+// infinite value of positive weight makes its column infinite. (The sums of
+// the whole part are taken again, by one warp: this is rare, and less of it
+// in the kernel keeps the registers of the rest.)
 template <int CT, int DH, int HT, int PL>
-__global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) paged_attend_kernel(const PagedAttnArgs a) {
+__device__ __noinline__ void plain_part(const PagedAttnArgs& a, int b, int jt, int t0, int t1, float* buf) {
+  using C = Cfg<CT, DH, HT, PL>;
+  constexpr int W = DH / 32;   // columns of a lane: lane, lane + 32, ..
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31, P = a.kv.page_size;
+  const int tiles_h = (a.group + HT - 1) / HT, jh = jt / tiles_h, h0 = (jt - jh * tiles_h) * HT;
+  const int* pages = a.table + b * a.table_stride;
+  const long long len = min((long long)a.width * P, (long long)a.lens[b]);
+  const long long begin = (long long)t0 * C::UK, end = min((long long)t1 * C::UK, len);
+#pragma unroll 1
+  for (int h = 0; h < HT; ++h) {
+    float m = -INFINITY, l = 0.f, q[W], o[W];
+    const bool on = h0 + h < a.group;
+    const long long row = b * a.ldq + ((long long)jh * a.group + h0 + h) * DH + lane;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      q[k] = on ? load_row(a.q, a.row_type, row + 32 * k) : 0.f;
+      o[k] = 0.f;
+    }
+#pragma unroll 1
+    for (long long key0 = begin; on && key0 < end; key0 += U) {
+      long long at[U];   // -1: no key
+      float s[U], v[U][W];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int key = (int)(key0 + u), id = key0 + u < end ? pages[key / P] : -1;
+        at[u] = id >= 0 && id < a.kv.n_pages
+                    ? id * a.kv.page_stride + jh * a.kv.head_stride + key % P * a.kv.tok_stride + lane
+                    : -1;
+        s[u] = 0.f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          if (at[u] >= 0) s[u] = fmaf(q[k], load_cache<CT>(a.kv, false, at[u] + 32 * k), s[u]);
+          v[u][k] = at[u] >= 0 ? load_cache<CT>(a.kv, true, at[u] + 32 * k) : 0.f;
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int w = 16; w; w >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+        s[u] = at[u] >= 0 ? s[u] * a.c : -INFINITY;
+        top = fmaxf(top, s[u]);
+      }
+      const float keep = m == -INFINITY ? 0.f : ex2(m - top);
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (int k = 0; k < W; ++k) o[k] *= keep;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float p = ex2(top == -INFINITY ? s[u] : s[u] - top);
+        l += p;
+#pragma unroll
+        for (int k = 0; k < W; ++k) o[k] = fmaf(p, v[u][k], o[k]);
+      }
+    }
+    const float lift = C::kLift == 0.f ? 1.f : 16384.f;
+    const int r = h >> 3, g = h & 7;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const int col = lane + 32 * k, w = col % 32;
+      // the output tile, lane of a group and half of its pair that column `col` belongs to
+      constexpr bool kRuns = CT == kCacheF32 || CT == kCacheQ8;
+      const int i = kRuns ? col / 32 * 4 + w % 4 : col / 8, c = kRuns ? w / 8 : w % 8 / 2, y = kRuns ? w % 8 / 4 : w & 1;
+      buf[((r * (C::OT / 2) + i / 2) * 32 + g * 4 + c) * 4 + (i & 1) * 2 + y] = o[k] * lift;
+    }
+    if (lane < 4) reinterpret_cast<float2*>(buf + C::OT * 2 * C::R * 32)[r * 32 + g * 4 + lane] = make_float2(m, l * lift);
+  }
+}
+
+template <int CT, int DH, int HT, int PL>
+__global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
+    paged_attend_kernel(const __grid_constant__ PagedAttnArgs a) {
   using C = Cfg<CT, DH, HT, PL>;
   constexpr int TK = C::TK, UK = C::UK, NT = C::NT, OT = C::OT, R = C::R, ST = C::ST;
-  // weights are kept times 2^14 where they are rounded to f16, so that small
-  // ones keep their bits (the factor is in the sums too and cancels)
-  constexpr float kLift = CT == kCacheF16 || CT == kCacheQ8 ? 14.f : 0.f;
+  constexpr float kLift = C::kLift;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint64_t valid[kAttnWarps][ST];   // keys of a staged tile that count
   __shared__ int last_flag;
@@ -702,6 +797,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
   // ---- this warp's sums over the current history
   float2 o[OT][R];
   float m[R], l[R], fac[R];
+  float2 l2[CT == kCacheQ8 ? R : 1];   // Q8_0: the sums of the weights in pairs, NaN once a score was not finite
   // Q8_0: the weights carry 2^lift_d, near 1 / the largest |V scale| so far, so that their products with the scales
   // fill the f16 range (the factor is in l too and cancels)
   int lift_d = 0;
@@ -817,6 +913,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       for (int r = 0; r < R; ++r) o[i][r] = make_float2(0.f, 0.f);
     have_d = false;
     lift_d = 0;
+    if constexpr (CT == kCacheQ8)
+      for (int r = 0; r < R; ++r) l2[r] = make_float2(0.f, 0.f);
     const uint32_t qb = smem_u32(region) + lane * 16, qh = smem_u32(region) + C::KS * 512 + lane * 8;
     auto q_at = [&](int p, int st) {   // register set p of step st
       if (C::kHalf && p == 1) {
@@ -935,6 +1033,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       // running maximum and weights: m = factor * the largest raw score
       constexpr uint64_t kAll = TK == 64 ? ~0ull : ((1ull << (TK & 63)) - 1);
       const bool masked = (ok & kAll) != kAll;
+      // (a Q8_0 block of infinite scale makes a score of -inf where the formula may have NaN: the sum of the weights
+      // becomes NaN, which sends the part to plain_part; masked rows are zeros here)
+      if constexpr (CT == kCacheQ8) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            l2[r] = fma2(make_float2(s[i][2 * r], s[i][2 * r + 1]), make_float2(0.f, 0.f), l2[r]);
+      }
       if (masked) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -988,7 +1095,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
           shrink[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx[r]);
           m[r] = mx[r];
           if constexpr (CT == kCacheQ8) shrink[r] *= ex2((float)(new_lift - (have_d ? lift_d : new_lift)));
-          l[r] *= shrink[r];
+          if constexpr (CT == kCacheQ8) l2[r] = mul2(l2[r], make_float2(shrink[r], shrink[r]));
+          else l[r] *= shrink[r];
         }
         lift_d = new_lift;
         have_d = true;
@@ -1014,8 +1122,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
             float p = ex2(x);
             if (masked && !((ok >> (8 * i + 2 * c + k)) & 1)) p = 0.f;   // (a factor of 0 makes -inf NaN)
             s[i][2 * r + k] = p;
-            l[r] += p;
+            if constexpr (CT != kCacheQ8) l[r] += p;
           }
+          if constexpr (CT == kCacheQ8) l2[r] = add2(l2[r], make_float2(s[i][2 * r], s[i][2 * r + 1]));
         }
       }
 
@@ -1185,7 +1294,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
       const float back = ex2(-(float)lift_d);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        l[r] *= back;
+        l[r] = (l2[r].x + l2[r].y) * back;
 #pragma unroll
         for (int i = 0; i < OT; ++i) ov[i][r] = mul2(ov[i][r], make_float2(back, back));
       }
@@ -1240,6 +1349,37 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC) pag
         __syncthreads();
         if (warp == 0) add(buf);
         __syncthreads();
+      }
+    }
+    if (warp == 0) {   // heads whose sums are not finite (a product with 0 is NaN then)
+      bool odd[R], any = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float2 zero = make_float2(l[r] * 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < OT; ++i) zero = fma2(ov[i][r], make_float2(0.f, 0.f), zero);
+        float z = zero.x + zero.y;
+        z += __shfl_xor_sync(0xffffffffu, z, 1);
+        z += __shfl_xor_sync(0xffffffffu, z, 2);
+        odd[r] = z != 0.f;
+        any |= odd[r];
+      }
+      if (__any_sync(0xffffffffu, any)) {
+        plain_part<CT, DH, HT, PL>(a, cur.b, cur.jt, t0, t1, buf);
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (!odd[r]) continue;
+          const float2 ml = reinterpret_cast<const float2*>(buf + OT * 2 * R * 32)[r * 32 + lane];
+          m[r] = ml.x;
+          l[r] = ml.y;
+#pragma unroll
+          for (int i = 0; i < OT; i += 2) {
+            const float4 y = reinterpret_cast<const float4*>(buf)[(r * (OT / 2) + i / 2) * 32 + lane];
+            ov[i][r] = make_float2(y.x, y.y);
+            ov[i + 1][r] = make_float2(y.z, y.w);
+          }
+        }
       }
     }
 
