@@ -275,11 +275,11 @@ int tb2_paged_plan(const tb2_paged_plan_args *args, void *stream);
 /* Finished requests give their pages back: for every b with done[b] != 0, in
  * order, the pages table[b][0 .. ceil(lens[b] / page_size)) are pushed on the
  * stack (the first page first), their table entries become -1 and lens_out[b]
- * = 0; other lengths are copied. state_out = {pages on the stack, status, 0,
- * pages pushed}; status 1: the stack would pass n_free entries; 4: a negative
- * length, one past its table row, or a stack count outside [0, n_free]; with
- * either nothing is changed. In place as tb2_paged_plan. n_req is at most
- * 16384. */
+ * = 0; other lengths are copied. An entry that is no page is cleared too, but
+ * not pushed. state_out = {pages on the stack, status, 0, pages pushed};
+ * status 1: the stack could pass n_free entries; 4: a negative length, one
+ * past its table row, or a stack count outside [0, n_free]; with either
+ * nothing is changed. In place as tb2_paged_plan. n_req is at most 16384. */
 typedef struct tb2_paged_release_args {
   const int *lens, *done;
   int n_req;

@@ -149,3 +149,49 @@ def test_attend_infinities(cuda, row, cache, H, KV, dh, P, lens):
         again = paged.attend(paged.PagedCache(pk, pv, pks, pvs), q, table, lt, scale=0.1)
         assert torch.equal(torch.nan_to_num(again, nan=7.0), torch.nan_to_num(out, nan=7.0))
     no_error()
+
+
+# ------------------------------------------------------------------ release
+@pytest.mark.parametrize("n,P,width", [(1, 16, 3), (40, 8, 5), (300, 4, 24), (900, 16, 40), (16384, 4, 2)])
+@pytest.mark.parametrize("share", [0.02, 0.5, 1.0])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_release_bad_pages(cuda, n, P, width, share, in_place):
+    """Table entries that are no page are cleared and reported, and do not reach the stack; the others do, in order."""
+    import random
+    from toy_b200 import paged
+    from toy_b200._lib import lib
+    r = random.Random(n * 7 + int(share * 100))
+    lens = [r.choice([0, 1, r.randrange(0, width * P + 1), width * P]) for _ in range(n)]
+    lens[0] = width * P
+    done = [int(r.random() < 0.7) for _ in range(n)]
+    done[0] = 1
+    n_pages = n * width + 1
+    held = [-(-x // P) for x in lens]
+    ids = r.sample(range(n_pages), sum(held))
+    table, at, bad = [], 0, 0
+    for b in range(n):
+        row = ids[at:at + held[b]]
+        at += held[b]
+        for i in range(held[b]):
+            if done[b] and (r.random() < share or (b == 0 and i == 1)):
+                row[i] = r.choice([-1, n_pages, 2 ** 31 - 1, -2 ** 31])
+                bad += 1
+        table.append(row + [-3] * (width - held[b]))
+    free = [5, 6]
+    cap = free + [-9] * (n_pages - len(free))
+    want = list(free)
+    for b in range(n):
+        if done[b]:
+            want += [p for p in table[b][:held[b]] if 0 <= p < n_pages]
+    L, D, T, F, S = i32(lens, cuda), i32(done, cuda), i32(table, cuda), i32(cap, cuda), i32([len(free), 9, 9, 9], cuda)
+    Lo, So = (L, S) if in_place else (i32([5] * n, cuda), i32([5] * 4, cuda))
+    paged.release(L, D, T, F, S, page_size=P, n_pages=n_pages, lens_out=Lo, state_out=So)
+    if len(free) + sum(h for h, d in zip(held, done) if d) > len(cap):     # the stack could pass its end: nothing done
+        assert So.tolist() == [len(free), 1, 0, 0] and F.tolist() == cap and T.tolist() == table
+        return no_error()
+    assert bad and lib().tb2_device_error() == 0x5001
+    assert So.tolist() == [len(want), 0, 0, len(want) - len(free)]
+    assert F[:len(want)].tolist() == want
+    assert Lo.tolist() == [0 if d else x for x, d in zip(lens, done)]
+    assert T.tolist() == [[-1] * h + row[h:] if d else row for row, h, d in zip(table, held, done)]
+    no_error()

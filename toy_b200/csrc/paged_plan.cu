@@ -18,7 +18,8 @@
 // Lengths and the stack's count may be updated in place: a single CTA writes
 // them after its own reads; a larger grid leaves that to a second, tiny
 // kernel. Measured on one B200: 5.0 us for 16 requests, 8.4 us for 524288 slots
-// of 1024 requests (8.4 MB written).
+// of 1024 requests (8.4 MB written). The return of pages is filled the same
+// way: 3.5 us for 16 requests, 6.9 us for 33000 pages of 1024.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -227,12 +228,40 @@ __global__ void paged_plan_commit_kernel(const tb2_paged_plan_args a) {
   if (b == 0) a.state_out[0] = a.state[0] - a.state_out[3];
 }
 
-__global__ void __launch_bounds__(kThreads) paged_release_kernel(const tb2_paged_release_args a, int in_place, int* err) {
+// Takes the entries below 0 out of x[0 .. n), in place and in order, by one
+// CTA; returns how many are left.
+__device__ int drop_negative(int* x, int n) {
+  __shared__ int wc[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  int kept = 0;
+  for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+    const int i = i0 + tid, v = i < n ? x[i] : -1;
+    const unsigned on = __ballot_sync(0xffffffffu, v >= 0);
+    if (lane == 0) wc[warp] = __popc(on);
+    __syncthreads();   // (and every entry of the round is read)
+    int at = kept, round = 0;
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) at += wc[w];
+      round += wc[w];
+    }
+    if (v >= 0) x[at + __popc(on & ((1u << lane) - 1))] = v;
+    kept += round;
+    __syncthreads();   // the counts are read
+  }
+  return kept;
+}
+
+// Pages go on the stack in the order of their numbers; an entry that is no page
+// goes there as -1 and is taken out again (rarely: it is an error), by this
+// kernel's only CTA or, counted in state_out[2], by the commit kernel.
+__global__ void __launch_bounds__(kThreads) paged_release_kernel(const tb2_paged_release_args a, int* err) {
   extern __shared__ int sm[];
+  __shared__ int none;   // entries that are no page, of a single CTA
   const int P = a.page_size, n = a.n_req;
   int* gone = sm;   // requests that are done, counted like tokens
   int* cu_pg = sm + n + 1;
   griddep_wait_release();
+  if (threadIdx.x == 0) none = 0;
   const int count = a.state[0];
   int bad = 0;
   for (int b = threadIdx.x; b < n; b += blockDim.x) {
@@ -247,34 +276,57 @@ __global__ void __launch_bounds__(kThreads) paged_release_kernel(const tb2_paged
   int status = tot.bad;
   if (count < 0 || count > a.n_free) status = 4;
   else if (!status && tot.pages > a.n_free - count) status = 1;
-  const int pages = status ? 0 : (int)tot.pages;
+  int pages = status ? 0 : (int)tot.pages;
   const int step = gridDim.x * blockDim.x;
+  const bool alone = gridDim.x == 1;
   for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < pages; i += step) {
     const int b = find_request(cu_pg, n, i);
     int* e = a.table + b * a.table_stride + (i - cu_pg[b]);
-    const int page = *e;
-    if (page < 0 || page >= a.n_pages) *err = kErrPagedPage;
+    int page = *e;
+    if (page < 0 || page >= a.n_pages) {
+      *err = kErrPagedPage;
+      atomicAdd(alone ? &none : a.state_out + 2, 1);
+      page = -1;
+    }
     a.free_pages[count + i] = page;
     *e = -1;
   }
-  const bool alone = gridDim.x == 1;
-  if (blockIdx.x == 0 && (alone || !in_place)) {
-    // (a length is read and written by one thread, and read by no other CTA after the first barrier of this one)
+  if (alone) {
+    __syncthreads();
+    if (none) pages = drop_negative(a.free_pages + count, pages);
+    // (a length is read and written by one thread after the first barrier)
     for (int b = threadIdx.x; b < n; b += blockDim.x) a.lens_out[b] = !status && gone[b + 1] > gone[b] ? 0 : a.lens[b];
-    if (threadIdx.x == 0) a.state_out[0] = count + pages;
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (alone) {
+      a.state_out[0] = count + pages;
+      a.state_out[2] = 0;
+    }
     a.state_out[1] = status;
-    a.state_out[2] = 0;
     a.state_out[3] = pages;
   }
 }
 
-__global__ void paged_release_commit_kernel(const tb2_paged_release_args a) {
+// Before a release on more than one CTA: its count of entries that are no page.
+__global__ void paged_release_begin_kernel(const tb2_paged_release_args a) {
+  griddep_wait_release();
+  if (threadIdx.x == 0) a.state_out[2] = 0;
+}
+
+// And after it: the lengths, the stack's count, and the stack without such entries.
+__global__ void __launch_bounds__(256) paged_release_commit_kernel(const tb2_paged_release_args a) {
   griddep_wait_release();
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b < a.n_req) a.lens_out[b] = !a.state_out[1] && a.done[b] ? 0 : a.lens[b];
-  if (b == 0) a.state_out[0] = a.state[0] + a.state_out[3];
+  if (blockIdx.x) return;
+  const int count = a.state[0];
+  int pages = a.state_out[3];
+  if (a.state_out[2]) pages = drop_negative(a.free_pages + count, pages);
+  __syncthreads();   // the state is read
+  if (threadIdx.x) return;
+  a.state_out[0] = count + pages;
+  a.state_out[2] = 0;
+  a.state_out[3] = pages;
 }
 
 int smem_setup(int) {
@@ -314,12 +366,10 @@ int paged_release_launch(const tb2_paged_release_args& a, int* err, cudaStream_t
   if (setup.ensure(smem_setup)) return -3;
   const size_t smem = 2 * (size_t)(a.n_req + 1) * sizeof(int);
   const long long items = (long long)a.n_req * a.table_width;   // (at most: the lengths are on the device)
-  const int grid = grid_for(items / 4);
-  const int in_place = placed(a.lens, a.lens_out, a.n_req) || placed(a.state, a.state_out, 4);
-  if (launch_pdl(paged_release_kernel, dim3(grid), dim3(threads_for(a.n_req, items)), smem, st, a, in_place, err))
-    return -3;
-  if (grid == 1 || !in_place) return 0;
-  return launch_pdl(paged_release_commit_kernel, dim3((a.n_req + 255) / 256), dim3(256), 0, st, a);
+  const int grid = grid_for(items / 4), threads = threads_for(a.n_req, items);
+  if (grid > 1 && launch_pdl(paged_release_begin_kernel, dim3(1), dim3(32), 0, st, a)) return -3;
+  if (launch_pdl(paged_release_kernel, dim3(grid), dim3(threads), smem, st, a, err)) return -3;
+  return grid == 1 ? 0 : launch_pdl(paged_release_commit_kernel, dim3((a.n_req + 255) / 256), dim3(256), 0, st, a);
 }
 
 }  // namespace tb2
