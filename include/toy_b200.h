@@ -236,7 +236,8 @@ typedef struct tb2_paged_kv {
 } tb2_paged_kv;
 
 /* One-time set-up of the paged operators on the current device (the device
- * error word, shared-memory limits); call it before capturing any of them. */
+ * error word, every kernel loaded and its shared-memory limit set; 15 ms and
+ * 8 MB the first time); call it before capturing any of them. */
 int tb2_paged_prepare(void);
 
 /* Pages for a step's new tokens. Request b holds lens[b] tokens in the pages

@@ -195,3 +195,61 @@ def test_release_bad_pages(cuda, n, P, width, share, in_place):
     assert Lo.tolist() == [0 if d else x for x, d in zip(lens, done)]
     assert T.tolist() == [[-1] * h + row[h:] if d else row for row, h, d in zip(table, held, done)]
     no_error()
+
+
+# ------------------------------------------------------------------ set-up
+FIRST_CALLS = """
+import ctypes, sys, time
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import paged_ref as R
+from toy_b200 import paged
+from toy_b200._lib import lib
+dev = torch.device("cuda:0")
+g = torch.Generator(device=dev).manual_seed(0)
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+H, KV, dh, P, n = {H}, {KV}, {dh}, 16, 3
+k, v, ks, vs = R.make_pools(12, KV, P, dh, {cache!r}, "heads", g, dev)
+qkv = torch.randn((n, (H + 2 * KV) * dh), generator=g, device=dev).to(R.TORCH[{row!r}])
+q, kn, vn = (qkv[:, a * dh:b * dh].view(n, b - a, dh) for a, b in ((0, H), (H, H + KV), (H + KV, H + 2 * KV)))
+lens, add, done = i32([0, 20, 5]), i32([1, 1, 1]), i32([1, 1, 1])
+table = torch.full((n, 4), -1, dtype=torch.int32, device=dev)
+table[1, :2], table[2, 0] = i32([7, 3]), 9
+free, state = i32([0, 1, 2, 4, 5, 6, 8, 10, 11, 0, 0, 0]), i32([9, 0, 0, 0])
+e = lambda m, t=torch.int32: torch.empty(m, dtype=t, device=dev)
+out = paged.Plan(e(n), e(4), e(n + 1), e(n, torch.int64), e(n), e(n))
+o, qo, tab2, free2, after = torch.empty_like(q.contiguous()), torch.empty_like(q.contiguous()), e((n, 4)), e(12), e(4)
+c = paged.PagedCache(k, v, ks, vs)
+ws = paged.attend_workspace(dev)
+lse = torch.empty((n, H), device=dev)
+torch.cuda.synchronize()
+gr = torch.cuda.CUDAGraph()
+with torch.cuda.graph(gr):
+    p = paged.plan(lens, add, table, free, state, page_size=P, n_pages=12, n_tokens=n, out=out)
+    paged.append(c, p.slots, kn, vn, q=q, q_out=qo)
+    paged.attend(c, qo, table, p.lens, out=o, lse=lse, workspace=ws)
+    tab2.copy_(table)
+    free2.copy_(free)
+    paged.release(p.lens, done, tab2, free2, p.state, page_size=P, n_pages=12, lens_out=e(n), state_out=after)
+gr.replay()
+torch.cuda.synchronize()
+assert out.lens.tolist() == [1, 21, 6] and out.state.tolist() == [8, 0, 3, 1]
+assert out.slots.tolist() == [11 * P, 3 * P + 4, 9 * P + 5]
+assert after.tolist() == [12, 0, 0, 4] and free2.tolist()[8:] == [11, 7, 3, 9]
+w, _, sums, ds = R.attend(R.values(k, ks), R.values(v, vs), q, table, [1, 21, 6], dh ** -0.5)
+b, _ = R.attend_bounds(w, w[..., 0], sums, ds, out.lens, dh, q.dtype)
+assert bool(((o.double() - w).abs() <= b).all()), float((o.double() - w).abs().max())
+assert lib().tb2_device_error() == 0
+print("captured first")
+"""
+
+
+@pytest.mark.parametrize("H,KV,dh,row,cache", [(4, 2, 128, "bf16", "bf16"), (12, 1, 96, "f32", "q8_0")])
+def test_first_calls_in_a_capture(cuda, H, KV, dh, row, cache):
+    """A process whose first calls of the operators are captured: tb2_paged_prepare (PagedCache calls it) has loaded
+    and set up what they launch."""
+    import subprocess
+    tests = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALLS.format(root=os.path.dirname(tests), tests=tests, H=H, KV=KV, dh=dh, row=row, cache=cache)
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "captured first" in p.stdout, p.stderr[-2000:]

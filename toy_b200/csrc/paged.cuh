@@ -78,6 +78,10 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Kernels loaded and set up on the current device, so that a first launch may be captured into a graph.
+int paged_plan_prepare();
+int paged_append_prepare();
+
 // Launches behind the C entries (arguments already checked).
 int paged_plan_launch(const tb2_paged_plan_args& a, int* err, cudaStream_t st);
 int paged_release_launch(const tb2_paged_release_args& a, int* err, cudaStream_t st);

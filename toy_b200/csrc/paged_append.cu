@@ -268,6 +268,18 @@ int launch(const tb2_paged_kv& c, const tb2_paged_append_args& a, int* err, cuda
 }
 
 template <class T>
+int load_kernels() {   // (asking for its attributes loads a kernel)
+  cudaFuncAttributes at;
+  return cudaFuncGetAttributes(&at, paged_append_kernel<T, float>) == cudaSuccess &&
+                 cudaFuncGetAttributes(&at, paged_append_kernel<T, __half>) == cudaSuccess &&
+                 cudaFuncGetAttributes(&at, paged_append_kernel<T, __nv_bfloat16>) == cudaSuccess &&
+                 cudaFuncGetAttributes(&at, paged_append_kernel<T, int8_t>) == cudaSuccess &&
+                 cudaFuncGetAttributes(&at, paged_append_96_kernel<T>) == cudaSuccess
+             ? 0
+             : -3;
+}
+
+template <class T>
 int launch_cache(const tb2_paged_kv& c, const tb2_paged_append_args& a, int* err, cudaStream_t st) {
   switch (c.kv_type) {
     case kTypeF32: return launch<T, float>(c, a, err, st);
@@ -278,6 +290,12 @@ int launch_cache(const tb2_paged_kv& c, const tb2_paged_append_args& a, int* err
 }
 
 }  // namespace
+
+int paged_append_prepare() {
+  static DeviceOnce setup;
+  return setup.ensure(
+      [](int) { return load_kernels<float>() || load_kernels<__half>() || load_kernels<__nv_bfloat16>() ? -3 : 0; });
+}
 
 int paged_append_launch(const tb2_paged_kv& c, const tb2_paged_append_args& a, int* err, cudaStream_t st) {
   switch (a.row_type) {

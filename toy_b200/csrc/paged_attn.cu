@@ -73,6 +73,10 @@ int tb2_paged_attend(const tb2_paged_kv* kv, const tb2_paged_attend_args* a, voi
   return tb2::paged_attend_launch(*kv, *a, err, static_cast<cudaStream_t>(stream));
 }
 
-int tb2_paged_prepare(void) { return tb2::device_error_word() ? 0 : -3; }
+int tb2_paged_prepare(void) {
+  using namespace tb2;
+  if (!device_error_word() || paged_plan_prepare() || paged_append_prepare()) return -3;
+  return paged_prepare_f32() || paged_prepare_f16() || paged_prepare_bf16() || paged_prepare_q8() ? -3 : 0;
+}
 
 }  // extern "C"

@@ -1575,20 +1575,36 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
   cp_wait<0>();
 }
 
+// The kernel's shared memory on the current device.
+template <int CT, int DH, int HT, int PL>
+int prepare_one() {
+  static DeviceOnce setup;
+  return setup.ensure([](int) {
+    return cudaFuncSetAttribute(paged_attend_kernel<CT, DH, HT, PL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Cfg<CT, DH, HT, PL>::kSmem) == cudaSuccess
+               ? 0
+               : -3;
+  });
+}
+
 template <int CT, int DH, int HT, int PL>
 int launch_one(const PagedAttnArgs& a, cudaStream_t st) {
   using C = Cfg<CT, DH, HT, PL>;
-  auto* k = paged_attend_kernel<CT, DH, HT, PL>;
-  static DeviceOnce setup;
-  if (setup.ensure([&](int) {
-        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) == cudaSuccess ? 0 : -3;
-      }))
-    return -3;
+  if (prepare_one<CT, DH, HT, PL>()) return -3;
   const long long most = (long long)a.width * a.kv.page_size;
   const long long units =
       (long long)a.n_req * a.kv.n_kv * ((a.group + HT - 1) / HT) * ((most + C::UK - 1) / C::UK);
   const int grid = (int)std::max<long long>(1, std::min<long long>(C::OCC * 148, units));
-  return launch_pdl(k, dim3(grid), dim3(kAttnWarps * 32), C::kSmem, st, a);
+  return launch_pdl(paged_attend_kernel<CT, DH, HT, PL>, dim3(grid), dim3(kAttnWarps * 32), C::kSmem, st, a);
+}
+
+template <int CT, int PL>
+int prepare_type() {
+  if (prepare_one<CT, 32, 8, PL>() || prepare_one<CT, 32, 16, PL>() || prepare_one<CT, 64, 8, PL>() ||
+      prepare_one<CT, 64, 16, PL>() || prepare_one<CT, 96, 8, PL>() || prepare_one<CT, 96, 16, PL>() ||
+      prepare_one<CT, 128, 8, PL>() || prepare_one<CT, 128, 16, PL>())
+    return -3;
+  return 0;
 }
 
 template <int CT, int PL>
@@ -1608,5 +1624,9 @@ int paged_attend_f32(const PagedAttnArgs& a, cudaStream_t st);
 int paged_attend_f16(const PagedAttnArgs& a, cudaStream_t st);
 int paged_attend_bf16(const PagedAttnArgs& a, cudaStream_t st);
 int paged_attend_q8(const PagedAttnArgs& a, cudaStream_t st);
+int paged_prepare_f32();
+int paged_prepare_f16();
+int paged_prepare_bf16();
+int paged_prepare_q8();
 
 }  // namespace tb2

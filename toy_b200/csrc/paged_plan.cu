@@ -331,7 +331,11 @@ __global__ void __launch_bounds__(256) paged_release_commit_kernel(const tb2_pag
 
 int smem_setup(int) {
   const int bytes = 3 * (kMaxReq + 1) * (int)sizeof(int);
-  if (cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+  cudaFuncAttributes at;   // (asking for them loads a kernel)
+  if (cudaFuncGetAttributes(&at, paged_plan_commit_kernel) != cudaSuccess ||
+      cudaFuncGetAttributes(&at, paged_release_begin_kernel) != cudaSuccess ||
+      cudaFuncGetAttributes(&at, paged_release_commit_kernel) != cudaSuccess ||
+      cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return -3;
   return cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
              ? 0
@@ -349,9 +353,13 @@ int placed(const int* x, const int* y, long long n) { return x == y ? 1 : x < y 
 
 }  // namespace
 
-int paged_plan_launch(const tb2_paged_plan_args& a, int* err, cudaStream_t st) {
+int paged_plan_prepare() {
   static DeviceOnce setup;
-  if (setup.ensure(smem_setup)) return -3;
+  return setup.ensure(smem_setup);
+}
+
+int paged_plan_launch(const tb2_paged_plan_args& a, int* err, cudaStream_t st) {
+  if (paged_plan_prepare()) return -3;
   const size_t smem = 3 * (size_t)(a.n_req + 1) * sizeof(int);
   const long long items = ((long long)a.n_tokens + kRun - 1) / kRun;
   const int grid = grid_for(items);
@@ -362,8 +370,7 @@ int paged_plan_launch(const tb2_paged_plan_args& a, int* err, cudaStream_t st) {
 }
 
 int paged_release_launch(const tb2_paged_release_args& a, int* err, cudaStream_t st) {
-  static DeviceOnce setup;
-  if (setup.ensure(smem_setup)) return -3;
+  if (paged_plan_prepare()) return -3;
   const size_t smem = 2 * (size_t)(a.n_req + 1) * sizeof(int);
   const long long items = (long long)a.n_req * a.table_width;   // (at most: the lengths are on the device)
   const int grid = grid_for(items / 4), threads = threads_for(a.n_req, items);
