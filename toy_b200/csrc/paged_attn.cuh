@@ -1445,6 +1445,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
       // of their number, by the CTA that completes a group, then the groups. 55 pieces (one request of 16384 tokens, 32 /
       // 8 heads of 128): 26.2 us in groups, 29.5 at once; 32 pieces (4096): 15.3 and 15.0; 16 pieces: 13.2 and 11.9.
       constexpr int kFew = 32;
+      static_assert(kFew <= 32 && kAttnMaxCtas <= 32 * 32, "at most 32 pieces, or groups, are added up at a time: a lane to each");
       int group = 1;
       while (group * group < pieces) ++group;
       if (pieces <= kFew) group = pieces;
@@ -1465,70 +1466,54 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
         // HW heads to a warp, a lane for four columns (d_head 128; fewer lanes below), kFly pieces' loads in flight (an
         // L2 read here takes 0.5 us or more, and one after another they were most of the time of a short call)
         constexpr int HW = HT / kAttnWarps, kFly = C::OCC == 3 ? 8 : 4;
-        float mm[HW], ll[HW];
-        float4 x[HW];
+        const int col4 = min(lane, DH / 4 - 1);
+        // this lane's piece (a lane past the end repeats the last one with weight 0), and the first sums
+        const bool on = lane < count;
+        const float* d = slot_of(lead + min(lane, count - 1) * stride) + HT * DH + warp;
+        float mm[HW], ll[HW], f[HW];
 #pragma unroll
         for (int i = 0; i < HW; ++i) {
-          mm[i] = -INFINITY;
-          ll[i] = 0.f;
+          mm[i] = __ldcg(d + i * kAttnWarps);
+          f[i] = __ldcg(d + HT + i * kAttnWarps);
+        }
+        float4 x[HW], y[kFly][HW];
+        auto read = [&](int k0) {
+#pragma unroll
+          for (int k = 0; k < kFly; ++k) {
+            const float4* src =
+                reinterpret_cast<const float4*>(slot_of(lead + min(k0 + k, count - 1) * stride) + warp * DH) + col4;
+#pragma unroll
+            for (int i = 0; i < HW; ++i) y[k][i] = __ldcg(src + i * kAttnWarps * (DH / 4));
+          }
+        };
+        read(0);
+#pragma unroll
+        for (int i = 0; i < HW; ++i) {
+          const float mp = mm[i];
+#pragma unroll
+          for (int w = 16; w; w >>= 1) mm[i] = fmaxf(mm[i], __shfl_xor_sync(0xffffffffu, mm[i], w));
+          // (a piece without a key, or with NaN scores only, has m -inf: its sums count as they are)
+          const float wp = !on ? 0.f : mp == -INFINITY ? 1.f : ex2(mp - mm[i]);
+          ll[i] = on ? f[i] * wp : 0.f;
+          f[i] = wp;
           x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        const int col4 = min(lane, DH / 4 - 1);
-        for (int p0 = 0; p0 < count; p0 += 32) {
-          const int k1 = min(32, count - p0);
-          // this lane's piece of 32 (a lane past the end repeats the last one with weight 0), and the first sums
-          const bool on = lane < k1;
-          const float* d = slot_of(lead + (p0 + min(lane, k1 - 1)) * stride) + HT * DH + warp;
-          float mp[HW], f[HW];
-#pragma unroll
-          for (int i = 0; i < HW; ++i) {
-            mp[i] = __ldcg(d + i * kAttnWarps);
-            f[i] = __ldcg(d + HT + i * kAttnWarps);
-          }
-          float4 y[kFly][HW];
-          auto read = [&](int k0) {
-#pragma unroll
-            for (int k = 0; k < kFly; ++k) {
-              const float4* src =
-                  reinterpret_cast<const float4*>(slot_of(lead + (p0 + min(k0 + k, k1 - 1)) * stride) + warp * DH) + col4;
-#pragma unroll
-              for (int i = 0; i < HW; ++i) y[k][i] = __ldcg(src + i * kAttnWarps * (DH / 4));
-            }
-          };
-          read(0);
-#pragma unroll
-          for (int i = 0; i < HW; ++i) {
-            float top = fmaxf(mm[i], mp[i]);   // (a repeat changes no maximum)
-#pragma unroll
-            for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            // (a piece without a key, or with NaN scores only, has m -inf: its sums count as they are)
-            const float keep = mm[i] == -INFINITY ? 1.f : ex2(mm[i] - top);
-            const float wp = !on ? 0.f : mp[i] == -INFINITY ? 1.f : ex2(mp[i] - top);
-            ll[i] = ll[i] * keep + (on ? f[i] * wp : 0.f);
-            x[i].x *= keep;
-            x[i].y *= keep;
-            x[i].z *= keep;
-            x[i].w *= keep;
-            mm[i] = top;
-            f[i] = wp;
-          }
 #pragma unroll 1
-          for (int k0 = 0;;) {
+        for (int k0 = 0;;) {
 #pragma unroll
-            for (int k = 0; k < kFly; ++k)
+          for (int k = 0; k < kFly; ++k)
 #pragma unroll
-              for (int i = 0; i < HW; ++i) {
-                const float fk = __shfl_sync(0xffffffffu, f[i], (k0 + k) & 31);
-                if (k0 + k >= k1) continue;
-                x[i].x += fk * y[k][i].x;
-                x[i].y += fk * y[k][i].y;
-                x[i].z += fk * y[k][i].z;
-                x[i].w += fk * y[k][i].w;
-              }
-            k0 += kFly;
-            if (k0 >= k1) break;
-            read(k0);
-          }
+            for (int i = 0; i < HW; ++i) {
+              const float fk = __shfl_sync(0xffffffffu, f[i], (k0 + k) & 31);
+              if (k0 + k >= count) continue;
+              x[i].x += fk * y[k][i].x;
+              x[i].y += fk * y[k][i].y;
+              x[i].z += fk * y[k][i].z;
+              x[i].w += fk * y[k][i].w;
+            }
+          k0 += kFly;
+          if (k0 >= count) break;
+          read(k0);
         }
 #pragma unroll
         for (int i = 0; i < HW; ++i)
