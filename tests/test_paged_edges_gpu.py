@@ -253,3 +253,72 @@ def test_first_calls_in_a_capture(cuda, H, KV, dh, row, cache):
     code = FIRST_CALLS.format(root=os.path.dirname(tests), tests=tests, H=H, KV=KV, dh=dh, row=row, cache=cache)
     p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert p.returncode == 0 and "captured first" in p.stdout, p.stderr[-2000:]
+
+
+# ------------------------------------------------------------------ unaligned rows, repeats
+@pytest.mark.parametrize("row", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cache", ["f32", "bf16", "q8_0"])
+@pytest.mark.parametrize("H,KV,dh,P,lens", [
+    (9, 3, 64, 16, [5, 0, 130, 900]), (12, 1, 32, 8, [33, 3000]), (4, 2, 96, 24, [1, 2000, 77]),
+    (20, 2, 128, 16, [64, 9000])])
+def test_attend_unaligned_rows(cuda, row, cache, H, KV, dh, P, lens):
+    """q and out that start at odd elements with odd row strides: the aligned call's results to the bit, nothing around
+    out touched; histories of one CTA and split ones."""
+    import torch
+    from toy_b200 import paged
+    g = torch.Generator(device=cuda).manual_seed(H)
+    n, width = len(lens), max(-(-x // P) for x in lens)
+    k, v, ks, vs = R.make_pools(n * width, KV, P, dh, cache, "heads", g, cuda)
+    c = paged.PagedCache(k, v, ks, vs)
+    table = torch.randperm(n * width, generator=g, device=cuda).int().view(n, width)
+    q = torch.randn((n, H, dh), generator=g, device=cuda).to(R.TORCH[row])
+    lt = i32(lens, cuda)
+    lse, lse2 = torch.empty((n, H), device=cuda), torch.empty((n, H), device=cuda)
+    want = paged.attend(c, q, table, lt, lse=lse)
+    W = H * dh
+    for at, pad in ((1, 2), (3, 1), (7, 5)):
+        qf = torch.zeros(n * (W + pad) + 16, device=cuda, dtype=q.dtype)
+        of = torch.full((n * (W + pad) + 16,), 5.0, device=cuda, dtype=q.dtype)
+        qv = qf.as_strided((n, H, dh), (W + pad, dh, 1), at)
+        ov = of.as_strided((n, H, dh), (W + pad, dh, 1), at)
+        qv.copy_(q)
+        paged.attend(c, qv, table, lt, out=ov, lse=lse2)
+        assert torch.equal(ov, want) and torch.equal(lse2, lse)
+        ov.fill_(5.0)
+        assert bool((of == 5.0).all())
+        # one side aligned, the other not
+        got = paged.attend(c, qv, table, lt)
+        paged.attend(c, q, table, lt, out=ov)
+        assert torch.equal(got, want) and torch.equal(ov, want)
+    no_error()
+
+
+@pytest.mark.parametrize("cache", ["f32", "bf16", "q8_0"])
+@pytest.mark.parametrize("lens,H,KV,dh", [([20000], 32, 8, 128), ([5000, 1, 777, 0, 4096], 9, 3, 64), ([600] * 40, 28, 4, 128)])
+def test_attend_repeats_itself(cuda, cache, lens, H, KV, dh):
+    """The same inputs in new tensors, with another call between and other work on a second stream: the same bits."""
+    import torch
+    from toy_b200 import paged
+    P, n = 16, len(lens)
+    width = max(-(-x // P) for x in lens)
+
+    def state(seed):
+        g = torch.Generator(device=cuda).manual_seed(seed)
+        k, v, ks, vs = R.make_pools(n * width, KV, P, dh, cache, "heads", g, cuda)
+        return (paged.PagedCache(k, v, ks, vs), torch.randn((n, H, dh), generator=g, device=cuda),
+                torch.randperm(n * width, generator=g, device=cuda).int().view(n, width), i32(lens, cuda))
+
+    first = paged.attend(*state(1))
+    ws, busy = paged.attend_workspace(cuda), torch.randn((4096, 4096), device=cuda)
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        a, b = state(1), state(2)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                busy = busy @ busy * 1e-3
+        paged.attend(*b, workspace=ws)
+        got = paged.attend(*a, workspace=ws)
+        torch.cuda.synchronize()
+        assert torch.equal(got, first)
+    no_error()
