@@ -568,10 +568,11 @@ __global__ void __launch_bounds__(kChunk) kv_attn_kernel(const AttnArgs a) {
 }
 
 // A step's slots and positions by sequence (the plan numbers only the sequences
-// that append): sequence b's token is number cu[b] when it has one.
-__global__ void kv_rows_kernel(const int* __restrict__ add, const int* __restrict__ cu,
-                               const long long* __restrict__ slots, const int* __restrict__ positions, int n,
-                               long long* __restrict__ row_slot, int* __restrict__ row_pos) {
+// that append): sequence b's token is number cu[b] when it has one. (What the
+// plan writes is read through the ordinary path: this kernel is launched beside
+// it, and reads marked as constant could come before the wait.)
+__global__ void kv_rows_kernel(const int* add, const int* cu, const long long* slots, const int* positions, int n,
+                               long long* row_slot, int* row_pos) {
   griddep_wait_release();
   const int b = threadIdx.x;
   if (b >= n) return;
