@@ -793,8 +793,11 @@ int tb2_kv_realize_paged(void *sess, int max_T, int n_seq, int kv_type, int page
  * the logits of the token after it computed; -1 leaves sequence b as it is
  * (its row of the logits means nothing). The first call captures the step as a
  * CUDA graph. Returns 0; -1 for a token out of range, a sequence that already
- * holds max_T tokens, or no token at all; -2 without a paged cache; -5 when
- * the pool has too few free pages for the step, which then changed nothing. */
+ * holds max_T tokens, or no token at all; -2 without a paged cache; -3 for a
+ * launch or copy that failed, after which tb2_kv_paged_state has the lengths
+ * and the sequences that were to grow hold undefined rows until they are
+ * released; -5 when the pool has too few free pages for the step, which then
+ * changed nothing. */
 int tb2_kv_decode_paged(void *sess, const long long *tokens, int n_seq, float *logits);
 /* Sequences with done[b] != 0 are emptied and their pages given back. */
 int tb2_kv_release(void *sess, const int *done, int n_seq);

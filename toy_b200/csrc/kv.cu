@@ -766,20 +766,17 @@ class KvEngine {
     if (cudaMemcpyAsync(tok_, host_in_, nb_ * sizeof(int), cudaMemcpyHostToDevice, st_) != cudaSuccess ||
         cudaMemcpyAsync(pg_->add, host_in_ + kMaxSeq, nb_ * sizeof(int), cudaMemcpyHostToDevice, st_) != cudaSuccess)
       return -3;
-    if (!graph_) {   // first step: eager (validates every launch), then captured for replay
-      if (int rc = enqueue()) return rc;
-      if (int rc = capture()) return rc;
-    } else if (cudaGraphLaunch(graph_, st_) != cudaSuccess) {
-      return -3;
-    }
-    if (logits_host && cudaMemcpyAsync(logits_host, logits_, (size_t)nb_ * c.vocab * 4, cudaMemcpyDeviceToHost, st_) !=
-                           cudaSuccess)
-      return -3;
     int state[4] = {0, 0, 0, 0};
-    if (cudaMemcpyAsync(state, pg_->state, sizeof state, cudaMemcpyDeviceToHost, st_) != cudaSuccess) return -3;
-    if (cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    if (int rc = run_paged(state, logits_host)) {
+      // whatever part of the step ran, its plan may have: the GPU's lengths hold
+      follow_lengths();
+      return rc;
+    }
     if (state[1]) return state[1] == 1 ? -5 : -3;   // no room: the plan, and so the step, changed nothing
     for (int b = 0; b < nb_; ++b) pg_->host_len[b] += tokens[b] >= 0;
+    // the first step ran eagerly (which validates every launch) and is captured for replay once it is complete and
+    // counted; where that fails the next step is eager too
+    if (!graph_ && capture()) cudaGetLastError();
     return 0;
   }
 
@@ -830,6 +827,27 @@ class KvEngine {
   int launches() const { return launches_; }
 
  private:
+  // A paged step on the inputs copied in, to its end; `state`: its plan's.
+  int run_paged(int (&state)[4], float* logits_host) {
+    if (!graph_) {
+      if (int rc = enqueue()) return rc;
+    } else if (cudaGraphLaunch(graph_, st_) != cudaSuccess) {
+      return -3;
+    }
+    const size_t bytes = (size_t)nb_ * e_.cfg().vocab * 4;
+    if (logits_host && cudaMemcpyAsync(logits_host, logits_, bytes, cudaMemcpyDeviceToHost, st_) != cudaSuccess) return -3;
+    if (cudaMemcpyAsync(state, pg_->state, sizeof state, cudaMemcpyDeviceToHost, st_) != cudaSuccess) return -3;
+    return cudaStreamSynchronize(st_) == cudaSuccess ? 0 : -3;
+  }
+
+  // The host's record of the lengths, read from the GPU (left as it is where that fails).
+  void follow_lengths() {
+    std::vector<int> lens(nb_);
+    if (cudaStreamSynchronize(st_) == cudaSuccess &&
+        cudaMemcpy(lens.data(), pg_->lens, nb_ * sizeof(int), cudaMemcpyDeviceToHost) == cudaSuccess)
+      pg_->host_len = lens;
+  }
+
   // The step's launches as a graph, for replay.
   int capture() {
     cudaGraph_t g = nullptr;
@@ -841,6 +859,7 @@ class KvEngine {
     }
     const cudaError_t ce = cudaGraphInstantiate(&graph_, g, 0);
     cudaGraphDestroy(g);
+    if (ce != cudaSuccess) graph_ = nullptr;
     return ce == cudaSuccess ? 0 : -3;
   }
 
