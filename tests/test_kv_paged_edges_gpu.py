@@ -1,0 +1,34 @@
+"""The paged decode engine (PagedKVDecoder) in the calls that its other tests do not make."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def engine(n_heads=4, n_kv=2, d_head=32, d_model=128, n_layers=2):
+    from toy_b200 import FromScratch, LlamaConfig, RecipeOptions
+    rec = FromScratch()
+    rec.realize(LlamaConfig(512, d_model, n_heads, n_kv, d_head, 256, n_layers, 1e4, 1e-5),
+                RecipeOptions(t_seq=64, t_batch=1, seed=3))
+    return rec.fs_cache
+
+
+def test_sizes_past_64_bits(cuda):
+    """Pools whose bytes pass 2^64 are refused as those that the GPU cannot hold (here 2^64 itself: 0 when cut)."""
+    from toy_b200._lib import lib
+    eng = engine(n_heads=8, n_kv=8, d_head=128, n_layers=4)
+    for n_pages in (1 << 30, 2 ** 31 - 1):
+        assert lib().tb2_kv_realize_paged(eng.sess, 32, 1, 0, 1 << 20, n_pages) == -3
+
+
+def test_many_pages(cuda):
+    """More free pages than are put on the stack at a time."""
+    from toy_b200.decode import PagedKVDecoder
+    eng = engine()
+    n = (1 << 20) + 3
+    dec = PagedKVDecoder(eng, max_T=8, n_seq=2, n_pages=n, page_size=1, kv_type="q8_0")
+    first = dec.decode_step([5, 6])
+    assert dec.state()[1] == n - 2
+    dec.reset()
+    assert dec.state()[1] == n and np.array_equal(dec.decode_step([5, 6]), first)
+    dec.close()

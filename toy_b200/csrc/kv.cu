@@ -872,6 +872,8 @@ class KvEngine {
       to = static_cast<std::remove_reference_t<decltype(to)>>(m);
       return cudaMemset(m, 0, std::max<size_t>(bytes, 16)) == cudaSuccess;
     };
+    // (past what any GPU holds, and well inside the 64 bits of the sizes below)
+    if ((double)L * p.n_pages * KV * p.page_size * dh * type_bytes(p.type) > 1e15) return -3;
     const size_t rows = (size_t)L * p.n_pages * KV * p.page_size, ws = tb2_paged_attend_workspace();
     if (!get(p.k, rows * dh * type_bytes(p.type)) || !get(p.v, rows * dh * type_bytes(p.type))) return -3;
     if (p.type == kTypeQ8_0 && (!get(p.ks, rows * (dh / 32) * 2) || !get(p.vs, rows * (dh / 32) * 2))) return -3;
@@ -892,12 +894,15 @@ class KvEngine {
   int reset_paged() {
     PagedState& p = *pg_;
     p.host_len.assign(nb_, 0);
-    std::vector<int> ids(p.n_pages);
-    for (int i = 0; i < p.n_pages; ++i) ids[i] = p.n_pages - 1 - i;   // page 0 on top
     const int state[4] = {p.n_pages, 0, 0, 0};
     if (cudaStreamSynchronize(st_) != cudaSuccess) return -3;
-    if (cudaMemcpy(p.free_pages, ids.data(), ids.size() * sizeof(int), cudaMemcpyHostToDevice) != cudaSuccess ||
-        cudaMemcpy(p.state, state, sizeof state, cudaMemcpyHostToDevice) != cudaSuccess ||
+    std::vector<int> ids(std::min(p.n_pages, 1 << 20));   // (a part at a time)
+    for (long long i0 = 0; i0 < p.n_pages; i0 += (long long)ids.size()) {
+      const int n = (int)std::min<long long>(ids.size(), p.n_pages - i0);
+      for (int i = 0; i < n; ++i) ids[i] = (int)(p.n_pages - 1 - (i0 + i));   // page 0 on top
+      if (cudaMemcpy(p.free_pages + i0, ids.data(), n * sizeof(int), cudaMemcpyHostToDevice) != cudaSuccess) return -3;
+    }
+    if (cudaMemcpy(p.state, state, sizeof state, cudaMemcpyHostToDevice) != cudaSuccess ||
         cudaMemset(p.lens, 0, nb_ * sizeof(int)) != cudaSuccess ||
         cudaMemset(p.table, 0xff, (size_t)nb_ * p.width * sizeof(int)) != cudaSuccess)
       return -3;
