@@ -32,3 +32,18 @@ def test_many_pages(cuda):
     dec.reset()
     assert dec.state()[1] == n and np.array_equal(dec.decode_step([5, 6]), first)
     dec.close()
+
+
+def test_release_refusals(cuda):
+    """Sequences that are none are refused; an empty list and repeats are not."""
+    from toy_b200.decode import PagedKVDecoder
+    dec = PagedKVDecoder(engine(), max_T=12, n_seq=3, n_pages=6, page_size=4, kv_type="f32")
+    dec.decode_step([1, 2, 3])
+    for bad in ([-1], [3], [0, -3], [1, 100]):
+        with pytest.raises(ValueError):
+            dec.release(bad)
+        assert dec.state()[0].tolist() == [1, 1, 1]
+    dec.release([])
+    dec.release([1, 1])
+    assert dec.state()[0].tolist() == [1, 0, 1] and dec.state()[1] == 4
+    dec.close()

@@ -89,9 +89,12 @@ class PagedKVDecoder:
         return self._logits.copy()
 
     def release(self, seqs: Sequence[int]) -> None:
-        """Empty these sequences and give their pages back."""
+        """Empty these sequences (0 .. n_seq - 1) and give their pages back."""
+        at = np.asarray(seqs, np.int64).reshape(-1)
+        if ((at < 0) | (at >= self.n_seq)).any():
+            raise ValueError(f"toy_b200: sequences are 0 to {self.n_seq - 1}")
         d = np.zeros(self.n_seq, np.int32)
-        d[np.asarray(seqs, np.int64)] = 1
+        d[at] = 1
         check(lib().tb2_kv_release(self.eng.sess, d.ctypes.data_as(C.POINTER(C.c_int)), self.n_seq), "tb2_kv_release")
 
     def state(self) -> tuple:
