@@ -34,6 +34,44 @@ def test_many_pages(cuda):
     dec.close()
 
 
+def test_generate_again(cuda):
+    """A second call starts anew: its continuations are those of a fresh decoder, whatever the sequences held."""
+    from toy_b200.decode import KVDecoder, PagedKVDecoder
+    eng = engine()
+    calls = [([[3, 1, 4], [1, 5]], 6), ([[9, 2, 6, 5], [3]], 5), ([[3, 1, 4], [1, 5]], 6)]
+    want = []
+    for prompts, n_new in calls:
+        want.append([])
+        for p in prompts:
+            d = KVDecoder(eng, max_T=16, n_seq=1)
+            want[-1].append(d.generate(np.asarray([p]), n_new)[0].tolist())
+            d.close()
+    dec = PagedKVDecoder(eng, max_T=16, n_seq=2, n_pages=8, page_size=4, kv_type="f32")
+    for (prompts, n_new), w in zip(calls, want):
+        assert dec.generate(prompts, n_new) == w
+        assert dec.state()[0].tolist() == [len(p) + n_new - 1 for p in prompts]
+        dec.decode_step([7, -1])                    # and what is appended between calls is gone
+    dec.close()
+
+
+def test_generate_refusals(cuda):
+    """What a call cannot complete is refused before it changes anything."""
+    from toy_b200.decode import PagedKVDecoder
+    dec = PagedKVDecoder(engine(), max_T=12, n_seq=2, n_pages=5, page_size=4, kv_type="f32")
+    dec.decode_step([1, 2])
+    dec.decode_step([3, -1])
+    held = dec.state()[0].tolist()
+    for prompts, n_new, error in (([[1] * 8, [1]], 6, ValueError), ([[1] * 8, [1] * 8], 5, MemoryError),
+                                  ([[1, -1], [1]], 2, ValueError), ([[1, 512], [1]], 2, ValueError),
+                                  ([[1], []], 2, ValueError), ([[1]], 2, ValueError)):
+        with pytest.raises(error):
+            dec.generate(prompts, n_new)
+        assert dec.state()[0].tolist() == held == [2, 1] and dec.state()[1] == 3
+    assert dec.generate([[1], [2]], 0) == [[], []] and dec.state()[0].tolist() == held
+    assert [len(x) for x in dec.generate([[1] * 8, [1] * 4], 5)] == [5, 5]    # 3 + 2 pages: just enough
+    dec.close()
+
+
 def test_release_refusals(cuda):
     """Sequences that are none are refused; an empty list and repeats are not."""
     from toy_b200.decode import PagedKVDecoder

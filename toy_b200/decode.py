@@ -105,10 +105,23 @@ class PagedKVDecoder:
         return lens, free.value
 
     def generate(self, prompts: Sequence[Sequence[int]], n_new: int) -> list:
-        """Greedy continuations of prompts of any lengths (one per sequence, at least a token each) by n_new tokens."""
+        """Greedy continuations of prompts of any lengths (one per sequence, at least a token each) by n_new tokens. The
+        sequences start empty, as KVDecoder.generate starts at position 0, and keep their prompt and continuation (but
+        the last token) when it returns. ValueError or MemoryError, before anything is changed, where max_T or n_pages
+        is too small for that."""
         feed = [list(map(int, p)) for p in prompts]
         if len(feed) != self.n_seq or any(not p for p in feed):
             raise ValueError("toy_b200: one prompt of a token or more per sequence")
+        if any(t < 0 or t >= self.vocab for p in feed for t in p):
+            raise ValueError(f"toy_b200: tokens are 0 to {self.vocab - 1}")
+        if n_new < 1:
+            return [[] for _ in feed]
+        held = [len(p) + n_new - 1 for p in feed]
+        if max(held) > self.max_T:
+            raise ValueError(f"toy_b200: a prompt and {n_new} new tokens pass max_T ({self.max_T})")
+        if sum(-(-h // self.page_size) for h in held) > self.n_pages:
+            raise MemoryError(f"toy_b200: {self.n_pages} pages do not hold the prompts and {n_new} new tokens each")
+        self.reset()
         out = [[] for _ in feed]
         at = [0] * self.n_seq
         while any(len(o) < n_new for o in out):
