@@ -322,3 +322,27 @@ def test_attend_repeats_itself(cuda, cache, lens, H, KV, dh):
         torch.cuda.synchronize()
         assert torch.equal(got, first)
     no_error()
+
+
+# ------------------------------------------------------------------ gradients
+def test_gradients_are_refused(cuda):
+    """An input that requires a gradient would get none: refused, but not under torch.no_grad()."""
+    import torch
+    from toy_b200 import paged
+    k = torch.zeros((4, 2, 16, 64), device=cuda)
+    c = paged.PagedCache(k, k.clone())
+    x = lambda h, g=False: torch.ones((2, h, 64), device=cuda, requires_grad=g)  # noqa: E731
+    table, lens, slots = i32([[0], [1]], cuda), i32([1, 1], cuda), torch.tensor([0, 16], device=cuda)
+    bias = torch.zeros(8 * 64, device=cuda, requires_grad=True)
+    calls = [lambda: paged.attend(c, x(4, True), table, lens), lambda: paged.append(c, slots, x(2, True), x(2)),
+             lambda: paged.append(c, slots, x(2), x(2, True)), lambda: paged.append(c, slots, x(2), x(2), q=x(4, True)),
+             lambda: paged.append(c, slots, x(2), x(2), q=x(4), bias=bias),
+             lambda: paged.attend(c, x(4, True) * 2, table, lens),
+             lambda: paged.attend(c, x(4), table, lens, out=x(4, True))]
+    for f in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            f()
+        with torch.no_grad():
+            f()
+    assert not paged.attend(c, x(4), table, lens).requires_grad
+    no_error()

@@ -9,7 +9,8 @@ call runs on torch's current stream of the tensors' device, synchronises
 nothing and can be captured into a CUDA graph when its outputs are given.
 Arguments that do not fit are refused with ValueError before anything runs.
 What only the device knows (page ids, slots, positions) is checked there: see
-`tb2_device_error` in the header.
+`tb2_device_error` in the header. No gradient passes through these calls: with
+gradients enabled, a tensor that requires one is refused.
 """
 from __future__ import annotations
 
@@ -57,6 +58,12 @@ def _call(index: int, what: str, *args) -> None:
             rc = f(*args, _raw_stream(index))
     if rc:
         check(rc, what)
+
+
+def _wants_grad() -> None:
+    """Refuses a call one of whose tensors requires a gradient, unless gradients are disabled."""
+    if torch.is_grad_enabled():
+        _bad("no gradient passes through this call (use it under torch.no_grad())")
 
 
 def _ints(t: torch.Tensor, n: int, index: int, what: str, dtype=_I32) -> int:
@@ -191,6 +198,9 @@ def append(cache: PagedCache, slots: torch.Tensor, k: torch.Tensor, v: torch.Ten
     n = k.shape[0]
     if dt not in _ROW:
         _bad("rows are f32, f16 or bf16")
+    if k.requires_grad or v.requires_grad or q is not None and q.requires_grad or \
+            bias is not None and bias.requires_grad:
+        _wants_grad()
     ldk, ldv = _rows(k, n, n_kv, dh, dt, dev, "k"), _rows(v, n, n_kv, dh, dt, dev, "v")
     heads = ldq = ldqo = 0
     qp = op = bp = rp = pp = None
@@ -243,6 +253,8 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lens: torch.
     dev, dt = cache.index, q.dtype
     if q.dim() != 3 or dt not in _ROW:
         _bad("q: f32, f16 or bf16 [n, n_heads, d_head]")
+    if q.requires_grad or out is not None and out.requires_grad:
+        _wants_grad()
     n, heads, _ = q.shape
     if heads < 1 or heads % n_kv:
         _bad("n_heads is a multiple of the cache's n_kv")
