@@ -6,6 +6,9 @@
 
 namespace tb2 {
 
+// The factor of a score in powers of two.
+static float scale_log2e(float scale) { return (float)(scale * 1.4426950408889634); }
+
 int paged_attend_launch(const tb2_paged_kv& c, const tb2_paged_attend_args& a, int* err, cudaStream_t st) {
   PagedAttnArgs k;
   k.kv = paged_kv_of(&c);
@@ -20,7 +23,7 @@ int paged_attend_launch(const tb2_paged_kv& c, const tb2_paged_attend_args& a, i
   k.tickets = static_cast<unsigned*>(a.workspace);
   k.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kAttnTicketBytes);
   k.err = err;
-  k.c = (float)(a.scale * 1.4426950408889634);   // log2(e)
+  k.c = scale_log2e(a.scale);
   k.q_vec = aligned(a.q, 16) && (a.ldq * type_bytes(a.row_type)) % 16 == 0;
   k.out_vec = aligned(a.out, 16) && (a.ldo * type_bytes(a.row_type)) % 16 == 0;
   k.n_req = a.n_req;
@@ -66,7 +69,7 @@ int tb2_paged_attend(const tb2_paged_kv* kv, const tb2_paged_attend_args* a, voi
   // (the units of every table row filled, at the smallest unit, are numbered in 31 bits)
   const long long tiles_h = (a->n_heads / kv->n_kv + 7) / 8;
   if ((((long long)a->table_width * kv->page_size + 31) / 32) * kv->n_kv * tiles_h > 0x7fffffffLL / a->n_req) return -1;
-  if (!std::isfinite(a->scale)) return -1;
+  if (!std::isfinite(a->scale) || !std::isfinite(tb2::scale_log2e(a->scale))) return -1;
   if (!a->workspace || a->workspace_bytes < tb2::kAttnWorkspace || !tb2::aligned(a->workspace, 16)) return -1;
   int* err = tb2::device_error_word();
   if (!err) return -3;
