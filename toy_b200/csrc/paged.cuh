@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "toy_b200.h"
 
@@ -25,6 +26,11 @@ constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeQ8_0 = 8, kTypeBF16 = 30;
 inline int type_bytes(int t) { return t == kTypeF32 ? 4 : t == kTypeQ8_0 ? 1 : 2; }
 inline bool row_type_ok(int t) { return t == kTypeF32 || t == kTypeF16 || t == kTypeBF16; }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+inline bool all_aligned(size_t a, std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (!aligned(p, a)) return false;
+  return true;
+}
 
 // Everything the kernels rely on about a descriptor: rows of d_head values
 // (a multiple of 32, at most 128) that start on 16-byte boundaries, pages and

@@ -324,6 +324,7 @@ int tb2_paged_append(const tb2_paged_kv* kv, const tb2_paged_append_args* a, voi
     return -1;
   if (a->rope && (!a->positions || a->rope_rows < 1 || !tb2::aligned(a->rope, 16))) return -1;
   if (a->bias && !tb2::aligned(a->bias, 16)) return -1;
+  if (!tb2::aligned(a->positions, 4) || !tb2::aligned(a->slots, 8)) return -1;
   int* err = tb2::device_error_word();
   if (!err) return -3;
   return tb2::paged_append_launch(*kv, *a, err, static_cast<cudaStream_t>(stream));

@@ -391,6 +391,10 @@ int tb2_paged_plan(const tb2_paged_plan_args* a, void* stream) {
   if (!a->lens || !a->add || !a->table || !a->state || !a->lens_out || !a->state_out || !a->cu_tokens ||
       (a->n_free && !a->free_pages) || (a->n_tokens && (!a->slots || !a->positions || !a->requests)))
     return -1;
+  if (!tb2::all_aligned(4, {a->lens, a->add, a->table, a->free_pages, a->state, a->lens_out, a->state_out, a->cu_tokens,
+                            a->positions, a->requests}) ||
+      !tb2::aligned(a->slots, 8))
+    return -1;
   if (tb2::placed(a->lens, a->lens_out, a->n_req) < 0 || tb2::placed(a->state, a->state_out, 4) < 0) return -1;
   if ((long long)a->table_width * a->page_size > 0x7fffff00LL) return -1;   // positions are 32 bits wide
   int* err = tb2::device_error_word();
@@ -405,6 +409,7 @@ int tb2_paged_release(const tb2_paged_release_args* a, void* stream) {
   if (!a->lens || !a->done || !a->table || !a->state || !a->lens_out || !a->state_out ||
       (a->n_free && !a->free_pages))
     return -1;
+  if (!tb2::all_aligned(4, {a->lens, a->done, a->table, a->free_pages, a->state, a->lens_out, a->state_out})) return -1;
   if (tb2::placed(a->lens, a->lens_out, a->n_req) < 0 || tb2::placed(a->state, a->state_out, 4) < 0) return -1;
   if ((long long)a->table_width * a->page_size > 0x7fffff00LL) return -1;
   int* err = tb2::device_error_word();
