@@ -346,3 +346,23 @@ def test_gradients_are_refused(cuda):
             f()
     assert not paged.attend(c, x(4), table, lens).requires_grad
     no_error()
+
+
+# ------------------------------------------------------------------ operands of an f32 cache
+@pytest.mark.parametrize("H,KV,dh", [(3, 1, 64), (8, 2, 128), (12, 1, 32), (16, 1, 96)])
+def test_attend_f32_values(cuda, H, KV, dh):
+    """A request of one key gives that key's value row: its weight is 1, so all that is lost is what the value's two
+    halves leave out, at most a unit of its last place (2^-23 of it)."""
+    import torch
+    from toy_b200 import paged
+    g = torch.Generator(device=cuda).manual_seed(dh)
+    n = 64
+    k, v, _, _ = R.make_pools(n, KV, 16, dh, "f32", "heads", g, cuda)
+    v *= 10.0 ** torch.randint(-30, 31, v.shape, generator=g, device=cuda)
+    v[0, 0, 0, 0], v[1, 0, 0, 0] = 3.4028234e38, -3.4028234e38       # (the ends of f32: `hi` rounds to infinity)
+    q = torch.randn((n, H, dh), generator=g, device=cuda)
+    out = paged.attend(paged.PagedCache(k, v), q, torch.arange(n, dtype=torch.int32, device=cuda)[:, None],
+                       i32([1] * n, cuda))
+    want = v[:, :, 0].repeat_interleave(H // KV, 1).double()
+    assert bool(((out.double() - want).abs() <= 2.0 ** -23 * want.abs()).all())
+    no_error()

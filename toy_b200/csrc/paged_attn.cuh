@@ -171,15 +171,16 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// An f32 value as two tf32 ones: its leading 11 bits, and the 13 that follow
-// rounded to 11 (at most 2^-23 of the value is left out; cut instead of
-// rounded, the sums of an f32 cache were 5.5e-7 off instead of 3.1e-7).
+// An f32 value as two tf32 ones: rounded to 11 bits, and what is left, which
+// has 12 at most and is cut to 11: no more than a unit of the value's last
+// place is left out (2^-23 of it). NaN may end in `lo` alone (the carry turns
+// its `hi` into a 0), an infinity makes `lo` NaN.
 struct Split {
   uint32_t hi, lo;
 };
 __device__ __forceinline__ Split tf32x2(float x) {
-  const uint32_t hi = __float_as_uint(x) & 0xffffe000u;
-  return {hi, (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u};
+  const uint32_t hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  return {hi, __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u};
 }
 // Two f32 operations in one instruction.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
