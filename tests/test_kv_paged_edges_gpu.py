@@ -85,3 +85,12 @@ def test_release_refusals(cuda):
     dec.release([1, 1])
     assert dec.state()[0].tolist() == [1, 0, 1] and dec.state()[1] == 4
     dec.close()
+
+
+def test_sizes_past_32_bits(cuda):
+    """Sizes that the entry point's 32 bits would cut."""
+    from toy_b200.decode import PagedKVDecoder
+    eng = engine()
+    for kw in (dict(n_pages=2 ** 32 + 4), dict(max_T=2 ** 32 + 4), dict(page_size=2 ** 32 + 4)):
+        with pytest.raises(ValueError):
+            PagedKVDecoder(eng, **{**dict(max_T=8, n_seq=1, n_pages=4, page_size=4), **kw})

@@ -366,3 +366,22 @@ def test_attend_f32_values(cuda, H, KV, dh):
     want = v[:, :, 0].repeat_interleave(H // KV, 1).double()
     assert bool(((out.double() - want).abs() <= 2.0 ** -23 * want.abs()).all())
     no_error()
+
+
+def test_sizes_past_32_bits_are_refused(cuda):
+    """Counts that the entry points' 32 bits would cut are refused (they would have been taken modulo 2^32)."""
+    import torch
+    from toy_b200 import paged
+    big = torch.empty(2 ** 32 + 4, dtype=torch.int32, device=cuda)
+    i, t = i32([0] * 4, cuda), i32([[0, 0]] * 4, cuda)
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged.plan(i, i, t, big, i, page_size=16, n_pages=4, n_tokens=0)
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged.release(i, i, t, big, i, page_size=16, n_pages=4)
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged.plan(big, i, t, i, i, page_size=16, n_pages=4, n_tokens=0)
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged.plan(i[:1], i, big[None, :], i, i, page_size=16, n_pages=4, n_tokens=0)
+    del big
+    torch.cuda.empty_cache()
+    no_error()

@@ -67,6 +67,8 @@ class PagedKVDecoder:
     def __init__(self, engine, max_T: int, n_seq: int, n_pages: int, page_size: int = 16, kv_type: str = "bf16"):
         if kv_type not in _KV_TYPES:
             raise ValueError(f"toy_b200: kv_type is one of {', '.join(_KV_TYPES)}, not {kv_type!r}")
+        if max(max_T, n_seq, n_pages, page_size) >= 2**31:
+            raise ValueError("toy_b200: max_T, n_seq, n_pages and page_size are below 2^31")
         self.eng = engine
         self.max_T, self.n_seq, self.n_pages, self.page_size = max_T, n_seq, n_pages, page_size
         self.vocab = engine.cfg.vocab

@@ -91,6 +91,8 @@ class PagedCache:
             _bad("scales belong to int8 pools, and only there")
         # an axis of size 1 has no stride of its own
         n_pages, n_kv, page, dh = k.shape
+        if max(k.shape) >= 2**31:
+            _bad("k: axes below 2^31")
         strides = [k.stride(i) if k.shape[i] > 1 else k.numel() for i in range(3)]
         if q8:
             for s in (k_scale, v_scale):
@@ -124,9 +126,16 @@ def _table(table: torch.Tensor, n: int, index: int) -> tuple:
         _bad(f"table: int32 [n_req, width] on cuda:{index}")
     rows, width = table.shape
     stride, one = table.stride()
-    if rows < n or width < 1 or (one != 1 and width > 1) or (rows > 1 and stride < width):
-        _bad("table: a contiguous row of at least one page per request")
+    if rows < n or not 0 < width < 2**31 or (one != 1 and width > 1) or (rows > 1 and stride < width):
+        _bad("table: a contiguous row of at least one page, and fewer than 2^31, per request")
     return table.data_ptr(), width, stride if rows > 1 else width
+
+
+def _stack(free_pages: torch.Tensor, index: int) -> tuple:
+    """(pointer, entries) of the stack of free pages."""
+    if free_pages.numel() >= 2**31:   # (the entry points count in 32 bits)
+        _bad("free_pages: fewer than 2^31 entries")
+    return _ints(free_pages, 0, index, "free_pages"), free_pages.numel()
 
 
 def plan(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, state: torch.Tensor, *,
@@ -136,8 +145,8 @@ def plan(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages:
     the sum of add). `out` may hold lens and state themselves. Check state[1] of the result when it reaches the host:
     a status other than 0 left everything as it was."""
     n, dev = lens.numel(), lens.get_device()
-    if dev < 0 or n < 1 or max(page_size, n_pages, n_tokens) >= 2**31 or n_tokens < 0:
-        _bad("lens: on a GPU, of one request or more; page_size, n_pages and n_tokens below 2^31")
+    if dev < 0 or n < 1 or max(n, page_size, n_pages, n_tokens) >= 2**31 or n_tokens < 0:
+        _bad("lens: on a GPU, of one request or more; requests, page_size, n_pages and n_tokens below 2^31")
     tp, width, stride = _table(table, n, dev)
     if out is None:   # two allocations, as each call into torch is a microsecond or more
         slots = lens.new_empty(n_tokens, dtype=_I64)
@@ -153,7 +162,7 @@ def plan(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages:
                 _ints(out.positions, n_tokens, dev, "out.positions"),
                 _ints(out.requests, n_tokens, dev, "out.requests"))
     a = PagedPlanArgs(_ints(lens, n, dev, "lens"), _ints(add, n, dev, "add"), n, tp, width, stride,
-                      _ints(free_pages, 0, dev, "free_pages"), free_pages.numel(), _ints(state, 4, dev, "state"),
+                      *_stack(free_pages, dev), _ints(state, 4, dev, "state"),
                       page_size, n_pages, n_tokens, *outs)
     _call(dev, "tb2_paged_plan", C.byref(a))
     return out
@@ -165,10 +174,10 @@ def release(lens: torch.Tensor, done: torch.Tensor, table: torch.Tensor, free_pa
     """The pages of every request with done[b] != 0 go back on the stack, its table row is cleared and its length set
     to 0; lens and state are updated in place unless other tensors are given."""
     n, dev = lens.numel(), lens.get_device()
-    if dev < 0 or n < 1 or max(page_size, n_pages) >= 2**31:
-        _bad("lens: on a GPU, of one request or more; page_size and n_pages below 2^31")
+    if dev < 0 or n < 1 or max(n, page_size, n_pages) >= 2**31:
+        _bad("lens: on a GPU, of one request or more; requests, page_size and n_pages below 2^31")
     a = PagedReleaseArgs(_ints(lens, n, dev, "lens"), _ints(done, n, dev, "done"), n, *_table(table, n, dev),
-                         _ints(free_pages, 0, dev, "free_pages"), free_pages.numel(), _ints(state, 4, dev, "state"),
+                         *_stack(free_pages, dev), _ints(state, 4, dev, "state"),
                          page_size, n_pages, _ints(lens if lens_out is None else lens_out, n, dev, "lens_out"),
                          _ints(state if state_out is None else state_out, 4, dev, "state_out"))
     _call(dev, "tb2_paged_release", C.byref(a))
@@ -176,9 +185,9 @@ def release(lens: torch.Tensor, done: torch.Tensor, table: torch.Tensor, free_pa
 
 def _rows(t: torch.Tensor, n: int, heads: int, dh: int, dtype, index: int, what: str) -> int:
     """The row stride of t [n, heads, dh], its last two axes dense."""
-    if t.dim() == 3 and t.dtype is dtype and t.get_device() == index:
+    if t.shape == (n, heads, dh) and t.dtype is dtype and t.get_device() == index:
         s0, s1, s2 = t.stride()
-        if t.shape == (n, heads, dh) and s2 == 1 and (s1 == dh or heads == 1):
+        if s2 == 1 and (s1 == dh or heads == 1):
             if n <= 1:
                 return heads * dh
             if s0 >= heads * dh:
@@ -196,8 +205,8 @@ def append(cache: PagedCache, slots: torch.Tensor, k: torch.Tensor, v: torch.Ten
     _, n_kv, _, dh = cache.shape
     dev, dt = cache.index, k.dtype
     n = k.shape[0]
-    if dt not in _ROW:
-        _bad("rows are f32, f16 or bf16")
+    if dt not in _ROW or n >= 2**31:
+        _bad("rows are f32, f16 or bf16, of fewer than 2^31 tokens")
     if k.requires_grad or v.requires_grad or q is not None and q.requires_grad or \
             bias is not None and bias.requires_grad:
         _wants_grad()
@@ -213,10 +222,11 @@ def append(cache: PagedCache, slots: torch.Tensor, k: torch.Tensor, v: torch.Ten
         ldqo = _rows(q_out, n, heads, dh, dt, dev, "q_out")
         qp, op = q.data_ptr(), q_out.data_ptr()
     if rope is not None:
+        rows, *pairs = rope.shape
         if positions is None or rope.dtype is not _F32 or rope.get_device() != dev or not rope.is_contiguous() or \
-                rope.dim() != 3 or rope.shape[1:] != (dh // 2, 2):
+                pairs != [dh // 2, 2]:
             _bad("rope: contiguous f32 [rows, d_head / 2, 2] with positions")
-        rp, rows = rope.data_ptr(), rope.shape[0]
+        rp = rope.data_ptr()
     if positions is not None:
         pp = _ints(positions, n, dev, "positions")
     if bias is not None:
