@@ -335,18 +335,22 @@ int tb2_paged_append(const tb2_paged_kv *kv, const tb2_paged_append_args *args, 
  * gives zeros and lse -inf; lengths past the table row are cut to it. q and
  * out are [n_req][n_heads][d_head] with request strides ldq, ldo, of row_type
  * 0 f32, 1 f16 or 30 bf16, independent of the cache's type; the softmax
- * statistics and sums are f32. Infinities and NaN in the history count as the
- * formula says: a key whose score is -inf weighs 0, an infinite value of
+ * statistics and sums are f32. The products' operands are K and V as stored
+ * and q and the weights within 2^-24 (f16 and Q8_0 caches: or 2^-29 of a row's
+ * largest |q| and 2^-39 of the largest weight, where that is more); over an
+ * f32 cache all four within 2^-23; over a bf16 cache with 16-bit rows q as it
+ * is and the weights within 2^-18. Infinities and NaN in the history count as
+ * the formula says: a key whose score is -inf weighs 0, an infinite value of
  * positive weight makes its column infinite, a score of +inf or NaN makes the
  * head's out and lse NaN (no other head's); a request whose scores are all
  * -inf counts as an empty one. (Such parts of a history are summed key by key,
- * at a hundredth of the usual rate.) The history is split over the GPU and joined
- * in a fixed order, so the same call gives the same bits; another batch, or
- * another table width, may split a request's history elsewhere. out does not
- * overlap q. n_req * n_kv * ceil(n_heads / n_kv / 8) * (tokens a table row
- * spans) is below 2^36. workspace holds tb2_paged_attend_workspace() bytes
- * (16-byte aligned) set up once by tb2_paged_attend_workspace_init; calls that
- * may overlap on the GPU (two streams, two graphs) need one each. */
+ * more than a hundred times slower.) The history is split over the GPU and
+ * joined in a fixed order, so the same call gives the same bits; another
+ * batch, or another table width, may split a request's history elsewhere. out
+ * does not overlap q. n_req * n_kv * ceil(n_heads / n_kv / 8) * (tokens a
+ * table row spans) is below 2^36. workspace holds tb2_paged_attend_workspace()
+ * bytes (16-byte aligned) set up once by tb2_paged_attend_workspace_init;
+ * calls that may overlap on the GPU (two streams, two graphs) need one each. */
 typedef struct tb2_paged_attend_args {
   int n_req, n_heads, row_type;
   const void *q;

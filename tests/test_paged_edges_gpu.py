@@ -385,3 +385,32 @@ def test_sizes_past_32_bits_are_refused(cuda):
     del big
     torch.cuda.empty_cache()
     no_error()
+
+
+@pytest.mark.parametrize("cache", ["f32", "f16", "bf16", "q8_0"])
+@pytest.mark.parametrize("L", [1, 40, 3000])
+def test_attend_all_minus_infinity(cuda, cache, L):
+    """A request whose scores are all -inf counts as an empty one; the heads beside it and the next request do not."""
+    import torch
+    from toy_b200 import paged
+    P, dh, width = 16, 64, -(-3000 // 16)
+    g = torch.Generator(device=cuda).manual_seed(L)
+    k, v, ks, vs = R.make_pools(2 * width, 1, P, dh, cache, "heads", g, cuda)
+    c = paged.PagedCache(k, v, ks, vs)
+    q = torch.randn((2, 5, dh), generator=g, device=cuda)
+    q[:, :2, :32] = q[:, :2, :32].abs() + 0.1
+    table = torch.arange(2 * width, dtype=torch.int32, device=cuda).view(2, width)
+    lens, lse, base = i32([L, 70], cuda), torch.empty((2, 5), device=cuda), torch.empty((2, 5), device=cuda)
+    want = paged.attend(c, q, table, lens, lse=base)
+    if cache == "q8_0":
+        k[:width, 0, :, :32] = -k[:width, 0, :, :32].abs().clamp(min=1)
+        ks[:width, 0, :, 0] = math.inf
+    else:
+        k[:width, 0, :, 0] = -math.inf
+    out = paged.attend(c, q, table, lens, lse=lse)
+    assert bool((out[0, :2] == 0).all()) and bool((lse[0, :2] == -math.inf).all())
+    assert torch.equal(out[1], want[1]) and torch.equal(lse[1], base[1])
+    neg = q[0, :, 0] < 0
+    if cache != "q8_0":                                 # scores of +inf
+        assert bool(out[0, neg].isnan().all()) and bool(lse[0, neg].isnan().all())
+    no_error()

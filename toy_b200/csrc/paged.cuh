@@ -32,10 +32,10 @@ inline bool all_aligned(size_t a, std::initializer_list<const void*> ps) {
   return true;
 }
 
-// Everything the kernels rely on about a descriptor: rows of d_head values
-// (a multiple of 32, at most 128) that start on 16-byte boundaries, pages and
-// heads that do not overlap by their strides, and for Q8_0 strides of whole
-// rows.
+// What a descriptor is checked for: rows of d_head values (a multiple of 32,
+// at most 128) that start on 16-byte boundaries, strides of a row at least, and
+// for Q8_0 of whole rows. (That rows do not overlap is the caller's word:
+// every access stays inside the strides' extent either way.)
 inline bool paged_kv_ok(const tb2_paged_kv* c) {
   if (!c || !c->k || !c->v || c->n_pages < 1 || c->page_size < 1 || c->n_kv < 1) return false;
   if (!row_type_ok(c->kv_type) && c->kv_type != kTypeQ8_0) return false;

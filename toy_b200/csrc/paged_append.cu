@@ -199,7 +199,10 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const PagedKv kv, con
 }
 
 // Q8_0 at d_head 96, whose blocks straddle the halves: one thread per element
-// of a head, q heads, then key heads, each with its value head.
+// of a head, q heads, then key heads, each with its value head. Right for a
+// decode step (16 tokens of 32 / 8 heads 2.7 us, as at d_head 64 and 128), bound
+// by its instructions and small CTAs for a prompt: 16384 tokens 675 us, 0.8
+// TB/s, where the kernel above takes 61 us at d_head 64 and 115 at 128.
 template <class T>
 __global__ void paged_append_96_kernel(const PagedKv kv, const tb2_paged_append_args a, int* err) {
   __shared__ float sh[128];
@@ -259,9 +262,11 @@ int launch(const tb2_paged_kv& c, const tb2_paged_append_args& a, int* err, cuda
     return launch_pdl(paged_append_96_kernel<T>, dim3(a.n_tokens, heads + c.n_kv), dim3(96), 0, st, paged_kv_of(&c), a,
                       err);
   const int items = (heads + 2 * c.n_kv) * (c.d_head / 2 / Row<T>::V);
-  // A decode step has its whole token in one round (250 tokens of 28 / 4 bf16 heads of 128: 3.1 us, 3.8 with 256
-  // threads); a prompt keeps more CTAs on an SM (16384 f32 tokens of 32 / 8 heads of 64 into bf16: 58 us, 6.4 TB/s, with
-  // 256 threads; 62 us with 512).
+  // A decode step has its whole token in one round: 28 / 4 bf16 heads of 128 with 512 (256) threads, 8 tokens 2.2 (2.8)
+  // us, 250 2.6 (3.2), 400 3.5 (3.5), 1000 5.4 (5.6). A prompt keeps more CTAs on an SM: 2000 tokens 11.9 (10.5), 4000
+  // 21.4 (19.0); f32 rows of 32 / 8 heads of 64 into bf16: 250 2.3 (2.8), 400 3.4 (3.0), 1000 4.4 (5.4), 2000 9.7 (9.5),
+  // 16384 61.7 (57.9; 6.4 TB/s). The bound is two such CTAs to an SM; between
+  // 300 and 1500 tokens either is right within a microsecond.
   const int most = a.n_tokens <= 2 * 148 ? 512 : 256;
   const int rounds = (items + most - 1) / most, threads = ((items + rounds - 1) / rounds + 31) / 32 * 32;
   return launch_pdl(paged_append_kernel<T, C>, dim3(a.n_tokens), dim3(threads), 0, st, paged_kv_of(&c), a, err);

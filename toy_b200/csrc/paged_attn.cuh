@@ -39,11 +39,13 @@
 // Measured on one B200 (cold inputs): 131072 tokens of one request, 32 / 8
 // heads of 128, bf16: 101 us, 5.3 TB/s with the launch and 6.3 TB/s between
 // 65536 and 131072 tokens; 64 histories up to 8191 (28 / 4 heads of 128, f32
-// rows over bf16): 113 us, 4.8 TB/s; 16 up to 2048 (16 / 16 of 128, f32): 73
+// rows over bf16): 112 us, 4.9 TB/s; 16 up to 2048 (16 / 16 of 128, f32): 73
 // us, 5.1 TB/s; 128 up to 4096 (9 / 3 of 64, Q8_0): 42 us, 2.6 TB/s; 77 tokens:
-// 6.5 us. A 16-bit or f32 cache waits for the memory (a third of the issue
-// slots used); Q8_0 at d_head 64 is bound by its 750 instructions per 32 keys,
-// half of them the conversions of quants and scales.
+// 6.8 us. A 16-bit or f32 cache waits for the memory (a third of the issue
+// slots used). Q8_0 at d_head 64 has 770 instructions per 32 keys, half of them
+// the conversions of quants and scales, and fills 58 % of the issue slots: its
+// warps wait for one another's results (convert, product, scale) more than for
+// the memory or for a slot.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -570,8 +572,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
   // A CTA for each history where there are as many (eight of one unit: 6.1 us, 8.9 when four CTAs take two each); more
   // only for kMinUnits each.
   // Equal histories and several CTAs to each: a whole number of them, where that leaves three quarters of the CTAs, so
-  // that none has the end of one and the start of the next, whose share it would do several us later (8 x 1024 tokens
-  // 19.6 us, 15.6 so; 1 x 8192: 24.9 and 19.3).
+  // that none has the end of one and the start of the next, whose share it would do several us later. Of 444 CTAs, bf16,
+  // 32 / 8 heads of 128, with (without): all used, 1 x 8192 tokens 19.4 (25.1) us; 392, 7 x 2000 20.6 (23.6); 384, 8 x
+  // 1024 15.5 (20.4); 360, 15 x 1000 21.5 (25.4). With fewer, short histories would gain still (320 CTAs, 20 x 512 17.5
+  // (22.4)) and long ones lose (20 x 4096 71.5 (68.2), 40 x 4096 126.6 (122.8)).
   int G = min((int)gridDim.x, max(units / kMinUnits, histories * KVH));
   const int even = G / (histories * KVH) * (histories * KVH);
   if ((long long)longest * histories == total && even * 4 >= G * 3) G = even;

@@ -7,8 +7,10 @@ each request appends, from lengths that stay on the GPU), then per layer
 per request over its pages); `release` returns finished requests' pages. Every
 call runs on torch's current stream of the tensors' device, synchronises
 nothing and can be captured into a CUDA graph when its outputs are given.
-Arguments that do not fit are refused with ValueError before anything runs.
-What only the device knows (page ids, slots, positions) is checked there: see
+Arguments that do not fit are refused before anything runs, tensors that do not
+go together with ValueError, what the entry points themselves refuse (a page
+size of 0, more than 16384 requests in a plan, rows off their 16 bytes) with
+RuntimeError. What only the device knows (page ids, slots, positions) is checked there: see
 `tb2_device_error` in the header. No gradient passes through these calls: with
 gradients enabled, a tensor that requires one is refused.
 """
