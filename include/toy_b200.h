@@ -209,9 +209,10 @@ int tb2_q8_0_dequantize(const void *q, void *hi, void *lo, float *f32, long long
  * on `stream` of the current device, read lengths and tables on the device
  * only (nothing is synchronised) and may be captured into a CUDA graph after
  * tb2_paged_prepare. They return 0, -1 for a bad argument (arrays off their
- * type's boundary among them), -3 for a failed launch. A page id, slot or position that is out of range on the device is
- * not followed: the access is skipped and tb2_device_error() reports 0x5001
- * (page), 0x5002 (slot) or 0x5003 (position).
+ * type's boundary among them), -3 for a failed launch. A page id, slot or
+ * position that is out of range on the device is not followed: the access is
+ * skipped and tb2_device_error() reports 0x5001 (page), 0x5002 (slot) or
+ * 0x5003 (position).
  *
  * One layer's page pools. Page p, key / value head j and offset o of a page
  * hold a row of d_head values at element p * page_stride + j * head_stride +

@@ -40,8 +40,8 @@ def test_append_arrays_off_their_boundary(bad):
     assert lib().tb2_paged_append(C.byref(kv()), C.byref(append_args(**bad)), None) == -1
 
 
-@pytest.mark.parametrize("bad", [dict(table=P + 1), dict(table=P + 2), dict(lens=P + 2), dict(lse=P + 2), dict(lse=P + 1)],
-                         ids=str)
+@pytest.mark.parametrize("bad", [dict(table=P + 1), dict(table=P + 2), dict(lens=P + 2), dict(lse=P + 2),
+                                 dict(lse=P + 1)], ids=str)
 def test_attend_arrays_off_their_boundary(bad):
     from toy_b200._lib import lib
     assert lib().tb2_paged_attend(C.byref(kv()), C.byref(attend_args(**bad)), None) == -1

@@ -88,6 +88,7 @@ def finite(x):
 @pytest.mark.parametrize("cache", ["f32", "f16", "bf16", "q8_0"])
 @pytest.mark.parametrize("H,KV,dh,P,lens", [
     (6, 2, 64, 16, [3, 40, 0, 700]), (12, 1, 128, 16, [1, 20000]), (3, 3, 32, 5, [9, 300, 2000]),
+    (40, 2, 64, 8, [5, 333]),
     (10, 1, 96, 32, [70, 5000])])
 def test_attend_infinities(cuda, row, cache, H, KV, dh, P, lens):
     """Keys and values with infinities in a live history, against the formula in 64 bits: a key whose score is -inf
@@ -294,7 +295,8 @@ def test_attend_unaligned_rows(cuda, row, cache, H, KV, dh, P, lens):
 
 
 @pytest.mark.parametrize("cache", ["f32", "bf16", "q8_0"])
-@pytest.mark.parametrize("lens,H,KV,dh", [([20000], 32, 8, 128), ([5000, 1, 777, 0, 4096], 9, 3, 64), ([600] * 40, 28, 4, 128)])
+@pytest.mark.parametrize("lens,H,KV,dh", [([20000], 32, 8, 128), ([5000, 1, 777, 0, 4096], 9, 3, 64),
+                                          ([600] * 40, 28, 4, 128)])
 def test_attend_repeats_itself(cuda, cache, lens, H, KV, dh):
     """The same inputs in new tensors, with another call between and other work on a second stream: the same bits."""
     import torch
@@ -414,3 +416,54 @@ def test_attend_all_minus_infinity(cuda, cache, L):
     if cache != "q8_0":                                 # scores of +inf
         assert bool(out[0, neg].isnan().all()) and bool(lse[0, neg].isnan().all())
     no_error()
+
+
+# ------------------------------------------------------------------ captured release
+@pytest.mark.parametrize("n,P,width", [(6, 16, 5), (900, 16, 40)])
+def test_release_captured(cuda, n, P, width):
+    """A release of one CTA and of several in a graph, twice in a row, replayed with other requests done and with an
+    entry that is no page, against the eager call."""
+    import torch
+    from toy_b200 import paged
+    from toy_b200._lib import lib
+    n_pages = n * width
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    table0 = torch.randperm(n_pages, generator=gen, device=cuda).int().view(n, width).contiguous()
+    lens0 = torch.full((n,), width * P, dtype=torch.int32, device=cuda)
+
+    def world():
+        return {"lens": lens0.clone(), "table": table0.clone(), "state": i32([0] * 4, cuda),
+                "free": torch.full((n_pages,), -9, dtype=torch.int32, device=cuda),
+                "a": torch.zeros(n, dtype=torch.int32, device=cuda), "b": torch.zeros(n, dtype=torch.int32, device=cuda)}
+
+    def step(w):
+        for done in ("a", "b"):
+            paged.release(w["lens"], w[done], w["table"], w["free"], w["state"], page_size=P, n_pages=n_pages)
+
+    graphed, eager = world(), world()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        step(graphed)
+    for i in range(4):
+        for w in (graphed, eager):
+            w["lens"].copy_(lens0)
+            w["table"].copy_(table0)
+            if i == 2:
+                w["table"][n // 2, 1], w["table"][0, 0] = n_pages, -5
+            w["state"].zero_()
+            pick = torch.arange(n, device=cuda) * 2654435761 % 4
+            w["a"].copy_(pick == i)
+            w["b"].copy_(pick == (i + 1) % 4)
+            if i == 2:
+                w["a"][n // 2] = w["b"][0] = 1
+        gr.replay()
+        step(eager)
+        for key in ("lens", "table", "state"):
+            assert torch.equal(graphed[key], eager[key]), (i, key)
+        top = int(eager["state"][0])
+        done = int(((eager["a"] != 0) | (eager["b"] != 0)).sum())
+        assert top == done * width - (2 if i == 2 else 0)
+        free = graphed["free"][:top]
+        assert torch.equal(free, eager["free"][:top]) and free.unique().numel() == top and int(free.min()) >= 0
+        assert lib().tb2_device_error() == (0x5001 if i == 2 else 0)

@@ -835,7 +835,8 @@ class KvEngine {
       return -3;
     }
     const size_t bytes = (size_t)nb_ * e_.cfg().vocab * 4;
-    if (logits_host && cudaMemcpyAsync(logits_host, logits_, bytes, cudaMemcpyDeviceToHost, st_) != cudaSuccess) return -3;
+    if (logits_host && cudaMemcpyAsync(logits_host, logits_, bytes, cudaMemcpyDeviceToHost, st_) != cudaSuccess)
+      return -3;
     if (cudaMemcpyAsync(state, pg_->state, sizeof state, cudaMemcpyDeviceToHost, st_) != cudaSuccess) return -3;
     return cudaStreamSynchronize(st_) == cudaSuccess ? 0 : -3;
   }

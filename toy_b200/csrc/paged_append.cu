@@ -264,8 +264,8 @@ int launch(const tb2_paged_kv& c, const tb2_paged_append_args& a, int* err, cuda
   const int items = (heads + 2 * c.n_kv) * (c.d_head / 2 / Row<T>::V);
   // A decode step has its whole token in one round: 28 / 4 bf16 heads of 128 with 512 (256) threads, 8 tokens 2.2 (2.8)
   // us, 250 2.6 (3.2), 400 3.5 (3.5), 1000 5.4 (5.6). A prompt keeps more CTAs on an SM: 2000 tokens 11.9 (10.5), 4000
-  // 21.4 (19.0); f32 rows of 32 / 8 heads of 64 into bf16: 250 2.3 (2.8), 400 3.4 (3.0), 1000 4.4 (5.4), 2000 9.7 (9.5),
-  // 16384 61.7 (57.9; 6.4 TB/s). The bound is two such CTAs to an SM; between
+  // 21.4 (19.0); f32 rows of 32 / 8 heads of 64 into bf16: 250 2.3 (2.8), 400 3.4 (3.0), 1000 4.4 (5.4), 2000 9.7
+  // (9.5), 16384 61.7 (57.9; 6.4 TB/s). The bound is two such CTAs to an SM; between
   // 300 and 1500 tokens either is right within a microsecond.
   const int most = a.n_tokens <= 2 * 148 ? 512 : 256;
   const int rounds = (items + most - 1) / most, threads = ((items + rounds - 1) / rounds + 31) / 32 * 32;

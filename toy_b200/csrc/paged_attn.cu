@@ -61,7 +61,8 @@ int tb2_paged_attend(const tb2_paged_kv* kv, const tb2_paged_attend_args* a, voi
   if (a->n_heads < 1 || a->n_heads % kv->n_kv || width > (1 << 24) || a->n_req > (1 << 20)) return -1;
   if (!a->q || !a->out || !a->lens || !a->table || a->ldq < width || a->ldo < width) return -1;
   const size_t e = (size_t)tb2::type_bytes(a->row_type);
-  if (!tb2::aligned(a->q, e) || !tb2::aligned(a->out, e) || !tb2::all_aligned(4, {a->table, a->lens, a->lse})) return -1;
+  if (!tb2::aligned(a->q, e) || !tb2::aligned(a->out, e)) return -1;
+  if (!tb2::all_aligned(4, {a->table, a->lens, a->lse})) return -1;
   // (positions, rounded up to whole units, are 32 bits wide)
   if (a->table_width < 1 || a->table_stride < a->table_width ||
       (long long)a->table_width * kv->page_size > 0x7fffff00LL)

@@ -487,10 +487,12 @@ __device__ __noinline__ void plain_part(const PagedAttnArgs& a, int b, int jt, i
       const int col = lane + 32 * k, w = col % 32;
       // the output tile, lane of a group and half of its pair that column `col` belongs to
       constexpr bool kRuns = CT == kCacheF32 || CT == kCacheQ8;
-      const int i = kRuns ? col / 32 * 4 + w % 4 : col / 8, c = kRuns ? w / 8 : w % 8 / 2, y = kRuns ? w % 8 / 4 : w & 1;
+      const int i = kRuns ? col / 32 * 4 + w % 4 : col / 8, c = kRuns ? w / 8 : w % 8 / 2;
+      const int y = kRuns ? w % 8 / 4 : w & 1;
       buf[((r * (C::OT / 2) + i / 2) * 32 + g * 4 + c) * 4 + (i & 1) * 2 + y] = o[k] * lift;
     }
-    if (lane < 4) reinterpret_cast<float2*>(buf + C::OT * 2 * C::R * 32)[r * 32 + g * 4 + lane] = make_float2(m, l * lift);
+    float2* ml = reinterpret_cast<float2*>(buf + C::OT * 2 * C::R * 32) + r * 32 + g * 4;
+    if (lane < 4) ml[lane] = make_float2(m, l * lift);
   }
 }
 
@@ -572,8 +574,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
   // A CTA for each history where there are as many (eight of one unit: 6.1 us, 8.9 when four CTAs take two each); more
   // only for kMinUnits each.
   // Equal histories and several CTAs to each: a whole number of them, where that leaves three quarters of the CTAs, so
-  // that none has the end of one and the start of the next, whose share it would do several us later. Of 444 CTAs, bf16,
-  // 32 / 8 heads of 128, with (without): all used, 1 x 8192 tokens 19.4 (25.1) us; 392, 7 x 2000 20.6 (23.6); 384, 8 x
+  // that none has the end of one and the start of the next, whose share it would do several us later. Of 444 CTAs,
+  // bf16, 32 / 8 heads of 128, with (without): all used, 1 x 8192 tokens 19.4 (25.1) us; 392, 7 x 2000 20.6 (23.6); 384, 8 x
   // 1024 15.5 (20.4); 360, 15 x 1000 21.5 (25.4). With fewer, short histories would gain still (320 CTAs, 20 x 512 17.5
   // (22.4)) and long ones lose (20 x 4096 71.5 (68.2), 40 x 4096 126.6 (122.8)).
   int G = min((int)gridDim.x, max(units / kMinUnits, histories * KVH));
@@ -918,8 +920,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
       for (int r = 0; r < R; ++r) o[i][r] = make_float2(0.f, 0.f);
     have_d = false;
     lift_d = 0;
-    if constexpr (CT == kCacheQ8)
+    if constexpr (CT == kCacheQ8) {
+#pragma unroll
       for (int r = 0; r < R; ++r) l2[r] = make_float2(0.f, 0.f);
+    }
     const uint32_t qb = smem_u32(region) + lane * 16, qh = smem_u32(region) + C::KS * 512 + lane * 8;
     auto q_at = [&](int p, int st) {   // register set p of step st
       if (C::kHalf && p == 1) {
@@ -1112,10 +1116,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        // 2^(s fac - m + lift), rounded at each of the three steps. The product as the maximum's was: with a fused one the
-        // largest key's exponent would be the rounding of m, which passes any range for scores of 2^30. The lift last:
-        // lift - m is a multiple of m's last place, so for m of 2^26 the largest weight would be 2^16 instead of 2^14,
-        // which f16 cannot hold.
+        // 2^(s fac - m + lift), rounded at each of the three steps. The product as the maximum's was: with a fused one
+        // the largest key's exponent would be the rounding of m, which passes any range for scores of 2^30. The lift
+        // last: lift - m is a multiple of m's last place, so for m of 2^26 the largest weight would be 2^16 instead of
+        // 2^14, which f16 cannot hold. (Scalar: the assembler fuses a packed product and sum.)
         const float less = m[r] == -INFINITY ? 0.f : -m[r];
         const float lifted = CT == kCacheQ8 ? kLift + (float)lift_d : kLift;
 #pragma unroll
@@ -1450,7 +1454,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, Cfg<CT, DH, HT, PL>::OCC)
       // of their number, by the CTA that completes a group, then the groups. 55 pieces (one request of 16384 tokens, 32 /
       // 8 heads of 128): 26.2 us in groups, 29.5 at once; 32 pieces (4096): 15.3 and 15.0; 16 pieces: 13.2 and 11.9.
       constexpr int kFew = 32;
-      static_assert(kFew <= 32 && kAttnMaxCtas <= 32 * 32, "at most 32 pieces, or groups, are added up at a time: a lane to each");
+      static_assert(kFew <= 32 && kAttnMaxCtas <= 32 * 32, "32 pieces, or groups, at most at a time: a lane to each");
       int group = 1;
       while (group * group < pieces) ++group;
       if (pieces <= kFew) group = pieces;
