@@ -371,6 +371,160 @@ size_t tb2_paged_attend_workspace(void);
 int tb2_paged_attend_workspace_init(void *workspace, size_t bytes, void *stream);
 int tb2_paged_attend(const tb2_paged_kv *kv, const tb2_paged_attend_args *args, void *stream);
 
+/* ===================================================================== */
+/* Operators of a training step over the caller's own rows and tensors   */
+/* (device-pointer primitives). No counterpart in the reference.         */
+/* ===================================================================== */
+/* Rows are f32, f16 or bf16 (type 0, 1 or 30), contiguous along a row, with
+ * any row stride of a row or more, on their type's boundary. All calls enqueue
+ * on `stream` of the current device, synchronise nothing, need no workspace
+ * and may be captured into a CUDA graph after tb2_rows_prepare. They return 0,
+ * -1 for a bad argument, -3 for a failed launch. Sums are f32, each result is
+ * rounded once, and the same call gives the same bits. */
+
+/* One-time set-up on the current device (the device error word, every kernel
+ * loaded); call it before capturing any of them. */
+int tb2_rows_prepare(void);
+
+/* Log probabilities. With z = scale * (row of logits), m = max z and s = sum
+ * exp(z - m), so that ln p_j = (z_j - m) - ln s:
+ *   logprob[i] = ln p of tokens[i] (0 for a negative token, that is none);
+ *   stats[i] = {m, ln s} (m + ln s is the log-sum-exp; tb2_logprobs_grad
+ *   reads them);
+ *   entropy[i] = -sum_j p_j ln p_j (when not NULL);
+ *   top_ids[i], top_logprobs[i]: the `top` largest logits, equal ones by the
+ *   lower index first, and their ln p. top is at most 32 and at most vocab.
+ * Logits of -inf are words of probability 0. A row of nothing else has stats
+ * {0, -inf}, log probabilities -inf, entropy 0. A NaN or +inf in a row makes
+ * its probabilities and entropy NaN; NaN counts as the largest logit. A token
+ * of vocab or more gives NaN and tb2_device_error() reports 0x5101. scale is
+ * finite and positive. tokens, stats and top_ids are on 8-byte boundaries. */
+typedef struct tb2_logprobs_args {
+  int n_rows, vocab, row_type;
+  const void *logits;
+  long long ld; /* elements */
+  float scale;
+  const long long *tokens;
+  float *logprob, *stats, *entropy;
+  int top;
+  long long *top_ids; /* [n_rows][top] */
+  float *top_logprobs;
+} tb2_logprobs_args;
+int tb2_logprobs(const tb2_logprobs_args *args, void *stream);
+
+/* The gradient of the above: with g_logprob, g_entropy and g_top (each NULL:
+ * none) the gradients of logprob, entropy and top_logprobs,
+ *   d_logits[i][j] = scale ( g_logprob ([j = token] - p_j)
+ *                          + sum_k g_top[k] ([j = top_ids[k]] - p_j)
+ *                          - g_entropy p_j (ln p_j + entropy) ).
+ * stats (and entropy, with g_entropy) are tb2_logprobs's of the same logits,
+ * scale and tokens; top_ids may be any words, the same one several times too.
+ * A negative token has no gradient; a token or alternative outside the
+ * vocabulary (for alternatives: negative too) is left out and reported as
+ * 0x5101. Words of probability 0 and rows of nothing else get 0 from p.
+ * d_logits has the logits' type and may be the logits themselves, with the
+ * same stride; otherwise they do not overlap. */
+typedef struct tb2_logprobs_grad_args {
+  int n_rows, vocab, row_type;
+  const void *logits;
+  long long ld;
+  float scale;
+  const long long *tokens;
+  const float *stats, *entropy;
+  const float *g_logprob, *g_entropy;
+  int top;
+  const float *g_top;
+  const long long *top_ids;
+  void *d_logits;
+  long long ldd;
+} tb2_logprobs_grad_args;
+int tb2_logprobs_grad(const tb2_logprobs_grad_args *args, void *stream);
+
+/* Slots sorted by expert. Slot i = token * n_used + choice goes to expert
+ * ids[i] (id_bytes 4 or 8: int or long long), or nowhere when that is negative.
+ * order lists the slots of expert 0, of expert 1, ..., each expert's in slot
+ * order, and -1 after the last; offsets[e] is where expert e's begin, and
+ * offsets[n_experts] the number of sorted slots; pos[i] is slot i's place in
+ * order, or -1. An id of n_experts or more counts as negative, and
+ * tb2_device_error() reports 0x5102. n_experts is at most 1024. */
+typedef struct tb2_expert_sort_args {
+  const void *ids;
+  int id_bytes;
+  int n_slots, n_experts;
+  int *offsets, *order, *pos;
+} tb2_expert_sort_args;
+int tb2_expert_sort(const tb2_expert_sort_args *args, void *stream);
+
+/* Rows to the experts and back. x is [n_tokens][d] (tokens), xs [n_rows][d]
+ * (sorted rows), pos [n_tokens][n_used] as tb2_expert_sort gives it; a slot of
+ * pos -1 takes no part, whatever its weight, and rows of xs that no slot has
+ * are not read, and not written either unless n_sorted (device memory, the
+ * last of the offsets; or NULL) is given: dispatch and combine_grad then set
+ * rows *n_sorted .. n_rows of their result to 0. A pos of n_rows or more is left out and
+ * tb2_device_error() reports 0x5103; places are distinct.
+ *   dispatch:     xs[pos[t][k]] = x[t].
+ *   combine:      x[t] = residual[t] + sum_k weights[t][k] xs[pos[t][k]], k
+ *                 ascending (residual NULL: 0; weights NULL: 1, which is the
+ *                 gradient of dispatch). x may be the residual itself.
+ *   combine_grad: x is the gradient of combine's result:
+ *                 d_xs[pos[t][k]] = weights[t][k] x[t],
+ *                 d_weights[t][k] = <x[t], xs[pos[t][k]]> (0 for pos -1);
+ *                 either may be NULL: not wanted. d_xs may be xs itself, with
+ *                 the same stride.
+ * Otherwise arrays that are written overlap no others. n_tokens * n_used is
+ * below 2^31. */
+typedef struct tb2_expert_rows_args {
+  int n_tokens, n_used, d, n_rows, row_type;
+  void *x;
+  long long ldx;
+  void *xs;
+  long long ldxs;
+  const int *pos;
+  const float *weights;
+  const void *residual;
+  long long ldr;
+  void *d_xs;
+  long long ldd;
+  float *d_weights;
+  const int *n_sorted;
+} tb2_expert_rows_args;
+int tb2_expert_dispatch(const tb2_expert_rows_args *args, void *stream);
+int tb2_expert_combine(const tb2_expert_rows_args *args, void *stream);
+int tb2_expert_combine_grad(const tb2_expert_rows_args *args, void *stream);
+
+/* An AdamW step over many tensors. With hp = [alpha, beta1, beta2, eps, wd,
+ * beta1h, beta2h] (tinynn/tinynn_ggml.h:457-465) and g = gradient *
+ * *grad_scale (NULL: 1), both device memory:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = (1 - alpha wd) p - alpha beta1h m / (sqrt(beta2h) sqrt(v) + eps),
+ * copy = p rounded to copy_type (copy NULL: none). state_bits 32: m and v are
+ * f32. state_bits 8: blocks of 256 consecutive values share an f32 scale
+ * (m_scale, v_scale: [ceil(n / 256)]), the smallest power of two of 2^-100 or
+ * more that brings the block within 448; m holds e4m3 codes of m / scale and v
+ * of sqrt(v) / scale, the step's exact values rounded once to nearest (even),
+ * a positive sqrt(v) never below the smallest code. All zeros (scales too) is
+ * an empty state. A block with a value that is not finite is NaN from then on.
+ * `tensors` is host memory, read during the call; its pointers are device
+ * memory and do not overlap; tensors of n = 0 are passed over. */
+typedef struct tb2_adamw_tensor {
+  void *p;
+  const void *g;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  void *copy;
+  long long n;
+} tb2_adamw_tensor;
+typedef struct tb2_adamw_multi_args {
+  const tb2_adamw_tensor *tensors;
+  int n_tensors;
+  int p_type, g_type, copy_type, state_bits;
+  const float *hp, *grad_scale;
+} tb2_adamw_multi_args;
+int tb2_adamw_multi(const tb2_adamw_multi_args *args, void *stream);
+/* The values that 8-bit moments stand for: p = m and copy = v, f32 (g is not
+ * used). put != 0: the other way, m, v and the scales from those values. */
+int tb2_adamw_moments(const tb2_adamw_tensor *tensors, int n_tensors, int put, void *stream);
+
 /* Read and clear the device-side error word of the current device
  * (non-zero when a kernel's bounded wait gave up). Synchronises the device. */
 int tb2_device_error(void);

@@ -74,6 +74,43 @@ class PagedAttendArgs(C.Structure):
                 ("workspace_bytes", C.c_size_t)]
 
 
+class LogprobsArgs(C.Structure):
+    _fields_ = [("n_rows", C.c_int), ("vocab", C.c_int), ("row_type", C.c_int), ("logits", C.c_void_p),
+                ("ld", C.c_longlong), ("scale", C.c_float), ("tokens", C.c_void_p), ("logprob", C.c_void_p),
+                ("stats", C.c_void_p), ("entropy", C.c_void_p), ("top", C.c_int), ("top_ids", C.c_void_p),
+                ("top_logprobs", C.c_void_p)]
+
+
+class LogprobsGradArgs(C.Structure):
+    _fields_ = [("n_rows", C.c_int), ("vocab", C.c_int), ("row_type", C.c_int), ("logits", C.c_void_p),
+                ("ld", C.c_longlong), ("scale", C.c_float), ("tokens", C.c_void_p), ("stats", C.c_void_p),
+                ("entropy", C.c_void_p), ("g_logprob", C.c_void_p), ("g_entropy", C.c_void_p), ("top", C.c_int),
+                ("g_top", C.c_void_p), ("top_ids", C.c_void_p), ("d_logits", C.c_void_p), ("ldd", C.c_longlong)]
+
+
+class ExpertSortArgs(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("id_bytes", C.c_int), ("n_slots", C.c_int), ("n_experts", C.c_int),
+                ("offsets", C.c_void_p), ("order", C.c_void_p), ("pos", C.c_void_p)]
+
+
+class ExpertRowsArgs(C.Structure):
+    _fields_ = [("n_tokens", C.c_int), ("n_used", C.c_int), ("d", C.c_int), ("n_rows", C.c_int),
+                ("row_type", C.c_int), ("x", C.c_void_p), ("ldx", C.c_longlong), ("xs", C.c_void_p),
+                ("ldxs", C.c_longlong), ("pos", C.c_void_p), ("weights", C.c_void_p), ("residual", C.c_void_p),
+                ("ldr", C.c_longlong), ("d_xs", C.c_void_p), ("ldd", C.c_longlong), ("d_weights", C.c_void_p),
+                ("n_sorted", C.c_void_p)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("copy", C.c_void_p), ("n", C.c_longlong)]
+
+
+class AdamwMultiArgs(C.Structure):
+    _fields_ = [("tensors", C.c_void_p), ("n_tensors", C.c_int), ("p_type", C.c_int), ("g_type", C.c_int),
+                ("copy_type", C.c_int), ("state_bits", C.c_int), ("hp", C.c_void_p), ("grad_scale", C.c_void_p)]
+
+
 _lib = None
 VP, D, DP, LP, SZ, I, LL = C.c_void_p, C.c_double, C.POINTER(C.c_double), C.POINTER(C.c_long), C.c_size_t, C.c_int, \
     C.c_longlong
@@ -154,6 +191,15 @@ _SIGS = [
     ("tb2_paged_attend_workspace", C.c_size_t, []),
     ("tb2_paged_attend_workspace_init", C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
     ("tb2_paged_attend", C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedAttendArgs), C.c_void_p]),
+    ("tb2_rows_prepare", C.c_int, []),
+    ("tb2_logprobs", C.c_int, [C.POINTER(LogprobsArgs), C.c_void_p]),
+    ("tb2_logprobs_grad", C.c_int, [C.POINTER(LogprobsGradArgs), C.c_void_p]),
+    ("tb2_expert_sort", C.c_int, [C.POINTER(ExpertSortArgs), C.c_void_p]),
+    ("tb2_expert_dispatch", C.c_int, [C.POINTER(ExpertRowsArgs), C.c_void_p]),
+    ("tb2_expert_combine", C.c_int, [C.POINTER(ExpertRowsArgs), C.c_void_p]),
+    ("tb2_expert_combine_grad", C.c_int, [C.POINTER(ExpertRowsArgs), C.c_void_p]),
+    ("tb2_adamw_multi", C.c_int, [C.POINTER(AdamwMultiArgs), C.c_void_p]),
+    ("tb2_adamw_moments", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     ("tb2_q8_0_quantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p]),
     ("tb2_q8_0_dequantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_longlong, C.c_int,
                                       C.c_void_p]),

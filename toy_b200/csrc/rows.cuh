@@ -1,0 +1,58 @@
+// What the operators over a caller's rows (logprobs.cu, experts.cu,
+// multi_adamw.cu) share: 16-byte pieces of f32, f16 or bf16 values as f32, the
+// launch shape, and the codes the kernels record in the device error word.
+#pragma once
+#include "paged.cuh"
+#include "pdl.cuh"
+
+namespace tb2 {
+
+enum RowsError : int {
+  kErrToken = 0x5101,     // a token or alternative outside the vocabulary
+  kErrExpert = 0x5102,    // an expert id outside [0, n_experts)
+  kErrExpertRow = 0x5103  // a sorted row outside the buffer
+};
+
+constexpr int kSMs = 148;
+
+// A kernel loaded on the current device, so that its first launch may be captured.
+template <class K>
+int load_kernel(K* k) {
+  cudaFuncAttributes at;
+  return cudaFuncGetAttributes(&at, k) == cudaSuccess ? 0 : -3;
+}
+int logprobs_prepare();
+int experts_prepare();
+int multi_adamw_prepare();
+
+// 16 bytes of T as f32, and back (one rounding)
+template <class T>
+struct Piece {
+  static constexpr int kN = 16 / (int)sizeof(T);
+  static __device__ __forceinline__ void get(const uint4& u, float (&f)[kN]) {
+    T t[kN];
+    memcpy(t, &u, 16);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) f[i] = to_f32<T>(t[i]);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&f)[kN]) {
+    T t[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) t[i] = from_f32<T>(f[i]);
+    uint4 u;
+    memcpy(&u, t, 16);
+    return u;
+  }
+};
+
+template <class F>
+int by_row_type(int type, F&& f) {
+  switch (type) {
+    case kTypeF32: return f(float());
+    case kTypeF16: return f(__half());
+    case kTypeBF16: return f(__nv_bfloat16());
+    default: return -1;
+  }
+}
+
+}  // namespace tb2

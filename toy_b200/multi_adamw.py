@@ -1,0 +1,155 @@
+"""An AdamW step over many torch CUDA tensors in one launch, moments in 32 or in 8
+bits: tb2_adamw_multi (include/toy_b200.h).
+
+The step is the framework's own (opt_step_adamw with the 7-slot row of
+`toy_b200.AdamW.hp`). With 8 bits a weight's two moments take 2.03 bytes instead
+of 8: blocks of 256 values share a power of two, m is held as e4m3 and v as the
+e4m3 of its square root, each the step's exact value rounded once.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence
+
+import torch
+
+from ._lib import AdamwMultiArgs, AdamwTensor
+from ._rows import F32, ROW_TYPE, bad, call, dense, prepare
+
+__all__ = ["MultiAdamW", "prepare"]
+BLOCK = 256
+_HELD = torch.float8_e4m3fn
+
+
+class MultiAdamW:
+    """The optimizer of `params`: contiguous tensors of one type (f32, f16 or bf16) on one GPU. copies: tensors of their
+    shapes, of one 16-bit type, that each step sets to the weights rounded (for weights kept in f32). state: (m, v,
+    m_scale, v_scale) to go on from, lists of tensors that the optimizer then owns, the scales None for 32 bits;
+    empty moments when None. The state is in the attributes of these names."""
+
+    def __init__(self, params: Sequence[torch.Tensor], *, bits: int = 8, copies: Optional[Sequence] = None,
+                 state: Optional[tuple] = None):
+        self.params = list(params)
+        if bits not in (8, 32):
+            bad("bits is 8 or 32")
+        if not self.params or not self.params[0].is_cuda or self.params[0].dtype not in ROW_TYPE:
+            bad("params: one f32, f16 or bf16 tensor or more on a GPU")
+        self.bits, self.dtype, self.index = bits, self.params[0].dtype, self.params[0].get_device()
+        self.device = self.params[0].device
+        n = [p.numel() for p in self.params]
+        self._shapes = [p.shape for p in self.params]
+        pp = [dense(p, p.shape, self.dtype, self.index, "params") for p in self.params]
+        self.copies = list(copies) if copies else None
+        self.copy_dtype = self.copies[0].dtype if copies else F32
+        if copies and (len(self.copies) != len(n) or self.copy_dtype not in (torch.float16, torch.bfloat16)):
+            bad("copies: one f16 or bf16 tensor per weight")
+        cp = [dense(c, s, self.copy_dtype, self.index, "copies")
+              for c, s in zip(self.copies, self._shapes)] if copies else [None] * len(n)
+        blocks = [-(-k // BLOCK) for k in n]
+        if state is None:
+            def zeros(sizes, dtype):
+                return [torch.zeros(k, device=self.device, dtype=dtype) for k in sizes]
+            if bits == 32:
+                state = (zeros(n, F32), zeros(n, F32), None, None)
+            else:
+                state = ([t.view(_HELD) for t in zeros(n, torch.uint8)], [t.view(_HELD) for t in zeros(n, torch.uint8)],
+                         zeros(blocks, F32), zeros(blocks, F32))
+        m, v, m_scale, v_scale = state
+        self.m, self.v = list(m), list(v)
+        held = F32 if bits == 32 else _HELD
+        if (m_scale is None) != (bits == 32) or (v_scale is None) != (bits == 32):
+            bad("state: scales for 8 bits, and only there")
+        lists = [self.m, self.v]
+        self.m_scale = self.v_scale = None
+        if bits == 8:
+            self.m_scale, self.v_scale = list(m_scale), list(v_scale)
+            lists += [self.m_scale, self.v_scale]
+        if any(len(x) != len(n) for x in lists):
+            bad("state: one tensor of each kind per weight")
+        at = []
+        for x, sizes, dtype in zip(lists, (n, n, blocks, blocks), (held, held, F32, F32)):
+            for t, k in zip(x, sizes):
+                if t.numel() != k or t.dtype is not dtype or t.get_device() != self.index or not t.is_contiguous():
+                    bad(f"state: contiguous {dtype} tensors of {k} values on cuda:{self.index}")
+            at.append([t.data_ptr() for t in x])
+        if bits == 32:
+            at += [[None] * len(n)] * 2
+        self._n = len(n)
+        self._t = (AdamwTensor * self._n)(*[AdamwTensor(*x) for x in zip(pp, [None] * self._n, *at, cp, n)])
+        self._now = (AdamwTensor * self._n)()
+        if self.index not in _ready():
+            prepare(self.device)
+
+    def step(self, grads: Sequence[Optional[torch.Tensor]], hp, *, grad_scale: Optional[torch.Tensor] = None) -> None:
+        """One step on the gradients (f32, f16 or bf16, all of one type, of the weights' shapes; None: the weight and
+        its moments stay). hp: the row of AdamW.hp, as an f32 [7] tensor on the GPU or as numbers; grad_scale: an f32
+        tensor of one value on the GPU that every gradient is multiplied by."""
+        if len(grads) != self._n:
+            bad("grads: one per weight")
+        if not isinstance(hp, torch.Tensor):
+            hp = torch.tensor([float(x) for x in hp], dtype=F32).to(self.device)
+        hp_at = dense(hp, (7,), F32, self.index, "hp")
+        scale_at = None
+        if grad_scale is not None:
+            if grad_scale.numel() != 1 or grad_scale.dtype is not F32 or grad_scale.get_device() != self.index:
+                bad(f"grad_scale: one f32 value on cuda:{self.index}")
+            scale_at = grad_scale.data_ptr()
+        dtype, k, dev = None, 0, self.index
+        t, now = self._t, self._now
+        for i, g in enumerate(grads):
+            if g is None:
+                continue
+            if dtype is None:
+                dtype = g.dtype
+                if dtype not in ROW_TYPE:
+                    bad("grads: f32, f16 or bf16")
+            if g.dtype is not dtype or g.shape != self._shapes[i] or g.get_device() != dev or not g.is_contiguous():
+                bad(f"grads[{i}]: contiguous {dtype} {list(self._shapes[i])} on cuda:{dev}")
+            now[k] = t[i]
+            now[k].g = g.data_ptr()
+            k += 1
+        if not k:
+            return
+        a = AdamwMultiArgs(C.addressof(now), k, ROW_TYPE[self.dtype], ROW_TYPE[dtype], ROW_TYPE[self.copy_dtype],
+                           self.bits, hp_at, scale_at)
+        call(dev, "tb2_adamw_multi", C.byref(a))
+
+    def _values(self, ms, vs, put: int) -> None:
+        if len(ms) != self._n or len(vs) != self._n:
+            bad("moments: one tensor of each kind per weight")
+        at = [[dense(t, s, F32, self.index, "moments") for t, s in zip(x, self._shapes)] for x in (ms, vs)]
+        x = (AdamwTensor * self._n)()
+        for i in range(self._n):
+            x[i] = self._t[i]
+            x[i].p, x[i].copy = at[0][i], at[1][i]
+        call(self.index, "tb2_adamw_moments", C.addressof(x), self._n, put)
+
+    def moments(self, *, out: Optional[tuple] = None) -> tuple:
+        """(m, v): the values of the moments, lists of f32 tensors of the weights' shapes (out: such lists to fill; in
+        32 bits without out the state itself)."""
+        if self.bits == 32:
+            if out is None:
+                return ([t.view(s) for t, s in zip(self.m, self._shapes)],
+                        [t.view(s) for t, s in zip(self.v, self._shapes)])
+            for to, x in zip(out, (self.m, self.v)):
+                for a, b in zip(to, x):
+                    a.copy_(b.view(a.shape))
+            return out
+        if out is None:
+            out = tuple([torch.empty(s, device=self.device, dtype=F32) for s in self._shapes] for _ in "mv")
+        self._values(out[0], out[1], 0)
+        return out
+
+    def set_moments(self, ms: Sequence[torch.Tensor], vs: Sequence[torch.Tensor]) -> None:
+        """The moments set to these values (f32, of the weights' shapes), rounded to the state's bits."""
+        if self.bits == 32:
+            for to, x in zip((self.m, self.v), (ms, vs)):
+                for a, b in zip(to, x):
+                    a.copy_(b.reshape(a.shape))
+            return
+        self._values(list(ms), list(vs), 1)
+
+
+def _ready() -> set:
+    from . import _rows
+    return _rows._prepared
