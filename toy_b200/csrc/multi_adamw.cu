@@ -12,7 +12,10 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
+#include <cstring>
+#include <iterator>
 
 #include "rows.cuh"
 #include "runtime.cuh"
@@ -21,131 +24,346 @@ namespace tb2 {
 namespace {
 
 constexpr int kBlock = 256;        // values that share a scale
-constexpr int kMaxTensors = 256;   // tensors a launch
+constexpr int kMaxTensors = 448;   // tensors a launch: their descriptors travel as its arguments (30.5 of 32 KB)
+constexpr int kThreads = 256, kWarps = kThreads / 32, kCtasPerSm = 4;
 
 struct Tensors {
   tb2_adamw_tensor t[kMaxTensors];
-  int first[kMaxTensors + 1];   // blocks before tensor i
+  int first[kMaxTensors + 1];             // blocks before tensor i
+  unsigned whole[(kMaxTensors + 31) / 32];   // bit i: tensor i's arrays are on the boundaries of four values
   int n;
 };
 
-// e4m3 of x (|x| <= 448), given to 64 bits: rounded once.
-__device__ __forceinline__ uint8_t e4m3_of(double x) {
-  const double a = fabs(x);
-  const int e = a < 0.015625 ? -6 : ilogb(a);
-  double q = rint(ldexp(a, 3 - e));   // eighths of the leading bit's weight; at the bottom, multiples of 2^-9
-  q = ldexp(q, e - 3);
-  return __nv_cvt_float_to_fp8((float)(x < 0 ? -q : q), __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ float e4m3_to(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-}
-
-// The power of two of a block whose largest magnitude is top.
-__device__ __forceinline__ float block_scale(double top) {
-  if (!isfinite(top)) return NAN;
-  int e;
-  const double f = frexp(top / 448.0, &e);
-  return ldexpf(1.f, max(top == 0.0 ? -100 : f == 0.5 ? e - 1 : e, -100));
+// The tensor that block b is of.
+__device__ __forceinline__ int tensor_of(const Tensors& ts, int b) {
+  int lo = 0, hi = ts.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (ts.first[mid] <= b) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
 }
 
-__device__ __forceinline__ double block_max(double v, double* sm) {
+// Four values: a lane has values 4 lane .. 4 lane + 3 and 128 more of a block, so that a warp's reads and writes are
+// contiguous in every type.
+template <class T>
+__device__ __forceinline__ void load4(const void* p, long long i, float* f) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const T*>(p) + i);
+    T t[4];
+    memcpy(t, &u, 8);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const double q = __shfl_xor_sync(0xffffffffu, v, o);
-    v = q > v || q != q ? q : v;
+    for (int k = 0; k < 4; ++k) f[k] = to_f32<T>(t[k]);
   }
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = v;
-  __syncthreads();
-  for (int w = 0; w < kBlock / 32; ++w) v = sm[w] > v || sm[w] != sm[w] ? sm[w] : v;
-  return v;
+}
+template <class T>
+__device__ __forceinline__ void store4(void* p, long long i, const float* f) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(f[0], f[1], f[2], f[3]);
+  } else {
+    T t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = from_f32<T>(f[k]);
+    uint2 u;
+    memcpy(&u, t, 8);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p) + i) = u;
+  }
+}
+__device__ __forceinline__ void load4_e4m3(unsigned u, float* f) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> 16 * k), __NV_E4M3));
+    f[2 * k] = __low2float(h);
+    f[2 * k + 1] = __high2float(h);
+  }
+}
+__device__ __forceinline__ unsigned pack4_e4m3(const float* f) {
+  const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+  const unsigned hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
 }
 
-__device__ __forceinline__ float load_value(const void* p, int type, long long i) {
-  return type == kTypeF32 ? static_cast<const float*>(p)[i]
-       : type == kTypeF16 ? to_f32(static_cast<const __half*>(p)[i])
-                          : to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void store_value(void* p, int type, long long i, float v) {
-  if (type == kTypeF32) static_cast<float*>(p)[i] = v;
-  else if (type == kTypeF16) static_cast<__half*>(p)[i] = from_f32<__half>(v);
-  else static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
+// The e4m3 code of t >= 0 (within 448), given to 64 bits: rounded once.
+__device__ __noinline__ unsigned e4m3_of(double t) {
+  const int e = t < 0.015625 ? -6 : ilogb(t);
+  const double q = ldexp(rint(ldexp(t, 3 - e)), e - 3);   // eighths of the leading bit; at the bottom, steps of 2^-9
+  return __nv_cvt_float_to_fp8((float)q, __NV_SATFINITE, __NV_E4M3);
 }
 
-// A CTA a block of 256 values.
-template <int BITS>
-__global__ void __launch_bounds__(kBlock) step_kernel(const __grid_constant__ Tensors ts, int p_type, int g_type,
-                                                      int copy_type, const float* hp, const float* factor) {
+// Whether t >= 0, as a multiple of the scale, is within `ulps` of the border between two codes: bits below an e4m3
+// value's three, next to their half. (Below 2^-6 codes are 2^-9 apart, as they are just above it.)
+__device__ __forceinline__ bool near_border(float t, unsigned ulps) {
+  const unsigned b = __float_as_uint(t < 0.015625f ? t + 0.015625f : t) & 0xfffffu;
+  return b - (0x80000u - ulps) <= 2 * ulps;
+}
+
+// A block's power of two, from the bits of its largest magnitude, and the factor to it: the smallest 2^e with top <=
+// 448 2^e (448 = 1.75 2^8), 2^-100 at least; NaN where top is not finite.
+__device__ __forceinline__ float block_scale(unsigned top, float& inverse) {
+  const int e = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), -100);
+  const bool ok = top < 0x7f800000u;
+  inverse = ok ? __uint_as_float((unsigned)(127 - e) << 23) : NAN;
+  return ok ? __uint_as_float((unsigned)(127 + e) << 23) : NAN;
+}
+
+// One value's step, in f32 but for 8-bit m: that is a sum of two terms of either sign, and rounding it once to a code
+// needs it to more bits than a product and a sum in f32 leave after a cancellation. FP64 has the room: two products
+// and three conversions a value are a tenth of what the FP64 pipe does in the time of a value's 16 bytes.
+struct Hyper {
+  float a, b1, b2, eps, keep, c1, c2, gf, d1, d2;
+  double db1, dgm;
+};
+
+template <class P, class G, int BITS>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid_constant__ Tensors ts, int copy_type,
+                                                                    const float* hp, const float* factor) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int all = ts.first[ts.n];
+  const int b0 = (int)((long long)all * blockIdx.x / gridDim.x), b1 = (int)((long long)all * (blockIdx.x + 1) / gridDim.x);
+  int i = tensor_of(ts, min(b0 + warp, all - 1));
   griddep_wait();
-  __shared__ double sm[kBlock / 32];
-  const float a = hp[0], b1 = hp[1], b2 = hp[2], eps = hp[3], wd = hp[4], c1 = hp[5], c2 = sqrtf(hp[6]);
-  const float gf = factor ? *factor : 1.f;
-  int i = 0;
-  while (i + 1 < ts.n && (int)blockIdx.x >= ts.first[i + 1]) ++i;
-  const tb2_adamw_tensor& t = ts.t[i];
-  const int blk = blockIdx.x - ts.first[i];
-  const long long k = (long long)blk * kBlock + threadIdx.x;
-  const bool on = k < t.n;
-  const double g = on ? (double)load_value(t.g, g_type, k) * gf : 0.0;
-  const float p = on ? load_value(t.p, p_type, k) : 0.f;
-  double m = 0.0, v = 0.0;
-  if (on && BITS == 8) {
-    m = e4m3_to(static_cast<uint8_t*>(t.m)[k]) * t.m_scale[blk];
-    v = e4m3_to(static_cast<uint8_t*>(t.v)[k]) * t.v_scale[blk];
-    v *= v;
-  } else if (on) {
-    m = static_cast<float*>(t.m)[k];
-    v = static_cast<float*>(t.v)[k];
-  }
-  m = m * b1 + g * (1.0 - b1);
-  v = v * b2 + g * g * (1.0 - b2);
-  const double r = sqrt(v);
-  if (on) {
-    const float w = p * (1.f - a * wd) - a * (float)m * c1 / ((float)r * c2 + eps);
-    store_value(t.p, p_type, k, w);
-    if (t.copy) store_value(t.copy, copy_type, k, p_type == kTypeF32 ? w : load_value(t.p, p_type, k));
-  }
-  if (BITS == 32) {
-    if (on) static_cast<float*>(t.m)[k] = (float)m, static_cast<float*>(t.v)[k] = (float)v;
-    return;
-  }
-  const float sm_ = block_scale(block_max(on ? fabs(m) : 0.0, sm)), sv = block_scale(block_max(on ? r : 0.0, sm));
-  if (on) {
-    static_cast<uint8_t*>(t.m)[k] = sm_ == sm_ ? e4m3_of(m / sm_) : 0x7f;
-    uint8_t q = sv == sv ? e4m3_of(r / sv) : 0x7f;
-    static_cast<uint8_t*>(t.v)[k] = q == 0 && r > 0.0 ? 1 : q;
-    if (threadIdx.x == 0) t.m_scale[blk] = sm_, t.v_scale[blk] = sv;
+  Hyper h;
+  h.a = hp[0]; h.b1 = hp[1]; h.b2 = hp[2]; h.eps = hp[3];
+  h.keep = 1.f - h.a * hp[4];
+  h.c1 = h.a * hp[5];
+  h.c2 = sqrtf(hp[6]);
+  h.gf = factor ? *factor : 1.f;
+  h.d1 = 1.f - h.b1;
+  h.d2 = 1.f - h.b2;
+  h.db1 = h.b1;
+  h.dgm = (1.0 - h.db1) * (double)h.gf;
+  for (int b = b0 + warp; b < b1; b += kWarps) {
+    while (ts.first[i + 1] <= b) ++i;
+    const tb2_adamw_tensor& t = ts.t[i];
+    const int blk = b - ts.first[i];
+    const long long k0 = (long long)blk * kBlock + 4 * lane;
+    const bool whole = (ts.whole[i / 32] >> (i % 32) & 1) && (long long)(blk + 1) * kBlock <= t.n;
+    float p[8], g[8], m[8], r[8];
+    float ms = 0.f, vs = 0.f;
+    if (BITS == 8) ms = t.m_scale[blk], vs = t.v_scale[blk];
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        load4<P>(t.p, k0 + 128 * j, p + 4 * j);
+        load4<G>(t.g, k0 + 128 * j, g + 4 * j);
+        if (BITS == 8) {
+          load4_e4m3(*reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(t.m) + k0 + 128 * j), m + 4 * j);
+          load4_e4m3(*reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(t.v) + k0 + 128 * j), r + 4 * j);
+        } else {
+          load4<float>(t.m, k0 + 128 * j, m + 4 * j);
+          load4<float>(t.v, k0 + 128 * j, r + 4 * j);
+        }
+      }
+    } else {   // a tensor's end, or one off its boundaries
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const long long k = k0 + 128 * (e / 4) + e % 4;
+        const bool on = k < t.n;
+        p[e] = on ? to_f32(static_cast<const P*>(t.p)[k]) : 0.f;
+        g[e] = on ? to_f32(static_cast<const G*>(t.g)[k]) : 0.f;
+        if (BITS == 8) {
+          m[e] = on ? __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(t.m)[k], __NV_E4M3))) : 0.f;
+          r[e] = on ? __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(t.v)[k], __NV_E4M3))) : 0.f;
+        } else {
+          m[e] = on ? static_cast<const float*>(t.m)[k] : 0.f;
+          r[e] = on ? static_cast<const float*>(t.v)[k] : 0.f;
+        }
+      }
+    }
+    double wide[8];   // m, to more bits
+    float r0[8];      // the held root of v
+    unsigned top_m = 0, top_r = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float gg = g[e] * h.gf;
+      float v;
+      if (BITS == 8) {
+        wide[e] = fma((double)(m[e] * ms), h.db1, (double)g[e] * h.dgm);
+        m[e] = (float)wide[e];
+        r0[e] = r[e] * vs;   // exact, its square too
+        v = fmaf(r0[e] * r0[e], h.b2, gg * gg * h.d2);
+        v = v < FLT_MIN ? 0.f : v;   // (what f32 does not hold to its full bits counts as 0)
+      } else {
+        m[e] = fmaf(m[e], h.b1, gg * h.d1);
+        v = fmaf(r[e], h.b2, gg * gg * h.d2);
+      }
+      const float root = sqrtf(v);
+      p[e] = fmaf(p[e], h.keep, -(h.c1 * m[e]) / fmaf(root, h.c2, h.eps));
+      r[e] = BITS == 8 ? root : v;
+      if (BITS == 8) {
+        top_m = max(top_m, __float_as_uint(fabsf(m[e])));
+        top_r = max(top_r, __float_as_uint(root));
+      }
+    }
+    unsigned mq[2], vq[2];
+    if (BITS == 8) {
+      float mi, ri;
+      const float nms = block_scale(__reduce_max_sync(0xffffffffu, top_m), mi);
+      const float nvs = block_scale(__reduce_max_sync(0xffffffffu, top_r), ri);
+      if (lane == 0) t.m_scale[blk] = nms, t.v_scale[blk] = nvs;
+      unsigned redo = 0;   // bit e: m's code, bit e + 8: the root's, to be rounded from more bits
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float tm[4], tr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = 4 * j + e;
+          tm[e] = m[k] * mi;
+          tr[e] = r[k] * ri;
+          redo |= near_border(fabsf(tm[e]), 1) << k;                                      // m is rounded once
+          redo |= near_border(tr[e], 8) << (k + 8);   // 4 units off at most (2^-24 each: g, its square, the product,
+          // the sum, half of these behind the root, and the root)
+        }
+        mq[j] = pack4_e4m3(tm);
+        vq[j] = pack4_e4m3(tr);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tr[e] > 0.f && (vq[j] >> 8 * e & 0xff) == 0) vq[j] |= 1u << 8 * e;   // a positive root stays so
+      }
+      if (redo && mi == mi && ri == ri) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int at = 8 * (k % 4);
+          if (redo >> k & 1) {
+            const unsigned q = e4m3_of(fabs(wide[k]) * mi) | (wide[k] < 0.0 ? 0x80 : 0);
+            mq[k / 4] = (mq[k / 4] & ~(0xffu << at)) | q << at;
+          }
+          if (redo >> (k + 8) & 1) {
+            const double gw = (double)g[k] * h.gf, vw = (double)r0[k] * r0[k] * h.b2 + gw * gw * (1.0 - (double)h.b2);
+            const unsigned q = max(e4m3_of(sqrt(vw) * ri), 1u);
+            vq[k / 4] = (vq[k / 4] & ~(0xffu << at)) | q << at;
+          }
+        }
+      }
+    }
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        store4<P>(t.p, k0 + 128 * j, p + 4 * j);
+        if (t.copy) {
+          if (sizeof(P) == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[4 * j + e] = to_f32(from_f32<P>(p[4 * j + e]));
+          }
+          if (copy_type == kTypeF16) store4<__half>(t.copy, k0 + 128 * j, p + 4 * j);
+          else if (copy_type == kTypeBF16) store4<__nv_bfloat16>(t.copy, k0 + 128 * j, p + 4 * j);
+          else store4<float>(t.copy, k0 + 128 * j, p + 4 * j);
+        }
+        if (BITS == 8) {
+          *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(t.m) + k0 + 128 * j) = mq[j];
+          *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(t.v) + k0 + 128 * j) = vq[j];
+        } else {
+          store4<float>(t.m, k0 + 128 * j, m + 4 * j);
+          store4<float>(t.v, k0 + 128 * j, r + 4 * j);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const long long k = k0 + 128 * (e / 4) + e % 4;
+        if (k >= t.n) continue;
+        const P q = from_f32<P>(p[e]);
+        static_cast<P*>(t.p)[k] = q;
+        if (t.copy) {
+          if (copy_type == kTypeF16) static_cast<__half*>(t.copy)[k] = from_f32<__half>(to_f32(q));
+          else if (copy_type == kTypeBF16) static_cast<__nv_bfloat16*>(t.copy)[k] = from_f32<__nv_bfloat16>(to_f32(q));
+          else static_cast<float*>(t.copy)[k] = to_f32(q);
+        }
+        if (BITS == 8) {
+          static_cast<uint8_t*>(t.m)[k] = (uint8_t)(mq[e / 4] >> 8 * (e % 4));
+          static_cast<uint8_t*>(t.v)[k] = (uint8_t)(vq[e / 4] >> 8 * (e % 4));
+        } else {
+          static_cast<float*>(t.m)[k] = m[e];
+          static_cast<float*>(t.v)[k] = r[e];
+        }
+      }
+    }
   }
 }
 
-// out: the values that 8-bit moments stand for (p: m's, copy: v's, f32), or (PUT) the moments from those values
+// The values that 8-bit moments stand for (p: m's, copy: v's, f32), or (PUT) the moments from those values.
 template <bool PUT>
-__global__ void __launch_bounds__(kBlock) moments_kernel(const __grid_constant__ Tensors ts) {
+__global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ Tensors ts) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int all = ts.first[ts.n];
+  const int b0 = (int)((long long)all * blockIdx.x / gridDim.x), b1 = (int)((long long)all * (blockIdx.x + 1) / gridDim.x);
+  int i = tensor_of(ts, min(b0 + warp, all - 1));
   griddep_wait();
-  __shared__ double sm[kBlock / 32];
-  int i = 0;
-  while (i + 1 < ts.n && (int)blockIdx.x >= ts.first[i + 1]) ++i;
-  const tb2_adamw_tensor& t = ts.t[i];
-  const int blk = blockIdx.x - ts.first[i];
-  const long long k = (long long)blk * kBlock + threadIdx.x;
-  const bool on = k < t.n;
-  uint8_t *mq = static_cast<uint8_t*>(t.m), *vq = static_cast<uint8_t*>(t.v);
-  float *mo = static_cast<float*>(t.p), *vo = static_cast<float*>(t.copy);
-  if (!PUT) {
-    if (!on) return;
-    const float r = e4m3_to(vq[k]) * t.v_scale[blk];
-    mo[k] = e4m3_to(mq[k]) * t.m_scale[blk];
-    vo[k] = r * r;
-    return;
-  }
-  const double m = on ? mo[k] : 0.0, r = on ? sqrt((double)vo[k]) : 0.0;
-  const float sm_ = block_scale(block_max(fabs(m), sm)), sv = block_scale(block_max(r, sm));
-  if (on) {
-    mq[k] = sm_ == sm_ ? e4m3_of(m / sm_) : 0x7f;
-    uint8_t q = sv == sv ? e4m3_of(r / sv) : 0x7f;
-    vq[k] = q == 0 && r > 0.0 ? 1 : q;
-    if (threadIdx.x == 0) t.m_scale[blk] = sm_, t.v_scale[blk] = sv;
+  for (int b = b0 + warp; b < b1; b += kWarps) {
+    while (ts.first[i + 1] <= b) ++i;
+    const tb2_adamw_tensor& t = ts.t[i];
+    const int blk = b - ts.first[i];
+    const long long k0 = (long long)blk * kBlock + 4 * lane;
+    const bool whole = (ts.whole[i / 32] >> (i % 32) & 1) && (long long)(blk + 1) * kBlock <= t.n;
+    uint8_t *mp = static_cast<uint8_t*>(t.m), *vp = static_cast<uint8_t*>(t.v);
+    float *mo = static_cast<float*>(t.p), *vo = static_cast<float*>(t.copy);
+    float m[8], r[8];
+    if (!PUT) {
+      const float ms = t.m_scale[blk], vs = t.v_scale[blk];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        unsigned mq = 0, vq = 0;
+        if (whole) {
+          mq = *reinterpret_cast<const unsigned*>(mp + k0 + 128 * j);
+          vq = *reinterpret_cast<const unsigned*>(vp + k0 + 128 * j);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k0 + 128 * j + e < t.n) {
+              mq |= (unsigned)mp[k0 + 128 * j + e] << 8 * e;
+              vq |= (unsigned)vp[k0 + 128 * j + e] << 8 * e;
+            }
+        }
+        load4_e4m3(mq, m + 4 * j);
+        load4_e4m3(vq, r + 4 * j);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] *= ms;
+        r[e] *= vs;
+        r[e] *= r[e];
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (whole) {
+          store4<float>(mo, k0 + 128 * j, m + 4 * j);
+          store4<float>(vo, k0 + 128 * j, r + 4 * j);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k0 + 128 * j + e < t.n) {
+              mo[k0 + 128 * j + e] = m[4 * j + e];
+              vo[k0 + 128 * j + e] = r[4 * j + e];
+            }
+        }
+      }
+      continue;
+    }
+    unsigned top_m = 0, top_r = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const long long k = k0 + 128 * (e / 4) + e % 4;
+      m[e] = k < t.n ? mo[k] : 0.f;
+      r[e] = k < t.n ? vo[k] : 0.f;
+      top_m = max(top_m, __float_as_uint(fabsf(m[e])));
+      top_r = max(top_r, __float_as_uint(r[e] < FLT_MIN && r[e] >= 0.f ? 0.f : sqrtf(r[e])));
+    }
+    float mi, ri;
+    const float ms = block_scale(__reduce_max_sync(0xffffffffu, top_m), mi);
+    const float vs = block_scale(__reduce_max_sync(0xffffffffu, top_r), ri);
+    if (lane == 0) t.m_scale[blk] = ms, t.v_scale[blk] = vs;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const long long k = k0 + 128 * (e / 4) + e % 4;
+      if (k >= t.n) continue;
+      const float x = mo[k], y = vo[k] < FLT_MIN ? 0.f : vo[k];
+      mp[k] = mi == mi ? (uint8_t)(e4m3_of(fabs((double)x * mi)) | (x < 0.f ? 0x80 : 0)) : 0x7f;
+      vp[k] = ri == ri ? (uint8_t)max(e4m3_of(sqrt((double)y) * ri), y > 0.f ? 1u : 0u) : 0x7f;
+    }
   }
 }
 
@@ -158,35 +376,47 @@ bool tensor_ok(const tb2_adamw_tensor& t, int p_type, int g_type, int copy_type,
   return t.m_scale && t.v_scale && all_aligned(4, {t.m_scale, t.v_scale});
 }
 
-// The tensors in groups of what a launch takes, empty ones left out.
-template <class F>
-int in_groups(const tb2_adamw_tensor* t, int n, F&& launch) {
+// The tensors in groups of what a launch takes, empty ones left out. whole(tensor): see Tensors.
+template <class W, class F>
+int in_groups(const tb2_adamw_tensor* t, int n, W&& whole, F&& launch) {
   Tensors g;
   for (int i = 0; i < n;) {
     g.n = 0;
+    std::fill(std::begin(g.whole), std::end(g.whole), 0u);
     long long blocks = 0;
     for (; i < n && g.n < kMaxTensors; ++i) {
       if (t[i].n == 0) continue;
       const long long b = (t[i].n + kBlock - 1) / kBlock;
       if (blocks + b > 0x7fffffffLL) break;
+      if (whole(t[i])) g.whole[g.n / 32] |= 1u << (g.n % 32);
       g.first[g.n] = (int)blocks;
       g.t[g.n++] = t[i];
       blocks += b;
     }
     g.first[g.n] = (int)blocks;
-    if (g.n)
-      if (int rc = launch(g, (int)blocks)) return rc;
+    if (g.n) {
+      // CTAs that stay, each with a run of blocks; as many as the blocks need where those are few
+      const long long ctas = std::min((blocks + kWarps - 1) / kWarps, (long long)kCtasPerSm * kSMs);
+      if (int rc = launch(g, (int)ctas)) return rc;
+    }
   }
   return 0;
+}
+
+template <class P, class G>
+int prepare_types() {
+  return load_kernel(step_kernel<P, G, 8>) || load_kernel(step_kernel<P, G, 32>) ? -3 : 0;
+}
+template <class P>
+int prepare_type() {
+  return prepare_types<P, float>() || prepare_types<P, __half>() || prepare_types<P, __nv_bfloat16>() ? -3 : 0;
 }
 
 }  // namespace
 
 int multi_adamw_prepare() {
-  return load_kernel(step_kernel<8>) || load_kernel(step_kernel<32>) || load_kernel(moments_kernel<true>) ||
-                 load_kernel(moments_kernel<false>)
-             ? -3
-             : 0;
+  if (load_kernel(moments_kernel<true>) || load_kernel(moments_kernel<false>)) return -3;
+  return prepare_type<float>() || prepare_type<__half>() || prepare_type<__nv_bfloat16>() ? -3 : 0;
 }
 
 }  // namespace tb2
@@ -200,9 +430,20 @@ int tb2_adamw_multi(const tb2_adamw_multi_args* a, void* stream) {
   if (!a->hp || !all_aligned(4, {a->hp, a->grad_scale})) return -1;
   for (int i = 0; i < a->n_tensors; ++i)
     if (!tensor_ok(a->tensors[i], a->p_type, a->g_type, a->copy_type, a->state_bits)) return -1;
-  return in_groups(a->tensors, a->n_tensors, [&](const Tensors& g, int blocks) {
-    return launch_pdl(a->state_bits == 8 ? step_kernel<8> : step_kernel<32>, dim3(blocks), dim3(kBlock), 0,
-                      static_cast<cudaStream_t>(stream), g, a->p_type, a->g_type, a->copy_type, a->hp, a->grad_scale);
+  const size_t pb = 4 * type_bytes(a->p_type), gb = 4 * type_bytes(a->g_type), cb = 4 * type_bytes(a->copy_type);
+  const size_t sb = a->state_bits == 8 ? 4 : 16;
+  auto whole = [&](const tb2_adamw_tensor& t) {
+    return aligned(t.p, pb) && aligned(t.g, gb) && aligned(t.copy, cb) && all_aligned(sb, {t.m, t.v});
+  };
+  return in_groups(a->tensors, a->n_tensors, whole, [&](const Tensors& g, int ctas) {
+    return by_row_type(a->p_type, [&](auto p) {
+      return by_row_type(a->g_type, [&](auto q) {
+        using P = decltype(p);
+        using G = decltype(q);
+        return launch_pdl(a->state_bits == 8 ? step_kernel<P, G, 8> : step_kernel<P, G, 32>, dim3(ctas), dim3(kThreads),
+                          0, static_cast<cudaStream_t>(stream), g, a->copy_type, a->hp, a->grad_scale);
+      });
+    });
   });
 }
 
@@ -216,8 +457,11 @@ int tb2_adamw_moments(const tb2_adamw_tensor* tensors, int n_tensors, int put, v
                 !all_aligned(4, {t.p, t.copy, t.m_scale, t.v_scale})))
       return -1;
   }
-  return in_groups(tensors, n_tensors, [&](const Tensors& g, int blocks) {
-    return launch_pdl(put ? moments_kernel<true> : moments_kernel<false>, dim3(blocks), dim3(kBlock), 0,
+  auto whole = [](const tb2_adamw_tensor& t) {
+    return all_aligned(16, {t.p, t.copy}) && all_aligned(4, {t.m, t.v});
+  };
+  return in_groups(tensors, n_tensors, whole, [&](const Tensors& g, int ctas) {
+    return launch_pdl(put ? moments_kernel<true> : moments_kernel<false>, dim3(ctas), dim3(kThreads), 0,
                       static_cast<cudaStream_t>(stream), g);
   });
 }
