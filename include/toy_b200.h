@@ -386,10 +386,10 @@ int tb2_paged_attend(const tb2_paged_kv *kv, const tb2_paged_attend_args *args, 
  * loaded); call it before capturing any of them. */
 int tb2_rows_prepare(void);
 
-/* Log probabilities. With z = scale * (row of logits), m = max z and s = sum
- * exp(z - m), so that ln p_j = (z_j - m) - ln s:
+/* Log probabilities. With x a row of logits, m = max x and s = sum exp(scale
+ * (x - m)), so that ln p_j = scale (x_j - m) - ln s:
  *   logprob[i] = ln p of tokens[i] (0 for a negative token, that is none);
- *   stats[i] = {m, ln s} (m + ln s is the log-sum-exp; tb2_logprobs_grad
+ *   stats[i] = {m, ln s} (scale m + ln s is the log-sum-exp; tb2_logprobs_grad
  *   reads them);
  *   entropy[i] = -sum_j p_j ln p_j (when not NULL);
  *   top_ids[i], top_logprobs[i]: the `top` largest logits, equal ones by the
@@ -502,7 +502,8 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args *args, void *stream);
  * (m_scale, v_scale: [ceil(n / 256)]), the smallest power of two of 2^-100 or
  * more that brings the block within 448; m holds e4m3 codes of m / scale and v
  * of sqrt(v) / scale, the step's exact values rounded once to nearest (even),
- * a positive sqrt(v) never below the smallest code. All zeros (scales too) is
+ * a positive sqrt(v) never below the smallest code, a v below 2^-126 as 0. All
+ * zeros (scales too) is
  * an empty state. A block with a value that is not finite is NaN from then on.
  * `tensors` is host memory, read during the call; its pointers are device
  * memory and do not overlap; tensors of n = 0 are passed over. */

@@ -1,8 +1,28 @@
 // Log probabilities of given tokens, entropy and the most likely alternatives
 // of each row of logits, and the gradient back to the logits.
 //
-// With z = a x (a the scale), m = max z, s = sum exp(z - m):
-//   ln p_j = (z_j - m) - ln s,   H = ln s - sum exp(z - m) (z - m) / s.
+// With a the scale, M = max x, d = x - M and s = sum exp(a d):
+//   ln p_j = a d_j - ln s,   H = ln s - a sum exp(a d) d / s.
+// (Differences first: a row may be full of the type's lowest value.)
+//
+// Both directions are one pass and bound by reading the logits: the forward
+// keeps a running maximum and rescales its sums when that grows, so that a row
+// is read once; the gradient reads it again and writes as much.
+//
+// The alternatives cost no second pass. Every thread keeps the maximum of each
+// of its four interleaved shares of the row, which the softmax needs anyway.
+// The top-th largest of 64 group maxima is a lower bound of the row's top-th
+// largest value, and only shares whose maximum reaches it can hold an
+// alternative: of a row's 1024 shares about 30 at top = 20 (the groups that the
+// first M values fall into are M's coupons: 64 (H_64 - H_44) = 24), so some 3 %
+// of the row is read again. Values above the bound are ranked by (value, lower
+// index). Bounds that many values equal (flat rows) take the lowest indices by
+// a scan in order; what passes the buffers (or holds a NaN) takes one round of
+// the row for each alternative.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "rows.cuh"
@@ -11,7 +31,10 @@
 namespace tb2 {
 namespace {
 
-constexpr int kThreads = 256, kMaxTop = 32;
+namespace cg = cooperative_groups;
+typedef unsigned long long u64;
+
+constexpr int kGradThreads = 256, kMaxTop = 32, kGroups = 64, kCand = 1024, kTies = 512, kUnroll = 4;
 
 struct ScoreArgs {
   const void* x;
@@ -21,92 +44,478 @@ struct ScoreArgs {
   long long* top_ids;
   int* err;
   float scale;
-  int n, V, top;
+  int n, V, top, split;   // split: CTAs (a cluster) to a row
 };
 
 // Values in the order of (x, lower index first) as whole numbers: NaN above everything, -0 equal to 0.
-__device__ __forceinline__ unsigned long long top_key(float x, int j) {
+__device__ __forceinline__ u64 top_key(float x, int j) {
   x += 0.0f;
   unsigned b = __float_as_uint(x);
   b = x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-  return (unsigned long long)b << 32 | (unsigned)(0x7fffffff - j);
+  return (u64)b << 32 | (unsigned)(0x7fffffff - j);
+}
+__device__ __forceinline__ float key_value(u64 k) {
+  const unsigned b = (unsigned)(k >> 32);
+  return b == 0xffffffffu ? NAN : __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ int key_index(u64 k) { return 0x7fffffff - (int)(unsigned)k; }
+
+// two f32 at a time
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<u64&>(r))
+      : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)), "l"(reinterpret_cast<u64&>(c)));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-template <class F>
-__device__ float block_reduce(float v, F&& f, float* sm) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = sm[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = f(v, sm[w]);
-  return v;
-}
-
+// The largest of a 16-byte piece (NaN passed over), and its values by twos.
 template <class T>
-__global__ void __launch_bounds__(kThreads) score_kernel(ScoreArgs a) {
-  griddep_wait();
-  __shared__ float sm[kThreads / 32];
-  __shared__ unsigned long long best[kThreads / 32];
-  const int V = a.V;
-  for (long long r = blockIdx.x; r < a.n; r += gridDim.x) {
-    const T* x = static_cast<const T*>(a.x) + r * a.ld;
-    float m = -INFINITY;
-    for (int j = threadIdx.x; j < V; j += kThreads) {
-      const float z = to_f32(x[j]) * a.scale;
-      m = z > m || z != z ? z : m;
-    }
-    m = block_reduce(m, [](float p, float q) { return p != p || p > q ? p : q; }, sm);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f, u = 0.f;
-    for (int j = threadIdx.x; j < V; j += kThreads) {
-      const float t = to_f32(x[j]) * a.scale - ref, e = expf(t);
-      s += e;
-      u += e * (t < -1000.f ? -1000.f : t);
-    }
-    auto add = [](float p, float q) { return p + q; };
-    s = block_reduce(s, add, sm);
-    u = block_reduce(u, add, sm);
-    const float ln = logf(s);
-    if (threadIdx.x == 0) {
-      a.stats[2 * r] = ref;
-      a.stats[2 * r + 1] = ln;
-      const long long t = a.tokens[r];
-      float lp = 0.f;
-      if (t >= V) {
-        atomicExch(a.err, (int)kErrToken);
-        lp = NAN;
-      } else if (t >= 0) {
-        lp = s > 0.f || s != s ? (to_f32(x[t]) * a.scale - ref) - ln : -INFINITY;
-      }
-      a.logprob[r] = lp;
-      if (a.entropy) a.entropy[r] = s == 0.f ? 0.f : ln - u / s;
-    }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < a.top; ++k) {
-      unsigned long long b = 0;
-      for (int j = threadIdx.x; j < V; j += kThreads) {
-        const unsigned long long key = top_key(to_f32(x[j]), j);
-        if (key < last && key > b) b = key;
-      }
+struct Logits;
+template <>
+struct Logits<float> {
+  static __device__ __forceinline__ float top(const uint4& u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& u, int i) {
+    return i ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w))
+             : make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+  }
+};
+template <>
+struct Logits<__nv_bfloat16> {
+  static __device__ __forceinline__ __nv_bfloat162 h(unsigned w) { return reinterpret_cast<__nv_bfloat162&>(w); }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(h(u.x), h(u.y)), __hmax2(h(u.z), h(u.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& u, int i) {
+    const unsigned w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+};
+template <>
+struct Logits<__half> {
+  static __device__ __forceinline__ __half2 h(unsigned w) { return reinterpret_cast<__half2&>(w); }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    const __half2 m = __hmax2(__hmax2(h(u.x), h(u.y)), __hmax2(h(u.z), h(u.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& u, int i) {
+    return __half22float2(h(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w));
+  }
+};
+
+// A share's softmax sums: the maximum m (-inf: nothing yet), s = sum exp(a (x - m)), u = sum exp(a (x - m)) (x - m).
+struct Sums {
+  float m = -INFINITY, s = 0.f, u = 0.f;
+};
+// The sums with the reference moved up to m.
+template <bool ENT>
+__device__ __forceinline__ void move_to(Sums& a, float m, float c) {
+  if (a.m == m) return;
+  const float d = a.m - m, k = a.m == -INFINITY ? 0.f : ex2(d * c);   // (s and u are 0 where the reference was -inf)
+  if (ENT) a.u = k == 0.f ? a.u * k : (a.u + a.s * d) * k;
+  a.s *= k;
+  a.m = m;
+}
+
+template <int NT>
+struct ScoreShared {
+  float group[kGroups];
+  float red[NT / 32 * 3];
+  u64 best[NT / 32];
+  float tau;
+  int n_shares, n_cand, n_ties, n_found;
+  unsigned short shares[kUnroll * NT];
+  u64 cand[kCand + kTies], ties[kTies];
+  // what the cluster's first CTA reads
+  float m, s, u;
+  u64 list[kMaxTop];
+};
+
+// A row in memory: h values up to the first 16-byte boundary, P pieces, and the rest.
+template <class T>
+struct RowShape {
+  const T* x;
+  int V, h, P, rest;
+  __device__ RowShape(const T* p, int v) : x(p), V(v) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+    h = min(V, (16 - off) % 16 / (int)sizeof(T));
+    P = (V - h) / Piece<T>::kN;
+    rest = V - h - P * Piece<T>::kN;
+  }
+  __device__ const uint4* pieces() const { return reinterpret_cast<const uint4*>(x + h); }
+  // the index of the i-th value outside the pieces (i < h + rest)
+  __device__ int edge(int i) const { return i < h ? i : V - rest + (i - h); }
+};
+
+// The CTA's lowest `need` indices of pieces [p0, p1) whose value is v, behind cand[n ..).
+template <class T, int NT>
+__device__ void scan_equal(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, float v, int need, int n) {
+  constexpr int N = Piece<T>::kN;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int found = 0;
+  for (int b = p0; b < p1 && found < need; b += NT) {
+    const int i = b + threadIdx.x;
+    unsigned hit = 0;
+    if (i < p1) {
+      float f[N];
+      Piece<T>::get(row.pieces()[i], f);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        const unsigned long long q = __shfl_xor_sync(0xffffffffu, b, o);
-        b = q > b ? q : b;
-      }
-      __syncthreads();
-      if (threadIdx.x % 32 == 0) best[threadIdx.x / 32] = b;
-      __syncthreads();
-      for (int w = 0; w < kThreads / 32; ++w) b = best[w] > b ? best[w] : b;
-      last = b;
-      if (threadIdx.x == 0) {
-        const int j = 0x7fffffff - (int)(unsigned)b;
-        a.top_ids[r * a.top + k] = j;
-        a.top_lp[r * a.top + k] = s == 0.f ? -INFINITY : (to_f32(x[j]) * a.scale - ref) - ln;
-      }
+      for (int e = 0; e < N; ++e) hit |= (f[e] == v) << e;
+    }
+    int incl = __popc(hit);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int q = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += q;
     }
     __syncthreads();
+    if (lane == 31) sh.red[warp] = __int_as_float(incl);
+    __syncthreads();
+    int at = found + incl - __popc(hit);
+    for (int w = 0; w < NT / 32; ++w) {
+      const int q = __float_as_int(sh.red[w]);
+      if (w < warp) at += q;
+      found += q;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (hit >> e & 1) {
+        if (at < need) sh.cand[n + at] = top_key(v, row.h + i * N + e);
+        ++at;
+      }
+  }
+  if (threadIdx.x == 0) sh.n_found = min(found, need);
+  __syncthreads();
+}
+
+// cand[0 .. n) by rank: the `top` largest to list (0 past them).
+template <int NT>
+__device__ void rank_keys(ScoreShared<NT>& sh, int n, int top) {
+  if (threadIdx.x < kMaxTop) sh.list[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const u64 k = sh.cand[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += sh.cand[j] > k;
+    if (r < top && k) sh.list[r] = k;
+  }
+  __syncthreads();
+}
+
+// One round of the CTA's share of the row for each alternative (-inf left out).
+template <class T, int NT>
+__device__ void top_by_rounds(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, int edges, int top) {
+  constexpr int N = Piece<T>::kN;
+  u64 last = ~0ull;
+  for (int k = 0; k < kMaxTop; ++k) {
+    u64 b = 0;
+    auto take = [&](float x, int j) {
+      const u64 key = x == -INFINITY ? 0 : top_key(x, j);
+      if (key < last && key > b) b = key;
+    };
+    if (k < top) {
+      for (int i = p0 + threadIdx.x; i < p1; i += NT) {
+        float f[N];
+        Piece<T>::get(row.pieces()[i], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) take(f[e], row.h + i * N + e);
+      }
+      if ((int)threadIdx.x < edges) take(to_f32(row.x[row.edge(threadIdx.x)]), row.edge(threadIdx.x));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const u64 q = __shfl_xor_sync(0xffffffffu, b, o);
+      b = q > b ? q : b;
+    }
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) sh.best[threadIdx.x / 32] = b;
+    __syncthreads();
+    for (int w = 0; w < NT / 32; ++w) b = sh.best[w] > b ? sh.best[w] : b;
+    last = b;
+    if (threadIdx.x == 0) sh.list[k] = b;
+  }
+  __syncthreads();
+}
+
+// The CTA's alternatives to list, from the maxima of its threads' shares.
+template <class T, int NT>
+__device__ void find_top(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, int edges, int top,
+                         const float (&share)[kUnroll], bool odd) {
+  constexpr int N = Piece<T>::kN, kLanes = NT / kGroups;
+  const int tid = threadIdx.x;
+  if (odd) {   // (uniform: the CTA's sum is not a number)
+    top_by_rounds(sh, row, p0, p1, edges, top);
+    return;
+  }
+  float g = fmaxf(fmaxf(share[0], share[1]), fmaxf(share[2], share[3]));
+#pragma unroll
+  for (int o = kLanes / 2; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if (tid % kLanes == 0) sh.group[tid / kLanes] = g;
+  if (tid == 0) sh.n_shares = sh.n_cand = sh.n_ties = 0;
+  __syncthreads();
+  if (tid < kGroups) {
+    const float v = sh.group[tid];
+    int r = 0;
+    for (int j = 0; j < kGroups; ++j) r += sh.group[j] > v || (sh.group[j] == v && j < tid);
+    if (r == top - 1) sh.tau = v;
+  }
+  __syncthreads();
+  const float tau = sh.tau;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    if (share[u] >= tau && share[u] > -INFINITY) sh.shares[atomicAdd(&sh.n_shares, 1)] = (unsigned short)(u * NT + tid);
+  auto take = [&](float x, int j) {
+    if (x > tau) {
+      const int at = atomicAdd(&sh.n_cand, 1);
+      if (at < kCand) sh.cand[at] = top_key(x, j);
+    } else if (x == tau && tau > -INFINITY) {
+      const int at = atomicAdd(&sh.n_ties, 1);
+      if (at < kTies) sh.ties[at] = top_key(x, j);
+    }
+  };
+  if (tid < edges) take(to_f32(row.x[row.edge(tid)]), row.edge(tid));
+  __syncthreads();
+  // the shares' pieces, dealt to all threads
+  const int per = (p1 - p0 + kUnroll * NT - 1) / (kUnroll * NT), items = sh.n_shares * per;
+#pragma unroll 2
+  for (int i = tid; i < items; i += NT) {
+    const int f = i / per, at = p0 + sh.shares[f] + (i - f * per) * (kUnroll * NT);
+    if (at >= p1) continue;
+    const uint4 q = row.pieces()[at];
+    if (Logits<T>::top(q) < tau) continue;
+    float v[N];
+    Piece<T>::get(q, v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) take(v[e], row.h + at * N + e);
+  }
+  __syncthreads();
+  const int n = sh.n_cand, ties = sh.n_ties;
+  if (n > kCand) {
+    top_by_rounds(sh, row, p0, p1, edges, top);
+    return;
+  }
+  int more = 0;
+  if (n < top && ties <= kTies) {
+    more = ties;
+    for (int i = tid; i < ties; i += NT) sh.cand[n + i] = sh.ties[i];
+  } else if (n < top) {
+    scan_equal<T, NT>(sh, row, p0, p1, tau, top - n, n);
+    more = sh.n_found;
+    if (tid < edges) {
+      const float x = to_f32(row.x[row.edge(tid)]);
+      sh.cand[n + more + tid] = x == tau ? top_key(x, row.edge(tid)) : 0;
+    }
+    more += edges;
+  }
+  __syncthreads();
+  rank_keys(sh, n + more, top);
+}
+
+// One row by `split` CTAs of a cluster (each a run of its pieces; the first has the values outside the pieces too).
+template <class T, int NT, bool ENT>
+__global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs a) {
+  constexpr int N = Piece<T>::kN;
+  __shared__ ScoreShared<NT> sh;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int C = a.split, part = blockIdx.x % C;
+  const long long r = blockIdx.x / C;
+  const RowShape<T> row(static_cast<const T*>(a.x) + r * a.ld, a.V);
+  const int p0 = (int)((long long)row.P * part / C), p1 = (int)((long long)row.P * (part + 1) / C);
+  const int edges = part == 0 ? row.h + row.rest : 0;
+  const float c = a.scale * 1.4426950408889634f;
+  griddep_wait();
+  Sums t;
+  float share[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) share[u] = -INFINITY;
+  float2 s2 = {0.f, 0.f}, u2 = {0.f, 0.f};
+  const float2 c2 = {c, c};
+  const uint4* piece = row.pieces();
+  long long token = -1;
+  float x_token = 0.f;
+  if (tid == 0 && part == 0) {   // (on its way while the row is read)
+    token = a.tokens[r];
+    if (token >= 0 && token < a.V) x_token = to_f32(row.x[token]);
+  }
+  // q[0 .. n): pieces of one share each
+  auto absorb = [&](const uint4(&q)[kUnroll], int n) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < n) {
+        share[u] = fmaxf(share[u], Logits<T>::top(q[u]));
+        m = fmaxf(m, share[u]);
+      }
+    if (m > t.m) {
+      t.s = s2.x + s2.y;
+      t.u = u2.x + u2.y;
+      move_to<ENT>(t, m, c);
+      s2 = {t.s, 0.f};
+      u2 = {t.u, 0.f};
+    }
+    const float ref = t.m == -INFINITY ? 0.f : -t.m;
+    const float2 ref2 = {ref, ref};
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < n) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float2 d = add2(Logits<T>::pair(q[u], i), ref2);
+          const float2 z = mul2(d, c2), e = {ex2(z.x), ex2(z.y)};
+          s2 = add2(s2, e);
+          if (ENT) {
+            d = {fmaxf(d.x, -FLT_MAX), fmaxf(d.y, -FLT_MAX)};   // (a word of probability 0 adds 0)
+            u2 = fma2(e, d, u2);
+          }
+        }
+      }
+  };
+  int b = p0 + tid;
+  for (; b + (kUnroll - 1) * NT < p1; b += kUnroll * NT) {
+    uint4 q[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(piece + b + u * NT);
+    absorb(q, kUnroll);
+  }
+  {
+    uint4 q[kUnroll];
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (b + u * NT < p1) {
+        q[u] = piece[b + u * NT];
+        n = u + 1;
+      }
+    absorb(q, n);
+  }
+  t.s = s2.x + s2.y;
+  t.u = u2.x + u2.y;
+  if (tid < edges) {   // a value outside the pieces
+    const float x = to_f32(row.x[row.edge(tid)]);
+    if (x > t.m) move_to<ENT>(t, x, c);
+    const float d = x - (t.m == -INFINITY ? 0.f : t.m), e = ex2(d * c);
+    t.s += e;
+    t.u += e * fmaxf(d, -FLT_MAX);
+  }
+  // the CTA's sums: the maximum first
+  float m = t.m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) sh.red[warp] = m;
+  __syncthreads();
+  for (int w = 0; w < NT / 32; ++w) m = fmaxf(m, sh.red[w]);
+  move_to<ENT>(t, m, c);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    t.s += __shfl_xor_sync(0xffffffffu, t.s, o);
+    if (ENT) t.u += __shfl_xor_sync(0xffffffffu, t.u, o);
+  }
+  if (lane == 0) {
+    sh.red[NT / 32 + warp] = t.s;
+    sh.red[2 * (NT / 32) + warp] = t.u;
+  }
+  __syncthreads();
+  t.s = t.u = 0.f;
+  for (int w = 0; w < NT / 32; ++w) {
+    t.s += sh.red[NT / 32 + w];
+    if (ENT) t.u += sh.red[2 * (NT / 32) + w];
+  }
+  if (a.top) {
+    __syncthreads();   // red is free
+    find_top<T, NT>(sh, row, p0, p1, edges, a.top, share, t.s != t.s);
+  }
+  if (C > 1) {   // the row's from its CTAs'
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) {
+      sh.m = t.m;
+      sh.s = t.s;
+      sh.u = t.u;
+    }
+    cluster.sync();
+    if (part == 0) {
+      m = t.m;
+      for (int k = 1; k < C; ++k) m = fmaxf(m, *cluster.map_shared_rank(&sh.m, k));
+      move_to<ENT>(t, m, c);
+      for (int k = 1; k < C; ++k) {
+        Sums o;
+        o.m = *cluster.map_shared_rank(&sh.m, k);
+        o.s = *cluster.map_shared_rank(&sh.s, k);
+        o.u = *cluster.map_shared_rank(&sh.u, k);
+        move_to<ENT>(o, m, c);
+        t.s += o.s;
+        t.u += o.u;
+      }
+      if (a.top) {
+        for (int i = tid; i < C * kMaxTop; i += NT)
+          sh.cand[i] = cluster.map_shared_rank(&sh, i / kMaxTop)->list[i % kMaxTop];
+        __syncthreads();
+        rank_keys(sh, C * kMaxTop, a.top);
+      }
+    }
+    cluster.sync();   // (what the first CTA reads is there until then)
+    if (part) return;
+  }
+  const float ref = t.m == -INFINITY ? 0.f : t.m, ln = logf(t.s);
+  auto ln_p = [&](float x) { return ln == -INFINITY ? -INFINITY : fmaf(x - ref, a.scale, -ln); };
+  if (tid == 0) {
+    a.stats[2 * r] = ref;
+    a.stats[2 * r + 1] = ln;
+    if (token >= a.V) atomicExch(a.err, (int)kErrToken);
+    a.logprob[r] = token < 0 ? 0.f : token < a.V ? ln_p(x_token) : NAN;
+    if (ENT) a.entropy[r] = t.s == 0.f ? 0.f : ln - a.scale * (t.u / t.s);
+  }
+  if (!a.top) return;
+  // fewer words than alternatives: those of probability 0, the lowest indices first
+  int have = 0;
+  for (int k = 0; k < a.top; ++k) have += sh.list[k] != 0;
+  if (have < a.top) {
+    if (tid == 0) sh.n_found = 0;
+    __syncthreads();
+    const int need = a.top - have;
+    for (int b0 = 0; b0 < a.V; b0 += NT) {
+      const int at = sh.n_found, j = b0 + tid;
+      if (at >= need) break;
+      const bool hit = j < a.V && to_f32(row.x[j]) == -INFINITY;
+      const unsigned mask = __ballot_sync(0xffffffffu, hit);
+      __syncthreads();
+      if (lane == 0) sh.red[warp] = __int_as_float(__popc(mask));
+      __syncthreads();
+      int k = at + __popc(mask & ((1u << lane) - 1)), all = at;
+      for (int w = 0; w < NT / 32; ++w) {
+        const int q = __float_as_int(sh.red[w]);
+        if (w < warp) k += q;
+        all += q;
+      }
+      if (hit && k < need) sh.list[have + k] = top_key(-INFINITY, j);
+      if (tid == 0) sh.n_found = all;
+      __syncthreads();
+    }
+    __syncthreads();
+  }
+  if (tid < a.top) {
+    const u64 k = sh.list[tid];
+    a.top_ids[r * a.top + tid] = key_index(k);
+    a.top_lp[r * a.top + tid] = ln_p(key_value(k));
   }
 }
 
@@ -120,46 +529,136 @@ struct GradArgs {
   long long ldd;
   int* err;
   float scale;
-  int n, V, top;
+  int n, V, top, split;   // split: CTAs to a row
 };
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) score_grad_kernel(GradArgs a) {
+// 16 bytes from byte sh of lo | hi
+__device__ __forceinline__ uint4 join_bytes(const uint4& lo, const uint4& hi, int sh) {
+  const int b = (sh & 3) * 8;
+  auto f = [&](unsigned p, unsigned q) { return __funnelshift_r(p, q, b); };
+  switch (sh >> 2) {   // (the same for a whole row)
+    case 0: return make_uint4(f(lo.x, lo.y), f(lo.y, lo.z), f(lo.z, lo.w), f(lo.w, hi.x));
+    case 1: return make_uint4(f(lo.y, lo.z), f(lo.z, lo.w), f(lo.w, hi.x), f(hi.x, hi.y));
+    case 2: return make_uint4(f(lo.z, lo.w), f(lo.w, hi.x), f(hi.x, hi.y), f(hi.y, hi.z));
+    default: return make_uint4(f(lo.w, hi.x), f(hi.x, hi.y), f(hi.y, hi.z), f(hi.z, hi.w));
+  }
+}
+
+// dx = p (A + B log2 p) with A = -a (g + g_H H), g the sum of the words' own gradients, B = -a g_H ln 2; the words with
+// a gradient of their own (the token, the alternatives) are put right at the end. A CTA has a run of the 16-byte pieces
+// of the result's row; a row of logits that starts elsewhere within its 16 bytes is read in aligned pieces and shifted
+// (509 rows of 50303 f16 words: see the table of measurements in the documentation).
+template <class T, bool ENT>
+__global__ void __launch_bounds__(kGradThreads, 4) score_grad_kernel(GradArgs a) {
+  constexpr int N = Piece<T>::kN, kWords = kMaxTop + 1;
+  __shared__ float x_at[kWords], g_at[kWords];
+  __shared__ int at[kWords];
+  const int tid = threadIdx.x, lane = tid % 32, V = a.V;
+  const int C = a.split, part = blockIdx.x % C;
+  const long long r = blockIdx.x / C;
+  const T* x = static_cast<const T*>(a.x) + r * a.ld;
+  const RowShape<T> row(static_cast<T*>(a.d) + r * a.ldd, V);
+  T* d = static_cast<T*>(a.d) + r * a.ldd;
   griddep_wait();
-  __shared__ float x_at[kMaxTop + 1], g_at[kMaxTop + 1];
-  __shared__ int at[kMaxTop + 1];
-  const int V = a.V, tid = threadIdx.x;
-  for (long long r = blockIdx.x; r < a.n; r += gridDim.x) {
-    const T* x = static_cast<const T*>(a.x) + r * a.ld;
-    T* d = static_cast<T*>(a.d) + r * a.ldd;
-    __syncthreads();
-    // the words with a gradient of their own: the token, then the alternatives
-    if (tid <= a.top) {
-      const long long j = tid == 0 ? a.tokens[r] : a.top_ids[r * a.top + tid - 1];
-      float g = tid == 0 ? (a.g_lp ? a.g_lp[r] : 0.f) : a.g_top[r * a.top + tid - 1];
-      const bool ok = j >= 0 && j < V && a.stats[2 * r + 1] != -INFINITY;   // (a row without a word has no gradient)
-      if (j >= V || (j < 0 && tid)) atomicExch(a.err, (int)kErrToken);
-      at[tid] = ok ? (int)j : -1;
-      g_at[tid] = ok ? g : 0.f;
-      x_at[tid] = ok ? to_f32(x[j]) : 0.f;
+  const float m = a.stats[2 * r], ln = a.stats[2 * r + 1];
+  const bool some = ln != -INFINITY;   // (a row without a word has no gradient)
+  // the words with a gradient of their own: every warp sums them, the CTA keeps them
+  auto word = [&](int k, float& g) {
+    const long long j = k == kMaxTop ? a.tokens[r] : k < a.top ? a.top_ids[r * a.top + k] : -1;
+    const bool ok = j >= 0 && j < V;
+    if (part == 0 && (j >= V || (j < 0 && k < a.top))) atomicExch(a.err, (int)kErrToken);
+    g = !ok || !some ? 0.f : k < kMaxTop ? a.g_top[r * a.top + k] : a.g_lp ? a.g_lp[r] : 0.f;
+    return ok && some ? (int)j : -1;
+  };
+  float g, g_token;
+  const int j_top = word(lane, g), j_token = word(kMaxTop, g_token);
+  if (tid < 32) {
+    at[tid] = j_top;
+    g_at[tid] = g;
+    x_at[tid] = j_top < 0 ? 0.f : to_f32(x[j_top]);
+    if (tid == 0) {
+      at[kMaxTop] = j_token;
+      g_at[kMaxTop] = g_token;
+      x_at[kMaxTop] = j_token < 0 ? 0.f : to_f32(x[j_token]);
     }
-    __syncthreads();
-    float g = 0.f;
-    for (int k = 0; k <= a.top; ++k) g += g_at[k];
-    const float m = a.stats[2 * r], ln = a.stats[2 * r + 1];
-    const float gh = a.g_h ? a.g_h[r] : 0.f, h = a.g_h ? a.entropy[r] : 0.f;
-    auto base = [&](float xv) {
-      const float t = (xv * a.scale - m) - ln;
-      const float p = ln == -INFINITY ? 0.f : expf(t);
-      return -p * (g + gh * ((t < -1000.f ? -1000.f : t) + h));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) g += __shfl_xor_sync(0xffffffffu, g, o);
+  g += g_token;
+  if (a.x == a.d) __syncthreads();   // (the words are read before any is overwritten)
+  const float gh = ENT && some ? a.g_h[r] : 0.f;
+  const float A = -a.scale * (g + (ENT ? gh * a.entropy[r] : 0.f)), B = -a.scale * gh * 0.6931471805599453f;
+  const float c = a.scale * 1.4426950408889634f, l2 = ln * 1.4426950408889634f;
+  const bool none = g == 0.f && gh == 0.f;
+  auto one = [&](float xv) {
+    if (none) return 0.f;
+    const float t = fmaf(xv - m, c, -l2), e = ex2(t);
+    return e * (ENT ? fmaf(fmaxf(t, -1e4f), B, A) : A);
+  };
+  const int p0 = (int)((long long)row.P * part / C), p1 = (int)((long long)row.P * (part + 1) / C);
+  uint4* dp = reinterpret_cast<uint4*>(d + row.h);
+  if (none) {
+    for (int i = p0 + tid; i < p1; i += kGradThreads) dp[i] = make_uint4(0, 0, 0, 0);
+  } else {
+    const float2 m2 = {-m, -m}, c2 = {c, c}, n2 = {-l2, -l2}, A2 = {A, A}, B2 = {B, B};
+    const uint8_t* xs = reinterpret_cast<const uint8_t*>(x + row.h);
+    const int sh = (int)(reinterpret_cast<uintptr_t>(xs) & 15);
+    const uint4* xp = reinterpret_cast<const uint4*>(xs - sh);
+    auto put = [&](int i, const uint4& q) {
+      float f[N];
+#pragma unroll
+      for (int k = 0; k < N / 2; ++k) {
+        float2 t = fma2(add2(Logits<T>::pair(q, k), m2), c2, n2);
+        float2 o = {ex2(t.x), ex2(t.y)};
+        if (ENT) {
+          t = {fmaxf(t.x, -1e4f), fmaxf(t.y, -1e4f)};   // (a word of probability 0 gets 0)
+          o = mul2(o, fma2(t, B2, A2));
+        } else {
+          o = mul2(o, A2);
+        }
+        f[2 * k] = o.x;
+        f[2 * k + 1] = o.y;
+      }
+      dp[i] = Piece<T>::put(f);
     };
-    for (int j = tid; j < V; j += kThreads) d[j] = from_f32<T>(base(to_f32(x[j])) * a.scale);
-    __syncthreads();
-    if (tid <= a.top && at[tid] >= 0) {
+    if (sh == 0) {
+      int i = p0 + tid;
+      for (; i + (kUnroll - 1) * kGradThreads < p1; i += kUnroll * kGradThreads) {
+        uint4 q[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(xp + i + u * kGradThreads);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) put(i + u * kGradThreads, q[u]);
+      }
+      for (; i < p1; i += kGradThreads) put(i, __ldcs(xp + i));
+    } else {
+      // a piece of the result spans two of the logits; those at the row's ends may reach past it
+      const int f0 = row.h * (int)sizeof(T) >= sh ? 0 : 1;
+      const long long left = (long long)(V - row.h) * (int)sizeof(T) + sh;   // bytes from xp to the row's end
+      const int f1 = (int)min((long long)row.P, (left - 16) / 16);
+      for (int i = p0 + tid; i < p1; i += kGradThreads) {
+        if (i >= f0 && i < f1) {
+          put(i, join_bytes(xp[i], xp[i + 1], sh));
+        } else {
+          for (int e = 0; e < N; ++e) d[row.h + i * N + e] = from_f32<T>(one(to_f32(x[row.h + i * N + e])));
+        }
+      }
+    }
+  }
+  if (part == 0 && tid < row.h + row.rest) {
+    const int j = row.edge(tid);
+    d[j] = from_f32<T>(one(to_f32(x[j])));
+  }
+  __syncthreads();
+  const int k0 = tid < kMaxTop ? tid : kMaxTop;
+  if (tid <= kMaxTop && at[k0] >= 0) {
+    const int j = at[k0], i = (j - row.h) / N;
+    const bool edge = j < row.h || j >= V - row.rest;
+    if (edge ? part == 0 : i >= p0 && i < p1) {
       float v = 0.f;
-      for (int k = 0; k <= a.top; ++k)
-        if (at[k] == at[tid]) v += g_at[k];
-      d[at[tid]] = from_f32<T>((base(x_at[tid]) + v) * a.scale);
+      for (int k = 0; k < kWords; ++k)
+        if (at[k] == j) v += g_at[k];
+      d[j] = from_f32<T>(fmaf(v, a.scale, one(x_at[k0])));
     }
   }
 }
@@ -168,11 +667,34 @@ bool rows_ok(long long ld, int V, const void* p, int type) {
   return p && ld >= V && aligned(p, type_bytes(type));
 }
 
-template <class T>
-int prepare_type() {
-  return load_kernel(score_kernel<T>) || load_kernel(score_grad_kernel<T>) ? -3 : 0;
+// CTAs to a row. With 4 CTAs of 256 threads an SM streams 11 B/ns a CTA, and a CTA has some 3 us to spend besides; the
+// split with the shortest ceil(CTAs / 592) (bytes / split / rate + 3 us) is taken. Where 8 CTAs to a row leave SMs
+// free, CTAs of 1024 threads have a row's whole share in flight at once.
+template <class T, bool ENT>
+int score_launch(ScoreArgs& k, cudaStream_t st) {
+  if ((long long)k.n * 8 <= kSMs) {
+    k.split = 8;
+    return launch_pdl_cluster(score_kernel<T, 1024, ENT>, dim3(k.n * 8), dim3(1024), 0, st, 8, k);
+  }
+  const double bytes = (double)k.V * sizeof(T);
+  double best = 1e300;
+  for (int c = 1; c <= 8; c *= 2) {
+    if ((long long)k.n * c > 0x7fffffffLL) break;
+    const long long waves = ((long long)k.n * c + 4 * kSMs - 1) / (4 * kSMs);
+    const double us = waves * (bytes / c / 11e3 + 3.0);
+    if (us < best) best = us, k.split = c;
+  }
+  return k.split == 1 ? launch_pdl(score_kernel<T, 256, ENT>, dim3(k.n), dim3(256), 0, st, k)
+                      : launch_pdl_cluster(score_kernel<T, 256, ENT>, dim3(k.n * k.split), dim3(256), 0, st, k.split, k);
 }
 
+template <class T>
+int prepare_type() {
+  if (load_kernel(score_kernel<T, 256, false>) || load_kernel(score_kernel<T, 256, true>) ||
+      load_kernel(score_kernel<T, 1024, false>) || load_kernel(score_kernel<T, 1024, true>))
+    return -3;
+  return load_kernel(score_grad_kernel<T, false>) || load_kernel(score_grad_kernel<T, true>) ? -3 : 0;
+}
 }  // namespace
 
 int logprobs_prepare() {
@@ -200,10 +722,11 @@ int tb2_logprobs(const tb2_logprobs_args* a, void* stream) {
   int* err = device_error_word();
   if (!err) return -3;
   ScoreArgs k = {a->logits, a->ld, a->tokens, a->logprob, a->stats, a->entropy, a->top_logprobs, a->top_ids, err,
-                 a->scale, a->n_rows, a->vocab, a->top};
+                 a->scale, a->n_rows, a->vocab, a->top, 1};
   return by_row_type(a->row_type, [&](auto t) {
-    return launch_pdl(score_kernel<decltype(t)>, dim3(a->n_rows), dim3(kThreads), 0, static_cast<cudaStream_t>(stream),
-                      k);
+    using T = decltype(t);
+    return a->entropy ? score_launch<T, true>(k, static_cast<cudaStream_t>(stream))
+                      : score_launch<T, false>(k, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -222,10 +745,15 @@ int tb2_logprobs_grad(const tb2_logprobs_grad_args* a, void* stream) {
   int* err = device_error_word();
   if (!err) return -3;
   GradArgs k = {a->logits, a->ld, a->tokens, a->stats, a->entropy, a->g_logprob, a->g_entropy, a->g_top, a->top_ids,
-                a->d_logits, a->ldd, err, a->scale, a->n_rows, a->vocab, a->top};
+                a->d_logits, a->ldd, err, a->scale, a->n_rows, a->vocab, a->top, 1};
   return by_row_type(a->row_type, [&](auto t) {
-    return launch_pdl(score_grad_kernel<decltype(t)>, dim3(a->n_rows), dim3(kThreads), 0,
-                      static_cast<cudaStream_t>(stream), k);
+    using T = decltype(t);
+    // runs of 64 KB, so that the last CTAs end together; less where that leaves SMs without one, 4 KB at least
+    const long long bytes = (long long)k.V * sizeof(T);
+    long long c = std::max((bytes + 65535) / 65536, std::min((4LL * kSMs + k.n - 1) / k.n, bytes / 4096));
+    k.split = (int)std::max(1LL, std::min(c, 0x7fffffffLL / k.n));
+    return launch_pdl(k.g_h ? score_grad_kernel<T, true> : score_grad_kernel<T, false>, dim3(k.n * k.split),
+                      dim3(kGradThreads), 0, static_cast<cudaStream_t>(stream), k);
   });
 }
 

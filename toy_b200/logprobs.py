@@ -31,7 +31,7 @@ class TokenLogprobs(NamedTuple):
     entropy: Optional[torch.Tensor]         # [n] f32
     top_ids: Optional[torch.Tensor]         # [n, top] i64, the largest logit first, equal ones by the lower index
     top_logprobs: Optional[torch.Tensor]    # [n, top] f32
-    stats: torch.Tensor                     # [n, 2] f32: m = max(scale * row) and ln sum exp(scale * row - m)
+    stats: torch.Tensor                     # [n, 2] f32: m = max(row) and ln sum exp(scale * (row - m))
 
 
 def _logits(x: torch.Tensor, tokens: torch.Tensor, scale: float, top: int) -> tuple:
