@@ -16,6 +16,7 @@
 #include <cmath>
 #include <cstring>
 #include <iterator>
+#include <type_traits>
 
 #include "rows.cuh"
 #include "runtime.cuh"
@@ -25,11 +26,11 @@ namespace {
 
 constexpr int kBlock = 256;        // values that share a scale
 constexpr int kMaxTensors = 448;   // tensors a launch: their descriptors travel as its arguments (30.5 of 32 KB)
-constexpr int kThreads = 256, kWarps = kThreads / 32, kCtasPerSm = 4;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kCtasPerSm = 3;
 
 struct Tensors {
   tb2_adamw_tensor t[kMaxTensors];
-  int first[kMaxTensors + 1];             // blocks before tensor i
+  int first[kMaxTensors + 2];             // blocks before tensor i; behind the last one, all
   unsigned whole[(kMaxTensors + 31) / 32];   // bit i: tensor i's arrays are on the boundaries of four values
   int n;
 };
@@ -45,21 +46,15 @@ __device__ __forceinline__ int tensor_of(const Tensors& ts, int b) {
   return lo;
 }
 
+// On from tensor i to the one that block b is of: a step or two, or a search where tensors are small.
+__device__ __forceinline__ int tensor_from(const Tensors& ts, int i, int b) {
+  if (ts.first[i + 1] > b) return i;
+  if (ts.first[i + 2] > b) return i + 1;   // (first has an entry past the last tensor's end)
+  return tensor_of(ts, b);
+}
+
 // Four values: a lane has values 4 lane .. 4 lane + 3 and 128 more of a block, so that a warp's reads and writes are
 // contiguous in every type.
-template <class T>
-__device__ __forceinline__ void load4(const void* p, long long i, float* f) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-  } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const T*>(p) + i);
-    T t[4];
-    memcpy(t, &u, 8);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f[k] = to_f32<T>(t[k]);
-  }
-}
 template <class T>
 __device__ __forceinline__ void store4(void* p, long long i, const float* f) {
   if constexpr (sizeof(T) == 4) {
@@ -94,69 +89,157 @@ __device__ __noinline__ unsigned e4m3_of(double t) {
   return __nv_cvt_float_to_fp8((float)q, __NV_SATFINITE, __NV_E4M3);
 }
 
-// Whether t >= 0, as a multiple of the scale, is within `ulps` of the border between two codes: bits below an e4m3
-// value's three, next to their half. (Below 2^-6 codes are 2^-9 apart, as they are just above it.)
-__device__ __forceinline__ bool near_border(float t, unsigned ulps) {
-  const unsigned b = __float_as_uint(t < 0.015625f ? t + 0.015625f : t) & 0xfffffu;
-  return b - (0x80000u - ulps) <= 2 * ulps;
+// Whether t >= 0, as a multiple of the scale, is within eight units in the last place of the border between two codes:
+// the bits below an e4m3 value's three, next to their half. (Below 2^-6 codes are 2^-9 apart, as they are just above.)
+__device__ __forceinline__ bool near_border(float t) {
+  const unsigned b = __float_as_uint(t < 0.015625f ? t + 0.015625f : t) * 4096u;
+  return b - ((0x80000u - 8) << 12) <= (16u << 12);
 }
 
-// A block's power of two, from the bits of its largest magnitude, and the factor to it: the smallest 2^e with top <=
-// 448 2^e (448 = 1.75 2^8), 2^-100 at least; NaN where top is not finite.
-__device__ __forceinline__ float block_scale(unsigned top, float& inverse) {
-  const int e = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), -100);
-  const bool ok = top < 0x7f800000u;
+__device__ __forceinline__ float sqrt_near(float x) {   // within 2^-23; below 2^-126: 0
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float inverse_near(float x) {   // within 2^-23
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The larger magnitude, NaN above all.
+__device__ __forceinline__ float top_of(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+
+// A block's power of two, from its largest magnitude, and the factor to it: the smallest 2^e with top <= 448 2^e (448 =
+// 1.75 2^8), 2^-100 at least; NaN where top is not finite.
+__device__ __forceinline__ float block_scale(float top, float& inverse) {
+  const unsigned b = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
+  const int e = max((int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u), -100);
+  const bool ok = b < 0x7f800000u;
   inverse = ok ? __uint_as_float((unsigned)(127 - e) << 23) : NAN;
   return ok ? __uint_as_float((unsigned)(127 + e) << 23) : NAN;
 }
 
-// One value's step, in f32 but for 8-bit m: that is a sum of two terms of either sign, and rounding it once to a code
-// needs it to more bits than a product and a sum in f32 leave after a cancellation. FP64 has the room: two products
-// and three conversions a value are a tenth of what the FP64 pipe does in the time of a value's 16 bytes.
+// f64 to f32 so that rounding the result to few bits rounds the f64 value once: cut, the last bit set where that left
+// something out.
+__device__ __forceinline__ float to_odd(double x) {
+  const float f = __double2float_rz(x);
+  return __uint_as_float(__float_as_uint(f) | ((__double2loint(x) & 0x1fffffff) != 0));
+}
+
+// The step's factors.
 struct Hyper {
-  float a, b1, b2, eps, keep, c1, c2, gf, d1, d2;
+  float b1, b2, eps, keep, c1, c2, gf, d1, d2;
+  float sb2, sd2;   // sqrt(b2), the factor times sqrt(1 - b2)
   double db1, dgm;
+};
+
+// The code of a second moment's root next to a border, from 64 bits.
+__device__ __noinline__ unsigned root_code(float g, float gf, float r0, float b2, float inverse) {
+  const double gw = (double)g * gf, v = (double)r0 * r0 * b2 + gw * gw * (1.0 - (double)b2);
+  return max(e4m3_of(sqrt(v) * inverse), 1u);
+}
+
+// A warp has a block at a time; a CTA a run of blocks.
+//
+// The step is f32 but for 8-bit m: that is a sum of two terms of either sign, and to be rounded once to a code it is
+// needed to more bits than a product and a sum in f32 leave after a cancellation. FP64 has the room (two products and
+// three conversions a value), and a conversion that keeps what it cuts as a set last bit needs no second look. The root
+// of v is all positive terms: with U = 2^-24, sqrt(b2) and the held root's factor, that product and its square 2 + 2 +
+// 2 + 1 U, the gradient's as much, the sum 1, which the root halves, and its own 2 U: 6 U. The few (one in 30000) that
+// come within 8 units in the last place (U or more each) of a border are rounded again from 64 bits.
+//
+// Bound by HBM in 32 bits. In 8 bits a value is 16 bytes and (with these choices) some 50 instructions, near both
+// limits: IEEE quotients and roots, flags for each value and a second look at m made it 103 and 508 us where the bytes
+// of 135M weights take 332.
+// A lane's values of a block as they lie in memory.
+template <class T>
+struct Raw4 {
+  typename std::conditional<sizeof(T) == 4, float4, typename std::conditional<sizeof(T) == 2, uint2, unsigned>::type>::type v;
+  __device__ __forceinline__ void load(const void* p, long long i) {
+    v = __ldcs(reinterpret_cast<const decltype(v)*>(static_cast<const T*>(p) + i));
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else if constexpr (sizeof(T) == 2) {
+      T t[4];
+      memcpy(t, &v, 8);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = to_f32<T>(t[k]);
+    } else {
+      load4_e4m3(v, f);
+    }
+  }
+};
+template <class P, class G, class S>
+struct RawBlock {
+  Raw4<P> p[2];
+  Raw4<G> g[2];
+  Raw4<S> m[2], v[2];
+  float ms, vs;
 };
 
 template <class P, class G, int BITS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid_constant__ Tensors ts, int copy_type,
                                                                     const float* hp, const float* factor) {
+  using S = typename std::conditional<BITS == 8, uint8_t, float>::type;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int all = ts.first[ts.n];
-  const int b0 = (int)((long long)all * blockIdx.x / gridDim.x), b1 = (int)((long long)all * (blockIdx.x + 1) / gridDim.x);
-  int i = tensor_of(ts, min(b0 + warp, all - 1));
+  const int warps = gridDim.x * kWarps;
+  int b = blockIdx.x * kWarps + warp;
+  int i = tensor_of(ts, min(b, all - 1));
   griddep_wait();
   Hyper h;
-  h.a = hp[0]; h.b1 = hp[1]; h.b2 = hp[2]; h.eps = hp[3];
-  h.keep = 1.f - h.a * hp[4];
-  h.c1 = h.a * hp[5];
+  h.b1 = hp[1]; h.b2 = hp[2]; h.eps = hp[3];
+  h.keep = 1.f - hp[0] * hp[4];
+  h.c1 = hp[0] * hp[5];
   h.c2 = sqrtf(hp[6]);
   h.gf = factor ? *factor : 1.f;
   h.d1 = 1.f - h.b1;
   h.d2 = 1.f - h.b2;
+  h.sb2 = sqrtf(h.b2);
+  h.sd2 = h.gf * sqrtf(h.d2);
   h.db1 = h.b1;
   h.dgm = (1.0 - h.db1) * (double)h.gf;
-  for (int b = b0 + warp; b < b1; b += kWarps) {
-    while (ts.first[i + 1] <= b) ++i;
+  // block b of tensor i: read as it lies where that is possible (a whole block on its boundaries)
+  RawBlock<P, G, S> raw;
+  auto fetch = [&](int b) {
     const tb2_adamw_tensor& t = ts.t[i];
     const int blk = b - ts.first[i];
     const long long k0 = (long long)blk * kBlock + 4 * lane;
     const bool whole = (ts.whole[i / 32] >> (i % 32) & 1) && (long long)(blk + 1) * kBlock <= t.n;
-    float p[8], g[8], m[8], r[8];
-    float ms = 0.f, vs = 0.f;
-    if (BITS == 8) ms = t.m_scale[blk], vs = t.v_scale[blk];
+    if (BITS == 8) raw.ms = t.m_scale[blk], raw.vs = t.v_scale[blk];
     if (whole) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        load4<P>(t.p, k0 + 128 * j, p + 4 * j);
-        load4<G>(t.g, k0 + 128 * j, g + 4 * j);
-        if (BITS == 8) {
-          load4_e4m3(*reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(t.m) + k0 + 128 * j), m + 4 * j);
-          load4_e4m3(*reinterpret_cast<const unsigned*>(static_cast<const uint8_t*>(t.v) + k0 + 128 * j), r + 4 * j);
-        } else {
-          load4<float>(t.m, k0 + 128 * j, m + 4 * j);
-          load4<float>(t.v, k0 + 128 * j, r + 4 * j);
-        }
+        raw.p[j].load(t.p, k0 + 128 * j);
+        raw.g[j].load(t.g, k0 + 128 * j);
+        raw.m[j].load(t.m, k0 + 128 * j);
+        raw.v[j].load(t.v, k0 + 128 * j);
+      }
+    }
+    return whole;
+  };
+  if (b >= all) return;
+  bool next_whole = fetch(b);
+  for (; b < all; b += warps) {
+    const tb2_adamw_tensor& t = ts.t[i];
+    const int blk = b - ts.first[i];
+    const long long k0 = (long long)blk * kBlock + 4 * lane;
+    const bool whole = next_whole;
+    float p[8], g[8], m[8], r[8];
+    const float ms = raw.ms, vs = raw.vs;
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        raw.p[j].get(p + 4 * j);
+        raw.g[j].get(g + 4 * j);
+        raw.m[j].get(m + 4 * j);
+        raw.v[j].get(r + 4 * j);
       }
     } else {   // a tensor's end, or one off its boundaries
 #pragma unroll
@@ -174,71 +257,67 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
         }
       }
     }
-    double wide[8];   // m, to more bits
-    float r0[8];      // the held root of v
-    unsigned top_m = 0, top_r = 0;
+    int i_next = i;
+    if (all - b > warps) {   // the next block is on its way while this one is computed
+      const int i_now = i;
+      i = tensor_from(ts, i, b + warps);
+      next_whole = fetch(b + warps);
+      i_next = i;
+      i = i_now;
+    }
+    float top_m = 0.f, top_r = 0.f;
+    const float rs = BITS == 8 ? vs * h.sb2 : 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float gg = g[e] * h.gf;
       float v;
       if (BITS == 8) {
-        wide[e] = fma((double)(m[e] * ms), h.db1, (double)g[e] * h.dgm);
-        m[e] = (float)wide[e];
-        r0[e] = r[e] * vs;   // exact, its square too
-        v = fmaf(r0[e] * r0[e], h.b2, gg * gg * h.d2);
-        v = v < FLT_MIN ? 0.f : v;   // (what f32 does not hold to its full bits counts as 0)
+        m[e] = to_odd(fma((double)(m[e] * ms), h.db1, (double)g[e] * h.dgm));
+        const float gs = g[e] * h.sd2, r0 = r[e] * rs;
+        v = fmaf(gs, gs, r0 * r0);
       } else {
+        const float gg = g[e] * h.gf;
         m[e] = fmaf(m[e], h.b1, gg * h.d1);
         v = fmaf(r[e], h.b2, gg * gg * h.d2);
       }
-      const float root = sqrtf(v);
-      p[e] = fmaf(p[e], h.keep, -(h.c1 * m[e]) / fmaf(root, h.c2, h.eps));
+      const float root = sqrt_near(v);
+      p[e] = fmaf(-h.c1 * m[e], inverse_near(fmaf(root, h.c2, h.eps)), p[e] * h.keep);
       r[e] = BITS == 8 ? root : v;
       if (BITS == 8) {
-        top_m = max(top_m, __float_as_uint(fabsf(m[e])));
-        top_r = max(top_r, __float_as_uint(root));
+        top_m = top_of(top_m, m[e]);
+        top_r = top_of(top_r, root);
       }
     }
     unsigned mq[2], vq[2];
     if (BITS == 8) {
       float mi, ri;
-      const float nms = block_scale(__reduce_max_sync(0xffffffffu, top_m), mi);
-      const float nvs = block_scale(__reduce_max_sync(0xffffffffu, top_r), ri);
-      if (lane == 0) t.m_scale[blk] = nms, t.v_scale[blk] = nvs;
-      unsigned redo = 0;   // bit e: m's code, bit e + 8: the root's, to be rounded from more bits
+      const float nms = block_scale(top_m, mi), nvs = block_scale(top_r, ri);
+      bool look = false;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float tm[4], tr[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int k = 4 * j + e;
-          tm[e] = m[k] * mi;
-          tr[e] = r[k] * ri;
-          redo |= near_border(fabsf(tm[e]), 1) << k;                                      // m is rounded once
-          redo |= near_border(tr[e], 8) << (k + 8);   // 4 units off at most (2^-24 each: g, its square, the product,
-          // the sum, half of these behind the root, and the root)
+          tm[e] = m[4 * j + e] * mi;
+          tr[e] = r[4 * j + e] * ri;
+          look |= near_border(tr[e]);
+          r[4 * j + e] = tr[e];
+          tr[e] = tr[e] > 0.f ? fmaxf(tr[e], 0.001953125f) : tr[e];   // a positive root keeps the smallest code
         }
         mq[j] = pack4_e4m3(tm);
         vq[j] = pack4_e4m3(tr);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (tr[e] > 0.f && (vq[j] >> 8 * e & 0xff) == 0) vq[j] |= 1u << 8 * e;   // a positive root stays so
       }
-      if (redo && mi == mi && ri == ri) {
+      if (look) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int at = 8 * (k % 4);
-          if (redo >> k & 1) {
-            const unsigned q = e4m3_of(fabs(wide[k]) * mi) | (wide[k] < 0.0 ? 0x80 : 0);
-            mq[k / 4] = (mq[k / 4] & ~(0xffu << at)) | q << at;
-          }
-          if (redo >> (k + 8) & 1) {
-            const double gw = (double)g[k] * h.gf, vw = (double)r0[k] * r0[k] * h.b2 + gw * gw * (1.0 - (double)h.b2);
-            const unsigned q = max(e4m3_of(sqrt(vw) * ri), 1u);
-            vq[k / 4] = (vq[k / 4] & ~(0xffu << at)) | q << at;
-          }
+        for (int e = 0; e < 8; ++e) {
+          if (!near_border(r[e])) continue;
+          const long long k = k0 + 128 * (e / 4) + e % 4;
+          if (k >= t.n) continue;
+          const float r0 = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(t.v)[k], __NV_E4M3)));
+          const unsigned q = root_code(to_f32(static_cast<const G*>(t.g)[k]), h.gf, r0 * vs, h.b2, ri);
+          vq[e / 4] = (vq[e / 4] & ~(0xffu << 8 * (e % 4))) | q << 8 * (e % 4);
         }
       }
+      if (lane == 0) t.m_scale[blk] = nms, t.v_scale[blk] = nvs;
     }
     if (whole) {
 #pragma unroll
@@ -282,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
         }
       }
     }
+    i = i_next;
   }
 }
 
@@ -290,15 +370,49 @@ template <bool PUT>
 __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ Tensors ts) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int all = ts.first[ts.n];
-  const int b0 = (int)((long long)all * blockIdx.x / gridDim.x), b1 = (int)((long long)all * (blockIdx.x + 1) / gridDim.x);
-  int i = tensor_of(ts, min(b0 + warp, all - 1));
+  const int warps = gridDim.x * kWarps;
+  constexpr int kRun = 4;   // blocks of a warp in a row: so many reads are on their way at once
+  long long b = ((long long)blockIdx.x * kWarps + warp) * kRun, end = min(b + kRun, (long long)all);
+  int i = tensor_of(ts, (int)min(b, all - 1LL));
   griddep_wait();
-  for (int b = b0 + warp; b < b1; b += kWarps) {
-    while (ts.first[i + 1] <= b) ++i;
+  while (b < all) {
+    i = tensor_from(ts, i, (int)b);
     const tb2_adamw_tensor& t = ts.t[i];
-    const int blk = b - ts.first[i];
+    const int blk = (int)(b - ts.first[i]);
     const long long k0 = (long long)blk * kBlock + 4 * lane;
-    const bool whole = (ts.whole[i / 32] >> (i % 32) & 1) && (long long)(blk + 1) * kBlock <= t.n;
+    const bool aligned = ts.whole[i / 32] >> (i % 32) & 1, whole = aligned && (long long)(blk + 1) * kBlock <= t.n;
+    const bool run = !PUT && aligned && b + kRun <= end && (long long)(blk + kRun) * kBlock <= t.n;
+    b += run ? kRun : 1;
+    if (b >= end) {   // on to the warp's next run
+      b = end + (warps - 1LL) * kRun;
+      end = min(b + kRun, (long long)all);
+    }
+    if (run) {
+      unsigned mq[2 * kRun], vq[2 * kRun];
+      float ms[kRun], vs[kRun];
+#pragma unroll
+      for (int j = 0; j < 2 * kRun; ++j) {
+        mq[j] = __ldcs(reinterpret_cast<const unsigned*>(static_cast<uint8_t*>(t.m) + k0 + 128 * j));
+        vq[j] = __ldcs(reinterpret_cast<const unsigned*>(static_cast<uint8_t*>(t.v) + k0 + 128 * j));
+      }
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) ms[j] = t.m_scale[blk + j], vs[j] = t.v_scale[blk + j];
+#pragma unroll
+      for (int j = 0; j < 2 * kRun; ++j) {
+        float m[4], r[4];
+        load4_e4m3(mq[j], m);
+        load4_e4m3(vq[j], r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          m[e] *= ms[j / 2];
+          r[e] *= vs[j / 2];
+          r[e] *= r[e];
+        }
+        store4<float>(t.p, k0 + 128 * j, m);
+        store4<float>(t.copy, k0 + 128 * j, r);
+      }
+      continue;
+    }
     uint8_t *mp = static_cast<uint8_t*>(t.m), *vp = static_cast<uint8_t*>(t.v);
     float *mo = static_cast<float*>(t.p), *vo = static_cast<float*>(t.copy);
     float m[8], r[8];
@@ -343,18 +457,17 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant
       }
       continue;
     }
-    unsigned top_m = 0, top_r = 0;
+    float top_m = 0.f, top_r = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const long long k = k0 + 128 * (e / 4) + e % 4;
       m[e] = k < t.n ? mo[k] : 0.f;
       r[e] = k < t.n ? vo[k] : 0.f;
-      top_m = max(top_m, __float_as_uint(fabsf(m[e])));
-      top_r = max(top_r, __float_as_uint(r[e] < FLT_MIN && r[e] >= 0.f ? 0.f : sqrtf(r[e])));
+      top_m = top_of(top_m, m[e]);
+      top_r = top_of(top_r, r[e] < FLT_MIN && r[e] >= 0.f ? 0.f : sqrtf(r[e]));
     }
     float mi, ri;
-    const float ms = block_scale(__reduce_max_sync(0xffffffffu, top_m), mi);
-    const float vs = block_scale(__reduce_max_sync(0xffffffffu, top_r), ri);
+    const float ms = block_scale(top_m, mi), vs = block_scale(top_r, ri);
     if (lane == 0) t.m_scale[blk] = ms, t.v_scale[blk] = vs;
 #pragma unroll 1
     for (int e = 0; e < 8; ++e) {
@@ -393,7 +506,7 @@ int in_groups(const tb2_adamw_tensor* t, int n, W&& whole, F&& launch) {
       g.t[g.n++] = t[i];
       blocks += b;
     }
-    g.first[g.n] = (int)blocks;
+    g.first[g.n] = g.first[g.n + 1] = (int)blocks;
     if (g.n) {
       // CTAs that stay, each with a run of blocks; as many as the blocks need where those are few
       const long long ctas = std::min((blocks + kWarps - 1) / kWarps, (long long)kCtasPerSm * kSMs);
