@@ -497,7 +497,7 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args *args, void *stream);
  * *grad_scale (NULL: 1), both device memory:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = (1 - alpha wd) p - alpha beta1h m / (sqrt(beta2h) sqrt(v) + eps),
- * copy = p rounded to copy_type (copy NULL: none). state_bits 32: m and v are
+ * copy = p rounded to copy_type, 1 or 30 (copy NULL: none). state_bits 32: m and v are
  * f32. state_bits 8: blocks of 256 consecutive values share an f32 scale
  * (m_scale, v_scale: [ceil(n / 256)]), the smallest power of two of 2^-100 or
  * more that brings the block within 448; m holds e4m3 codes of m / scale and v

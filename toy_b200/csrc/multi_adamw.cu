@@ -26,7 +26,8 @@ namespace {
 
 constexpr int kBlock = 256;        // values that share a scale
 constexpr int kMaxTensors = 448;   // tensors a launch: their descriptors travel as its arguments (30.5 of 32 KB)
-constexpr int kThreads = 256, kWarps = kThreads / 32, kCtasPerSm = 3;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kRun = 4;
+constexpr int kCtas8 = 3, kCtas32 = 2;   // CTAs an SM: 80 and 128 registers a thread
 
 struct Tensors {
   tb2_adamw_tensor t[kMaxTensors];
@@ -60,11 +61,14 @@ __device__ __forceinline__ void store4(void* p, long long i, const float* f) {
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(f[0], f[1], f[2], f[3]);
   } else {
-    T t[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) t[k] = from_f32<T>(f[k]);
     uint2 u;
-    memcpy(&u, t, 8);
+    if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h[2] = {__floats2half2_rn(f[0], f[1]), __floats2half2_rn(f[2], f[3])};
+      memcpy(&u, h, 8);
+    } else {
+      const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
+      memcpy(&u, h, 8);
+    }
     *reinterpret_cast<uint2*>(static_cast<T*>(p) + i) = u;
   }
 }
@@ -87,13 +91,6 @@ __device__ __noinline__ unsigned e4m3_of(double t) {
   const int e = t < 0.015625 ? -6 : ilogb(t);
   const double q = ldexp(rint(ldexp(t, 3 - e)), e - 3);   // eighths of the leading bit; at the bottom, steps of 2^-9
   return __nv_cvt_float_to_fp8((float)q, __NV_SATFINITE, __NV_E4M3);
-}
-
-// Whether t >= 0, as a multiple of the scale, is within eight units in the last place of the border between two codes:
-// the bits below an e4m3 value's three, next to their half. (Below 2^-6 codes are 2^-9 apart, as they are just above.)
-__device__ __forceinline__ bool near_border(float t) {
-  const unsigned b = __float_as_uint(t < 0.015625f ? t + 0.015625f : t) * 4096u;
-  return b - ((0x80000u - 8) << 12) <= (16u << 12);
 }
 
 __device__ __forceinline__ float sqrt_near(float x) {   // within 2^-23; below 2^-126: 0
@@ -123,6 +120,12 @@ __device__ __forceinline__ float block_scale(float top, float& inverse) {
   return ok ? __uint_as_float((unsigned)(127 + e) << 23) : NAN;
 }
 
+// The step's factors; dg is (1 - b1) times the gradients' factor, sb2 sqrt(b2), sd2 sqrt(1 - b2) times that factor.
+struct Hyper {
+  double b1_64, dg_64;
+  float b1, b2, eps, keep, c1, c2, gf, dg, d2, sb2, sd2;
+};
+
 // f64 to f32 so that rounding the result to few bits rounds the f64 value once: cut, the last bit set where that left
 // something out.
 __device__ __forceinline__ float to_odd(double x) {
@@ -130,31 +133,27 @@ __device__ __forceinline__ float to_odd(double x) {
   return __uint_as_float(__float_as_uint(f) | ((__double2loint(x) & 0x1fffffff) != 0));
 }
 
-// The step's factors.
-struct Hyper {
-  float b1, b2, eps, keep, c1, c2, gf, d1, d2;
-  float sb2, sd2;   // sqrt(b2), the factor times sqrt(1 - b2)
-  double db1, dgm;
-};
-
-// The code of a second moment's root next to a border, from 64 bits.
+// The code of a root next to a border, from 64 bits and the operands in memory.
 __device__ __noinline__ unsigned root_code(float g, float gf, float r0, float b2, float inverse) {
   const double gw = (double)g * gf, v = (double)r0 * r0 * b2 + gw * gw * (1.0 - (double)b2);
   return max(e4m3_of(sqrt(v) * inverse), 1u);
 }
+__device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) { w = (w & ~(0xffu << 8 * at)) | q << 8 * at; }
 
-// A warp has a block at a time; a CTA a run of blocks.
+// A warp has a block at a time; the blocks are dealt over the whole grid, so that all CTAs work in the same few pages
+// of every array (a run of blocks to each CTA: 489 us instead of 449 for 135M weights in 8 bits).
 //
-// The step is f32 but for 8-bit m: that is a sum of two terms of either sign, and to be rounded once to a code it is
-// needed to more bits than a product and a sum in f32 leave after a cancellation. FP64 has the room (two products and
-// three conversions a value), and a conversion that keeps what it cuts as a set last bit needs no second look. The root
-// of v is all positive terms: with U = 2^-24, sqrt(b2) and the held root's factor, that product and its square 2 + 2 +
-// 2 + 1 U, the gradient's as much, the sum 1, which the root halves, and its own 2 U: 6 U. The few (one in 30000) that
-// come within 8 units in the last place (U or more each) of a border are rounded again from 64 bits.
+// 8-bit moments are the exact values rounded once, although the step is f32. m is a sum of two terms of either sign, and
+// with few bits in its old value it falls on a border again and again (0.9 of 120 is 108, between 104 and 112: 0.8 % of
+// the values of a run with b1 = 0.9 are closer to one than f32 tells), so it is computed in f64, two products and three
+// conversions a value, and converted so that the code is rounded from all its bits. A root's code is taken of both ends
+// of an interval that holds the exact one, and where the two differ (one value in 90000) it is rounded from 64 bits.
+// With U = 2^-24: the root's square is a sum of squares, the held root's factor and product 2 + 1 U, the gradient's 3 +
+// 1, doubled by squaring, 1 for a square and 1 for the sum; the root halves these 10, and is off by 2 U itself: 7 U of 8.
 //
-// Bound by HBM in 32 bits. In 8 bits a value is 16 bytes and (with these choices) some 50 instructions, near both
-// limits: IEEE quotients and roots, flags for each value and a second look at m made it 103 and 508 us where the bytes
-// of 135M weights take 332.
+// Bound by HBM in 32 bits. In 8 bits a value is 16 bytes, the time of some 75 instructions at most: a look at the
+// distance of every root from a border made it 58 (445 us where the bytes of 135M weights take 332), IEEE quotients and
+// roots besides 103 (508 us).
 // A lane's values of a block as they lie in memory.
 template <class T>
 struct Raw4 {
@@ -183,9 +182,75 @@ struct RawBlock {
   float ms, vs;
 };
 
+// A lane's eight values, stepped: p the new weights, m the new first moments, r the new second moments (32 bits) or
+// their roots (8 bits).
+template <int BITS>
+__device__ __forceinline__ void step8(const Hyper& h, float (&p)[8], const float (&g)[8], float (&m)[8], float (&r)[8],
+                                      float ms, float vs) {
+  const float rs = vs * h.sb2;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float v;
+    if (BITS == 8) {
+      m[e] = to_odd(fma((double)(m[e] * ms), h.b1_64, (double)g[e] * h.dg_64));
+      const float gs = g[e] * h.sd2, r0 = r[e] * rs;
+      v = fmaf(gs, gs, r0 * r0);
+    } else {
+      const float gg = g[e] * h.gf;
+      m[e] = fmaf(m[e], h.b1, g[e] * h.dg);
+      v = fmaf(r[e], h.b2, gg * gg * h.d2);
+    }
+    const float root = sqrt_near(v);
+    p[e] = fmaf(-h.c1 * m[e], inverse_near(fmaf(root, h.c2, h.eps)), p[e] * h.keep);
+    r[e] = BITS == 8 ? root : v;
+  }
+}
+
+// The block's codes and scales. again(e): value e's root code from 64 bits, given the factor.
+template <class F>
+__device__ __forceinline__ void hold8(float (&m)[8], const float (&r)[8], unsigned (&mq)[2], unsigned (&vq)[2], float& ms,
+                                      float& vs, F&& again) {
+  float top_m = 0.f, top_r = 0.f, mi, ri;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top_m = top_of(top_m, m[e]);
+    top_r = top_of(top_r, r[e]);
+  }
+  ms = block_scale(top_m, mi);
+  vs = block_scale(top_r, ri);
+  const float low = ri * (1.f - 0x1p-21f), high = ri * (1.f + 0x1p-21f);
+  unsigned look[2];   // nonzero bytes: roots to be looked at
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float a[4], z[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      m[4 * j + e] *= mi;
+      a[e] = r[4 * j + e] * low;
+      z[e] = r[4 * j + e] * high;
+    }
+    mq[j] = pack4_e4m3(m + 4 * j);
+    vq[j] = pack4_e4m3(z);
+    // (and those of code 0: a positive root keeps the smallest one)
+    look[j] = (vq[j] ^ pack4_e4m3(a)) | (~(vq[j] + 0x7f7f7f7fu) & 0x80808080u);
+  }
+  if (look[0] | look[1]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if ((look[e / 4] >> 8 * (e % 4) & 0xff) && r[e] > 0.f && ri == ri) put_byte(vq[e / 4], e % 4, again(e, ri));
+  }
+}
+
+__device__ __forceinline__ float held_code(const void* v, long long k) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(v)[k], __NV_E4M3)));
+}
+
+// The next block is read while one is computed where it lies whole on its boundaries; a tensor's end, or one off its
+// boundaries, goes value by value. (Reads staged further ahead, by asynchronous copies to shared memory or in runs of
+// four blocks with one address each, took as long in 8 bits, 454 and 467 us: what is left is not the reads' latency.)
 template <class P, class G, int BITS>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid_constant__ Tensors ts, int copy_type,
-                                                                    const float* hp, const float* factor) {
+__global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
+    step_kernel(const __grid_constant__ Tensors ts, int copy_type, const float* hp, const float* factor) {
   using S = typename std::conditional<BITS == 8, uint8_t, float>::type;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int all = ts.first[ts.n];
@@ -199,14 +264,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
   h.c1 = hp[0] * hp[5];
   h.c2 = sqrtf(hp[6]);
   h.gf = factor ? *factor : 1.f;
-  h.d1 = 1.f - h.b1;
+  h.b1_64 = h.b1;
+  h.dg_64 = (1.0 - h.b1_64) * (double)h.gf;
+  h.dg = (float)h.dg_64;
   h.d2 = 1.f - h.b2;
   h.sb2 = sqrtf(h.b2);
   h.sd2 = h.gf * sqrtf(h.d2);
-  h.db1 = h.b1;
-  h.dgm = (1.0 - h.db1) * (double)h.gf;
-  // block b of tensor i: read as it lies where that is possible (a whole block on its boundaries)
   RawBlock<P, G, S> raw;
+  // block b of tensor i on its way; whether it is one that is read so
   auto fetch = [&](int b) {
     const tb2_adamw_tensor& t = ts.t[i];
     const int blk = b - ts.first[i];
@@ -226,11 +291,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
   };
   if (b >= all) return;
   bool next_whole = fetch(b);
-  for (; b < all; b += warps) {
+  while (true) {
     const tb2_adamw_tensor& t = ts.t[i];
     const int blk = b - ts.first[i];
     const long long k0 = (long long)blk * kBlock + 4 * lane;
-    const bool whole = next_whole;
+    const bool whole = next_whole, more = all - b > warps;
     float p[8], g[8], m[8], r[8];
     const float ms = raw.ms, vs = raw.vs;
     if (whole) {
@@ -241,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
         raw.m[j].get(m + 4 * j);
         raw.v[j].get(r + 4 * j);
       }
-    } else {   // a tensor's end, or one off its boundaries
+    } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const long long k = k0 + 128 * (e / 4) + e % 4;
@@ -249,74 +314,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
         p[e] = on ? to_f32(static_cast<const P*>(t.p)[k]) : 0.f;
         g[e] = on ? to_f32(static_cast<const G*>(t.g)[k]) : 0.f;
         if (BITS == 8) {
-          m[e] = on ? __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(t.m)[k], __NV_E4M3))) : 0.f;
-          r[e] = on ? __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(t.v)[k], __NV_E4M3))) : 0.f;
+          m[e] = on ? held_code(t.m, k) : 0.f;
+          r[e] = on ? held_code(t.v, k) : 0.f;
         } else {
           m[e] = on ? static_cast<const float*>(t.m)[k] : 0.f;
           r[e] = on ? static_cast<const float*>(t.v)[k] : 0.f;
         }
       }
     }
-    int i_next = i;
-    if (all - b > warps) {   // the next block is on its way while this one is computed
-      const int i_now = i;
-      i = tensor_from(ts, i, b + warps);
+    if (more) {
+      i = tensor_from(ts, i, b + warps);   // (t is still block b's)
       next_whole = fetch(b + warps);
-      i_next = i;
-      i = i_now;
     }
-    float top_m = 0.f, top_r = 0.f;
-    const float rs = BITS == 8 ? vs * h.sb2 : 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float v;
-      if (BITS == 8) {
-        m[e] = to_odd(fma((double)(m[e] * ms), h.db1, (double)g[e] * h.dgm));
-        const float gs = g[e] * h.sd2, r0 = r[e] * rs;
-        v = fmaf(gs, gs, r0 * r0);
-      } else {
-        const float gg = g[e] * h.gf;
-        m[e] = fmaf(m[e], h.b1, gg * h.d1);
-        v = fmaf(r[e], h.b2, gg * gg * h.d2);
-      }
-      const float root = sqrt_near(v);
-      p[e] = fmaf(-h.c1 * m[e], inverse_near(fmaf(root, h.c2, h.eps)), p[e] * h.keep);
-      r[e] = BITS == 8 ? root : v;
-      if (BITS == 8) {
-        top_m = top_of(top_m, m[e]);
-        top_r = top_of(top_r, root);
-      }
-    }
+    step8<BITS>(h, p, g, m, r, ms, vs);
     unsigned mq[2], vq[2];
     if (BITS == 8) {
-      float mi, ri;
-      const float nms = block_scale(top_m, mi), nvs = block_scale(top_r, ri);
-      bool look = false;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float tm[4], tr[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          tm[e] = m[4 * j + e] * mi;
-          tr[e] = r[4 * j + e] * ri;
-          look |= near_border(tr[e]);
-          r[4 * j + e] = tr[e];
-          tr[e] = tr[e] > 0.f ? fmaxf(tr[e], 0.001953125f) : tr[e];   // a positive root keeps the smallest code
-        }
-        mq[j] = pack4_e4m3(tm);
-        vq[j] = pack4_e4m3(tr);
-      }
-      if (look) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!near_border(r[e])) continue;
-          const long long k = k0 + 128 * (e / 4) + e % 4;
-          if (k >= t.n) continue;
-          const float r0 = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(t.v)[k], __NV_E4M3)));
-          const unsigned q = root_code(to_f32(static_cast<const G*>(t.g)[k]), h.gf, r0 * vs, h.b2, ri);
-          vq[e / 4] = (vq[e / 4] & ~(0xffu << 8 * (e % 4))) | q << 8 * (e % 4);
-        }
-      }
+      float nms, nvs;
+      hold8(m, r, mq, vq, nms, nvs, [&](int e, float ri) {
+        const long long k = k0 + 128 * (e / 4) + e % 4;
+        return k < t.n ? root_code(to_f32(static_cast<const G*>(t.g)[k]), h.gf, held_code(t.v, k) * vs, h.b2, ri) : 0u;
+      });
       if (lane == 0) t.m_scale[blk] = nms, t.v_scale[blk] = nvs;
     }
     if (whole) {
@@ -329,8 +346,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
             for (int e = 0; e < 4; ++e) p[4 * j + e] = to_f32(from_f32<P>(p[4 * j + e]));
           }
           if (copy_type == kTypeF16) store4<__half>(t.copy, k0 + 128 * j, p + 4 * j);
-          else if (copy_type == kTypeBF16) store4<__nv_bfloat16>(t.copy, k0 + 128 * j, p + 4 * j);
-          else store4<float>(t.copy, k0 + 128 * j, p + 4 * j);
+          else store4<__nv_bfloat16>(t.copy, k0 + 128 * j, p + 4 * j);
         }
         if (BITS == 8) {
           *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(t.m) + k0 + 128 * j) = mq[j];
@@ -349,8 +365,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
         static_cast<P*>(t.p)[k] = q;
         if (t.copy) {
           if (copy_type == kTypeF16) static_cast<__half*>(t.copy)[k] = from_f32<__half>(to_f32(q));
-          else if (copy_type == kTypeBF16) static_cast<__nv_bfloat16*>(t.copy)[k] = from_f32<__nv_bfloat16>(to_f32(q));
-          else static_cast<float*>(t.copy)[k] = to_f32(q);
+          else static_cast<__nv_bfloat16*>(t.copy)[k] = from_f32<__nv_bfloat16>(to_f32(q));
         }
         if (BITS == 8) {
           static_cast<uint8_t*>(t.m)[k] = (uint8_t)(mq[e / 4] >> 8 * (e % 4));
@@ -361,7 +376,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) step_kernel(const __grid
         }
       }
     }
-    i = i_next;
+    if (!more) return;
+    b += warps;
   }
 }
 
@@ -370,8 +386,7 @@ template <bool PUT>
 __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ Tensors ts) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int all = ts.first[ts.n];
-  const int warps = gridDim.x * kWarps;
-  constexpr int kRun = 4;   // blocks of a warp in a row: so many reads are on their way at once
+  const int warps = gridDim.x * kWarps;   // (each has kRun blocks in a row: so many reads are on their way at once)
   long long b = ((long long)blockIdx.x * kWarps + warp) * kRun, end = min(b + kRun, (long long)all);
   int i = tensor_of(ts, (int)min(b, all - 1LL));
   griddep_wait();
@@ -489,6 +504,11 @@ bool tensor_ok(const tb2_adamw_tensor& t, int p_type, int g_type, int copy_type,
   return t.m_scale && t.v_scale && all_aligned(4, {t.m_scale, t.v_scale});
 }
 
+// CTAs that stay; as many as the warps' runs of blocks need where those are few.
+unsigned ctas_of(long long blocks, int run, int per_sm) {
+  return (unsigned)std::min((blocks + kWarps * run - 1) / (kWarps * run), (long long)per_sm * kSMs);
+}
+
 // The tensors in groups of what a launch takes, empty ones left out. whole(tensor): see Tensors.
 template <class W, class F>
 int in_groups(const tb2_adamw_tensor* t, int n, W&& whole, F&& launch) {
@@ -507,11 +527,8 @@ int in_groups(const tb2_adamw_tensor* t, int n, W&& whole, F&& launch) {
       blocks += b;
     }
     g.first[g.n] = g.first[g.n + 1] = (int)blocks;
-    if (g.n) {
-      // CTAs that stay, each with a run of blocks; as many as the blocks need where those are few
-      const long long ctas = std::min((blocks + kWarps - 1) / kWarps, (long long)kCtasPerSm * kSMs);
-      if (int rc = launch(g, (int)ctas)) return rc;
-    }
+    if (g.n)
+      if (int rc = launch(g, blocks)) return rc;
   }
   return 0;
 }
@@ -539,7 +556,8 @@ extern "C" {
 int tb2_adamw_multi(const tb2_adamw_multi_args* a, void* stream) {
   using namespace tb2;
   if (!a || a->n_tensors < 0 || (a->n_tensors && !a->tensors) || (a->state_bits != 8 && a->state_bits != 32)) return -1;
-  if (!row_type_ok(a->p_type) || !row_type_ok(a->g_type) || !row_type_ok(a->copy_type)) return -1;
+  if (!row_type_ok(a->p_type) || !row_type_ok(a->g_type)) return -1;
+  if (a->copy_type != kTypeF16 && a->copy_type != kTypeBF16) return -1;
   if (!a->hp || !all_aligned(4, {a->hp, a->grad_scale})) return -1;
   for (int i = 0; i < a->n_tensors; ++i)
     if (!tensor_ok(a->tensors[i], a->p_type, a->g_type, a->copy_type, a->state_bits)) return -1;
@@ -548,12 +566,13 @@ int tb2_adamw_multi(const tb2_adamw_multi_args* a, void* stream) {
   auto whole = [&](const tb2_adamw_tensor& t) {
     return aligned(t.p, pb) && aligned(t.g, gb) && aligned(t.copy, cb) && all_aligned(sb, {t.m, t.v});
   };
-  return in_groups(a->tensors, a->n_tensors, whole, [&](const Tensors& g, int ctas) {
+  const int per = a->state_bits == 8 ? kCtas8 : kCtas32;
+  return in_groups(a->tensors, a->n_tensors, whole, [&](const Tensors& g, long long blocks) {
     return by_row_type(a->p_type, [&](auto p) {
       return by_row_type(a->g_type, [&](auto q) {
         using P = decltype(p);
         using G = decltype(q);
-        return launch_pdl(a->state_bits == 8 ? step_kernel<P, G, 8> : step_kernel<P, G, 32>, dim3(ctas), dim3(kThreads),
+        return launch_pdl(a->state_bits == 8 ? step_kernel<P, G, 8> : step_kernel<P, G, 32>, dim3(ctas_of(blocks, 1, per)), dim3(kThreads),
                           0, static_cast<cudaStream_t>(stream), g, a->copy_type, a->hp, a->grad_scale);
       });
     });
@@ -573,8 +592,8 @@ int tb2_adamw_moments(const tb2_adamw_tensor* tensors, int n_tensors, int put, v
   auto whole = [](const tb2_adamw_tensor& t) {
     return all_aligned(16, {t.p, t.copy}) && all_aligned(4, {t.m, t.v});
   };
-  return in_groups(tensors, n_tensors, whole, [&](const Tensors& g, int ctas) {
-    return launch_pdl(put ? moments_kernel<true> : moments_kernel<false>, dim3(ctas), dim3(kThreads), 0,
+  return in_groups(tensors, n_tensors, whole, [&](const Tensors& g, long long blocks) {
+    return launch_pdl(put ? moments_kernel<true> : moments_kernel<false>, dim3(ctas_of(blocks, kRun, 4)), dim3(kThreads), 0,
                       static_cast<cudaStream_t>(stream), g);
   });
 }

@@ -40,7 +40,7 @@ class MultiAdamW:
         self._shapes = [p.shape for p in self.params]
         pp = [dense(p, p.shape, self.dtype, self.index, "params") for p in self.params]
         self.copies = list(copies) if copies else None
-        self.copy_dtype = self.copies[0].dtype if copies else F32
+        self.copy_dtype = self.copies[0].dtype if copies else torch.bfloat16
         if copies and (len(self.copies) != len(n) or self.copy_dtype not in (torch.float16, torch.bfloat16)):
             bad("copies: one f16 or bf16 tensor per weight")
         cp = [dense(c, s, self.copy_dtype, self.index, "copies")
