@@ -32,12 +32,16 @@ def prepare(device=None) -> None:
     _prepared.add(index)
 
 
+# (the current device without torch.cuda's checks around it, where torch has it)
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def call(index: int, what: str, *args) -> None:
     """An entry point on torch's current stream of GPU `index`, which is made current for the call where it is not."""
     if index not in _prepared:
         prepare(torch.device("cuda", index))
     f = getattr(lib(), what)
-    if torch.cuda.current_device() == index:
+    if _current() == index:
         rc = f(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):

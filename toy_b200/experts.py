@@ -43,12 +43,14 @@ def sort(ids: torch.Tensor, n_experts: int, *, out: Optional[Routing] = None) ->
         bad(f"n_experts is 1 to {MAX_EXPERTS}")
     dev, n = ids.get_device(), ids.numel()
     if out is None:
-        part = ids.new_empty(2 * n + n_experts + 1, dtype=I32)
-        pos, order, offsets = part.split((n, n, n_experts + 1))
-        out = Routing(offsets, order, pos.view(ids.shape))
-    a = ExpertSortArgs(ids.data_ptr(), ids.element_size(), n, n_experts,
-                       dense(out.offsets, (n_experts + 1,), I32, dev, "out.offsets"),
-                       dense(out.order, (n,), I32, dev, "out.order"), dense(out.pos, ids.shape, I32, dev, "out.pos"))
+        out = Routing(ids.new_empty(n_experts + 1, dtype=I32), ids.new_empty(n, dtype=I32),
+                      ids.new_empty(ids.shape, dtype=I32))
+    else:
+        dense(out.offsets, (n_experts + 1,), I32, dev, "out.offsets")
+        dense(out.order, (n,), I32, dev, "out.order")
+        dense(out.pos, ids.shape, I32, dev, "out.pos")
+    a = ExpertSortArgs(ids.data_ptr(), 4 if ids.dtype is I32 else 8, n, n_experts, out.offsets.data_ptr(),
+                       out.order.data_ptr(), out.pos.data_ptr())
     call(dev, "tb2_expert_sort", C.byref(a))
     return out
 
@@ -74,15 +76,23 @@ def _sorted(r: Routing, dev: int) -> int:
     return dense(r.offsets, (max(n, 1),), I32, dev, "offsets") + 4 * (n - 1)
 
 
+def _wanted(*tensors) -> bool:
+    """Whether a gradient of one of the tensors is wanted."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            return True
+    return False
+
+
 def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _wanted(*tensors):
         bad("no gradient passes through this call (use it under torch.no_grad())")
 
 
 def _dispatch(x, r, out):
     fresh = out is None
     if fresh:
-        out = torch.empty((r.pos.numel(), x.shape[1] if x.dim() == 2 else 0), device=x.device, dtype=x.dtype)
+        out = x.new_empty((r.pos.numel(), x.shape[1] if x.dim() == 2 else 0))
     dev, a = _args(r, x, out, None)
     if fresh:
         a.n_sorted = _sorted(r, dev)
@@ -92,7 +102,7 @@ def _dispatch(x, r, out):
 
 def _combine(z, r, weights, residual, out):
     if out is None:
-        out = torch.empty((r.pos.shape[0], z.shape[1] if z.dim() == 2 else 0), device=z.device, dtype=z.dtype)
+        out = z.new_empty((r.pos.shape[0], z.shape[1] if z.dim() == 2 else 0))
     dev, a = _args(r, out, z, weights)
     if residual is not None:
         a.ldr = rows(residual, a.n_tokens, a.d, z.dtype, dev, "residual")
@@ -139,7 +149,7 @@ def _whole(g: torch.Tensor) -> torch.Tensor:
 def dispatch(x: torch.Tensor, r: Routing, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The rows of x [tokens, d] at their slots' places, [tokens * used, d]: rows past the last slot's are zero, or as
     they were where `out` is given. Differentiable in x (without out)."""
-    if out is None and x.requires_grad and torch.is_grad_enabled():
+    if out is None and _wanted(x):
         return _Dispatch.apply(x, *r)
     _no_grad(x, out)
     return _dispatch(x, r, out)
@@ -156,8 +166,7 @@ def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None,
     """residual [tokens, d] (None: 0) plus each token's sum of weights (f32 [tokens, used]; None: 1) times its slots'
     rows of z [rows, d], choices ascending, in f32, rounded once. out may be the residual. Differentiable in z, weights
     and residual (without out)."""
-    if out is None and torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                                       for t in (z, weights, residual)):
+    if out is None and _wanted(z, weights, residual):
         return _Combine.apply(z, weights, residual, *r)
     _no_grad(z, weights, residual, out)
     return _combine(z, r, weights, residual, out)
@@ -166,9 +175,9 @@ def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None,
 def _combine_grad(dy, z, r, weights, out, want_z, want_w):
     fresh = out is None and want_z
     if fresh:
-        out = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        out = z.new_empty(z.shape)
     dev, a = _args(r, dy, z, weights)
-    dw = torch.empty(r.pos.shape, device=z.device, dtype=F32) if want_w else None
+    dw = z.new_empty(r.pos.shape, dtype=F32) if want_w else None
     if want_z:
         a.ldd = rows(out, a.n_rows, a.d, z.dtype, dev, "out")
         a.d_xs = out.data_ptr()

@@ -13,7 +13,6 @@ the vocabulary are reported on the device (`tb2_device_error` in the header).
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -44,33 +43,31 @@ def _logits(x: torch.Tensor, tokens: torch.Tensor, scale: float, top: int) -> tu
         bad("logits: one word or more, rows and words below 2^31")
     if not 0 <= top <= min(MAX_TOP, vocab):
         bad(f"top is 0 to {MAX_TOP}, and no more than the vocabulary")
-    if not (scale > 0 and math.isfinite(C.c_float(scale).value) and C.c_float(scale).value > 0):
-        bad("scale is positive and finite")
+    if not 2.0**-126 <= scale <= 2.0**126:
+        bad("scale is positive, and neither it nor its inverse past f32's range")
     dense(tokens, (n,), I64, dev, "tokens")
     return n, vocab, dev, rows(x, n, vocab, x.dtype, dev, "logits")
 
 
-def _forward(x, tokens, scale, entropy, top, apart=False) -> TokenLogprobs:
+def _forward(x, tokens, scale, entropy, top) -> TokenLogprobs:
     n, vocab, dev, ld = _logits(x, tokens, scale, top)
-    sizes = (2 * n, n, n * bool(entropy), n * top)      # the 8-byte pairs first
-    if apart:
-        parts = [x.new_empty(k, dtype=F32) for k in sizes]
-    else:                                               # one allocation, as each costs a microsecond
-        parts = x.new_empty(sum(sizes), dtype=F32).split(sizes)
-    ids = x.new_empty((n, top), dtype=I64) if top else None
+    lp, stats = x.new_empty(n, dtype=F32), x.new_empty((n, 2), dtype=F32)
+    ent = x.new_empty(n, dtype=F32) if entropy else None
+    ids = top_lp = None
+    if top:
+        ids, top_lp = x.new_empty((n, top), dtype=I64), x.new_empty((n, top), dtype=F32)
     if n:
-        stats, lp, ent, top_lp = (t.data_ptr() for t in parts)
-        a = LogprobsArgs(n, vocab, ROW_TYPE[x.dtype], x.data_ptr(), ld, scale, tokens.data_ptr(), lp, stats,
-                         ent if entropy else None, top, ids.data_ptr() if top else None, top_lp if top else None)
+        a = LogprobsArgs(n, vocab, ROW_TYPE[x.dtype], x.data_ptr(), ld, scale, tokens.data_ptr(), lp.data_ptr(),
+                         stats.data_ptr(), ent.data_ptr() if entropy else None, top, ids.data_ptr() if top else None,
+                         top_lp.data_ptr() if top else None)
         call(dev, "tb2_logprobs", C.byref(a))
-    return TokenLogprobs(parts[1], parts[2] if entropy else None, ids, parts[3].view(n, top) if top else None,
-                         parts[0].view(n, 2))
+    return TokenLogprobs(lp, ent, ids, top_lp, stats)
 
 
 class _Score(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, scale, entropy, top):
-        r = _forward(logits, tokens, scale, entropy, top, apart=True)
+        r = _forward(logits, tokens, scale, entropy, top)
         ctx.mark_non_differentiable(*[t for t in (r.stats, r.top_ids) if t is not None])
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, tokens, r.stats, r.entropy, r.top_ids)

@@ -9,8 +9,10 @@ e4m3 of its square root, each the step's exact value rounded once.
 from __future__ import annotations
 
 import ctypes as C
+from operator import attrgetter
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from ._lib import AdamwMultiArgs, AdamwTensor
@@ -19,6 +21,19 @@ from ._rows import F32, ROW_TYPE, bad, call, dense, prepare
 __all__ = ["MultiAdamW", "prepare"]
 BLOCK = 256
 _HELD = torch.float8_e4m3fn
+_SHAPE, _DTYPE = attrgetter("shape"), attrgetter("dtype")
+_POINTER, _DEVICE, _DENSE = torch.Tensor.data_ptr, torch.Tensor.get_device, torch.Tensor.is_contiguous
+# tb2_adamw_tensor, by columns
+_COLUMNS = np.dtype([(name, np.int64 if kind is C.c_longlong else np.uint64) for name, kind in AdamwTensor._fields_])
+
+
+def _pointers(tensors: Sequence[torch.Tensor], shapes: list, dtype, index: int, what: str) -> list:
+    """The addresses of contiguous tensors of these shapes, of one type, on GPU `index`. (Checked attribute by
+    attribute: for hundreds of small tensors this is the call's time.)"""
+    if list(map(_SHAPE, tensors)) != shapes or any(d is not dtype for d in set(map(_DTYPE, tensors))) or \
+            set(map(_DEVICE, tensors)) != {index} or not all(map(_DENSE, tensors)):
+        bad(f"{what}: contiguous {dtype} tensors of the weights' shapes on cuda:{index}")
+    return list(map(_POINTER, tensors))
 
 
 class MultiAdamW:
@@ -44,7 +59,7 @@ class MultiAdamW:
         if copies and (len(self.copies) != len(n) or self.copy_dtype not in (torch.float16, torch.bfloat16)):
             bad("copies: one f16 or bf16 tensor per weight")
         cp = [dense(c, s, self.copy_dtype, self.index, "copies")
-              for c, s in zip(self.copies, self._shapes)] if copies else [None] * len(n)
+              for c, s in zip(self.copies, self._shapes)] if copies else [0] * len(n)
         blocks = [-(-k // BLOCK) for k in n]
         if state is None:
             def zeros(sizes, dtype):
@@ -73,10 +88,11 @@ class MultiAdamW:
                     bad(f"state: contiguous {dtype} tensors of {k} values on cuda:{self.index}")
             at.append([t.data_ptr() for t in x])
         if bits == 32:
-            at += [[None] * len(n)] * 2
+            at += [[0] * len(n)] * 2
         self._n = len(n)
-        self._t = (AdamwTensor * self._n)(*[AdamwTensor(*x) for x in zip(pp, [None] * self._n, *at, cp, n)])
-        self._now = (AdamwTensor * self._n)()
+        self._t = np.zeros(self._n, _COLUMNS)
+        for name, x in zip(_COLUMNS.names, (pp, [0] * self._n, *at, cp, n)):
+            self._t[name] = x
         if self.index not in _ready():
             prepare(self.device)
 
@@ -94,35 +110,27 @@ class MultiAdamW:
             if grad_scale.numel() != 1 or grad_scale.dtype is not F32 or grad_scale.get_device() != self.index:
                 bad(f"grad_scale: one f32 value on cuda:{self.index}")
             scale_at = grad_scale.data_ptr()
-        dtype, k, dev = None, 0, self.index
-        t, now = self._t, self._now
-        for i, g in enumerate(grads):
-            if g is None:
-                continue
-            if dtype is None:
-                dtype = g.dtype
-                if dtype not in ROW_TYPE:
-                    bad("grads: f32, f16 or bf16")
-            if g.dtype is not dtype or g.shape != self._shapes[i] or g.get_device() != dev or not g.is_contiguous():
-                bad(f"grads[{i}]: contiguous {dtype} {list(self._shapes[i])} on cuda:{dev}")
-            now[k] = t[i]
-            now[k].g = g.data_ptr()
-            k += 1
-        if not k:
-            return
-        a = AdamwMultiArgs(C.addressof(now), k, ROW_TYPE[self.dtype], ROW_TYPE[dtype], ROW_TYPE[self.copy_dtype],
+        grads, shapes, t = list(grads), self._shapes, self._t
+        if any(g is None for g in grads):
+            on = [i for i, g in enumerate(grads) if g is not None]
+            if not on:
+                return
+            grads, shapes, t = [grads[i] for i in on], [shapes[i] for i in on], t[on]
+        dtype = grads[0].dtype
+        if dtype not in ROW_TYPE:
+            bad("grads: f32, f16 or bf16")
+        t["g"] = _pointers(grads, shapes, dtype, self.index, "grads")
+        a = AdamwMultiArgs(t.ctypes.data, len(t), ROW_TYPE[self.dtype], ROW_TYPE[dtype], ROW_TYPE[self.copy_dtype],
                            self.bits, hp_at, scale_at)
-        call(dev, "tb2_adamw_multi", C.byref(a))
+        call(self.index, "tb2_adamw_multi", C.byref(a))
 
     def _values(self, ms, vs, put: int) -> None:
         if len(ms) != self._n or len(vs) != self._n:
             bad("moments: one tensor of each kind per weight")
-        at = [[dense(t, s, F32, self.index, "moments") for t, s in zip(x, self._shapes)] for x in (ms, vs)]
-        x = (AdamwTensor * self._n)()
-        for i in range(self._n):
-            x[i] = self._t[i]
-            x[i].p, x[i].copy = at[0][i], at[1][i]
-        call(self.index, "tb2_adamw_moments", C.addressof(x), self._n, put)
+        x = self._t.copy()
+        x["p"] = _pointers(ms, self._shapes, F32, self.index, "moments")
+        x["copy"] = _pointers(vs, self._shapes, F32, self.index, "moments")
+        call(self.index, "tb2_adamw_moments", x.ctypes.data, self._n, put)
 
     def moments(self, *, out: Optional[tuple] = None) -> tuple:
         """(m, v): the values of the moments, lists of f32 tensors of the weights' shapes (out: such lists to fill; in
