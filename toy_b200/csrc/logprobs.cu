@@ -139,7 +139,7 @@ __device__ __forceinline__ void move_to(Sums& a, float m, float c) {
 
 template <int NT>
 struct ScoreShared {
-  float group[kGroups];
+  alignas(16) float group[kGroups];
   float red[NT / 32 * 3];
   u64 best[NT / 32];
   float tau;
@@ -213,11 +213,15 @@ template <int NT>
 __device__ void rank_keys(ScoreShared<NT>& sh, int n, int top) {
   if (threadIdx.x < kMaxTop) sh.list[threadIdx.x] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const u64 k = sh.cand[i];
+  const int lane = threadIdx.x % 32;
+  for (int i = threadIdx.x / 32 * 8; i < n; i += NT / 32 * 8) {   // four lanes to a key
+    const u64 k = i + lane / 4 < n ? sh.cand[i + lane / 4] : 0;
     int r = 0;
-    for (int j = 0; j < n; ++j) r += sh.cand[j] > k;
-    if (r < top && k) sh.list[r] = k;
+#pragma unroll 4
+    for (int j = lane % 4; j < n; j += 4) r += sh.cand[j] > k;
+    r += __shfl_xor_sync(0xffffffffu, r, 1);
+    r += __shfl_xor_sync(0xffffffffu, r, 2);
+    if (lane % 4 == 0 && r < top && k) sh.list[r] = k;
   }
   __syncthreads();
 }
@@ -276,7 +280,12 @@ __device__ void find_top(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, in
   if (tid < kGroups) {
     const float v = sh.group[tid];
     int r = 0;
-    for (int j = 0; j < kGroups; ++j) r += sh.group[j] > v || (sh.group[j] == v && j < tid);
+#pragma unroll 16
+    for (int j = 0; j < kGroups; j += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(&sh.group[j]);
+      r += (q.x > v || (q.x == v && j < tid)) + (q.y > v || (q.y == v && j + 1 < tid)) +
+           (q.z > v || (q.z == v && j + 2 < tid)) + (q.w > v || (q.w == v && j + 3 < tid));
+    }
     if (r == top - 1) sh.tau = v;
   }
   __syncthreads();
@@ -423,7 +432,10 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs 
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) sh.red[warp] = m;
   __syncthreads();
-  for (int w = 0; w < NT / 32; ++w) m = fmaxf(m, sh.red[w]);
+  m = lane < NT / 32 ? sh.red[lane] : -INFINITY;
+#pragma unroll
+  for (int o = NT / 64; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  m = __shfl_sync(0xffffffffu, m, 0);
   move_to<ENT>(t, m, c);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -435,11 +447,15 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs 
     sh.red[2 * (NT / 32) + warp] = t.u;
   }
   __syncthreads();
-  t.s = t.u = 0.f;
-  for (int w = 0; w < NT / 32; ++w) {
-    t.s += sh.red[NT / 32 + w];
-    if (ENT) t.u += sh.red[2 * (NT / 32) + w];
+  t.s = lane < NT / 32 ? sh.red[NT / 32 + lane] : 0.f;
+  t.u = ENT && lane < NT / 32 ? sh.red[2 * (NT / 32) + lane] : 0.f;
+#pragma unroll
+  for (int o = NT / 64; o; o >>= 1) {
+    t.s += __shfl_xor_sync(0xffffffffu, t.s, o);
+    if (ENT) t.u += __shfl_xor_sync(0xffffffffu, t.u, o);
   }
+  t.s = __shfl_sync(0xffffffffu, t.s, 0);
+  if (ENT) t.u = __shfl_sync(0xffffffffu, t.u, 0);
   if (a.top) {
     __syncthreads();   // red is free
     find_top<T, NT>(sh, row, p0, p1, edges, a.top, share, t.s != t.s);
@@ -453,23 +469,31 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs 
     }
     cluster.sync();
     if (part == 0) {
-      m = t.m;
-      for (int k = 1; k < C; ++k) m = fmaxf(m, *cluster.map_shared_rank(&sh.m, k));
-      move_to<ENT>(t, m, c);
-      for (int k = 1; k < C; ++k) {
-        Sums o;
-        o.m = *cluster.map_shared_rank(&sh.m, k);
-        o.s = *cluster.map_shared_rank(&sh.s, k);
-        o.u = *cluster.map_shared_rank(&sh.u, k);
-        move_to<ENT>(o, m, c);
-        t.s += o.s;
-        t.u += o.u;
+      Sums o;
+      if (lane < C) {
+        o.m = *cluster.map_shared_rank(&sh.m, lane);
+        o.s = *cluster.map_shared_rank(&sh.s, lane);
+        o.u = *cluster.map_shared_rank(&sh.u, lane);
       }
+      m = o.m;
+#pragma unroll
+      for (int k = 4; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+      m = __shfl_sync(0xffffffffu, m, 0);
+      move_to<ENT>(o, m, c);
+#pragma unroll
+      for (int k = 4; k; k >>= 1) {
+        o.s += __shfl_xor_sync(0xffffffffu, o.s, k);
+        o.u += __shfl_xor_sync(0xffffffffu, o.u, k);
+      }
+      t.m = m;
+      t.s = __shfl_sync(0xffffffffu, o.s, 0);
+      t.u = __shfl_sync(0xffffffffu, o.u, 0);
       if (a.top) {
         for (int i = tid; i < C * kMaxTop; i += NT)
-          sh.cand[i] = cluster.map_shared_rank(&sh, i / kMaxTop)->list[i % kMaxTop];
+          if (i % kMaxTop < a.top)
+            sh.cand[i / kMaxTop * a.top + i % kMaxTop] = cluster.map_shared_rank(&sh, i / kMaxTop)->list[i % kMaxTop];
         __syncthreads();
-        rank_keys(sh, C * kMaxTop, a.top);
+        rank_keys(sh, C * a.top, a.top);
       }
     }
     cluster.sync();   // (what the first CTA reads is there until then)
@@ -486,8 +510,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs 
   }
   if (!a.top) return;
   // fewer words than alternatives: those of probability 0, the lowest indices first
-  int have = 0;
-  for (int k = 0; k < a.top; ++k) have += sh.list[k] != 0;
+  const int have = __popc(__ballot_sync(0xffffffffu, lane < a.top && sh.list[lane] != 0));
   if (have < a.top) {
     if (tid == 0) sh.n_found = 0;
     __syncthreads();
