@@ -34,7 +34,8 @@ namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int kGradThreads = 256, kMaxTop = 32, kGroups = 64, kCand = 1024, kTies = 512, kUnroll = 4;
+constexpr int NT = 256;   // threads a CTA, both directions
+constexpr int kMaxTop = 32, kGroups = 64, kCand = 1024, kTies = 512, kUnroll = 4;
 
 struct ScoreArgs {
   const void* x;
@@ -137,7 +138,6 @@ __device__ __forceinline__ void move_to(Sums& a, float m, float c) {
   a.m = m;
 }
 
-template <int NT>
 struct ScoreShared {
   alignas(16) float group[kGroups];
   float red[NT / 32 * 3];
@@ -168,8 +168,8 @@ struct RowShape {
 };
 
 // The CTA's lowest `need` indices of pieces [p0, p1) whose value is v, behind cand[n ..).
-template <class T, int NT>
-__device__ void scan_equal(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, float v, int need, int n) {
+template <class T>
+__device__ void scan_equal(ScoreShared& sh, const RowShape<T>& row, int p0, int p1, float v, int need, int n) {
   constexpr int N = Piece<T>::kN;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int found = 0;
@@ -209,8 +209,7 @@ __device__ void scan_equal(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, 
 }
 
 // cand[0 .. n) by rank: the `top` largest to list (0 past them).
-template <int NT>
-__device__ void rank_keys(ScoreShared<NT>& sh, int n, int top) {
+__device__ void rank_keys(ScoreShared& sh, int n, int top) {
   if (threadIdx.x < kMaxTop) sh.list[threadIdx.x] = 0;
   __syncthreads();
   const int lane = threadIdx.x % 32;
@@ -226,9 +225,31 @@ __device__ void rank_keys(ScoreShared<NT>& sh, int n, int top) {
   __syncthreads();
 }
 
+// The `top` largest keys of C lists in falling order (kMaxTop entries each, 0 past the last) in cand: a key's place is the
+// number of larger ones, found in every list by halving.
+__device__ void merge_lists(ScoreShared& sh, int C, int top) {
+  if (threadIdx.x < kMaxTop) sh.list[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < C * kMaxTop; i += NT) {
+    const u64 k = sh.cand[i];
+    if (!k) continue;
+    int r = 0;
+    for (int l = 0; l < C; ++l) {
+      const u64* q = sh.cand + l * kMaxTop;
+      int c = 0;   // entries of the list before c are larger
+#pragma unroll
+      for (int step = kMaxTop / 2; step; step >>= 1)
+        if (q[c + step - 1] > k) c += step;
+      r += c + (q[c] > k);
+    }
+    if (r < top) sh.list[r] = k;
+  }
+  __syncthreads();
+}
+
 // One round of the CTA's share of the row for each alternative (-inf left out).
-template <class T, int NT>
-__device__ void top_by_rounds(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, int edges, int top) {
+template <class T>
+__device__ void top_by_rounds(ScoreShared& sh, const RowShape<T>& row, int p0, int p1, int edges, int top) {
   constexpr int N = Piece<T>::kN;
   u64 last = ~0ull;
   for (int k = 0; k < kMaxTop; ++k) {
@@ -262,8 +283,8 @@ __device__ void top_by_rounds(ScoreShared<NT>& sh, const RowShape<T>& row, int p
 }
 
 // The CTA's alternatives to list, from the maxima of its threads' shares.
-template <class T, int NT>
-__device__ void find_top(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, int edges, int top,
+template <class T>
+__device__ void find_top(ScoreShared& sh, const RowShape<T>& row, int p0, int p1, int edges, int top,
                          const float (&share)[kUnroll], bool odd) {
   constexpr int N = Piece<T>::kN, kLanes = NT / kGroups;
   const int tid = threadIdx.x;
@@ -328,7 +349,7 @@ __device__ void find_top(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, in
     more = ties;
     for (int i = tid; i < ties; i += NT) sh.cand[n + i] = sh.ties[i];
   } else if (n < top) {
-    scan_equal<T, NT>(sh, row, p0, p1, tau, top - n, n);
+    scan_equal<T>(sh, row, p0, p1, tau, top - n, n);
     more = sh.n_found;
     if (tid < edges) {
       const float x = to_f32(row.x[row.edge(tid)]);
@@ -341,10 +362,10 @@ __device__ void find_top(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, in
 }
 
 // One row by `split` CTAs of a cluster (each a run of its pieces; the first has the values outside the pieces too).
-template <class T, int NT, bool ENT>
-__global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs a) {
+template <class T, bool ENT>
+__global__ void __launch_bounds__(NT, 4) score_kernel(ScoreArgs a) {
   constexpr int N = Piece<T>::kN;
-  __shared__ ScoreShared<NT> sh;
+  __shared__ ScoreShared sh;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int C = a.split, part = blockIdx.x % C;
   const long long r = blockIdx.x / C;
@@ -458,7 +479,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs 
   if (ENT) t.u = __shfl_sync(0xffffffffu, t.u, 0);
   if (a.top) {
     __syncthreads();   // red is free
-    find_top<T, NT>(sh, row, p0, p1, edges, a.top, share, t.s != t.s);
+    find_top<T>(sh, row, p0, p1, edges, a.top, share, t.s != t.s);
   }
   if (C > 1) {   // the row's from its CTAs'
     cg::cluster_group cluster = cg::this_cluster();
@@ -490,10 +511,9 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) score_kernel(ScoreArgs 
       t.u = __shfl_sync(0xffffffffu, o.u, 0);
       if (a.top) {
         for (int i = tid; i < C * kMaxTop; i += NT)
-          if (i % kMaxTop < a.top)
-            sh.cand[i / kMaxTop * a.top + i % kMaxTop] = cluster.map_shared_rank(&sh, i / kMaxTop)->list[i % kMaxTop];
+          sh.cand[i] = cluster.map_shared_rank(&sh, i / kMaxTop)->list[i % kMaxTop];
         __syncthreads();
-        rank_keys(sh, C * a.top, a.top);
+        merge_lists(sh, C, a.top);
       }
     }
     cluster.sync();   // (what the first CTA reads is there until then)
@@ -572,7 +592,7 @@ __device__ __forceinline__ uint4 join_bytes(const uint4& lo, const uint4& hi, in
 // of the result's row; a row of logits that starts elsewhere within its 16 bytes is read in aligned pieces and shifted
 // (509 rows of 50303 f16 words: see the table of measurements in the documentation).
 template <class T, bool ENT>
-__global__ void __launch_bounds__(kGradThreads, 4) score_grad_kernel(GradArgs a) {
+__global__ void __launch_bounds__(NT, 4) score_grad_kernel(GradArgs a) {
   constexpr int N = Piece<T>::kN, kWords = kMaxTop + 1;
   __shared__ float x_at[kWords], g_at[kWords];
   __shared__ int at[kWords];
@@ -621,7 +641,7 @@ __global__ void __launch_bounds__(kGradThreads, 4) score_grad_kernel(GradArgs a)
   const int p0 = (int)((long long)row.P * part / C), p1 = (int)((long long)row.P * (part + 1) / C);
   uint4* dp = reinterpret_cast<uint4*>(d + row.h);
   if (none) {
-    for (int i = p0 + tid; i < p1; i += kGradThreads) dp[i] = make_uint4(0, 0, 0, 0);
+    for (int i = p0 + tid; i < p1; i += NT) dp[i] = make_uint4(0, 0, 0, 0);
   } else {
     const float2 m2 = {-m, -m}, c2 = {c, c}, n2 = {-l2, -l2}, A2 = {A, A}, B2 = {B, B};
     const uint8_t* xs = reinterpret_cast<const uint8_t*>(x + row.h);
@@ -646,20 +666,20 @@ __global__ void __launch_bounds__(kGradThreads, 4) score_grad_kernel(GradArgs a)
     };
     if (sh == 0) {
       int i = p0 + tid;
-      for (; i + (kUnroll - 1) * kGradThreads < p1; i += kUnroll * kGradThreads) {
+      for (; i + (kUnroll - 1) * NT < p1; i += kUnroll * NT) {
         uint4 q[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(xp + i + u * kGradThreads);
+        for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(xp + i + u * NT);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) put(i + u * kGradThreads, q[u]);
+        for (int u = 0; u < kUnroll; ++u) put(i + u * NT, q[u]);
       }
-      for (; i < p1; i += kGradThreads) put(i, __ldcs(xp + i));
+      for (; i < p1; i += NT) put(i, __ldcs(xp + i));
     } else {
       // a piece of the result spans two of the logits; those at the row's ends may reach past it
       const int f0 = row.h * (int)sizeof(T) >= sh ? 0 : 1;
       const long long left = (long long)(V - row.h) * (int)sizeof(T) + sh;   // bytes from xp to the row's end
       const int f1 = (int)min((long long)row.P, (left - 16) / 16);
-      for (int i = p0 + tid; i < p1; i += kGradThreads) {
+      for (int i = p0 + tid; i < p1; i += NT) {
         if (i >= f0 && i < f1) {
           put(i, join_bytes(xp[i], xp[i + 1], sh));
         } else {
@@ -691,14 +711,11 @@ bool rows_ok(long long ld, int V, const void* p, int type) {
 }
 
 // CTAs to a row. With 4 CTAs of 256 threads an SM streams 11 B/ns a CTA, and a CTA has some 3 us to spend besides; the
-// split with the shortest ceil(CTAs / 592) (bytes / split / rate + 3 us) is taken. Where 8 CTAs to a row leave SMs
-// free, CTAs of 1024 threads have a row's whole share in flight at once.
+// split with the shortest ceil(CTAs / 592) (bytes / split / rate + 3 us) is taken. (CTAs of 1024 threads for a few rows,
+// each with its whole share in flight: 4.5 us instead of 3.5 for one row of 49152 f32, and 16 clusters of eight such
+// CTAs do not fit the GPU at once, 18.2 us instead of 9.0 for 16 rows of 128256 with 20 alternatives.)
 template <class T, bool ENT>
 int score_launch(ScoreArgs& k, cudaStream_t st) {
-  if ((long long)k.n * 8 <= kSMs) {
-    k.split = 8;
-    return launch_pdl_cluster(score_kernel<T, 1024, ENT>, dim3(k.n * 8), dim3(1024), 0, st, 8, k);
-  }
   const double bytes = (double)k.V * sizeof(T);
   double best = 1e300;
   for (int c = 1; c <= 8; c *= 2) {
@@ -707,15 +724,13 @@ int score_launch(ScoreArgs& k, cudaStream_t st) {
     const double us = waves * (bytes / c / 11e3 + 3.0);
     if (us < best) best = us, k.split = c;
   }
-  return k.split == 1 ? launch_pdl(score_kernel<T, 256, ENT>, dim3(k.n), dim3(256), 0, st, k)
-                      : launch_pdl_cluster(score_kernel<T, 256, ENT>, dim3(k.n * k.split), dim3(256), 0, st, k.split, k);
+  return k.split == 1 ? launch_pdl(score_kernel<T, ENT>, dim3(k.n), dim3(256), 0, st, k)
+                      : launch_pdl_cluster(score_kernel<T, ENT>, dim3(k.n * k.split), dim3(256), 0, st, k.split, k);
 }
 
 template <class T>
 int prepare_type() {
-  if (load_kernel(score_kernel<T, 256, false>) || load_kernel(score_kernel<T, 256, true>) ||
-      load_kernel(score_kernel<T, 1024, false>) || load_kernel(score_kernel<T, 1024, true>))
-    return -3;
+  if (load_kernel(score_kernel<T, false>) || load_kernel(score_kernel<T, true>)) return -3;
   return load_kernel(score_grad_kernel<T, false>) || load_kernel(score_grad_kernel<T, true>) ? -3 : 0;
 }
 }  // namespace
@@ -776,7 +791,7 @@ int tb2_logprobs_grad(const tb2_logprobs_grad_args* a, void* stream) {
     long long c = std::max((bytes + 65535) / 65536, std::min((4LL * kSMs + k.n - 1) / k.n, bytes / 4096));
     k.split = (int)std::max(1LL, std::min(c, 0x7fffffffLL / k.n));
     return launch_pdl(k.g_h ? score_grad_kernel<T, true> : score_grad_kernel<T, false>, dim3(k.n * k.split),
-                      dim3(kGradThreads), 0, static_cast<cudaStream_t>(stream), k);
+                      dim3(NT), 0, static_cast<cudaStream_t>(stream), k);
   });
 }
 
