@@ -387,14 +387,14 @@ __global__ void __launch_bounds__(NT, 4) score_kernel(ScoreArgs a) {
     token = a.tokens[r];
     if (token >= 0 && token < a.V) x_token = to_f32(row.x[token]);
   }
-  // q[0 .. n): pieces of one share each
-  auto absorb = [&](const uint4(&q)[kUnroll], int n) {
+  // q[0 .. n): pieces of the shares from `first` on
+  auto absorb = [&](const uint4(&q)[2], int first, int n) {
     float m = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < 2; ++u)
       if (u < n) {
-        share[u] = fmaxf(share[u], Logits<T>::top(q[u]));
-        m = fmaxf(m, share[u]);
+        share[first + u] = fmaxf(share[first + u], Logits<T>::top(q[u]));
+        m = fmaxf(m, share[first + u]);
       }
     if (m > t.m) {
       t.s = s2.x + s2.y;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(NT, 4) score_kernel(ScoreArgs a) {
     const float ref = t.m == -INFINITY ? 0.f : -t.m;
     const float2 ref2 = {ref, ref};
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < 2; ++u)
       if (u < n) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
@@ -420,24 +420,35 @@ __global__ void __launch_bounds__(NT, 4) score_kernel(ScoreArgs a) {
         }
       }
   };
+  // two pieces are computed while the next two are on their way
   int b = p0 + tid;
-  for (; b + (kUnroll - 1) * NT < p1; b += kUnroll * NT) {
-    uint4 q[kUnroll];
+  uint4 qa[2], qb[2];
+  auto fetch = [&](uint4(&q)[2], int first) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(piece + b + u * NT);
-    absorb(q, kUnroll);
+    for (int u = 0; u < 2; ++u) q[u] = __ldcs(piece + b + (first + u) * NT);
+  };
+  if (b + 3 * NT < p1) {
+    fetch(qa, 0);
+    fetch(qb, 2);
+    while (true) {
+      b += kUnroll * NT;
+      const bool more = b + 3 * NT < p1;
+      absorb(qa, 0, 2);
+      if (more) fetch(qa, 0);
+      absorb(qb, 2, 2);
+      if (!more) break;
+      fetch(qb, 2);
+    }
   }
-  {
-    uint4 q[kUnroll];
-    int n = 0;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (b + u * NT < p1) {
-        q[u] = piece[b + u * NT];
-        n = u + 1;
-      }
-    absorb(q, n);
+  for (int f = 0; f < kUnroll; f += 2) {
+    uint4(&q)[2] = f ? qb : qa;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (b + (f + u) * NT < p1) q[u] = piece[b + (f + u) * NT];
   }
+  absorb(qa, 0, min(2, (p1 - b + NT - 1) / NT));
+  absorb(qb, 2, min(2, (p1 - b + NT - 1) / NT - 2));
   t.s = s2.x + s2.y;
   t.u = u2.x + u2.y;
   if (tid < edges) {   // a value outside the pieces
@@ -666,12 +677,26 @@ __global__ void __launch_bounds__(NT, 4) score_grad_kernel(GradArgs a) {
     };
     if (sh == 0) {
       int i = p0 + tid;
-      for (; i + (kUnroll - 1) * NT < p1; i += kUnroll * NT) {
-        uint4 q[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(xp + i + u * NT);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) put(i + u * NT, q[u]);
+      if (i + 3 * NT < p1) {   // as in the forward
+        uint4 qa[2], qb[2];
+        auto fetch = [&](uint4(&q)[2], int at) {
+          q[0] = __ldcs(xp + at);
+          q[1] = __ldcs(xp + at + NT);
+        };
+        fetch(qa, i);
+        fetch(qb, i + 2 * NT);
+        while (true) {
+          const int at = i;
+          i += kUnroll * NT;
+          const bool more = i + 3 * NT < p1;
+          put(at, qa[0]);
+          put(at + NT, qa[1]);
+          if (more) fetch(qa, i);
+          put(at + 2 * NT, qb[0]);
+          put(at + 3 * NT, qb[1]);
+          if (!more) break;
+          fetch(qb, i + 2 * NT);
+        }
       }
       for (; i < p1; i += NT) put(i, __ldcs(xp + i));
     } else {
@@ -708,6 +733,19 @@ __global__ void __launch_bounds__(NT, 4) score_grad_kernel(GradArgs a) {
 
 bool rows_ok(long long ld, int V, const void* p, int type) {
   return p && ld >= V && aligned(p, type_bytes(type));
+}
+
+// CTAs to a row of the gradient, by the same rule: a CTA reads and writes 5.5 B/ns each and has 2 us to spend besides;
+// it has 4 KB at least.
+int grad_split(int n, double bytes) {
+  double best = 1e300;
+  int split = 1;
+  for (int c = 1; c <= 64 && (c == 1 || bytes / c >= 4096.0) && (long long)n * c <= 0x7fffffffLL; c *= 2) {
+    const long long waves = ((long long)n * c + 4 * kSMs - 1) / (4 * kSMs);
+    const double us = waves * (bytes / c / 5.5e3 + 2.0);
+    if (us < best) best = us, split = c;
+  }
+  return split;
 }
 
 // CTAs to a row. With 4 CTAs of 256 threads an SM streams 11 B/ns a CTA, and a CTA has some 3 us to spend besides; the
@@ -786,10 +824,7 @@ int tb2_logprobs_grad(const tb2_logprobs_grad_args* a, void* stream) {
                 a->d_logits, a->ldd, err, a->scale, a->n_rows, a->vocab, a->top, 1};
   return by_row_type(a->row_type, [&](auto t) {
     using T = decltype(t);
-    // runs of 64 KB, so that the last CTAs end together; less where that leaves SMs without one, 4 KB at least
-    const long long bytes = (long long)k.V * sizeof(T);
-    long long c = std::max((bytes + 65535) / 65536, std::min((4LL * kSMs + k.n - 1) / k.n, bytes / 4096));
-    k.split = (int)std::max(1LL, std::min(c, 0x7fffffffLL / k.n));
+    k.split = grad_split(k.n, (double)k.V * sizeof(T));
     return launch_pdl(k.g_h ? score_grad_kernel<T, true> : score_grad_kernel<T, false>, dim3(k.n * k.split),
                       dim3(NT), 0, static_cast<cudaStream_t>(stream), k);
   });
