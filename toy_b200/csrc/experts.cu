@@ -14,100 +14,161 @@
 
 #include "rows.cuh"
 #include "runtime.cuh"
+#include "warp_reduce.cuh"
 
 namespace tb2 {
 namespace {
 
 namespace cg = cooperative_groups;
 
+constexpr int kOneCta = 256, kOrderApart = 8192;   // slots
 constexpr int kMaxExperts = 1024, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCtas = 8;
 
-__device__ __forceinline__ int expert_of(const void* ids, int wide, long long i, int E) {
+// A slot's expert, or E: none (past: the id is no expert's).
+__device__ __forceinline__ int expert_of(const void* ids, int wide, long long i, int E, bool& past) {
   const long long e = wide ? static_cast<const long long*>(ids)[i] : static_cast<const int*>(ids)[i];
-  return e >= E ? kMaxExperts : e < 0 ? -1 : (int)e;   // kMaxExperts: no expert's
+  past |= e >= E;
+  return e >= E || e < 0 ? E : (int)e;
+}
+
+// The lanes with this lane's value of BITS bits. (A ballot a bit; __match_any_sync took longer: sorting 262144 slots 67 us
+// instead of 44.)
+template <int BITS>
+__device__ __forceinline__ unsigned same_lanes(int e) {
+  unsigned same = 0xffffffffu;
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) same &= __ballot_sync(0xffffffffu, e >> b & 1) ^ ((unsigned)(e >> b & 1) - 1u);
+  return same;
 }
 
 // A stable counting sort in one launch of a cluster. Every warp has a run of
-// the slots. It counts its run's experts in shared memory, one atomic-free
-// update per distinct expert of 32 slots (match_any); the runs' counts are
+// the slots. It counts its run's experts in shared memory; the runs' counts are
 // summed over warps and CTAs (distributed shared memory), which gives every
-// warp the place of its first slot of each expert, and the second walk of the
-// run hands out the places in slot order. No workspace, no second launch.
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(const void* ids, int wide, int n, int E, int* offsets,
-                                                            int* order, int* pos, int* err) {
-  extern __shared__ int count[];                   // [kSortWarps][E]: then each warp's next place
+// warp the place of its first slot of each expert; and the second walk of the
+// run hands out the places in slot order, 32 slots at a time by the lanes that
+// share an expert. No workspace. What it takes is latency where slots are few
+// (ids are read eight times 32 at once and kept where a run is no longer, and
+// as many warps take part as have 32 slots, so that few counts are summed) and
+// the instructions of eight SMs where they are many.
+constexpr int kAhead = 8;
+template <int BITS>
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const void* ids, int wide, int n, int E, int warps,
+                                                            int* offsets, int* order, int* pos, int* err) {
+  // order NULL: a launch of its own writes it
+  extern __shared__ int count[];                   // [warps][E]: then each warp's next place
   __shared__ int total[kMaxExperts];               // this CTA's slots of each expert
   __shared__ int warp_sum[kSortWarps];
   __shared__ int live;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  for (int i = tid; i < kSortWarps * E; i += kSortThreads) count[i] = 0;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, threads = blockDim.x;
+  for (int i = tid; i < warps * E; i += threads) count[i] = 0;
   // runs of a multiple of 32 slots
-  const long long run = ((long long)n + 32 * C * kSortWarps - 1) / (32 * C * kSortWarps) * 32;
-  const long long i0 = min((long long)n, run * (part * kSortWarps + warp)), i1 = min((long long)n, i0 + run);
+  const long long run = ((long long)n + 32 * C * warps - 1) / (32 * C * warps) * 32;
+  const long long i0 = warp < warps ? min((long long)n, run * (part * warps + warp)) : n, i1 = min((long long)n, i0 + run);
   griddep_wait();
+  int e[kAhead];
+  bool past = false;
+  auto read = [&](long long b) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      e[k] = b + 32 * k + lane < i1 ? expert_of(ids, wide, b + 32 * k + lane, E, past) : E;
+  };
+  read(i0);
   __syncthreads();
   int* mine = count + warp * E;
-  bool bad = false;
-  for (long long b = i0; b < i1; b += 32) {
-    const int e = b + lane < i1 ? expert_of(ids, wide, b + lane, E) : -1;
-    bad |= e == kMaxExperts;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && e < E && (same & ((1u << lane) - 1)) == 0) mine[e] += __popc(same);
-    __syncwarp();
+  for (long long b = i0; b < i1; b += 32 * kAhead) {
+    if (b > i0) read(b);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (e[k] < E) atomicAdd(&mine[e[k]], 1);
+    }
   }
-  if (bad) atomicExch(err, (int)kErrExpert);
+  if (past) atomicExch(err, (int)kErrExpert);
   __syncthreads();
   // a thread an expert: its warps' counts become their offsets in this CTA
-  int sum = 0;
-  if (tid < E)
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = count[w * E + tid];
-      count[w * E + tid] = sum;
+  for (int x = tid; x < E; x += threads) {
+    int sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) {
+      const int c = count[w * E + x];
+      count[w * E + x] = sum;
       sum += c;
     }
-  if (tid < E) total[tid] = sum;
-  cluster.sync();
-  int before = 0, all = 0;   // this expert's slots in earlier CTAs, and in all
-  if (tid < E)
-    for (int k = 0; k < C; ++k) {
-      const int c = cluster.map_shared_rank(total, k)[tid];
-      before += k < part ? c : 0;
-      all += c;
-    }
-  // the experts before this one
-  int incl = all;
+    total[x] = sum;
+  }
+  if (C > 1) cluster.sync();
+  else __syncthreads();
+  // the experts in blocks of a CTA's threads
+  for (int x0 = 0, base0 = 0; x0 < E; x0 += threads) {
+    const int x = x0 + tid;
+    int before = 0, all = 0;   // this expert's slots in earlier CTAs, and in all
+    if (x < E) {
+      int c[kSortCtas];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int q = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += q;
+      for (int k = 0; k < kSortCtas; ++k) c[k] = k < C ? cluster.map_shared_rank(total, k)[x] : 0;
+#pragma unroll
+      for (int k = 0; k < kSortCtas; ++k) {
+        before += k < part ? c[k] : 0;
+        all += c[k];
+      }
+    }
+    // the experts before this one
+    int incl = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int q = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += q;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int ahead = lane < threads / 32 && lane < warp ? warp_sum[lane] : 0, sum = lane < threads / 32 ? warp_sum[lane] : 0;
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    const int base = base0 + ahead + incl - all;
+    if (x < E) {
+      if (part == 0) offsets[x] = base;
+      if (x == E - 1) {
+        live = base + all;
+        if (part == 0) offsets[E] = base + all;
+      }
+#pragma unroll 8
+      for (int w = 0; w < warps; ++w) count[w * E + x] += base + before;
+    }
+    base0 += sum;
+    __syncthreads();
   }
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  int base = incl - all;
-  for (int w = 0; w < kSortWarps; ++w) base += w < warp ? warp_sum[w] : 0;
-  if (tid == E - 1) live = base + all;
-  if (part == 0 && tid < E) {
-    offsets[tid] = base;
-    if (tid == E - 1) offsets[E] = base + all;
+  for (long long b = i0; b < i1; b += 32 * kAhead) {
+    if (run > 32 * kAhead) read(b);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const long long i = b + 32 * k + lane;
+      if (b + 32 * k >= i1) break;
+      const unsigned same = same_lanes<BITS>(e[k]), lower = same & ((1u << lane) - 1);
+      const bool on = e[k] < E;
+      const int at = on ? mine[e[k]] + __popc(lower) : -1;
+      __syncwarp();
+      if (on && lower == 0) mine[e[k]] += __popc(same);
+      __syncwarp();
+      if (i < i1) pos[i] = at;
+      if (on && order) order[at] = (int)i;
+    }
   }
-  if (tid < E)
-    for (int w = 0; w < kSortWarps; ++w) count[w * E + tid] += base + before;
-  __syncthreads();
-  for (long long b = i0; b < i1; b += 32) {
-    const int e = b + lane < i1 ? expert_of(ids, wide, b + lane, E) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e), lower = same & ((1u << lane) - 1);
-    const bool on = e >= 0 && e < E;
-    const int at = on ? mine[e] + __popc(lower) : -1;
-    __syncwarp();
-    if (on && lower == 0) mine[e] += __popc(same);
-    __syncwarp();
-    if (b + lane < i1) pos[b + lane] = at;
-    if (on) order[at] = (int)(b + lane);
+  if (order)
+    for (long long i = (long long)live + part * threads + tid; i < n; i += (long long)C * threads) order[i] = -1;
+  if (C > 1) cluster.sync();   // (the totals are read until here)
+}
+
+// order from its inverse, over the whole GPU: eight SMs write 32 places a warp one after another (32768 slots: see
+// tb2_expert_sort).
+__global__ void __launch_bounds__(256) order_kernel(const int* pos, const int* live, int n, int* order) {
+  griddep_wait();
+  const int from = *live;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+    const int p = pos[i];
+    if (p >= 0) order[p] = i;
+    if (i >= from) order[i] = -1;
   }
-  for (long long i = (long long)live + part * kSortThreads + tid; i < n; i += (long long)C * kSortThreads) order[i] = -1;
-  cluster.sync();   // (the totals are read until here)
 }
 
 struct RowsArgs {
@@ -119,8 +180,13 @@ struct RowsArgs {
   long long ldx, ldz, ldr, ldy, lddz;
   int* err;
   int T, K, d, rows;
-  int per;   // pieces to a row
+  int per;             // pieces to a row
+  unsigned magic;      // ceil(2^(31 + shift) / per), 2^shift >= per: i / per = i magic >> (31 + shift) for i < 2^31
+  int shift;
 };
+__device__ __forceinline__ long long row_of(const RowsArgs& a, long long i) {
+  return i >> 31 ? i / a.per : (long long)((unsigned long long)(unsigned)i * a.magic >> (31 + a.shift));
+}
 
 __device__ __forceinline__ int place(const RowsArgs& a, long long slot) {
   const int p = a.pos[slot];
@@ -128,7 +194,7 @@ __device__ __forceinline__ int place(const RowsArgs& a, long long slot) {
   return p < a.rows ? p : -1;
 }
 
-// A piece of a row: 16 bytes where every row starts on 16 bytes and is made of them (V = uint4), else one value.
+// A piece of a row of T: the most bytes (16, 8, 4 or 2) that every row given starts on and consists of.
 template <class T, class V>
 struct Chunk {
   static constexpr int kN = sizeof(V) / sizeof(T);
@@ -164,97 +230,140 @@ __device__ void clear_rest(const RowsArgs& a, void* y, long long ld) {
   const long long from = max(*a.n_sorted, 0), all = ((long long)a.rows - from) * a.per;
   V zero;
   memset(&zero, 0, sizeof zero);
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL)
-    Chunk<T, V>::store(y, from + i / a.per, ld, (int)(i % a.per), zero);
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+    const long long r = row_of(a, i);
+    Chunk<T, V>::store(y, from + r, ld, (int)(i - r * a.per), zero);
+  }
 }
 
-// A thread has one piece of one token's row: read once, written to the token's places (one place read ahead).
-template <class T, class V>
+// A thread has one piece of U tokens' rows: read once, written to the tokens' places.
+template <class T, class V, int U>
 __global__ void __launch_bounds__(256) dispatch_kernel(RowsArgs a) {
   griddep_wait();
-  const long long all = (long long)a.T * a.per;
+  const long long groups = ((long long)a.T + U - 1) / U, all = groups * a.per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
-    const long long t = i / a.per;
-    const int c = (int)(i - t * a.per);
-    const V v = Chunk<T, V>::load_once(a.x, t, a.ldx, c);
+    const long long g = row_of(a, i), t = g * U;
+    const int c = (int)(i - g * a.per), n = (int)min((long long)U, a.T - t);
+    V v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < n) v[u] = Chunk<T, V>::load_once(a.x, t + u, a.ldx, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < n) {
 #pragma unroll 8
-    for (int k = 0; k < a.K; ++k) {
-      const int p = place(a, t * a.K + k);
-      if (p >= 0) Chunk<T, V>::store(a.y, p, a.ldy, c, v);
-    }
+        for (int k = 0; k < a.K; ++k) {
+          const int p = place(a, (t + u) * a.K + k);
+          if (p >= 0) Chunk<T, V>::store(a.y, p, a.ldy, c, v[u]);
+        }
+      }
   }
   clear_rest<T, V>(a, a.y, a.ldy);
 }
 
-// A thread has one piece of one token's row; the places' pieces are read eight at a time.
-template <class T, class V>
+// A thread has one piece of U tokens' rows; their places' pieces are read K at a time (U K on their way at once).
+template <class T, class V, int U, int K>
 __global__ void __launch_bounds__(256) combine_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
-  constexpr int kAhead = 8;
   griddep_wait();
-  const long long all = (long long)a.T * a.per;
+  const long long groups = ((long long)a.T + U - 1) / U, all = groups * a.per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
-    const long long t = i / a.per;
-    const int c = (int)(i - t * a.per);
-    float y[H::kN];
+    const long long g = row_of(a, i), t = g * U;
+    const int c = (int)(i - g * a.per), n = (int)min((long long)U, a.T - t);
+    float y[U][H::kN];
+    if (a.res) {
+      V r[U];
 #pragma unroll
-    for (int e = 0; e < H::kN; ++e) y[e] = 0.f;
-    if (a.res) H::get(H::load_once(a.res, t, a.ldr, c), y);
-    for (int k0 = 0; k0 < a.K; k0 += kAhead) {
-      V z[kAhead];
-      int p[kAhead];
+      for (int u = 0; u < U; ++u)
+        if (u < n) r[u] = H::load_once(a.res, t + u, a.ldr, c);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        p[k] = k0 + k < a.K ? place(a, t * a.K + k0 + k) : -1;
-        if (p[k] >= 0) z[k] = H::load_once(a.z, p[k], a.ldz, c);
-      }
+      for (int u = 0; u < U; ++u)
+        if (u < n) H::get(r[u], y[u]);
+    } else {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (p[k] >= 0) {
-          const float w = a.w ? a.w[t * a.K + k0 + k] : 1.f;
-          float f[H::kN];
-          H::get(z[k], f);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < H::kN; ++e) y[e] = fmaf(w, f[e], y[e]);
-        }
+        for (int e = 0; e < H::kN; ++e) y[u][e] = 0.f;
     }
-    H::store(a.y, t, a.ldy, c, H::put(y));
+    for (int k0 = 0; k0 < a.K; k0 += K) {
+      V z[U][K];
+      int p[U][K];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < K; ++k) p[u][k] = u < n && k0 + k < a.K ? place(a, (t + u) * a.K + k0 + k) : -1;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (p[u][k] >= 0) z[u][k] = H::load_once(a.z, p[u][k], a.ldz, c);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (p[u][k] >= 0) {
+            const float w = a.w ? a.w[(t + u) * a.K + k0 + k] : 1.f;
+            float f[H::kN];
+            H::get(z[u][k], f);
+#pragma unroll
+            for (int e = 0; e < H::kN; ++e) y[u][e] = fmaf(w, f[e], y[u][e]);
+          }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < n) H::store(a.y, t + u, a.ldy, c, H::put(y[u]));
   }
 }
 
-// A warp has a slot: its token's gradient and its row are read once (the token's other slots, next in line, find the
-// gradient in the caches).
-template <class T, class V>
+// A warp has K slots of a token (its last ones may be fewer): the token's gradient is read once for them, their rows'
+// pieces are on their way together.
+template <class T, class V, int K>
 __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
   griddep_wait();
-  const int lane = threadIdx.x % 32;
-  const long long slots = (long long)a.T * a.K;
-  for (long long s = blockIdx.x * 8LL + threadIdx.x / 32; s < slots; s += gridDim.x * 8LL) {
-    const int p = place(a, s);
-    const long long t = s / a.K;
-    float dot = 0.f;
-    if (p >= 0) {
-      const float w = a.w ? a.w[s] : 1.f;
-#pragma unroll 4
-      for (int c = lane; c < a.per; c += 32) {
-        float g[H::kN], f[H::kN];
-        H::get(H::load(a.x, t, a.ldx, c), g);
-        if (a.dw) {
-          H::get(H::load_once(a.z, p, a.ldz, c), f);
+  const int lane = threadIdx.x % 32, parts = (a.K + K - 1) / K;
+  const long long all = (long long)a.T * parts;
+  for (long long i = blockIdx.x * 8LL + threadIdx.x / 32; i < all; i += gridDim.x * 8LL) {
+    const long long t = i / parts, s = t * a.K + i % parts * K;
+    const int n = (int)min((long long)K, (t + 1) * a.K - s);
+    int p[K];
+    float w[K], dot[K];
 #pragma unroll
-          for (int e = 0; e < H::kN; ++e) dot = fmaf(g[e], f[e], dot);
-        }
-        if (a.dz) {
-#pragma unroll
-          for (int e = 0; e < H::kN; ++e) f[e] = w * g[e];
-          H::store(a.dz, p, a.lddz, c, H::put(f));
-        }
-      }
+    for (int k = 0; k < K; ++k) {
+      p[k] = k < n ? place(a, s + k) : -1;
+      w[k] = p[k] >= 0 && a.w ? a.w[s + k] : 1.f;
+      dot[k] = 0.f;
     }
+    for (int c = lane; c < a.per; c += 32) {
+      V z[K];
+      if (a.dw) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (lane == 0 && a.dw) a.dw[s] = dot;
+        for (int k = 0; k < K; ++k)
+          if (p[k] >= 0) z[k] = H::load_once(a.z, p[k], a.ldz, c);
+      }
+      float g[H::kN];
+      H::get(H::load(a.x, t, a.ldx, c), g);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (p[k] >= 0) {
+          float f[H::kN];
+          if (a.dw) {
+            H::get(z[k], f);
+#pragma unroll
+            for (int e = 0; e < H::kN; ++e) dot[k] = fmaf(g[e], f[e], dot[k]);
+          }
+          if (a.dz) {
+#pragma unroll
+            for (int e = 0; e < H::kN; ++e) f[e] = w[k] * g[e];
+            H::store(a.dz, p[k], a.lddz, c, H::put(f));
+          }
+        }
+    }
+    if (a.dw) {
+      const float d = warp_sum_multi<K>(dot, lane);
+      const int k = warp_sum_multi_index<K>(lane);
+      if (warp_sum_multi_leader<K>(lane) && k < n) a.dw[s + k] = d;
+    }
   }
   if (a.dz) clear_rest<T, V>(a, a.dz, a.lddz);
 }
@@ -264,45 +373,112 @@ bool shape_ok(int T, int K, int d, int rows, int type) {
 }
 bool row_ok(const void* p, long long ld, int d, int type) { return p && ld >= d && aligned(p, type_bytes(type)); }
 
-template <class T, class V>
-int prepare_type() {
-  return load_kernel(dispatch_kernel<T, V>) || load_kernel(combine_kernel<T, V>) || load_kernel(combine_grad_kernel<T, V>)
-             ? -3
-             : 0;
-}
-
-// The kernel's shared-memory limit on the current device, and the largest portable cluster.
+// The kernel's shared-memory limit on the current device.
+template <int BITS>
 int sort_setup() {
   static DeviceOnce once;
   return once.ensure([](int) {
-    return cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(sort_kernel<BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 kSortWarps * kMaxExperts * (int)sizeof(int)) == cudaSuccess
                ? 0
                : -3;
   });
 }
+template <int BITS>
+int sort_launch(const tb2_expert_sort_args& a, int* err, cudaStream_t st) {
+  if (sort_setup<BITS>()) return -3;
+  // one CTA for few slots, and no more warps than have 32 slots
+  const int ctas = a.n_slots <= kOneCta ? 1 : kSortCtas;
+  const int warps = std::max(1, (int)std::min((long long)kSortWarps, ((long long)a.n_slots + 32 * ctas - 1) / (32 * ctas)));
+  const int threads = std::max(warps * 32, std::min(kSortThreads, (a.n_experts + 31) / 32 * 32));
+  const bool apart = a.n_slots > kOrderApart;
+  if (launch_pdl_cluster(sort_kernel<BITS>, dim3(ctas), dim3(threads), (size_t)warps * a.n_experts * sizeof(int), st, ctas,
+                         a.ids, (int)(a.id_bytes == 8), a.n_slots, a.n_experts, warps, a.offsets,
+                         apart ? (int*)nullptr : a.order, a.pos, err))
+    return -3;
+  if (!apart) return 0;
+  return launch_pdl(order_kernel, dim3(std::min((a.n_slots + 255) / 256, 8 * kSMs)), dim3(256), 0, st, (const int*)a.pos,
+                    (const int*)a.offsets + a.n_experts, a.n_slots, a.order);
+}
 
-// f(a value of the row type, a piece): 16-byte pieces where all the rows given consist of them.
+// f(a value of the row type, a piece): see Chunk.
 template <class F>
 int by_piece(RowsArgs& k, int type, std::initializer_list<std::pair<const void*, long long>> rows, F&& f) {
   const long long e = type_bytes(type);
-  bool whole = k.d * e % 16 == 0;
-  for (const auto& r : rows) whole = whole && aligned(r.first, 16) && r.second * e % 16 == 0;
-  k.per = whole ? (int)(k.d * e / 16) : k.d;
-  return by_row_type(type, [&](auto t) { return whole ? f(t, uint4()) : f(t, t); });
+  int bytes = 16;
+  while (bytes > e) {
+    bool fits = k.d * e % bytes == 0;
+    for (const auto& r : rows) fits = fits && aligned(r.first, bytes) && (r.second * e % bytes == 0 || !r.first);
+    if (fits) break;
+    bytes /= 2;
+  }
+  k.per = (int)(k.d * e / bytes);
+  k.shift = 0;
+  while ((1LL << k.shift) < k.per) ++k.shift;
+  k.magic = (unsigned)(((1ULL << (31 + k.shift)) + k.per - 1) / k.per);
+  return by_row_type(type, [&](auto t) {
+    if constexpr (sizeof(t) == 2)
+      if (bytes == 2) return f(t, (unsigned short)0);
+    return bytes == 16 ? f(t, uint4()) : bytes == 8 ? f(t, uint2()) : f(t, 0u);
+  });
 }
+
+// Tokens to a thread: pieces of 4 bytes and less, or few slots, are read for several, where there are threads enough.
+constexpr long long kManyThreads = 1024LL * kSMs;
 unsigned grid_of(long long threads) {
   return (unsigned)std::max(1LL, std::min((threads + 255) / 256, (long long)INT_MAX));
+}
+template <class T, class V, int U>
+int dispatch_launch(const RowsArgs& k, cudaStream_t st) {
+  return launch_pdl(dispatch_kernel<T, V, U>, dim3(grid_of((k.T + U - 1LL) / U * k.per)), dim3(256), 0, st, k);
+}
+template <class T, class V, int U, int K>
+int combine_launch(const RowsArgs& k, cudaStream_t st) {
+  return launch_pdl(combine_kernel<T, V, U, K>, dim3(grid_of((k.T + U - 1LL) / U * k.per)), dim3(256), 0, st, k);
+}
+template <class T, class V>
+int combine_by(const RowsArgs& k, cudaStream_t st) {
+  return k.K <= 2 ? combine_launch<T, V, 1, 2>(k, st)
+       : k.K <= 4 ? combine_launch<T, V, 1, 4>(k, st)
+                  : combine_launch<T, V, 1, 8>(k, st);
+}
+// Slots to a warp: as many as leave 16 warps an SM.
+template <class T, class V, int K>
+int combine_grad_launch(const RowsArgs& k, cudaStream_t st) {
+  return launch_pdl(combine_grad_kernel<T, V, K>, dim3(grid_of((long long)k.T * ((k.K + K - 1) / K) * 32)), dim3(256), 0,
+                    st, k);
+}
+template <class T, class V>
+int combine_grad_by(const RowsArgs& k, cudaStream_t st) {
+  const auto enough = [&](int n) { return (long long)k.T * ((k.K + n - 1) / n) >= 16LL * kSMs; };
+  if (k.K > 4 && enough(8)) return combine_grad_launch<T, V, 8>(k, st);
+  if (k.K > 2 && enough(4)) return combine_grad_launch<T, V, 4>(k, st);
+  if (k.K > 1 && enough(2)) return combine_grad_launch<T, V, 2>(k, st);
+  return combine_grad_launch<T, V, 1>(k, st);
+}
+
+template <class T, class V>
+int prepare_piece() {
+  return load_kernel(dispatch_kernel<T, V, 1>) || load_kernel(dispatch_kernel<T, V, 4>) ||
+                 load_kernel(combine_kernel<T, V, 1, 8>) || load_kernel(combine_kernel<T, V, 1, 4>) ||
+                 load_kernel(combine_kernel<T, V, 1, 2>) ||
+                 load_kernel(combine_grad_kernel<T, V, 1>) || load_kernel(combine_grad_kernel<T, V, 2>) ||
+                 load_kernel(combine_grad_kernel<T, V, 4>) || load_kernel(combine_grad_kernel<T, V, 8>)
+             ? -3
+             : 0;
+}
+template <class T>
+int prepare_type() {
+  if constexpr (sizeof(T) == 2)
+    if (prepare_piece<T, unsigned short>()) return -3;
+  return prepare_piece<T, uint4>() || prepare_piece<T, uint2>() || prepare_piece<T, unsigned>() ? -3 : 0;
 }
 
 }  // namespace
 
 int experts_prepare() {
-  if (sort_setup() || load_kernel(sort_kernel)) return -3;
-  if (prepare_type<float, uint4>() || prepare_type<__half, uint4>() || prepare_type<__nv_bfloat16, uint4>()) return -3;
-  return prepare_type<float, float>() || prepare_type<__half, __half>() || prepare_type<__nv_bfloat16, __nv_bfloat16>()
-             ? -3
-             : 0;
+  if (sort_setup<4>() || sort_setup<7>() || sort_setup<11>() || load_kernel(order_kernel)) return -3;
+  return prepare_type<float>() || prepare_type<__half>() || prepare_type<__nv_bfloat16>() ? -3 : 0;
 }
 
 }  // namespace tb2
@@ -317,12 +493,9 @@ int tb2_expert_sort(const tb2_expert_sort_args* a, void* stream) {
   if (!aligned(a->ids, a->id_bytes) || !all_aligned(4, {a->offsets, a->order, a->pos})) return -1;
   int* err = device_error_word();
   if (!err) return -3;
-  if (sort_setup()) return -3;
-  // one CTA where 32 slots a warp do
-  const int ctas = a->n_slots <= kSortThreads ? 1 : kSortCtas;
-  return launch_pdl_cluster(sort_kernel, dim3(ctas), dim3(kSortThreads), (size_t)kSortWarps * a->n_experts * sizeof(int),
-                            static_cast<cudaStream_t>(stream), ctas, a->ids, (int)(a->id_bytes == 8), a->n_slots,
-                            a->n_experts, a->offsets, a->order, a->pos, err);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);   // (values 0 .. n_experts)
+  return a->n_experts < 16 ? sort_launch<4>(*a, err, st)
+       : a->n_experts < 128 ? sort_launch<7>(*a, err, st) : sort_launch<11>(*a, err, st);
 }
 
 int tb2_expert_dispatch(const tb2_expert_rows_args* a, void* stream) {
@@ -336,8 +509,11 @@ int tb2_expert_dispatch(const tb2_expert_rows_args* a, void* stream) {
   k.T = a->n_tokens; k.K = a->n_used; k.d = a->d; k.rows = a->n_rows;
   if (!(k.err = device_error_word())) return -3;
   return by_piece(k, a->row_type, {{k.x, k.ldx}, {k.y, k.ldy}}, [&](auto t, auto v) {
-    return launch_pdl(dispatch_kernel<decltype(t), decltype(v)>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0,
-                      static_cast<cudaStream_t>(stream), k);
+    using T = decltype(t);
+    using V = decltype(v);
+    return sizeof(V) <= 4 && (long long)k.T * k.per >= kManyThreads
+               ? dispatch_launch<T, V, 4>(k, static_cast<cudaStream_t>(stream))
+               : dispatch_launch<T, V, 1>(k, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -354,8 +530,7 @@ int tb2_expert_combine(const tb2_expert_rows_args* a, void* stream) {
   k.T = a->n_tokens; k.K = a->n_used; k.d = a->d; k.rows = a->n_rows;
   if (!(k.err = device_error_word())) return -3;
   return by_piece(k, a->row_type, {{k.z, k.ldz}, {k.y, k.ldy}, {k.res, k.ldr}}, [&](auto t, auto v) {
-    return launch_pdl(combine_kernel<decltype(t), decltype(v)>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0,
-                      static_cast<cudaStream_t>(stream), k);
+    return combine_by<decltype(t), decltype(v)>(k, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -372,8 +547,7 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args* a, void* stream) {
   k.T = a->n_tokens; k.K = a->n_used; k.d = a->d; k.rows = a->n_rows;
   if (!(k.err = device_error_word())) return -3;
   return by_piece(k, a->row_type, {{k.x, k.ldx}, {k.z, k.ldz}, {k.dz, k.lddz}}, [&](auto t, auto v) {
-    return launch_pdl(combine_grad_kernel<decltype(t), decltype(v)>, dim3(grid_of((long long)k.T * k.K * 32)), dim3(256),
-                      0, static_cast<cudaStream_t>(stream), k);
+    return combine_grad_by<decltype(t), decltype(v)>(k, static_cast<cudaStream_t>(stream));
   });
 }
 
