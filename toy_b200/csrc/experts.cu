@@ -236,88 +236,150 @@ __device__ void clear_rest(const RowsArgs& a, void* y, long long ld) {
   }
 }
 
-// A thread has one piece of U tokens' rows: read once, written to the tokens' places.
-template <class T, class V, int U>
-__global__ void __launch_bounds__(256) dispatch_kernel(RowsArgs a) {
+// A thread has one piece of a token's row: read once, written to the token's places.
+template <class T, class V>
+__global__ void __launch_bounds__(256, 5) dispatch_kernel(RowsArgs a) {
   griddep_wait();
-  const long long groups = ((long long)a.T + U - 1) / U, all = groups * a.per;
+  const long long all = (long long)a.T * a.per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
-    const long long g = row_of(a, i), t = g * U;
-    const int c = (int)(i - g * a.per), n = (int)min((long long)U, a.T - t);
-    V v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (u < n) v[u] = Chunk<T, V>::load_once(a.x, t + u, a.ldx, c);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (u < n) {
+    const long long t = row_of(a, i);
+    const int c = (int)(i - t * a.per);
+    const V v = Chunk<T, V>::load_once(a.x, t, a.ldx, c);
 #pragma unroll 8
-        for (int k = 0; k < a.K; ++k) {
-          const int p = place(a, (t + u) * a.K + k);
-          if (p >= 0) Chunk<T, V>::store(a.y, p, a.ldy, c, v[u]);
-        }
-      }
+    for (int k = 0; k < a.K; ++k) {
+      const int p = place(a, t * a.K + k);
+      if (p >= 0) Chunk<T, V>::store(a.y, p, a.ldy, c, v);
+    }
   }
   clear_rest<T, V>(a, a.y, a.ldy);
 }
 
-// A thread has one piece of U tokens' rows; their places' pieces are read K at a time (U K on their way at once).
-template <class T, class V, int U, int K>
+// Pieces of less than 16 bytes: a warp has kCols of a token's, eight to a lane, so that the places and the rows'
+// addresses are found once for eight. (A thread a piece was bound by its instructions, 220 us instead of ... for 9902
+// tokens of 3 f32 rows of 3395.)
+constexpr int kCols = 256;
+template <class T, class V>
+__global__ void __launch_bounds__(256) dispatch_narrow_kernel(RowsArgs a) {
+  griddep_wait();
+  const int lane = threadIdx.x % 32, groups = (a.per + kCols - 1) / kCols;
+  const long long all = (long long)a.T * groups;
+  for (long long i = blockIdx.x * 8LL + threadIdx.x / 32; i < all; i += gridDim.x * 8LL) {
+    const long long t = i / groups;
+    const int c = (int)(i - t * groups) * kCols + lane;
+    V v[kCols / 32];
+#pragma unroll
+    for (int q = 0; q < kCols / 32; ++q)
+      if (c + 32 * q < a.per) v[q] = Chunk<T, V>::load_once(a.x, t, a.ldx, c + 32 * q);
+    for (int k = 0; k < a.K; ++k) {
+      const int p = place(a, t * a.K + k);
+      if (p < 0) continue;
+#pragma unroll
+      for (int q = 0; q < kCols / 32; ++q)
+        if (c + 32 * q < a.per) Chunk<T, V>::store(a.y, p, a.ldy, c + 32 * q, v[q]);
+    }
+  }
+  clear_rest<T, V>(a, a.y, a.ldy);
+}
+
+// A thread has one piece of a token's row; its places' pieces are read K at a time. (Several tokens to a thread were
+// slower, 75 us instead of 55 for 8192 tokens of 4 f32 rows of 2048: fewer threads fit an SM.)
+template <class T, class V, int K>
 __global__ void __launch_bounds__(256) combine_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
   griddep_wait();
-  const long long groups = ((long long)a.T + U - 1) / U, all = groups * a.per;
+  const long long all = (long long)a.T * a.per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
-    const long long g = row_of(a, i), t = g * U;
-    const int c = (int)(i - g * a.per), n = (int)min((long long)U, a.T - t);
-    float y[U][H::kN];
+    const long long t = row_of(a, i);
+    const int c = (int)(i - t * a.per);
+    V r;
+    if (a.res) r = H::load_once(a.res, t, a.ldr, c);
+    float y[H::kN];
+    for (int k0 = 0; k0 < a.K; k0 += K) {
+      V z[K];
+      int p[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        p[k] = k0 + k < a.K ? place(a, t * a.K + k0 + k) : -1;
+        if (p[k] >= 0) z[k] = H::load_once(a.z, p[k], a.ldz, c);
+      }
+      if (k0 == 0) {
+        if (a.res) {
+          H::get(r, y);
+        } else {
+#pragma unroll
+          for (int e = 0; e < H::kN; ++e) y[e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (p[k] >= 0) {
+          const float w = a.w ? a.w[t * a.K + k0 + k] : 1.f;
+          float f[H::kN];
+          H::get(z[k], f);
+#pragma unroll
+          for (int e = 0; e < H::kN; ++e) y[e] = fmaf(w, f[e], y[e]);
+        }
+    }
+    H::store(a.y, t, a.ldy, c, H::put(y));
+  }
+}
+
+template <class T, class V, int K>
+__global__ void __launch_bounds__(256) combine_narrow_kernel(RowsArgs a) {
+  using H = Chunk<T, V>;
+  constexpr int Q = kCols / 32;
+  griddep_wait();
+  const int lane = threadIdx.x % 32, groups = (a.per + kCols - 1) / kCols;
+  const long long all = (long long)a.T * groups;
+  for (long long i = blockIdx.x * 8LL + threadIdx.x / 32; i < all; i += gridDim.x * 8LL) {
+    const long long t = i / groups;
+    const int c = (int)(i - t * groups) * kCols + lane;
+    float y[Q][H::kN];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+      for (int e = 0; e < H::kN; ++e) y[q][e] = 0.f;
     if (a.res) {
-      V r[U];
+      V r[Q];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < n) r[u] = H::load_once(a.res, t + u, a.ldr, c);
+      for (int q = 0; q < Q; ++q)
+        if (c + 32 * q < a.per) r[q] = H::load_once(a.res, t, a.ldr, c + 32 * q);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < n) H::get(r[u], y[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < H::kN; ++e) y[u][e] = 0.f;
+      for (int q = 0; q < Q; ++q)
+        if (c + 32 * q < a.per) H::get(r[q], y[q]);
     }
     for (int k0 = 0; k0 < a.K; k0 += K) {
-      V z[U][K];
-      int p[U][K];
+      V z[K][Q];
+      float w[K];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int k = 0; k < K; ++k) {
+        const int p = k0 + k < a.K ? place(a, t * a.K + k0 + k) : -1;
+        w[k] = p < 0 ? 0.f : a.w ? a.w[t * a.K + k0 + k] : 1.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) p[u][k] = u < n && k0 + k < a.K ? place(a, (t + u) * a.K + k0 + k) : -1;
+        for (int q = 0; q < Q; ++q) {
+          memset(&z[k][q], 0, sizeof(V));
+          if (p >= 0 && c + 32 * q < a.per) z[k][q] = H::load_once(a.z, p, a.ldz, c + 32 * q);
+        }
+      }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int k = 0; k < K; ++k)   // (a slot that takes no part adds 0 times 0)
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (p[u][k] >= 0) z[u][k] = H::load_once(a.z, p[u][k], a.ldz, c);
+        for (int q = 0; q < Q; ++q) {
+          float f[H::kN];
+          H::get(z[k][q], f);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (p[u][k] >= 0) {
-            const float w = a.w ? a.w[(t + u) * a.K + k0 + k] : 1.f;
-            float f[H::kN];
-            H::get(z[u][k], f);
-#pragma unroll
-            for (int e = 0; e < H::kN; ++e) y[u][e] = fmaf(w, f[e], y[u][e]);
-          }
+          for (int e = 0; e < H::kN; ++e) y[q][e] = fmaf(w[k], f[e], y[q][e]);
+        }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (u < n) H::store(a.y, t + u, a.ldy, c, H::put(y[u]));
+    for (int q = 0; q < Q; ++q)
+      if (c + 32 * q < a.per) H::store(a.y, t, a.ldy, c + 32 * q, H::put(y[q]));
   }
 }
 
 // A warp has K slots of a token (its last ones may be fewer): the token's gradient is read once for them, their rows'
 // pieces are on their way together.
-template <class T, class V, int K>
+template <class T, class V, int K, int Q>
 __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
   griddep_wait();
@@ -334,30 +396,37 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
       w[k] = p[k] >= 0 && a.w ? a.w[s + k] : 1.f;
       dot[k] = 0.f;
     }
-    for (int c = lane; c < a.per; c += 32) {
-      V z[K];
+    for (int c0 = lane; c0 < a.per; c0 += 32 * Q) {
+      V z[K][Q];
       if (a.dw) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
-          if (p[k] >= 0) z[k] = H::load_once(a.z, p[k], a.ldz, c);
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+            if (p[k] >= 0 && c0 + 32 * q < a.per) z[k][q] = H::load_once(a.z, p[k], a.ldz, c0 + 32 * q);
       }
-      float g[H::kN];
-      H::get(H::load(a.x, t, a.ldx, c), g);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (p[k] >= 0) {
-          float f[H::kN];
-          if (a.dw) {
-            H::get(z[k], f);
+      for (int q = 0; q < Q; ++q) {
+        const int c = c0 + 32 * q;
+        if (Q > 1 && c >= a.per) break;
+        float g[H::kN];
+        H::get(H::load(a.x, t, a.ldx, c), g);
 #pragma unroll
-            for (int e = 0; e < H::kN; ++e) dot[k] = fmaf(g[e], f[e], dot[k]);
+        for (int k = 0; k < K; ++k)
+          if (p[k] >= 0) {
+            float f[H::kN];
+            if (a.dw) {
+              H::get(z[k][q], f);
+#pragma unroll
+              for (int e = 0; e < H::kN; ++e) dot[k] = fmaf(g[e], f[e], dot[k]);
+            }
+            if (a.dz) {
+#pragma unroll
+              for (int e = 0; e < H::kN; ++e) f[e] = w[k] * g[e];
+              H::store(a.dz, p[k], a.lddz, c, H::put(f));
+            }
           }
-          if (a.dz) {
-#pragma unroll
-            for (int e = 0; e < H::kN; ++e) f[e] = w[k] * g[e];
-            H::store(a.dz, p[k], a.lddz, c, H::put(f));
-          }
-        }
+      }
     }
     if (a.dw) {
       const float d = warp_sum_multi<K>(dot, lane);
@@ -423,30 +492,35 @@ int by_piece(RowsArgs& k, int type, std::initializer_list<std::pair<const void*,
   });
 }
 
-// Tokens to a thread: pieces of 4 bytes and less, or few slots, are read for several, where there are threads enough.
-constexpr long long kManyThreads = 1024LL * kSMs;
 unsigned grid_of(long long threads) {
   return (unsigned)std::max(1LL, std::min((threads + 255) / 256, (long long)INT_MAX));
 }
-template <class T, class V, int U>
-int dispatch_launch(const RowsArgs& k, cudaStream_t st) {
-  return launch_pdl(dispatch_kernel<T, V, U>, dim3(grid_of((k.T + U - 1LL) / U * k.per)), dim3(256), 0, st, k);
+unsigned narrow_grid(const RowsArgs& k) { return grid_of((long long)k.T * ((k.per + kCols - 1) / kCols) * 32); }
+template <class T, class V>
+int dispatch_by(const RowsArgs& k, cudaStream_t st) {
+  if constexpr (sizeof(V) < 16) return launch_pdl(dispatch_narrow_kernel<T, V>, dim3(narrow_grid(k)), dim3(256), 0, st, k);
+  else return launch_pdl(dispatch_kernel<T, V>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0, st, k);
 }
-template <class T, class V, int U, int K>
+template <class T, class V, int K>
 int combine_launch(const RowsArgs& k, cudaStream_t st) {
-  return launch_pdl(combine_kernel<T, V, U, K>, dim3(grid_of((k.T + U - 1LL) / U * k.per)), dim3(256), 0, st, k);
+  return launch_pdl(combine_kernel<T, V, K>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0, st, k);
 }
 template <class T, class V>
 int combine_by(const RowsArgs& k, cudaStream_t st) {
-  return k.K <= 2 ? combine_launch<T, V, 1, 2>(k, st)
-       : k.K <= 4 ? combine_launch<T, V, 1, 4>(k, st)
-                  : combine_launch<T, V, 1, 8>(k, st);
+  if constexpr (sizeof(V) < 16)
+    return launch_pdl(k.K <= 2 ? combine_narrow_kernel<T, V, 2> : combine_narrow_kernel<T, V, 4>, dim3(narrow_grid(k)),
+                      dim3(256), 0, st, k);
+  else
+    return k.K <= 2 ? combine_launch<T, V, 2>(k, st)
+         : k.K <= 4 ? combine_launch<T, V, 4>(k, st) : combine_launch<T, V, 8>(k, st);
 }
 // Slots to a warp: as many as leave 16 warps an SM.
+template <class V>
+constexpr int kGradCols = sizeof(V) == 16 ? 1 : sizeof(V) == 8 ? 2 : 4;
 template <class T, class V, int K>
 int combine_grad_launch(const RowsArgs& k, cudaStream_t st) {
-  return launch_pdl(combine_grad_kernel<T, V, K>, dim3(grid_of((long long)k.T * ((k.K + K - 1) / K) * 32)), dim3(256), 0,
-                    st, k);
+  return launch_pdl(combine_grad_kernel<T, V, K, kGradCols<V>>, dim3(grid_of((long long)k.T * ((k.K + K - 1) / K) * 32)),
+                    dim3(256), 0, st, k);
 }
 template <class T, class V>
 int combine_grad_by(const RowsArgs& k, cudaStream_t st) {
@@ -459,13 +533,20 @@ int combine_grad_by(const RowsArgs& k, cudaStream_t st) {
 
 template <class T, class V>
 int prepare_piece() {
-  return load_kernel(dispatch_kernel<T, V, 1>) || load_kernel(dispatch_kernel<T, V, 4>) ||
-                 load_kernel(combine_kernel<T, V, 1, 8>) || load_kernel(combine_kernel<T, V, 1, 4>) ||
-                 load_kernel(combine_kernel<T, V, 1, 2>) ||
-                 load_kernel(combine_grad_kernel<T, V, 1>) || load_kernel(combine_grad_kernel<T, V, 2>) ||
-                 load_kernel(combine_grad_kernel<T, V, 4>) || load_kernel(combine_grad_kernel<T, V, 8>)
-             ? -3
-             : 0;
+  constexpr int Q = kGradCols<V>;
+  if (load_kernel(combine_grad_kernel<T, V, 1, Q>) || load_kernel(combine_grad_kernel<T, V, 2, Q>) ||
+      load_kernel(combine_grad_kernel<T, V, 4, Q>) || load_kernel(combine_grad_kernel<T, V, 8, Q>))
+    return -3;
+  if constexpr (sizeof(V) < 16)
+    return load_kernel(dispatch_narrow_kernel<T, V>) || load_kernel(combine_narrow_kernel<T, V, 2>) ||
+                   load_kernel(combine_narrow_kernel<T, V, 4>)
+               ? -3
+               : 0;
+  else
+    return load_kernel(dispatch_kernel<T, V>) || load_kernel(combine_kernel<T, V, 2>) ||
+                   load_kernel(combine_kernel<T, V, 4>) || load_kernel(combine_kernel<T, V, 8>)
+               ? -3
+               : 0;
 }
 template <class T>
 int prepare_type() {
@@ -509,11 +590,7 @@ int tb2_expert_dispatch(const tb2_expert_rows_args* a, void* stream) {
   k.T = a->n_tokens; k.K = a->n_used; k.d = a->d; k.rows = a->n_rows;
   if (!(k.err = device_error_word())) return -3;
   return by_piece(k, a->row_type, {{k.x, k.ldx}, {k.y, k.ldy}}, [&](auto t, auto v) {
-    using T = decltype(t);
-    using V = decltype(v);
-    return sizeof(V) <= 4 && (long long)k.T * k.per >= kManyThreads
-               ? dispatch_launch<T, V, 4>(k, static_cast<cudaStream_t>(stream))
-               : dispatch_launch<T, V, 1>(k, static_cast<cudaStream_t>(stream));
+    return dispatch_by<decltype(t), decltype(v)>(k, static_cast<cudaStream_t>(stream));
   });
 }
 
