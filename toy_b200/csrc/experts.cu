@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(256, 5) dispatch_kernel(RowsArgs a) {
 }
 
 // Pieces of less than 16 bytes: a warp has kCols of a token's, eight to a lane, so that the places and the rows'
-// addresses are found once for eight. (A thread a piece was bound by its instructions, 220 us instead of ... for 9902
-// tokens of 3 f32 rows of 3395.)
+// addresses are found once for eight. (A thread a piece was bound by its instructions: combine of 9902 tokens of 3 f32
+// rows of 3395 220 us instead of 104.)
 constexpr int kCols = 256;
 template <class T, class V>
 __global__ void __launch_bounds__(256) dispatch_narrow_kernel(RowsArgs a) {
@@ -377,8 +377,10 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(RowsArgs a) {
   }
 }
 
-// A warp has K slots of a token (its last ones may be fewer): the token's gradient is read once for them, their rows'
-// pieces are on their way together.
+// A warp has K slots of a token (its last ones may be fewer), Q pieces to a lane at a time: the token's gradient is read
+// once for them, and all their pieces are on their way together. (4096 tokens of 8 bf16 rows of 2048: a warp a slot 62
+// us, a warp eight 54, with the gradient's pieces read behind the rows' 54, now 50. A CTA a token, its warps' parts
+// added up through shared memory, 63.)
 template <class T, class V, int K, int Q>
 __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
@@ -397,20 +399,24 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
       dot[k] = 0.f;
     }
     for (int c0 = lane; c0 < a.per; c0 += 32 * Q) {
-      V z[K][Q];
-      if (a.dw) {
+      V z[K][Q], x[Q];
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+      for (int q = 0; q < Q; ++q) {
+        const int c = c0 + 32 * q;
+        if (c >= a.per) continue;
+        x[q] = H::load(a.x, t, a.ldx, c);
+        if (a.dw) {
 #pragma unroll
-          for (int q = 0; q < Q; ++q)
-            if (p[k] >= 0 && c0 + 32 * q < a.per) z[k][q] = H::load_once(a.z, p[k], a.ldz, c0 + 32 * q);
+          for (int k = 0; k < K; ++k)
+            if (p[k] >= 0) z[k][q] = H::load_once(a.z, p[k], a.ldz, c);
+        }
       }
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         const int c = c0 + 32 * q;
-        if (Q > 1 && c >= a.per) break;
+        if (c >= a.per) continue;
         float g[H::kN];
-        H::get(H::load(a.x, t, a.ldx, c), g);
+        H::get(x[q], g);
 #pragma unroll
         for (int k = 0; k < K; ++k)
           if (p[k] >= 0) {
@@ -514,9 +520,10 @@ int combine_by(const RowsArgs& k, cudaStream_t st) {
     return k.K <= 2 ? combine_launch<T, V, 2>(k, st)
          : k.K <= 4 ? combine_launch<T, V, 4>(k, st) : combine_launch<T, V, 8>(k, st);
 }
-// Slots to a warp: as many as leave 16 warps an SM.
+// Two slots to a warp, one where that would leave less than 16 warps an SM or pieces are of 4 bytes and less (180 us
+// instead of 203 for 9902 tokens of 3 f32 rows of 3395).
 template <class V>
-constexpr int kGradCols = sizeof(V) == 16 ? 1 : sizeof(V) == 8 ? 2 : 4;
+constexpr int kGradCols = sizeof(V) == 16 ? 2 : sizeof(V) == 8 ? 4 : 8;
 template <class T, class V, int K>
 int combine_grad_launch(const RowsArgs& k, cudaStream_t st) {
   return launch_pdl(combine_grad_kernel<T, V, K, kGradCols<V>>, dim3(grid_of((long long)k.T * ((k.K + K - 1) / K) * 32)),
@@ -524,19 +531,17 @@ int combine_grad_launch(const RowsArgs& k, cudaStream_t st) {
 }
 template <class T, class V>
 int combine_grad_by(const RowsArgs& k, cudaStream_t st) {
-  const auto enough = [&](int n) { return (long long)k.T * ((k.K + n - 1) / n) >= 16LL * kSMs; };
-  if (k.K > 4 && enough(8)) return combine_grad_launch<T, V, 8>(k, st);
-  if (k.K > 2 && enough(4)) return combine_grad_launch<T, V, 4>(k, st);
-  if (k.K > 1 && enough(2)) return combine_grad_launch<T, V, 2>(k, st);
+  if constexpr (sizeof(V) > 4)
+    if (k.K > 1 && (long long)k.T * ((k.K + 1) / 2) >= 16LL * kSMs) return combine_grad_launch<T, V, 2>(k, st);
   return combine_grad_launch<T, V, 1>(k, st);
 }
 
 template <class T, class V>
 int prepare_piece() {
   constexpr int Q = kGradCols<V>;
-  if (load_kernel(combine_grad_kernel<T, V, 1, Q>) || load_kernel(combine_grad_kernel<T, V, 2, Q>) ||
-      load_kernel(combine_grad_kernel<T, V, 4, Q>) || load_kernel(combine_grad_kernel<T, V, 8, Q>))
-    return -3;
+  if (load_kernel(combine_grad_kernel<T, V, 1, Q>)) return -3;
+  if constexpr (sizeof(V) > 4)
+    if (load_kernel(combine_grad_kernel<T, V, 2, Q>)) return -3;
   if constexpr (sizeof(V) < 16)
     return load_kernel(dispatch_narrow_kernel<T, V>) || load_kernel(combine_narrow_kernel<T, V, 2>) ||
                    load_kernel(combine_narrow_kernel<T, V, 4>)
