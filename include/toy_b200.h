@@ -644,6 +644,11 @@ int tb2_step_launches(void *sess);
 int tb2_set_use_graph(void *sess, int on);
 int tb2_forward_only(void *sess);
 int tb2_sync(void *sess);
+/* Log probabilities of targets [t_batch * t_seq] (negative: none, 0) from the
+ * last forward's logits (a step's or tb2_forward_only's), which stay on the GPU
+ * (tb2_logprobs), and the entropies (when not NULL), of softmax(scale *
+ * logits); host arrays. 0, -1, -2 before a forward, -3. */
+int tb2_llama_logprobs(void *sess, const long long *targets, int n, float scale, float *logprob, float *entropy);
 /* Run n training steps on the already-uploaded inputs (CUDA-graph replay) and
  * report their device time in *ms (CUDA events on the step stream). The
  * device-timed counterpart of the reference's TNN_STEP_PROFILE split
@@ -934,6 +939,14 @@ int tb2_kv_reset(void *sess);
 int tb2_kv_decode(void *sess, const long long *tokens, const long long *positions, int n_seq, float *logits);
 /* The last step's logits [n_seq][vocab] (n = n_seq * vocab). */
 int tb2_kv_logits(void *sess, float *out, long long n);
+/* Log probabilities from the last step's logits, which stay on the GPU
+ * (tb2_logprobs): of tokens[b] for sequence b (negative: none), the entropy
+ * (when not NULL) and the `top` (at most 32) most likely tokens [n_seq][top]
+ * with theirs, all of softmax(scale * logits); host arrays. Works after
+ * tb2_kv_decode (whose logits may then be NULL) and tb2_kv_decode_paged. -2
+ * before a step. */
+int tb2_kv_logprobs(void *sess, const long long *tokens, int n_seq, float scale, int top, float *logprob,
+                    float *entropy, long long *top_ids, float *top_logprobs);
 /* steps replays of the last decode step's graph timed by CUDA events (ms);
  * the kernels launched per step. */
 int tb2_kv_run(void *sess, int steps, float *ms);

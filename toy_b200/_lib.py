@@ -140,6 +140,7 @@ _SIGS = [
     ("tb2_set_use_graph", I, [VP, I]),
     ("tb2_forward_only", I, [VP]),
     ("tb2_sync", I, [VP]),
+    ("tb2_llama_logprobs", I, [VP, C.POINTER(C.c_longlong), I, C.c_float, C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     ("tb2_debug_activation", LL, [VP, I, I, C.POINTER(C.c_float), LL]),
     ("tb2_run_steps", I, [VP, I, C.POINTER(C.c_float)]),
     ("tb2_llama_set_grad_accumulation", I, [VP, I]),
@@ -342,6 +343,8 @@ _SIGS = [
     ("tb2_kv_reset", I, [VP]),
     ("tb2_kv_decode", I, [VP, C.POINTER(C.c_longlong), C.POINTER(C.c_longlong), I, C.POINTER(C.c_float)]),
     ("tb2_kv_logits", I, [VP, C.POINTER(C.c_float), LL]),
+    ("tb2_kv_logprobs", I, [VP, C.POINTER(C.c_longlong), I, C.c_float, I, C.POINTER(C.c_float), C.POINTER(C.c_float),
+                            C.POINTER(C.c_longlong), C.POINTER(C.c_float)]),
     ("tb2_kv_run", I, [VP, I, C.POINTER(C.c_float)]),
     ("tb2_kv_launches", I, [VP]),
     ("tb2_kv_free", I, [VP]),

@@ -208,6 +208,11 @@ int tb2_forward_only(void* sess) {
   return S(sess)->eng->forward_only();
 }
 
+int tb2_llama_logprobs(void* sess, const long long* targets, int n, float scale, float* logprob, float* entropy) {
+  if (!sess || !S(sess)->eng) return -2;
+  return S(sess)->eng->token_logprobs(targets, n, scale, logprob, entropy);
+}
+
 int tb2_llama_set_grad_accumulation(void* sess, int n_micro) {
   if (!sess || !S(sess)->eng) return -2;
   return S(sess)->eng->set_grad_accumulation(n_micro);

@@ -11,6 +11,7 @@
 #include "flash_attn.cuh"
 #include "lora.cuh"
 #include "runtime.cuh"
+#include "toy_b200.h"
 
 namespace tb2 {
 
@@ -511,7 +512,9 @@ int LlamaEngine::realize() {
       M.gu = f32(NK * 2 * ff);
       M.a = pl(NK * ff);
       M.ye = f32(NK * d);
-      M.gtab = reinterpret_cast<int*>(f32(3 * (NK / 128 + E + 1)));
+      M.offsets = reinterpret_cast<int*>(f32(E + 1));
+      M.ntiles = (int)(NK / 128 + E);
+      M.gtab = reinterpret_cast<int*>(f32(3LL * M.ntiles));
     }
     moe_logits_ = f32((long long)N * E);
     moe_xs_ = pl(NK * d);
@@ -521,10 +524,6 @@ int LlamaEngine::realize() {
     moe_dxs_ = f32(NK * d);
     moe_dw_ = f32(NK);
     moe_dlog_ = pl((long long)N * E);
-    moe_hidx_.resize(NK);
-    moe_hperm_.resize(NK);
-    moe_hpos_.resize(NK);
-    use_graph_ = false;   // host round trip per block: eager steps
   }
   if (!flash_) S_ = f32(att);
   logits_ = f32((long long)N * V);
@@ -1545,8 +1544,8 @@ Operand LlamaEngine::expert_op(const Param& p, int e, int rows, int cols, int mn
   return o;
 }
 
-// The MoE FFN of block l: router GEMM, routing, slots ordered by expert on the
-// host, the experts' gate / up GEMMs over their slot rows (Q8_0 dequantised in
+// The MoE FFN of block l: router GEMM, routing, slots ordered by expert, the
+// experts' gate / up GEMMs over their slot rows (Q8_0 dequantised in
 // the GEMM), SwiGLU, down GEMMs, and the weighted sum back onto the tokens
 // with the residual: x[l + 1] = x1 + sum_k w_k y_k.
 int LlamaEngine::moe_forward(int l) {
@@ -1562,36 +1561,10 @@ int LlamaEngine::moe_forward(int l) {
   gr.epi = epi_rowmajor(kEpiStoreF32, moe_logits_, E);
   CK(gemm(gr));
   KL(launch_moe_route(moe_logits_, N, E, K, c.norm_topk, M.probs, M.idx, M.w, stream_));
-  // slots (token * K + choice) in expert order, ascending within an expert
-  CU(cudaMemcpyAsync(moe_hidx_.data(), M.idx, NK * 4, cudaMemcpyDeviceToHost, stream_));
-  CU(cudaStreamSynchronize(stream_));
-  M.count.assign(E, 0);
-  for (long long i = 0; i < NK; ++i) {
-    const int e = moe_hidx_[i];
-    if (e < 0 || e >= E) return -3;
-    ++M.count[e];
-  }
-  M.offset.assign(E + 1, 0);
-  for (int e = 0; e < E; ++e) M.offset[e + 1] = M.offset[e] + M.count[e];
-  std::vector<int> fill(M.offset.begin(), M.offset.end() - 1);
-  for (long long i = 0; i < NK; ++i) {
-    const int at = fill[moe_hidx_[i]]++;
-    moe_hperm_[at] = (int)i;
-    moe_hpos_[i] = at;
-  }
-  CU(cudaMemcpyAsync(M.perm, moe_hperm_.data(), NK * 4, cudaMemcpyHostToDevice, stream_));
-  CU(cudaMemcpyAsync(M.pos, moe_hpos_.data(), NK * 4, cudaMemcpyHostToDevice, stream_));
-  // the experts' 128-slot M tiles for the grouped GEMMs (one launch per product for all experts)
-  M.htab.clear();
-  for (int e = 0; e < E; ++e)
-    for (int t0 = 0; t0 < M.count[e]; t0 += 128) {
-      M.htab.push_back(e);
-      M.htab.push_back(M.offset[e] + t0);
-      M.htab.push_back(M.offset[e] + std::min(M.count[e], t0 + 128));
-    }
-  M.ntiles = (int)(M.htab.size() / 3);
-  if (M.ntiles > NK / 128 + E + 1) return -3;
-  CU(cudaMemcpyAsync(M.gtab, M.htab.data(), M.htab.size() * 4, cudaMemcpyHostToDevice, stream_));
+  // slots (token * K + choice) in expert order, ascending within an expert, and the experts' 128-slot M tiles for the
+  // grouped GEMMs (one launch per product for all experts)
+  KL(launch_moe_sort(M.idx, NK, E, M.offsets, M.pos, err_, stream_));
+  KL(launch_moe_order(M.offsets, M.pos, NK, E, M.perm, M.gtab, M.ntiles, stream_));
   KL(launch_moe_gather(h2_[l], d, M.perm, NK, K, d, moe_xs_, stream_));
   const Param& Wg = P(pre + "ffn_gate_exps.weight");
   const Param& Wu = P(pre + "ffn_up_exps.weight");
@@ -1674,6 +1647,7 @@ int LlamaEngine::enqueue_forward() {
   const float scale = 1.0f / std::sqrt((float)dh);
   const bool lora = c.mode == 1;
   const Param& E = P("token_embd.weight");
+  forward_made_ = true;
   side_ = wst_ && !profiling_;   // the forward's side work: ring fills one block ahead
   side_forked_ = false;
   sev_next_ = 0;
@@ -2256,6 +2230,26 @@ int LlamaEngine::forward_only() {
   if (!realized_) return -2;
   counting_ = 0;
   return enqueue_forward();
+}
+
+int LlamaEngine::token_logprobs(const long long* targets, int n, float scale, float* logprob, float* entropy) {
+  if (!realized_ || !forward_made_) return -2;
+  if (!targets || !logprob || n != N()) return -1;
+  CU(cudaSetDevice(device_));
+  if (!lp_.p) CK(alloc(lp_, (size_t)n * (8 + 4 * 4)));
+  long long* t = static_cast<long long*>(lp_.p);
+  float *stats = reinterpret_cast<float*>(t + n), *lp = stats + 2LL * n, *ent = lp + n;
+  CK(staged((size_t)n * 8));
+  CU(cudaStreamSynchronize(stream_));
+  memcpy(stage_, targets, (size_t)n * 8);
+  CU(cudaMemcpyAsync(t, stage_, (size_t)n * 8, cudaMemcpyHostToDevice, stream_));
+  const tb2_logprobs_args a = {n, cfg_.vocab, 0, logits_, cfg_.vocab, scale, t, lp, stats, entropy ? ent : nullptr,
+                               0, nullptr, nullptr};
+  if (int rc = tb2_logprobs(&a, stream_)) return rc;
+  CU(cudaMemcpyAsync(logprob, lp, (size_t)n * 4, cudaMemcpyDeviceToHost, stream_));
+  if (entropy) CU(cudaMemcpyAsync(entropy, ent, (size_t)n * 4, cudaMemcpyDeviceToHost, stream_));
+  CU(cudaStreamSynchronize(stream_));
+  return 0;
 }
 
 float LlamaEngine::last_loss() {

@@ -132,6 +132,8 @@ class LlamaEngine {
   // the Adam moments first (tnn_graph_reset semantics).
   int step(bool is_first, bool run_optimizer = true);
   int forward_only();                    // loss only
+  // Log probabilities of targets [N] from the last forward's logits (tb2_logprobs); host arrays, entropy may be null.
+  int token_logprobs(const long long* targets, int n, float scale, float* logprob, float* entropy);
   float last_loss();                     // synchronises
   int sync();
 
@@ -309,17 +311,14 @@ class LlamaEngine {
   bool moe_ = false;
   struct MoeLayer {
     float *probs = nullptr, *w = nullptr, *gu = nullptr, *ye = nullptr;
-    int *idx = nullptr, *perm = nullptr, *pos = nullptr;
+    int *idx = nullptr, *perm = nullptr, *pos = nullptr, *offsets = nullptr;
     int* gtab = nullptr;            // the experts' M tiles (expert, first slot, end slot) for the grouped GEMMs
-    int ntiles = 0;
-    std::vector<int> htab;
+    int ntiles = 0;                 // as many as any routing has; those past the last have no rows
     Planes a;
-    std::vector<int> count, offset;
   };
   std::vector<MoeLayer> moe_l_;
   float *moe_logits_ = nullptr, *moe_das_ = nullptr, *moe_dxs_ = nullptr, *moe_dw_ = nullptr;
   Planes moe_xs_, moe_dye_, moe_dgu_, moe_dlog_;
-  std::vector<int> moe_hidx_, moe_hperm_, moe_hpos_;
   std::vector<float*> qkpre_;   // QK-norm: per block the pre-norm q | k [N][(H + KV) d_head]
   int moe_forward(int l);
   int moe_backward(int l);
@@ -429,6 +428,8 @@ class LlamaEngine {
   float* lora_part_ = nullptr;                 // weight-gradient partial sums
   float2* lse_part_ = nullptr;                 // LM head: (max, sum exp) per 64-column vocab chunk [V/64][N]
   float2* lse_ms_ = nullptr;                   // per row (max, sum exp) [N]
+  DeviceBuf lp_;   // token_logprobs: targets, stats, log probabilities, entropies
+  bool forward_made_ = false;   // logits_ is a forward's
   float *qkv_ = nullptr, *S_ = nullptr, *logits_ = nullptr, *loss_rows_ = nullptr, *loss_ = nullptr;
   float *dx_ = nullptr, *dh_ = nullptr, *da_ = nullptr, *dO32_ = nullptr, *dQ_ = nullptr, *dK_ = nullptr,
         *dV_ = nullptr, *gpart_ = nullptr, *du32_ = nullptr;

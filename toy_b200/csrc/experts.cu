@@ -466,7 +466,7 @@ int sort_launch(const tb2_expert_sort_args& a, int* err, cudaStream_t st) {
   const int ctas = a.n_slots <= kOneCta ? 1 : kSortCtas;
   const int warps = std::max(1, (int)std::min((long long)kSortWarps, ((long long)a.n_slots + 32 * ctas - 1) / (32 * ctas)));
   const int threads = std::max(warps * 32, std::min(kSortThreads, (a.n_experts + 31) / 32 * 32));
-  const bool apart = a.n_slots > kOrderApart;
+  const bool apart = a.order && a.n_slots > kOrderApart;
   if (launch_pdl_cluster(sort_kernel<BITS>, dim3(ctas), dim3(threads), (size_t)warps * a.n_experts * sizeof(int), st, ctas,
                          a.ids, (int)(a.id_bytes == 8), a.n_slots, a.n_experts, warps, a.offsets,
                          apart ? (int*)nullptr : a.order, a.pos, err))
@@ -562,6 +562,11 @@ int prepare_type() {
 
 }  // namespace
 
+int expert_sort_launch(const tb2_expert_sort_args& a, int* err, cudaStream_t st) {
+  return a.n_experts < 16 ? sort_launch<4>(a, err, st)   // (values 0 .. n_experts)
+       : a.n_experts < 128 ? sort_launch<7>(a, err, st) : sort_launch<11>(a, err, st);
+}
+
 int experts_prepare() {
   if (sort_setup<4>() || sort_setup<7>() || sort_setup<11>() || load_kernel(order_kernel)) return -3;
   return prepare_type<float>() || prepare_type<__half>() || prepare_type<__nv_bfloat16>() ? -3 : 0;
@@ -579,9 +584,7 @@ int tb2_expert_sort(const tb2_expert_sort_args* a, void* stream) {
   if (!aligned(a->ids, a->id_bytes) || !all_aligned(4, {a->offsets, a->order, a->pos})) return -1;
   int* err = device_error_word();
   if (!err) return -3;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);   // (values 0 .. n_experts)
-  return a->n_experts < 16 ? sort_launch<4>(*a, err, st)
-       : a->n_experts < 128 ? sort_launch<7>(*a, err, st) : sort_launch<11>(*a, err, st);
+  return expert_sort_launch(*a, err, static_cast<cudaStream_t>(stream));
 }
 
 int tb2_expert_dispatch(const tb2_expert_rows_args* a, void* stream) {

@@ -128,7 +128,7 @@ __device__ __forceinline__ Unit decode(const KArgs& a, int u) {
     r.z = t / a.tiles_m;
     r.m1 = a.M;
   }
-  r.skip = a.causal == 1 && r.n0 > r.m0 + BM - 1;
+  r.skip = (a.causal == 1 && r.n0 > r.m0 + BM - 1) || r.m1 <= r.m0;   // (a listed tile without rows: past the last)
   int kbt = a.kb_total;
   if (a.causal == 2) {
     const int kmax = min(a.K, r.m0 + BM);

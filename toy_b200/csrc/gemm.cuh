@@ -133,7 +133,8 @@ struct GemmDesc {
   // Grouped product (the experts of a mixture-of-experts block): group_mtiles
   // M tiles listed in device memory as triples (group, first row, end row),
   // rows of at most 128 per tile; a tile's rows read A (unbatched, rows of the
-  // whole product) and batch `group` of B, and write only rows below its end.
+  // whole product) and batch `group` of B, and write only rows below its end;
+  // a tile that ends where it begins is passed over.
   // M is the total row count; no K splits, no CTA pairs, batch 1.
   const int* group_tiles = nullptr;
   int group_mtiles = 0;

@@ -183,6 +183,11 @@ namespace tb2 {
 // ---- mixture-of-experts FFN and QK-RMSNorm (moe.cu)
 int launch_moe_route(const float* logits, int N, int E, int K, int norm_topk, float* probs, int* idx, float* w,
                      cudaStream_t st);
+// The slots by expert (offsets [E + 1], pos [NK]), and from these the slots in that order (perm) and the experts' tiles
+// of 128 slots for the grouped GEMMs (tiles [n_tiles][3]: expert, first and end slot, an end at the first past the last).
+int launch_moe_sort(const int* idx, long long NK, int E, int* offsets, int* pos, int* err, cudaStream_t st);
+int launch_moe_order(const int* offsets, const int* pos, long long NK, int E, int* perm, int* tiles, int n_tiles,
+                     cudaStream_t st);
 int launch_moe_gather(Planes h, long long ldh, const int* perm, long long NK, int K, int d, Planes xs, cudaStream_t st);
 int launch_moe_combine(const float* x1, const float* ye, const int* pos, const float* w, int N, int K, int d, float* x2,
                        cudaStream_t st);

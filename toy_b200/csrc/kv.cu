@@ -619,6 +619,7 @@ class KvEngine {
     if (graph_) cudaGraphExecDestroy(graph_);
     for (void* p : bufs_) cudaFree(p);
     if (host_in_) cudaFreeHost(host_in_);
+    if (lp_host_) cudaFreeHost(lp_host_);
     if (st_) cudaStreamDestroy(st_);
   }
 
@@ -658,6 +659,8 @@ class KvEngine {
     a_ = f32((long long)nb_ * ff);
     part_ = f32((long long)nb_ * H * nsplit_ * (dh + 2));
     logits_ = f32((long long)nb_ * V);
+    lp_ids_ = reinterpret_cast<long long*>(f32(2LL * nb_ * (1 + kMaxTop)));
+    lp_out_ = f32((long long)nb_ * (4 + kMaxTop));
     int* io = reinterpret_cast<int*>(f32(2 * kMaxSeq));
     tok_ = io;
     pos_ = io + kMaxSeq;
@@ -695,7 +698,9 @@ class KvEngine {
     }
     for (void* p : bufs_)
       if (!p) return -3;
-    if (cudaMallocHost(&host_in_, 2 * kMaxSeq * sizeof(int)) != cudaSuccess) return -3;
+    if (cudaMallocHost(&host_in_, 2 * kMaxSeq * sizeof(int)) != cudaSuccess ||
+        cudaMallocHost(&lp_host_, kMaxSeq * sizeof(long long)) != cudaSuccess)
+      return -3;
     // every weight view must exist (the training engine was realised with this model)
     for (int l = 0; l < L; ++l) {
       const std::string pre = "blk." + std::to_string(l) + ".";
@@ -708,6 +713,7 @@ class KvEngine {
 
   int reset() {
     cudaSetDevice(e_.device());
+    stepped_ = false;
     const LlamaConfig& c = e_.cfg();
     if (pg_) return reset_paged();
     const long long cache = (long long)c.n_layers * nb_ * c.n_kv * max_T_ * c.d_head;
@@ -733,6 +739,7 @@ class KvEngine {
     }
     if (cudaMemcpyAsync(tok_, host_in_, 2 * kMaxSeq * sizeof(int), cudaMemcpyHostToDevice, st_) != cudaSuccess)
       return -3;
+    stepped_ = false;
     if (!graph_) {   // first step: eager (validates every launch), then captured for replay
       if (int rc = enqueue()) return rc;
       if (int rc = capture()) return rc;
@@ -743,7 +750,8 @@ class KvEngine {
       if (cudaMemcpyAsync(logits_host, logits_, (size_t)nb_ * c.vocab * 4, cudaMemcpyDeviceToHost, st_) != cudaSuccess)
         return -3;
     }
-    return cudaStreamSynchronize(st_) == cudaSuccess ? 0 : -3;
+    stepped_ = cudaStreamSynchronize(st_) == cudaSuccess;
+    return stepped_ ? 0 : -3;
   }
 
   // One step over the paged cache: token[b] >= 0 is appended to sequence b and its logits computed, -1 leaves b alone.
@@ -767,12 +775,15 @@ class KvEngine {
         cudaMemcpyAsync(pg_->add, host_in_ + kMaxSeq, nb_ * sizeof(int), cudaMemcpyHostToDevice, st_) != cudaSuccess)
       return -3;
     int state[4] = {0, 0, 0, 0};
+    stepped_ = false;
     if (int rc = run_paged(state, logits_host)) {
       // whatever part of the step ran, its plan may have: the GPU's lengths hold
       follow_lengths();
       return rc;
     }
-    if (state[1]) return state[1] == 1 ? -5 : -3;   // no room: the plan, and so the step, changed nothing
+    // no room: the plan, and so the step, changed nothing (but the rows of the logits, which mean nothing now)
+    stepped_ = !state[1];
+    if (state[1]) return state[1] == 1 ? -5 : -3;
     for (int b = 0; b < nb_; ++b) pg_->host_len[b] += tokens[b] >= 0;
     // the first step ran eagerly (which validates every launch) and is captured for replay once it is complete and
     // counted; where that fails the next step is eager too
@@ -822,6 +833,30 @@ class KvEngine {
     if (!out || n != (long long)nb_ * c.vocab) return -1;
     if (cudaStreamSynchronize(st_) != cudaSuccess) return -3;
     return cudaMemcpy(out, logits_, n * 4, cudaMemcpyDeviceToHost) == cudaSuccess ? 0 : -3;
+  }
+
+  // Log probabilities from the last step's logits, which stay on the GPU (tb2_logprobs); host arrays.
+  int logprobs(const long long* tokens, int n, float scale, int top, float* logprob, float* entropy, long long* top_ids,
+               float* top_lp) {
+    if (!stepped_) return -2;
+    if (!tokens || !logprob || n != nb_ || top < 0 || top > kMaxTop || (top && (!top_ids || !top_lp))) return -1;
+    if (cudaSetDevice(e_.device()) != cudaSuccess || cudaStreamSynchronize(st_) != cudaSuccess) return -3;
+    // floats: stats, log probabilities, entropies, the alternatives'
+    float *stats = lp_out_, *lp = stats + 2 * nb_, *ent = lp + nb_, *alt = ent + nb_;
+    std::copy(tokens, tokens + nb_, lp_host_);
+    if (cudaMemcpyAsync(lp_ids_, lp_host_, nb_ * sizeof(long long), cudaMemcpyHostToDevice, st_) != cudaSuccess) return -3;
+    const int V = e_.cfg().vocab;
+    const tb2_logprobs_args a = {nb_, V,  kTypeF32, logits_, V, scale, lp_ids_, lp, stats, entropy ? ent : nullptr,
+                                 top, lp_ids_ + nb_, alt};
+    if (int rc = tb2_logprobs(&a, st_)) return rc;
+    auto down = [&](void* to, const void* from, size_t bytes) {
+      return !bytes || !to || cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToHost, st_) == cudaSuccess;
+    };
+    const size_t f4 = sizeof(float);
+    if (!down(logprob, lp, nb_ * f4) || !down(entropy, ent, nb_ * f4) || !down(top_lp, alt, (size_t)nb_ * top * f4) ||
+        !down(top_ids, lp_ids_ + nb_, (size_t)nb_ * top * sizeof(long long)))
+      return -3;
+    return cudaStreamSynchronize(st_) == cudaSuccess ? 0 : -3;
   }
 
   int launches() const { return launches_; }
@@ -1117,6 +1152,11 @@ class KvEngine {
   uint16_t *ks_ = nullptr, *vs_ = nullptr;
   int *tok_ = nullptr, *pos_ = nullptr;
   int* host_in_ = nullptr;
+  // log probabilities: tokens and alternatives, their values, the tokens on the host
+  static constexpr int kMaxTop = 32;
+  bool stepped_ = false;   // logits_ holds a step's
+  long long *lp_ids_ = nullptr, *lp_host_ = nullptr;
+  float* lp_out_ = nullptr;
 };
 
 void kv_free(Session* s) {
@@ -1188,6 +1228,13 @@ int tb2_kv_decode(void* sess, const long long* tokens, const long long* position
 int tb2_kv_logits(void* sess, float* out, long long n) {
   if (!sess || !static_cast<tb2::Session*>(sess)->kv) return -2;
   return static_cast<tb2::Session*>(sess)->kv->logits(out, n);
+}
+
+int tb2_kv_logprobs(void* sess, const long long* tokens, int n_seq, float scale, int top, float* logprob,
+                    float* entropy, long long* top_ids, float* top_logprobs) {
+  if (!sess || !static_cast<tb2::Session*>(sess)->kv) return -2;
+  return static_cast<tb2::Session*>(sess)->kv->logprobs(tokens, n_seq, scale, top, logprob, entropy, top_ids,
+                                                        top_logprobs);
 }
 
 int tb2_kv_run(void* sess, int steps, float* ms) {

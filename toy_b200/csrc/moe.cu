@@ -6,6 +6,9 @@
 //               their weights (renormalised to sum 1 with norm_topk)
 //               -- llama_kv_engine.rb build_moe_ffn :2073 (tnn_softmax,
 //               tnn_top_k, tnn_get_rows of the probabilities);
+//   sort:       the slots by expert on the GPU (experts.cu), the order they are
+//               in and the experts' M tiles for the grouped GEMMs: no round
+//               trip over the host, so the step is captured like the others;
 //   gather:     the (token, k) slots' input rows in expert order, so each
 //               expert's rows are one contiguous GEMM operand (mul_mat_id);
 //   combine:    x2 = x1 + sum_k w_k y_(token, k), k ascending (deterministic);
@@ -25,6 +28,7 @@
 
 #include "kernels.cuh"
 #include "pdl.cuh"
+#include "rows.cuh"
 
 namespace tb2 {
 
@@ -123,9 +127,9 @@ __global__ void moe_route_kernel(const float* __restrict__ logits, int N, int E,
       for (int j = 0; j < kMoeMaxE / 32; ++j)
         if (lane + 32 * j == bi) pv[j] = -2.f;   // taken
       sel_sum += bv;
-      if (lane == k) {
-        mine = bv;
-        mine_i = bi;
+      if (lane == k) {   // (a row of NaN has no largest: some expert of its own for each choice, with the weight NaN)
+        mine = bi < E ? bv : NAN;
+        mine_i = bi < E ? bi : k;
       }
     }
     if (lane < K) {
@@ -133,6 +137,38 @@ __global__ void moe_route_kernel(const float* __restrict__ logits, int N, int E,
       w[n * K + lane] = norm_topk ? mine / sel_sum : mine;
     }
   }
+}
+
+// perm from its inverse pos; the first CTA, a thread an expert, lists the experts' tiles.
+__global__ void __launch_bounds__(256) moe_order_kernel(const int* offsets, const int* pos, long long NK, int E, int* perm,
+                                                        int* tiles, int n_tiles) {
+  griddep_wait();
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < NK; i += gridDim.x * 256LL)
+    if (pos[i] >= 0) perm[pos[i]] = (int)i;
+  if (blockIdx.x) return;
+  __shared__ int sum[8];
+  const int e = threadIdx.x, lane = e % 32;
+  const int lo = e < E ? offsets[e] : 0, hi = e < E ? offsets[e + 1] : 0, n = (hi - lo + 127) / 128;
+  int incl = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int q = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += q;
+  }
+  if (lane == 31) sum[e / 32] = incl;
+  __syncthreads();
+  int at = incl - n, all = 0;
+  for (int w = 0; w < 8; ++w) {
+    at += w < e / 32 ? sum[w] : 0;
+    all += sum[w];
+  }
+  for (int k = 0; k < n && at + k < n_tiles; ++k) {
+    int* t = tiles + 3 * (at + k);
+    t[0] = e;
+    t[1] = lo + 128 * k;
+    t[2] = min(hi, lo + 128 * k + 128);
+  }
+  for (int k = all + e; k < n_tiles; k += 256) tiles[3 * k] = tiles[3 * k + 1] = tiles[3 * k + 2] = 0;
 }
 
 // Xs[i] = h[perm[i] / K] (planes, d columns; h has row pitch ldh)
@@ -302,6 +338,25 @@ int launch_moe_route(const float* logits, int N, int E, int K, int norm_topk, fl
                      cudaStream_t st) {
   if (E < 1 || E > kMoeMaxE || K < 1 || K > kMoeMaxK || K > E || K > 32) return -1;
   launch_pdl(moe_route_kernel, dim3(grid_warps(N)), dim3(256), 0, st, logits, N, E, K, norm_topk, probs, idx, w);
+  return ok();
+}
+
+int launch_moe_sort(const int* idx, long long NK, int E, int* offsets, int* pos, int* err, cudaStream_t st) {
+  if (E < 1 || E > kMoeMaxE || NK < 1 || NK > 0x7fffffffLL) return -1;
+  tb2_expert_sort_args a = {};
+  a.ids = idx;
+  a.id_bytes = 4;
+  a.n_slots = (int)NK;
+  a.n_experts = E;
+  a.offsets = offsets;
+  a.pos = pos;
+  return expert_sort_launch(a, err, st);
+}
+
+int launch_moe_order(const int* offsets, const int* pos, long long NK, int E, int* perm, int* tiles, int n_tiles,
+                     cudaStream_t st) {
+  if (E > kMoeMaxE) return -1;
+  launch_pdl(moe_order_kernel, dim3(grid_items(NK)), dim3(256), 0, st, offsets, pos, NK, E, perm, tiles, n_tiles);
   return ok();
 }
 

@@ -21,6 +21,9 @@ int load_kernel(K* k) {
   cudaFuncAttributes at;
   return cudaFuncGetAttributes(&at, k) == cudaSuccess ? 0 : -3;
 }
+// The slots of ids [n] (0 .. E - 1, or negative: none) by expert: see tb2_expert_sort. order may be NULL.
+int expert_sort_launch(const tb2_expert_sort_args& a, int* err, cudaStream_t st);
+
 int logprobs_prepare();
 int experts_prepare();
 int multi_adamw_prepare();

@@ -7,14 +7,41 @@ or after load_gguf); every step is one graph replay on the GPU."""
 from __future__ import annotations
 
 import ctypes as C
-from typing import Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 
 from ._lib import check, lib
 
 
-class KVDecoder:
+class StepLogprobs(NamedTuple):
+    """What `logprobs` computed for every sequence: see tb2_kv_logprobs."""
+    logprob: np.ndarray                   # [n_seq] f32: ln p of the sequence's token, 0 where that is negative
+    entropy: Optional[np.ndarray]         # [n_seq] f32
+    top_ids: Optional[np.ndarray]         # [n_seq, top] i64, the most likely first, equal logits by the lower index
+    top_logprobs: Optional[np.ndarray]    # [n_seq, top] f32
+
+
+class _Logprobs:
+    def logprobs(self, tokens: Optional[Sequence[int]] = None, *, scale: float = 1.0, entropy: bool = False,
+                 top: int = 0) -> StepLogprobs:
+        """ln p of one token per sequence (negative, or tokens None: none) under softmax(scale * the last step's
+        logits), with the entropy and the `top` (at most 32) most likely tokens where asked for. The logits stay on
+        the GPU: a step whose logits nobody reads is made with logits=False."""
+        t = np.full(self.n_seq, -1, np.int64) if tokens is None else \
+            np.ascontiguousarray(np.asarray(tokens, np.int64).reshape(self.n_seq))
+        if (t >= self.vocab).any() or not 0 <= top <= min(32, self.vocab):
+            raise ValueError(f"toy_b200: tokens below {self.vocab}, top 0 to 32")
+        lp, ent = np.empty(self.n_seq, np.float32), np.empty(self.n_seq, np.float32)
+        ids, alt = np.empty((self.n_seq, top), np.int64), np.empty((self.n_seq, top), np.float32)
+        f, i = C.POINTER(C.c_float), C.POINTER(C.c_longlong)
+        check(lib().tb2_kv_logprobs(self.eng.sess, t.ctypes.data_as(i), self.n_seq, scale, top, lp.ctypes.data_as(f),
+                                    ent.ctypes.data_as(f) if entropy else None, ids.ctypes.data_as(i),
+                                    alt.ctypes.data_as(f)), "tb2_kv_logprobs")
+        return StepLogprobs(lp, ent if entropy else None, ids if top else None, alt if top else None)
+
+
+class KVDecoder(_Logprobs):
     def __init__(self, engine, max_T: int, n_seq: int = 1, kv_q8: bool = False):
         self.eng = engine
         self.max_T, self.n_seq = max_T, n_seq
@@ -25,14 +52,16 @@ class KVDecoder:
     def reset(self) -> None:
         check(lib().tb2_kv_reset(self.eng.sess), "tb2_kv_reset")
 
-    def decode_step(self, tokens: Sequence[int], positions: Sequence[int]) -> np.ndarray:
-        """One token per sequence at its position; returns logits [n_seq, vocab]."""
+    def decode_step(self, tokens: Sequence[int], positions: Sequence[int], logits: bool = True) -> Optional[np.ndarray]:
+        """One token per sequence at its position; returns logits [n_seq, vocab] (None with logits=False: they stay on
+        the GPU, for `logprobs`)."""
         t = np.ascontiguousarray(np.asarray(tokens, np.int64).reshape(self.n_seq))
         p = np.ascontiguousarray(np.asarray(positions, np.int64).reshape(self.n_seq))
         check(lib().tb2_kv_decode(self.eng.sess, t.ctypes.data_as(C.POINTER(C.c_longlong)),
                                   p.ctypes.data_as(C.POINTER(C.c_longlong)), self.n_seq,
-                                  self._logits.ctypes.data_as(C.POINTER(C.c_float))), "tb2_kv_decode")
-        return self._logits.copy()
+                                  self._logits.ctypes.data_as(C.POINTER(C.c_float)) if logits else None),
+              "tb2_kv_decode")
+        return self._logits.copy() if logits else None
 
     def decode_batch(self, token_ids: np.ndarray, pos0: int = 0) -> np.ndarray:
         """Run [n_seq, n] prompt tokens through the cache from position pos0;
@@ -43,13 +72,14 @@ class KVDecoder:
     def generate(self, prompt: np.ndarray, n_new: int) -> np.ndarray:
         """Greedy continuation of [n_seq, n] prompts by n_new tokens each."""
         ids = np.asarray(prompt, np.int64).reshape(self.n_seq, -1)
-        logits = self.decode_batch(ids)[-1]
+        for i in range(ids.shape[1]):
+            self.decode_step(ids[:, i], np.full(self.n_seq, i), logits=False)
         out = []
         pos = ids.shape[1]
         for _ in range(n_new):
-            nxt = np.argmax(logits, axis=-1)
+            nxt = self.logprobs(top=1).top_ids[:, 0]   # (the logits stay on the GPU)
             out.append(nxt)
-            logits = self.decode_step(nxt, np.full(self.n_seq, pos))
+            self.decode_step(nxt, np.full(self.n_seq, pos), logits=False)
             pos += 1
         return np.stack(out, axis=1)
 
@@ -60,7 +90,7 @@ class KVDecoder:
 _KV_TYPES = {"f32": 0, "f16": 1, "q8_0": 8, "bf16": 30}
 
 
-class PagedKVDecoder:
+class PagedKVDecoder(_Logprobs):
     """Decode over a paged cache: up to n_seq sequences of unlike lengths share n_pages pages of page_size tokens
     (tb2_kv_*_paged). kv_type: "f32", "f16", "bf16" or "q8_0"."""
 
@@ -79,16 +109,16 @@ class PagedKVDecoder:
     def reset(self) -> None:
         check(lib().tb2_kv_reset(self.eng.sess), "tb2_kv_reset")
 
-    def decode_step(self, tokens: Sequence[int]) -> np.ndarray:
-        """tokens[b] appended to sequence b (-1: nothing); logits [n_seq, vocab] of the tokens after them. MemoryError
-        when the pool has too few free pages: the step did nothing, and may be repeated after a release."""
+    def decode_step(self, tokens: Sequence[int], logits: bool = True) -> Optional[np.ndarray]:
+        """tokens[b] appended to sequence b (-1: nothing); logits [n_seq, vocab] of the tokens after them (None with
+        logits=False: they stay on the GPU, for `logprobs`). MemoryError when the pool has too few free pages: the step did nothing, and may be repeated after a release."""
         t = np.ascontiguousarray(np.asarray(tokens, np.int64).reshape(self.n_seq))
         rc = lib().tb2_kv_decode_paged(self.eng.sess, t.ctypes.data_as(C.POINTER(C.c_longlong)), self.n_seq,
-                                       self._logits.ctypes.data_as(C.POINTER(C.c_float)))
+                                       self._logits.ctypes.data_as(C.POINTER(C.c_float)) if logits else None)
         if rc == -5:
             raise MemoryError("toy_b200: no free pages for this decode step")
         check(rc, "tb2_kv_decode_paged")
-        return self._logits.copy()
+        return self._logits.copy() if logits else None
 
     def release(self, seqs: Sequence[int]) -> None:
         """Empty these sequences (0 .. n_seq - 1) and give their pages back."""
@@ -128,13 +158,15 @@ class PagedKVDecoder:
         at = [0] * self.n_seq
         while any(len(o) < n_new for o in out):
             toks = [feed[b][at[b]] if len(out[b]) < n_new else -1 for b in range(self.n_seq)]
-            logits = self.decode_step(toks)
+            self.decode_step(toks, logits=False)
+            best = self.logprobs(top=1).top_ids[:, 0] if any(
+                toks[b] >= 0 and at[b] + 1 == len(feed[b]) for b in range(self.n_seq)) else None
             for b in range(self.n_seq):
                 if toks[b] < 0:
                     continue
                 at[b] += 1
                 if at[b] == len(feed[b]):
-                    nxt = int(np.argmax(logits[b]))
+                    nxt = int(best[b])
                     out[b].append(nxt)
                     feed[b].append(nxt)
         return out

@@ -258,6 +258,28 @@ class LlamaSeqEngine:
         what = 1 | (2 if frozen else 0) | (4 if moments else 0) | (8 if stacked else 0)
         check(lib().tb2_llama_save_gguf(self.sess, path.encode(), what), "tb2_llama_save_gguf")
 
+    # ---- log probabilities
+    def token_logprobs(self, targets, scale: float = 1.0, entropy: bool = False):
+        """ln p of targets [t_batch * t_seq] (negative: none, 0) under softmax(scale * the last forward's logits),
+        f32, and with entropy also each token's entropy: (logprob, entropy). The logits stay on the GPU."""
+        t = np.ascontiguousarray(np.asarray(targets, np.int64).reshape(-1))
+        if t.size != self.t_seq * self.t_batch or (t >= self.cfg.vocab).any():
+            raise ValueError(f"toy_b200: {self.t_seq * self.t_batch} targets below {self.cfg.vocab}")
+        out, ent = np.empty(t.size, np.float32), np.empty(t.size, np.float32)
+        f = C.POINTER(C.c_float)
+        check(lib().tb2_llama_logprobs(self.sess, t.ctypes.data_as(C.POINTER(C.c_longlong)), t.size, scale,
+                                       out.ctypes.data_as(f), ent.ctypes.data_as(f) if entropy else None),
+              "tb2_llama_logprobs")
+        return (out, ent) if entropy else out
+
+    def score(self, seq_ids, positions, targets, scale: float = 1.0, entropy: bool = False):
+        """A forward on a batch, without a step, and `token_logprobs` of its targets."""
+        TinyNN.upload_int_array(self.sess, self.t_seq_token_ids, seq_ids)
+        TinyNN.upload_int_array(self.sess, self.t_seq_positions, positions)
+        TinyNN.upload_label_ids(self.sess, lib().tb2_llama_io(self.sess, IO_LABELS), targets)
+        check(lib().tb2_forward_only(self.sess), "tb2_forward_only")
+        return self.token_logprobs(targets, scale, entropy)
+
     def set_grad_accumulation(self, n_micro: int) -> None:
         """Accumulate gradients over n_micro step calls; AdamW runs on every
         n_micro-th call with the mean gradient (the joined-batch step)."""
