@@ -25,9 +25,11 @@ namespace tb2 {
 namespace {
 
 constexpr int kBlock = 256;        // values that share a scale
+constexpr long long kMaxValues = 1LL << 37;   // of a tensor (its blocks, and a launch's, are counted in 30 bits)
 constexpr int kMaxTensors = 448;   // tensors a launch: their descriptors travel as its arguments (30.5 of 32 KB)
 constexpr int kThreads = 256, kWarps = kThreads / 32, kRun = 4;
-constexpr int kCtas8 = 3, kCtas32 = 2;   // CTAs an SM: 80 and 128 registers a thread
+constexpr int kRun32 = 2;
+constexpr int kCtas8 = 3, kCtas32 = 3;   // CTAs an SM: 80 registers a thread
 
 struct Tensors {
   tb2_adamw_tensor t[kMaxTensors];
@@ -138,18 +140,23 @@ __device__ __noinline__ unsigned root_code(float g, float gf, float r0, float b2
   const double gw = (double)g * gf, v = (double)r0 * r0 * b2 + gw * gw * (1.0 - (double)b2);
   return max(e4m3_of(sqrt(v) * inverse), 1u);
 }
-__device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) { w = (w & ~(0xffu << 8 * at)) | q << 8 * at; }
+__device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) {
+  w = (w & ~(0xffu << 8 * at)) | q << 8 * at;
+}
 
-// A warp has a block at a time; the blocks are dealt over the whole grid, so that all CTAs work in the same few pages
-// of every array (a run of blocks to each CTA: 489 us instead of 449 for 135M weights in 8 bits).
+// A warp has a block at a time. Where CTAs end after a few blocks the GPU works in few pages at any time, which is what
+// HBM likes best (135M weights: f32 moments 561 us, with a grid that stays and deals the blocks out 586, with a run of
+// blocks to each CTA 617; the values of 8-bit moments 210, 240 and 267). The 8-bit step has more to compute, and with
+// CTAs that start anew with the factors it takes 475 us instead of 442.
 //
-// 8-bit moments are the exact values rounded once, although the step is f32. m is a sum of two terms of either sign, and
-// with few bits in its old value it falls on a border again and again (0.9 of 120 is 108, between 104 and 112: 0.8 % of
-// the values of a run with b1 = 0.9 are closer to one than f32 tells), so it is computed in f64, two products and three
+// 8-bit moments are the exact values rounded once, although the step is f32. m is a sum of two terms of either sign,
+// and with few bits in its old value it falls on a border again and again (0.9 of 120 is 108, between 104 and 112: 0.8
+// % of the values of a run with b1 = 0.9 are closer to one than f32 tells), so it is computed in f64, two products and three
 // conversions a value, and converted so that the code is rounded from all its bits. A root's code is taken of both ends
 // of an interval that holds the exact one, and where the two differ (one value in 90000) it is rounded from 64 bits.
 // With U = 2^-24: the root's square is a sum of squares, the held root's factor and product 2 + 1 U, the gradient's 3 +
-// 1, doubled by squaring, 1 for a square and 1 for the sum; the root halves these 10, and is off by 2 U itself: 7 U of 8.
+// 1, doubled by squaring, 1 for a square and 1 for the sum; the root halves these 10, and is off by 2 U itself: 7 U of
+// the 8 allowed.
 //
 // Bound by HBM in 32 bits. In 8 bits a value is 16 bytes, the time of some 75 instructions at most: a look at the
 // distance of every root from a border made it 58 (445 us where the bytes of 135M weights take 332), IEEE quotients and
@@ -157,7 +164,8 @@ __device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) { w = 
 // A lane's values of a block as they lie in memory.
 template <class T>
 struct Raw4 {
-  typename std::conditional<sizeof(T) == 4, float4, typename std::conditional<sizeof(T) == 2, uint2, unsigned>::type>::type v;
+  using Bits = typename std::conditional<sizeof(T) == 2, uint2, unsigned>::type;
+  typename std::conditional<sizeof(T) == 4, float4, Bits>::type v;
   __device__ __forceinline__ void load(const void* p, long long i) {
     v = __ldcs(reinterpret_cast<const decltype(v)*>(static_cast<const T*>(p) + i));
   }
@@ -208,8 +216,8 @@ __device__ __forceinline__ void step8(const Hyper& h, float (&p)[8], const float
 
 // The block's codes and scales. again(e): value e's root code from 64 bits, given the factor.
 template <class F>
-__device__ __forceinline__ void hold8(float (&m)[8], const float (&r)[8], unsigned (&mq)[2], unsigned (&vq)[2], float& ms,
-                                      float& vs, F&& again) {
+__device__ __forceinline__ void hold8(float (&m)[8], const float (&r)[8], unsigned (&mq)[2], unsigned (&vq)[2],
+                                      float& ms, float& vs, F&& again) {
   float top_m = 0.f, top_r = 0.f, mi, ri;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -253,10 +261,12 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
     step_kernel(const __grid_constant__ Tensors ts, int copy_type, const float* hp, const float* factor) {
   using S = typename std::conditional<BITS == 8, uint8_t, float>::type;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int all = ts.first[ts.n];
-  const int warps = gridDim.x * kWarps;
-  int b = blockIdx.x * kWarps + warp;
-  int i = tensor_of(ts, min(b, all - 1));
+  // 8 bits: blocks dealt over a grid that stays; 32 bits: kRun32 blocks to a warp of a CTA that ends with them
+  const int all = ts.first[ts.n], first = blockIdx.x * (BITS == 8 ? kWarps : kWarps * kRun32);
+  const int end = BITS == 8 ? all : min(all, first + kWarps * kRun32);
+  const int stride = BITS == 8 ? (int)gridDim.x * kWarps : kWarps;
+  int b = first + warp;
+  int i = tensor_of(ts, min(b, end - 1));
   griddep_wait();
   Hyper h;
   h.b1 = hp[1]; h.b2 = hp[2]; h.eps = hp[3];
@@ -289,13 +299,13 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
     }
     return whole;
   };
-  if (b >= all) return;
+  if (b >= end) return;
   bool next_whole = fetch(b);
   while (true) {
     const tb2_adamw_tensor& t = ts.t[i];
     const int blk = b - ts.first[i];
     const long long k0 = (long long)blk * kBlock + 4 * lane;
-    const bool whole = next_whole, more = all - b > warps;
+    const bool whole = next_whole, more = end - b > stride;
     float p[8], g[8], m[8], r[8];
     const float ms = raw.ms, vs = raw.vs;
     if (whole) {
@@ -323,8 +333,8 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
       }
     }
     if (more) {
-      i = tensor_from(ts, i, b + warps);   // (t is still block b's)
-      next_whole = fetch(b + warps);
+      i = tensor_from(ts, i, b + stride);   // (t is still block b's)
+      next_whole = fetch(b + stride);
     }
     step8<BITS>(h, p, g, m, r, ms, vs);
     unsigned mq[2], vq[2];
@@ -377,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
       }
     }
     if (!more) return;
-    b += warps;
+    b += stride;
   }
 }
 
@@ -386,11 +396,12 @@ template <bool PUT>
 __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ Tensors ts) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int all = ts.first[ts.n];
-  const int warps = gridDim.x * kWarps;   // (each has kRun blocks in a row: so many reads are on their way at once)
-  long long b = ((long long)blockIdx.x * kWarps + warp) * kRun, end = min(b + kRun, (long long)all);
+  // a warp has kRun blocks in a row: so many reads are on their way at once
+  long long b = ((long long)blockIdx.x * kWarps + warp) * kRun;
+  const long long end = min(b + kRun, (long long)all);
   int i = tensor_of(ts, (int)min(b, all - 1LL));
   griddep_wait();
-  while (b < all) {
+  while (b < end) {
     i = tensor_from(ts, i, (int)b);
     const tb2_adamw_tensor& t = ts.t[i];
     const int blk = (int)(b - ts.first[i]);
@@ -398,10 +409,6 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant
     const bool aligned = ts.whole[i / 32] >> (i % 32) & 1, whole = aligned && (long long)(blk + 1) * kBlock <= t.n;
     const bool run = !PUT && aligned && b + kRun <= end && (long long)(blk + kRun) * kBlock <= t.n;
     b += run ? kRun : 1;
-    if (b >= end) {   // on to the warp's next run
-      b = end + (warps - 1LL) * kRun;
-      end = min(b + kRun, (long long)all);
-    }
     if (run) {
       unsigned mq[2 * kRun], vq[2 * kRun];
       float ms[kRun], vs[kRun];
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant
 }
 
 bool tensor_ok(const tb2_adamw_tensor& t, int p_type, int g_type, int copy_type, int bits) {
-  if (t.n < 0 || t.n > (1LL << 38)) return false;
+  if (t.n < 0 || t.n > kMaxValues) return false;
   if (t.n == 0) return true;
   if (!t.p || !t.g || !t.m || !t.v || (t.copy && !aligned(t.copy, type_bytes(copy_type)))) return false;
   if (!aligned(t.p, type_bytes(p_type)) || !aligned(t.g, type_bytes(g_type))) return false;
@@ -504,10 +511,7 @@ bool tensor_ok(const tb2_adamw_tensor& t, int p_type, int g_type, int copy_type,
   return t.m_scale && t.v_scale && all_aligned(4, {t.m_scale, t.v_scale});
 }
 
-// CTAs that stay; as many as the warps' runs of blocks need where those are few.
-unsigned ctas_of(long long blocks, int run, int per_sm) {
-  return (unsigned)std::min((blocks + kWarps * run - 1) / (kWarps * run), (long long)per_sm * kSMs);
-}
+unsigned ctas_of(long long blocks, int run) { return (unsigned)((blocks + kWarps * run - 1) / (kWarps * run)); }
 
 // The tensors in groups of what a launch takes, empty ones left out. whole(tensor): see Tensors.
 template <class W, class F>
@@ -520,7 +524,7 @@ int in_groups(const tb2_adamw_tensor* t, int n, W&& whole, F&& launch) {
     for (; i < n && g.n < kMaxTensors; ++i) {
       if (t[i].n == 0) continue;
       const long long b = (t[i].n + kBlock - 1) / kBlock;
-      if (blocks + b > 0x7fffffffLL) break;
+      if (blocks + b > 0x3fffffffLL) break;
       if (whole(t[i])) g.whole[g.n / 32] |= 1u << (g.n % 32);
       g.first[g.n] = (int)blocks;
       g.t[g.n++] = t[i];
@@ -566,13 +570,14 @@ int tb2_adamw_multi(const tb2_adamw_multi_args* a, void* stream) {
   auto whole = [&](const tb2_adamw_tensor& t) {
     return aligned(t.p, pb) && aligned(t.g, gb) && aligned(t.copy, cb) && all_aligned(sb, {t.m, t.v});
   };
-  const int per = a->state_bits == 8 ? kCtas8 : kCtas32;
   return in_groups(a->tensors, a->n_tensors, whole, [&](const Tensors& g, long long blocks) {
+    const unsigned ctas =
+        a->state_bits == 8 ? std::min(ctas_of(blocks, 1), (unsigned)(kCtas8 * kSMs)) : ctas_of(blocks, kRun32);
     return by_row_type(a->p_type, [&](auto p) {
       return by_row_type(a->g_type, [&](auto q) {
         using P = decltype(p);
         using G = decltype(q);
-        return launch_pdl(a->state_bits == 8 ? step_kernel<P, G, 8> : step_kernel<P, G, 32>, dim3(ctas_of(blocks, 1, per)), dim3(kThreads),
+        return launch_pdl(a->state_bits == 8 ? step_kernel<P, G, 8> : step_kernel<P, G, 32>, dim3(ctas), dim3(kThreads),
                           0, static_cast<cudaStream_t>(stream), g, a->copy_type, a->hp, a->grad_scale);
       });
     });
@@ -584,7 +589,7 @@ int tb2_adamw_moments(const tb2_adamw_tensor* tensors, int n_tensors, int put, v
   if (n_tensors < 0 || (n_tensors && !tensors)) return -1;
   for (int i = 0; i < n_tensors; ++i) {
     const tb2_adamw_tensor& t = tensors[i];
-    if (t.n < 0 || t.n > (1LL << 38)) return -1;
+    if (t.n < 0 || t.n > kMaxValues) return -1;
     if (t.n && (!t.p || !t.copy || !t.m || !t.v || !t.m_scale || !t.v_scale ||
                 !all_aligned(4, {t.p, t.copy, t.m_scale, t.v_scale})))
       return -1;
@@ -593,8 +598,8 @@ int tb2_adamw_moments(const tb2_adamw_tensor* tensors, int n_tensors, int put, v
     return all_aligned(16, {t.p, t.copy}) && all_aligned(4, {t.m, t.v});
   };
   return in_groups(tensors, n_tensors, whole, [&](const Tensors& g, long long blocks) {
-    return launch_pdl(put ? moments_kernel<true> : moments_kernel<false>, dim3(ctas_of(blocks, kRun, 4)), dim3(kThreads), 0,
-                      static_cast<cudaStream_t>(stream), g);
+    return launch_pdl(put ? moments_kernel<true> : moments_kernel<false>, dim3(ctas_of(blocks, kRun)), dim3(kThreads),
+                      0, static_cast<cudaStream_t>(stream), g);
   });
 }
 
