@@ -71,3 +71,12 @@ def rows(t: torch.Tensor, n: int, d: int, dtype, index: int, what: str) -> int:
             if s0 >= d:
                 return s0
     bad(f"{what}: {dtype} [{n}, {d}] on cuda:{index}, rows contiguous and apart")
+
+
+def no_captured_leaf(*tensors) -> None:
+    """Refuses a leaf's gradient in a CUDA graph: it is added to the leaf on the stream that the leaf was first used on,
+    which a capture of another stream may not wait for."""
+    if any(t is not None and t.requires_grad and t.is_leaf for t in tensors) and \
+            torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("toy_b200: a leaf's gradient is not captured into a CUDA graph (capture the gradient's own "
+                           "call instead)")

@@ -31,8 +31,8 @@ __device__ __forceinline__ int expert_of(const void* ids, int wide, long long i,
   return e >= E || e < 0 ? E : (int)e;
 }
 
-// The lanes with this lane's value of BITS bits. (A ballot a bit; __match_any_sync took longer: sorting 262144 slots 67 us
-// instead of 44.)
+// The lanes with this lane's value of BITS bits. (A ballot a bit; __match_any_sync took longer: sorting 262144 slots 67
+// us instead of 44.)
 template <int BITS>
 __device__ __forceinline__ unsigned same_lanes(int e) {
   unsigned same = 0xffffffffu;
@@ -65,7 +65,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const void* ids, int
   for (int i = tid; i < warps * E; i += threads) count[i] = 0;
   // runs of a multiple of 32 slots
   const long long run = ((long long)n + 32 * C * warps - 1) / (32 * C * warps) * 32;
-  const long long i0 = warp < warps ? min((long long)n, run * (part * warps + warp)) : n, i1 = min((long long)n, i0 + run);
+  const long long i0 = warp < warps ? min((long long)n, run * (part * warps + warp)) : n;
+  const long long i1 = min((long long)n, i0 + run);
   griddep_wait();
   int e[kAhead];
   bool past = false;
@@ -377,9 +378,9 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(RowsArgs a) {
   }
 }
 
-// A warp has K slots of a token (its last ones may be fewer), Q pieces to a lane at a time: the token's gradient is read
-// once for them, and all their pieces are on their way together. (4096 tokens of 8 bf16 rows of 2048: a warp a slot 62
-// us, a warp eight 54, with the gradient's pieces read behind the rows' 54, now 50. A CTA a token, its warps' parts
+// A warp has K slots of a token (its last ones may be fewer), Q pieces to a lane at a time: the token's gradient is
+// read once for them, and all their pieces are on their way together. (4096 tokens of 8 bf16 rows of 2048: a warp a
+// slot 62 us, a warp eight 54, with the gradient's pieces read behind the rows' 54, now 50. A CTA a token, its warps' parts
 // added up through shared memory, 63.)
 template <class T, class V, int K, int Q>
 __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
@@ -464,16 +465,17 @@ int sort_launch(const tb2_expert_sort_args& a, int* err, cudaStream_t st) {
   if (sort_setup<BITS>()) return -3;
   // one CTA for few slots, and no more warps than have 32 slots
   const int ctas = a.n_slots <= kOneCta ? 1 : kSortCtas;
-  const int warps = std::max(1, (int)std::min((long long)kSortWarps, ((long long)a.n_slots + 32 * ctas - 1) / (32 * ctas)));
+  const long long groups = ((long long)a.n_slots + 32 * ctas - 1) / (32 * ctas);
+  const int warps = (int)std::max(1LL, std::min((long long)kSortWarps, groups));
   const int threads = std::max(warps * 32, std::min(kSortThreads, (a.n_experts + 31) / 32 * 32));
   const bool apart = a.order && a.n_slots > kOrderApart;
-  if (launch_pdl_cluster(sort_kernel<BITS>, dim3(ctas), dim3(threads), (size_t)warps * a.n_experts * sizeof(int), st, ctas,
-                         a.ids, (int)(a.id_bytes == 8), a.n_slots, a.n_experts, warps, a.offsets,
+  if (launch_pdl_cluster(sort_kernel<BITS>, dim3(ctas), dim3(threads), (size_t)warps * a.n_experts * sizeof(int), st,
+                         ctas, a.ids, (int)(a.id_bytes == 8), a.n_slots, a.n_experts, warps, a.offsets,
                          apart ? (int*)nullptr : a.order, a.pos, err))
     return -3;
   if (!apart) return 0;
-  return launch_pdl(order_kernel, dim3(std::min((a.n_slots + 255) / 256, 8 * kSMs)), dim3(256), 0, st, (const int*)a.pos,
-                    (const int*)a.offsets + a.n_experts, a.n_slots, a.order);
+  return launch_pdl(order_kernel, dim3((unsigned)std::min((a.n_slots + 255LL) / 256, 8LL * kSMs)), dim3(256), 0, st,
+                    (const int*)a.pos, (const int*)a.offsets + a.n_experts, a.n_slots, a.order);
 }
 
 // f(a value of the row type, a piece): see Chunk.
@@ -504,8 +506,10 @@ unsigned grid_of(long long threads) {
 unsigned narrow_grid(const RowsArgs& k) { return grid_of((long long)k.T * ((k.per + kCols - 1) / kCols) * 32); }
 template <class T, class V>
 int dispatch_by(const RowsArgs& k, cudaStream_t st) {
-  if constexpr (sizeof(V) < 16) return launch_pdl(dispatch_narrow_kernel<T, V>, dim3(narrow_grid(k)), dim3(256), 0, st, k);
-  else return launch_pdl(dispatch_kernel<T, V>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0, st, k);
+  if constexpr (sizeof(V) < 16)
+    return launch_pdl(dispatch_narrow_kernel<T, V>, dim3(narrow_grid(k)), dim3(256), 0, st, k);
+  else
+    return launch_pdl(dispatch_kernel<T, V>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0, st, k);
 }
 template <class T, class V, int K>
 int combine_launch(const RowsArgs& k, cudaStream_t st) {
@@ -526,8 +530,8 @@ template <class V>
 constexpr int kGradCols = sizeof(V) == 16 ? 2 : sizeof(V) == 8 ? 4 : 8;
 template <class T, class V, int K>
 int combine_grad_launch(const RowsArgs& k, cudaStream_t st) {
-  return launch_pdl(combine_grad_kernel<T, V, K, kGradCols<V>>, dim3(grid_of((long long)k.T * ((k.K + K - 1) / K) * 32)),
-                    dim3(256), 0, st, k);
+  const long long warps = (long long)k.T * ((k.K + K - 1) / K);
+  return launch_pdl(combine_grad_kernel<T, V, K, kGradCols<V>>, dim3(grid_of(32 * warps)), dim3(256), 0, st, k);
 }
 template <class T, class V>
 int combine_grad_by(const RowsArgs& k, cudaStream_t st) {

@@ -844,7 +844,8 @@ class KvEngine {
     // floats: stats, log probabilities, entropies, the alternatives'
     float *stats = lp_out_, *lp = stats + 2 * nb_, *ent = lp + nb_, *alt = ent + nb_;
     std::copy(tokens, tokens + nb_, lp_host_);
-    if (cudaMemcpyAsync(lp_ids_, lp_host_, nb_ * sizeof(long long), cudaMemcpyHostToDevice, st_) != cudaSuccess) return -3;
+    if (cudaMemcpyAsync(lp_ids_, lp_host_, nb_ * sizeof(long long), cudaMemcpyHostToDevice, st_) != cudaSuccess)
+      return -3;
     const int V = e_.cfg().vocab;
     const tb2_logprobs_args a = {nb_, V,  kTypeF32, logits_, V, scale, lp_ids_, lp, stats, entropy ? ent : nullptr,
                                  top, lp_ids_ + nb_, alt};

@@ -225,8 +225,8 @@ __device__ void rank_keys(ScoreShared& sh, int n, int top) {
   __syncthreads();
 }
 
-// The `top` largest keys of C lists in falling order (kMaxTop entries each, 0 past the last) in cand: a key's place is the
-// number of larger ones, found in every list by halving.
+// The `top` largest keys of C lists in falling order (kMaxTop entries each, 0 past the last) in cand: a key's place is
+// the number of larger ones, found in every list by halving.
 __device__ void merge_lists(ScoreShared& sh, int C, int top) {
   if (threadIdx.x < kMaxTop) sh.list[threadIdx.x] = 0;
   __syncthreads();
@@ -601,7 +601,7 @@ __device__ __forceinline__ uint4 join_bytes(const uint4& lo, const uint4& hi, in
 // dx = p (A + B log2 p) with A = -a (g + g_H H), g the sum of the words' own gradients, B = -a g_H ln 2; the words with
 // a gradient of their own (the token, the alternatives) are put right at the end. A CTA has a run of the 16-byte pieces
 // of the result's row; a row of logits that starts elsewhere within its 16 bytes is read in aligned pieces and shifted
-// (509 rows of 50303 f16 words: see the table of measurements in the documentation).
+// (509 rows of 50303 f16 words that lie so: 27 us where the bytes take 16).
 template <class T, bool ENT>
 __global__ void __launch_bounds__(NT, 4) score_grad_kernel(GradArgs a) {
   constexpr int N = Piece<T>::kN, kWords = kMaxTop + 1;
@@ -749,9 +749,9 @@ int grad_split(int n, double bytes) {
 }
 
 // CTAs to a row. With 4 CTAs of 256 threads an SM streams 11 B/ns a CTA, and a CTA has some 3 us to spend besides; the
-// split with the shortest ceil(CTAs / 592) (bytes / split / rate + 3 us) is taken. (CTAs of 1024 threads for a few rows,
-// each with its whole share in flight: 4.5 us instead of 3.5 for one row of 49152 f32, and 16 clusters of eight such
-// CTAs do not fit the GPU at once, 18.2 us instead of 9.0 for 16 rows of 128256 with 20 alternatives.)
+// split with the shortest ceil(CTAs / 592) (bytes / split / rate + 3 us) is taken. (CTAs of 1024 threads for a few
+// rows, each with its whole share in flight: 4.5 us instead of 3.5 for one row of 49152 f32, and 16 clusters of eight
+// such CTAs do not fit the GPU at once, 18.2 us instead of 9.0 for 16 rows of 128256 with 20 alternatives.)
 template <class T, bool ENT>
 int score_launch(ScoreArgs& k, cudaStream_t st) {
   const double bytes = (double)k.V * sizeof(T);

@@ -140,8 +140,8 @@ __global__ void moe_route_kernel(const float* __restrict__ logits, int N, int E,
 }
 
 // perm from its inverse pos; the first CTA, a thread an expert, lists the experts' tiles.
-__global__ void __launch_bounds__(256) moe_order_kernel(const int* offsets, const int* pos, long long NK, int E, int* perm,
-                                                        int* tiles, int n_tiles) {
+__global__ void __launch_bounds__(256) moe_order_kernel(const int* offsets, const int* pos, long long NK, int E,
+                                                        int* perm, int* tiles, int n_tiles) {
   griddep_wait();
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < NK; i += gridDim.x * 256LL)
     if (pos[i] >= 0) perm[pos[i]] = (int)i;

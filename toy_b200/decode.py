@@ -111,7 +111,8 @@ class PagedKVDecoder(_Logprobs):
 
     def decode_step(self, tokens: Sequence[int], logits: bool = True) -> Optional[np.ndarray]:
         """tokens[b] appended to sequence b (-1: nothing); logits [n_seq, vocab] of the tokens after them (None with
-        logits=False: they stay on the GPU, for `logprobs`). MemoryError when the pool has too few free pages: the step did nothing, and may be repeated after a release."""
+        logits=False: they stay on the GPU, for `logprobs`). MemoryError when the pool has too few free pages: the step
+        did nothing, and may be repeated after a release."""
         t = np.ascontiguousarray(np.asarray(tokens, np.int64).reshape(self.n_seq))
         rc = lib().tb2_kv_decode_paged(self.eng.sess, t.ctypes.data_as(C.POINTER(C.c_longlong)), self.n_seq,
                                        self._logits.ctypes.data_as(C.POINTER(C.c_float)) if logits else None)

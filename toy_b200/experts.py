@@ -20,7 +20,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import ExpertRowsArgs, ExpertSortArgs
-from ._rows import F32, I32, I64, ROW_TYPE, bad, call, dense, prepare, rows
+from ._rows import F32, I32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows
 
 __all__ = ["Routing", "combine", "combine_grad", "dispatch", "dispatch_grad", "prepare", "sort"]
 MAX_EXPERTS = 1024
@@ -150,6 +150,7 @@ def dispatch(x: torch.Tensor, r: Routing, *, out: Optional[torch.Tensor] = None)
     """The rows of x [tokens, d] at their slots' places, [tokens * used, d]: rows past the last slot's are zero, or as
     they were where `out` is given. Differentiable in x (without out)."""
     if out is None and _wanted(x):
+        no_captured_leaf(x)
         return _Dispatch.apply(x, *r)
     _no_grad(x, out)
     return _dispatch(x, r, out)
@@ -167,6 +168,7 @@ def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None,
     rows of z [rows, d], choices ascending, in f32, rounded once. out may be the residual. Differentiable in z, weights
     and residual (without out)."""
     if out is None and _wanted(z, weights, residual):
+        no_captured_leaf(z, weights, residual)
         return _Combine.apply(z, weights, residual, *r)
     _no_grad(z, weights, residual, out)
     return _combine(z, r, weights, residual, out)

@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import LogprobsArgs, LogprobsGradArgs
-from ._rows import F32, I64, ROW_TYPE, bad, call, dense, prepare, rows
+from ._rows import F32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows
 
 __all__ = ["TokenLogprobs", "prepare", "token_logprobs", "token_logprobs_grad"]
 MAX_TOP = 32
@@ -92,6 +92,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float =
     the `top` (at most 32) most likely words where asked for. Logits are f32, f16 or bf16; -inf is a word of
     probability 0. Differentiable in the logits."""
     if logits.requires_grad and torch.is_grad_enabled():
+        no_captured_leaf(logits)
         return TokenLogprobs(*_Score.apply(logits, tokens, scale, entropy, top))
     return _forward(logits, tokens, scale, entropy, top)
 

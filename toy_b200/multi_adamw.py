@@ -36,6 +36,13 @@ def _pointers(tensors: Sequence[torch.Tensor], shapes: list, dtype, index: int, 
     return list(map(_POINTER, tensors))
 
 
+def _apart(lists: Sequence[Sequence[torch.Tensor]]) -> None:
+    """Refuses tensors that share memory: a step writes all of them."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for x in lists for t in x if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        bad("weights, copies and state do not share memory")
+
+
 class MultiAdamW:
     """The optimizer of `params`: contiguous tensors of one type (f32, f16 or bf16) on one GPU. copies: tensors of their
     shapes, of one 16-bit type, that each step sets to the weights rounded (for weights kept in f32). state: (m, v,
@@ -89,6 +96,7 @@ class MultiAdamW:
             at.append([t.data_ptr() for t in x])
         if bits == 32:
             at += [[0] * len(n)] * 2
+        _apart([x for x in (self.params, self.copies, self.m, self.v, self.m_scale, self.v_scale) if x])
         self._n = len(n)
         self._t = np.zeros(self._n, _COLUMNS)
         for name, x in zip(_COLUMNS.names, (pp, [0] * self._n, *at, cp, n)):
