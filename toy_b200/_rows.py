@@ -10,6 +10,7 @@ from ._lib import check, lib
 ROW_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 F32, I32, I64 = torch.float32, torch.int32, torch.int64
 _prepared: set = set()
+_entries: dict = {}
 
 
 def _raw_stream(index: int) -> int:
@@ -38,9 +39,11 @@ _current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 def call(index: int, what: str, *args) -> None:
     """An entry point on torch's current stream of GPU `index`, which is made current for the call where it is not."""
+    f = _entries.get(what)
+    if f is None:
+        f = _entries[what] = getattr(lib(), what)
     if index not in _prepared:
         prepare(torch.device("cuda", index))
-    f = getattr(lib(), what)
     if _current() == index:
         rc = f(*args, _raw_stream(index))
     else:

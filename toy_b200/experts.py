@@ -14,7 +14,6 @@ the device (`tb2_device_error` in the header).
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
@@ -36,12 +35,12 @@ class Routing(NamedTuple):
 def sort(ids: torch.Tensor, n_experts: int, *, out: Optional[Routing] = None) -> Routing:
     """The slots of ids [tokens, used] (i32 or i64; negative: no expert) sorted by expert, each expert's in slot
     order."""
-    if ids.dim() != 2 or ids.dtype not in (I32, I64) or not ids.is_cuda or not ids.is_contiguous() or \
-            ids.numel() >= 2**31 or ids.shape[1] < 1:
+    dev, n, wide = ids.get_device(), ids.numel(), ids.dtype is I64
+    if dev < 0 or ids.dim() != 2 or not (wide or ids.dtype is I32) or not ids.is_contiguous() or n >= 2**31 or \
+            ids.shape[1] < 1:
         bad("ids: contiguous i32 or i64 [tokens, used] on a GPU, fewer than 2^31")
     if not 1 <= n_experts <= MAX_EXPERTS:
         bad(f"n_experts is 1 to {MAX_EXPERTS}")
-    dev, n = ids.get_device(), ids.numel()
     if out is None:
         out = Routing(ids.new_empty(n_experts + 1, dtype=I32), ids.new_empty(n, dtype=I32),
                       ids.new_empty(ids.shape, dtype=I32))
@@ -49,31 +48,30 @@ def sort(ids: torch.Tensor, n_experts: int, *, out: Optional[Routing] = None) ->
         dense(out.offsets, (n_experts + 1,), I32, dev, "out.offsets")
         dense(out.order, (n,), I32, dev, "out.order")
         dense(out.pos, ids.shape, I32, dev, "out.pos")
-    a = ExpertSortArgs(ids.data_ptr(), 4 if ids.dtype is I32 else 8, n, n_experts, out.offsets.data_ptr(),
-                       out.order.data_ptr(), out.pos.data_ptr())
-    call(dev, "tb2_expert_sort", C.byref(a))
+    a = ExpertSortArgs(ids.data_ptr(), 8 if wide else 4, n, n_experts, out.offsets.data_ptr(), out.order.data_ptr(),
+                       out.pos.data_ptr())
+    call(dev, "tb2_expert_sort", a)
     return out
 
 
 def _args(r: Routing, x: torch.Tensor, xs: torch.Tensor, weights: Optional[torch.Tensor]) -> tuple:
     """(device, arguments) of tokens x [tokens, d] and sorted rows xs [rows, d]."""
-    if r.pos.dim() != 2 or x.dim() != 2 or xs.dim() != 2 or x.dtype not in ROW_TYPE or not x.is_cuda:
+    pos, dtype, dev = r.pos, x.dtype, x.get_device()
+    if pos.dim() != 2 or x.dim() != 2 or xs.dim() != 2 or dtype not in ROW_TYPE or dev < 0:
         bad("rows are f32, f16 or bf16, tokens [tokens, d] and sorted rows [rows, d] on a GPU")
-    (tokens, used), d, n = r.pos.shape, x.shape[1], xs.shape[0]
-    dev = x.get_device()
-    if d < 1 or max(d, n) >= 2**31:
+    shape, d, n = pos.shape, x.shape[1], xs.shape[0]
+    if d < 1 or d >= 2**31 or n >= 2**31:
         bad("rows are of one value or more, and fewer than 2^31 of fewer than 2^31")
-    return dev, ExpertRowsArgs(tokens, used, d, n, ROW_TYPE[x.dtype], x.data_ptr(),
-                               rows(x, tokens, d, x.dtype, dev, "tokens"), xs.data_ptr(),
-                               rows(xs, n, d, x.dtype, dev, "sorted rows"),
-                               dense(r.pos, (tokens, used), I32, dev, "pos"),
-                               None if weights is None else dense(weights, (tokens, used), F32, dev, "weights"))
+    return dev, ExpertRowsArgs(shape[0], shape[1], d, n, ROW_TYPE[dtype], x.data_ptr(),
+                               rows(x, shape[0], d, dtype, dev, "tokens"), xs.data_ptr(),
+                               rows(xs, n, d, dtype, dev, "sorted rows"), dense(pos, shape, I32, dev, "pos"),
+                               None if weights is None else dense(weights, shape, F32, dev, "weights"))
 
 
 def _sorted(r: Routing, dev: int) -> int:
     """The address of the number of sorted slots, the last of the offsets."""
-    n = r.offsets.shape[0] if r.offsets.dim() == 1 else 0
-    return dense(r.offsets, (max(n, 1),), I32, dev, "offsets") + 4 * (n - 1)
+    n = r.offsets.numel()
+    return dense(r.offsets, (n,) if n else None, I32, dev, "offsets") + 4 * (n - 1)
 
 
 def _wanted(*tensors) -> bool:
@@ -96,7 +94,7 @@ def _dispatch(x, r, out):
     dev, a = _args(r, x, out, None)
     if fresh:
         a.n_sorted = _sorted(r, dev)
-    call(dev, "tb2_expert_dispatch", C.byref(a))
+    call(dev, "tb2_expert_dispatch", a)
     return out
 
 
@@ -107,7 +105,7 @@ def _combine(z, r, weights, residual, out):
     if residual is not None:
         a.ldr = rows(residual, a.n_tokens, a.d, z.dtype, dev, "residual")
         a.residual = residual.data_ptr()
-    call(dev, "tb2_expert_combine", C.byref(a))
+    call(dev, "tb2_expert_combine", a)
     return out
 
 
@@ -189,7 +187,7 @@ def _combine_grad(dy, z, r, weights, out, want_z, want_w):
                 out.zero_()
     if want_w:
         a.d_weights = dw.data_ptr()
-    call(dev, "tb2_expert_combine_grad", C.byref(a))
+    call(dev, "tb2_expert_combine_grad", a)
     return out, dw
 
 

@@ -12,7 +12,6 @@ the vocabulary are reported on the device (`tb2_device_error` in the header).
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
@@ -35,18 +34,18 @@ class TokenLogprobs(NamedTuple):
 
 def _logits(x: torch.Tensor, tokens: torch.Tensor, scale: float, top: int) -> tuple:
     """(rows, vocabulary, device, row stride) of checked logits."""
-    if x.dim() != 2 or x.dtype not in ROW_TYPE or not x.is_cuda:
+    dev, dtype = x.get_device(), x.dtype
+    if dev < 0 or x.dim() != 2 or dtype not in ROW_TYPE:
         bad("logits: f32, f16 or bf16 [n, vocab] on a GPU")
     n, vocab = x.shape
-    dev = x.get_device()
-    if vocab < 1 or max(n, vocab) >= 2**31:
+    if vocab < 1 or n >= 2**31 or vocab >= 2**31:
         bad("logits: one word or more, rows and words below 2^31")
-    if not 0 <= top <= min(MAX_TOP, vocab):
+    if not 0 <= top <= MAX_TOP or top > vocab:
         bad(f"top is 0 to {MAX_TOP}, and no more than the vocabulary")
     if not 2.0**-126 <= scale <= 2.0**126:
         bad("scale is positive, and neither it nor its inverse past f32's range")
     dense(tokens, (n,), I64, dev, "tokens")
-    return n, vocab, dev, rows(x, n, vocab, x.dtype, dev, "logits")
+    return n, vocab, dev, rows(x, n, vocab, dtype, dev, "logits")
 
 
 def _forward(x, tokens, scale, entropy, top) -> TokenLogprobs:
@@ -60,7 +59,7 @@ def _forward(x, tokens, scale, entropy, top) -> TokenLogprobs:
         a = LogprobsArgs(n, vocab, ROW_TYPE[x.dtype], x.data_ptr(), ld, scale, tokens.data_ptr(), lp.data_ptr(),
                          stats.data_ptr(), ent.data_ptr() if entropy else None, top, ids.data_ptr() if top else None,
                          top_lp.data_ptr() if top else None)
-        call(dev, "tb2_logprobs", C.byref(a))
+        call(dev, "tb2_logprobs", a)
     return TokenLogprobs(lp, ent, ids, top_lp, stats)
 
 
@@ -121,5 +120,5 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, result: Toke
         a = LogprobsGradArgs(n, vocab, ROW_TYPE[logits.dtype], logits.data_ptr(), ld, scale, tokens.data_ptr(),
                              dense(result.stats, (n, 2), F32, dev, "result.stats"), ent, g[0], g[1], top,
                              g[2] if top else None, ids, out.data_ptr(), ldd)
-        call(dev, "tb2_logprobs_grad", C.byref(a))
+        call(dev, "tb2_logprobs_grad", a)
     return out
