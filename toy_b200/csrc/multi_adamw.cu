@@ -28,7 +28,7 @@ constexpr int kBlock = 256;        // values that share a scale
 constexpr long long kMaxValues = 1LL << 37;   // of a tensor (its blocks, and a launch's, are counted in 30 bits)
 constexpr int kMaxTensors = 448;   // tensors a launch: their descriptors travel as its arguments (30.5 of 32 KB)
 constexpr int kThreads = 256, kWarps = kThreads / 32, kRun = 4;
-constexpr int kRun32 = 2;
+constexpr int kStepRun = 2;
 constexpr int kCtas8 = 3, kCtas32 = 3;   // CTAs an SM: 80 registers a thread
 
 struct Tensors {
@@ -146,8 +146,9 @@ __device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) {
 
 // A warp has a block at a time. Where CTAs end after a few blocks the GPU works in few pages at any time, which is what
 // HBM likes best (135M weights: f32 moments 561 us, with a grid that stays and deals the blocks out 586, with a run of
-// blocks to each CTA 617; the values of 8-bit moments 210, 240 and 267). The 8-bit step has more to compute, and with
-// CTAs that start anew with the factors it takes 475 us instead of 442.
+// blocks to each CTA 617; the values of 8-bit moments 210, 240 and 267). The 8-bit step has more to compute, and CTAs
+// that start anew with the factors take 475 us: its grid stays, and each CTA has two blocks a warp in a row (429 us;
+// one 447, four 443, a run of all its blocks 489).
 //
 // 8-bit moments are the exact values rounded once, although the step is f32. m is a sum of two terms of either sign,
 // and with few bits in its old value it falls on a border again and again (0.9 of 120 is 108, between 104 and 112: 0.8
@@ -261,11 +262,11 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
     step_kernel(const __grid_constant__ Tensors ts, int copy_type, const float* hp, const float* factor) {
   using S = typename std::conditional<BITS == 8, uint8_t, float>::type;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  // 8 bits: blocks dealt over a grid that stays; 32 bits: kRun32 blocks to a warp of a CTA that ends with them
-  const int all = ts.first[ts.n], first = blockIdx.x * (BITS == 8 ? kWarps : kWarps * kRun32);
-  const int end = BITS == 8 ? all : min(all, first + kWarps * kRun32);
-  const int stride = BITS == 8 ? (int)gridDim.x * kWarps : kWarps;
-  int b = first + warp;
+  // kStepRun blocks to a warp; then a 32-bit CTA ends, and an 8-bit one goes on behind all the grid's
+  constexpr int kCta = kWarps * kStepRun;
+  const int all = ts.first[ts.n], first = blockIdx.x * kCta;
+  const int end = BITS == 8 ? all : min(all, first + kCta);
+  int b = first + warp, left = kStepRun - 1;
   int i = tensor_of(ts, min(b, end - 1));
   griddep_wait();
   Hyper h;
@@ -305,6 +306,11 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
     const tb2_adamw_tensor& t = ts.t[i];
     const int blk = b - ts.first[i];
     const long long k0 = (long long)blk * kBlock + 4 * lane;
+    int stride = kWarps;
+    if (BITS == 8 && left-- == 0) {
+      stride += ((int)gridDim.x - 1) * kCta;
+      left = kStepRun - 1;
+    }
     const bool whole = next_whole, more = end - b > stride;
     float p[8], g[8], m[8], r[8];
     const float ms = raw.ms, vs = raw.vs;
@@ -571,8 +577,7 @@ int tb2_adamw_multi(const tb2_adamw_multi_args* a, void* stream) {
     return aligned(t.p, pb) && aligned(t.g, gb) && aligned(t.copy, cb) && all_aligned(sb, {t.m, t.v});
   };
   return in_groups(a->tensors, a->n_tensors, whole, [&](const Tensors& g, long long blocks) {
-    const unsigned ctas =
-        a->state_bits == 8 ? std::min(ctas_of(blocks, 1), (unsigned)(kCtas8 * kSMs)) : ctas_of(blocks, kRun32);
+    const unsigned most = a->state_bits == 8 ? kCtas8 * kSMs : ~0u, ctas = std::min(ctas_of(blocks, kStepRun), most);
     return by_row_type(a->p_type, [&](auto p) {
       return by_row_type(a->g_type, [&](auto q) {
         using P = decltype(p);
