@@ -398,7 +398,8 @@ int tb2_rows_prepare(void);
  * {0, -inf}, log probabilities -inf, entropy 0. A NaN or +inf in a row makes
  * its probabilities and entropy NaN; NaN counts as the largest logit. A token
  * of vocab or more gives NaN and tb2_device_error() reports 0x5101. scale is
- * finite and positive. tokens, stats and top_ids are on 8-byte boundaries. */
+ * between 2^-126 and 2^126. tokens, stats and top_ids are on 8-byte
+ * boundaries. */
 typedef struct tb2_logprobs_args {
   int n_rows, vocab, row_type;
   const void *logits;
@@ -465,7 +466,8 @@ int tb2_expert_sort(const tb2_expert_sort_args *args, void *stream);
  *   dispatch:     xs[pos[t][k]] = x[t].
  *   combine:      x[t] = residual[t] + sum_k weights[t][k] xs[pos[t][k]], k
  *                 ascending (residual NULL: 0; weights NULL: 1, which is the
- *                 gradient of dispatch). x may be the residual itself.
+ *                 gradient of dispatch). x may be the residual itself, with the
+ *                 same stride.
  *   combine_grad: x is the gradient of combine's result:
  *                 d_xs[pos[t][k]] = weights[t][k] x[t],
  *                 d_weights[t][k] = <x[t], xs[pos[t][k]]> (0 for pos -1);

@@ -349,6 +349,20 @@ def test_autograd(cuda):
         assert not L.token_logprobs(b, t).logprob.requires_grad
 
 
+def test_written_tensors_are_noted(cuda):
+    """What autograd saved of logits that a gradient was written over is refused, not used."""
+    import torch
+    from toy_b200 import logprobs as L
+    x, t = make(4, 100, torch.float32)
+    a = x.clone().requires_grad_()
+    z = a * 2.0
+    r = L.token_logprobs(z, t)
+    with torch.no_grad():
+        L.token_logprobs_grad(z, t, r, torch.ones(4, device="cuda"), out=z)
+    with pytest.raises(RuntimeError):
+        r.logprob.sum().backward()
+
+
 def test_streams_and_graphs(cuda):
     import torch
     from toy_b200 import logprobs as L

@@ -85,6 +85,27 @@ def test_greedy_continuations(cuda, paged):
     d.close()
 
 
+def test_scoring_between_the_steps_of_a_qlora(cuda):
+    """The steps around it give the bits they give without (the forward's work on the second stream included)."""
+    from toy_b200 import LlamaConfig, LoRA, LoraOptions, RecipeOptions
+
+    def run(score):
+        rec = LoRA()
+        rec.realize(LlamaConfig(512, 128, 4, 2, 32, 256, 3, 1e4, 1e-5), 8, RecipeOptions(t_seq=64, t_batch=2, seed=2),
+                    LoraOptions(rank=8, targets=("q", "v")))
+        eng, out = rec.lora_cache, []
+        for step in range(1, 5):
+            ids = O.token_ids(step, 128, 512)
+            args = (ids, O.positions(64, 2), O.next_token_labels(ids, 64, 2, 512))
+            if score:
+                eng.score(O.token_ids(90 + step, 128, 512), args[1], np.full(128, step))
+            out.append(rec.step(*args, O.hp_lora(1e-3, step), step == 1))
+        return out, eng.param("blk.2.attn_q.lora_b")
+
+    (a, pa), (b, pb) = run(False), run(True)
+    assert a == b and np.array_equal(pa, pb)
+
+
 def test_training_engine(cuda):
     """A batch's log probabilities: of the labels, the mean of which is the loss; of others, from the same logits."""
     from toy_b200._lib import lib

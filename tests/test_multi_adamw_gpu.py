@@ -224,6 +224,17 @@ def test_streams_and_graphs(cuda):
         assert torch.equal(x, y)
 
 
+def test_written_weights_are_noted(cuda):
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    w = torch.ones(300, device="cuda", requires_grad=True)
+    opt = MultiAdamW([w])
+    y = (w * w).sum()
+    opt.step([torch.ones(300, device="cuda")], hp_row())
+    with pytest.raises(RuntimeError):
+        y.backward()
+
+
 def test_refusals(cuda):
     import torch
     from toy_b200.multi_adamw import MultiAdamW
@@ -237,7 +248,8 @@ def test_refusals(cuda):
     for bad in (lambda: MultiAdamW([]), lambda: MultiAdamW([p[0].cpu()]), lambda: MultiAdamW(p, bits=16),
                 lambda: MultiAdamW([p[0], p[1].half()]), lambda: MultiAdamW([p[0].t()]),
                 lambda: MultiAdamW(p, copies=[p[0].half()]), lambda: MultiAdamW(p, copies=p),
-                lambda: MultiAdamW(p, copies=[p[0].half(), p[0].half()]),
+                lambda: MultiAdamW(p, copies=[p[0].half(), p[0].half()]), lambda: MultiAdamW([p[0], p[0]]),
+                lambda: MultiAdamW([p[1][:200], p[1][100:]]), lambda: MultiAdamW(p, state=(z8, z8, sc, sc)),
                 lambda: MultiAdamW(p, state=(z8, z8, None, None)),
                 lambda: MultiAdamW(p, state=(z8, z8, sc, sc[:1])), lambda: MultiAdamW(p, state=(z8, z8, sc, sc[::-1])),
                 lambda: MultiAdamW(p, bits=32, state=(z8, z8, None, None)),

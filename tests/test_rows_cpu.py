@@ -31,7 +31,8 @@ def test_logprobs_arguments():
               g_entropy=P, top=2, g_top=P, top_ids=P, d_logits=P, ldd=10)
     for k, v in (("vocab", 0), ("row_type", 1 << 20), ("logits", P + 1), ("ld", 9), ("ldd", 9), ("d_logits", None),
                  ("d_logits", P + 1), ("scale", 0.0), ("tokens", None), ("stats", None), ("entropy", None), ("top", 33),
-                 ("g_top", None), ("top_ids", None), ("g_logprob", P + 2), ("g_entropy", P + 1)):
+                 ("g_top", None), ("top_ids", None), ("g_logprob", P + 2), ("g_entropy", P + 1), ("scale", 1e-39),
+                 ("scale", 1e38), ("ldd", 11)):      # (the logits' own memory, with another stride)
         assert lib().tb2_logprobs_grad(C.byref(LogprobsGradArgs(**{**ok, k: v})), None) == -1, (k, v)
     assert lib().tb2_logprobs_grad(None, None) == -1
 
@@ -51,7 +52,8 @@ def test_expert_arguments():
                         ("xs", None, every), ("ldxs", 15, every), ("pos", None, every), ("pos", P + 2, every),
                         ("weights", P + 2, every[1:]), ("residual", P + 2, every[1:2]), ("ldr", 15, every[1:2]),
                         ("ldd", 15, every[2:]), ("d_xs", P + 1, every[2:]), ("d_weights", P + 1, every[2:]),
-                        ("n_sorted", P + 1, (every[0], every[2])), ("n_used", 1 << 30, every)):
+                        ("n_sorted", P + 1, (every[0], every[2])), ("n_used", 1 << 30, every),
+                        ("ldr", 17, every[1:2]), ("ldd", 17, every[2:])):      # (the same memory, another stride)
         for f in calls:
             assert getattr(lib(), f)(C.byref(ExpertRowsArgs(**{**ok, k: v})), None) == -1, (k, v, f)
     for f in every:

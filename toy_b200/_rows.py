@@ -76,6 +76,11 @@ def rows(t: torch.Tensor, n: int, d: int, dtype, index: int, what: str) -> int:
     bad(f"{what}: {dtype} [{n}, {d}] on cuda:{index}, rows contiguous and apart")
 
 
+def written(*tensors) -> None:
+    """Notes for autograd that the tensors' values have changed (what it saved of them is stale)."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def no_captured_leaf(*tensors) -> None:
     """Refuses a leaf's gradient in a CUDA graph: it is added to the leaf on the stream that the leaf was first used on,
     which a capture of another stream may not wait for."""

@@ -612,6 +612,7 @@ int tb2_expert_combine(const tb2_expert_rows_args* a, void* stream) {
   if (a->n_tokens == 0) return 0;
   if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !row_ok(a->xs, a->ldxs, a->d, a->row_type)) return -1;
   if (a->residual && !row_ok(a->residual, a->ldr, a->d, a->row_type)) return -1;
+  if (a->residual == a->x && a->ldr != a->ldx && a->n_tokens > 1) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->weights})) return -1;
   RowsArgs k = {};
   k.z = a->xs; k.ldz = a->ldxs; k.y = a->x; k.ldy = a->ldx; k.res = a->residual; k.ldr = a->ldr; k.pos = a->pos;
@@ -629,6 +630,7 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args* a, void* stream) {
   if (a->n_tokens == 0) return 0;
   if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !row_ok(a->xs, a->ldxs, a->d, a->row_type)) return -1;
   if (a->d_xs && !row_ok(a->d_xs, a->ldd, a->d, a->row_type)) return -1;
+  if (a->d_xs == a->xs && a->ldd != a->ldxs && a->n_rows > 1) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->weights, a->d_weights, a->n_sorted})) return -1;
   RowsArgs k = {};
   k.x = a->x; k.ldx = a->ldx; k.z = a->xs; k.ldz = a->ldxs; k.dz = a->d_xs; k.lddz = a->ldd; k.pos = a->pos;

@@ -23,7 +23,6 @@
 
 #include <algorithm>
 #include <cfloat>
-#include <cmath>
 
 #include "rows.cuh"
 #include "runtime.cuh"
@@ -731,6 +730,8 @@ __global__ void __launch_bounds__(NT, 4) score_grad_kernel(GradArgs a) {
   }
 }
 
+// (the factor of a difference in powers of two, and its inverse, are f32 numbers)
+bool scale_ok(float s) { return s >= 0x1p-126f && s <= 0x1p126f; }
 bool rows_ok(long long ld, int V, const void* p, int type) {
   return p && ld >= V && aligned(p, type_bytes(type));
 }
@@ -790,7 +791,7 @@ int tb2_logprobs(const tb2_logprobs_args* a, void* stream) {
   using namespace tb2;
   if (!a || a->n_rows < 0 || a->vocab < 1 || !row_type_ok(a->row_type)) return -1;
   if (a->n_rows == 0) return 0;
-  if (!rows_ok(a->ld, a->vocab, a->logits, a->row_type) || !(a->scale > 0.f) || !std::isfinite(a->scale)) return -1;
+  if (!rows_ok(a->ld, a->vocab, a->logits, a->row_type) || !scale_ok(a->scale)) return -1;
   if (!a->tokens || !a->logprob || !a->stats || a->top < 0 || a->top > kMaxTop || a->top > a->vocab) return -1;
   if (a->top && (!a->top_ids || !a->top_logprobs)) return -1;
   if (!all_aligned(8, {a->tokens, a->stats, a->top_ids}) || !all_aligned(4, {a->logprob, a->entropy, a->top_logprobs}))
@@ -810,8 +811,9 @@ int tb2_logprobs_grad(const tb2_logprobs_grad_args* a, void* stream) {
   using namespace tb2;
   if (!a || a->n_rows < 0 || a->vocab < 1 || !row_type_ok(a->row_type)) return -1;
   if (a->n_rows == 0) return 0;
-  if (!rows_ok(a->ld, a->vocab, a->logits, a->row_type) || !(a->scale > 0.f) || !std::isfinite(a->scale)) return -1;
+  if (!rows_ok(a->ld, a->vocab, a->logits, a->row_type) || !scale_ok(a->scale)) return -1;
   if (!rows_ok(a->ldd, a->vocab, a->d_logits, a->row_type)) return -1;
+  if (a->d_logits == a->logits && a->ldd != a->ld && a->n_rows > 1) return -1;
   if (!a->tokens || !a->stats || a->top < 0 || a->top > kMaxTop || a->top > a->vocab) return -1;
   if (a->top && (!a->top_ids || !a->g_top)) return -1;
   if (a->g_entropy && !a->entropy) return -1;

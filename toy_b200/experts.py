@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import ExpertRowsArgs, ExpertSortArgs
-from ._rows import F32, I32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows
+from ._rows import F32, I32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows, written
 
 __all__ = ["Routing", "combine", "combine_grad", "dispatch", "dispatch_grad", "prepare", "sort"]
 MAX_EXPERTS = 1024
@@ -151,12 +151,16 @@ def dispatch(x: torch.Tensor, r: Routing, *, out: Optional[torch.Tensor] = None)
         no_captured_leaf(x)
         return _Dispatch.apply(x, *r)
     _no_grad(x, out)
+    if out is not None:
+        written(out)
     return _dispatch(x, r, out)
 
 
 def dispatch_grad(dxs: torch.Tensor, r: Routing, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient of `dispatch`: each token's sum of its slots' rows of dxs, choices ascending."""
     _no_grad(dxs, out)
+    if out is not None:
+        written(out)
     return _combine(dxs, r, None, None, out)
 
 
@@ -169,6 +173,8 @@ def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None,
         no_captured_leaf(z, weights, residual)
         return _Combine.apply(z, weights, residual, *r)
     _no_grad(z, weights, residual, out)
+    if out is not None:
+        written(out)
     return _combine(z, r, weights, residual, out)
 
 
@@ -196,4 +202,6 @@ def combine_grad(dy: torch.Tensor, z: torch.Tensor, r: Routing, weights: Optiona
     """(dz, dw) of `combine`: the slots' rows of dz are weights * dy, dw = <dy, z> (0 for slots of no expert). Rows of
     dz that no slot has are zero, or as they were where `out` is given; out may be z."""
     _no_grad(dy, z, weights, out)
+    if out is not None:
+        written(out)
     return _combine_grad(dy, z, r, weights, out, True, True)

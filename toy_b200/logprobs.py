@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import LogprobsArgs, LogprobsGradArgs
-from ._rows import F32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows
+from ._rows import F32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows, written
 
 __all__ = ["TokenLogprobs", "prepare", "token_logprobs", "token_logprobs_grad"]
 MAX_TOP = 32
@@ -115,6 +115,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, result: Toke
     ids = dense(result.top_ids, (n, top), I64, dev, "result.top_ids") if top else None
     if out is None:
         out = torch.empty((n, vocab), device=logits.device, dtype=logits.dtype)
+    else:
+        written(out)
     ldd = rows(out, n, vocab, logits.dtype, dev, "out")
     if n:
         a = LogprobsGradArgs(n, vocab, ROW_TYPE[logits.dtype], logits.data_ptr(), ld, scale, tokens.data_ptr(),

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from ._lib import AdamwMultiArgs, AdamwTensor
-from ._rows import F32, ROW_TYPE, bad, call, dense, prepare
+from ._rows import F32, ROW_TYPE, bad, call, dense, prepare, written
 
 __all__ = ["MultiAdamW", "prepare"]
 BLOCK = 256
@@ -97,6 +97,7 @@ class MultiAdamW:
         if bits == 32:
             at += [[0] * len(n)] * 2
         _apart([x for x in (self.params, self.copies, self.m, self.v, self.m_scale, self.v_scale) if x])
+        self._saved = any(p.requires_grad for p in self.params)   # (autograd may have saved their values)
         self._n = len(n)
         self._t = np.zeros(self._n, _COLUMNS)
         for name, x in zip(_COLUMNS.names, (pp, [0] * self._n, *at, cp, n)):
@@ -130,7 +131,9 @@ class MultiAdamW:
         t["g"] = _pointers(grads, shapes, dtype, self.index, "grads")
         a = AdamwMultiArgs(t.ctypes.data, len(t), ROW_TYPE[self.dtype], ROW_TYPE[dtype], ROW_TYPE[self.copy_dtype],
                            self.bits, hp_at, scale_at)
-        call(self.index, "tb2_adamw_multi", C.byref(a))
+        call(self.index, "tb2_adamw_multi", a)
+        if self._saved:
+            written(*self.params)
 
     def _values(self, ms, vs, put: int) -> None:
         if len(ms) != self._n or len(vs) != self._n:
