@@ -144,7 +144,7 @@ struct ScoreShared {
   float tau;
   int n_shares, n_cand, n_ties, n_found;
   unsigned short shares[kUnroll * NT];
-  u64 cand[kCand + kTies], ties[kTies];
+  u64 cand[kCand + kMaxTop + 16], ties[kTies];   // (16: the values outside the pieces)
   // what the cluster's first CTA reads
   float m, s, u;
   u64 list[kMaxTop];
@@ -207,16 +207,16 @@ __device__ void scan_equal(ScoreShared& sh, const RowShape<T>& row, int p0, int 
   __syncthreads();
 }
 
-// cand[0 .. n) by rank: the `top` largest to list (0 past them).
-__device__ void rank_keys(ScoreShared& sh, int n, int top) {
-  if (threadIdx.x < kMaxTop) sh.list[threadIdx.x] = 0;
-  __syncthreads();
-  const int lane = threadIdx.x % 32;
-  for (int i = threadIdx.x / 32 * 8; i < n; i += NT / 32 * 8) {   // four lanes to a key
-    const u64 k = i + lane / 4 < n ? sh.cand[i + lane / 4] : 0;
+// cand[0 .. n) and ties[0 .. more) by rank: the `top` largest to list, which holds zeros.
+__device__ void rank_keys(ScoreShared& sh, int n, int more, int top) {
+  const int lane = threadIdx.x % 32, all = n + more;
+  for (int i = threadIdx.x / 32 * 8; i < all; i += NT / 32 * 8) {   // four lanes to a key
+    const int me = i + lane / 4;
+    const u64 k = me < n ? sh.cand[me] : me < all ? sh.ties[me - n] : 0;
     int r = 0;
 #pragma unroll 4
     for (int j = lane % 4; j < n; j += 4) r += sh.cand[j] > k;
+    for (int j = lane % 4; j < more; j += 4) r += sh.ties[j] > k;
     r += __shfl_xor_sync(0xffffffffu, r, 1);
     r += __shfl_xor_sync(0xffffffffu, r, 2);
     if (lane % 4 == 0 && r < top && k) sh.list[r] = k;
@@ -296,17 +296,21 @@ __device__ void find_top(ScoreShared& sh, const RowShape<T>& row, int p0, int p1
   for (int o = kLanes / 2; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
   if (tid % kLanes == 0) sh.group[tid / kLanes] = g;
   if (tid == 0) sh.n_shares = sh.n_cand = sh.n_ties = 0;
+  if (tid < kMaxTop) sh.list[tid] = 0;
   __syncthreads();
-  if (tid < kGroups) {
-    const float v = sh.group[tid];
+  {   // the group whose maximum is the top-th: every lane of a group compares it with a part of the others
+    constexpr int kPart = kGroups / kLanes;
+    const int me = tid / kLanes, from = tid % kLanes * kPart;
     int r = 0;
-#pragma unroll 16
-    for (int j = 0; j < kGroups; j += 4) {
+#pragma unroll
+    for (int j = from; j < from + kPart; j += 4) {
       const float4 q = *reinterpret_cast<const float4*>(&sh.group[j]);
-      r += (q.x > v || (q.x == v && j < tid)) + (q.y > v || (q.y == v && j + 1 < tid)) +
-           (q.z > v || (q.z == v && j + 2 < tid)) + (q.w > v || (q.w == v && j + 3 < tid));
+      r += (q.x > g || (q.x == g && j < me)) + (q.y > g || (q.y == g && j + 1 < me)) +
+           (q.z > g || (q.z == g && j + 2 < me)) + (q.w > g || (q.w == g && j + 3 < me));
     }
-    if (r == top - 1) sh.tau = v;
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+    if (r == top - 1) sh.tau = g;
   }
   __syncthreads();
   const float tau = sh.tau;
@@ -343,21 +347,20 @@ __device__ void find_top(ScoreShared& sh, const RowShape<T>& row, int p0, int p1
     top_by_rounds(sh, row, p0, p1, edges, top);
     return;
   }
-  int more = 0;
-  if (n < top && ties <= kTies) {
-    more = ties;
-    for (int i = tid; i < ties; i += NT) sh.cand[n + i] = sh.ties[i];
-  } else if (n < top) {
+  if (n >= top) {
+    rank_keys(sh, n, 0, top);
+  } else if (ties <= kTies) {
+    rank_keys(sh, n, ties, top);
+  } else {
     scan_equal<T>(sh, row, p0, p1, tau, top - n, n);
-    more = sh.n_found;
+    const int more = sh.n_found;
     if (tid < edges) {
       const float x = to_f32(row.x[row.edge(tid)]);
       sh.cand[n + more + tid] = x == tau ? top_key(x, row.edge(tid)) : 0;
     }
-    more += edges;
+    __syncthreads();
+    rank_keys(sh, n + more + edges, 0, top);
   }
-  __syncthreads();
-  rank_keys(sh, n + more, top);
 }
 
 // One row by `split` CTAs of a cluster (each a run of its pieces; the first has the values outside the pieces too).
@@ -749,18 +752,19 @@ int grad_split(int n, double bytes) {
   return split;
 }
 
-// CTAs to a row. With 4 CTAs of 256 threads an SM streams 11 B/ns a CTA, and a CTA has some 3 us to spend besides; the
-// split with the shortest ceil(CTAs / 592) (bytes / split / rate + 3 us) is taken. (CTAs of 1024 threads for a few
-// rows, each with its whole share in flight: 4.5 us instead of 3.5 for one row of 49152 f32, and 16 clusters of eight
-// such CTAs do not fit the GPU at once, 18.2 us instead of 9.0 for 16 rows of 128256 with 20 alternatives.)
+// CTAs to a row: the split with the shortest time by what was measured. An SM with k of the grid's CTAs reads 44 B/ns, one
+// CTA 22 (f32) or 14 (16 bits: instructions), and each round of four CTAs adds 2 us (a cluster 4) and with alternatives
+// 3 us more (4). (CTAs of 1024 threads for a few rows, each with its whole share in flight: 4.5 us instead of 3.5 for one
+// row of 49152 f32, and 16 clusters of eight such CTAs do not fit the GPU at once, 18.2 us instead of 9.0 for 16 rows of
+// 128256 with 20 alternatives.)
 template <class T, bool ENT>
 int score_launch(ScoreArgs& k, cudaStream_t st) {
   const double bytes = (double)k.V * sizeof(T);
   double best = 1e300;
-  for (int c = 1; c <= 8; c *= 2) {
-    if ((long long)k.n * c > 0x7fffffffLL) break;
-    const long long waves = ((long long)k.n * c + 4 * kSMs - 1) / (4 * kSMs);
-    const double us = waves * (bytes / c / 11e3 + 3.0);
+  for (int c = 1; c <= 8 && (long long)k.n * c <= 0x7fffffffLL; c *= 2) {
+    const long long per = ((long long)k.n * c + kSMs - 1) / kSMs;   // of an SM
+    const double read = std::max(per * bytes / c / 44e3, bytes / c / (sizeof(T) == 4 ? 22e3 : 14e3));
+    const double us = read + (per + 3) / 4 * ((c == 1 ? 2.0 : 4.0) + (!k.top ? 0.0 : c == 1 ? 3.0 : 4.0));
     if (us < best) best = us, k.split = c;
   }
   return k.split == 1 ? launch_pdl(score_kernel<T, ENT>, dim3(k.n), dim3(256), 0, st, k)
