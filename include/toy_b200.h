@@ -503,7 +503,10 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args *args, void *stream);
  * f32. state_bits 8: blocks of 256 consecutive values share an f32 scale
  * (m_scale, v_scale: [ceil(n / 256)]), the smallest power of two of 2^-100 or
  * more that brings the block within 448; m holds e4m3 codes of m / scale and v
- * of sqrt(v) / scale, the step's exact values rounded once to nearest (even),
+ * of sqrt(v) / scale, the step's exact values rounded once to nearest (even)
+ * or, with a seed (device memory; NULL: nearest), to the code above or below
+ * with the probability of their place between the two, by bits that are a
+ * function of *seed and the value's place alone (give each step another seed),
  * a positive sqrt(v) never below the smallest code, a v below 2^-126 as 0. All
  * zeros (scales too) is
  * an empty state. A block with a value that is not finite is NaN from then on.
@@ -522,6 +525,7 @@ typedef struct tb2_adamw_multi_args {
   int n_tensors;
   int p_type, g_type, copy_type, state_bits;
   const float *hp, *grad_scale;
+  const long long *seed;
 } tb2_adamw_multi_args;
 int tb2_adamw_multi(const tb2_adamw_multi_args *args, void *stream);
 /* The values that 8-bit moments stand for: p = m and copy = v, f32 (g is not

@@ -152,6 +152,73 @@ def test_many_values(cuda):
             assert torch.equal(got.double(), want * want if floor else want)
 
 
+def test_rounding_at_random(cuda):
+    """Each held value is a code next to the exact one, the upper one as often as its place between them says; the same
+    seed gives the same bits, another seed others; nothing else of the step changes."""
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n = 1 << 20
+    gr = torch.randn(n, device="cuda", generator=g)
+    # one value of 448 in each block, so that codes are of the values themselves
+    gr.view(-1, 256)[:, 0] = 1.0
+    size = torch.exp2(-18 * torch.rand(n, device="cuda", generator=g))
+    start = torch.rand(n, device="cuda", generator=g) * 400 * size
+    start.view(-1, 256)[:, 0] = 448.0
+    hp = torch.tensor([1e-3, 0.5, 0.5, 1e-8, 0.0, 1.0, 1.0], device="cuda")
+
+    def run(seed):
+        p = [torch.zeros(n, device="cuda")]
+        opt = MultiAdamW(p)
+        opt.set_moments([start], [start * start])
+        held_m, held_v = (x[0].double() for x in opt.moments())
+        opt.step([gr], hp, seed=seed)
+        return p[0], opt.moments()[0][0].double(), opt.moments()[1][0].double().sqrt(), held_m, held_v
+    p, m, r, m0, v0 = run(5)
+    assert all(torch.equal(a, b) for a, b in zip((p, m, r), run(torch.tensor([5], device="cuda"))))
+    other = run(6)
+    assert torch.equal(p, other[0]) and not torch.equal(m, other[1]) and not torch.equal(r, other[2])
+    exact_m = 0.5 * m0 + 0.5 * gr.double()
+    exact_r = (0.5 * v0 + 0.5 * gr.double() ** 2).sqrt()
+    for got, want in ((m, exact_m), (r, exact_r)):
+        top = want.abs().view(-1, 256).amax(-1, keepdim=True)
+        f, e = torch.frexp(top / 448)
+        scale = torch.ldexp(torch.ones_like(f), torch.where(f == 0.5, e - 1, e))
+        t, q = want.view(-1, 256) / scale, got.view(-1, 256) / scale
+        step = torch.ldexp(torch.ones_like(t), torch.frexp(t.abs().clamp(min=2.0 ** -6)).exponent - 4)
+        assert ((q - t).abs() <= step * (1 + 1e-5)).all()      # (f32: off by some 2^-22 of the value)
+        ok = t.abs() > 2.0 ** -9 if got is r else torch.ones_like(t, dtype=torch.bool)   # (a root keeps the first code)
+        off = ((q - t) / step)[ok]
+        # places are uniform or not, the mean of the errors is 0 with a deviation of at most half a step each
+        assert off.mean().abs() <= 5 * 0.5 / off.numel() ** 0.5 + 2.0 ** -16
+        place = ((t / step) - torch.floor(t / step))[ok]
+        up = (off > 0).double()
+        for lo in (0.1, 0.4, 0.8):                              # of those a tenth above a code, four tenths, ...
+            at = (place > lo) & (place < lo + 0.02)
+            rate = up[at].mean()
+            assert (rate - (lo + 0.01)).abs() <= 5 * 0.5 / at.sum().item() ** 0.5 + 0.01
+
+
+def test_moments_follow_at_random(cuda):
+    """300 steps of the same gradients, beta2 = 0.999: v comes to 1 - 0.999^300 of their squares on average. (Rounded to
+    nearest it stops after a dozen steps.)"""
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    n = 1 << 16
+    g = [torch.ones(n, device="cuda").view(256, 256) * (1 + torch.arange(256, device="cuda") / 256.0)]
+    got = {}
+    for seeded in (False, True):
+        opt = MultiAdamW([torch.zeros((256, 256), device="cuda")])
+        for k in range(300):
+            opt.step(g, [0.0, 0.9, 0.999, 1e-8, 0.0, 1.0, 1.0], seed=k if seeded else None)
+        m, v = (x[0] for x in opt.moments())
+        got[seeded] = (v / g[0] ** 2).mean().item() / (1 - 0.999 ** 300)
+        # (to nearest m stops too: at 0.75 a step moves it by 0.1 (1 - 0.75) = 0.025, less than half its codes' 0.0625)
+        assert not seeded or ((m / g[0]).mean() - 1).abs() <= 0.1
+    # the square of a root that is right on average is above by its variance, a few per cent
+    assert abs(got[True] - 1) <= 0.1 and got[False] < 0.2, got
+
+
 def test_moments_there_and_back(cuda):
     import torch
     from toy_b200.multi_adamw import MultiAdamW

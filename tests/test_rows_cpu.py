@@ -73,7 +73,7 @@ def test_adamw_arguments():
                  ("v_scale", P + 2), ("copy", P + 1), ("n", -1), ("n", 1 << 60)):
         assert step({**t_ok, k: v}, a_ok) == -1, (k, v)
     for k, v in (("n_tensors", -1), ("p_type", 8), ("g_type", 3), ("copy_type", 0), ("state_bits", 16), ("hp", None),
-                 ("hp", P + 2), ("grad_scale", P + 1)):
+                 ("hp", P + 2), ("grad_scale", P + 1), ("seed", P + 4)):
         assert step(t_ok, {**a_ok, k: v}) == -1, (k, v)
     assert step({**t_ok, "m": P + 2}, {**a_ok, "state_bits": 32}) == -1
     assert lib().tb2_adamw_multi(None, None) == -1

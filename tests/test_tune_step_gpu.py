@@ -87,7 +87,8 @@ def test_gradients_and_steps(cuda):
                 w[k].grad = None
             loss_on_gpu(w, *dev)[0].backward()
         norm = torch.stack([w[k].grad.norm() for k in names]).norm()
-        opt.step([w[k].grad for k in names], hp.hp(step + 1), grad_scale=(1.0 / norm.clamp(min=1.0)).view(1))
+        opt.step([w[k].grad for k in names], hp.hp(step + 1), grad_scale=(1.0 / norm.clamp(min=1.0)).view(1),
+                 seed=step)
     for k, c in zip(names, copies):
         d = (w[k].detach() - before[k]).abs()
         assert d.max() > 0 and d.max() <= 3.5e-3          # three steps of at most the rate each, but for roundings

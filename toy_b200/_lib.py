@@ -108,7 +108,8 @@ class AdamwTensor(C.Structure):
 
 class AdamwMultiArgs(C.Structure):
     _fields_ = [("tensors", C.c_void_p), ("n_tensors", C.c_int), ("p_type", C.c_int), ("g_type", C.c_int),
-                ("copy_type", C.c_int), ("state_bits", C.c_int), ("hp", C.c_void_p), ("grad_scale", C.c_void_p)]
+                ("copy_type", C.c_int), ("state_bits", C.c_int), ("hp", C.c_void_p), ("grad_scale", C.c_void_p),
+                ("seed", C.c_void_p)]
 
 
 _lib = None

@@ -49,7 +49,9 @@ __device__ __forceinline__ unsigned same_lanes(int e) {
 // share an expert. No workspace. What it takes is latency where slots are few
 // (ids are read eight times 32 at once and kept where a run is no longer, and
 // as many warps take part as have 32 slots, so that few counts are summed) and
-// the instructions of eight SMs where they are many.
+// the instructions of eight SMs where they are many: 128 slots 2.7 us, 4096 4.5,
+// 32768 8.6, 262144 27 (in whose time a tenth of their rows, 2048 bf16 each, is
+// moved).
 constexpr int kAhead = 8;
 template <int BITS>
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(const void* ids, int wide, int n, int E, int warps,
@@ -160,8 +162,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const void* ids, int
   if (C > 1) cluster.sync();   // (the totals are read until here)
 }
 
-// order from its inverse, over the whole GPU: eight SMs write 32 places a warp one after another (32768 slots: see
-// tb2_expert_sort).
+// order from its inverse, over the whole GPU: the eight SMs of the sort have enough to do.
 __global__ void __launch_bounds__(256) order_kernel(const int* pos, const int* live, int n, int* order) {
   griddep_wait();
   const int from = *live;
@@ -237,7 +238,8 @@ __device__ void clear_rest(const RowsArgs& a, void* y, long long ld) {
   }
 }
 
-// A thread has one piece of a token's row: read once, written to the token's places.
+// A thread has one piece of a token's row: read once, written to the token's places. Bound by writing: 4096 tokens of 8
+// bf16 rows of 2048 26.3 us (23.2 for the bytes), 8192 of 4 f32 rows 54 (52).
 template <class T, class V>
 __global__ void __launch_bounds__(256, 5) dispatch_kernel(RowsArgs a) {
   griddep_wait();
@@ -283,7 +285,8 @@ __global__ void __launch_bounds__(256) dispatch_narrow_kernel(RowsArgs a) {
 }
 
 // A thread has one piece of a token's row; its places' pieces are read K at a time. (Several tokens to a thread were
-// slower, 75 us instead of 55 for 8192 tokens of 4 f32 rows of 2048: fewer threads fit an SM.)
+// slower, 75 us instead of 55 for 8192 tokens of 4 f32 rows of 2048, the bytes' 52: fewer threads fit an SM.) 4096
+// tokens of 8 bf16 rows and a residual 29.1 us (25.8).
 template <class T, class V, int K>
 __global__ void __launch_bounds__(256) combine_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
@@ -380,8 +383,8 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(RowsArgs a) {
 
 // A warp has K slots of a token (its last ones may be fewer), Q pieces to a lane at a time: the token's gradient is
 // read once for them, and all their pieces are on their way together. (4096 tokens of 8 bf16 rows of 2048: a warp a
-// slot 62 us, a warp eight 54, with the gradient's pieces read behind the rows' 54, now 50. A CTA a token, its warps' parts
-// added up through shared memory, 63.)
+// slot 62 us, a warp eight 54, with the gradient's pieces read behind the rows' 54, now 50, the bytes' 44. A CTA a
+// token, its warps' parts added up through shared memory, 63.)
 template <class T, class V, int K, int Q>
 __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
   using H = Chunk<T, V>;

@@ -36,6 +36,7 @@ struct Tensors {
   int first[kMaxTensors + 2];             // blocks before tensor i; behind the last one, all
   unsigned whole[(kMaxTensors + 31) / 32];   // bit i: tensor i's arrays are on the boundaries of four values
   int n;
+  long long before;                       // blocks of earlier launches
 };
 
 // The tensor that block b is of.
@@ -150,14 +151,15 @@ __device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) {
 // that start anew with the factors take 475 us: its grid stays, and each CTA has two blocks a warp in a row (429 us;
 // one 447, four 443, a run of all its blocks 489).
 //
-// 8-bit moments are the exact values rounded once, although the step is f32. m is a sum of two terms of either sign,
-// and with few bits in its old value it falls on a border again and again (0.9 of 120 is 108, between 104 and 112: 0.8
-// % of the values of a run with b1 = 0.9 are closer to one than f32 tells), so it is computed in f64, two products and three
-// conversions a value, and converted so that the code is rounded from all its bits. A root's code is taken of both ends
-// of an interval that holds the exact one, and where the two differ (one value in 90000) it is rounded from 64 bits.
-// With U = 2^-24: the root's square is a sum of squares, the held root's factor and product 2 + 1 U, the gradient's 3 +
-// 1, doubled by squaring, 1 for a square and 1 for the sum; the root halves these 10, and is off by 2 U itself: 7 U of
-// the 8 allowed.
+// 8-bit moments without a seed are the exact values rounded once, although the step is f32. m is a sum of two terms of
+// either sign, and with few bits in its old value it falls on a border again and again (0.9 of 120 is 108, between 104
+// and 112: 0.8 % of the values of a run with b1 = 0.9 are closer to one than f32 tells), so it is computed in f64, two
+// products and three conversions a value, and converted so that the code is rounded from all its bits. A root's code is
+// taken of both ends of an interval that holds the exact one, and where the two differ (one value in 90000) it is
+// rounded from 64 bits. With U = 2^-24: the root's square is a sum of squares, the held root's factor and product 2 + 1
+// U, the gradient's 3 + 1, doubled by squaring, 1 for a square and 1 for the sum; the root halves these 10, and is off
+// by 2 U itself: 7 U of the 8 allowed. With a seed the step stays in f32, and the random bits take its place (461 us
+// instead of 435 for 135M weights; 484 with bits of their own for m and the root).
 //
 // Bound by HBM in 32 bits. In 8 bits a value is 16 bytes, the time of some 75 instructions at most: a look at the
 // distance of every root from a border made it 58 (445 us where the bytes of 135M weights take 332), IEEE quotients and
@@ -193,7 +195,7 @@ struct RawBlock {
 
 // A lane's eight values, stepped: p the new weights, m the new first moments, r the new second moments (32 bits) or
 // their roots (8 bits).
-template <int BITS>
+template <int BITS, bool RANDOM>
 __device__ __forceinline__ void step8(const Hyper& h, float (&p)[8], const float (&g)[8], float (&m)[8], float (&r)[8],
                                       float ms, float vs) {
   const float rs = vs * h.sb2;
@@ -201,7 +203,8 @@ __device__ __forceinline__ void step8(const Hyper& h, float (&p)[8], const float
   for (int e = 0; e < 8; ++e) {
     float v;
     if (BITS == 8) {
-      m[e] = to_odd(fma((double)(m[e] * ms), h.b1_64, (double)g[e] * h.dg_64));
+      m[e] = RANDOM ? fmaf(m[e] * ms, h.b1, g[e] * h.dg)
+                    : to_odd(fma((double)(m[e] * ms), h.b1_64, (double)g[e] * h.dg_64));
       const float gs = g[e] * h.sd2, r0 = r[e] * rs;
       v = fmaf(gs, gs, r0 * r0);
     } else {
@@ -215,10 +218,25 @@ __device__ __forceinline__ void step8(const Hyper& h, float (&p)[8], const float
   }
 }
 
-// The block's codes and scales. again(e): value e's root code from 64 bits, given the factor.
-template <class F>
+// 32 bits that look random, of x.
+__device__ __forceinline__ unsigned mixed(unsigned x) {
+  x = (x ^ x >> 16) * 0x7feb352du;
+  x = (x ^ x >> 15) * 0x846ca68bu;
+  return x ^ x >> 16;
+}
+// t (|t| <= 448) rounded to an e4m3 value next to it, the upper one with the probability of t's place between the two:
+// 16 random bits are added below the three that stay. (Codes below 2^-6 are 2^-9 apart, as they are just above it.)
+__device__ __forceinline__ float rounded_by(float t, unsigned bits16) {
+  const float low = fabsf(t) < 0.015625f ? 0.015625f : 0.f;
+  const unsigned b = (__float_as_uint(fabsf(t) + low) + (bits16 << 4)) & 0xfff00000u;
+  return copysignf(__uint_as_float(b) - low, t);
+}
+
+// The block's codes and scales. RANDOM: rounded by random bits of `key`; else again(e) gives value e's root code from
+// 64 bits, given the factor.
+template <bool RANDOM, class F>
 __device__ __forceinline__ void hold8(float (&m)[8], const float (&r)[8], unsigned (&mq)[2], unsigned (&vq)[2],
-                                      float& ms, float& vs, F&& again) {
+                                      float& ms, float& vs, unsigned key, F&& again) {
   float top_m = 0.f, top_r = 0.f, mi, ri;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -227,6 +245,24 @@ __device__ __forceinline__ void hold8(float (&m)[8], const float (&r)[8], unsign
   }
   ms = block_scale(top_m, mi);
   vs = block_scale(top_r, ri);
+  if (RANDOM) {
+    unsigned bits = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float a[4], z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e % 2 == 0) bits = mixed(key + (4 * j + e) * 0x9e3779b9u);   // 16 for each value, m's and the root's
+        const unsigned mine = e % 2 ? bits >> 16 : bits & 0xffffu;
+        a[e] = rounded_by(m[4 * j + e] * mi, mine);
+        z[e] = rounded_by(r[4 * j + e] * ri, mine);
+        z[e] = r[4 * j + e] > 0.f ? fmaxf(z[e], 0x1p-9f) : z[e];   // a positive root keeps the smallest code
+      }
+      mq[j] = pack4_e4m3(a);
+      vq[j] = pack4_e4m3(z);
+    }
+    return;
+  }
   const float low = ri * (1.f - 0x1p-21f), high = ri * (1.f + 0x1p-21f);
   unsigned look[2];   // nonzero bytes: roots to be looked at
 #pragma unroll
@@ -257,9 +293,10 @@ __device__ __forceinline__ float held_code(const void* v, long long k) {
 // The next block is read while one is computed where it lies whole on its boundaries; a tensor's end, or one off its
 // boundaries, goes value by value. (Reads staged further ahead, by asynchronous copies to shared memory or in runs of
 // four blocks with one address each, took as long in 8 bits, 454 and 467 us: what is left is not the reads' latency.)
-template <class P, class G, int BITS>
+template <class P, class G, int BITS, bool RANDOM>
 __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
-    step_kernel(const __grid_constant__ Tensors ts, int copy_type, const float* hp, const float* factor) {
+    step_kernel(const __grid_constant__ Tensors ts, int copy_type, const float* hp, const float* factor,
+                const long long* seed) {
   using S = typename std::conditional<BITS == 8, uint8_t, float>::type;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   // kStepRun blocks to a warp; then a 32-bit CTA ends, and an 8-bit one goes on behind all the grid's
@@ -281,6 +318,13 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
   h.d2 = 1.f - h.b2;
   h.sb2 = sqrtf(h.b2);
   h.sd2 = h.gf * sqrtf(h.d2);
+  // random bits: of the seed, the block's number among all and the lane
+  unsigned key0 = 0, key1 = 0;
+  if (RANDOM) {
+    const unsigned long long x = (unsigned long long)*seed;
+    key0 = mixed((unsigned)x) ^ (unsigned)(ts.before >> 32);
+    key1 = mixed((unsigned)(x >> 32) + 0x51ed270bu) + lane * 0x85ebca6bu;
+  }
   RawBlock<P, G, S> raw;
   // block b of tensor i on its way; whether it is one that is read so
   auto fetch = [&](int b) {
@@ -342,11 +386,12 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? kCtas8 : kCtas32)
       i = tensor_from(ts, i, b + stride);   // (t is still block b's)
       next_whole = fetch(b + stride);
     }
-    step8<BITS>(h, p, g, m, r, ms, vs);
+    step8<BITS, RANDOM>(h, p, g, m, r, ms, vs);
     unsigned mq[2], vq[2];
     if (BITS == 8) {
       float nms, nvs;
-      hold8(m, r, mq, vq, nms, nvs, [&](int e, float ri) {
+      const unsigned key = RANDOM ? mixed(mixed((unsigned)(ts.before + b) ^ key0) + key1) : 0;
+      hold8<RANDOM>(m, r, mq, vq, nms, nvs, key, [&](int e, float ri) {
         const long long k = k0 + 128 * (e / 4) + e % 4;
         return k < t.n ? root_code(to_f32(static_cast<const G*>(t.g)[k]), h.gf, held_code(t.v, k) * vs, h.b2, ri) : 0u;
       });
@@ -523,6 +568,7 @@ unsigned ctas_of(long long blocks, int run) { return (unsigned)((blocks + kWarps
 template <class W, class F>
 int in_groups(const tb2_adamw_tensor* t, int n, W&& whole, F&& launch) {
   Tensors g;
+  g.before = 0;
   for (int i = 0; i < n;) {
     g.n = 0;
     std::fill(std::begin(g.whole), std::end(g.whole), 0u);
@@ -539,13 +585,17 @@ int in_groups(const tb2_adamw_tensor* t, int n, W&& whole, F&& launch) {
     g.first[g.n] = g.first[g.n + 1] = (int)blocks;
     if (g.n)
       if (int rc = launch(g, blocks)) return rc;
+    g.before += blocks;
   }
   return 0;
 }
 
 template <class P, class G>
 int prepare_types() {
-  return load_kernel(step_kernel<P, G, 8>) || load_kernel(step_kernel<P, G, 32>) ? -3 : 0;
+  return load_kernel(step_kernel<P, G, 8, false>) || load_kernel(step_kernel<P, G, 8, true>) ||
+                 load_kernel(step_kernel<P, G, 32, false>)
+             ? -3
+             : 0;
 }
 template <class P>
 int prepare_type() {
@@ -568,7 +618,7 @@ int tb2_adamw_multi(const tb2_adamw_multi_args* a, void* stream) {
   if (!a || a->n_tensors < 0 || (a->n_tensors && !a->tensors) || (a->state_bits != 8 && a->state_bits != 32)) return -1;
   if (!row_type_ok(a->p_type) || !row_type_ok(a->g_type)) return -1;
   if (a->copy_type != kTypeF16 && a->copy_type != kTypeBF16) return -1;
-  if (!a->hp || !all_aligned(4, {a->hp, a->grad_scale})) return -1;
+  if (!a->hp || !all_aligned(4, {a->hp, a->grad_scale}) || !aligned(a->seed, 8)) return -1;
   for (int i = 0; i < a->n_tensors; ++i)
     if (!tensor_ok(a->tensors[i], a->p_type, a->g_type, a->copy_type, a->state_bits)) return -1;
   const size_t pb = 4 * type_bytes(a->p_type), gb = 4 * type_bytes(a->g_type), cb = 4 * type_bytes(a->copy_type);
@@ -582,8 +632,11 @@ int tb2_adamw_multi(const tb2_adamw_multi_args* a, void* stream) {
       return by_row_type(a->g_type, [&](auto q) {
         using P = decltype(p);
         using G = decltype(q);
-        return launch_pdl(a->state_bits == 8 ? step_kernel<P, G, 8> : step_kernel<P, G, 32>, dim3(ctas), dim3(kThreads),
-                          0, static_cast<cudaStream_t>(stream), g, a->copy_type, a->hp, a->grad_scale);
+        auto* kernel = a->state_bits == 32 ? step_kernel<P, G, 32, false>
+                       : a->seed           ? step_kernel<P, G, 8, true>
+                                           : step_kernel<P, G, 8, false>;
+        return launch_pdl(kernel, dim3(ctas), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), g, a->copy_type,
+                          a->hp, a->grad_scale, a->seed);
       });
     });
   });

@@ -4,7 +4,14 @@ bits: tb2_adamw_multi (include/toy_b200.h).
 The step is the framework's own (opt_step_adamw with the 7-slot row of
 `toy_b200.AdamW.hp`). With 8 bits a weight's two moments take 2.03 bytes instead
 of 8: blocks of 256 values share a power of two, m is held as e4m3 and v as the
-e4m3 of its square root, each the step's exact value rounded once.
+e4m3 of its square root, each the step's value rounded once.
+
+Train with a seed. A step moves v by a thousandth of its way (beta2 = 0.999), and
+the nearest of codes that lie 6 to 12 % apart is the one it had: without a seed v
+stops growing after a dozen steps. With one, a value goes to the code above or
+below with the probability of its place between them, so that v follows on
+average. (Without: for states that are to be the exact ones' nearest codes, and
+for moments that a step moves by more than that.)
 """
 from __future__ import annotations
 
@@ -16,7 +23,7 @@ import numpy as np
 import torch
 
 from ._lib import AdamwMultiArgs, AdamwTensor
-from ._rows import F32, ROW_TYPE, bad, call, dense, prepare, written
+from ._rows import F32, I64, ROW_TYPE, bad, call, dense, prepare, written
 
 __all__ = ["MultiAdamW", "prepare"]
 BLOCK = 256
@@ -105,10 +112,12 @@ class MultiAdamW:
         if self.index not in _ready():
             prepare(self.device)
 
-    def step(self, grads: Sequence[Optional[torch.Tensor]], hp, *, grad_scale: Optional[torch.Tensor] = None) -> None:
+    def step(self, grads: Sequence[Optional[torch.Tensor]], hp, *, grad_scale: Optional[torch.Tensor] = None,
+             seed=None) -> None:
         """One step on the gradients (f32, f16 or bf16, all of one type, of the weights' shapes; None: the weight and
         its moments stay). hp: the row of AdamW.hp, as an f32 [7] tensor on the GPU or as numbers; grad_scale: an f32
-        tensor of one value on the GPU that every gradient is multiplied by."""
+        tensor of one value on the GPU that every gradient is multiplied by; seed: 8-bit moments rounded at random, a
+        number or an i64 tensor of one value on the GPU, another for each step (the step's own number does)."""
         if len(grads) != self._n:
             bad("grads: one per weight")
         if not isinstance(hp, torch.Tensor):
@@ -119,6 +128,14 @@ class MultiAdamW:
             if grad_scale.numel() != 1 or grad_scale.dtype is not F32 or grad_scale.get_device() != self.index:
                 bad(f"grad_scale: one f32 value on cuda:{self.index}")
             scale_at = grad_scale.data_ptr()
+        seed_at = None
+        if seed is not None:
+            if not isinstance(seed, torch.Tensor):
+                seed = torch.full((1,), int(seed), dtype=I64, device=self.device)
+            if seed.numel() != 1 or seed.dtype is not I64 or seed.get_device() != self.index:
+                bad(f"seed: a number, or one i64 value on cuda:{self.index}")
+            if self.bits == 8:
+                seed_at = seed.data_ptr()
         grads, shapes, t = list(grads), self._shapes, self._t
         if any(g is None for g in grads):
             on = [i for i, g in enumerate(grads) if g is not None]
@@ -130,7 +147,7 @@ class MultiAdamW:
             bad("grads: f32, f16 or bf16")
         t["g"] = _pointers(grads, shapes, dtype, self.index, "grads")
         a = AdamwMultiArgs(t.ctypes.data, len(t), ROW_TYPE[self.dtype], ROW_TYPE[dtype], ROW_TYPE[self.copy_dtype],
-                           self.bits, hp_at, scale_at)
+                           self.bits, hp_at, scale_at, seed_at)
         call(self.index, "tb2_adamw_multi", a)
         if self._saved:
             written(*self.params)
