@@ -595,8 +595,7 @@ typedef struct tb2_llama_config {
    * blk.N.ffn_{gate,up}_exps.weight [n_experts d_ff x d] and
    * blk.N.ffn_down_exps.weight [n_experts d x d_ff]. Adapters only on q, k, v, o.
    * The backward runs through the experts, the routing weights and the router's
-   * softmax. Such a step runs eagerly (one host round trip per block to order
-   * the routed tokens by expert). 0 = dense FFN. */
+   * softmax. The routed tokens are ordered by expert on the GPU. 0 = dense FFN. */
   int n_experts, n_experts_used, norm_topk;
   /* 2: RMSNorm over the whole q and k vectors before RoPE (OLMoE), frozen
    * gammas blk.N.attn_{q,k}_norm.weight; 0 none. QLoRA only. */
