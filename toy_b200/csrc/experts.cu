@@ -21,7 +21,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kOneCta = 256, kOrderApart = 8192;   // slots
+constexpr int kOneCta = 256;         // slots that one CTA sorts
+// Slots above which order, scattered 4-byte writes, is left to a kernel of all SMs. In the sort's own kernel, and in the
+// other: 16384 slots 7.3 and 7.6 us, 32768 of 128 experts 8.8 and 9.3, 65536 10.9 and 10.4, 262144 30 and 27.
+constexpr int kOrderApart = 32768;
 constexpr int kMaxExperts = 1024, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCtas = 8;
 
 // A slot's expert, or E: none (past: the id is no expert's).
@@ -50,7 +53,7 @@ __device__ __forceinline__ unsigned same_lanes(int e) {
 // (ids are read eight times 32 at once and kept where a run is no longer, and
 // as many warps take part as have 32 slots, so that few counts are summed) and
 // the instructions of eight SMs where they are many: 128 slots 2.7 us, 4096 4.5,
-// 32768 8.6, 262144 27 (in whose time a tenth of their rows, 2048 bf16 each, is
+// 32768 8.4, 262144 27 (in whose time a tenth of their rows, 2048 bf16 each, is
 // moved).
 constexpr int kAhead = 8;
 template <int BITS>
