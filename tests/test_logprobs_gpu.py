@@ -70,11 +70,20 @@ def close(got, want, tol):
     assert (off <= tol.expand_as(want)[~inf]).all(), (off.max(), off / tol.expand_as(want)[~inf])
 
 
-def check(x, t, scale=1.0, top=0, r=None):
+def taken(res, rows):
+    return type(res)(*(None if a is None else a[rows] for a in res))
+
+
+def check(x, t, scale=1.0, top=0, r=None, rows=slice(None)):
+    """A call on all of x, whose `rows` are looked at."""
     import torch
     from toy_b200 import logprobs as L
     V = x.shape[1]
     got = L.token_logprobs(x, t, scale=scale, entropy=True, top=top)
+    again = L.token_logprobs(x, t, scale=scale, entropy=True, top=top)
+    for a, b in zip(got, again):
+        assert a is None or torch.equal(a, b)
+    got, x, t = taken(got, rows), x[rows], t[rows]
     scale = torch.tensor(scale, dtype=torch.float32).double().item()
     r = r or reference(x, t, scale, top)
     live = t.cpu() >= 0
@@ -88,9 +97,6 @@ def check(x, t, scale=1.0, top=0, r=None):
         d0 = torch.where(d.isinf(), torch.zeros_like(d), d)
         tol = bound({k: r[k][:, None] for k in ("mean", "lns")}, d0, V)
         close(got.top_logprobs, r["lp"].gather(1, r["ids"]), tol)
-    again = L.token_logprobs(x, t, scale=scale, entropy=True, top=top)
-    for a, b in zip(got, again):
-        assert a is None or torch.equal(a, b)
     return got
 
 
@@ -103,6 +109,18 @@ SIZES = [(1, 1), (1, 2), (3, 7), (2, 8), (5, 31), (19, 257), (700, 300), (18, 10
 def test_sizes(cuda, n, V, name):
     x, t = make(n, V, dt(name), seed=V + n)
     check(x, t, top=min(V, 20))
+
+
+@pytest.mark.parametrize("name,V", [("f32", 24001), ("bf16", 48005), ("f16", 50303)])
+@pytest.mark.parametrize("n", [591, 593, 600, 888, 889, 1185])
+def test_rounds_with_a_rest(cuda, n, V, name):
+    """More rows than run at once: those of the last round may be split."""
+    x, t = make(n, V, dt(name), seed=n)
+    x[n - 1] = -math.inf
+    t[n - 2] = -1
+    rows = [0, 1, 295, 590, n - 2, n - 1] + [i for i in (591, 592, 593, 887, 888, 1183, 1184) if i < n]
+    check(x, t, scale=0.7, top=7 if n % 2 else 0, rows=rows)
+    check_grad(x, t, scale=0.7, top=3 if n % 2 else 0, entropy=n % 2 == 0, rows=rows)
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
@@ -203,7 +221,7 @@ def grad_reference(x, t, scale, r, gl, gh, ids, gt):
     return torch.where(some, d * scale, torch.zeros_like(d)), a
 
 
-def check_grad(x, t, scale=1.0, top=0, entropy=True, out=None, seed=5, token=True):
+def check_grad(x, t, scale=1.0, top=0, entropy=True, out=None, seed=5, token=True, rows=None):
     import torch
     from toy_b200 import logprobs as L
     n, V = x.shape
@@ -212,9 +230,12 @@ def check_grad(x, t, scale=1.0, top=0, entropy=True, out=None, seed=5, token=Tru
     gl, gh, gt = rnd(n) if token else None, rnd(n) if entropy else None, rnd(n, top) if top else None
     res = L.token_logprobs(x, t, scale=scale, entropy=entropy, top=top)
     s64 = torch.tensor(scale, dtype=torch.float32).double().item()
+    got = L.token_logprobs_grad(x, t, res, gl, grad_entropy=gh, grad_top=gt, scale=scale, out=out)
+    if rows is not None:
+        res, x, t, got = taken(res, rows), x[rows], t[rows], got[rows]
+        gl, gh, gt = (None if a is None else a[rows] for a in (gl, gh, gt))
     r = reference(x, t, s64, top)
     want, a = grad_reference(x, t, s64, r, gl, gh, res.top_ids, gt)
-    got = L.token_logprobs_grad(x, t, res, gl, grad_entropy=gh, grad_top=gt, scale=scale, out=out)
     # p is off by its exponent's roundings, ex2's and ln s's error; the words' own gradients are sums of a few terms
     lp = torch.where(r["lp"].isinf(), torch.zeros_like(r["lp"]), r["lp"]).abs()
     rel = sum_error(r, V)[:, None] + U * (4 * lp + 2 * r["lns"][:, None] + 8)

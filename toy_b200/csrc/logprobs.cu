@@ -20,9 +20,9 @@
 // lowest indices by a scan in order; what passes the buffers (or holds a NaN)
 // takes one round of the row for each alternative.
 //
-// Measured: 4096 rows of 152064 bf16 195 us (191 for the bytes at 6506 GB/s),
-// of 128256 168, with the entropy 179 (161; two more instructions a value, the
-// issue slots are 65 % busy), with 20 alternatives too 220 (the re-read's
+// Measured: 4096 rows of 152064 bf16 190 us (191 for the bytes at 6506 GB/s),
+// of 128256 164, with the entropy 175 (161; two more instructions a value, the
+// issue slots are 65 % busy), with 20 alternatives too 214 (the re-read's
 // latency, in all the CTAs of a round at once); the gradient 338 (323). One row
 // of 49152 f32 3.6, with five alternatives 6.4; 16 of 128256 5.2 and 9.0.
 #include <cooperative_groups.h>
@@ -40,6 +40,7 @@ namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
 constexpr int NT = 256;   // threads a CTA, both directions
+constexpr int kRound = 4 * kSMs;   // CTAs at once
 constexpr int kMaxTop = 32, kGroups = 64, kCand = 1024, kTies = 512, kUnroll = 4;
 
 struct ScoreArgs {
@@ -50,7 +51,7 @@ struct ScoreArgs {
   long long* top_ids;
   int* err;
   float scale;
-  int n, V, top, split;   // split: CTAs (a cluster) to a row
+  int n, V, top, whole, split;   // CTAs to a row: one for the first `whole`, then a cluster of `split`
 };
 
 // Values in the order of (x, lower index first) as whole numbers: NaN above everything, -0 equal to 0.
@@ -369,14 +370,18 @@ __device__ void find_top(ScoreShared& sh, const RowShape<T>& row, int p0, int p1
   }
 }
 
-// One row by `split` CTAs of a cluster (each a run of its pieces; the first has the values outside the pieces too).
-template <class T, bool ENT>
+// A row by one CTA, or (CLUSTER) after the first a.whole rows by `split` CTAs of a cluster, each with a run of its
+// pieces and the first with the values outside the pieces too. (Without the cluster's code 8192 rows of 32000 bf16 take
+// 94 us, not 100, and 8000 of 4000 f32 37, not 41. CTAs that go on to a next row, read ahead, were no faster: 100 and
+// 37, but 4096 of 128256 180, not 168; with a ring of asynchronous copies in shared memory 131, 48 and 228.)
+template <class T, bool ENT, bool CLUSTER>
 __global__ void __launch_bounds__(NT, 4) score_kernel(ScoreArgs a) {
   constexpr int N = Piece<T>::kN;
   __shared__ ScoreShared sh;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int C = a.split, part = blockIdx.x % C;
-  const long long r = blockIdx.x / C;
+  const bool one = !CLUSTER || (int)blockIdx.x < a.whole;
+  const int C = one ? 1 : a.split, part = one ? 0 : blockIdx.x % C;   // (a.whole is a multiple of a.split)
+  const long long r = one ? blockIdx.x : a.whole + (blockIdx.x - a.whole) / C;
   const RowShape<T> row(static_cast<const T*>(a.x) + r * a.ld, a.V);
   const int p0 = (int)((long long)row.P * part / C), p1 = (int)((long long)row.P * (part + 1) / C);
   const int edges = part == 0 ? row.h + row.rest : 0;
@@ -591,7 +596,7 @@ struct GradArgs {
   long long ldd;
   int* err;
   float scale;
-  int n, V, top, split;   // split: CTAs to a row
+  int n, V, top, whole, split;   // CTAs to a row: one for the first `whole`, then `split`
 };
 
 // 16 bytes from byte sh of lo | hi
@@ -616,8 +621,9 @@ __global__ void __launch_bounds__(NT, 4) score_grad_kernel(GradArgs a) {
   __shared__ float x_at[kWords], g_at[kWords];
   __shared__ int at[kWords];
   const int tid = threadIdx.x, lane = tid % 32, V = a.V;
-  const int C = a.split, part = blockIdx.x % C;
-  const long long r = blockIdx.x / C;
+  const bool alone = (int)blockIdx.x < a.whole;
+  const int C = alone ? 1 : a.split, part = alone ? 0 : (blockIdx.x - a.whole) % C;
+  const long long r = alone ? blockIdx.x : a.whole + (blockIdx.x - a.whole) / C;
   const T* x = static_cast<const T*>(a.x) + r * a.ld;
   const RowShape<T> row(static_cast<T*>(a.d) + r * a.ldd, V);
   T* d = static_cast<T*>(a.d) + r * a.ldd;
@@ -773,13 +779,20 @@ int score_launch(ScoreArgs& k, cudaStream_t st) {
     const double us = read + (per + 3) / 4 * ((c == 1 ? 2.0 : 4.0) + (!k.top ? 0.0 : c == 1 ? 3.0 : 4.0));
     if (us < best) best = us, k.split = c;
   }
-  return k.split == 1 ? launch_pdl(score_kernel<T, ENT>, dim3(k.n), dim3(256), 0, st, k)
-                      : launch_pdl_cluster(score_kernel<T, ENT>, dim3(k.n * k.split), dim3(256), 0, st, k.split, k);
+  // the last, half empty round's rows by pairs: 600 rows of 128256 bf16 32.4 us instead of 37.3, 1300 57 instead of 60
+  // (by fours 39 and 60; rows of 64 KB are too short, 2500 of 32000 36.6 instead of 35.9)
+  k.whole = k.split == 1 ? k.n : 0;
+  const int rest = k.n % kRound;
+  if (k.split == 1 && k.n > kRound && rest && rest <= kRound / 2 && bytes >= 96e3) k.split = 2, k.whole -= rest;
+  const int grid = k.whole + (k.n - k.whole) * k.split;
+  return k.split == 1 ? launch_pdl(score_kernel<T, ENT, false>, dim3(grid), dim3(NT), 0, st, k)
+                      : launch_pdl_cluster(score_kernel<T, ENT, true>, dim3(grid), dim3(NT), 0, st, k.split, k);
 }
 
 template <class T>
 int prepare_type() {
-  if (load_kernel(score_kernel<T, false>) || load_kernel(score_kernel<T, true>)) return -3;
+  if (load_kernel(score_kernel<T, false, false>) || load_kernel(score_kernel<T, false, true>)) return -3;
+  if (load_kernel(score_kernel<T, true, false>) || load_kernel(score_kernel<T, true, true>)) return -3;
   return load_kernel(score_grad_kernel<T, false>) || load_kernel(score_grad_kernel<T, true>) ? -3 : 0;
 }
 }  // namespace
@@ -809,7 +822,7 @@ int tb2_logprobs(const tb2_logprobs_args* a, void* stream) {
   int* err = device_error_word();
   if (!err) return -3;
   ScoreArgs k = {a->logits, a->ld, a->tokens, a->logprob, a->stats, a->entropy, a->top_logprobs, a->top_ids, err,
-                 a->scale, a->n_rows, a->vocab, a->top, 1};
+                 a->scale, a->n_rows, a->vocab, a->top, 0, 1};
   return by_row_type(a->row_type, [&](auto t) {
     using T = decltype(t);
     return a->entropy ? score_launch<T, true>(k, static_cast<cudaStream_t>(stream))
@@ -833,12 +846,16 @@ int tb2_logprobs_grad(const tb2_logprobs_grad_args* a, void* stream) {
   int* err = device_error_word();
   if (!err) return -3;
   GradArgs k = {a->logits, a->ld, a->tokens, a->stats, a->entropy, a->g_logprob, a->g_entropy, a->g_top, a->top_ids,
-                a->d_logits, a->ldd, err, a->scale, a->n_rows, a->vocab, a->top, 1};
+                a->d_logits, a->ldd, err, a->scale, a->n_rows, a->vocab, a->top, 0, 1};
   return by_row_type(a->row_type, [&](auto t) {
     using T = decltype(t);
-    k.split = grad_split(k.n, (double)k.V * sizeof(T));
-    return launch_pdl(k.g_h ? score_grad_kernel<T, true> : score_grad_kernel<T, false>, dim3(k.n * k.split),
-                      dim3(NT), 0, static_cast<cudaStream_t>(stream), k);
+    // full rounds take a row to a CTA, and only the rows of the last are split (700 rows of 128256 bf16 63 us, all
+    // alike 69); longer rows are better split throughout (600 of 400000 159 us, not 167: CTAs do not end together)
+    const double bytes = (double)k.V * sizeof(T);
+    if (k.n > kRound && bytes <= 3e5) k.whole = k.n - k.n % kRound;
+    if (k.whole < k.n) k.split = grad_split(k.n - k.whole, bytes);
+    return launch_pdl(k.g_h ? score_grad_kernel<T, true> : score_grad_kernel<T, false>,
+                      dim3(k.whole + (k.n - k.whole) * k.split), dim3(NT), 0, static_cast<cudaStream_t>(stream), k);
   });
 }
 
