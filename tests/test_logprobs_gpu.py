@@ -52,8 +52,9 @@ def reference(x, t, scale, top):
 
 def sum_error(r, V):
     """Bound of ln s's error: every term is off by its exponent's three roundings (difference, constant, product) and
-    by ex2's 2^-22, the sum by a thread's chain and the tree behind it."""
-    return U * (3 * r["mean"] + 4 + V / 512 + 48 + 2 * r["lns"])
+    by ex2's 2^-22, the sum by a thread's chain and the tree behind it. (A thread has two chains of every second value,
+    of V / 256 where a row has 128 threads, and of at most 64, V / 256 + 32, where one of 8192 or fewer has 64.)"""
+    return U * (3 * r["mean"] + 4 + V / 256 + 80 + 2 * r["lns"])
 
 
 def bound(r, d, V):
@@ -101,7 +102,7 @@ def check(x, t, scale=1.0, top=0, r=None, rows=slice(None)):
 
 
 SIZES = [(1, 1), (1, 2), (3, 7), (2, 8), (5, 31), (19, 257), (700, 300), (18, 1000), (40, 4099), (1, 50303),
-         (19, 50303), (160, 20001), (300, 9000), (1300, 2048)]
+         (19, 50303), (160, 20001), (300, 9000), (1300, 2048), (1300, 33), (1185, 100), (1190, 4097), (700, 20001)]
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
@@ -111,7 +112,7 @@ def test_sizes(cuda, n, V, name):
     check(x, t, top=min(V, 20))
 
 
-@pytest.mark.parametrize("name,V", [("f32", 24001), ("bf16", 48005), ("f16", 50303)])
+@pytest.mark.parametrize("name,V", [("f32", 28001), ("bf16", 56005), ("f16", 60001)])
 @pytest.mark.parametrize("n", [591, 593, 600, 888, 889, 1185])
 def test_rounds_with_a_rest(cuda, n, V, name):
     """More rows than run at once: those of the last round may be split."""
@@ -125,7 +126,7 @@ def test_rounds_with_a_rest(cuda, n, V, name):
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("pad,shift", [(0, 1), (1, 0), (3, 5), (8, 0), (5, 8)])
-@pytest.mark.parametrize("n,V", [(3, 1003), (700, 515), (2, 6)])
+@pytest.mark.parametrize("n,V", [(3, 1003), (700, 515), (2, 6), (1200, 1003), (600, 9001)])
 def test_rows_off_their_boundaries(cuda, n, V, pad, shift, name):
     x, t = make(n, V, dt(name), seed=7, pad=pad, shift=shift)
     check(x, t, scale=0.7, top=min(V, 32))
@@ -141,7 +142,7 @@ def test_top_and_scale(cuda, top, scale):
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("n,V", [(2, 70), (3, 30001), (900, 8003)])
+@pytest.mark.parametrize("n,V", [(2, 70), (3, 30001), (900, 8003), (1200, 2003)])
 def test_equal_logits(cuda, n, V, name):
     """Flat rows, rows of two values, rows that rise or fall: ties go to the lower index."""
     import torch
@@ -160,7 +161,7 @@ def test_equal_logits(cuda, n, V, name):
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("n,V", [(12, 90), (12, 9001), (900, 2003)])
+@pytest.mark.parametrize("n,V", [(12, 90), (12, 9001), (900, 2003), (1200, 2003), (600, 20003)])
 def test_masks(cuda, n, V, name):
     """-inf and the type's lowest value; rows that they leave one word, few words or none."""
     import torch
@@ -189,7 +190,7 @@ def test_not_a_number(cuda):
     """A NaN or +inf makes its row's probabilities NaN, and no other's; NaN counts as the largest."""
     import torch
     from toy_b200 import logprobs as L
-    for n in (6, 700):
+    for n in (6, 700, 1200):
         x, t = make(n, 5000, torch.float32, seed=1)
         want = reference(x, t, 1.0, 8)
         x[1, 40], x[2, 4999], x[4, 7], x[4, 9] = math.nan, math.inf, math.nan, -math.nan
@@ -271,7 +272,7 @@ def test_grad_sizes(cuda, n, V, name):
                                                   (8, 8, 1, 0)])
 def test_grad_rows_off_their_boundaries(cuda, pad, shift, opad, oshift, name):
     import torch
-    for n, V in ((3, 1003), (700, 515), (2, 6), (1, 40001)):
+    for n, V in ((3, 1003), (700, 515), (2, 6), (1, 40001), (600, 9001)):
         x, t = make(n, V, dt(name), seed=7, pad=pad, shift=shift)
         buf = torch.full((n * (V + opad) + oshift + 32,), 7.0, device="cuda", dtype=x.dtype)
         out = buf[oshift:oshift + n * (V + opad)].view(n, V + opad)[:, :V]
@@ -285,7 +286,7 @@ def test_grad_rows_off_their_boundaries(cuda, pad, shift, opad, oshift, name):
 def test_grad_in_place(cuda, name):
     import torch
     from toy_b200 import logprobs as L
-    for n, V, pad in ((5, 70001, 0), (900, 1003, 5), (1, 300, 0)):
+    for n, V, pad in ((5, 70001, 0), (900, 1003, 5), (1, 300, 0), (600, 9001, 3), (600, 30001, 0)):
         x, t = make(n, V, dt(name), seed=2, pad=pad)
         res = L.token_logprobs(x, t, entropy=True, top=16)
         g = torch.randn(n, device="cuda")

@@ -13,9 +13,9 @@
 // of its four interleaved shares of the row, which the softmax needs anyway.
 // The top-th largest of 64 group maxima is a lower bound of the row's top-th
 // largest value, and only shares whose maximum reaches it can hold an
-// alternative: of a row's 1024 shares about 24 at top = 20 (values fall into
-// groups like coupons: 20 of 64 groups are hit by the first 64 (H_64 - H_44) =
-// 24), so some 3 % of the row is read again. Values above the bound are ranked
+// alternative: of the 1024 shares of 256 threads about 24 at top = 20 (values
+// fall into groups like coupons: 20 of 64 groups are hit by the first 64 (H_64
+// - H_44) = 24), so some 3 % of the row is read again. Values above the bound are ranked
 // by (value, lower index). Bounds that many values equal (flat rows) take the
 // lowest indices by a scan in order; what passes the buffers (or holds a NaN)
 // takes one round of the row for each alternative.
@@ -39,8 +39,8 @@ namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int NT = 256;   // threads a CTA, both directions
-constexpr int kRound = 4 * kSMs;   // CTAs at once
+constexpr int kThreads = 1024;   // an SM's, in CTAs of NT
+constexpr int kRound = 4 * kSMs;   // CTAs of 256 threads at once
 constexpr int kMaxTop = 32, kGroups = 64, kCand = 1024, kTies = 512, kUnroll = 4;
 
 struct ScoreArgs {
@@ -144,6 +144,7 @@ __device__ __forceinline__ void move_to(Sums& a, float m, float c) {
   a.m = m;
 }
 
+template <int NT>
 struct ScoreShared {
   alignas(16) float group[kGroups];
   float red[NT / 32 * 3];
@@ -174,8 +175,8 @@ struct RowShape {
 };
 
 // The CTA's lowest `need` indices of pieces [p0, p1) whose value is v, behind cand[n ..).
-template <class T>
-__device__ void scan_equal(ScoreShared& sh, const RowShape<T>& row, int p0, int p1, float v, int need, int n) {
+template <int NT, class T>
+__device__ void scan_equal(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, float v, int need, int n) {
   constexpr int N = Piece<T>::kN;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int found = 0;
@@ -215,7 +216,8 @@ __device__ void scan_equal(ScoreShared& sh, const RowShape<T>& row, int p0, int 
 }
 
 // cand[0 .. n) and ties[0 .. more) by rank: the `top` largest to list, which holds zeros.
-__device__ void rank_keys(ScoreShared& sh, int n, int more, int top) {
+template <int NT>
+__device__ void rank_keys(ScoreShared<NT>& sh, int n, int more, int top) {
   const int lane = threadIdx.x % 32, all = n + more;
   for (int i = threadIdx.x / 32 * 8; i < all; i += NT / 32 * 8) {   // four lanes to a key
     const int me = i + lane / 4;
@@ -233,7 +235,8 @@ __device__ void rank_keys(ScoreShared& sh, int n, int more, int top) {
 
 // The `top` largest keys of C lists in falling order (kMaxTop entries each, 0 past the last) in cand: a key's place is
 // the number of larger ones, found in every list by halving.
-__device__ void merge_lists(ScoreShared& sh, int C, int top) {
+template <int NT>
+__device__ void merge_lists(ScoreShared<NT>& sh, int C, int top) {
   if (threadIdx.x < kMaxTop) sh.list[threadIdx.x] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < C * kMaxTop; i += NT) {
@@ -254,8 +257,8 @@ __device__ void merge_lists(ScoreShared& sh, int C, int top) {
 }
 
 // One round of the CTA's share of the row for each alternative (-inf left out).
-template <class T>
-__device__ void top_by_rounds(ScoreShared& sh, const RowShape<T>& row, int p0, int p1, int edges, int top) {
+template <int NT, class T>
+__device__ void top_by_rounds(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, int edges, int top) {
   constexpr int N = Piece<T>::kN;
   u64 last = ~0ull;
   for (int k = 0; k < kMaxTop; ++k) {
@@ -289,8 +292,8 @@ __device__ void top_by_rounds(ScoreShared& sh, const RowShape<T>& row, int p0, i
 }
 
 // The CTA's alternatives to list, from the maxima of its threads' shares.
-template <class T>
-__device__ void find_top(ScoreShared& sh, const RowShape<T>& row, int p0, int p1, int edges, int top,
+template <int NT, class T>
+__device__ void find_top(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, int p1, int edges, int top,
                          const float (&share)[kUnroll], bool odd) {
   constexpr int N = Piece<T>::kN, kLanes = NT / kGroups;
   const int tid = threadIdx.x;
@@ -359,7 +362,7 @@ __device__ void find_top(ScoreShared& sh, const RowShape<T>& row, int p0, int p1
   } else if (ties <= kTies) {
     rank_keys(sh, n, ties, top);
   } else {
-    scan_equal<T>(sh, row, p0, p1, tau, top - n, n);
+    scan_equal<NT, T>(sh, row, p0, p1, tau, top - n, n);
     const int more = sh.n_found;
     if (tid < edges) {
       const float x = to_f32(row.x[row.edge(tid)]);
@@ -371,13 +374,14 @@ __device__ void find_top(ScoreShared& sh, const RowShape<T>& row, int p0, int p1
 }
 
 // A row by one CTA, or (CLUSTER) after the first a.whole rows by `split` CTAs of a cluster, each with a run of its
-// pieces and the first with the values outside the pieces too. (Without the cluster's code 8192 rows of 32000 bf16 take
-// 94 us, not 100, and 8000 of 4000 f32 37, not 41. CTAs that go on to a next row, read ahead, were no faster: 100 and
-// 37, but 4096 of 128256 180, not 168; with a ring of asynchronous copies in shared memory 131, 48 and 228.)
-template <class T, bool ENT, bool CLUSTER>
-__global__ void __launch_bounds__(NT, 4) score_kernel(ScoreArgs a) {
+// pieces and the first with the values outside the pieces too. (Without the cluster's code, in CTAs of 256, 8192 rows of
+// 32000 bf16 take 94 us, not 100, and 8000 of 4000 f32 37, not 41. CTAs that go on to a next row, read ahead, were no
+// faster: 100 and 37, but 4096 of 128256 180, not 168; with a ring of asynchronous copies in shared memory 131, 48 and
+// 228.)
+template <int NT, class T, bool ENT, bool CLUSTER>
+__global__ void __launch_bounds__(NT, kThreads / NT) score_kernel(ScoreArgs a) {
   constexpr int N = Piece<T>::kN;
-  __shared__ ScoreShared sh;
+  __shared__ ScoreShared<NT> sh;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const bool one = !CLUSTER || (int)blockIdx.x < a.whole;
   const int C = one ? 1 : a.split, part = one ? 0 : blockIdx.x % C;   // (a.whole is a multiple of a.split)
@@ -503,7 +507,7 @@ __global__ void __launch_bounds__(NT, 4) score_kernel(ScoreArgs a) {
   if (ENT) t.u = __shfl_sync(0xffffffffu, t.u, 0);
   if (a.top) {
     __syncthreads();   // red is free
-    find_top<T>(sh, row, p0, p1, edges, a.top, share, t.s != t.s);
+    find_top<NT, T>(sh, row, p0, p1, edges, a.top, share, t.s != t.s);
   }
   if (C > 1) {   // the row's from its CTAs'
     cg::cluster_group cluster = cg::this_cluster();
@@ -615,8 +619,8 @@ __device__ __forceinline__ uint4 join_bytes(const uint4& lo, const uint4& hi, in
 // a gradient of their own (the token, the alternatives) are put right at the end. A CTA has a run of the 16-byte pieces
 // of the result's row; a row of logits that starts elsewhere within its 16 bytes is read in aligned pieces and shifted
 // (509 rows of 50303 f16 words that lie so: 27 us where the bytes take 16).
-template <class T, bool ENT>
-__global__ void __launch_bounds__(NT, 4) score_grad_kernel(GradArgs a) {
+template <int NT, class T, bool ENT>
+__global__ void __launch_bounds__(NT, kThreads / NT) score_grad_kernel(GradArgs a) {
   constexpr int N = Piece<T>::kN, kWords = kMaxTop + 1;
   __shared__ float x_at[kWords], g_at[kWords];
   __shared__ int at[kWords];
@@ -751,7 +755,14 @@ bool rows_ok(long long ld, int V, const void* p, int type) {
   return p && ld >= V && aligned(p, type_bytes(type));
 }
 
-// CTAs to a row of the gradient, by the same rule: a CTA reads and writes 5.5 B/ns each and has 2 us to spend besides;
+// Threads to a CTA of the gradient: see score_threads (8192 rows by 256, 128 and 64 threads: 1000 bf16 36, 19 and 14
+// us, 8000 bf16 80, 59, 53, 18240 bf16 113, 106, 108, 50304 bf16 262, 267, 273; 592 of 4096 bf16 3.5, 3.0, 3.3).
+int grad_threads(int n, double bytes) {
+  if (n <= kRound) return n > kSMs && bytes <= 8192 ? 128 : 256;
+  return bytes <= 16384 ? 64 : bytes <= 49152 ? 128 : 256;
+}
+
+// CTAs to a row of the gradient: a CTA reads and writes 5.5 B/ns each and has 2 us to spend besides;
 // it has 4 KB at least.
 int grad_split(int n, double bytes) {
   double best = 1e300;
@@ -764,36 +775,68 @@ int grad_split(int n, double bytes) {
   return split;
 }
 
-// CTAs to a row: the split with the shortest time by what was measured. An SM with k of the grid's CTAs reads 44 B/ns,
-// one CTA 22 (f32) or 14 (16 bits: instructions), and each round of four CTAs adds 2 us (a cluster 4) and with
-// alternatives 3 us more (4). (CTAs of 1024 threads for a few rows, each with its whole share in flight: 4.5 us instead
-// of 3.5 for one row of 49152 f32, and 16 clusters of eight such CTAs do not fit the GPU at once, 18.2 us instead of
-// 9.0 for 16 rows of 128256 with 20 alternatives.)
+// f(the number as a type)
+template <class F>
+int by_threads(int threads, F&& f) {
+  return threads == 64 ? f(std::integral_constant<int, 64>()) : threads == 128 ? f(std::integral_constant<int, 128>())
+                                                                               : f(std::integral_constant<int, 256>());
+}
+
+// Threads to a CTA that has a row: what a row costs besides its bytes is latency and its warps' instructions, so short
+// rows are for few warps, and more rows at a time (8192 rows by 256, 128 and 64 threads: 1000 bf16 31, 16 and 10 us,
+// 8000 bf16 44, 31, 29, 18240 bf16 64, 53, 58 and with 20 alternatives 123, 96, 124, 50304 bf16 135, 129, 143 and with
+// 20 alternatives 200, 203, 271; 592 of 2048 bf16 2.7, 2.3, 2.6, of 4096 2.8, 2.9, 3.1).
+int score_threads(int n, double bytes, int top) {
+  if (n <= kRound) return bytes <= 4096 ? 128 : 256;
+  if (n > 2 * kRound && bytes <= 16384) return 64;
+  return bytes <= (top > 8 ? 49152 : 110e3) ? 128 : 256;
+}
+
+// CTAs to a row: the split with the shortest time by what was measured. A CTA reads 16-bit rows at 20 B/ns where it has
+// the SM alone, at 10 where four share it (instructions), f32 at 21 and 16, HBM gives 6500, and each round of CTAs adds
+// 2 us (a cluster 4) and with alternatives 3 us more (4). (CTAs of 1024 threads for a few rows, each with its whole
+// share in flight: 4.5 us instead of 3.5 for one row of 49152 f32, and 16 clusters of eight such CTAs do not fit the
+// GPU at once, 18.2 us instead of 9.0 for 16 rows of 128256 with 20 alternatives. Nor do 74 clusters of eight of 256:
+// 11.7 us, of four 9.0.)
 template <class T, bool ENT>
 int score_launch(ScoreArgs& k, cudaStream_t st) {
-  const double bytes = (double)k.V * sizeof(T);
+  constexpr double kRate[4] = {sizeof(T) == 4 ? 21e3 : 20e3, sizeof(T) == 4 ? 20.5e3 : 17.5e3,
+                               sizeof(T) == 4 ? 18e3 : 13e3, sizeof(T) == 4 ? 16e3 : 10e3};
+  const double row = (double)k.V * sizeof(T);
   double best = 1e300;
   for (int c = 1; c <= 8 && (long long)k.n * c <= 0x7fffffffLL; c *= 2) {
-    const long long per = ((long long)k.n * c + kSMs - 1) / kSMs;   // of an SM
-    const double read = std::max(per * bytes / c / 44e3, bytes / c / (sizeof(T) == 4 ? 22e3 : 14e3));
-    const double us = read + (per + 3) / 4 * ((c == 1 ? 2.0 : 4.0) + (!k.top ? 0.0 : c == 1 ? 3.0 : 4.0));
+    const double bytes = row / c;
+    const int room = c == 8 ? 512 : kRound, full = k.n * c / room, rest = k.n * c % room;
+    double us = full * std::max(room * bytes / 6500e3, bytes / kRate[3]);
+    if (rest) us += std::max(rest * bytes / 6500e3, bytes / kRate[std::min(3, (rest - 1) / kSMs)]);
+    us += (full + (rest > 0)) * ((c == 1 ? 2.0 : 4.0) + (!k.top ? 0.0 : c == 1 ? 3.0 : 4.0));
     if (us < best) best = us, k.split = c;
   }
+  const int threads = k.split == 1 ? score_threads(k.n, row, k.top) : 256;
   // the last, half empty round's rows by pairs: 600 rows of 128256 bf16 32.4 us instead of 37.3, 1300 57 instead of 60
-  // (by fours 39 and 60; rows of 64 KB are too short, 2500 of 32000 36.6 instead of 35.9)
+  // (by fours 39 and 60; with 20 alternatives 2500 of 32000 56, not 52)
   k.whole = k.split == 1 ? k.n : 0;
   const int rest = k.n % kRound;
-  if (k.split == 1 && k.n > kRound && rest && rest <= kRound / 2 && bytes >= 96e3) k.split = 2, k.whole -= rest;
+  if (threads == 256 && k.split == 1 && k.n > kRound && rest && rest <= kRound / 2 && row >= 96e3)
+    k.split = 2, k.whole -= rest;
   const int grid = k.whole + (k.n - k.whole) * k.split;
-  return k.split == 1 ? launch_pdl(score_kernel<T, ENT, false>, dim3(grid), dim3(NT), 0, st, k)
-                      : launch_pdl_cluster(score_kernel<T, ENT, true>, dim3(grid), dim3(NT), 0, st, k.split, k);
+  if (k.split > 1) return launch_pdl_cluster(score_kernel<256, T, ENT, true>, dim3(grid), dim3(256), 0, st, k.split, k);
+  return by_threads(threads, [&](auto nt) {
+    constexpr int NT = decltype(nt)::value;
+    return launch_pdl(score_kernel<NT, T, ENT, false>, dim3(grid), dim3(NT), 0, st, k);
+  });
 }
 
 template <class T>
 int prepare_type() {
-  if (load_kernel(score_kernel<T, false, false>) || load_kernel(score_kernel<T, false, true>)) return -3;
-  if (load_kernel(score_kernel<T, true, false>) || load_kernel(score_kernel<T, true, true>)) return -3;
-  return load_kernel(score_grad_kernel<T, false>) || load_kernel(score_grad_kernel<T, true>) ? -3 : 0;
+  int bad = load_kernel(score_kernel<256, T, false, true>) | load_kernel(score_kernel<256, T, true, true>);
+  for (int threads : {64, 128, 256})
+    bad |= by_threads(threads, [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      return load_kernel(score_kernel<NT, T, false, false>) | load_kernel(score_kernel<NT, T, true, false>) |
+             load_kernel(score_grad_kernel<NT, T, false>) | load_kernel(score_grad_kernel<NT, T, true>);
+    });
+  return bad;
 }
 }  // namespace
 
@@ -849,13 +892,18 @@ int tb2_logprobs_grad(const tb2_logprobs_grad_args* a, void* stream) {
                 a->d_logits, a->ldd, err, a->scale, a->n_rows, a->vocab, a->top, 0, 1};
   return by_row_type(a->row_type, [&](auto t) {
     using T = decltype(t);
+    const double bytes = (double)k.V * sizeof(T);
+    const int threads = grad_threads(k.n, bytes);
     // full rounds take a row to a CTA, and only the rows of the last are split (700 rows of 128256 bf16 63 us, all
     // alike 69); longer rows are better split throughout (600 of 400000 159 us, not 167: CTAs do not end together)
-    const double bytes = (double)k.V * sizeof(T);
-    if (k.n > kRound && bytes <= 3e5) k.whole = k.n - k.n % kRound;
+    if (threads < 256) k.whole = k.n;
+    else if (k.n > kRound && bytes <= 3e5) k.whole = k.n - k.n % kRound;
     if (k.whole < k.n) k.split = grad_split(k.n - k.whole, bytes);
-    return launch_pdl(k.g_h ? score_grad_kernel<T, true> : score_grad_kernel<T, false>,
-                      dim3(k.whole + (k.n - k.whole) * k.split), dim3(NT), 0, static_cast<cudaStream_t>(stream), k);
+    return by_threads(threads, [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      return launch_pdl(k.g_h ? score_grad_kernel<NT, T, true> : score_grad_kernel<NT, T, false>,
+                        dim3(k.whole + (k.n - k.whole) * k.split), dim3(NT), 0, static_cast<cudaStream_t>(stream), k);
+    });
   });
 }
 
