@@ -374,10 +374,10 @@ __device__ void find_top(ScoreShared<NT>& sh, const RowShape<T>& row, int p0, in
 }
 
 // A row by one CTA, or (CLUSTER) after the first a.whole rows by `split` CTAs of a cluster, each with a run of its
-// pieces and the first with the values outside the pieces too. (Without the cluster's code, in CTAs of 256, 8192 rows of
-// 32000 bf16 take 94 us, not 100, and 8000 of 4000 f32 37, not 41. CTAs that go on to a next row, read ahead, were no
-// faster: 100 and 37, but 4096 of 128256 180, not 168; with a ring of asynchronous copies in shared memory 131, 48 and
-// 228.)
+// pieces and the first with the values outside the pieces too. (Without the cluster's code, in CTAs of 256, 8192 rows
+// of 32000 bf16 take 94 us, not 100, and 8000 of 4000 f32 37, not 41. CTAs that go on to a next row, read ahead, were
+// no faster: 100 and 37, but 4096 of 128256 180, not 168; with a ring of asynchronous copies in shared memory 131, 48
+// and 228.)
 template <int NT, class T, bool ENT, bool CLUSTER>
 __global__ void __launch_bounds__(NT, kThreads / NT) score_kernel(ScoreArgs a) {
   constexpr int N = Piece<T>::kN;
