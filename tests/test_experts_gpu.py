@@ -74,7 +74,8 @@ def rows_in(n, d, dtype, seed, pad=0, shift=0):
 
 SHAPES = [(1, 1, 1, 1, 0, 0), (5, 2, 4, 7, 0, 0), (16, 8, 64, 2048, 0, 0), (300, 3, 8, 1000, 0, 0),
           (300, 3, 8, 1001, 0, 0), (70, 8, 16, 256, 8, 8), (70, 8, 16, 250, 3, 1), (40, 16, 64, 72, 0, 0),
-          (1000, 5, 128, 64, 0, 0), (2500, 1, 3, 96, 0, 0)]
+          (1000, 5, 128, 64, 0, 0), (2500, 1, 3, 96, 0, 0), (1501, 2, 16, 136, 0, 0), (111, 4, 8, 520, 8, 8),
+          (67, 6, 64, 1032, 0, 0), (130, 7, 9, 64, 0, 0), (50, 9, 32, 256, 0, 0), (1, 1, 8, 72, 0, 0)]
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])

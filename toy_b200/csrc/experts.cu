@@ -22,8 +22,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kOneCta = 256;         // slots that one CTA sorts
-// Slots above which order, scattered 4-byte writes, is left to a kernel of all SMs. In the sort's own kernel, and in the
-// other: 16384 slots 7.3 and 7.6 us, 32768 of 128 experts 8.8 and 9.3, 65536 10.9 and 10.4, 262144 30 and 27.
+// Slots above which order, scattered 4-byte writes, is left to a kernel of all SMs. In the sort's own kernel, and in
+// the other: 16384 slots 7.3 and 7.6 us, 32768 of 128 experts 8.8 and 9.3, 65536 10.9 and 10.4, 262144 30 and 27.
 constexpr int kOrderApart = 32768;
 constexpr int kMaxExperts = 1024, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCtas = 8;
 
@@ -260,6 +260,35 @@ __global__ void __launch_bounds__(256, 5) dispatch_kernel(RowsArgs a) {
   clear_rest<T, V>(a, a.y, a.ldy);
 }
 
+// A slot or two to a token: P pieces to a thread, 256 apart among all, so that enough of them are on their way (31672
+// tokens of one bf16 row of 1024 22.6 us instead of 26.9, the bytes' 19.9; of two 32.2, 34.4, 29.9; four pieces 23.8).
+template <class T, class V, int P>
+__global__ void __launch_bounds__(256) dispatch_few_kernel(RowsArgs a) {
+  griddep_wait();
+  const long long all = (long long)a.T * a.per;
+  for (long long i0 = blockIdx.x * (256LL * P) + threadIdx.x; i0 < all; i0 += gridDim.x * (256LL * P)) {
+    long long t[P];
+    int c[P];
+    V v[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const long long i = min(i0 + 256 * j, all - 1);
+      t[j] = row_of(a, i);
+      c[j] = (int)(i - t[j] * a.per);
+      v[j] = Chunk<T, V>::load_once(a.x, t[j], a.ldx, c[j]);
+    }
+    for (int k = 0; k < a.K; ++k) {
+      int p[P];
+#pragma unroll
+      for (int j = 0; j < P; ++j) p[j] = i0 + 256 * j < all ? place(a, t[j] * a.K + k) : -1;
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        if (p[j] >= 0) Chunk<T, V>::store(a.y, p[j], a.ldy, c[j], v[j]);
+    }
+  }
+  clear_rest<T, V>(a, a.y, a.ldy);
+}
+
 // Pieces of less than 16 bytes: a warp has kCols of a token's, eight to a lane, so that the places and the rows'
 // addresses are found once for eight. (A thread a piece was bound by its instructions: combine of 9902 tokens of 3 f32
 // rows of 3395 220 us instead of 104.)
@@ -287,11 +316,11 @@ __global__ void __launch_bounds__(256) dispatch_narrow_kernel(RowsArgs a) {
   clear_rest<T, V>(a, a.y, a.ldy);
 }
 
-// A thread has one piece of a token's row; its places' pieces are read K at a time. (Several tokens to a thread were
-// slower, 75 us instead of 55 for 8192 tokens of 4 f32 rows of 2048, the bytes' 52: fewer threads fit an SM.) 4096
-// tokens of 8 bf16 rows and a residual 29.1 us (25.8).
-template <class T, class V, int K>
+// A thread has one piece of a token's row; its places' pieces are read eight at a time. 4096 tokens of 8 bf16 rows of
+// 2048 and a residual 28.5 us (25.8).
+template <class T, class V>
 __global__ void __launch_bounds__(256) combine_kernel(RowsArgs a) {
+  constexpr int K = 8;
   using H = Chunk<T, V>;
   griddep_wait();
   const long long all = (long long)a.T * a.per;
@@ -328,6 +357,59 @@ __global__ void __launch_bounds__(256) combine_kernel(RowsArgs a) {
         }
     }
     H::store(a.y, t, a.ldy, c, H::put(y));
+  }
+}
+
+// K slots to a token, and P of its pieces to a thread, 256 apart among all. One slot leaves room for four pieces: 31672
+// tokens of one bf16 row of 1024 and a residual 30.4 us (29.9 for the bytes) instead of 46.6 by the kernel above; 16384
+// of two f32 rows of 2048 83 instead of 105 (82.5; two pieces 88), 8192 of four 61 instead of 66, 2696 of five f16 rows
+// 14.4 instead of 16.6. (Eight slots are too many at once, 512 tokens of bf16 rows 6.8 instead of 5.7.)
+template <class T, class V, int K, int P>
+__global__ void __launch_bounds__(256) combine_slots_kernel(RowsArgs a) {
+  using H = Chunk<T, V>;
+  griddep_wait();
+  const long long all = (long long)a.T * a.per;
+  for (long long i0 = blockIdx.x * (256LL * P) + threadIdx.x; i0 < all; i0 += gridDim.x * (256LL * P)) {
+    long long t[P];
+    int c[P], p[P][K];
+    V r[P], z[P][K];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const long long i = min(i0 + 256 * j, all - 1);
+      t[j] = row_of(a, i);
+      c[j] = (int)(i - t[j] * a.per);
+      if (a.res) r[j] = H::load_once(a.res, t[j], a.ldr, c[j]);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        p[j][k] = place(a, t[j] * K + k);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (p[j][k] >= 0) z[j][k] = H::load_once(a.z, p[j][k], a.ldz, c[j]);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      if (i0 + 256 * j >= all) continue;
+      float y[H::kN];
+      if (a.res) {
+        H::get(r[j], y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < H::kN; ++e) y[e] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (p[j][k] >= 0) {
+          const float w = a.w ? a.w[t[j] * K + k] : 1.f;
+          float f[H::kN];
+          H::get(z[j][k], f);
+#pragma unroll
+          for (int e = 0; e < H::kN; ++e) y[e] = fmaf(w, f[e], y[e]);
+        }
+      H::store(a.y, t[j], a.ldy, c[j], H::put(y));
+    }
   }
 }
 
@@ -509,17 +591,19 @@ int by_piece(RowsArgs& k, int type, std::initializer_list<std::pair<const void*,
 unsigned grid_of(long long threads) {
   return (unsigned)std::max(1LL, std::min((threads + 255) / 256, (long long)INT_MAX));
 }
+unsigned few_grid(const RowsArgs& k, int pieces) { return grid_of(((long long)k.T * k.per + pieces - 1) / pieces); }
 unsigned narrow_grid(const RowsArgs& k) { return grid_of((long long)k.T * ((k.per + kCols - 1) / kCols) * 32); }
 template <class T, class V>
 int dispatch_by(const RowsArgs& k, cudaStream_t st) {
   if constexpr (sizeof(V) < 16)
     return launch_pdl(dispatch_narrow_kernel<T, V>, dim3(narrow_grid(k)), dim3(256), 0, st, k);
   else
-    return launch_pdl(dispatch_kernel<T, V>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0, st, k);
+    return k.K <= 2 ? launch_pdl(dispatch_few_kernel<T, V, 2>, dim3(few_grid(k, 2)), dim3(256), 0, st, k)
+                    : launch_pdl(dispatch_kernel<T, V>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0, st, k);
 }
-template <class T, class V, int K>
-int combine_launch(const RowsArgs& k, cudaStream_t st) {
-  return launch_pdl(combine_kernel<T, V, K>, dim3(grid_of((long long)k.T * k.per)), dim3(256), 0, st, k);
+template <class T, class V, int K, int P>
+int combine_slots(const RowsArgs& k, cudaStream_t st) {
+  return launch_pdl(combine_slots_kernel<T, V, K, P>, dim3(few_grid(k, P)), dim3(256), 0, st, k);
 }
 template <class T, class V>
 int combine_by(const RowsArgs& k, cudaStream_t st) {
@@ -527,17 +611,26 @@ int combine_by(const RowsArgs& k, cudaStream_t st) {
     return launch_pdl(k.K <= 2 ? combine_narrow_kernel<T, V, 2> : combine_narrow_kernel<T, V, 4>, dim3(narrow_grid(k)),
                       dim3(256), 0, st, k);
   else
-    return k.K <= 2 ? combine_launch<T, V, 2>(k, st)
-         : k.K <= 4 ? combine_launch<T, V, 4>(k, st) : combine_launch<T, V, 8>(k, st);
+    switch (k.K) {
+      case 1: return combine_slots<T, V, 1, 4>(k, st);
+      case 2: return combine_slots<T, V, 2, 1>(k, st);
+      case 3: return combine_slots<T, V, 3, 1>(k, st);
+      case 4: return combine_slots<T, V, 4, 1>(k, st);
+      case 5: return combine_slots<T, V, 5, 1>(k, st);
+      case 6: return combine_slots<T, V, 6, 1>(k, st);
+      case 7: return combine_slots<T, V, 7, 1>(k, st);
+      default: return launch_pdl(combine_kernel<T, V>, dim3(few_grid(k, 1)), dim3(256), 0, st, k);
+    }
 }
 // Two slots to a warp, one where that would leave less than 16 warps an SM or pieces are of 4 bytes and less (180 us
-// instead of 203 for 9902 tokens of 3 f32 rows of 3395).
-template <class V>
-constexpr int kGradCols = sizeof(V) == 16 ? 2 : sizeof(V) == 8 ? 4 : 8;
+// instead of 203 for 9902 tokens of 3 f32 rows of 3395). One slot has four 16-byte pieces to a lane (32768 tokens of
+// one bf16 row of 576 25 us, with two 29).
+template <class V, int K>
+constexpr int kGradCols = sizeof(V) == 16 ? 4 / K : sizeof(V) == 8 ? 4 : 8;
 template <class T, class V, int K>
 int combine_grad_launch(const RowsArgs& k, cudaStream_t st) {
   const long long warps = (long long)k.T * ((k.K + K - 1) / K);
-  return launch_pdl(combine_grad_kernel<T, V, K, kGradCols<V>>, dim3(grid_of(32 * warps)), dim3(256), 0, st, k);
+  return launch_pdl(combine_grad_kernel<T, V, K, kGradCols<V, K>>, dim3(grid_of(32 * warps)), dim3(256), 0, st, k);
 }
 template <class T, class V>
 int combine_grad_by(const RowsArgs& k, cudaStream_t st) {
@@ -548,18 +641,20 @@ int combine_grad_by(const RowsArgs& k, cudaStream_t st) {
 
 template <class T, class V>
 int prepare_piece() {
-  constexpr int Q = kGradCols<V>;
-  if (load_kernel(combine_grad_kernel<T, V, 1, Q>)) return -3;
+  if (load_kernel(combine_grad_kernel<T, V, 1, kGradCols<V, 1>>)) return -3;
   if constexpr (sizeof(V) > 4)
-    if (load_kernel(combine_grad_kernel<T, V, 2, Q>)) return -3;
+    if (load_kernel(combine_grad_kernel<T, V, 2, kGradCols<V, 2>>)) return -3;
   if constexpr (sizeof(V) < 16)
     return load_kernel(dispatch_narrow_kernel<T, V>) || load_kernel(combine_narrow_kernel<T, V, 2>) ||
                    load_kernel(combine_narrow_kernel<T, V, 4>)
                ? -3
                : 0;
   else
-    return load_kernel(dispatch_kernel<T, V>) || load_kernel(combine_kernel<T, V, 2>) ||
-                   load_kernel(combine_kernel<T, V, 4>) || load_kernel(combine_kernel<T, V, 8>)
+    return load_kernel(dispatch_kernel<T, V>) || load_kernel(dispatch_few_kernel<T, V, 2>) ||
+                   load_kernel(combine_kernel<T, V>) || load_kernel(combine_slots_kernel<T, V, 1, 4>) ||
+                   load_kernel(combine_slots_kernel<T, V, 2, 1>) || load_kernel(combine_slots_kernel<T, V, 3, 1>) ||
+                   load_kernel(combine_slots_kernel<T, V, 4, 1>) || load_kernel(combine_slots_kernel<T, V, 5, 1>) ||
+                   load_kernel(combine_slots_kernel<T, V, 6, 1>) || load_kernel(combine_slots_kernel<T, V, 7, 1>)
                ? -3
                : 0;
 }
