@@ -360,10 +360,11 @@ __global__ void __launch_bounds__(256) combine_kernel(RowsArgs a) {
   }
 }
 
-// K slots to a token, and P of its pieces to a thread, 256 apart among all. One slot leaves room for four pieces: 31672
-// tokens of one bf16 row of 1024 and a residual 30.4 us (29.9 for the bytes) instead of 46.6 by the kernel above; 16384
-// of two f32 rows of 2048 83 instead of 105 (82.5; two pieces 88), 8192 of four 61 instead of 66, 2696 of five f16 rows
-// 14.4 instead of 16.6. (Eight slots are too many at once, 512 tokens of bf16 rows 6.8 instead of 5.7.)
+// K slots to a token, and P pieces to a thread, 256 apart among all. With the slots known the addresses cost less,
+// and one slot leaves room for four pieces: 31672 tokens of one bf16 row of 1024 and a residual 30.4 us (29.9 for the
+// bytes) instead of 46.6 by slots in a loop; 16384 of two f32 rows of 2048 83 instead of 105 (82.5; two pieces 88),
+// 8192 of four 61 instead of 66, 2696 of five f16 rows 14.4 instead of 16.6. (Eight slots are too many at once, 512
+// tokens of bf16 rows 6.8 instead of 5.7.)
 template <class T, class V, int K, int P>
 __global__ void __launch_bounds__(256) combine_slots_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
@@ -380,9 +381,7 @@ __global__ void __launch_bounds__(256) combine_slots_kernel(RowsArgs a) {
       c[j] = (int)(i - t[j] * a.per);
       if (a.res) r[j] = H::load_once(a.res, t[j], a.ldr, c[j]);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        p[j][k] = place(a, t[j] * K + k);
-      }
+      for (int k = 0; k < K; ++k) p[j][k] = place(a, t[j] * K + k);
     }
 #pragma unroll
     for (int j = 0; j < P; ++j)
