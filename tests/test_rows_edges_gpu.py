@@ -1,0 +1,37 @@
+"""Where the row operators go wrong easily: buffers of a routing that are filled
+again, derivatives that they do not have, sorted rows that are none, more slots
+than 32 bits count comfortably."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_slots_next_to_two_to_the_31(cuda):
+    """The largest call: 2^31 - 1 slots, whose places come out as counted."""
+    import torch
+    from toy_b200 import experts as X
+    n = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[1] < 100 * 2 ** 30:
+        pytest.skip("needs a GPU of 100 GB")
+    ids = torch.zeros((n, 1), device="cuda", dtype=torch.int32)
+    ids[1::2] = 1                                   # slots of two experts in turn
+    ids[n - 1000000:n - 999990] = -1                # ten of none, near the end
+    r = X.sort(ids, 2)
+    del ids
+    ones = n // 2 - 5
+    zeros = n - n // 2 - 5
+    assert r.offsets.tolist() == [0, zeros, zeros + ones]
+    step = 1 << 27
+    for a in range(0, n, step):
+        slot = torch.arange(a, min(n, a + step), device="cuda")
+        # of the ten slots that go nowhere five are of either expert: those of this slot's parity that lie before it
+        lo = n - 1000000
+        rank = slot // 2 - ((slot - lo - (slot - lo) % 2) // 2).clamp(0, 5)
+        want = torch.where(slot % 2 == 1, zeros + rank, rank)
+        want = torch.where((slot >= n - 1000000) & (slot < n - 999990), -1, want)
+        assert torch.equal(r.pos[a:a + step, 0].long(), want)
+        on = want >= 0
+        assert torch.equal(r.order[want[on]].long(), slot[on])
+    assert (r.order[zeros + ones:] == -1).all()
+    del r, slot, rank, want, on
+    torch.cuda.empty_cache()

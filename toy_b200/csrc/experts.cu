@@ -169,9 +169,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const void* ids, int
 __global__ void __launch_bounds__(256) order_kernel(const int* pos, const int* live, int n, int* order) {
   griddep_wait();
   const int from = *live;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {   // (past n may be past 2^31)
     const int p = pos[i];
-    if (p >= 0) order[p] = i;
+    if (p >= 0) order[p] = (int)i;
     if (i >= from) order[i] = -1;
   }
 }
