@@ -474,7 +474,7 @@ int tb2_expert_sort(const tb2_expert_sort_args *args, void *stream);
  *                 either may be NULL: not wanted. d_xs may be xs itself, with
  *                 the same stride.
  * Otherwise arrays that are written overlap no others. n_tokens * n_used is
- * below 2^31. */
+ * below 2^31, d below 2^31 - 256. */
 typedef struct tb2_expert_rows_args {
   int n_tokens, n_used, d, n_rows, row_type;
   void *x;

@@ -531,8 +531,10 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
   if (a.dz) clear_rest<T, V>(a, a.dz, a.lddz);
 }
 
+// (a row's pieces are counted in 32 bits up to a group or a step of 256 past its last)
 bool shape_ok(int T, int K, int d, int rows, int type) {
-  return T >= 0 && K >= 1 && d >= 1 && rows >= 0 && row_type_ok(type) && (long long)T * K <= INT_MAX;
+  return T >= 0 && K >= 1 && d >= 1 && d <= INT_MAX - 256 && rows >= 0 && row_type_ok(type) &&
+         (long long)T * K <= INT_MAX;
 }
 bool row_ok(const void* p, long long ld, int d, int type) { return p && ld >= d && aligned(p, type_bytes(type)); }
 

@@ -60,8 +60,8 @@ def _args(r: Routing, x: torch.Tensor, xs: torch.Tensor, weights: Optional[torch
     if pos.dim() != 2 or x.dim() != 2 or xs.dim() != 2 or dtype not in ROW_TYPE or dev < 0:
         bad("rows are f32, f16 or bf16, tokens [tokens, d] and sorted rows [rows, d] on a GPU")
     shape, d, n = pos.shape, x.shape[1], xs.shape[0]
-    if d < 1 or d >= 2**31 or n >= 2**31:
-        bad("rows are of one value or more, and fewer than 2^31 of fewer than 2^31")
+    if d < 1 or d >= 2**31 - 256 or n >= 2**31:
+        bad("rows are of one value or more, and fewer than 2^31 of fewer than 2^31 - 256")
     return dev, ExpertRowsArgs(shape[0], shape[1], d, n, ROW_TYPE[dtype], x.data_ptr(),
                                rows(x, shape[0], d, dtype, dev, "tokens"), xs.data_ptr(),
                                rows(xs, n, d, dtype, dev, "sorted rows"), dense(pos, shape, I32, dev, "pos"),
