@@ -54,7 +54,9 @@ class MultiAdamW:
     """The optimizer of `params`: contiguous tensors of one type (f32, f16 or bf16) on one GPU. copies: tensors of their
     shapes, of one 16-bit type, that each step sets to the weights rounded (for weights kept in f32). state: (m, v,
     m_scale, v_scale) to go on from, lists of tensors that the optimizer then owns, the scales None for 32 bits;
-    empty moments when None. The state is in the attributes of these names."""
+    empty moments when None. The state is in the attributes of these names, in the memory that it has at first (copy_
+    into it, or set_moments, changes it); weights and copies are followed where theirs changes, and refused where they
+    no longer fit."""
 
     def __init__(self, params: Sequence[torch.Tensor], *, bits: int = 8, copies: Optional[Sequence] = None,
                  state: Optional[tuple] = None):
@@ -67,13 +69,10 @@ class MultiAdamW:
         self.device = self.params[0].device
         n = [p.numel() for p in self.params]
         self._shapes = [p.shape for p in self.params]
-        pp = [dense(p, p.shape, self.dtype, self.index, "params") for p in self.params]
         self.copies = list(copies) if copies else None
         self.copy_dtype = self.copies[0].dtype if copies else torch.bfloat16
         if copies and (len(self.copies) != len(n) or self.copy_dtype not in (torch.float16, torch.bfloat16)):
             bad("copies: one f16 or bf16 tensor per weight")
-        cp = [dense(c, s, self.copy_dtype, self.index, "copies")
-              for c, s in zip(self.copies, self._shapes)] if copies else [0] * len(n)
         blocks = [-(-k // BLOCK) for k in n]
         if state is None:
             def zeros(sizes, dtype):
@@ -103,14 +102,36 @@ class MultiAdamW:
             at.append([t.data_ptr() for t in x])
         if bits == 32:
             at += [[0] * len(n)] * 2
-        _apart([x for x in (self.params, self.copies, self.m, self.v, self.m_scale, self.v_scale) if x])
+        # (its memory stays the optimizer's whatever becomes of the tensors: a step writes there)
+        self._state = [t.untyped_storage() for x in lists for t in x]
         self._saved = any(p.requires_grad for p in self.params)   # (autograd may have saved their values)
         self._n = len(n)
         self._t = np.zeros(self._n, _COLUMNS)
-        for name, x in zip(_COLUMNS.names, (pp, [0] * self._n, *at, cp, n)):
+        for name, x in zip(("m", "v", "m_scale", "v_scale", "n"), (*at, n)):
             self._t[name] = x
+        self._place()
         if self.index not in _ready():
             prepare(self.device)
+
+    def _place(self) -> None:
+        """Notes where weights and copies are, once they are what the step takes."""
+        if len(self.params) != self._n or len(self.copies or self.params) != self._n:
+            bad("params, copies: one tensor per weight")
+        at = []
+        for x, dtype, what in ((self.params, self.dtype, "params"), (self.copies or (), self.copy_dtype, "copies")):
+            for t, shape in zip(x, self._shapes):
+                at.append(dense(t, shape, dtype, self.index, what))
+                if not at[-1] and t.numel():
+                    bad(f"{what}: tensors with memory of their own")
+        _apart([x for x in (self.params, self.copies, self.m, self.v, self.m_scale, self.v_scale) if x])
+        self._t["p"] = at[:self._n]
+        self._t["copy"] = at[self._n:] if self.copies else 0
+        self._at = at
+
+    def _follow(self) -> None:
+        """Weights and copies may have other memory at each step (`p.data = ...`, a module moved or flattened)."""
+        if list(map(_POINTER, [*self.params, *self.copies] if self.copies else self.params)) != self._at:
+            self._place()
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], hp, *, grad_scale: Optional[torch.Tensor] = None,
              seed=None) -> None:
@@ -120,6 +141,7 @@ class MultiAdamW:
         number or an i64 tensor of one value on the GPU, another for each step (the step's own number does)."""
         if len(grads) != self._n:
             bad("grads: one per weight")
+        self._follow()
         if not isinstance(hp, torch.Tensor):
             hp = torch.tensor([float(x) for x in hp], dtype=F32).to(self.device)
         hp_at = dense(hp, (7,), F32, self.index, "hp")
