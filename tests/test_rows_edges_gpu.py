@@ -35,3 +35,25 @@ def test_slots_next_to_two_to_the_31(cuda):
     assert (r.order[zeros + ones:] == -1).all()
     del r, slot, rank, want, on
     torch.cuda.empty_cache()
+
+
+def randn(*shape, **kw):
+    import torch
+    return torch.randn(shape, device="cuda", **kw)
+
+
+def test_a_routing_filled_again_is_noted(cuda):
+    """sort(out=) into buffers that a backward still needs: that backward is refused, not made with the new places."""
+    import torch
+    from toy_b200 import experts as X
+    ids = torch.randint(0, 4, (10, 2), device="cuda", dtype=torch.int32)
+    for op in ("dispatch", "combine"):
+        r = X.sort(ids, 4)
+        if op == "dispatch":
+            y = X.dispatch(randn(10, 16, requires_grad=True), r)
+        else:
+            y = X.combine(randn(20, 16, requires_grad=True), r, torch.rand((10, 2), device="cuda"))
+        again = X.sort((ids + 1) % 4, 4, out=r)
+        assert again is r
+        with pytest.raises(RuntimeError):
+            y.sum().backward()

@@ -34,7 +34,7 @@ class Routing(NamedTuple):
 
 def sort(ids: torch.Tensor, n_experts: int, *, out: Optional[Routing] = None) -> Routing:
     """The slots of ids [tokens, used] (i32 or i64; negative: no expert) sorted by expert, each expert's in slot
-    order."""
+    order. out: buffers to fill (a backward that still needs what they held is refused)."""
     dev, n, wide = ids.get_device(), ids.numel(), ids.dtype is I64
     if dev < 0 or ids.dim() != 2 or not (wide or ids.dtype is I32) or not ids.is_contiguous() or n >= 2**31 or \
             ids.shape[1] < 1:
@@ -48,6 +48,7 @@ def sort(ids: torch.Tensor, n_experts: int, *, out: Optional[Routing] = None) ->
         dense(out.offsets, (n_experts + 1,), I32, dev, "out.offsets")
         dense(out.order, (n,), I32, dev, "out.order")
         dense(out.pos, ids.shape, I32, dev, "out.pos")
+        written(*out)
     a = ExpertSortArgs(ids.data_ptr(), 8 if wide else 4, n, n_experts, out.offsets.data_ptr(), out.order.data_ptr(),
                        out.pos.data_ptr())
     call(dev, "tb2_expert_sort", a)
