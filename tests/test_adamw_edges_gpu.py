@@ -47,3 +47,41 @@ def test_weights_whose_storage_moves(cuda, bits):
     opt.step(gs, HP, seed=4)
     want.step(gs, HP, seed=4)
     assert torch.equal(a.detach(), want.params[0]) and torch.equal(b.detach(), want.params[1])
+
+
+@pytest.mark.parametrize("what", ["detached", "frozen", "copy", "later", "moments", "state"])
+def test_every_written_tensor_is_noted(cuda, what):
+    """What autograd saved of a tensor that a step (or moments(out=)) has written since is refused, not used: weights
+    given detached, weights saved for another tensor's gradient, 16-bit copies, weights that require a gradient only
+    later, f32 moments."""
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    w = ones(16, 16)
+    c = ones(16, 16, dtype=torch.bfloat16)
+    x = torch.randn((4, 16), device="cuda", requires_grad=True)
+    leaf = w.requires_grad_() if what == "detached" else w
+    opt = MultiAdamW([leaf.detach() if what == "detached" else w], copies=[c], bits=32 if what == "state" else 8)
+    out = ([ones(16, 16)], [ones(16, 16)])
+    if what == "later":
+        w.requires_grad_()
+    y = {"detached": lambda: (leaf * leaf).sum(), "frozen": lambda: (x @ w).sum(),
+         "copy": lambda: (x.bfloat16() @ c).sum(), "later": lambda: (w * w).sum(),
+         "moments": lambda: (x @ out[0][0]).sum(), "state": lambda: (x @ opt.moments()[1][0]).sum()}[what]()
+    if what == "moments":
+        opt.moments(out=out)
+    else:
+        opt.step([ones(16, 16)], HP, seed=0)
+    with pytest.raises(RuntimeError):
+        y.backward()
+
+
+def test_resting_weights_are_not_noted(cuda):
+    """A weight whose gradient is None is not written, and a backward through it stands."""
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    w, v = (ones(300).requires_grad_() for _ in range(2))
+    opt = MultiAdamW([w, v])
+    y = (w * w).sum()
+    opt.step([None, ones(300)], HP, seed=0)
+    y.backward()
+    assert (w.grad == 2).all()

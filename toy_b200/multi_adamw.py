@@ -104,7 +104,6 @@ class MultiAdamW:
             at += [[0] * len(n)] * 2
         # (its memory stays the optimizer's whatever becomes of the tensors: a step writes there)
         self._state = [t.untyped_storage() for x in lists for t in x]
-        self._saved = any(p.requires_grad for p in self.params)   # (autograd may have saved their values)
         self._n = len(n)
         self._t = np.zeros(self._n, _COLUMNS)
         for name, x in zip(("m", "v", "m_scale", "v_scale", "n"), (*at, n)):
@@ -159,11 +158,14 @@ class MultiAdamW:
             if self.bits == 8:
                 seed_at = seed.data_ptr()
         grads, shapes, t = list(grads), self._shapes, self._t
+        # what autograd may have saved: values that a forward reads, whether they require a gradient or not
+        lists = [x for x in (self.params, self.copies, *((self.m, self.v) if self.bits == 32 else ())) if x]
         if any(g is None for g in grads):
             on = [i for i, g in enumerate(grads) if g is not None]
             if not on:
                 return
             grads, shapes, t = [grads[i] for i in on], [shapes[i] for i in on], t[on]
+            lists = [[x[i] for i in on] for x in lists]
         dtype = grads[0].dtype
         if dtype not in ROW_TYPE:
             bad("grads: f32, f16 or bf16")
@@ -171,8 +173,8 @@ class MultiAdamW:
         a = AdamwMultiArgs(t.ctypes.data, len(t), ROW_TYPE[self.dtype], ROW_TYPE[dtype], ROW_TYPE[self.copy_dtype],
                            self.bits, hp_at, scale_at, seed_at)
         call(self.index, "tb2_adamw_multi", a)
-        if self._saved:
-            written(*self.params)
+        for x in lists:
+            written(*x)
 
     def _values(self, ms, vs, put: int) -> None:
         if len(ms) != self._n or len(vs) != self._n:
@@ -196,6 +198,7 @@ class MultiAdamW:
         if out is None:
             out = tuple([torch.empty(s, device=self.device, dtype=F32) for s in self._shapes] for _ in "mv")
         self._values(out[0], out[1], 0)
+        written(*out[0], *out[1])
         return out
 
     def set_moments(self, ms: Sequence[torch.Tensor], vs: Sequence[torch.Tensor]) -> None:
