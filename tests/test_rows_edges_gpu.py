@@ -57,3 +57,30 @@ def test_a_routing_filled_again_is_noted(cuda):
         assert again is r
         with pytest.raises(RuntimeError):
             y.sum().backward()
+
+
+def test_forward_mode_is_refused(cuda):
+    """A tensor with a tangent gives a result that has one, or an error; never a result without."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+    from toy_b200 import experts as X, logprobs as L
+    ids = torch.randint(0, 4, (10, 2), device="cuda", dtype=torch.int32)
+    r = X.sort(ids, 4)
+    x, z, w = randn(10, 16), randn(20, 16), torch.rand((10, 2), device="cuda")
+    t, g = torch.zeros(10, dtype=torch.int64, device="cuda"), torch.ones(10, device="cuda")
+    s = L.token_logprobs(x, t)
+    with fwd.dual_level():
+        def dual(v):
+            return fwd.make_dual(v, torch.ones_like(v))
+        for call in (lambda: L.token_logprobs(dual(x), t), lambda: L.token_logprobs_grad(dual(x), t, s, g),
+                     lambda: L.token_logprobs_grad(x, t, s, dual(g)), lambda: X.dispatch(dual(x), r),
+                     lambda: X.dispatch(dual(x), r, out=z.clone()), lambda: X.combine(dual(z), r, w),
+                     lambda: X.combine(z, r, dual(w)), lambda: X.combine(z, r, w, residual=dual(x)),
+                     lambda: X.dispatch_grad(dual(z), r), lambda: X.combine_grad(dual(x), z, r, w),
+                     lambda: X.combine_grad(x, z, r, dual(w)), lambda: X.dispatch(x, r, out=dual(z))):
+            with pytest.raises(ValueError):
+                call()
+        # without tangents all of it works at such a level too
+        L.token_logprobs_grad(x, t, L.token_logprobs(x, t), g)
+        y = X.combine(X.dispatch(x.clone().requires_grad_(), r), r, w)
+    y.sum().backward()

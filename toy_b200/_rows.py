@@ -3,6 +3,7 @@ on torch's current stream, and checks of row tensors."""
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from ._lib import check, lib
 
@@ -79,6 +80,15 @@ def rows(t: torch.Tensor, n: int, d: int, dtype, index: int, what: str) -> int:
 def written(*tensors) -> None:
     """Notes for autograd that the tensors' values have changed (what it saved of them is stale)."""
     torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
+def no_tangent(*tensors) -> None:
+    """Refuses tensors with a tangent: none of the operators has a derivative in forward mode, and a result without one
+    would stand for a derivative of zero."""
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                bad("no forward-mode derivative (the tensor has a tangent)")
 
 
 def no_captured_leaf(*tensors) -> None:

@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import ExpertRowsArgs, ExpertSortArgs
-from ._rows import F32, I32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows, written
+from ._rows import F32, I32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, no_tangent, prepare, rows, written
 
 __all__ = ["Routing", "combine", "combine_grad", "dispatch", "dispatch_grad", "prepare", "sort"]
 MAX_EXPERTS = 1024
@@ -89,6 +89,7 @@ def _no_grad(*tensors) -> None:
 
 
 def _dispatch(x, r, out):
+    no_tangent(x, out)
     fresh = out is None
     if fresh:
         out = x.new_empty((r.pos.numel(), x.shape[1] if x.dim() == 2 else 0))
@@ -100,6 +101,7 @@ def _dispatch(x, r, out):
 
 
 def _combine(z, r, weights, residual, out):
+    no_tangent(z, weights, residual, out)
     if out is None:
         out = z.new_empty((r.pos.shape[0], z.shape[1] if z.dim() == 2 else 0))
     dev, a = _args(r, out, z, weights)
@@ -149,6 +151,7 @@ def dispatch(x: torch.Tensor, r: Routing, *, out: Optional[torch.Tensor] = None)
     """The rows of x [tokens, d] at their slots' places, [tokens * used, d]: rows past the last slot's are zero, or as
     they were where `out` is given. Differentiable in x (without out)."""
     if out is None and _wanted(x):
+        no_tangent(x)
         no_captured_leaf(x)
         return _Dispatch.apply(x, *r)
     _no_grad(x, out)
@@ -171,6 +174,7 @@ def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None,
     rows of z [rows, d], choices ascending, in f32, rounded once. out may be the residual. Differentiable in z, weights
     and residual (without out)."""
     if out is None and _wanted(z, weights, residual):
+        no_tangent(z, weights, residual)
         no_captured_leaf(z, weights, residual)
         return _Combine.apply(z, weights, residual, *r)
     _no_grad(z, weights, residual, out)
@@ -180,6 +184,7 @@ def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None,
 
 
 def _combine_grad(dy, z, r, weights, out, want_z, want_w):
+    no_tangent(dy, z, weights, out)
     fresh = out is None and want_z
     if fresh:
         out = z.new_empty(z.shape)

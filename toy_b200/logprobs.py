@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import LogprobsArgs, LogprobsGradArgs
-from ._rows import F32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, prepare, rows, written
+from ._rows import F32, I64, ROW_TYPE, bad, call, dense, no_captured_leaf, no_tangent, prepare, rows, written
 
 __all__ = ["TokenLogprobs", "prepare", "token_logprobs", "token_logprobs_grad"]
 MAX_TOP = 32
@@ -90,6 +90,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float =
     """ln p of tokens [n] (i64; negative: none, 0) under softmax(scale * logits [n, vocab]), with the rows' entropy and
     the `top` (at most 32) most likely words where asked for. Logits are f32, f16 or bf16; -inf is a word of
     probability 0. Differentiable in the logits."""
+    no_tangent(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         no_captured_leaf(logits)
         return TokenLogprobs(*_Score.apply(logits, tokens, scale, entropy, top))
@@ -103,6 +104,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, result: Toke
     """The logits' gradient, [n, vocab] of their type, from the gradients of logprob [n], entropy [n] and top_logprobs
     [n, top] (f32; None: none). `result` is token_logprobs's of the same logits, tokens and scale; out may be the logits
     themselves."""
+    no_tangent(logits, grad_logprob, grad_entropy, grad_top, out)
     top = grad_top.shape[1] if grad_top is not None and grad_top.dim() == 2 else 0
     n, vocab, dev, ld = _logits(logits, tokens, scale, top)
     if torch.is_grad_enabled() and (logits.requires_grad or out is not None and out.requires_grad):
