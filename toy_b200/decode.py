@@ -72,6 +72,8 @@ class KVDecoder(_Logprobs):
     def generate(self, prompt: np.ndarray, n_new: int) -> np.ndarray:
         """Greedy continuation of [n_seq, n] prompts by n_new tokens each."""
         ids = np.asarray(prompt, np.int64).reshape(self.n_seq, -1)
+        if not ids.shape[1]:
+            raise ValueError("toy_b200: prompts of one token or more (there are no logits to continue from)")
         for i in range(ids.shape[1]):
             self.decode_step(ids[:, i], np.full(self.n_seq, i), logits=False)
         out = []
