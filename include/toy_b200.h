@@ -504,7 +504,8 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args *args, void *stream);
  * (m_scale, v_scale: [ceil(n / 256)]), the smallest power of two of 2^-100 or
  * more that brings the block within 448; m holds e4m3 codes of m / scale and v
  * of sqrt(v) / scale, the step's exact values rounded once to nearest (even)
- * or, with a seed (device memory; NULL: nearest), to the code above or below
+ * or, with a seed (device memory; NULL: nearest), the step's f32 values, within
+ * 2^-21 of the exact ones, to the code above or below
  * with the probability of their place between the two, by bits that are a
  * function of *seed and the value's place alone (give each step another seed),
  * a positive sqrt(v) never below the smallest code, a v below 2^-126 as 0. All

@@ -85,3 +85,52 @@ def test_resting_weights_are_not_noted(cuda):
     opt.step([None, ones(300)], HP, seed=0)
     y.backward()
     assert (w.grad == 2).all()
+
+
+def check_roots(opt, root):
+    """The first weight's held roots and their scales are those of the exact ones, root [blocks, 256] f64."""
+    import torch
+    top = root.amax(-1, keepdim=True)
+    e = torch.floor(torch.log2(top / 448)) - 1
+    for _ in range(3):
+        e = torch.where(top > 448 * torch.exp2(e), e + 1, e)
+    scale = torch.exp2(e.clamp(min=-100))
+    assert torch.equal(opt.v_scale[0].double(), scale[:, 0])
+    t = root / scale
+    step = torch.ldexp(torch.ones_like(t), torch.frexp(t.clamp(min=2.0 ** -6)).exponent - 4)
+    q = (t / step).round() * step
+    q = torch.where((t > 0) & (q == 0), 2.0 ** -9, q) * scale
+    assert torch.equal(opt.moments()[1][0].double(), q * q)
+
+
+def test_block_scales_at_the_border(cuda):
+    """A block's largest root at 448 times a power of two and a few f32 steps to either side of it: the scale is the
+    smallest power of two that brings the block within 448, and the small roots beside it are the exact ones'
+    roundings. From an empty state with beta2 = 0.75, so that the root is half the gradient, exactly; and on from held
+    roots, with gradients that bring the largest within some 2^-23 of the border."""
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    rows = [(e, k) for e in range(-16, 30) for k in range(-8, 9)]
+    g = torch.rand((len(rows), 256), device="cuda", generator=gen) * \
+        torch.exp2(-17 * torch.rand((len(rows), 256), device="cuda", generator=gen))
+    for i, (e, k) in enumerate(rows):
+        g[i] *= 2.0 ** e
+        g[i, 7 + i % 200] = 896.0 * 2.0 ** e * (1 + k * 2.0 ** -23 if k >= 0 else 1 + k * 2.0 ** -24)
+    opt = MultiAdamW([torch.zeros_like(g)])
+    opt.step([g], [0.0, 0.5, 0.75, 1e-8, 0.0, 1.0, 1.0])
+    check_roots(opt, g.double() / 2)
+    n = 1 << 14
+    for b2 in (0.75, 0.9, 0.999):
+        opt = MultiAdamW([torch.zeros((n, 256), device="cuda")])
+        start = torch.rand((n, 256), device="cuda", generator=gen)
+        start[:, 9] = 300 + 100 * torch.rand(n, device="cuda", generator=gen)
+        opt.set_moments([start], [start * start])
+        v0 = opt.moments()[1][0].double()
+        hp = torch.tensor([0.0, 0.5, b2, 1e-8, 0.0, 1.0, 1.0], device="cuda")
+        b2 = hp[2].double()
+        g = torch.zeros((n, 256), device="cuda")
+        near = 1 + (torch.rand(n, device="cuda", generator=gen).double() - 0.5) * 2.0 ** -21
+        g[:, 9] = (((448.0 * near) ** 2 - b2 * v0[:, 9]) / (1 - b2)).sqrt().float()
+        opt.step([g], hp)
+        check_roots(opt, (b2 * v0 + (1 - b2) * g.double() ** 2).sqrt())
