@@ -499,15 +499,15 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args *args, void *stream);
  * *grad_scale (NULL: 1), both device memory:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = (1 - alpha wd) p - alpha beta1h m / (sqrt(beta2h) sqrt(v) + eps),
- * copy = p rounded to copy_type, 1 or 30 (copy NULL: none). state_bits 32: m and v are
- * f32. state_bits 8: blocks of 256 consecutive values share an f32 scale
+ * copy = p rounded to copy_type, 1 or 30 (copy NULL: none); the root and the
+ * quotient are within 2^-22. state_bits 32: m and v are f32. state_bits 8: blocks of 256 consecutive values share an f32 scale
  * (m_scale, v_scale: [ceil(n / 256)]), the smallest power of two of 2^-100 or
  * more that brings the block within 448; m holds e4m3 codes of m / scale and v
  * of sqrt(v) / scale, the step's exact values rounded once to nearest (even)
- * or, with a seed (device memory; NULL: nearest), the step's f32 values, within
- * 2^-21 of the exact ones, to the code above or below
- * with the probability of their place between the two, by bits that are a
- * function of *seed and the value's place alone (give each step another seed),
+ * or, with a seed (device memory; NULL: nearest), the step's f32 values to the
+ * code above or below with the probability of their place between the two, by
+ * bits that are a function of *seed and the value's place alone (give each step
+ * another seed),
  * a positive sqrt(v) never below the smallest code, a v below 2^-126 as 0. All
  * zeros (scales too) is
  * an empty state. A block with a value that is not finite is NaN from then on.

@@ -134,3 +134,19 @@ def test_block_scales_at_the_border(cuda):
         g[:, 9] = (((448.0 * near) ** 2 - b2 * v0[:, 9]) / (1 - b2)).sqrt().float()
         opt.step([g], hp)
         check_roots(opt, (b2 * v0 + (1 - b2) * g.double() ** 2).sqrt())
+
+
+def test_second_moments_below_the_normal_numbers(cuda):
+    """f32 moments: roots of second moments below 2^-126 count, as in the framework's other AdamW."""
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    g = torch.logspace(-22, -17, 1000, device="cuda")
+    p = [torch.zeros(1000, device="cuda")]
+    opt = MultiAdamW(p, bits=32)
+    opt.step([g], [1.0, 0.9, 0.5, 1e-30, 0.0, 1.0, 1.0])
+    m, v = (x[0].double() for x in opt.moments())
+    assert (v < 2.0 ** -126).any() and (v[v > 0] > 0).any()
+    want = -m / (v.sqrt() + 1e-30)
+    on = v > 0
+    # the root and the sum within half a step each, the quotient and the difference too; eps itself rounded
+    assert ((p[0].double() - want)[on].abs() <= 8 * 2.0 ** -24 * want[on].abs()).all()

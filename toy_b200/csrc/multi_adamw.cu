@@ -96,9 +96,14 @@ __device__ __noinline__ unsigned e4m3_of(double t) {
   return __nv_cvt_float_to_fp8((float)q, __NV_SATFINITE, __NV_E4M3);
 }
 
-__device__ __forceinline__ float sqrt_near(float x) {   // within 2^-23; below 2^-126: 0
+// Within 2^-23. FTZ: a number below 2^-126 is 0, which 8-bit moments allow; second moments in f32 go on below that, and
+// their roots are far above it. (With f32 moments the correctly rounded root and quotient took 623 us instead of 562 for
+// 135M weights: their rare paths cost registers.)
+template <bool FTZ>
+__device__ __forceinline__ float sqrt_near(float x) {
   float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  if (FTZ) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  else asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 __device__ __forceinline__ float inverse_near(float x) {   // within 2^-23
@@ -221,7 +226,7 @@ __device__ __forceinline__ void step8(const Hyper& h, float (&p)[8], const float
       m[e] = fmaf(m[e], h.b1, g[e] * h.dg);
       v = fmaf(r[e], h.b2, gg * gg * h.d2);
     }
-    const float root = sqrt_near(v);
+    const float root = sqrt_near<BITS == 8>(v);
     p[e] = fmaf(-h.c1 * m[e], inverse_near(fmaf(root, h.c2, h.eps)), p[e] * h.keep);
     r[e] = BITS == 8 ? root : v;
   }

@@ -2,7 +2,7 @@
 bits: tb2_adamw_multi (include/toy_b200.h).
 
 The step is the framework's own (opt_step_adamw with the 7-slot row of
-`toy_b200.AdamW.hp`). With 8 bits a weight's two moments take 2.03 bytes instead
+`toy_b200.AdamW.hp`), its root and quotient within 2^-22. With 8 bits a weight's two moments take 2.03 bytes instead
 of 8: blocks of 256 values share a power of two, m is held as e4m3 and v as the
 e4m3 of its square root, each the step's value rounded once.
 
