@@ -150,3 +150,23 @@ def test_second_moments_below_the_normal_numbers(cuda):
     on = v > 0
     # the root and the sum within half a step each, the quotient and the difference too; eps itself rounded
     assert ((p[0].double() - want)[on].abs() <= 8 * 2.0 ** -24 * want[on].abs()).all()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_moments_lists_that_do_not_fit(cuda, bits):
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW
+    opt = MultiAdamW([ones(9), ones(2, 3)], bits=bits)
+
+    def both():
+        return [ones(9), ones(2, 3)]
+    for ms, vs in ((both()[:1], both()), (both(), both()[:1]), (both() + [ones(1)], both()),
+                   ([ones(9), ones(3)], both()), (both(), [ones(9), ones(2, 4)]), (both(), [ones(1), ones(2, 3)])):
+        with pytest.raises(ValueError):
+            opt.set_moments(ms, vs)
+        with pytest.raises(ValueError):
+            opt.moments(out=(ms, vs))
+    assert all((x == 0).all() for y in opt.moments() for x in y)       # nothing was set
+    opt.set_moments(both(), both())
+    got = opt.moments(out=(both(), both()))
+    assert all((x == 1).all() for y in got for x in y)

@@ -184,6 +184,12 @@ class MultiAdamW:
         x["copy"] = _pointers(vs, self._shapes, F32, self.index, "moments")
         call(self.index, "tb2_adamw_moments", x.ctypes.data, self._n, put)
 
+    def _whole(self, ms, vs) -> None:
+        """Refuses lists that are not a tensor of its size for every weight."""
+        for x in (ms, vs):
+            if [t.numel() for t in x] != [s.numel() for s in self._shapes]:
+                bad("moments: one tensor of each kind per weight, of its size")
+
     def moments(self, *, out: Optional[tuple] = None) -> tuple:
         """(m, v): the values of the moments, lists of f32 tensors of the weights' shapes (out: such lists to fill; in
         32 bits without out the state itself)."""
@@ -191,6 +197,7 @@ class MultiAdamW:
             if out is None:
                 return ([t.view(s) for t, s in zip(self.m, self._shapes)],
                         [t.view(s) for t, s in zip(self.v, self._shapes)])
+            self._whole(*out)
             for to, x in zip(out, (self.m, self.v)):
                 for a, b in zip(to, x):
                     a.copy_(b.view(a.shape))
@@ -204,6 +211,8 @@ class MultiAdamW:
     def set_moments(self, ms: Sequence[torch.Tensor], vs: Sequence[torch.Tensor]) -> None:
         """The moments set to these values (f32, of the weights' shapes), rounded to the state's bits."""
         if self.bits == 32:
+            ms, vs = list(ms), list(vs)
+            self._whole(ms, vs)
             for to, x in zip((self.m, self.v), (ms, vs)):
                 for a, b in zip(to, x):
                     a.copy_(b.reshape(a.shape))
