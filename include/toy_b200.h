@@ -462,7 +462,8 @@ int tb2_expert_sort(const tb2_expert_sort_args *args, void *stream);
  * are not read, and not written either unless n_sorted (device memory, the
  * last of the offsets; or NULL) is given: dispatch and combine_grad then set
  * rows *n_sorted .. n_rows of their result to 0. A pos of n_rows or more is left out and
- * tb2_device_error() reports 0x5103; places are distinct.
+ * tb2_device_error() reports 0x5103; places are distinct. With n_rows 0 xs may
+ * be NULL.
  *   dispatch:     xs[pos[t][k]] = x[t].
  *   combine:      x[t] = residual[t] + sum_k weights[t][k] xs[pos[t][k]], k
  *                 ascending (residual NULL: 0; weights NULL: 1, which is the

@@ -84,3 +84,24 @@ def test_forward_mode_is_refused(cuda):
         L.token_logprobs_grad(x, t, L.token_logprobs(x, t), g)
         y = X.combine(X.dispatch(x.clone().requires_grad_(), r), r, w)
     y.sum().backward()
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 9])
+def test_no_sorted_rows(cuda, K):
+    """Tokens of which none goes to an expert, with sorted rows cut to those there are: none."""
+    import torch
+    from toy_b200 import experts as X
+    from toy_b200._lib import lib
+    ids = torch.full((6, K), -1, device="cuda", dtype=torch.int32)
+    r = X.sort(ids, 4)
+    for d in (32, 33):
+        x, z, w = randn(6, d), randn(6 * K, d)[:0], torch.rand((6, K), device="cuda")
+        assert torch.equal(X.combine(z, r, w, residual=x), x)
+        assert (X.combine(z, r) == 0).all() and (X.dispatch_grad(z, r) == 0).all()
+        dz, dw = X.combine_grad(x, z, r, w)
+        assert dz.shape == (0, d) and (dw == 0).all()
+        assert X.dispatch(x, r, out=z) is z
+        a, b, c = x.clone().requires_grad_(), z.clone().requires_grad_(), w.clone().requires_grad_()
+        X.combine(b, r, c, residual=a).sum().backward()
+        assert (a.grad == 1).all() and b.grad.shape == (0, d) and (c.grad == 0).all()
+    assert lib().tb2_device_error() == 0

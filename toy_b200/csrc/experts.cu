@@ -537,6 +537,8 @@ bool shape_ok(int T, int K, int d, int rows, int type) {
          (long long)T * K <= INT_MAX;
 }
 bool row_ok(const void* p, long long ld, int d, int type) { return p && ld >= d && aligned(p, type_bytes(type)); }
+// Sorted rows; where there are none they have no address either (every slot is of no expert).
+bool sorted_ok(const tb2_expert_rows_args& a) { return a.n_rows == 0 || row_ok(a.xs, a.ldxs, a.d, a.row_type); }
 
 // The kernel's shared-memory limit on the current device.
 template <int BITS>
@@ -697,7 +699,7 @@ int tb2_expert_dispatch(const tb2_expert_rows_args* a, void* stream) {
   using namespace tb2;
   if (!a || !shape_ok(a->n_tokens, a->n_used, a->d, a->n_rows, a->row_type)) return -1;
   if (a->n_tokens == 0) return 0;
-  if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !row_ok(a->xs, a->ldxs, a->d, a->row_type)) return -1;
+  if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !sorted_ok(*a)) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->n_sorted})) return -1;
   RowsArgs k = {};
   k.x = a->x; k.ldx = a->ldx; k.y = a->xs; k.ldy = a->ldxs; k.pos = a->pos; k.n_sorted = a->n_sorted;
@@ -712,7 +714,7 @@ int tb2_expert_combine(const tb2_expert_rows_args* a, void* stream) {
   using namespace tb2;
   if (!a || !shape_ok(a->n_tokens, a->n_used, a->d, a->n_rows, a->row_type)) return -1;
   if (a->n_tokens == 0) return 0;
-  if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !row_ok(a->xs, a->ldxs, a->d, a->row_type)) return -1;
+  if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !sorted_ok(*a)) return -1;
   if (a->residual && !row_ok(a->residual, a->ldr, a->d, a->row_type)) return -1;
   if (a->residual == a->x && a->ldr != a->ldx && a->n_tokens > 1) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->weights})) return -1;
@@ -730,7 +732,7 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args* a, void* stream) {
   using namespace tb2;
   if (!a || !shape_ok(a->n_tokens, a->n_used, a->d, a->n_rows, a->row_type)) return -1;
   if (a->n_tokens == 0) return 0;
-  if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !row_ok(a->xs, a->ldxs, a->d, a->row_type)) return -1;
+  if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !sorted_ok(*a)) return -1;
   if (a->d_xs && !row_ok(a->d_xs, a->ldd, a->d, a->row_type)) return -1;
   if (a->d_xs == a->xs && a->ldd != a->ldxs && a->n_rows > 1) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->weights, a->d_weights, a->n_sorted})) return -1;
