@@ -463,7 +463,7 @@ int tb2_expert_sort(const tb2_expert_sort_args *args, void *stream);
  * last of the offsets; or NULL) is given: dispatch and combine_grad then set
  * rows *n_sorted .. n_rows of their result to 0. A pos of n_rows or more is left out and
  * tb2_device_error() reports 0x5103; places are distinct. With n_rows 0 xs may
- * be NULL.
+ * be NULL; with n_tokens 0 nothing is written, rows to be cleared neither.
  *   dispatch:     xs[pos[t][k]] = x[t].
  *   combine:      x[t] = residual[t] + sum_k weights[t][k] xs[pos[t][k]], k
  *                 ascending (residual NULL: 0; weights NULL: 1, which is the

@@ -19,3 +19,11 @@ def test_rows_of_almost_two_to_the_31_values():
         a = ExpertRowsArgs(**ok, d=d, x=P, ldx=d, xs=P + (1 << 40), ldxs=d)
         for f in ("tb2_expert_dispatch", "tb2_expert_combine", "tb2_expert_combine_grad"):
             assert getattr(lib(), f)(C.byref(a), None) == -1, (d, f)
+
+
+def test_no_tokens_write_nothing():
+    """A call without tokens ends before it looks at the rows: those that would be cleared stay."""
+    from toy_b200._lib import ExpertRowsArgs
+    a = ExpertRowsArgs(n_tokens=0, n_used=2, d=16, n_rows=8, row_type=0, xs=P, ldxs=16, d_xs=P, ldd=16, n_sorted=P)
+    for f in ("tb2_expert_dispatch", "tb2_expert_combine", "tb2_expert_combine_grad"):
+        assert getattr(lib(), f)(C.byref(a), None) == 0        # (no GPU here: nothing was launched)
