@@ -105,3 +105,32 @@ def test_no_sorted_rows(cuda, K):
         X.combine(b, r, c, residual=a).sum().backward()
         assert (a.grad == 1).all() and b.grad.shape == (0, d) and (c.grad == 0).all()
     assert lib().tb2_device_error() == 0
+
+
+def test_results_over_their_operands(cuda):
+    """Refused with ValueError where a result would lie over what it is made from; rows between each other's are not."""
+    import torch
+    from toy_b200 import experts as X, logprobs as L
+    ids = torch.randperm(40, device="cuda").remainder(4).int()[:, None]
+    r = X.sort(ids, 4)
+    order = r.order.long()
+    buf = randn(40, 64)
+    a, b = buf[:, :32], buf[:, 32:]
+    x = a.clone()
+    t, g = torch.zeros(39, dtype=torch.int64, device="cuda"), torch.ones(39, device="cuda")
+    s = L.token_logprobs(a[1:], t)
+    for bad in (lambda: X.dispatch(a, r, out=a), lambda: X.dispatch(a, r, out=buf[:, 31:63]),
+                lambda: X.combine(a, r, out=a), lambda: X.dispatch_grad(a, r, out=buf[:, 16:48]),
+                lambda: X.combine(b.clone(), r, residual=a, out=buf[:, 1:33]),
+                lambda: X.combine_grad(a, b, r, out=a), lambda: X.combine_grad(x, b, r, out=buf[:, 31:63]),
+                lambda: L.token_logprobs_grad(a[1:], t, s, g, out=a[:39])):
+        was = buf.clone()
+        with pytest.raises(ValueError):
+            bad()
+        assert torch.equal(buf, was)
+    X.dispatch(a, r, out=b)
+    assert torch.equal(b, x[order]) and torch.equal(a, x)
+    X.combine(a, r, out=b)
+    assert torch.equal(b[order], x) and torch.equal(a, x)
+    want = L.token_logprobs_grad(a[1:].clone(), t, s, g)
+    assert torch.equal(L.token_logprobs_grad(a[1:], t, s, g, out=b[1:]), want)

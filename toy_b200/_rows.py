@@ -50,6 +50,8 @@ def call(index: int, what: str, *args) -> None:
     else:
         with torch.cuda.device(index):
             rc = f(*args, _raw_stream(index))
+    if rc == -1:
+        bad(f"{what}: arguments that do not fit (a result that lies over an operand, but for those that may)")
     if rc:
         check(rc, what)
 

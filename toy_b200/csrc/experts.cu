@@ -537,6 +537,11 @@ bool shape_ok(int T, int K, int d, int rows, int type) {
          (long long)T * K <= INT_MAX;
 }
 bool row_ok(const void* p, long long ld, int d, int type) { return p && ld >= d && aligned(p, type_bytes(type)); }
+// A result's rows that lie over an operand's and are not that operand in place: other threads read what it writes.
+bool over(const tb2_expert_rows_args& a, const void* p, long long ld, int n, const void* q, long long ldq, int m) {
+  return !rows_apart(p, ld, n, q, ldq, m, a.d, a.row_type);
+}
+
 // Sorted rows; where there are none they have no address either (every slot is of no expert).
 bool sorted_ok(const tb2_expert_rows_args& a) { return a.n_rows == 0 || row_ok(a.xs, a.ldxs, a.d, a.row_type); }
 
@@ -701,6 +706,7 @@ int tb2_expert_dispatch(const tb2_expert_rows_args* a, void* stream) {
   if (a->n_tokens == 0) return 0;
   if (!row_ok(a->x, a->ldx, a->d, a->row_type) || !sorted_ok(*a)) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->n_sorted})) return -1;
+  if (over(*a, a->xs, a->ldxs, a->n_rows, a->x, a->ldx, a->n_tokens)) return -1;
   RowsArgs k = {};
   k.x = a->x; k.ldx = a->ldx; k.y = a->xs; k.ldy = a->ldxs; k.pos = a->pos; k.n_sorted = a->n_sorted;
   k.T = a->n_tokens; k.K = a->n_used; k.d = a->d; k.rows = a->n_rows;
@@ -718,6 +724,8 @@ int tb2_expert_combine(const tb2_expert_rows_args* a, void* stream) {
   if (a->residual && !row_ok(a->residual, a->ldr, a->d, a->row_type)) return -1;
   if (a->residual == a->x && a->ldr != a->ldx && a->n_tokens > 1) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->weights})) return -1;
+  if (over(*a, a->x, a->ldx, a->n_tokens, a->xs, a->ldxs, a->n_rows)) return -1;
+  if (a->residual != a->x && over(*a, a->x, a->ldx, a->n_tokens, a->residual, a->ldr, a->n_tokens)) return -1;
   RowsArgs k = {};
   k.z = a->xs; k.ldz = a->ldxs; k.y = a->x; k.ldy = a->ldx; k.res = a->residual; k.ldr = a->ldr; k.pos = a->pos;
   k.w = a->weights;
@@ -736,6 +744,8 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args* a, void* stream) {
   if (a->d_xs && !row_ok(a->d_xs, a->ldd, a->d, a->row_type)) return -1;
   if (a->d_xs == a->xs && a->ldd != a->ldxs && a->n_rows > 1) return -1;
   if (!a->pos || !all_aligned(4, {a->pos, a->weights, a->d_weights, a->n_sorted})) return -1;
+  if (over(*a, a->d_xs, a->ldd, a->n_rows, a->x, a->ldx, a->n_tokens)) return -1;
+  if (a->d_xs != a->xs && over(*a, a->d_xs, a->ldd, a->n_rows, a->xs, a->ldxs, a->n_rows)) return -1;
   RowsArgs k = {};
   k.x = a->x; k.ldx = a->ldx; k.z = a->xs; k.ldz = a->ldxs; k.dz = a->d_xs; k.lddz = a->ldd; k.pos = a->pos;
   k.w = a->weights; k.dw = a->d_weights; k.n_sorted = a->n_sorted;

@@ -880,6 +880,9 @@ int tb2_logprobs_grad(const tb2_logprobs_grad_args* a, void* stream) {
   if (!rows_ok(a->ld, a->vocab, a->logits, a->row_type) || !scale_ok(a->scale)) return -1;
   if (!rows_ok(a->ldd, a->vocab, a->d_logits, a->row_type)) return -1;
   if (a->d_logits == a->logits && a->ldd != a->ld && a->n_rows > 1) return -1;
+  if (a->d_logits != a->logits &&
+      !rows_apart(a->d_logits, a->ldd, a->n_rows, a->logits, a->ld, a->n_rows, a->vocab, a->row_type))
+    return -1;
   if (!a->tokens || !a->stats || a->top < 0 || a->top > kMaxTop || a->top > a->vocab) return -1;
   if (a->top && (!a->top_ids || !a->g_top)) return -1;
   if (a->g_entropy && !a->entropy) return -1;

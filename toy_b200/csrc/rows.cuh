@@ -48,6 +48,20 @@ struct Piece {
   }
 };
 
+// Whether na rows at a and nb rows at b, of d values each, share no memory. Rows may lie between one another's; of unlike
+// strides that is left to the caller.
+inline bool rows_apart(const void* a, long long lda, long long na, const void* b, long long ldb, long long nb, int d,
+                       int type) {
+  if (!a || !b || na < 1 || nb < 1) return true;
+  typedef unsigned long long u64;
+  const u64 e = type_bytes(type), row = d * e, x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  const u64 la = (na > 1 ? lda : nb > 1 ? ldb : d) * e, lb = (nb > 1 ? ldb : na > 1 ? lda : d) * e;
+  if (x + (na - 1) * la + row <= y || y + (nb - 1) * lb + row <= x) return true;
+  if (la != lb) return true;
+  const u64 off = x < y ? (y - x) % la : (x - y) % la;   // where the later one's rows begin in the earlier one's
+  return off >= row && la - off >= row;
+}
+
 template <class F>
 int by_row_type(int type, F&& f) {
   switch (type) {
