@@ -134,3 +134,23 @@ def test_results_over_their_operands(cuda):
     assert torch.equal(b[order], x) and torch.equal(a, x)
     want = L.token_logprobs_grad(a[1:].clone(), t, s, g)
     assert torch.equal(L.token_logprobs_grad(a[1:], t, s, g, out=b[1:]), want)
+
+
+def test_outputs_that_do_not_fit_are_not_noted(cuda):
+    """A refused call has written nothing, and what autograd saved of its `out` stands."""
+    import torch
+    from toy_b200 import experts as X, logprobs as L
+    ids = torch.randint(0, 4, (10, 2), device="cuda", dtype=torch.int32)
+    r = X.sort(ids, 4)
+    x, z = randn(10, 16), randn(20, 16)
+    t, g = torch.zeros(10, dtype=torch.int64, device="cuda"), torch.ones(10, device="cuda")
+    s = L.token_logprobs(x, t)
+    for call in (lambda o: X.dispatch(x, r, out=o), lambda o: X.dispatch_grad(z, r, out=o),
+                 lambda o: X.combine(z, r, out=o), lambda o: X.combine_grad(x, z, r, out=o),
+                 lambda o: L.token_logprobs_grad(x, t, s, g, out=o)):
+        out = randn(3, 3)
+        a = torch.ones((3, 3), device="cuda", requires_grad=True)
+        y = (a * out).sum()
+        with pytest.raises(ValueError):
+            call(out)
+        y.backward()

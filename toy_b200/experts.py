@@ -88,6 +88,13 @@ def _no_grad(*tensors) -> None:
         bad("no gradient passes through this call (use it under torch.no_grad())")
 
 
+def _noted(out: Optional[torch.Tensor], result):
+    """The result of a call that has written out: autograd is told, of a call that was not refused."""
+    if out is not None:
+        written(out)
+    return result
+
+
 def _dispatch(x, r, out):
     no_tangent(x, out)
     fresh = out is None
@@ -155,17 +162,13 @@ def dispatch(x: torch.Tensor, r: Routing, *, out: Optional[torch.Tensor] = None)
         no_captured_leaf(x)
         return _Dispatch.apply(x, *r)
     _no_grad(x, out)
-    if out is not None:
-        written(out)
-    return _dispatch(x, r, out)
+    return _noted(out, _dispatch(x, r, out))
 
 
 def dispatch_grad(dxs: torch.Tensor, r: Routing, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient of `dispatch`: each token's sum of its slots' rows of dxs, choices ascending."""
     _no_grad(dxs, out)
-    if out is not None:
-        written(out)
-    return _combine(dxs, r, None, None, out)
+    return _noted(out, _combine(dxs, r, None, None, out))
 
 
 def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None, *,
@@ -178,9 +181,7 @@ def combine(z: torch.Tensor, r: Routing, weights: Optional[torch.Tensor] = None,
         no_captured_leaf(z, weights, residual)
         return _Combine.apply(z, weights, residual, *r)
     _no_grad(z, weights, residual, out)
-    if out is not None:
-        written(out)
-    return _combine(z, r, weights, residual, out)
+    return _noted(out, _combine(z, r, weights, residual, out))
 
 
 def _combine_grad(dy, z, r, weights, out, want_z, want_w):
@@ -208,6 +209,4 @@ def combine_grad(dy: torch.Tensor, z: torch.Tensor, r: Routing, weights: Optiona
     """(dz, dw) of `combine`: the slots' rows of dz are weights * dy, dw = <dy, z> (0 for slots of no expert). Rows of
     dz that no slot has are zero, or as they were where `out` is given; out may be z."""
     _no_grad(dy, z, weights, out)
-    if out is not None:
-        written(out)
-    return _combine_grad(dy, z, r, weights, out, True, True)
+    return _noted(out, _combine_grad(dy, z, r, weights, out, True, True))

@@ -115,14 +115,15 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, result: Toke
         bad("result: with the entropy and the alternatives that have a gradient")
     ent = dense(result.entropy, (n,), F32, dev, "result.entropy") if grad_entropy is not None else None
     ids = dense(result.top_ids, (n, top), I64, dev, "result.top_ids") if top else None
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty((n, vocab), device=logits.device, dtype=logits.dtype)
-    else:
-        written(out)
     ldd = rows(out, n, vocab, logits.dtype, dev, "out")
     if n:
         a = LogprobsGradArgs(n, vocab, ROW_TYPE[logits.dtype], logits.data_ptr(), ld, scale, tokens.data_ptr(),
                              dense(result.stats, (n, 2), F32, dev, "result.stats"), ent, g[0], g[1], top,
                              g[2] if top else None, ids, out.data_ptr(), ldd)
         call(dev, "tb2_logprobs_grad", a)
+    if not fresh:
+        written(out)
     return out
