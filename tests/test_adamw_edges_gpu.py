@@ -170,3 +170,28 @@ def test_moments_lists_that_do_not_fit(cuda, bits):
     opt.set_moments(both(), both())
     got = opt.moments(out=(both(), both()))
     assert all((x == 1).all() for y in got for x in y)
+
+
+def test_a_captured_step_takes_its_seed_as_a_tensor(cuda):
+    """A number would be the same in each replay, and so the random bits."""
+    import torch
+    from toy_b200.multi_adamw import MultiAdamW, prepare
+    prepare()
+    opt, g, hp = MultiAdamW([ones(300)]), [ones(300)], torch.tensor(HP, device="cuda")
+    seed = torch.zeros(1, device="cuda", dtype=torch.int64)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device="cuda")
+        with pytest.raises(ValueError):
+            opt.step(g, hp, seed=3)
+        with pytest.raises(ValueError):
+            opt.step(g, HP, seed=seed)
+        opt.step(g, hp, seed=seed)
+    want = MultiAdamW([ones(300)])
+    for k in range(3):
+        seed.fill_(k)
+        graph.replay()
+        want.step(g, HP, seed=k)
+        assert all(torch.equal(a, b) for a, b in zip(opt.m_scale + opt.params, want.m_scale + want.params))
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(opt.m + opt.v,
+                                                                                         want.m + want.v))

@@ -137,10 +137,14 @@ class MultiAdamW:
         """One step on the gradients (f32, f16 or bf16, all of one type, of the weights' shapes; None: the weight and
         its moments stay). hp: the row of AdamW.hp, as an f32 [7] tensor on the GPU or as numbers; grad_scale: an f32
         tensor of one value on the GPU that every gradient is multiplied by; seed: 8-bit moments rounded at random, a
-        number or an i64 tensor of one value on the GPU, another for each step (the step's own number does)."""
+        number or an i64 tensor of one value on the GPU, another for each step (the step's own number does). A step that
+        is captured into a CUDA graph takes both as tensors."""
         if len(grads) != self._n:
             bad("grads: one per weight")
         self._follow()
+        numbers = not isinstance(hp, torch.Tensor) or self.bits == 8 and not isinstance(seed, (torch.Tensor, type(None)))
+        if numbers and torch.cuda.is_current_stream_capturing():
+            bad("a captured step takes hp and seed as tensors on the GPU (numbers would stay those of the capture)")
         if not isinstance(hp, torch.Tensor):
             hp = torch.tensor([float(x) for x in hp], dtype=F32).to(self.device)
         hp_at = dense(hp, (7,), F32, self.index, "hp")
