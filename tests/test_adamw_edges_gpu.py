@@ -195,3 +195,18 @@ def test_a_captured_step_takes_its_seed_as_a_tensor(cuda):
         assert all(torch.equal(a, b) for a, b in zip(opt.m_scale + opt.params, want.m_scale + want.params))
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(opt.m + opt.v,
                                                                                          want.m + want.v))
+
+
+def test_steps_to_nearest_are_warned_of(cuda):
+    """8-bit moments do not follow small steps without a seed: said once for each optimizer, and nowhere else."""
+    import warnings
+    from toy_b200.multi_adamw import MultiAdamW
+
+    def heard(*steps, **kw):
+        opt = MultiAdamW([ones(300)], **kw)
+        with warnings.catch_warnings(record=True) as w:
+            warnings.simplefilter("always")
+            for seed in steps:
+                opt.step([ones(300)], HP, seed=seed)
+        return len(w)
+    assert heard(None, None, None) == 1 and heard(1, 2) == 0 and heard(None, None, bits=32) == 0

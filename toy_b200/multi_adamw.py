@@ -2,9 +2,10 @@
 bits: tb2_adamw_multi (include/toy_b200.h).
 
 The step is the framework's own (opt_step_adamw with the 7-slot row of
-`toy_b200.AdamW.hp`), its root and quotient within 2^-22. With 8 bits a weight's two moments take 2.03 bytes instead
-of 8: blocks of 256 values share a power of two, m is held as e4m3 and v as the
-e4m3 of its square root, each the step's value rounded once.
+`toy_b200.AdamW.hp`), its root and quotient within 2^-22. With 8 bits a weight's
+two moments take 2.03 bytes instead of 8: blocks of 256 values share a power of
+two, m is held as e4m3 and v as the e4m3 of its square root, each the step's
+value rounded once.
 
 Train with a seed. A step moves v by a thousandth of its way (beta2 = 0.999), and
 the nearest of codes that lie 6 to 12 % apart is the one it had: without a seed v
@@ -16,6 +17,7 @@ for moments that a step moves by more than that.)
 from __future__ import annotations
 
 import ctypes as C
+import warnings
 from operator import attrgetter
 from typing import Optional, Sequence
 
@@ -105,6 +107,7 @@ class MultiAdamW:
         # (its memory stays the optimizer's whatever becomes of the tensors: a step writes there)
         self._state = [t.untyped_storage() for x in lists for t in x]
         self._n = len(n)
+        self._warned = False
         self._t = np.zeros(self._n, _COLUMNS)
         for name, x in zip(("m", "v", "m_scale", "v_scale", "n"), (*at, n)):
             self._t[name] = x
@@ -137,8 +140,9 @@ class MultiAdamW:
         """One step on the gradients (f32, f16 or bf16, all of one type, of the weights' shapes; None: the weight and
         its moments stay). hp: the row of AdamW.hp, as an f32 [7] tensor on the GPU or as numbers; grad_scale: an f32
         tensor of one value on the GPU that every gradient is multiplied by; seed: 8-bit moments rounded at random, a
-        number or an i64 tensor of one value on the GPU, another for each step (the step's own number does). A step that
-        is captured into a CUDA graph takes both as tensors."""
+        number or an i64 tensor of one value on the GPU, another for each step (the step's own number does; without one
+        they are rounded to nearest, which an optimizer's first such step warns of). A step that is captured into a CUDA
+        graph takes both as tensors."""
         if len(grads) != self._n:
             bad("grads: one per weight")
         self._follow()
@@ -174,6 +178,10 @@ class MultiAdamW:
         if dtype not in ROW_TYPE:
             bad("grads: f32, f16 or bf16")
         t["g"] = _pointers(grads, shapes, dtype, self.index, "grads")
+        if seed is None and self.bits == 8 and not self._warned:
+            self._warned = True
+            warnings.warn("toy_b200: 8-bit moments rounded to nearest stop following the gradients after some steps; "
+                          "train with MultiAdamW.step(..., seed=)", stacklevel=2)
         a = AdamwMultiArgs(t.ctypes.data, len(t), ROW_TYPE[self.dtype], ROW_TYPE[dtype], ROW_TYPE[self.copy_dtype],
                            self.bits, hp_at, scale_at, seed_at)
         call(self.index, "tb2_adamw_multi", a)
