@@ -1647,7 +1647,7 @@ int LlamaEngine::enqueue_forward() {
   const float scale = 1.0f / std::sqrt((float)dh);
   const bool lora = c.mode == 1;
   const Param& E = P("token_embd.weight");
-  forward_made_ = true;
+  forward_made_ = false;   // (until its logits are on their way)
   side_ = wst_ && !profiling_;   // the forward's side work: ring fills one block ahead
   side_forked_ = false;
   sev_next_ = 0;
@@ -1802,6 +1802,7 @@ int LlamaEngine::enqueue_forward() {
     KL(launch_cross_entropy(logits_, labels_, labels_dense_, loss_rows_, dlog_, N, V, stream_));
   }
   KL(launch_loss_reduce(loss_rows_, N, loss_, stream_));
+  forward_made_ = true;
   return 0;
 }
 
