@@ -398,7 +398,9 @@ int tb2_rows_prepare(void);
  * {0, -inf}, log probabilities -inf, entropy 0. A NaN or +inf in a row makes
  * its probabilities and entropy NaN; NaN counts as the largest logit. A token
  * of vocab or more gives NaN and tb2_device_error() reports 0x5101. scale is
- * between 2^-126 and 2^126. tokens, stats and top_ids are on 8-byte
+ * between 2^-126 and 2^126; below 2^-64 differences of logits past f32's range
+ * count as infinite, and an entropy whose vocab / scale is past it is not
+ * finite. tokens, stats and top_ids are on 8-byte
  * boundaries. */
 typedef struct tb2_logprobs_args {
   int n_rows, vocab, row_type;
@@ -442,7 +444,8 @@ typedef struct tb2_logprobs_grad_args {
 int tb2_logprobs_grad(const tb2_logprobs_grad_args *args, void *stream);
 
 /* Slots sorted by expert. Slot i = token * n_used + choice goes to expert
- * ids[i] (id_bytes 4 or 8: int or long long), or nowhere when that is negative.
+ * ids[i] (id_bytes 4 or 8: int or long long), or nowhere when that is negative;
+ * the arrays share no memory.
  * order lists the slots of expert 0, of expert 1, ..., each expert's in slot
  * order, and -1 after the last; offsets[e] is where expert e's begin, and
  * offsets[n_experts] the number of sorted slots; pos[i] is slot i's place in

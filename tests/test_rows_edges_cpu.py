@@ -49,3 +49,15 @@ def test_results_over_their_operands():
     grad = dict(n_rows=4, vocab=d, row_type=0, logits=P, ld=64, scale=1.0, tokens=far, stats=far, g_logprob=far, ldd=64)
     for dl in (P + e, P + row, P - row, P + (d - 1) * e, P - (d - 1) * e):
         assert lib().tb2_logprobs_grad(C.byref(LogprobsGradArgs(**grad, d_logits=dl)), None) == -1, dl - P
+
+
+def test_a_sort_over_its_ids():
+    """Places are scattered while ids are still read: buffers that share memory are refused."""
+    from toy_b200._lib import ExpertSortArgs
+    n = 1000
+    ok = dict(ids=P, id_bytes=8, n_slots=n, n_experts=4, offsets=P + 8 * n, order=P + 8 * n + 20,
+              pos=P + 12 * n + 20)
+    for k, v in (("order", P), ("pos", P + 8 * n - 4), ("offsets", P + 8 * n - 4), ("pos", P + 12 * n + 16),
+                 ("order", P + 8 * n + 16), ("pos", P + 8 * n + 20), ("ids", P + 16 * n + 16)):
+        assert lib().tb2_expert_sort(C.byref(ExpertSortArgs(**{**ok, k: v})), None) == -1, (k, v - P)
+    assert lib().tb2_expert_sort(C.byref(ExpertSortArgs(**ok)), None) != -1       # (no GPU: it gets as far as that)

@@ -695,6 +695,15 @@ int tb2_expert_sort(const tb2_expert_sort_args* a, void* stream) {
     return -1;
   if (!a->offsets || (a->n_slots && (!a->ids || !a->order || !a->pos))) return -1;
   if (!aligned(a->ids, a->id_bytes) || !all_aligned(4, {a->offsets, a->order, a->pos})) return -1;
+  // (places are scattered while other ids are still read)
+  const long long n = a->n_slots;
+  const std::pair<const void*, long long> parts[4] = {
+      {a->ids, n * a->id_bytes}, {a->offsets, 4LL * (a->n_experts + 1)}, {a->order, 4 * n}, {a->pos, 4 * n}};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j) {
+      const char *p = static_cast<const char*>(parts[i].first), *q = static_cast<const char*>(parts[j].first);
+      if (parts[i].second && parts[j].second && p < q + parts[j].second && q < p + parts[i].second) return -1;
+    }
   int* err = device_error_word();
   if (!err) return -3;
   return expert_sort_launch(*a, err, static_cast<cudaStream_t>(stream));
