@@ -154,3 +154,21 @@ def test_outputs_that_do_not_fit_are_not_noted(cuda):
         with pytest.raises(ValueError):
             call(out)
         y.backward()
+
+
+@pytest.mark.parametrize("T,K", [(40, 1), (40, 2), (3000, 2)])
+def test_small_products_behind_a_large_one(cuda, T, K):
+    """combine's gradient of the weights: in each lane's 64 products one of 1 comes first, and the others, 2^-25, are
+    too small to be added to it one by one."""
+    import torch
+    from toy_b200 import experts as X
+    d = 2048
+    ids = torch.randint(0, 4, (T, K), device="cuda", dtype=torch.int32)
+    r = X.sort(ids, 4)
+    dy = torch.full((T, d), 2.0 ** -25, device="cuda")
+    dy[:, :128:4] = 1.0
+    z = torch.ones((T * K, d), device="cuda")
+    dw = X.combine_grad(dy, z, r)[1].double()
+    want = dy[0].double().sum()
+    # at most 16 products in a row, the d / 512 sums of those, and five halvings (and one rounding to spare)
+    assert ((dw - want).abs() <= (16 + d / 512 + 6) * 2.0 ** -24 * want).all()

@@ -472,6 +472,10 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(RowsArgs a) {
 template <class T, class V, int K, int Q>
 __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
+  // a piece's products are summed by themselves, so that a lane's 64 of a row of 2048 are no chain of 64 roundings (f32:
+  // dw off by 1.1e-7 instead of 1.6e-7, in the same time); of small pieces the Q that are read together (for large ones
+  // that took 51.6 us instead of 49.1)
+  constexpr bool kPieces = H::kN >= 4;
   griddep_wait();
   const int lane = threadIdx.x % 32, parts = (a.K + K - 1) / K;
   const long long all = (long long)a.T * parts;
@@ -488,6 +492,7 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
     }
     for (int c0 = lane; c0 < a.per; c0 += 32 * Q) {
       V z[K][Q], x[Q];
+      float part[K] = {};
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         const int c = c0 + 32 * q;
@@ -511,8 +516,10 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
             float f[H::kN];
             if (a.dw) {
               H::get(z[k][q], f);
+              if (kPieces) part[k] = 0.f;
 #pragma unroll
-              for (int e = 0; e < H::kN; ++e) dot[k] = fmaf(g[e], f[e], dot[k]);
+              for (int e = 0; e < H::kN; ++e) part[k] = fmaf(g[e], f[e], part[k]);
+              if (kPieces) dot[k] += part[k];
             }
             if (a.dz) {
 #pragma unroll
@@ -520,6 +527,10 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
               H::store(a.dz, p[k], a.lddz, c, H::put(f));
             }
           }
+      }
+      if (!kPieces) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) dot[k] += part[k];
       }
     }
     if (a.dw) {
