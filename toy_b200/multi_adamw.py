@@ -25,11 +25,12 @@ import numpy as np
 import torch
 
 from ._lib import AdamwMultiArgs, AdamwTensor
-from ._rows import F32, I64, ROW_TYPE, bad, call, dense, prepare, written
+from ._rows import F32, I64, ROW_TYPE, bad, call, dense, prepare
 
 __all__ = ["MultiAdamW", "prepare"]
 BLOCK = 256
 _HELD = torch.float8_e4m3fn
+_note = torch.autograd.graph.increment_version   # of a list: autograd is told that its tensors' values have changed
 _SHAPE, _DTYPE = attrgetter("shape"), attrgetter("dtype")
 _POINTER, _DEVICE, _DENSE = torch.Tensor.data_ptr, torch.Tensor.get_device, torch.Tensor.is_contiguous
 # tb2_adamw_tensor, by columns
@@ -186,7 +187,7 @@ class MultiAdamW:
                            self.bits, hp_at, scale_at, seed_at)
         call(self.index, "tb2_adamw_multi", a)
         for x in lists:
-            written(*x)
+            _note(x)
 
     def _values(self, ms, vs, put: int) -> None:
         if len(ms) != self._n or len(vs) != self._n:
@@ -217,7 +218,8 @@ class MultiAdamW:
         if out is None:
             out = tuple([torch.empty(s, device=self.device, dtype=F32) for s in self._shapes] for _ in "mv")
         self._values(out[0], out[1], 0)
-        written(*out[0], *out[1])
+        for x in out:
+            _note(x)
         return out
 
     def set_moments(self, ms: Sequence[torch.Tensor], vs: Sequence[torch.Tensor]) -> None:
