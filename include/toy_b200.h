@@ -398,10 +398,9 @@ int tb2_rows_prepare(void);
  * {0, -inf}, log probabilities -inf, entropy 0. A NaN or +inf in a row makes
  * its probabilities and entropy NaN; NaN counts as the largest logit. A token
  * of vocab or more gives NaN and tb2_device_error() reports 0x5101. scale is
- * between 2^-126 and 2^126; below 2^-64 differences of logits past f32's range
- * count as infinite, and an entropy whose vocab / scale is past it is not
- * finite. tokens, stats and top_ids are on 8-byte
- * boundaries. */
+ * between 2^-126 and 2^126; below 2^-64, differences of logits past f32's range
+ * count as infinite, and where their sum is past it the entropy is not finite.
+ * tokens, stats and top_ids are on 8-byte boundaries. */
 typedef struct tb2_logprobs_args {
   int n_rows, vocab, row_type;
   const void *logits;
@@ -426,7 +425,7 @@ int tb2_logprobs(const tb2_logprobs_args *args, void *stream);
  * vocabulary (for alternatives: negative too) is left out and reported as
  * 0x5101. Words of probability 0 and rows of nothing else get 0 from p.
  * d_logits has the logits' type and may be the logits themselves, with the
- * same stride; otherwise they do not overlap. */
+ * same stride; otherwise they do not overlap (-1 where their strides show it). */
 typedef struct tb2_logprobs_grad_args {
   int n_rows, vocab, row_type;
   const void *logits;
@@ -444,13 +443,13 @@ typedef struct tb2_logprobs_grad_args {
 int tb2_logprobs_grad(const tb2_logprobs_grad_args *args, void *stream);
 
 /* Slots sorted by expert. Slot i = token * n_used + choice goes to expert
- * ids[i] (id_bytes 4 or 8: int or long long), or nowhere when that is negative;
- * the arrays share no memory.
+ * ids[i] (id_bytes 4 or 8: int or long long), or nowhere when that is negative.
  * order lists the slots of expert 0, of expert 1, ..., each expert's in slot
  * order, and -1 after the last; offsets[e] is where expert e's begin, and
  * offsets[n_experts] the number of sorted slots; pos[i] is slot i's place in
  * order, or -1. An id of n_experts or more counts as negative, and
- * tb2_device_error() reports 0x5102. n_experts is at most 1024. */
+ * tb2_device_error() reports 0x5102. n_experts is at most 1024. The four arrays
+ * share no memory. */
 typedef struct tb2_expert_sort_args {
   const void *ids;
   int id_bytes;
@@ -477,8 +476,8 @@ int tb2_expert_sort(const tb2_expert_sort_args *args, void *stream);
  *                 d_weights[t][k] = <x[t], xs[pos[t][k]]> (0 for pos -1);
  *                 either may be NULL: not wanted. d_xs may be xs itself, with
  *                 the same stride.
- * Otherwise arrays that are written overlap no others. n_tokens * n_used is
- * below 2^31, d below 2^31 - 256. */
+ * Otherwise arrays that are written overlap no others (-1 where their strides
+ * show it). n_tokens * n_used is below 2^31, d below 2^31 - 256. */
 typedef struct tb2_expert_rows_args {
   int n_tokens, n_used, d, n_rows, row_type;
   void *x;
@@ -504,19 +503,18 @@ int tb2_expert_combine_grad(const tb2_expert_rows_args *args, void *stream);
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = (1 - alpha wd) p - alpha beta1h m / (sqrt(beta2h) sqrt(v) + eps),
  * copy = p rounded to copy_type, 1 or 30 (copy NULL: none); the root and the
- * quotient are within 2^-22. state_bits 32: m and v are f32. state_bits 8: blocks of 256 consecutive values share an f32 scale
- * (m_scale, v_scale: [ceil(n / 256)]), the smallest power of two of 2^-100 or
- * more that brings the block within 448; m holds e4m3 codes of m / scale and v
- * of sqrt(v) / scale, the step's exact values rounded once to nearest (even)
- * or, with a seed (device memory; NULL: nearest), the step's f32 values to the
- * code above or below with the probability of their place between the two, by
- * bits that are a function of *seed and the value's place alone (give each step
- * another seed),
- * a positive sqrt(v) never below the smallest code, a v below 2^-126 as 0. All
- * zeros (scales too) is
- * an empty state. A block with a value that is not finite is NaN from then on.
- * `tensors` is host memory, read during the call; its pointers are device
- * memory and do not overlap; tensors of n = 0 are passed over. */
+ * quotient are within 2^-22. state_bits 32: m and v are f32. state_bits 8: blocks
+ * of 256 consecutive values share an f32 scale (m_scale, v_scale: [ceil(n /
+ * 256)]), the smallest power of two of 2^-100 or more that brings the block within
+ * 448; m holds e4m3 codes of m / scale and v of sqrt(v) / scale, the step's exact
+ * values rounded once to nearest (even) or, with a seed (device memory; NULL:
+ * nearest), the step's f32 values to the code above or below with the probability
+ * of their place between the two, by bits that are a function of *seed and the
+ * value's place alone (give each step another seed), a positive sqrt(v) never
+ * below the smallest code, a v below 2^-126 as 0. All zeros (scales too) is an
+ * empty state. A block with a value that is not finite is NaN from then on.
+ * `tensors` is host memory, read during the call; its pointers are device memory
+ * and do not overlap; tensors of n = 0 are passed over. */
 typedef struct tb2_adamw_tensor {
   void *p;
   const void *g;

@@ -20,7 +20,8 @@
 // lowest indices by a scan in order; what passes the buffers (or holds a NaN)
 // takes one round of the row for each alternative.
 //
-// Measured: 4096 rows of 152064 bf16 190 us (191 for the bytes at 6506 GB/s),
+// Measured: 4096 rows of 152064 bf16 208 to 221 us where other work has filled the
+// L2 (191 for the bytes at 6506 GB/s; 190 over and over, part of them in the L2),
 // of 128256 164, with the entropy 175 (161; two more instructions a value, the
 // issue slots are 65 % busy), with 20 alternatives too 214 (the re-read's
 // latency, in all the CTAs of a round at once); the gradient 338 (323). One row

@@ -160,7 +160,7 @@ __device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) {
 }
 
 // A warp has a block at a time. Where CTAs end after a few blocks the GPU works in few pages at any time, which is what
-// HBM likes best (135M weights: f32 moments 561 us, with a grid that stays and deals the blocks out 586, with a run of
+// HBM likes best (135M weights: f32 moments 563 us, with a grid that stays and deals the blocks out 586, with a run of
 // blocks to each CTA 617; the values of 8-bit moments 210, 240 and 267). The 8-bit step has more to compute, and CTAs
 // that start anew with the factors take 475 us: its grid stays, and each CTA has two blocks a warp in a row (429 us;
 // one 447, four 443, a run of all its blocks 489).
@@ -172,8 +172,8 @@ __device__ __forceinline__ void put_byte(unsigned& w, int at, unsigned q) {
 // taken of both ends of an interval that holds the exact one, and where the two differ (one value in 90000) it is
 // rounded from 64 bits. With U = 2^-24: the root's square is a sum of squares, the held root's factor and product 2 + 1
 // U, the gradient's 3 + 1, doubled by squaring, 1 for a square and 1 for the sum; the root halves these 10, and is off
-// by 2 U itself: 7 U of the 8 allowed. With a seed the step stays in f32, and the random bits take its place (461 us
-// instead of 435 for 135M weights; 484 with bits of their own for m and the root).
+// by 2 U itself: 7 U of the 8 allowed. With a seed the step stays in f32, and the random bits take its place (456 us
+// instead of 425 for 135M weights; 484 with bits of their own for m and the root).
 //
 // Bound by HBM in 32 bits. In 8 bits a value is 16 bytes, the time of some 75 instructions at most: a look at the
 // distance of every root from a border made it 58 (445 us where the bytes of 135M weights take 332), IEEE quotients and
@@ -232,7 +232,8 @@ __device__ __forceinline__ void step8(const Hyper& h, float (&p)[8], const float
   }
 }
 
-// 32 bits that look random, of x.
+// 32 bits that look random, of x: the low-bias integer hash that C. Wellons published (xor, shift and multiply, with
+// constants found by search).
 __device__ __forceinline__ unsigned mixed(unsigned x) {
   x = (x ^ x >> 16) * 0x7feb352du;
   x = (x ^ x >> 15) * 0x846ca68bu;
