@@ -472,9 +472,9 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(RowsArgs a) {
 template <class T, class V, int K, int Q>
 __global__ void __launch_bounds__(256) combine_grad_kernel(RowsArgs a) {
   using H = Chunk<T, V>;
-  // a piece's products are summed by themselves, so that a lane's 64 of a row of 2048 are no chain of 64 roundings (f32:
-  // dw off by 1.1e-7 instead of 1.6e-7, in the same time); of small pieces the Q that are read together (for large ones
-  // that took 51.6 us instead of 49.1)
+  // a piece's products are summed by themselves, so that a lane's 64 of a row of 2048 are no chain of 64 roundings
+  // (f32: dw off by 1.1e-7 instead of 1.6e-7, in the same time); of small pieces the Q that are read together (for
+  // large ones that took 51.6 us instead of 49.1)
   constexpr bool kPieces = H::kN >= 4;
   griddep_wait();
   const int lane = threadIdx.x % 32, parts = (a.K + K - 1) / K;

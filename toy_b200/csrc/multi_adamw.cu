@@ -97,8 +97,8 @@ __device__ __noinline__ unsigned e4m3_of(double t) {
 }
 
 // Within 2^-23. FTZ: a number below 2^-126 is 0, which 8-bit moments allow; second moments in f32 go on below that, and
-// their roots are far above it. (With f32 moments the correctly rounded root and quotient took 623 us instead of 562 for
-// 135M weights: their rare paths cost registers.)
+// their roots are far above it. (With f32 moments the correctly rounded root and quotient took 623 us instead of 562
+// for 135M weights: their rare paths cost registers.)
 template <bool FTZ>
 __device__ __forceinline__ float sqrt_near(float x) {
   float r;
@@ -122,8 +122,8 @@ __device__ __forceinline__ float top_of(float a, float b) {
 __device__ __forceinline__ unsigned block_top(float top) {
   return __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
 }
-// A block's power of two, from the bits of its largest magnitude, and the factor to it: the smallest 2^e with top <= 448
-// 2^e (448 = 1.75 2^8), 2^-100 at least; NaN where top is not finite.
+// A block's power of two, from the bits of its largest magnitude, and the factor to it: the smallest 2^e with top <=
+// 448 2^e (448 = 1.75 2^8), 2^-100 at least; NaN where top is not finite.
 __device__ __forceinline__ float block_scale(unsigned b, float& inverse) {
   const int e = max((int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u), -100);
   const bool ok = b < 0x7f800000u;

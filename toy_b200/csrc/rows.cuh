@@ -48,8 +48,8 @@ struct Piece {
   }
 };
 
-// Whether na rows at a and nb rows at b, of d values each, share no memory. Rows may lie between one another's; of unlike
-// strides that is left to the caller.
+// Whether na rows at a and nb rows at b, of d values each, share no memory. Rows may lie between one another's; of
+// unlike strides that is left to the caller.
 inline bool rows_apart(const void* a, long long lda, long long na, const void* b, long long ldb, long long nb, int d,
                        int type) {
   if (!a || !b || na < 1 || nb < 1) return true;

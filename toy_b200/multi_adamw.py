@@ -147,7 +147,8 @@ class MultiAdamW:
         if len(grads) != self._n:
             bad("grads: one per weight")
         self._follow()
-        numbers = not isinstance(hp, torch.Tensor) or self.bits == 8 and not isinstance(seed, (torch.Tensor, type(None)))
+        numbers = not isinstance(hp, torch.Tensor) or \
+            self.bits == 8 and seed is not None and not isinstance(seed, torch.Tensor)
         if numbers and torch.cuda.is_current_stream_capturing():
             bad("a captured step takes hp and seed as tensors on the GPU (numbers would stay those of the capture)")
         if not isinstance(hp, torch.Tensor):
