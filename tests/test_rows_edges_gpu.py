@@ -172,3 +172,17 @@ def test_small_products_behind_a_large_one(cuda, T, K):
     want = dy[0].double().sum()
     # at most 16 products in a row, the d / 512 sums of those, and five halvings (and one rounding to spare)
     assert ((dw - want).abs() <= (16 + d / 512 + 6) * 2.0 ** -24 * want).all()
+
+
+def test_a_refused_sort_notes_nothing(cuda):
+    import torch
+    from toy_b200 import experts as X
+    ids = torch.randint(0, 4, (10, 2), device="cuda", dtype=torch.int32)
+    r = X.sort(ids, 4)
+    was, versions = [t.clone() for t in r], [t._version for t in r]
+    for out in (r._replace(order=ids.view(-1)), r._replace(pos=r.order.view(10, 2)), r._replace(pos=r.pos.long())):
+        with pytest.raises(ValueError):
+            X.sort(ids, 4, out=out)
+    assert [t._version for t in r] == versions and all(torch.equal(a, b) for a, b in zip(r, was))
+    X.sort(ids, 4, out=r)
+    assert all(t._version == v + 1 for t, v in zip(r, versions))

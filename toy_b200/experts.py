@@ -41,17 +41,19 @@ def sort(ids: torch.Tensor, n_experts: int, *, out: Optional[Routing] = None) ->
         bad("ids: contiguous i32 or i64 [tokens, used] on a GPU, fewer than 2^31")
     if not 1 <= n_experts <= MAX_EXPERTS:
         bad(f"n_experts is 1 to {MAX_EXPERTS}")
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = Routing(ids.new_empty(n_experts + 1, dtype=I32), ids.new_empty(n, dtype=I32),
                       ids.new_empty(ids.shape, dtype=I32))
     else:
         dense(out.offsets, (n_experts + 1,), I32, dev, "out.offsets")
         dense(out.order, (n,), I32, dev, "out.order")
         dense(out.pos, ids.shape, I32, dev, "out.pos")
-        written(*out)
     a = ExpertSortArgs(ids.data_ptr(), 8 if wide else 4, n, n_experts, out.offsets.data_ptr(), out.order.data_ptr(),
                        out.pos.data_ptr())
     call(dev, "tb2_expert_sort", a)
+    if not fresh:
+        written(*out)
     return out
 
 
